@@ -160,7 +160,8 @@ int bonsai_b200_set_option(const char *key, int64_t value);
 /* Status word written by device-side bounded waits: 0 = no kernel of this library has given up on a
  * wait on the current device since the word was last cleared; 1 = a wait on a shared-memory barrier or
  * counter ran out; 2 = a wait for other CTAs or other ranks ran out (the launch still ends by itself and
- * the context stays usable; the outputs of that launch are incomplete).  Both calls synchronise the device
+ * the context stays usable; the outputs of that launch are incomplete); 3 = a call for several sequences met numbers on the device that do not
+ * fit (it left what they concern alone).  Both calls synchronise the device
  * (cudaDeviceSynchronize), so neither may be made while a stream of the device is being captured.
  * Failures of the calls themselves come back as 1000 + the CUDA error code. */
 int bonsai_b200_device_status(void);
@@ -258,6 +259,59 @@ int bonsai_b200_kv_arrays(struct bonsai_kv_cache *kv, void **k, void **v, int64_
  * at once (negative: as many as on the current device; 0: none): out = CTAs per cluster, clusters, positions per CTA.  Launches nothing;
  * with both numbers given it needs no GPU.  For tests.  Returns 1 for bad arguments or where clusters of 8 do not run. */
 int bonsai_b200_kv_splits(int n_pos, int resident8, int resident16, int64_t out[3]);
+
+/* ---- many tokens of several sequences: what a layer does between its projections (no counterpart in the reference, which decodes one
+ * sequence and says nothing of its attention's norms, include/bonsai_p40.h:44-56) -------------------------------------------------------------
+ * Rows of a call's tensors are tokens.  Where a call serves several sequences, `start` (device memory, n_seq + 1 ascending numbers from 0 to at most n_tok)
+ * says which rows are whose: sequence s has rows start[s] .. start[s + 1] - 1, none where the two are equal.  Rows from start[n_seq] on belong to nobody:
+ * they are not read, and outputs leave theirs as they were.  What lies on the device (start, lengths, tables, slots) is read when the call runs, so a
+ * captured call can be replayed with other numbers.  Numbers that do not fit (rows outside the call, a page that the pool does not have, a slot that
+ * two sequences name) stop that sequence and no other: its outputs and states are incomplete or as they were, and the status word
+ * (bonsai_b200_device_status) becomes 3.  Workspaces belong to one call at a time: calls, and replays of graphs, that share one follow each other. */
+
+/* Norms of queries and keys for each head, with the position rotation in the same pass: row = x / sqrt(mean(x^2) + eps) * weight, then the pairs
+ * (row[i], row[i + n_rot / 2]), i < n_rot / 2, turned by the angle pos[token] * freq[i]; values from n_rot on are not turned.  q holds n_tok x n_head
+ * rows of head_dim floats (1 .. 256; n_rot even, at most head_dim) at token * q_tok_stride + head * q_head_stride floats, k likewise n_head_kv: a
+ * projection that also gives something else per head needs no copy.  Rows may not overlap.  q_out, k_out are packed [n_tok][heads][head_dim]; they
+ * may be q and k where those are packed too, and may not overlap the inputs in any other way.  Weights have head_dim floats; pos is int32, freq
+ * double (radians per position, n_rot / 2 of them, up to 1): the angle is formed in 64 bits, however far the position.  n_head or n_head_kv may be 0.  Returns 1 for
+ * sizes and strides that are not those, 0 without a launch if n_tok <= 0. */
+int bonsai_b200_qk_norm_rope(const float *q, const float *k, const float *q_weight, const float *k_weight, const int32_t *pos, const double *freq, float *q_out,
+                             float *k_out, int64_t n_tok, int n_head, int n_head_kv, int head_dim, int n_rot, int64_t q_tok_stride, int64_t q_head_stride,
+                             int64_t k_tok_stride, int64_t k_head_stride, float eps, bonsai_stream stream);
+
+/* A K/V cache in pages.  The pool is the caller's memory (16-byte aligned), n_pages pages of
+ *   [n_layers][K, V][n_head_kv][BONSAI_B200_PAGE_POSITIONS][256 / 32 blocks of 34 bytes]
+ * with Q8_0 blocks as bonsai_kv_append lays them out.  A block's scale is its largest magnitude times 1 / 127, rounded once, in fp32 and then to fp16
+ * (bonsai_kv_append divides: the scale's last bit differs in one block of 23, about one code in 10^7).  Sequence s has len[s] positions, the new tokens of the call (rows start[s] ..) being the last of them;
+ * position p lies in page table[s * table_stride + p / 64], row p % 64.  Sequences may share pages that none of the call's rows goes to. */
+#define BONSAI_B200_PAGE_POSITIONS 64
+typedef struct bonsai_b200_pages {
+    void *pool;
+    const int32_t *table, *len, *start;       /* device memory: [n_seq][table_stride], [n_seq], [n_seq + 1] */
+    int32_t n_pages, n_layers, n_head_kv, n_seq, table_stride, n_tok;
+} bonsai_b200_pages;
+/* Stores the rows k, v ([n_tok][n_head_kv][256]) of the new tokens of one layer. */
+int bonsai_b200_pages_append(const bonsai_b200_pages *pages, int layer, const float *k, const float *v, bonsai_stream stream);
+/* Attention of the new tokens (q, out [n_tok][n_head][256]) of one layer over the cache, their own rows included: each as bonsai_kv_attn_decode computes it at
+ * its position -- queries quantised to Q8_0 (as above), positions up to its own seen -- within 1e-5 of the largest output of a head.  A token without a position
+ * (len[s] smaller than its new tokens) sees nothing: zeros.  max_len: no smaller than every len, for the division of the work; longer sequences are served
+ * all the same, more slowly.  workspace: 16-byte aligned device memory of bonsai_b200_pages_attn_workspace(the same sizes) bytes (NULL where that is 0). */
+int64_t bonsai_b200_pages_attn_workspace(int n_tok, int max_len, int n_seq, int n_head, int n_head_kv);
+int bonsai_b200_pages_attn(const bonsai_b200_pages *pages, int layer, const float *q, float *out, int n_head, int max_len, void *workspace,
+                           int64_t workspace_bytes, float scale, bonsai_stream stream);
+/* Copies pages of page_bytes (a multiple of 16) inside a pool: page src[i] to page dst[i], i < n.  src and dst are HOST memory, read before the call returns.  Returns 1,
+ * and copies nothing, where a page is not one of the n_pages, is written twice or is both read and written. */
+int bonsai_b200_pages_copy(void *pool, int64_t page_bytes, int n_pages, const int32_t *src, const int32_t *dst, int n, bonsai_stream stream);
+
+/* The gated delta rule over the new tokens of several sequences: bonsai_p40_gdn_step for each token in turn (q, k [n_tok][n_k_heads][K], v, out
+ * [n_tok][n_v_heads][V], g, beta [n_tok][n_v_heads]), the same shapes and within 1e-5 of the largest output.  state: n_slots states [n_v_heads][K][V],
+ * updated in place; sequence s has state slot[s], or s where slot is NULL (then n_slots >= n_seq).  A sequence without new tokens keeps its state.
+ * workspace: 16-byte aligned device memory of bonsai_b200_gdn_seqs_workspace(the same sizes) bytes (NULL where that is 0). */
+int64_t bonsai_b200_gdn_seqs_workspace(int n_tok, int n_seq, int n_k_heads, int n_v_heads, int K, int V);
+int bonsai_b200_gdn_seqs(float *state, const float *q, const float *k, const float *v, const float *g, const float *beta, float *out, const int32_t *start,
+                         const int32_t *slot, void *workspace, int64_t workspace_bytes, int n_seq, int n_slots, int n_tok, int n_k_heads, int n_v_heads, int K, int V,
+                         bonsai_stream stream);
 
 /* Version of this build as major * 100 + minor. */
 int bonsai_b200_version(void);

@@ -56,6 +56,13 @@ SIGNATURES = {
     "bonsai_b200_chain_info": (_INT, [_VP, _VP]),
     "bonsai_b200_kv_arrays": (_INT, [_VP, _VP, _VP, _VP]),
     "bonsai_b200_kv_splits": (_INT, [_INT, _INT, _INT, _VP]),
+    "bonsai_b200_qk_norm_rope": (_INT, [_VP] * 8 + [_I64] + [_INT] * 4 + [_I64] * 4 + [_F, _VP]),
+    "bonsai_b200_pages_append": (_INT, [_VP, _INT, _VP, _VP, _VP]),
+    "bonsai_b200_pages_attn_workspace": (_I64, [_INT] * 5),
+    "bonsai_b200_pages_attn": (_INT, [_VP, _INT, _VP, _VP, _INT, _INT, _VP, _I64, _F, _VP]),
+    "bonsai_b200_pages_copy": (_INT, [_VP, _I64, _INT, _VP, _VP, _INT, _VP]),
+    "bonsai_b200_gdn_seqs_workspace": (_I64, [_INT] * 6),
+    "bonsai_b200_gdn_seqs": (_INT, [_VP] * 10 + [_I64] + [_INT] * 7 + [_VP]),
     "bonsai_kv_bytes": (_I64, [_INT]),
     "bonsai_kv_gdn_bytes": (_I64, []),
     "bonsai_kv_create": (_VP, [_INT, _VP]),
@@ -91,7 +98,8 @@ def lib():
 # The functions that enqueue work are native (csrc/python_calls.cpp): a call here is checked, given torch's current stream
 # and launched in about the time of the launch itself.  `_calls` name -> exported symbol.
 _NATIVE = {n: "bonsai_p40_" + n for n in ("gemv", "quant_activations", "gemm", "repack", "gemv_repack", "fwht", "rmsnorm", "gdn_step", "attn")}
-_NATIVE.update({n: "bonsai_b200_" + n for n in ("fwht_quant", "swiglu", "quant_batch", "linear", "linear_static", "chain_run")})
+_NATIVE.update({n: "bonsai_b200_" + n for n in ("fwht_quant", "swiglu", "quant_batch", "linear", "linear_static", "chain_run", "qk_norm_rope", "pages_append", "pages_attn",
+                                               "pages_copy", "gdn_seqs")})
 _NATIVE.update({n: "bonsai_" + n for n in ("kv_append", "kv_append_batch", "kv_attn_decode")})
 _calls = None
 
@@ -249,6 +257,30 @@ def linear_static(W, x, signs, y, n_out, n_in):
     return _native().linear_static(W, x, signs, y, n_out, n_in)
 
 
+def qk_norm_rope(q, k, q_weight, k_weight, pos, freq, q_out, k_out, n_tok, n_head, n_head_kv, head_dim, n_rot, q_tok_stride, q_head_stride, k_tok_stride,
+                 k_head_stride, eps):
+    """q and k need not be contiguous: their strides are arguments, in floats."""
+    return _native().qk_norm_rope(q, k, q_weight, k_weight, pos, freq, q_out, k_out, n_tok, n_head, n_head_kv, head_dim, n_rot, q_tok_stride, q_head_stride,
+                                  k_tok_stride, k_head_stride, eps)
+
+
+def pages_attn_workspace(n_tok, max_len, n_seq, n_head, n_head_kv):
+    return lib().bonsai_b200_pages_attn_workspace(n_tok, max_len, n_seq, n_head, n_head_kv)
+
+
+def pages_copy(pool, page_bytes, n_pages, src, dst, n):
+    """src and dst are int32 tensors in host memory."""
+    return _native().pages_copy(pool, page_bytes, n_pages, src, dst, n)
+
+
+def gdn_seqs_workspace(n_tok, n_seq, n_k_heads, n_v_heads, K, V):
+    return lib().bonsai_b200_gdn_seqs_workspace(n_tok, n_seq, n_k_heads, n_v_heads, K, V)
+
+
+def gdn_seqs(state, q, k, v, g, beta, out, start, slot, workspace, workspace_bytes, n_seq, n_slots, n_tok, n_k_heads, n_v_heads, K, V):
+    return _native().gdn_seqs(state, q, k, v, g, beta, out, start, slot, workspace, workspace_bytes, n_seq, n_slots, n_tok, n_k_heads, n_v_heads, K, V)
+
+
 # ---- a list of projections in one launch -------------------------------------------------------------
 OP_ROTATE, OP_DEPENDS, OP_SAME_INPUT, OP_RMSNORM, OP_SWIGLU, OP_RESCALE = 1, 2, 4, 8, 16, 32
 
@@ -357,3 +389,46 @@ class KVCache:
         except Exception:
             pass
 
+
+# ---- a K/V cache in pages (include/bonsai_b200_ext.h) ------------------------------------------------------
+PAGE_POSITIONS, ROW_BYTES = 64, 256 // 32 * 34
+
+
+class PagesStruct(C.Structure):
+    """struct bonsai_b200_pages"""
+    _fields_ = [("pool", C.c_void_p), ("table", C.c_void_p), ("len", C.c_void_p), ("start", C.c_void_p),
+                ("n_pages", C.c_int32), ("n_layers", C.c_int32), ("n_head_kv", C.c_int32), ("n_seq", C.c_int32), ("table_stride", C.c_int32), ("n_tok", C.c_int32)]
+
+
+class Pages:
+    """A call's view of a paged cache: bonsai_b200_pages and the calls that take it.  `pool` is a uint8 tensor of whole pages
+    ([n_layers][K, V][n_head_kv][64 positions][272 bytes] each), `table` int32 [n_seq][pages of the longest sequence], `length` int32
+    [n_seq], `start` int32 [n_seq + 1], all on the current device; the object keeps them alive and reads their numbers when a call runs."""
+
+    def __init__(self, pool, table, length, start, n_layers, n_head_kv, n_tok):
+        import torch
+        for t, name, dtype in ((pool, "pool", torch.uint8), (table, "table", torch.int32), (length, "length", torch.int32), (start, "start", torch.int32)):
+            _dev(t, name)
+            if t.dtype != dtype or t.device.index != torch.cuda.current_device():
+                raise RuntimeError(f"{name} must be a {dtype} tensor on the current device")
+        page = n_layers * 2 * n_head_kv * PAGE_POSITIONS * ROW_BYTES
+        n_seq = length.numel()
+        if n_layers <= 0 or n_head_kv <= 0 or pool.numel() == 0 or pool.numel() % page != 0:
+            raise RuntimeError(f"the pool must be whole pages of {page} bytes")
+        if table.dim() != 2 or table.shape[0] != n_seq or start.numel() != n_seq + 1:
+            raise RuntimeError("table, length and start must be of as many sequences")
+        self._keep = (pool, table, length, start)
+        self._s = PagesStruct(pool.data_ptr(), table.data_ptr(), length.data_ptr(), start.data_ptr(), pool.numel() // page, n_layers, n_head_kv, n_seq,
+                              table.shape[1], n_tok)
+        self._p = C.addressof(self._s)
+        self.page_bytes, self.n_pages, self.n_seq, self.n_tok = page, pool.numel() // page, n_seq, n_tok
+
+    def append(self, layer, k, v):
+        return _native().pages_append(self._p, layer, k, v)
+
+    def attn_workspace(self, max_len, n_head):
+        return pages_attn_workspace(self.n_tok, max_len, self.n_seq, n_head, self._s.n_head_kv)
+
+    def attn(self, layer, q, out, n_head, max_len, workspace, scale):
+        """workspace: a tensor of attn_workspace(max_len, n_head) bytes, or None where that is 0."""
+        return _native().pages_attn(self._p, layer, q, out, n_head, max_len, workspace, 0 if workspace is None else workspace.nbytes, scale)

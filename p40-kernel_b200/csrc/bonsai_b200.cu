@@ -17,8 +17,11 @@
 #include "gemv_chain.cuh"
 #include "gemv_few.cuh"
 #include "gemv_mma.cuh"
+#include "gdn_seqs.cuh"
+#include "heads.cuh"
 #include "kv.cuh"
 #include "ops.cuh"
+#include "pages.cuh"
 #include "probe.cuh"
 #include "ptq.cuh"
 #include "repack.cuh"
@@ -1895,6 +1898,194 @@ int bonsai_b200_kv_arrays(bonsai_kv_cache *kv, void **k, void **v, int64_t *byte
     *v = kv->d_v;
     *bytes_each = kv_array_bytes(kv->capacity);
     return 0;
+}
+
+
+// ---- several sequences: what a layer does between its projections --------------------------------------------------
+namespace {
+inline bool aligned8(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
+
+// 0: a cache that calls may use; 1: not one; -1: one, but no new tokens.
+int check_pages(const bonsai_b200_pages *p, int layer, PageCache *C) {
+    if (!p || p->n_pages <= 0 || p->n_layers <= 0 || p->n_head_kv <= 0 || p->n_head_kv > 65535 || p->table_stride <= 0 || p->n_seq < 0 || p->n_tok < 0) return 1;
+    if (layer < 0 || layer >= p->n_layers) return 1;
+    if (p->n_seq == 0 || p->n_tok == 0) return -1;
+    if (!p->pool || !p->table || !p->len || !p->start || !aligned16(p->pool) || !aligned4(p->table) || !aligned4(p->len) || !aligned4(p->start)) return 1;
+    *C = {static_cast<uint8_t *>(p->pool), p->table, p->len, p->start, p->n_pages, p->n_layers, p->n_head_kv, p->n_seq, p->table_stride, p->n_tok};
+    return 0;
+}
+
+// How pages_attn divides a call: 16 rowt rows a CTA, a span of pages a CTA, CTAs per kv head.
+struct PagesPlan {
+    int rowt, pages_per_split, splits;
+    int64_t tiles;
+};
+PagesPlan plan_pages(int n_tok, int max_len, int n_seq, int n_head, int n_head_kv) {
+    PagesPlan p;
+    const int64_t rows = (int64_t)n_tok * (n_head / n_head_kv), each = (rows + n_seq - 1) / n_seq;
+    p.rowt = each <= 16 ? 1 : each <= 32 ? 2 : 4;
+    const int64_t high = 16 * p.rowt;
+    p.tiles = (rows + (int64_t)std::min(n_seq, n_tok) * (high - 1)) / high;
+    const int64_t items = std::max<int64_t>(1, rows / high) * n_head_kv, pages = std::max(1, (int)(((int64_t)max_len + PG_POS - 1) / PG_POS));
+    const int64_t want = std::max<int64_t>(4, (items * pages + 4 * 2 * SM_COUNT - 1) / (4 * 2 * SM_COUNT));
+    p.pages_per_split = (int)std::min(want, pages);
+    p.splits = (int)((pages + p.pages_per_split - 1) / p.pages_per_split);
+    return p;
+}
+inline bool pages_attn_sizes(int n_tok, int max_len, int n_seq, int n_head, int n_head_kv) {
+    return n_tok > 0 && n_seq > 0 && max_len > 0 && n_head > 0 && n_head_kv > 0 && n_head % n_head_kv == 0 && (int64_t)n_tok * (n_head / n_head_kv) <= INT32_MAX / 2;
+}
+}  // namespace
+
+int bonsai_b200_qk_norm_rope(const float *q, const float *k, const float *q_weight, const float *k_weight, const int32_t *pos, const double *freq, float *q_out,
+                             float *k_out, int64_t n_tok, int n_head, int n_head_kv, int head_dim, int n_rot, int64_t q_tok_stride, int64_t q_head_stride,
+                             int64_t k_tok_stride, int64_t k_head_stride, float eps, bonsai_stream stream) {
+    if (head_dim <= 0 || head_dim > QKN_MAX_DIM || n_rot < 0 || n_rot > head_dim || n_rot % 2 != 0 || n_head < 0 || n_head_kv < 0 || n_head > (1 << 18) || n_head_kv > (1 << 18)) return 1;
+    const int heads = n_head + n_head_kv;
+    if (n_tok <= 0 || heads == 0) return 0;
+    if (n_tok > INT32_MAX || (n_rot && (!pos || !freq || !aligned4(pos) || !aligned8(freq)))) return 1;
+    QkNormParams P = {{q, k}, {q_weight, k_weight}, {q_out, k_out}, {q_tok_stride, k_tok_stride}, {q_head_stride, k_head_stride}, pos, freq, {n_head, n_head_kv}, head_dim, n_rot, eps};
+    bool vec = head_dim % 4 == 0;
+    for (int i = 0; i < 2; ++i) {
+        if (!P.n_head[i]) continue;
+        if (!P.x[i] || !P.w[i] || !P.y[i] || !aligned4(P.x[i]) || !aligned4(P.w[i]) || !aligned4(P.y[i])) return 1;
+        // rows that overlap each other, or an output that is not the input row for row, would be read after they are written
+        const bool one_tok = n_tok == 1, one_head = P.n_head[i] == 1;
+        const int64_t ts = P.tok_stride[i], hs = P.head_stride[i];
+        if ((!one_head && hs < head_dim) || (!one_tok && ts < 0) || (one_head ? false : (!one_tok && ts < (P.n_head[i] - 1) * hs + head_dim && hs < (n_tok - 1) * ts + head_dim))) return 1;
+        if (one_head && !one_tok && ts < head_dim) return 1;
+        vec = vec && aligned16(P.x[i]) && aligned16(P.w[i]) && aligned16(P.y[i]) && (one_tok || ts % 4 == 0) && (one_head || hs % 4 == 0);
+    }
+    const int groups = (heads + QKN_MAX_WARPS - 1) / QKN_MAX_WARPS, warps = (heads + groups - 1) / groups;
+    if (groups > 65535) return 1;
+    auto run = [&](auto kernel) { return (int)launch(kernel, dim3((unsigned)n_tok, (unsigned)groups), dim3(32 * (unsigned)warps), 0, as_stream(stream), true, P); };
+    if (n_tok * groups <= SM_COUNT) return vec ? run(qk_norm_rope_kernel<true, true>) : run(qk_norm_rope_kernel<false, true>);
+    return vec ? run(qk_norm_rope_kernel<true, false>) : run(qk_norm_rope_kernel<false, false>);
+}
+
+int bonsai_b200_pages_append(const bonsai_b200_pages *pages, int layer, const float *k, const float *v, bonsai_stream stream) {
+    PageCache C;
+    const int rc = check_pages(pages, layer, &C);
+    if (rc) return rc < 0 ? 0 : rc;
+    const int64_t ctas = ((int64_t)C.n_tok * C.n_head_kv + KV_APPEND_WARPS - 1) / KV_APPEND_WARPS;
+    if (!k || !v || !aligned4(k) || !aligned4(v) || ctas > INT32_MAX) return 1;
+    auto run = [&](auto kernel) { return (int)launch(kernel, dim3((unsigned)ctas), dim3(32 * KV_APPEND_WARPS), 0, as_stream(stream), true, C, k, v, layer); };
+    return aligned16(k) && aligned16(v) ? run(pages_append_kernel<true>) : run(pages_append_kernel<false>);
+}
+
+int64_t bonsai_b200_pages_attn_workspace(int n_tok, int max_len, int n_seq, int n_head, int n_head_kv) {
+    if (!pages_attn_sizes(n_tok, max_len, n_seq, n_head, n_head_kv)) return 0;
+    const PagesPlan plan = plan_pages(n_tok, max_len, n_seq, n_head, n_head_kv);
+    return plan.splits == 1 ? 0 : (int64_t)plan.splits * n_tok * n_head * (KV_D + 2) * (int64_t)sizeof(float);
+}
+
+int bonsai_b200_pages_attn(const bonsai_b200_pages *pages, int layer, const float *q, float *out, int n_head, int max_len, void *workspace,
+                           int64_t workspace_bytes, float scale, bonsai_stream stream) {
+    PageAttn P = {};
+    if (n_head <= 0 || max_len < 0) return 1;
+    const int rc = check_pages(pages, layer, &P.C);
+    if (rc) return rc < 0 ? 0 : rc;
+    const PageCache &C = P.C;
+    max_len = std::max(1, max_len);
+    if (!q || !out || !aligned4(q) || !aligned4(out) || !pages_attn_sizes(C.n_tok, max_len, C.n_seq, n_head, C.n_head_kv)) return 1;
+    const PagesPlan plan = plan_pages(C.n_tok, max_len, C.n_seq, n_head, C.n_head_kv);
+    if (plan.tiles > INT32_MAX || plan.splits > 65535) return 1;
+    P.q = q;
+    P.out = out;
+    P.layer = layer;
+    P.n_head = n_head;
+    P.group = n_head / C.n_head_kv;
+    P.pages_per_split = plan.pages_per_split;
+    P.splits = plan.splits;
+    P.scale = scale;
+    if (plan.splits > 1) {
+        const int64_t rows = (int64_t)plan.splits * C.n_tok * n_head;
+        if (!workspace || !aligned16(workspace) || workspace_bytes < rows * (KV_D + 2) * (int64_t)sizeof(float)) return 1;
+        P.part_acc = static_cast<float *>(workspace);
+        P.part_ml = reinterpret_cast<float2 *>(P.part_acc + rows * KV_D);
+    }
+    static SmemOptIn opt[3];
+    auto run = [&](auto kernel, SmemOptIn &o) {
+        const cudaError_t e = o.ensure(kernel);
+        if (e != cudaSuccess) return e;
+        return launch(kernel, dim3((unsigned)plan.tiles, (unsigned)C.n_head_kv, (unsigned)plan.splits), dim3(PGA_THREADS), (size_t)pga_smem_bytes(plan.rowt), as_stream(stream), true, P);
+    };
+    cudaError_t e = plan.rowt == 1 ? run(pages_attn_kernel<1>, opt[0]) : plan.rowt == 2 ? run(pages_attn_kernel<2>, opt[1]) : run(pages_attn_kernel<4>, opt[2]);
+    if (e == cudaSuccess && plan.splits > 1) {
+        const int64_t ctas = ((int64_t)C.n_tok * n_head + PGJ_WARPS - 1) / PGJ_WARPS;
+        if (ctas > INT32_MAX) return 1;
+        e = launch(pages_join_kernel, dim3((unsigned)ctas), dim3(32 * PGJ_WARPS), 0, as_stream(stream), true, P);
+    }
+    return (int)e;
+}
+
+int bonsai_b200_pages_copy(void *pool, int64_t page_bytes, int n_pages, const int32_t *src, const int32_t *dst, int n, bonsai_stream stream) {
+    if (page_bytes <= 0 || page_bytes % 16 != 0 || n_pages <= 0 || n < 0) return 1;
+    if (n == 0) return 0;
+    if (!pool || !aligned16(pool) || !src || !dst) return 1;
+    // per page: 1 read, 2 written.  Written twice, or read and written, would leave what is copied to the order of the copies.
+    unsigned char *use = new (std::nothrow) unsigned char[n_pages]();
+    if (!use) return (int)cudaErrorMemoryAllocation;
+    bool bad = false;
+    for (int i = 0; i < n && !bad; ++i) {
+        bad = src[i] < 0 || src[i] >= n_pages || dst[i] < 0 || dst[i] >= n_pages;
+        if (!bad) {
+            bad = (use[dst[i]] & 2) != 0;
+            use[src[i]] |= 1;
+            use[dst[i]] |= 2;
+        }
+    }
+    for (int i = 0; i < n && !bad; ++i) bad = use[src[i]] == 3;
+    delete[] use;
+    if (bad) return 1;
+    const int64_t words = page_bytes / 16, parts = (words + PG_COPY_THREADS * PG_COPY_WORDS - 1) / (PG_COPY_THREADS * PG_COPY_WORDS);
+    for (int at = 0; at < n; at += PG_COPY_PAIRS) {
+        PagePairs L;
+        const int m = std::min(n - at, PG_COPY_PAIRS);
+        std::memcpy(L.src, src + at, m * sizeof(int32_t));
+        std::memcpy(L.dst, dst + at, m * sizeof(int32_t));
+        const int64_t items = m * parts;
+        const cudaError_t e = launch(pages_copy_kernel, dim3((unsigned)std::min<int64_t>(items, 8 * SM_COUNT)), dim3(PG_COPY_THREADS), 0, as_stream(stream), true, L,
+                                     static_cast<uint8_t *>(pool), words, parts, items);
+        if (e != cudaSuccess) return (int)e;
+    }
+    return 0;
+}
+
+static bool gdn_shapes(int n_k_heads, int n_v_heads, int K, int V) {
+    return V > 0 && V % 32 == 0 && K > 0 && K <= GDN_KMAX && n_v_heads > 0 && n_k_heads > 0 && n_v_heads % n_k_heads == 0 && (int64_t)n_v_heads * (V / 32) <= INT32_MAX;
+}
+// Chunks that the sequences can have between them (0: every sequence goes token by token).
+static int64_t gdn_chunk_count(int n_tok, int n_seq, int K, int V) {
+    if (K != GDC_D || V != GDC_D || n_tok <= GDC_STEP_MOST) return 0;
+    const int64_t longer = std::min<int64_t>(n_seq, n_tok / (GDC_STEP_MOST + 1));           // sequences of more tokens than that
+    return ((int64_t)n_tok + longer * (GDC_T - 1)) / GDC_T;
+}
+int64_t bonsai_b200_gdn_seqs_workspace(int n_tok, int n_seq, int n_k_heads, int n_v_heads, int K, int V) {
+    if (!gdn_shapes(n_k_heads, n_v_heads, K, V) || n_tok <= 0 || n_seq <= 0) return 0;
+    return gdn_chunk_count(n_tok, n_seq, K, V) * n_v_heads * GDC_REC * (int64_t)sizeof(float);
+}
+int bonsai_b200_gdn_seqs(float *state, const float *q, const float *k, const float *v, const float *g, const float *beta, float *out, const int32_t *start,
+                         const int32_t *slot, void *workspace, int64_t workspace_bytes, int n_seq, int n_slots, int n_tok, int n_k_heads, int n_v_heads, int K, int V,
+                         bonsai_stream stream) {
+    if (!gdn_shapes(n_k_heads, n_v_heads, K, V) || n_seq < 0 || n_seq > 65535 || n_tok < 0 || n_slots < 0 || (!slot && n_slots < n_seq)) return 1;
+    if (n_seq == 0 || n_tok == 0) return 0;
+    for (const void *p : {(const void *)state, (const void *)q, (const void *)k, (const void *)v, (const void *)g, (const void *)beta, (const void *)out, (const void *)start})
+        if (!p || !aligned4(p)) return 1;
+    if (!aligned4(slot)) return 1;
+    const int64_t chunks = gdn_chunk_count(n_tok, n_seq, K, V);
+    if (chunks > INT32_MAX || n_k_heads > 65535 || (int64_t)n_v_heads * GDC_SLICES > INT32_MAX) return 1;
+    if (chunks && (!workspace || !aligned16(workspace) || workspace_bytes < chunks * n_v_heads * GDC_REC * (int64_t)sizeof(float))) return 1;
+    const GdnSeqs P = {state, q, k, v, g, beta, out, start, slot, n_seq, n_slots, n_tok, n_k_heads, n_v_heads, K, V};
+    const cudaStream_t st = as_stream(stream);
+    cudaError_t e = launch(gdn_seqs_step_kernel, dim3((unsigned)(n_v_heads * (V / 32)), (unsigned)n_seq), dim3(GDN_WARPS * 32), 0, st, true, P, chunks ? GDC_STEP_MOST : INT32_MAX);
+    if (!chunks || e != cudaSuccess) return (int)e;
+    static SmemOptIn opt[2];
+    float *recs = static_cast<float *>(workspace);
+    if ((e = opt[0].ensure(gdn_chunk_kernel)) == cudaSuccess && (e = opt[1].ensure(gdn_scan_kernel)) == cudaSuccess)
+        e = launch(gdn_chunk_kernel, dim3((unsigned)chunks, (unsigned)n_k_heads), dim3(GDC_THREADS), (size_t)gdc_chunk_smem(), st, true, P, recs);
+    if (e == cudaSuccess) e = launch(gdn_scan_kernel, dim3((unsigned)(n_v_heads * GDC_SLICES), (unsigned)n_seq), dim3(GDC_THREADS), (size_t)gdc_scan_smem(), st, true, P, (const float *)recs);
+    return (int)e;
 }
 
 }  // extern "C"

@@ -1,0 +1,97 @@
+// heads.cuh -- norms of queries and keys for each head, with the position rotation in the same pass: what an attention layer does
+// between its q / k projections and its cache.
+//
+//   y = x / sqrt(mean(x^2) + eps) * w          over the head_dim values of one head of one token, w shared by the heads
+//   y_i, y_(i + n_rot / 2) <- turned by the angle pos * freq_i, i < n_rot / 2; values from n_rot on are not turned
+//
+// The angle is formed in 64 bits and brought into [-pi, pi] there: at position 262143 an fp32 product is off by 0.016 of a turn's radian.
+#pragma once
+
+#include "common.cuh"
+#include "ops.cuh"
+
+namespace b200 {
+
+constexpr int QKN_MAX_DIM = 256, QKN_MAX_WARPS = 8;
+
+struct QkNormParams {
+    const float *x[2], *w[2];               // q, k
+    float *y[2];
+    int64_t tok_stride[2], head_stride[2];  // of x, in floats; y is packed
+    const int32_t *pos;
+    const double *freq;
+    int n_head[2], head_dim, n_rot;
+    float eps;
+};
+
+// cos and sin of pos * freq.  Two parts of 2 pi (Cody and Waite's reduction): the rest is exact to 2^-50 for any int32 position and freq <= 1.
+__device__ __forceinline__ float2 rotation_of(int pos, double freq) {
+    const double a = __dmul_rn((double)pos, freq), turns = rint(__dmul_rn(a, 0.15915494309189535));
+    const double r = __fma_rn(-turns, 2.4492935982947064e-16, __fma_rn(-turns, 6.283185307179586, a));
+    float s, c;
+    sincosf((float)r, &s, &c);
+    return make_float2(c, s);
+}
+
+// grid (tokens, groups of heads); a warp per head.  VEC: head_dim and the strides are multiples of 4, all pointers 16-byte aligned.
+template <bool VEC, bool EARLY>
+__global__ void __launch_bounds__(32 * QKN_MAX_WARPS) qk_norm_rope_kernel(const __grid_constant__ QkNormParams P) {
+    __shared__ __align__(16) float rows[QKN_MAX_WARPS][QKN_MAX_DIM];
+    __shared__ float2 turn[QKN_MAX_DIM / 2];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = (int)blockDim.x >> 5;
+    const int64_t tok = blockIdx.x;
+    int head = (int)blockIdx.y * warps + warp;
+    const bool live = head < P.n_head[0] + P.n_head[1];
+    const int which = head >= P.n_head[0];
+    if (which) head -= P.n_head[0];
+    const int n = P.head_dim, half = P.n_rot >> 1;
+    pdl_wait_prior_grid();
+    if (EARLY) pdl_launch_dependents();
+    float4 f[2], w[2];
+    if (live) {
+        const float *x = P.x[which] + tok * P.tok_stride[which] + head * P.head_stride[which];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) f[j] = rms_load<VEC>(x, 128 * j + 4 * lane, n);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) w[j] = rms_load<VEC>(P.w[which], 128 * j + 4 * lane, n);
+    }
+    for (int i = threadIdx.x; i < half; i += blockDim.x) turn[i] = rotation_of(P.pos[tok], P.freq[i]);
+    __syncthreads();
+    if (!live) return;
+    const float sc = rms_scale(__fadd_rn(slice_sumsq(f[0]), n > 128 ? slice_sumsq(f[1]) : 0.0f), n, P.eps);
+    float *row = rows[warp];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        f[j].x = __fmul_rn(__fmul_rn(f[j].x, sc), w[j].x);
+        f[j].y = __fmul_rn(__fmul_rn(f[j].y, sc), w[j].y);
+        f[j].z = __fmul_rn(__fmul_rn(f[j].z, sc), w[j].z);
+        f[j].w = __fmul_rn(__fmul_rn(f[j].w, sc), w[j].w);
+        reinterpret_cast<float4 *>(row)[32 * j + lane] = f[j];
+    }
+    __syncwarp();
+    float *y = P.y[which] + (tok * P.n_head[which] + head) * n;
+    auto turned = [&](int i, float own) {
+        if (i >= P.n_rot) return own;
+        const bool second = i >= half;
+        const float2 t = turn[second ? i - half : i];
+        const float other = row[second ? i - half : i + half];
+        return second ? __fmaf_rn(own, t.x, __fmul_rn(other, t.y)) : __fmaf_rn(own, t.x, -__fmul_rn(other, t.y));
+    };
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int i = 128 * j + 4 * lane;
+        if (i < n) {
+            const float4 o = make_float4(turned(i, f[j].x), turned(i + 1, f[j].y), turned(i + 2, f[j].z), turned(i + 3, f[j].w));
+            if (VEC) {
+                *reinterpret_cast<float4 *>(y + i) = o;
+            } else {
+                y[i] = o.x;
+                if (i + 1 < n) y[i + 1] = o.y;
+                if (i + 2 < n) y[i + 2] = o.z;
+                if (i + 3 < n) y[i + 3] = o.w;
+            }
+        }
+    }
+}
+
+}  // namespace b200

@@ -1,0 +1,573 @@
+// pages.cuh -- a Q8_0 K/V cache in pages of 64 positions: append, attention of several sequences' new tokens over it, copies.
+//
+// Layout: pool[page][layer][K | V][kv head][64 positions][272 bytes]; a row is the row of kv.cuh (8 blocks of 34 bytes), so the rows of a page for one
+// layer and kv head are ONE span of 17408 bytes.  Position p of sequence s lies in page table[s][p / 64], row p % 64.
+#pragma once
+
+#include "common.cuh"
+#include "kv.cuh"
+#include "seqs.cuh"
+
+namespace b200 {
+
+constexpr int PG_POS = 64, PG_HEAD_BYTES = PG_POS * KV_ROW;
+static_assert(PG_POS == KV_TILE, "");
+
+struct PageCache {
+    uint8_t *pool;
+    const int32_t *table, *len, *start;
+    int n_pages, n_layers, n_head_kv, n_seq, table_stride, n_tok;
+};
+
+__device__ __forceinline__ uint8_t *page_rows(const PageCache &C, int page, int layer, int kv, int head) {
+    return C.pool + ((((size_t)page * C.n_layers + layer) * 2 + kv) * C.n_head_kv + head) * PG_HEAD_BYTES;
+}
+
+// ---- append -----------------------------------------------------------------------------------------------------------------------------------
+// One warp per (token, kv head) row of K and of V, as kv_append_kernel.  A block's scale is its largest magnitude times 1 / 127, one rounded product where that kernel
+// divides: a scale's last bit differs in one block of 23, and with it about one code in 10^7.
+constexpr float PG_SCALE = 1.0f / 127.0f;
+template <bool VEC>
+__global__ void __launch_bounds__(32 * KV_APPEND_WARPS) pages_append_kernel(const __grid_constant__ PageCache C, const float *ksrc, const float *vsrc, int layer) {
+    __shared__ __align__(16) uint8_t rows[KV_APPEND_WARPS][2][KV_ROW];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t row = (int64_t)blockIdx.x * KV_APPEND_WARPS + warp;          // token * n_head_kv + head
+    if (row >= (int64_t)C.n_tok * C.n_head_kv) return;
+    const int tok = (int)(row / C.n_head_kv), h = (int)(row - (int64_t)tok * C.n_head_kv);
+    const int blk = lane >> 2, sub = lane & 3;
+    const float *kr = ksrc + row * KV_D + blk * 32 + sub * 8;
+    const float *vr = vsrc + row * KV_D + blk * 32 + sub * 8;
+    float kx[8], vx[8];
+    pdl_wait_prior_grid();
+    pdl_launch_dependents();
+    const int s = seq_of_row(C.start, C.n_seq, tok, lane);
+    if (VEC) {
+        const float4 a = *reinterpret_cast<const float4 *>(kr), b = *reinterpret_cast<const float4 *>(kr + 4);
+        const float4 c = *reinterpret_cast<const float4 *>(vr), e = *reinterpret_cast<const float4 *>(vr + 4);
+        kx[0] = a.x; kx[1] = a.y; kx[2] = a.z; kx[3] = a.w; kx[4] = b.x; kx[5] = b.y; kx[6] = b.z; kx[7] = b.w;
+        vx[0] = c.x; vx[1] = c.y; vx[2] = c.z; vx[3] = c.w; vx[4] = e.x; vx[5] = e.y; vx[6] = e.z; vx[7] = e.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { kx[i] = kr[i]; vx[i] = vr[i]; }
+    }
+    if (s >= C.n_seq) return;                                   // rows behind the last sequence
+    const SeqRange r = seq_range(C.start, s, C.n_tok);
+    const int64_t pos = (int64_t)C.len[s] - r.n + (tok - r.begin);
+    int page = -1;
+    if (r.n > 0 && tok >= r.begin && pos >= 0 && pos / PG_POS < C.table_stride) page = C.table[(size_t)s * C.table_stride + pos / PG_POS];
+    if (page < 0 || page >= C.n_pages) {
+        if (lane == 0) bad_sequence();
+        return;
+    }
+    const size_t at = (size_t)(pos % PG_POS) * KV_ROW;
+    // the reciprocals of K by the even lanes of the four, of V by the odd ones
+    const float kmax = kv_amax_8(kx), vmax = kv_amax_8(vx), d = __fmul_rn(sub & 1 ? vmax : kmax, PG_SCALE), id = d > 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
+    const uint32_t d16 = f32_to_f16_bits_ties_away(d);
+    uint32_t kw[2], vw[2];
+    kv_words_8(kx, __shfl_sync(0xffffffffu, id, lane & ~3), kw);
+    kv_words_8(vx, __shfl_sync(0xffffffffu, id, lane | 1), vw);
+    uint8_t *kb = rows[warp][0], *vb = rows[warp][1];           // put together by halfwords, stored by 16-byte words
+    unsigned short *kp = reinterpret_cast<unsigned short *>(kb + 34 * blk), *vp = reinterpret_cast<unsigned short *>(vb + 34 * blk);
+    if (sub < 2) (sub ? vp : kp)[0] = (unsigned short)d16;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        kp[1 + 4 * sub + 2 * j] = (unsigned short)(kw[j] & 0xFFFFu); kp[2 + 4 * sub + 2 * j] = (unsigned short)(kw[j] >> 16);
+        vp[1 + 4 * sub + 2 * j] = (unsigned short)(vw[j] & 0xFFFFu); vp[2 + 4 * sub + 2 * j] = (unsigned short)(vw[j] >> 16);
+    }
+    __syncwarp();
+    if (lane < KV_ROW / 16) {
+        reinterpret_cast<uint4 *>(page_rows(C, page, layer, 0, h) + at)[lane] = reinterpret_cast<const uint4 *>(kb)[lane];
+        reinterpret_cast<uint4 *>(page_rows(C, page, layer, 1, h) + at)[lane] = reinterpret_cast<const uint4 *>(vb)[lane];
+    }
+}
+
+// ---- copies -----------------------------------------------------------------------------------------------------------------------------------
+constexpr int PG_COPY_PAIRS = 480, PG_COPY_THREADS = 256, PG_COPY_WORDS = 8;            // 16-byte words a thread holds
+struct PagePairs { int32_t src[PG_COPY_PAIRS], dst[PG_COPY_PAIRS]; };
+// No page is written twice or both read and written (the host has looked), so the order does not matter.
+__global__ void __launch_bounds__(PG_COPY_THREADS) pages_copy_kernel(const __grid_constant__ PagePairs L, uint8_t *pool, int64_t page_words, int64_t parts, int64_t items) {
+    constexpr int PART = PG_COPY_THREADS * PG_COPY_WORDS;
+    pdl_wait_prior_grid();
+    for (int64_t i = blockIdx.x; i < items; i += gridDim.x) {
+        const int64_t pair = i / parts, w0 = (i - pair * parts) * PART + threadIdx.x;
+        const uint4 *src = reinterpret_cast<const uint4 *>(pool) + L.src[pair] * page_words;
+        uint4 *dst = reinterpret_cast<uint4 *>(pool) + L.dst[pair] * page_words;
+        uint4 x[PG_COPY_WORDS];
+#pragma unroll
+        for (int j = 0; j < PG_COPY_WORDS; ++j)
+            if (w0 + j * PG_COPY_THREADS < page_words) x[j] = src[w0 + j * PG_COPY_THREADS];
+#pragma unroll
+        for (int j = 0; j < PG_COPY_WORDS; ++j)
+            if (w0 + j * PG_COPY_THREADS < page_words) dst[w0 + j * PG_COPY_THREADS] = x[j];
+    }
+}
+
+// ---- attention --------------------------------------------------------------------------------------------------------------------------------
+// The value is that of kv_attn_kernel for each new token by itself: its queries are quantised to Q8_0 and see the positions up to their own.
+//   score    scale * sum over the blocks of dq dk (q8 . k8)              int8 products on mma.sync (m16n8k32), int32 sums, scaled per block in fp32
+//   output   sum of p dv v8 / sum of p, p = e^(score - maximum)          p dv in two fp16 planes, v8 as fp16 (exact), fp32 sums
+//
+// Rows: a token's query heads that share a kv head are rows of one matrix: row r of a sequence is head r % group of new token r / group.  A CTA is four warps and
+// takes 16 ROWT rows of one kv head and one span of the sequence's pages.  A warp has 16 rows (ROWT row tiles) and all 64 positions of a page
+// (ROWT = 4), half of them (2) or a quarter (1); a warp's sums are its own, the warps of the same rows meet at the end.
+// K and V rows come by one bulk copy each for a page, PGA_BUFS pages on their way.
+constexpr int PGA_WARPS = 4, PGA_THREADS = 32 * PGA_WARPS, PGA_BUFS = 2;
+constexpr int PGA_Q_STRIDE = 64 + 4;                            // words of a quantised row: 4 g + t are 32 different banks
+constexpr int PGA_OUT_BYTES = PGA_WARPS * 16 * KV_D * 4;
+constexpr int PGA_RING_BYTES = PGA_BUFS * 2 * PG_HEAD_BYTES;
+static_assert(PGA_OUT_BYTES <= PGA_RING_BYTES, "the outputs reuse the ring");
+constexpr int pga_smem_bytes(int rowt) { return 128 + PGA_RING_BYTES + 2 * 8 * PG_POS * 4 + 16 * 4 + rowt * 16 * (PGA_Q_STRIDE + 8) * 4 + PGA_WARPS * 16 * 8; }
+
+struct PageAttn {
+    PageCache C;
+    const float *q;
+    float *out;
+    float *part_acc;            // [splits][token * n_head + head][256], with more than one split
+    float2 *part_ml;            // [splits][token * n_head + head]: maximum, sum of weights
+    int layer, n_head, group, pages_per_split, splits;
+    float scale;
+};
+
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t"
+        ".reg .b64 a, b, d;\n\t"
+        "mov.b64 a, {%2, %3};\n\t"
+        "mov.b64 b, {%4, %5};\n\t"
+        "mul.rn.f32x2 d, a, b;\n\t"
+        "mov.b64 {%0, %1}, d;\n\t"
+        "}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+// int8 products of one 32-value block on top of the bits of 12582912: read as floats they are 12582912 + the sum, exactly (|sum| < 2^20)
+__device__ __forceinline__ void pga_mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0x4B400000));
+}
+// bytes (lo, hi halves: of two positions) of the signed words a, b -> fp16 pairs, exactly: 1024 + (byte ^ 128) - 1152
+__device__ __forceinline__ void pga_halves(uint32_t a, uint32_t b, uint32_t (&out)[4]) {
+    a ^= 0x80808080u;
+    b ^= 0x80808080u;
+    const uint32_t lo = __byte_perm(a, b, 0x5140), hi = __byte_perm(a, b, 0x7362);      // a0 b0 a1 b1 | a2 b2 a3 b3
+    const __half2 off = __half2half2(__ushort_as_half((unsigned short)0x6480));       // 1152
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t w = __byte_perm(i < 2 ? lo : hi, 0x64646464u, (i & 1) ? 0x4342 : 0x4140);
+        const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&w), off);
+        out[i] = *reinterpret_cast<const uint32_t *>(&h);
+    }
+}
+
+// grid (row tiles of all sequences and some that find none, kv heads, splits)
+template <int ROWT>
+__global__ void __launch_bounds__(PGA_THREADS, 2) pages_attn_kernel(const __grid_constant__ PageAttn P) {
+    constexpr int KEYW = PGA_WARPS / ROWT;              // warps of the same rows
+    constexpr int KEYS = PG_POS / KEYW, NT = KEYS / 8, ROWS = 16 * ROWT;
+    extern __shared__ __align__(128) uint8_t smem[];
+    uint64_t *kfull = reinterpret_cast<uint64_t *>(smem), *vfull = kfull + PGA_BUFS;
+    int *held = reinterpret_cast<int *>(vfull + PGA_BUFS);                       // [PGA_BUFS] positions of the page that there are
+    uint8_t *ring = smem + 128;
+    float *ks = reinterpret_cast<float *>(ring + PGA_RING_BYTES);                // [8 blocks][64 positions]
+    float *vs = ks + 8 * PG_POS;                                                 // ... times 2^(13 - e), e the exponent of the block's largest
+    float *vfac = vs + 8 * PG_POS;                                               // [8] 2^(e - 13), negative: a second pair of planes is needed; [8] pad
+    uint32_t *q8 = reinterpret_cast<uint32_t *>(vfac + 16);                      // [ROWS][PGA_Q_STRIDE]
+    float *qd = reinterpret_cast<float *>(q8 + ROWS * PGA_Q_STRIDE);             // [ROWS][8] scales of the queries, times the softmax scale
+    float2 *ml = reinterpret_cast<float2 *>(qd + ROWS * 8);                      // [4 warps][16 rows]
+
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int g = lane >> 2, t = lane & 3;
+    const int rt = warp / KEYW, kw = warp % KEYW;
+    const int kvh = blockIdx.y, split = blockIdx.z;
+    const PageCache &C = P.C;
+    if (tid == 0) {
+        for (int b = 0; b < PGA_BUFS; ++b) mbar_init(&kfull[b], 1), mbar_init(&vfull[b], 1);
+        mbar_fence_init();
+    }
+    pdl_wait_prior_grid();
+    pdl_launch_dependents();
+    // whose rows: the sequences' tiles one after the other, every warp for itself
+    int seq, tile;
+    if (!seq_of_item(C.start, C.n_seq, C.n_tok, (int)blockIdx.x, lane, [&](int n) { return ((int64_t)n * P.group + ROWS - 1) / ROWS; }, seq, tile)) return;        // CTA-uniform
+    const SeqRange range = seq_range(C.start, seq, C.n_tok);
+    const int len = C.len[seq];
+    if (len < 0 || len > (int64_t)C.table_stride * PG_POS) {
+        if (tid == 0) bad_sequence();
+        return;
+    }
+    const int n_rows = min(ROWS, range.n * P.group - tile * ROWS);                      // of this tile
+    const int first_tok = tile * ROWS / P.group, last_tok = (tile * ROWS + n_rows - 1) / P.group;
+    const int before = len - range.n;                                                   // positions in front of the new tokens
+    // positions that any row of the tile sees, in pages; this split's
+    const int seen = min(len, before + last_tok + 1);
+    const int pages = (max(seen, 0) + PG_POS - 1) / PG_POS;
+    const int page0 = split * P.pages_per_split, page1 = split == P.splits - 1 ? pages : min(page0 + P.pages_per_split, pages);      // (the last takes what is left)
+    const int ntiles = page1 - page0;
+    if (ntiles <= 0 && split > 0) return;               // (the first split writes the rows that see nothing)
+
+    auto issue = [&](int i) {                           // one thread
+        const int b = i % PGA_BUFS, page = C.table[(size_t)seq * C.table_stride + page0 + i];
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        if (page < 0 || page >= C.n_pages) {
+            bad_sequence();
+            held[b] = 0;
+            mbar_arrive(&kfull[b]);
+            mbar_arrive(&vfull[b]);
+            return;
+        }
+        const uint64_t pol = policy_evict_normal();
+        const int n = min(PG_POS, seen - (page0 + i) * PG_POS);
+        const uint32_t bytes = (uint32_t)n * KV_ROW;
+        uint8_t *dst = ring + (size_t)b * 2 * PG_HEAD_BYTES;
+        held[b] = n;
+        mbar_expect_tx(&kfull[b], bytes);
+        bulk_g2s(dst, page_rows(C, page, P.layer, 0, kvh), bytes, &kfull[b], pol);
+        mbar_expect_tx(&vfull[b], bytes);
+        bulk_g2s(dst + PG_HEAD_BYTES, page_rows(C, page, P.layer, 1, kvh), bytes, &vfull[b], pol);
+    };
+    __syncthreads();
+    if (tid == 0)
+        for (int i = 0; i < min(ntiles, PGA_BUFS); ++i) issue(i);
+    // the rows' queries, quantised as the cache rows are
+    {
+        const int blk = lane >> 2, sub = lane & 3;
+        const bool vec = (reinterpret_cast<uintptr_t>(P.q) & 15u) == 0;
+        for (int r = warp; r < ROWS; r += PGA_WARPS) {
+            float x[8];
+            const int row = tile * ROWS + r, tok = row / P.group, h = row - tok * P.group;
+            const float *qr = P.q + ((size_t)(range.begin + tok) * P.n_head + kvh * P.group + h) * KV_D + blk * 32 + sub * 8;
+            if (r >= n_rows) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = 0.0f;
+            } else if (vec) {
+                const float4 a = *reinterpret_cast<const float4 *>(qr), c = *reinterpret_cast<const float4 *>(qr + 4);
+                x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = c.x; x[5] = c.y; x[6] = c.z; x[7] = c.w;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = qr[i];
+            }
+            const float d = __fmul_rn(kv_amax_8(x), PG_SCALE), id = d > 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
+            uint32_t w[2];
+            kv_words_8(x, id, w);
+            // in the order in which the K rows are read: of an even block slot 0 = values 0, 1, 30, 31, slot i = values 4 i - 2 .. 4 i + 1
+            const uint32_t below = __shfl_up_sync(0xffffffffu, w[1], 1), last = __shfl_sync(0xffffffffu, w[1], lane | 3);
+            uint32_t s0 = w[0], s1 = w[1];
+            if (!(blk & 1)) {
+                s0 = sub ? __byte_perm(below, w[0], 0x5432) : __byte_perm(w[0], last, 0x7610);
+                s1 = __byte_perm(w[0], w[1], 0x5432);
+            }
+            *reinterpret_cast<uint2 *>(q8 + r * PGA_Q_STRIDE + blk * 8 + 2 * sub) = make_uint2(s0, s1);
+            if (sub == 0) qd[r * 8 + blk] = __fmul_rn(f16_bits_to_f32(f32_to_f16_bits_ties_away(d)), P.scale);
+        }
+    }
+    float acc[8][4][4];                                 // block, byte of the slot; (row g | g + 8, slot 2 t | 2 t + 1)
+#pragma unroll
+    for (int b = 0; b < 8; ++b)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[b][j][i] = 0.0f;
+    float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.0f, 0.0f};            // rows g, g + 8; l of this thread's columns
+    // the last position that rows g and g + 8 see
+    int limit[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int r = 16 * rt + g + 8 * i;
+        limit[i] = r < n_rows ? before + (tile * ROWS + r) / P.group : -1;
+    }
+    const int all_see = before + first_tok;             // every row of the tile sees the positions up to this one
+    bool ok = true;
+    for (int i = 0; i < ntiles; ++i) {
+        const int b = i % PGA_BUFS, p0 = (page0 + i) * PG_POS;
+        const uint32_t par = (uint32_t)((i / PGA_BUFS) & 1);
+        const uint8_t *kt = ring + (size_t)b * 2 * PG_HEAD_BYTES, *vt = kt + PG_HEAD_BYTES;
+        ok = mbar_wait_hot(&kfull[b], par) && ok;
+        ok = mbar_wait_hot(&vfull[b], par) && ok;
+        const int n = held[b];
+        {   // the scales, as floats; those behind the last position are zeros
+#pragma unroll
+            for (int blk = 2 * warp; blk < 2 * warp + 2; ++blk) {                // a warp's two blocks, lane = position
+                const int off = 34 * blk;
+                float x[2];
+                uint32_t top = 0, low = 0x7FFFu;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int k = lane + 32 * e;
+                    const uint32_t hk = k < n ? *reinterpret_cast<const unsigned short *>(kt + k * KV_ROW + off) : 0u;
+                    const uint32_t hv = k < n ? *reinterpret_cast<const unsigned short *>(vt + k * KV_ROW + off) : 0u;
+                    ks[blk * PG_POS + k] = f16_bits_to_f32(hk);
+                    x[e] = f16_bits_to_f32(hv);
+                    const uint32_t mag = hv & 0x7FFFu;
+                    if (mag < 0x7C00u) top = max(top, mag);
+                    if (mag) low = min(low, mag);
+                }
+                top = __reduce_max_sync(0xffffffffu, top);
+                low = __reduce_min_sync(0xffffffffu, low);
+                const int e = max((int)(top >> 10), 1);                          // biased fp16 exponent
+                const float up = __uint_as_float((uint32_t)(127 + 28 - e) << 23);                // 2^(13 - (e - 15))
+#pragma unroll
+                for (int j = 0; j < 2; ++j) vs[blk * PG_POS + lane + 32 * j] = __fmul_rn(x[j], up);
+                if (lane == 0) {
+                    const float down = __uint_as_float((uint32_t)(127 - 28 + e) << 23);
+                    vfac[blk] = top && e - max((int)(low >> 10), 1) > KV_V_RANGE ? -down : down;
+                }
+            }
+        }
+        if (!__syncthreads_and(ok ? 1 : 0)) break;      // (a wait ran out: the CTA leaves as a whole)
+        // ---- scores: rows 16 rt .., positions KEYS kw ..
+        float s[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[nt][e] = 0.0f;
+        const uint32_t *qa = q8 + (16 * rt + g) * PGA_Q_STRIDE + t;
+        const float *qs = qd + (16 * rt + g) * 8;
+        const uint32_t *kr = reinterpret_cast<const uint32_t *>(kt) + (size_t)(KEYS * kw + g) * (KV_ROW / 4);
+#pragma unroll
+        for (int blk = 0; blk < 8; ++blk) {
+            const uint32_t a0 = qa[blk * 8], a1 = qa[blk * 8 + 8 * PGA_Q_STRIDE], a2 = qa[blk * 8 + 4], a3 = qa[blk * 8 + 4 + 8 * PGA_Q_STRIDE];
+            const float dq0 = qs[blk], dq1 = qs[64 + blk];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const uint32_t *u = kr + nt * 8 * (KV_ROW / 4) + 17 * (blk >> 1);
+                uint32_t b0, b1;
+                if (blk & 1) {
+                    b0 = u[9 + t];
+                    b1 = u[13 + t];
+                } else {
+                    b0 = u[t];
+                    b1 = u[4 + t];
+                    if (t == 0) b0 = __byte_perm(b0, u[8], 0x5432);
+                }
+                int d[4];
+                pga_mma_s8(d, a0, a1, a2, a3, b0, b1);
+                const float2 dk = *reinterpret_cast<const float2 *>(ks + blk * PG_POS + KEYS * kw + 8 * nt + 2 * t);
+                const float2 low = make_float2(-12582912.0f, -12582912.0f);
+                const float2 x0 = mul2(add2(make_float2(__int_as_float(d[0]), __int_as_float(d[1])), low), dk);
+                const float2 x1 = mul2(add2(make_float2(__int_as_float(d[2]), __int_as_float(d[3])), low), dk);
+                const float2 y0 = fma2(x0, make_float2(dq0, dq0), make_float2(s[nt][0], s[nt][1]));
+                const float2 y1 = fma2(x1, make_float2(dq1, dq1), make_float2(s[nt][2], s[nt][3]));
+                s[nt][0] = y0.x; s[nt][1] = y0.y; s[nt][2] = y1.x; s[nt][3] = y1.y;
+            }
+        }
+        // ---- softmax step of the warp's positions
+        const bool edge = p0 + PG_POS - 1 > all_see || n < PG_POS;               // some row does not see some position
+        if (edge) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int k = KEYS * kw + 8 * nt + 2 * t + (e & 1);
+                    if (p0 + k > limit[e >> 1] || k >= n) s[nt][e] = -INFINITY;
+                }
+        }
+        float alpha[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float mx = s[0][2 * h];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mx = fmaxf(mx, fmaxf(s[nt][2 * h], s[nt][2 * h + 1]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            const float m_new = fmaxf(m_run[h], mx), base = m_new == -INFINITY ? 0.0f : m_new;
+            alpha[h] = expf(__fsub_rn(m_run[h], base));
+            float sum = 0.0f;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                s[nt][2 * h] = expf(__fsub_rn(s[nt][2 * h], base));
+                s[nt][2 * h + 1] = expf(__fsub_rn(s[nt][2 * h + 1], base));
+                sum = __fadd_rn(sum, __fadd_rn(s[nt][2 * h], s[nt][2 * h + 1]));
+            }
+            l_run[h] = __fadd_rn(__fmul_rn(l_run[h], alpha[h]), sum);
+            m_run[h] = m_new;
+        }
+        // ---- values, block by block into fresh sums
+        const uint32_t *vr = reinterpret_cast<const uint32_t *>(vt) + (size_t)(KEYS * kw + 2 * t) * (KV_ROW / 4);
+#pragma unroll
+        for (int blk = 0; blk < 8; ++blk) {
+            float o[4][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
+            const float fac = vfac[blk];
+            auto pass = [&](auto restc) {
+                constexpr bool REST = decltype(restc)::value;
+#pragma unroll
+                for (int kstep = 0; kstep < NT / 2; ++kstep) {
+                    uint32_t ah[4], al[4];
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const float2 dv = *reinterpret_cast<const float2 *>(vs + blk * PG_POS + KEYS * kw + 16 * kstep + 8 * half + 2 * t);
+                        const float *sp = s[2 * kstep + half];
+                        float2 x0 = mul2(make_float2(sp[0], sp[1]), dv), x1 = mul2(make_float2(sp[2], sp[3]), dv);
+                        if (edge) {                     // a position that a row does not see adds nothing, whatever it holds
+                            if (sp[0] == 0.0f) x0.x = 0.0f;
+                            if (sp[1] == 0.0f) x0.y = 0.0f;
+                            if (sp[2] == 0.0f) x1.x = 0.0f;
+                            if (sp[3] == 0.0f) x1.y = 0.0f;
+                        }
+                        split_f16x2(x0.x, x0.y, ah[2 * half], al[2 * half]);
+                        split_f16x2(x1.x, x1.y, ah[2 * half + 1], al[2 * half + 1]);
+                        if (REST) {
+                            uint32_t h2, l2;
+                            h2 = ah[2 * half], l2 = al[2 * half];
+                            split_rest_f16x2(x0.x, x0.y, h2, l2);
+                            ah[2 * half] = h2, al[2 * half] = l2;
+                            h2 = ah[2 * half + 1], l2 = al[2 * half + 1];
+                            split_rest_f16x2(x1.x, x1.y, h2, l2);
+                            ah[2 * half + 1] = h2, al[2 * half + 1] = l2;
+                        }
+                    }
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t *u = vr + (16 * kstep + (e & 1) + 8 * (e >> 1)) * (KV_ROW / 4) + 17 * (blk >> 1);
+                        if (blk & 1) {
+                            w[e] = u[9 + g];
+                        } else {
+                            w[e] = u[g];
+                            if (g == 0) w[e] = __byte_perm(w[e], u[8], 0x5432);
+                        }
+                    }
+                    uint32_t b0[4], b1[4];
+                    pga_halves(w[0], w[1], b0);
+                    pga_halves(w[2], w[3], b1);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        mma_f16_16816(o[j], al[0], al[1], al[2], al[3], b0[j], b1[j]);
+                        mma_f16_16816(o[j], ah[0], ah[1], ah[2], ah[3], b0[j], b1[j]);
+                    }
+                }
+            };
+            if (fac < 0.0f) {                           // scales too far apart for one pair of planes: first what it leaves, times 2^24
+                pass(std::true_type{});
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[j][e] = __fmul_rn(o[j][e], 0x1p-24f);
+            }
+            pass(std::false_type{});
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[blk][j][e] = __fmaf_rn(o[j][e], fabsf(fac), __fmul_rn(acc[blk][j][e], alpha[e >> 1]));
+        }
+        __syncthreads();                                // the page has been read, and the scales
+        if (tid == 0 && i + PGA_BUFS < ntiles) issue(i + PGA_BUFS);
+    }
+    // ---- the warps' sums meet, and leave by whole lines
+    float l[2], m[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        l[h] = __fadd_rn(l_run[h], __shfl_xor_sync(0xffffffffu, l_run[h], 1));
+        l[h] = __fadd_rn(l[h], __shfl_xor_sync(0xffffffffu, l[h], 2));
+        m[h] = m_run[h];
+        if (t == 0) ml[warp * 16 + g + 8 * h] = make_float2(m[h], l[h]);
+    }
+    if (!__syncthreads_and(ok ? 1 : 0)) return;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int w = 0; w < KEYW; ++w) m[h] = fmaxf(m[h], ml[(KEYW * rt + w) * 16 + g + 8 * h].x);
+        const float f = m_run[h] == m[h] ? 1.0f : expf(__fsub_rn(m_run[h], m[h]));       // (also where neither has seen a position)
+        float *dst = reinterpret_cast<float *>(ring) + (size_t)(warp * 16 + g + 8 * h) * KV_D;
+#pragma unroll
+        for (int blk = 0; blk < 8; ++blk)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {               // slot 2 t + c of the block: four values from dim 4 slot (odd block) or 4 slot - 2 (even, round the end)
+                const int slot = 2 * t + c;
+                const float x0 = __fmul_rn(acc[blk][0][2 * h + c], f), x1 = __fmul_rn(acc[blk][1][2 * h + c], f);
+                const float x2 = __fmul_rn(acc[blk][2][2 * h + c], f), x3 = __fmul_rn(acc[blk][3][2 * h + c], f);
+                float *d0 = dst + 32 * blk + ((blk & 1) ? 4 * slot : (slot ? 4 * slot - 2 : 0));
+                float *d1 = dst + 32 * blk + ((blk & 1) ? 4 * slot + 2 : (slot ? 4 * slot : 30));
+                *reinterpret_cast<float2 *>(d0) = make_float2(x0, x1);
+                *reinterpret_cast<float2 *>(d1) = make_float2(x2, x3);
+            }
+    }
+    __syncthreads();
+    const float4 *box = reinterpret_cast<const float4 *>(ring);
+    for (int i = tid; i < n_rows * (KV_D / 4); i += PGA_THREADS) {
+        const int r = i / (KV_D / 4), c = i % (KV_D / 4), part0 = (r >> 4) * KEYW * 16 + (r & 15);       // the first warp's copy of the row
+        float4 x = box[(size_t)part0 * (KV_D / 4) + c];
+        float mm = ml[part0].x;
+#pragma unroll
+        for (int w = 1; w < KEYW; ++w) {
+            const float4 y = box[(size_t)(part0 + 16 * w) * (KV_D / 4) + c];
+            x = make_float4(__fadd_rn(x.x, y.x), __fadd_rn(x.y, y.y), __fadd_rn(x.z, y.z), __fadd_rn(x.w, y.w));
+            mm = fmaxf(mm, ml[part0 + 16 * w].x);
+        }
+        float ll = 0.0f;
+#pragma unroll
+        for (int w = 0; w < KEYW; ++w) {
+            const float2 x = ml[part0 + 16 * w];
+            ll = __fadd_rn(ll, __fmul_rn(x.y, x.x == mm ? 1.0f : expf(__fsub_rn(x.x, mm))));
+        }
+        const int row = tile * ROWS + r, tok = row / P.group;
+        const size_t at = (size_t)(range.begin + tok) * P.n_head + kvh * P.group + (row - tok * P.group);
+        if (P.splits == 1) {
+            const float inv = ll == 0.0f ? 0.0f : __fdiv_rn(1.0f, ll);           // a row that sees nothing is zeros
+            x = make_float4(__fmul_rn(x.x, inv), __fmul_rn(x.y, inv), __fmul_rn(x.z, inv), __fmul_rn(x.w, inv));
+            float *o = P.out + at * KV_D + 4 * c;
+            if ((reinterpret_cast<uintptr_t>(P.out) & 15u) == 0) {
+                *reinterpret_cast<float4 *>(o) = x;
+            } else {
+                o[0] = x.x; o[1] = x.y; o[2] = x.z; o[3] = x.w;
+            }
+        } else {
+            const size_t part = (size_t)split * C.n_tok * P.n_head + at;
+            reinterpret_cast<float4 *>(P.part_acc)[part * (KV_D / 4) + c] = x;
+            if (c == 0) P.part_ml[part] = make_float2(mm, ll);
+        }
+    }
+}
+
+// The splits of a row added up: a warp per row (token, head), eight dims a lane.  A row's splits are those that its sequence's positions reach.
+constexpr int PGJ_WARPS = 4;
+__global__ void __launch_bounds__(32 * PGJ_WARPS) pages_join_kernel(const __grid_constant__ PageAttn P) {
+    const PageCache &C = P.C;
+    const int lane = threadIdx.x & 31;
+    const int64_t row = (int64_t)blockIdx.x * PGJ_WARPS + (threadIdx.x >> 5), rows = (int64_t)C.n_tok * P.n_head;
+    pdl_wait_prior_grid();
+    pdl_launch_dependents();
+    if (row >= rows) return;
+    const int tok = (int)(row / P.n_head);
+    const int s = seq_of_row(C.start, C.n_seq, tok, lane);
+    if (s >= C.n_seq) return;
+    const SeqRange r = seq_range(C.start, s, C.n_tok);
+    const int len = C.len[s];
+    if (r.n <= 0 || tok < r.begin || len < 0 || len > (int64_t)C.table_stride * PG_POS) return;        // not a sequence: the attention has said so
+    // rows of a tile were written by every split that the tile's last row reaches; this row's own positions are enough
+    const int seen = min(len, len - r.n + (tok - r.begin) + 1);
+    const int n = max(1, min(P.splits, ((max(seen, 0) + PG_POS - 1) / PG_POS + P.pages_per_split - 1) / P.pages_per_split));
+    float m = -INFINITY;
+    for (int i = lane; i < n; i += 32) m = fmaxf(m, P.part_ml[i * rows + row].x);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+    float l = 0.0f;
+    for (int i = 0; i < n; ++i) {
+        const float2 x = P.part_ml[i * rows + row];
+        const float w = x.x == m ? 1.0f : expf(__fsub_rn(x.x, m));
+        const float4 *src = reinterpret_cast<const float4 *>(P.part_acc) + (i * rows + row) * (KV_D / 4) + lane;
+        const float4 c = src[0], d = src[32];
+        l = __fmaf_rn(x.y, w, l);
+        a = make_float4(__fmaf_rn(c.x, w, a.x), __fmaf_rn(c.y, w, a.y), __fmaf_rn(c.z, w, a.z), __fmaf_rn(c.w, w, a.w));
+        b = make_float4(__fmaf_rn(d.x, w, b.x), __fmaf_rn(d.y, w, b.y), __fmaf_rn(d.z, w, b.z), __fmaf_rn(d.w, w, b.w));
+    }
+    const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+    float *o = P.out + row * KV_D + 4 * lane;
+    const float x[8] = {__fmul_rn(a.x, inv), __fmul_rn(a.y, inv), __fmul_rn(a.z, inv), __fmul_rn(a.w, inv),
+                        __fmul_rn(b.x, inv), __fmul_rn(b.y, inv), __fmul_rn(b.z, inv), __fmul_rn(b.w, inv)};
+    if ((reinterpret_cast<uintptr_t>(P.out) & 15u) == 0) {
+        *reinterpret_cast<float4 *>(o) = make_float4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<float4 *>(o + 128) = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = x[e], o[128 + e] = x[4 + e];
+    }
+}
+
+}  // namespace b200

@@ -8,6 +8,7 @@
 // The library itself is not linked: bind() takes the addresses that the loaded library exports, so that one build of
 // this module serves any build of the library.
 #include <torch/csrc/autograd/python_variable.h>
+#include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 
 #include <cstdint>
@@ -21,6 +22,9 @@ namespace {
 // Kinds of argument beside plain numbers: device memory (a CUDA tensor or None), a handle (an integer or an object with
 // an integer `value`, as ctypes makes them), a truth value.
 struct Mem { void *p; };
+struct Dev { void *p; };                // device memory of the current device
+struct Strided { void *p; };            // ... whose strides are arguments of the call, so that it need not be contiguous
+struct Ints { const void *p; int64_t n; };      // host memory: an int32 tensor
 struct Handle { void *p; };
 struct Truth { int v; };
 
@@ -68,6 +72,43 @@ bool get(PyObject *o, const char *name, Mem &out) {
     out.p = t.mutable_data_ptr();           // outputs are written: a tensor that shares its memory until then gets its own, as by data_ptr()
     return true;
 }
+bool here(PyObject *o, const char *name) {
+    if (o == Py_None || !THPVariable_Check(o) || !THPVariable_Unpack(o).is_cuda()) return true;
+    const int at = (int)THPVariable_Unpack(o).get_device(), now = (int)c10::cuda::current_device();
+    if (at != now) PyErr_Format(PyExc_RuntimeError, "%s is on device %d, the current device is %d", name, at, now);
+    return at == now;
+}
+bool get(PyObject *o, const char *name, Dev &out) {
+    Mem m{};
+    if (!here(o, name) || !get(o, name, m)) return false;
+    out.p = m.p;
+    return true;
+}
+bool get(PyObject *o, const char *name, Strided &out) {
+    if (!THPVariable_Check(o)) {
+        Mem m{};
+        if (!get(o, name, m)) return false;
+        out.p = m.p;
+        return true;
+    }
+    const at::Tensor &t = THPVariable_Unpack(o);
+    if (!t.is_cuda()) {
+        PyErr_Format(PyExc_RuntimeError, "%s must be a CUDA tensor: this library has no CPU path", name);
+        return false;
+    }
+    if (!here(o, name)) return false;
+    out.p = t.mutable_data_ptr();
+    return true;
+}
+bool get(PyObject *o, const char *name, Ints &out) {
+    if (!THPVariable_Check(o) || !THPVariable_Unpack(o).is_cpu() || THPVariable_Unpack(o).scalar_type() != at::kInt || !THPVariable_Unpack(o).is_contiguous()) {
+        PyErr_Format(PyExc_RuntimeError, "%s must be a contiguous int32 tensor in host memory", name);
+        return false;
+    }
+    out.p = THPVariable_Unpack(o).data_ptr();
+    out.n = THPVariable_Unpack(o).numel();
+    return true;
+}
 bool get(PyObject *o, const char *, Handle &out) {
     if (o == Py_None) {
         out.p = nullptr;
@@ -108,12 +149,19 @@ bool get(PyObject *o, const char *, float &out) {
 }
 
 void *raw(Mem m) { return m.p; }
+void *raw(Dev m) { return m.p; }
+void *raw(Strided m) { return m.p; }
+const void *raw(Ints m) { return m.p; }
 void *raw(Handle h) { return h.p; }
 int raw(Truth t) { return t.v; }
 template <typename T> T raw(T v) { return v; }
 template <typename T> using Raw = decltype(raw(std::declval<T>()));
 
-constexpr int MAX_ARGS = 12;
+constexpr int MAX_ARGS = 20;
+
+// Host lists are as long as the call's last argument says.
+template <typename T> bool long_enough(const T &, int64_t) { return true; }
+inline bool long_enough(const Ints &v, int64_t n) { return v.n >= n; }
 
 // One exported function: its address, filled in by bind(), and the names of its arguments.
 template <typename... A>
@@ -128,6 +176,12 @@ struct Call {
     PyObject *go(PyObject *const *v, std::index_sequence<I...>) {
         std::tuple<A...> a{};
         if (!(get(v[I], args[I], std::get<I>(a)) && ...)) return nullptr;
+        if constexpr ((std::is_same_v<A, Ints> || ...)) {
+            if (!(long_enough(std::get<I>(a), std::get<N - 1>(a)) && ...)) {
+                PyErr_Format(PyExc_RuntimeError, "%s: a list is shorter than %s", name, args[N - 1]);
+                return nullptr;
+            }
+        }
         void *stream = c10::cuda::getCurrentCUDAStream().stream();
         int rc;
         Py_BEGIN_ALLOW_THREADS
@@ -191,6 +245,16 @@ Call<Mem, Mem, Mem, int64_t, int64_t, Truth> quant_batch{"quant_batch", {"X", "s
 Call<Mem, Mem, Mem, Mem, Mem, int64_t, int64_t> linear{"linear", {"W", "x", "signs", "y", "xq_scratch", "n_out", "n_in"}};
 Call<Mem, Mem, Mem, Mem, int64_t, int64_t> linear_static{"linear_static", {"W", "x", "signs", "y", "n_out", "n_in"}};
 Call<Handle> chain_run{"chain_run", {"chain"}};
+Call<Strided, Strided, Dev, Dev, Dev, Dev, Dev, Dev, int64_t, int, int, int, int, int64_t, int64_t, int64_t, int64_t, float> qk_norm_rope{
+    "qk_norm_rope", {"q", "k", "q_weight", "k_weight", "pos", "freq", "q_out", "k_out", "n_tok", "n_head", "n_head_kv", "head_dim", "n_rot", "q_tok_stride",
+                     "q_head_stride", "k_tok_stride", "k_head_stride", "eps"}};
+Call<Handle, int, Dev, Dev> pages_append{"pages_append", {"pages", "layer", "k", "v"}};
+Call<Handle, int, Dev, Dev, int, int, Dev, int64_t, float> pages_attn{
+    "pages_attn", {"pages", "layer", "q", "out", "n_head", "max_len", "workspace", "workspace_bytes", "scale"}};
+Call<Dev, int64_t, int, Ints, Ints, int> pages_copy{"pages_copy", {"pool", "page_bytes", "n_pages", "src", "dst", "n"}};
+Call<Dev, Dev, Dev, Dev, Dev, Dev, Dev, Dev, Dev, Dev, int64_t, int, int, int, int, int, int, int> gdn_seqs{
+    "gdn_seqs", {"state", "q", "k", "v", "g", "beta", "out", "start", "slot", "workspace", "workspace_bytes", "n_seq", "n_slots", "n_tok", "n_k_heads",
+                 "n_v_heads", "K", "V"}};
 // include/bonsai_kv.h
 Call<Handle, int, int, Mem, Mem> kv_append{"kv_append", {"kv", "layer", "pos", "k", "v"}};
 Call<Handle, int, int, int, Mem, Mem> kv_append_batch{"kv_append_batch", {"kv", "layer", "pos0", "n_tok", "k", "v"}};
@@ -199,7 +263,7 @@ Call<Handle, int, int, Mem, Mem> kv_attn_decode{"kv_attn_decode", {"kv", "layer"
 #define EACH_CALL(X)                                                                                                  \
     X(gemv) X(quant_activations) X(gemm) X(repack) X(gemv_repack) X(fwht) X(rmsnorm) X(gdn_step) X(attn)                \
     X(fwht_quant) X(swiglu) X(quant_batch) X(linear) X(linear_static) X(chain_run) X(kv_append) X(kv_append_batch)      \
-    X(kv_attn_decode)
+    X(kv_attn_decode) X(qk_norm_rope) X(pages_append) X(pages_attn) X(pages_copy) X(gdn_seqs)
 
 #define WRAPPER(f)                                                                                                    \
     PyObject *py_##f(PyObject *, PyObject *const *v, Py_ssize_t n, PyObject *kw) { return f.call(v, n, kw); }

@@ -1,0 +1,190 @@
+"""Calls for several sequences: what is refused before anything is launched, workspace sizes, and the host's book of pages."""
+import ctypes as C
+import random
+
+import pytest
+
+ONE = 16            # an aligned address that no refused call reads
+
+
+def test_head_norm_refusals():
+    import bonsai_b200
+    f = bonsai_b200.lib().bonsai_b200_qk_norm_rope
+
+    def call(n_tok=2, n_head=4, n_head_kv=2, dim=256, n_rot=64, qt=1024, qh=256, kt=512, kh=256, q=ONE, pos=ONE, freq=ONE):
+        return f(q, ONE, ONE, ONE, pos, freq, ONE, ONE, n_tok, n_head, n_head_kv, dim, n_rot, qt, qh, kt, kh, 1e-6, None)
+    for bad in ({"dim": 0}, {"dim": 257}, {"n_rot": 63}, {"n_rot": 258}, {"n_rot": -2}, {"n_head": -1}, {"n_head_kv": -1}, {"q": None}, {"q": 18}, {"pos": None},
+                {"freq": None}, {"freq": 20}, {"qh": 255}, {"qt": 1023}, {"qt": -1024}, {"kt": 511}, {"n_tok": 1 << 31}):
+        assert call(**bad) == 1, bad
+    assert call(n_tok=0) == 0 and call(n_head=0, n_head_kv=0) == 0
+
+
+def struct(**kw):
+    import bonsai_b200
+    have = dict(pool=ONE, table=ONE, len=ONE, start=ONE, n_pages=4, n_layers=2, n_head_kv=4, n_seq=2, table_stride=3, n_tok=5)
+    have.update(kw)
+    return bonsai_b200.PagesStruct(**have)
+
+
+BAD_CACHES = ({"pool": None}, {"pool": 24}, {"table": None}, {"table": 18}, {"len": None}, {"start": 17}, {"n_pages": 0}, {"n_layers": 0}, {"n_head_kv": 0}, {"n_seq": -1},
+              {"table_stride": 0}, {"n_tok": -1})
+
+
+def test_cache_refusals():
+    import bonsai_b200
+    L = bonsai_b200.lib()
+
+    def append(layer=0, k=ONE, v=ONE, **kw):
+        return L.bonsai_b200_pages_append(C.byref(struct(**kw)), layer, k, v, None)
+
+    def attn(layer=0, q=ONE, out=ONE, n_head=24, max_len=100, ws=None, ws_bytes=0, **kw):
+        return L.bonsai_b200_pages_attn(C.byref(struct(**kw)), layer, q, out, n_head, max_len, ws, ws_bytes, 0.0625, None)
+    for bad in BAD_CACHES + ({"layer": -1}, {"layer": 2}):
+        assert append(**bad) == 1, bad
+        assert attn(**bad) == 1, bad
+    assert append(k=None) == 1 and append(v=18) == 1
+    assert L.bonsai_b200_pages_append(None, 0, ONE, ONE, None) == 1
+    assert attn(n_head=0) == 1 and attn(n_head=6) == 1 and attn(max_len=-1) == 1 and attn(q=None) == 1 and attn(out=18) == 1
+    for none in ({"n_seq": 0}, {"n_tok": 0}):
+        assert append(**none) == 0 and attn(**none) == 0
+    # a workspace that is too small, missing or not aligned
+    need = L.bonsai_b200_pages_attn_workspace(5, 30000, 2, 24, 4)
+    assert need > 0
+    assert attn(max_len=30000) == 1 and attn(max_len=30000, ws=ONE, ws_bytes=need - 1) == 1 and attn(max_len=30000, ws=24, ws_bytes=need) == 1
+
+
+def test_workspace_sizes():
+    import bonsai_b200 as bb
+    assert bb.pages_attn_workspace(1, 64, 1, 24, 4) == 0
+    for bad in ((0, 64, 1, 24, 4), (1, 0, 1, 24, 4), (1, 64, 0, 24, 4), (1, 64, 1, 24, 5), (1, 64, 1, 0, 4), (1, 64, 1, 24, 0), (1 << 30, 64, 1, 24, 4)):
+        assert bb.pages_attn_workspace(*bad) == 0
+    assert bb.pages_attn_workspace(1, 262144, 1, 24, 4) % 16 == 0
+    for bad in ((0, 1, 16, 48, 128, 128), (1, 0, 16, 48, 128, 128), (1, 1, 16, 47, 128, 128), (1, 1, 16, 48, 129, 128), (1, 1, 16, 48, 128, 100)):
+        assert bb.gdn_seqs_workspace(*bad) == 0
+
+
+def test_copy_refusals():
+    import bonsai_b200
+    f = bonsai_b200.lib().bonsai_b200_pages_copy
+
+    def call(src, dst, pool=ONE, page_bytes=32, n_pages=8):
+        n = len(src)
+        ints = lambda v: (C.c_int32 * max(1, n))(*v)  # noqa: E731
+        return f(pool, page_bytes, n_pages, ints(src), ints(dst), n, None)
+    assert call([0], [8]) == 1 and call([-1], [0]) == 1 and call([8], [0]) == 1 and call([0], [-1]) == 1
+    assert call([0, 1], [5, 5]) == 1            # written twice
+    assert call([0, 5], [5, 6]) == 1            # written and read, either order
+    assert call([5, 0], [6, 5]) == 1
+    assert call([3], [3]) == 1
+    assert call([0], [1], pool=None) == 1 and call([0], [1], pool=8) == 1 and call([0], [1], page_bytes=24) == 1 and call([0], [1], page_bytes=0) == 1
+    assert call([0], [1], n_pages=0) == 1
+    assert call([], []) == 0
+    assert f(ONE, 32, 8, None, None, 1, None) == 1 and f(ONE, 32, 8, None, None, -1, None) == 1
+
+
+def test_delta_refusals():
+    import bonsai_b200
+    f = bonsai_b200.lib().bonsai_b200_gdn_seqs
+
+    def call(state=ONE, start=ONE, slot=None, n_seq=2, n_slots=2, n_tok=5, kh=16, vh=48, K=128, V=128):
+        return f(state, ONE, ONE, ONE, ONE, ONE, ONE, start, slot, None, 0, n_seq, n_slots, n_tok, kh, vh, K, V, None)
+    for bad in ({"state": None}, {"start": 18}, {"slot": 18}, {"n_seq": -1}, {"n_slots": 1}, {"n_slots": -1, "slot": ONE}, {"n_tok": -1}, {"kh": 15}, {"vh": 0}, {"kh": 0}, {"K": 0},
+                {"K": 129}, {"V": 33}, {"V": 0}, {"n_seq": 65536, "n_slots": 65536}):
+        assert call(**bad) == 1, bad
+    assert call(n_tok=0) == 0 and call(n_seq=0) == 0
+
+
+def test_python_refusals():
+    import torch
+    import bonsai_b200 as bb
+    x = torch.zeros(64)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        bb.qk_norm_rope(x, x, x, x, x, x, x, x, 1, 1, 1, 64, 0, 64, 64, 64, 64, 1e-6)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        bb.gdn_seqs(x, x, x, x, x, x, x, x, None, None, 0, 1, 1, 1, 1, 1, 32, 32)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        bb.Pages(x.byte(), x.int().reshape(1, -1), x[:1].int(), x[:2].int(), 1, 1, 1)
+
+
+# ---- the book ------------------------------------------------------------------------------------------
+def check(book, n_pages):
+    users = [0] * n_pages
+    for pages, length in book._seqs.values():
+        assert len(pages) == -(-length // 64) and len(set(pages)) == len(pages)
+        for p in pages:
+            users[p] += 1
+    assert users == book.users and sorted(book._free) == [p for p in range(n_pages) if not users[p]]
+
+
+def test_book_against_contents():
+    """What each position holds, followed through a thousand random calls by a pool of marks."""
+    from bonsai_b200.pages import NoRoom, PageBook
+    rng = random.Random(7)
+    n_pages = 40
+    book, pool, want, mark = PageBook(n_pages), [[None] * 64 for _ in range(n_pages)], {}, 0
+
+    def copy(src, dst):
+        assert len(src) == len(dst) and not set(src) & set(dst) and len(set(dst)) == len(dst)
+        for s, d in zip(src, dst):
+            pool[d] = list(pool[s])
+    for _ in range(1000):
+        seqs = list(want)
+        op = rng.choice(["new", "extend", "extend", "extend", "fork", "truncate", "free", "compact"])
+        if op == "new" and len(seqs) < 8:
+            want[book.new()] = []
+        elif op == "compact":
+            copy(*book.compact())
+            used = n_pages - book.free_pages
+            assert all(book.users[:used]) and not any(book.users[used:])
+        elif seqs:
+            s = rng.choice(seqs)
+            if op == "extend":
+                n, was = rng.choice([0, 1, 5, 63, 64, 130]), (list(book.users), book.pages(s), book.length(s))
+                try:
+                    copy(*book.extend(s, n))
+                except NoRoom:
+                    assert was == (book.users, book.pages(s), book.length(s))
+                    continue
+                for _ in range(n):
+                    mark += 1
+                    p = len(want[s])
+                    pool[book.pages(s)[p // 64]][p % 64] = mark
+                    want[s].append(mark)
+            elif op == "fork" and len(seqs) < 8:
+                want[book.fork(s)] = list(want[s])
+            elif op == "truncate":
+                n = rng.randint(0, len(want[s]))
+                book.truncate(s, n)
+                del want[s][n:]
+            elif op == "free" and rng.random() < 0.3:
+                book.free(s)
+                del want[s]
+        check(book, n_pages)
+        for s, marks in want.items():
+            assert book.length(s) == len(marks)
+            assert [pool[book.pages(s)[p // 64]][p % 64] for p in range(len(marks))] == marks
+
+
+def test_book_refusals():
+    from bonsai_b200.pages import NoRoom, PageBook
+    with pytest.raises(ValueError):
+        PageBook(0)
+    book = PageBook(2)
+    s = book.new()
+    assert book.extend(s, 65) == ([], [])
+    with pytest.raises(NoRoom):
+        book.extend(s, 64)
+    with pytest.raises(ValueError):
+        book.extend(s, -1)
+    with pytest.raises(ValueError):
+        book.truncate(s, 66)
+    with pytest.raises(ValueError):
+        book.tables([s], 1)
+    assert book.tables([s], 3) == ([[0, 1, 0]], [65])
+    t = book.fork(s)
+    with pytest.raises(NoRoom):                 # the shared last page would have to be copied
+        book.extend(t, 1)
+    book.free(s)
+    assert book.extend(t, 1) == ([], []) and book.free_pages == 0
+    with pytest.raises(KeyError):
+        book.length(s)
