@@ -1926,8 +1926,10 @@ PagesPlan plan_pages(int n_tok, int max_len, int n_seq, int n_head, int n_head_k
     p.rowt = each <= 16 ? 1 : each <= 32 ? 2 : 4;
     const int64_t high = 16 * p.rowt;
     p.tiles = (rows + (int64_t)std::min(n_seq, n_tok) * (high - 1)) / high;
-    const int64_t items = std::max<int64_t>(1, rows / high) * n_head_kv, pages = std::max(1, (int)(((int64_t)max_len + PG_POS - 1) / PG_POS));
-    const int64_t want = std::max<int64_t>(4, (items * pages + 4 * 2 * SM_COUNT - 1) / (4 * 2 * SM_COUNT));
+    // A span of pages for each of the CTAs that are resident at once.  Of several sequences the longest is known only: they are taken to hold 3 / 8 of that.
+    const int64_t items = std::max<int64_t>(1, (rows + high - 1) / high) * n_head_kv, pages = std::max(1, (int)(((int64_t)max_len + PG_POS - 1) / PG_POS));
+    const int64_t load = n_seq > 1 ? items * pages * 3 / 8 : items * pages;
+    const int64_t want = std::max<int64_t>(2, (load + 2 * SM_COUNT - 1) / (2 * SM_COUNT));
     p.pages_per_split = (int)std::min(want, pages);
     p.splits = (int)((pages + p.pages_per_split - 1) / p.pages_per_split);
     return p;
@@ -2012,9 +2014,11 @@ int bonsai_b200_pages_attn(const bonsai_b200_pages *pages, int layer, const floa
     };
     cudaError_t e = plan.rowt == 1 ? run(pages_attn_kernel<1>, opt[0]) : plan.rowt == 2 ? run(pages_attn_kernel<2>, opt[1]) : run(pages_attn_kernel<4>, opt[2]);
     if (e == cudaSuccess && plan.splits > 1) {
-        const int64_t ctas = ((int64_t)C.n_tok * n_head + PGJ_WARPS - 1) / PGJ_WARPS;
+        const int roww = plan.splits >= 24 ? 8 : plan.splits >= 6 ? 2 : 1;
+        const int64_t ctas = ((int64_t)C.n_tok * n_head * roww + PGJ_WARPS - 1) / PGJ_WARPS;
         if (ctas > INT32_MAX) return 1;
-        e = launch(pages_join_kernel, dim3((unsigned)ctas), dim3(32 * PGJ_WARPS), 0, as_stream(stream), true, P);
+        auto join = [&](auto kernel) { return launch(kernel, dim3((unsigned)ctas), dim3(32 * PGJ_WARPS), 0, as_stream(stream), true, P); };
+        e = roww == 8 ? join(pages_join_kernel<8>) : roww == 2 ? join(pages_join_kernel<2>) : join(pages_join_kernel<1>);
     }
     return (int)e;
 }

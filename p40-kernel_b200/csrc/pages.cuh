@@ -108,15 +108,21 @@ __global__ void __launch_bounds__(PG_COPY_THREADS) pages_copy_kernel(const __gri
 //   output   sum of p dv v8 / sum of p, p = e^(score - maximum)          p dv in two fp16 planes, v8 as fp16 (exact), fp32 sums
 //
 // Rows: a token's query heads that share a kv head are rows of one matrix: row r of a sequence is head r % group of new token r / group.  A CTA is four warps and
-// takes 16 ROWT rows of one kv head and one span of the sequence's pages.  A warp has 16 rows (ROWT row tiles) and all 64 positions of a page
-// (ROWT = 4), half of them (2) or a quarter (1); a warp's sums are its own, the warps of the same rows meet at the end.
-// K and V rows come by one bulk copy each for a page, PGA_BUFS pages on their way.
+// takes 16 ROWT rows of one kv head and one span of the sequence's pages, a page at a time:
+//   scales   the page's fp16 scales as floats, the V ones of a block under a power of two of their own
+//   scores   a warp has 16 rows and all 64 positions (ROWT = 4), half of them (2) or a quarter (1); weights in fp32 to shared memory
+//   outputs  a warp has all rows and 64 dims (two blocks): V's bytes become fp16 once for all rows.  A page's sums are fresh ones, added to the fp32 output by rounded
+//            operations (the tensor core cuts the last bits of a sum off)
+// K and V rows come by one bulk copy each for a page; a page's room is given to the next but one when every warp has left it.
 constexpr int PGA_WARPS = 4, PGA_THREADS = 32 * PGA_WARPS, PGA_BUFS = 2;
 constexpr int PGA_Q_STRIDE = 64 + 4;                            // words of a quantised row: 4 g + t are 32 different banks
-constexpr int PGA_OUT_BYTES = PGA_WARPS * 16 * KV_D * 4;
+constexpr int PGA_W_STRIDE = PG_POS + 8;                        // weights of a row: pairs at 8 g + 2 t, of four rows, are 32 different banks
 constexpr int PGA_RING_BYTES = PGA_BUFS * 2 * PG_HEAD_BYTES;
-static_assert(PGA_OUT_BYTES <= PGA_RING_BYTES, "the outputs reuse the ring");
-constexpr int pga_smem_bytes(int rowt) { return 128 + PGA_RING_BYTES + 2 * 8 * PG_POS * 4 + 16 * 4 + rowt * 16 * (PGA_Q_STRIDE + 8) * 4 + PGA_WARPS * 16 * 8; }
+static_assert(64 * KV_D * 4 <= PGA_RING_BYTES, "the outputs reuse the ring");
+constexpr int pga_smem_bytes(int rowt) {
+    const int rows = 16 * rowt, keyw = PGA_WARPS / rowt;
+    return 128 + PGA_RING_BYTES + 3 * 8 * PG_POS * 4 + 16 * 4 + rows * (PGA_Q_STRIDE + 8 + PGA_W_STRIDE) * 4 + rows * (2 + 2 * keyw) * 4;
+}
 
 struct PageAttn {
     PageCache C;
@@ -164,18 +170,21 @@ __device__ __forceinline__ void pga_halves(uint32_t a, uint32_t b, uint32_t (&ou
 // grid (row tiles of all sequences and some that find none, kv heads, splits)
 template <int ROWT>
 __global__ void __launch_bounds__(PGA_THREADS, 2) pages_attn_kernel(const __grid_constant__ PageAttn P) {
-    constexpr int KEYW = PGA_WARPS / ROWT;              // warps of the same rows
+    constexpr int KEYW = PGA_WARPS / ROWT;              // warps that share the scores of 16 rows
     constexpr int KEYS = PG_POS / KEYW, NT = KEYS / 8, ROWS = 16 * ROWT;
     extern __shared__ __align__(128) uint8_t smem[];
     uint64_t *kfull = reinterpret_cast<uint64_t *>(smem), *vfull = kfull + PGA_BUFS;
     int *held = reinterpret_cast<int *>(vfull + PGA_BUFS);                       // [PGA_BUFS] positions of the page that there are
+    int *wide0 = held + PGA_BUFS;                                                // [2][8] the block's scales of V are too far apart for one pair of planes
     uint8_t *ring = smem + 128;
     float *ks = reinterpret_cast<float *>(ring + PGA_RING_BYTES);                // [8 blocks][64 positions]
-    float *vs = ks + 8 * PG_POS;                                                 // ... times 2^(13 - e), e the exponent of the block's largest
-    float *vfac = vs + 8 * PG_POS;                                               // [8] 2^(e - 13), negative: a second pair of planes is needed; [8] pad
-    uint32_t *q8 = reinterpret_cast<uint32_t *>(vfac + 16);                      // [ROWS][PGA_Q_STRIDE]
+    float *vs0 = ks + 8 * PG_POS;                                                // the same of V times 2^(13 - e), e the exponent of the block's largest; pages alternate
+    float *vfac0 = vs0 + 2 * 8 * PG_POS;                                         // [2][8] 2^(e - 13), negative: the block is to be looked at closely
+    uint32_t *q8 = reinterpret_cast<uint32_t *>(vfac0 + 16);                     // [ROWS][PGA_Q_STRIDE]
     float *qd = reinterpret_cast<float *>(q8 + ROWS * PGA_Q_STRIDE);             // [ROWS][8] scales of the queries, times the softmax scale
-    float2 *ml = reinterpret_cast<float2 *>(qd + ROWS * 8);                      // [4 warps][16 rows]
+    float *wt = qd + ROWS * 8;                                                   // [ROWS][PGA_W_STRIDE] weights
+    float *alphas = wt + ROWS * PGA_W_STRIDE, *sums = alphas + ROWS;             // [ROWS] each: e^(old maximum - new), sum of weights
+    float *most = sums + ROWS, *part = most + KEYW * ROWS;                       // [KEYW][ROWS] each: a warp's maxima, its sums
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t = lane & 3;
@@ -192,6 +201,9 @@ __global__ void __launch_bounds__(PGA_THREADS, 2) pages_attn_kernel(const __grid
     int seq, tile;
     if (!seq_of_item(C.start, C.n_seq, C.n_tok, (int)blockIdx.x, lane, [&](int n) { return ((int64_t)n * P.group + ROWS - 1) / ROWS; }, seq, tile)) return;        // CTA-uniform
     const SeqRange range = seq_range(C.start, seq, C.n_tok);
+    const int page0 = split * P.pages_per_split;
+    const int32_t *table = C.table + (size_t)seq * C.table_stride;
+    const int ahead[2] = {page0 < C.table_stride ? table[page0] : -1, page0 + 1 < C.table_stride ? table[page0 + 1] : -1};       // asked for beside the length
     const int len = C.len[seq];
     if (len < 0 || len > (int64_t)C.table_stride * PG_POS) {
         if (tid == 0) bad_sequence();
@@ -203,12 +215,12 @@ __global__ void __launch_bounds__(PGA_THREADS, 2) pages_attn_kernel(const __grid
     // positions that any row of the tile sees, in pages; this split's
     const int seen = min(len, before + last_tok + 1);
     const int pages = (max(seen, 0) + PG_POS - 1) / PG_POS;
-    const int page0 = split * P.pages_per_split, page1 = split == P.splits - 1 ? pages : min(page0 + P.pages_per_split, pages);      // (the last takes what is left)
+    const int page1 = split == P.splits - 1 ? pages : min(page0 + P.pages_per_split, pages);          // (the last takes what is left)
     const int ntiles = page1 - page0;
     if (ntiles <= 0 && split > 0) return;               // (the first split writes the rows that see nothing)
 
     auto issue = [&](int i) {                           // one thread
-        const int b = i % PGA_BUFS, page = C.table[(size_t)seq * C.table_stride + page0 + i];
+        const int b = i % PGA_BUFS, page = i < 2 ? ahead[i] : table[page0 + i];
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         if (page < 0 || page >= C.n_pages) {
             bad_sequence();
@@ -234,6 +246,7 @@ __global__ void __launch_bounds__(PGA_THREADS, 2) pages_attn_kernel(const __grid
     {
         const int blk = lane >> 2, sub = lane & 3;
         const bool vec = (reinterpret_cast<uintptr_t>(P.q) & 15u) == 0;
+#pragma unroll 4
         for (int r = warp; r < ROWS; r += PGA_WARPS) {
             float x[8];
             const int row = tile * ROWS + r, tok = row / P.group, h = row - tok * P.group;
@@ -262,15 +275,17 @@ __global__ void __launch_bounds__(PGA_THREADS, 2) pages_attn_kernel(const __grid
             if (sub == 0) qd[r * 8 + blk] = __fmul_rn(f16_bits_to_f32(f32_to_f16_bits_ties_away(d)), P.scale);
         }
     }
-    float acc[8][4][4];                                 // block, byte of the slot; (row g | g + 8, slot 2 t | 2 t + 1)
+    float acc[ROWT][2][4][4];                           // row tile, the warp's block, byte of the slot; (row g | g + 8, slot 2 t | 2 t + 1)
 #pragma unroll
-    for (int b = 0; b < 8; ++b)
+    for (int m = 0; m < ROWT; ++m)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[b][j][i] = 0.0f;
-    float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.0f, 0.0f};            // rows g, g + 8; l of this thread's columns
-    // the last position that rows g and g + 8 see
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[m][b][j][i] = 0.0f;
+    float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.0f, 0.0f};            // rows 16 rt + g, + 8; l of this thread's columns
+    // the last position that they see
     int limit[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -283,78 +298,87 @@ __global__ void __launch_bounds__(PGA_THREADS, 2) pages_attn_kernel(const __grid
         const int b = i % PGA_BUFS, p0 = (page0 + i) * PG_POS;
         const uint32_t par = (uint32_t)((i / PGA_BUFS) & 1);
         const uint8_t *kt = ring + (size_t)b * 2 * PG_HEAD_BYTES, *vt = kt + PG_HEAD_BYTES;
+        float *vs = vs0 + (i & 1) * 8 * PG_POS, *vfac = vfac0 + (i & 1) * 8;
         ok = mbar_wait_hot(&kfull[b], par) && ok;
         ok = mbar_wait_hot(&vfull[b], par) && ok;
         const int n = held[b];
-        {   // the scales, as floats; those behind the last position are zeros
+        // ---- scales; those behind the last position are zeros
 #pragma unroll
-            for (int blk = 2 * warp; blk < 2 * warp + 2; ++blk) {                // a warp's two blocks, lane = position
-                const int off = 34 * blk;
-                float x[2];
-                uint32_t top = 0, low = 0x7FFFu;
+        for (int blk = 2 * warp; blk < 2 * warp + 2; ++blk) {                    // a warp's two blocks, lane = position
+            const int off = 34 * blk;
+            float x[2];
+            uint32_t top = 0, low = 0x7FFFu;
+            bool odd = false;
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int k = lane + 32 * e;
-                    const uint32_t hk = k < n ? *reinterpret_cast<const unsigned short *>(kt + k * KV_ROW + off) : 0u;
-                    const uint32_t hv = k < n ? *reinterpret_cast<const unsigned short *>(vt + k * KV_ROW + off) : 0u;
-                    ks[blk * PG_POS + k] = f16_bits_to_f32(hk);
-                    x[e] = f16_bits_to_f32(hv);
-                    const uint32_t mag = hv & 0x7FFFu;
-                    if (mag < 0x7C00u) top = max(top, mag);
-                    if (mag) low = min(low, mag);
-                }
-                top = __reduce_max_sync(0xffffffffu, top);
-                low = __reduce_min_sync(0xffffffffu, low);
-                const int e = max((int)(top >> 10), 1);                          // biased fp16 exponent
-                const float up = __uint_as_float((uint32_t)(127 + 28 - e) << 23);                // 2^(13 - (e - 15))
+            for (int e = 0; e < 2; ++e) {
+                const int k = lane + 32 * e;
+                const uint32_t hk = k < n ? *reinterpret_cast<const unsigned short *>(kt + k * KV_ROW + off) : 0u;
+                const uint32_t hv = k < n ? *reinterpret_cast<const unsigned short *>(vt + k * KV_ROW + off) : 0u;
+                ks[blk * PG_POS + k] = f16_bits_to_f32(hk);
+                x[e] = f16_bits_to_f32(hv);
+                const uint32_t mag = hv & 0x7FFFu;
+                if (mag < 0x7C00u) top = max(top, mag);
+                else odd = true;
+                if (mag) low = min(low, mag);
+            }
+            top = __reduce_max_sync(0xffffffffu, top);
+            low = __reduce_min_sync(0xffffffffu, low);
+            odd = __any_sync(0xffffffffu, odd);
+            const int e = max((int)(top >> 10), 1);                              // biased fp16 exponent
+            const float up = __uint_as_float((uint32_t)(127 + 28 - e) << 23), down = __uint_as_float((uint32_t)(127 - 28 + e) << 23);       // 2^(13 - (e - 15))
 #pragma unroll
-                for (int j = 0; j < 2; ++j) vs[blk * PG_POS + lane + 32 * j] = __fmul_rn(x[j], up);
-                if (lane == 0) {
-                    const float down = __uint_as_float((uint32_t)(127 - 28 + e) << 23);
-                    vfac[blk] = top && e - max((int)(low >> 10), 1) > KV_V_RANGE ? -down : down;
-                }
+            for (int j = 0; j < 2; ++j) vs[blk * PG_POS + lane + 32 * j] = __fmul_rn(x[j], up);
+            if (lane == 0) {
+                const bool wide = top && e - max((int)(low >> 10), 1) > KV_V_RANGE;
+                vfac[blk] = odd || wide ? -down : down;
+                wide0[(i & 1) * 8 + blk] = wide;
             }
         }
         if (!__syncthreads_and(ok ? 1 : 0)) break;      // (a wait ran out: the CTA leaves as a whole)
+        if (tid == 0 && i > 0 && i - 1 + PGA_BUFS < ntiles) issue(i - 1 + PGA_BUFS);      // every warp is behind the page before
         // ---- scores: rows 16 rt .., positions KEYS kw ..
         float s[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[nt][e] = 0.0f;
-        const uint32_t *qa = q8 + (16 * rt + g) * PGA_Q_STRIDE + t;
-        const float *qs = qd + (16 * rt + g) * 8;
-        const uint32_t *kr = reinterpret_cast<const uint32_t *>(kt) + (size_t)(KEYS * kw + g) * (KV_ROW / 4);
+        {
+            const uint32_t *qa = q8 + (16 * rt + g) * PGA_Q_STRIDE + t;
+            const float *qs = qd + (16 * rt + g) * 8, *kd = ks + KEYS * kw + 2 * t;
+            const uint32_t *kr = reinterpret_cast<const uint32_t *>(kt) + (size_t)(KEYS * kw + g) * (KV_ROW / 4);
+            const float2 low = make_float2(-12582912.0f, -12582912.0f);
+#pragma unroll 1
+            for (int pair = 0; pair < 4; ++pair, qa += 16, qs += 2, kd += 2 * PG_POS, kr += 17) {
 #pragma unroll
-        for (int blk = 0; blk < 8; ++blk) {
-            const uint32_t a0 = qa[blk * 8], a1 = qa[blk * 8 + 8 * PGA_Q_STRIDE], a2 = qa[blk * 8 + 4], a3 = qa[blk * 8 + 4 + 8 * PGA_Q_STRIDE];
-            const float dq0 = qs[blk], dq1 = qs[64 + blk];
+                for (int odd = 0; odd < 2; ++odd) {
+                    const uint32_t a0 = qa[8 * odd], a1 = qa[8 * odd + 8 * PGA_Q_STRIDE], a2 = qa[8 * odd + 4], a3 = qa[8 * odd + 4 + 8 * PGA_Q_STRIDE];
+                    const float dq0 = qs[odd], dq1 = qs[64 + odd];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                const uint32_t *u = kr + nt * 8 * (KV_ROW / 4) + 17 * (blk >> 1);
-                uint32_t b0, b1;
-                if (blk & 1) {
-                    b0 = u[9 + t];
-                    b1 = u[13 + t];
-                } else {
-                    b0 = u[t];
-                    b1 = u[4 + t];
-                    if (t == 0) b0 = __byte_perm(b0, u[8], 0x5432);
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const uint32_t *u = kr + nt * 8 * (KV_ROW / 4);
+                        uint32_t b0, b1;
+                        if (odd) {
+                            b0 = u[9 + t];
+                            b1 = u[13 + t];
+                        } else {
+                            b0 = u[t];
+                            b1 = u[4 + t];
+                            if (t == 0) b0 = __byte_perm(b0, u[8], 0x5432);
+                        }
+                        int d[4];
+                        pga_mma_s8(d, a0, a1, a2, a3, b0, b1);
+                        const float2 dk = *reinterpret_cast<const float2 *>(kd + odd * PG_POS + 8 * nt);
+                        const float2 x0 = mul2(add2(make_float2(__int_as_float(d[0]), __int_as_float(d[1])), low), dk);
+                        const float2 x1 = mul2(add2(make_float2(__int_as_float(d[2]), __int_as_float(d[3])), low), dk);
+                        const float2 y0 = fma2(x0, make_float2(dq0, dq0), make_float2(s[nt][0], s[nt][1]));
+                        const float2 y1 = fma2(x1, make_float2(dq1, dq1), make_float2(s[nt][2], s[nt][3]));
+                        s[nt][0] = y0.x; s[nt][1] = y0.y; s[nt][2] = y1.x; s[nt][3] = y1.y;
+                    }
                 }
-                int d[4];
-                pga_mma_s8(d, a0, a1, a2, a3, b0, b1);
-                const float2 dk = *reinterpret_cast<const float2 *>(ks + blk * PG_POS + KEYS * kw + 8 * nt + 2 * t);
-                const float2 low = make_float2(-12582912.0f, -12582912.0f);
-                const float2 x0 = mul2(add2(make_float2(__int_as_float(d[0]), __int_as_float(d[1])), low), dk);
-                const float2 x1 = mul2(add2(make_float2(__int_as_float(d[2]), __int_as_float(d[3])), low), dk);
-                const float2 y0 = fma2(x0, make_float2(dq0, dq0), make_float2(s[nt][0], s[nt][1]));
-                const float2 y1 = fma2(x1, make_float2(dq1, dq1), make_float2(s[nt][2], s[nt][3]));
-                s[nt][0] = y0.x; s[nt][1] = y0.y; s[nt][2] = y1.x; s[nt][3] = y1.y;
             }
         }
-        // ---- softmax step of the warp's positions
-        const bool edge = p0 + PG_POS - 1 > all_see || n < PG_POS;               // some row does not see some position
-        if (edge) {
+        // ---- softmax step
+        if (p0 + PG_POS - 1 > all_see || n < PG_POS) {  // some row does not see some position
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -363,152 +387,156 @@ __global__ void __launch_bounds__(PGA_THREADS, 2) pages_attn_kernel(const __grid
                     if (p0 + k > limit[e >> 1] || k >= n) s[nt][e] = -INFINITY;
                 }
         }
-        float alpha[2];
+        float mx[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            float mx = s[0][2 * h];
+            mx[h] = s[0][2 * h];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mx = fmaxf(mx, fmaxf(s[nt][2 * h], s[nt][2 * h + 1]));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            const float m_new = fmaxf(m_run[h], mx), base = m_new == -INFINITY ? 0.0f : m_new;
-            alpha[h] = expf(__fsub_rn(m_run[h], base));
+            for (int nt = 0; nt < NT; ++nt) mx[h] = fmaxf(mx[h], fmaxf(s[nt][2 * h], s[nt][2 * h + 1]));
+            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+        }
+        if (KEYW > 1) {
+            if (t == 0) most[kw * ROWS + 16 * rt + g] = mx[0], most[kw * ROWS + 16 * rt + g + 8] = mx[1];
+            __syncthreads();
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int w = 0; w < KEYW; ++w) mx[h] = fmaxf(mx[h], most[w * ROWS + 16 * rt + g + 8 * h]);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int r = 16 * rt + g + 8 * h;
+            const float m_new = fmaxf(m_run[h], mx[h]), base = m_new == -INFINITY ? 0.0f : m_new;
+            const float alpha = expf(__fsub_rn(m_run[h], base));
             float sum = 0.0f;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                s[nt][2 * h] = expf(__fsub_rn(s[nt][2 * h], base));
-                s[nt][2 * h + 1] = expf(__fsub_rn(s[nt][2 * h + 1], base));
-                sum = __fadd_rn(sum, __fadd_rn(s[nt][2 * h], s[nt][2 * h + 1]));
+                const float x = expf(__fsub_rn(s[nt][2 * h], base)), y = expf(__fsub_rn(s[nt][2 * h + 1], base));
+                sum = __fadd_rn(sum, __fadd_rn(x, y));
+                *reinterpret_cast<float2 *>(wt + r * PGA_W_STRIDE + KEYS * kw + 8 * nt + 2 * t) = make_float2(x, y);
             }
-            l_run[h] = __fadd_rn(__fmul_rn(l_run[h], alpha[h]), sum);
+            l_run[h] = __fadd_rn(__fmul_rn(l_run[h], alpha), sum);
             m_run[h] = m_new;
+            if (kw == 0 && t == 0) alphas[r] = alpha;
         }
-        // ---- values, block by block into fresh sums
-        const uint32_t *vr = reinterpret_cast<const uint32_t *>(vt) + (size_t)(KEYS * kw + 2 * t) * (KV_ROW / 4);
+        __syncthreads();
+        // ---- outputs: blocks 2 warp, 2 warp + 1
+        const uint32_t *vr0 = reinterpret_cast<const uint32_t *>(vt) + (size_t)(2 * t) * (KV_ROW / 4) + 17 * warp;
 #pragma unroll
-        for (int blk = 0; blk < 8; ++blk) {
-            float o[4][4];
+        for (int bl = 0; bl < 2; ++bl) {
+            const float *dv0 = vs + (2 * warp + bl) * PG_POS + 2 * t;
+            const float fac = vfac[2 * warp + bl];
+            float o[ROWT][4][4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
-            const float fac = vfac[blk];
-            auto pass = [&](auto restc) {
-                constexpr bool REST = decltype(restc)::value;
-#pragma unroll
-                for (int kstep = 0; kstep < NT / 2; ++kstep) {
-                    uint32_t ah[4], al[4];
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const float2 dv = *reinterpret_cast<const float2 *>(vs + blk * PG_POS + KEYS * kw + 16 * kstep + 8 * half + 2 * t);
-                        const float *sp = s[2 * kstep + half];
-                        float2 x0 = mul2(make_float2(sp[0], sp[1]), dv), x1 = mul2(make_float2(sp[2], sp[3]), dv);
-                        if (edge) {                     // a position that a row does not see adds nothing, whatever it holds
-                            if (sp[0] == 0.0f) x0.x = 0.0f;
-                            if (sp[1] == 0.0f) x0.y = 0.0f;
-                            if (sp[2] == 0.0f) x1.x = 0.0f;
-                            if (sp[3] == 0.0f) x1.y = 0.0f;
-                        }
-                        split_f16x2(x0.x, x0.y, ah[2 * half], al[2 * half]);
-                        split_f16x2(x1.x, x1.y, ah[2 * half + 1], al[2 * half + 1]);
-                        if (REST) {
-                            uint32_t h2, l2;
-                            h2 = ah[2 * half], l2 = al[2 * half];
-                            split_rest_f16x2(x0.x, x0.y, h2, l2);
-                            ah[2 * half] = h2, al[2 * half] = l2;
-                            h2 = ah[2 * half + 1], l2 = al[2 * half + 1];
-                            split_rest_f16x2(x1.x, x1.y, h2, l2);
-                            ah[2 * half + 1] = h2, al[2 * half + 1] = l2;
-                        }
-                    }
-                    uint32_t w[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const uint32_t *u = vr + (16 * kstep + (e & 1) + 8 * (e >> 1)) * (KV_ROW / 4) + 17 * (blk >> 1);
-                        if (blk & 1) {
-                            w[e] = u[9 + g];
-                        } else {
-                            w[e] = u[g];
-                            if (g == 0) w[e] = __byte_perm(w[e], u[8], 0x5432);
-                        }
-                    }
-                    uint32_t b0[4], b1[4];
-                    pga_halves(w[0], w[1], b0);
-                    pga_halves(w[2], w[3], b1);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        mma_f16_16816(o[j], al[0], al[1], al[2], al[3], b0[j], b1[j]);
-                        mma_f16_16816(o[j], ah[0], ah[1], ah[2], ah[3], b0[j], b1[j]);
-                    }
-                }
-            };
-            if (fac < 0.0f) {                           // scales too far apart for one pair of planes: first what it leaves, times 2^24
-                pass(std::true_type{});
+            for (int m = 0; m < ROWT; ++m)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[j][e] = __fmul_rn(o[j][e], 0x1p-24f);
+                    for (int e = 0; e < 4; ++e) o[m][j][e] = 0.0f;
+            // CAREFUL: a position without weight adds nothing, whatever it holds; REST: what one pair of planes leaves, times 2^24
+            auto pass = [&](auto carefulc, auto restc) {
+                constexpr bool CAREFUL = decltype(carefulc)::value, REST = decltype(restc)::value;
+#pragma unroll 1
+                for (int k = 0; k < PG_POS / 16; ++k) {
+                    uint32_t w[4], b0[4], b1[4];
+                    const uint32_t *u = vr0 + (size_t)(16 * k) * (KV_ROW / 4);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t *x = u + ((e & 1) + 8 * (e >> 1)) * (KV_ROW / 4);
+                        if (bl) {
+                            w[e] = x[9 + g];
+                        } else {
+                            w[e] = x[g];
+                            if (g == 0) w[e] = __byte_perm(w[e], x[8], 0x5432);
+                        }
+                    }
+                    pga_halves(w[0], w[1], b0);
+                    pga_halves(w[2], w[3], b1);
+                    const float2 dv[2] = {*reinterpret_cast<const float2 *>(dv0 + 16 * k), *reinterpret_cast<const float2 *>(dv0 + 16 * k + 8)};
+#pragma unroll
+                    for (int m = 0; m < ROWT; ++m) {
+                        uint32_t ah[4], al[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {   // rows g, g + 8 of positions 2 t, then of 2 t + 8
+                            const float2 p = *reinterpret_cast<const float2 *>(wt + (16 * m + g + 8 * (e & 1)) * PGA_W_STRIDE + 16 * k + 8 * (e >> 1) + 2 * t);
+                            float2 x = mul2(p, dv[e >> 1]);
+                            if (CAREFUL) {
+                                if (p.x == 0.0f) x.x = 0.0f;
+                                if (p.y == 0.0f) x.y = 0.0f;
+                            }
+                            split_f16x2(x.x, x.y, ah[e], al[e]);
+                            if (REST) split_rest_f16x2(x.x, x.y, ah[e], al[e]);
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) mma_f16_16816(o[m][j], al[0], al[1], al[2], al[3], b0[j], b1[j]);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) mma_f16_16816(o[m][j], ah[0], ah[1], ah[2], ah[3], b0[j], b1[j]);
+                    }
+                }
+            };
+            if (fac > 0.0f) {
+                pass(std::false_type{}, std::false_type{});
+            } else {
+                if (wide0[(i & 1) * 8 + 2 * warp + bl]) {
+                    pass(std::true_type{}, std::true_type{});
+#pragma unroll
+                    for (int m = 0; m < ROWT; ++m)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[m][j][e] = __fmul_rn(o[m][j][e], 0x1p-24f);
+                }
+                pass(std::true_type{}, std::false_type{});
             }
-            pass(std::false_type{});
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int m = 0; m < ROWT; ++m) {
+                const float al[2] = {alphas[16 * m + g], alphas[16 * m + g + 8]};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[blk][j][e] = __fmaf_rn(o[j][e], fabsf(fac), __fmul_rn(acc[blk][j][e], alpha[e >> 1]));
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[m][bl][j][e] = __fmaf_rn(o[m][j][e], fabsf(fac), __fmul_rn(acc[m][bl][j][e], al[e >> 1]));
+            }
         }
-        __syncthreads();                                // the page has been read, and the scales
-        if (tid == 0 && i + PGA_BUFS < ntiles) issue(i + PGA_BUFS);
     }
-    // ---- the warps' sums meet, and leave by whole lines
-    float l[2], m[2];
+    // ---- the sums leave by whole lines
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        l[h] = __fadd_rn(l_run[h], __shfl_xor_sync(0xffffffffu, l_run[h], 1));
-        l[h] = __fadd_rn(l[h], __shfl_xor_sync(0xffffffffu, l[h], 2));
-        m[h] = m_run[h];
-        if (t == 0) ml[warp * 16 + g + 8 * h] = make_float2(m[h], l[h]);
+        float l = __fadd_rn(l_run[h], __shfl_xor_sync(0xffffffffu, l_run[h], 1));
+        l = __fadd_rn(l, __shfl_xor_sync(0xffffffffu, l, 2));
+        if (t == 0) part[kw * ROWS + 16 * rt + g + 8 * h] = l, most[kw * ROWS + 16 * rt + g + 8 * h] = m_run[h];
     }
-    if (!__syncthreads_and(ok ? 1 : 0)) return;
+    if (!__syncthreads_and(ok ? 1 : 0)) return;         // (and every warp has left the last page)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int m = 0; m < ROWT; ++m)
 #pragma unroll
-        for (int w = 0; w < KEYW; ++w) m[h] = fmaxf(m[h], ml[(KEYW * rt + w) * 16 + g + 8 * h].x);
-        const float f = m_run[h] == m[h] ? 1.0f : expf(__fsub_rn(m_run[h], m[h]));       // (also where neither has seen a position)
-        float *dst = reinterpret_cast<float *>(ring) + (size_t)(warp * 16 + g + 8 * h) * KV_D;
+        for (int bl = 0; bl < 2; ++bl)
 #pragma unroll
-        for (int blk = 0; blk < 8; ++blk)
+            for (int h = 0; h < 2; ++h) {
+                float *dst = reinterpret_cast<float *>(ring) + (size_t)(16 * m + g + 8 * h) * KV_D + 32 * (2 * warp + bl);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {               // slot 2 t + c of the block: four values from dim 4 slot (odd block) or 4 slot - 2 (even, round the end)
-                const int slot = 2 * t + c;
-                const float x0 = __fmul_rn(acc[blk][0][2 * h + c], f), x1 = __fmul_rn(acc[blk][1][2 * h + c], f);
-                const float x2 = __fmul_rn(acc[blk][2][2 * h + c], f), x3 = __fmul_rn(acc[blk][3][2 * h + c], f);
-                float *d0 = dst + 32 * blk + ((blk & 1) ? 4 * slot : (slot ? 4 * slot - 2 : 0));
-                float *d1 = dst + 32 * blk + ((blk & 1) ? 4 * slot + 2 : (slot ? 4 * slot : 30));
-                *reinterpret_cast<float2 *>(d0) = make_float2(x0, x1);
-                *reinterpret_cast<float2 *>(d1) = make_float2(x2, x3);
+                for (int c = 0; c < 2; ++c) {           // slot 2 t + c of the block: four values from dim 4 slot (odd block) or 4 slot - 2 (even, round the end)
+                    const int slot = 2 * t + c;
+                    float *d0 = dst + (bl ? 4 * slot : (slot ? 4 * slot - 2 : 0)), *d1 = dst + (bl ? 4 * slot + 2 : (slot ? 4 * slot : 30));
+                    *reinterpret_cast<float2 *>(d0) = make_float2(acc[m][bl][0][2 * h + c], acc[m][bl][1][2 * h + c]);
+                    *reinterpret_cast<float2 *>(d1) = make_float2(acc[m][bl][2][2 * h + c], acc[m][bl][3][2 * h + c]);
+                }
             }
+    if (tid < ROWS) {
+        float l = part[tid];
+#pragma unroll
+        for (int w = 1; w < KEYW; ++w) l = __fadd_rn(l, part[w * ROWS + tid]);
+        sums[tid] = l;
     }
     __syncthreads();
-    const float4 *box = reinterpret_cast<const float4 *>(ring);
     for (int i = tid; i < n_rows * (KV_D / 4); i += PGA_THREADS) {
-        const int r = i / (KV_D / 4), c = i % (KV_D / 4), part0 = (r >> 4) * KEYW * 16 + (r & 15);       // the first warp's copy of the row
-        float4 x = box[(size_t)part0 * (KV_D / 4) + c];
-        float mm = ml[part0].x;
-#pragma unroll
-        for (int w = 1; w < KEYW; ++w) {
-            const float4 y = box[(size_t)(part0 + 16 * w) * (KV_D / 4) + c];
-            x = make_float4(__fadd_rn(x.x, y.x), __fadd_rn(x.y, y.y), __fadd_rn(x.z, y.z), __fadd_rn(x.w, y.w));
-            mm = fmaxf(mm, ml[part0 + 16 * w].x);
-        }
-        float ll = 0.0f;
-#pragma unroll
-        for (int w = 0; w < KEYW; ++w) {
-            const float2 x = ml[part0 + 16 * w];
-            ll = __fadd_rn(ll, __fmul_rn(x.y, x.x == mm ? 1.0f : expf(__fsub_rn(x.x, mm))));
-        }
+        const int r = i / (KV_D / 4), c = i % (KV_D / 4);
+        float4 x = reinterpret_cast<const float4 *>(ring)[(size_t)r * (KV_D / 4) + c];
+        const float l = sums[r];
         const int row = tile * ROWS + r, tok = row / P.group;
         const size_t at = (size_t)(range.begin + tok) * P.n_head + kvh * P.group + (row - tok * P.group);
         if (P.splits == 1) {
-            const float inv = ll == 0.0f ? 0.0f : __fdiv_rn(1.0f, ll);           // a row that sees nothing is zeros
+            const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);             // a row that sees nothing is zeros
             x = make_float4(__fmul_rn(x.x, inv), __fmul_rn(x.y, inv), __fmul_rn(x.z, inv), __fmul_rn(x.w, inv));
             float *o = P.out + at * KV_D + 4 * c;
             if ((reinterpret_cast<uintptr_t>(P.out) & 15u) == 0) {
@@ -517,46 +545,67 @@ __global__ void __launch_bounds__(PGA_THREADS, 2) pages_attn_kernel(const __grid
                 o[0] = x.x; o[1] = x.y; o[2] = x.z; o[3] = x.w;
             }
         } else {
-            const size_t part = (size_t)split * C.n_tok * P.n_head + at;
-            reinterpret_cast<float4 *>(P.part_acc)[part * (KV_D / 4) + c] = x;
-            if (c == 0) P.part_ml[part] = make_float2(mm, ll);
+            const size_t at2 = (size_t)split * C.n_tok * P.n_head + at;
+            reinterpret_cast<float4 *>(P.part_acc)[at2 * (KV_D / 4) + c] = x;
+            if (c == 0) P.part_ml[at2] = make_float2(most[r], l);
         }
     }
 }
 
-// The splits of a row added up: a warp per row (token, head), eight dims a lane.  A row's splits are those that its sequence's positions reach.
-constexpr int PGJ_WARPS = 4;
+// The splits of a row added up: ROWW warps per row (token, head), four dims and four more a lane.  A row's splits are those that its own positions reach.
+constexpr int PGJ_WARPS = 8;
+template <int ROWW>
 __global__ void __launch_bounds__(32 * PGJ_WARPS) pages_join_kernel(const __grid_constant__ PageAttn P) {
+    __shared__ float4 sums[PGJ_WARPS][2][32];
+    __shared__ float2 ml[PGJ_WARPS];
     const PageCache &C = P.C;
-    const int lane = threadIdx.x & 31;
-    const int64_t row = (int64_t)blockIdx.x * PGJ_WARPS + (threadIdx.x >> 5), rows = (int64_t)C.n_tok * P.n_head;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, mine = warp % ROWW;
+    const int64_t rows = (int64_t)C.n_tok * P.n_head, row = (int64_t)blockIdx.x * (PGJ_WARPS / ROWW) + warp / ROWW;
     pdl_wait_prior_grid();
     pdl_launch_dependents();
-    if (row >= rows) return;
-    const int tok = (int)(row / P.n_head);
-    const int s = seq_of_row(C.start, C.n_seq, tok, lane);
-    if (s >= C.n_seq) return;
-    const SeqRange r = seq_range(C.start, s, C.n_tok);
-    const int len = C.len[s];
-    if (r.n <= 0 || tok < r.begin || len < 0 || len > (int64_t)C.table_stride * PG_POS) return;        // not a sequence: the attention has said so
-    // rows of a tile were written by every split that the tile's last row reaches; this row's own positions are enough
-    const int seen = min(len, len - r.n + (tok - r.begin) + 1);
-    const int n = max(1, min(P.splits, ((max(seen, 0) + PG_POS - 1) / PG_POS + P.pages_per_split - 1) / P.pages_per_split));
-    float m = -INFINITY;
+    int n = 0;                                          // 0: not a row of a sequence that was served
+    if (row < rows) {
+        const int tok = (int)(row / P.n_head);
+        const int s = seq_of_row(C.start, C.n_seq, tok, lane);
+        if (s < C.n_seq) {
+            const SeqRange r = seq_range(C.start, s, C.n_tok);
+            const int len = C.len[s];
+            if (r.n > 0 && tok >= r.begin && len >= 0 && len <= (int64_t)C.table_stride * PG_POS) {
+                const int seen = len - r.n + (tok - r.begin) + 1;
+                n = max(1, min(P.splits, ((max(seen, 0) + PG_POS - 1) / PG_POS + P.pages_per_split - 1) / P.pages_per_split));
+            }
+        }
+    }
+    float m = -INFINITY, l = 0.0f;
     for (int i = lane; i < n; i += 32) m = fmaxf(m, P.part_ml[i * rows + row].x);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-    float l = 0.0f;
-    for (int i = 0; i < n; ++i) {
+#pragma unroll 4
+    for (int i = mine; i < n; i += ROWW) {
         const float2 x = P.part_ml[i * rows + row];
-        const float w = x.x == m ? 1.0f : expf(__fsub_rn(x.x, m));
         const float4 *src = reinterpret_cast<const float4 *>(P.part_acc) + (i * rows + row) * (KV_D / 4) + lane;
         const float4 c = src[0], d = src[32];
+        const float w = x.x == m ? 1.0f : expf(__fsub_rn(x.x, m));
         l = __fmaf_rn(x.y, w, l);
         a = make_float4(__fmaf_rn(c.x, w, a.x), __fmaf_rn(c.y, w, a.y), __fmaf_rn(c.z, w, a.z), __fmaf_rn(c.w, w, a.w));
         b = make_float4(__fmaf_rn(d.x, w, b.x), __fmaf_rn(d.y, w, b.y), __fmaf_rn(d.z, w, b.z), __fmaf_rn(d.w, w, b.w));
     }
+    if (ROWW > 1) {
+        sums[warp][0][lane] = a;
+        sums[warp][1][lane] = b;
+        if (lane == 0) ml[warp] = make_float2(0.0f, l);
+        __syncthreads();
+        if (mine) return;
+#pragma unroll
+        for (int w = 1; w < ROWW; ++w) {
+            const float4 c = sums[warp + w][0][lane], d = sums[warp + w][1][lane];
+            l = __fadd_rn(l, ml[warp + w].y);
+            a = make_float4(__fadd_rn(a.x, c.x), __fadd_rn(a.y, c.y), __fadd_rn(a.z, c.z), __fadd_rn(a.w, c.w));
+            b = make_float4(__fadd_rn(b.x, d.x), __fadd_rn(b.y, d.y), __fadd_rn(b.z, d.z), __fadd_rn(b.w, d.w));
+        }
+    }
+    if (n == 0) return;
     const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
     float *o = P.out + row * KV_D + 4 * lane;
     const float x[8] = {__fmul_rn(a.x, inv), __fmul_rn(a.y, inv), __fmul_rn(a.z, inv), __fmul_rn(a.w, inv),
