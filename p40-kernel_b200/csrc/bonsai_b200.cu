@@ -2067,7 +2067,7 @@ static int64_t gdn_chunk_count(int n_tok, int n_seq, int K, int V) {
 }
 int64_t bonsai_b200_gdn_seqs_workspace(int n_tok, int n_seq, int n_k_heads, int n_v_heads, int K, int V) {
     if (!gdn_shapes(n_k_heads, n_v_heads, K, V) || n_tok <= 0 || n_seq <= 0) return 0;
-    return gdn_chunk_count(n_tok, n_seq, K, V) * n_v_heads * GDC_REC * (int64_t)sizeof(float);
+    return gdn_chunk_count(n_tok, n_seq, K, V) * ((int64_t)n_k_heads * GDC_KQ_REC + (int64_t)n_v_heads * GDC_TP_REC);
 }
 int bonsai_b200_gdn_seqs(float *state, const float *q, const float *k, const float *v, const float *g, const float *beta, float *out, const int32_t *start,
                          const int32_t *slot, void *workspace, int64_t workspace_bytes, int n_seq, int n_slots, int n_tok, int n_k_heads, int n_v_heads, int K, int V,
@@ -2078,17 +2078,19 @@ int bonsai_b200_gdn_seqs(float *state, const float *q, const float *k, const flo
         if (!p || !aligned4(p)) return 1;
     if (!aligned4(slot)) return 1;
     const int64_t chunks = gdn_chunk_count(n_tok, n_seq, K, V);
-    if (chunks > INT32_MAX || n_k_heads > 65535 || (int64_t)n_v_heads * GDC_SLICES > INT32_MAX) return 1;
-    if (chunks && (!workspace || !aligned16(workspace) || workspace_bytes < chunks * n_v_heads * GDC_REC * (int64_t)sizeof(float))) return 1;
+    if (chunks > INT32_MAX || n_v_heads > 65535 || (int64_t)n_v_heads * GDC_SLICES > INT32_MAX) return 1;
+    if (chunks && (!workspace || !aligned16(workspace) || workspace_bytes < chunks * ((int64_t)n_k_heads * GDC_KQ_REC + (int64_t)n_v_heads * GDC_TP_REC))) return 1;
     const GdnSeqs P = {state, q, k, v, g, beta, out, start, slot, n_seq, n_slots, n_tok, n_k_heads, n_v_heads, K, V};
     const cudaStream_t st = as_stream(stream);
     cudaError_t e = launch(gdn_seqs_step_kernel, dim3((unsigned)(n_v_heads * (V / 32)), (unsigned)n_seq), dim3(GDN_WARPS * 32), 0, st, true, P, chunks ? GDC_STEP_MOST : INT32_MAX);
     if (!chunks || e != cudaSuccess) return (int)e;
     static SmemOptIn opt[2];
-    float *recs = static_cast<float *>(workspace);
+    uint8_t *kq = static_cast<uint8_t *>(workspace), *tp = kq + chunks * n_k_heads * GDC_KQ_REC;
     if ((e = opt[0].ensure(gdn_chunk_kernel)) == cudaSuccess && (e = opt[1].ensure(gdn_scan_kernel)) == cudaSuccess)
-        e = launch(gdn_chunk_kernel, dim3((unsigned)chunks, (unsigned)n_k_heads), dim3(GDC_THREADS), (size_t)gdc_chunk_smem(), st, true, P, recs);
-    if (e == cudaSuccess) e = launch(gdn_scan_kernel, dim3((unsigned)(n_v_heads * GDC_SLICES), (unsigned)n_seq), dim3(GDC_THREADS), (size_t)gdc_scan_smem(), st, true, P, (const float *)recs);
+        e = launch(gdn_planes_kernel, dim3((unsigned)chunks, (unsigned)n_k_heads), dim3(GDC_THREADS), 0, st, true, P, kq);
+    if (e == cudaSuccess) e = launch(gdn_chunk_kernel, dim3((unsigned)chunks, (unsigned)n_v_heads), dim3(GDC_PREP_THREADS), (size_t)gdc_prep_smem(), st, true, P, (const uint8_t *)kq, tp);
+    if (e == cudaSuccess)
+        e = launch(gdn_scan_kernel, dim3((unsigned)(n_v_heads * GDC_SLICES), (unsigned)n_seq), dim3(GDC_THREADS), (size_t)gdc_scan_smem(), st, true, P, (const uint8_t *)kq, (const uint8_t *)tp);
     return (int)e;
 }
 

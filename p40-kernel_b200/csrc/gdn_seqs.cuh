@@ -1,7 +1,9 @@
 // gdn_seqs.cuh -- the gated delta rule over the tokens of several sequences.
 #pragma once
 
+#include "attn_tc.cuh"
 #include "common.cuh"
+#include "kv.cuh"
 #include "ops.cuh"
 #include "seqs.cuh"
 
@@ -108,108 +110,95 @@ __global__ void __launch_bounds__(GDN_WARPS * 32) gdn_seqs_step_kernel(const __g
 //   u_i = beta_i (v_i - e^G_i k_i S - sum over j < i of e^(G_i - G_j) (k_i . k_j) u_j)                U = Tb (V - e^G K S), Tb = (1 + A)^-1 diag(beta)
 //   o_i = e^G_i q_i S + sum over j <= i of e^(G_i - G_j) (q_i . k_j) u_j                              O = e^G Q S + P U
 //   S' = e^G_63 S + sum of k_j e^(G_63 - G_j) u_j                                                     S' = e^G_63 S + K^T (e^(G_63 - G) U)
-// with A_ij = beta_i e^(G_i - G_j) (k_i . k_j), j < i.  gdn_chunk_kernel forms Tb and P of every chunk at once; gdn_scan_kernel carries the state through
+// with A_ij = beta_i e^(G_i - G_j) (k_i . k_j), j < i.  gdn_planes_kernel and gdn_chunk_kernel form the planes of K and Q, and Tb and P, of every chunk at once; gdn_scan_kernel carries the state through
 // the chunks of a sequence, a CTA per value head and 48 or 40 columns of it (the columns do not know of each other).
 //
-// Products are fp32 to 2^-22: each operand is split into two TF32 parts (11 bits each, any exponent), three of the four products on mma.sync (m16n8k8), sums fp32.
-constexpr int GDC_T = 64, GDC_D = 128, GDC_THREADS = 256;
-constexpr int GDC_KS = GDC_D + 4, GDC_TS = GDC_T + 4;                 // row strides: 4 g + t are 32 different banks
-constexpr int GDC_COLS = 48, GDC_CS = GDC_COLS + 8, GDC_NT = GDC_COLS / 8, GDC_SLICES = 3;       // 24 t + g are 32 different banks
+// Products are fp32 to about 2^-22: each operand is two fp16 planes, high and low, of its values times a power of two -- K, Q, Tb and P a row, S, V - e^G K S and U eight columns
+// -- of which a plane pair holds 2^-38 of the largest; three of the four products on mma.sync (m16n8k16), sums fp32.  (Two TF32 parts, which need no powers of
+// two, are four times the instructions for the same: the tensor core's 554 TFLOP/s of fp16 are 278 of TF32, and the parts were made anew by every warp.)
+// The tensor core cuts the last bits of a sum off instead of rounding it, so a sum is of one step of 16 values, small products first, and rounded additions join the
+// steps.  (One sum over all steps, the state's own among them: error of 2048 tokens' outputs against 64 bits 1.6e-6, now 2.3e-7.)
+constexpr int GDC_T = 64, GDC_D = 128;
+constexpr int GDC_PREP_THREADS = 128, GDC_THREADS = 256;
+constexpr int GDC_COLS = 48, GDC_NT = GDC_COLS / 8, GDC_SLICES = 3;
+// row strides in bytes of planes in shared memory: 16-byte pieces of eight rows lie in different banks
+constexpr int GDC_KB = GDC_D * 2 + 16, GDC_TB = GDC_T * 2 + 16, GDC_CB = GDC_COLS * 2 + 16;
+constexpr int GDC_KP = GDC_T * GDC_KB, GDC_TP = GDC_T * GDC_TB, GDC_SP = GDC_D * GDC_CB, GDC_UP = GDC_T * GDC_CB;        // a plane of K or Q, Tb or P, S, U
+constexpr int GDC_TS = GDC_T + 4;                                     // floats: a row of A and of its inverse
 constexpr int GDC_STEP_MOST = 16;                                     // tokens of a sequence that go one by one
-// What the first kernel leaves of a chunk and value head: Tb, P [64][64], e^G, e^(G_63 - G) [64], and whether the chunk is to go token by token
-constexpr int GDC_REC = 2 * GDC_T * GDC_T + 2 * GDC_T + 4;            // floats, 16-byte aligned
-constexpr int gdc_chunk_smem() { return (2 * GDC_T * GDC_KS + 4 * GDC_T * GDC_TS) * 4 + GDC_T * 8 + GDC_T * 4; }
-constexpr int gdc_scan_smem() { return (3 * GDC_T * GDC_KS + 3 * GDC_T * GDC_TS + GDC_T * GDC_COLS + (GDC_D + 2 * GDC_T) * GDC_CS + 4 * GDC_T + 8) * 4; }
+// What the first two kernels leave, in bytes, planes with the row strides of shared memory so that one bulk copy fetches them: of a chunk and key head the planes of K and Q and
+// the exponents s of their rows' powers of two; of a chunk and value head the planes of Tb and P, then floats: per row e^G 2^-s of K, e^G 2^-s of Q, e^(G_63 - G) 2^(s_min - s) of K,
+// 2^-s of Tb, 2^-s of P; then e^G_63, 2^-s_min, whether the chunk is to go token by token.
+constexpr int GDC_KQ_REC = 4 * GDC_KP + 2 * GDC_T * 4, GDC_TP_PLANES = 4 * GDC_TP, GDC_VEC = 5 * GDC_T + 4, GDC_TP_REC = GDC_TP_PLANES + GDC_VEC * 4;
+constexpr int gdc_prep_smem() { return 4 * GDC_KP + GDC_T * 8 + 3 * GDC_T * 4 + 32; }
+constexpr int gdc_scan_smem() { return 6 * GDC_KP + 4 * GDC_TP + GDC_T * GDC_COLS * 4 + 2 * GDC_SP + 4 * GDC_UP + GDC_VEC * 4 + 5 * 8 * 4 + 4 * 8; }
+static_assert(2 * GDC_UP <= 2 * GDC_KP && GDC_D * GDC_CB * 2 >= GDC_D * GDC_COLS * 4 && 2 * GDC_T * GDC_TS * 4 <= 2 * GDC_KP, "");
 
 __device__ __forceinline__ int gdc_chunks(int n) { return n > GDC_STEP_MOST ? (n + GDC_T - 1) / GDC_T : 0; }
 
-__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
-    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-// x = hi + lo: hi rounded to 11 bits, lo to the 11 behind them
-__device__ __forceinline__ uint32_t tf32_of(float x) { return (__float_as_uint(x) + 0x1000u) & 0xFFFFE000u; }
-__device__ __forceinline__ void tf32_split(float x, uint32_t &hi, uint32_t &lo) {
-    hi = tf32_of(x);
-    lo = tf32_of(__fsub_rn(x, __uint_as_float(hi)));
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-// c += A B over 8 `steps` values, an even number of steps: A 16 rows, element (i, k) at a[i * as + k * ak], B 8 NT columns, (k, j) at b[k * bs + j * bj]; a and b point at the lane's own
-// corner, (g, t) and (t, g).  A's value k is multiplied by the lane's factor(k) first.
-// The tensor core cuts the last bits of a sum off instead of rounding it: a sum is of two steps of 8, small products first, and rounded additions join them.  (One sum over all
-// steps, the state's own among them: error of 2048 tokens' outputs against 64 bits 1.6e-6.)
-template <int NT, typename F>
-__device__ __forceinline__ void gdc_product(float (&c)[NT][4], const float *a, int as, int ak, const float *b, int bs, int bj, int steps, F factor) {
-#pragma unroll 1
-    for (int s = 0; s < steps; s += 2, a += 16 * ak, b += 16 * bs) {
-        float sum[NT][4];
-        uint32_t ah[2][4], al[2][4], bh[2][NT][2], bl[2][NT][2];
+__device__ __forceinline__ void ldsm2_t(uint32_t (&r)[4], uint32_t addr) {       // (into the first two)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(addr) : "memory");
+}
+// The first product of a sum.
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+// c[m] = A[m] B over 16 STEPS values, each A 16 rows, B 8 NT columns.  a[m], b: the lane's addresses of the high planes, the low ones a_low and b_low behind, a step a_step and
+// b_step behind the one before; of a pair of column tiles b_pair.  AT: A lies by columns; BT: B lies by rows.
+template <int MT, int NT, int STEPS, bool AT, bool BT>
+__device__ __forceinline__ void gdc_product(float (&c)[MT][NT][4], const uint32_t (&a)[MT], uint32_t a_low, uint32_t a_step, uint32_t b, uint32_t b_low, uint32_t b_step, uint32_t b_pair) {
+    constexpr int PAIRS = (NT + 1) / 2;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const float f0 = factor(8 * (s + h)), f1 = factor(8 * (s + h) + 4);
-            const float *x = a + 8 * h * ak, *y = b + 8 * h * bs;
-            tf32_split(__fmul_rn(x[0], f0), ah[h][0], al[h][0]);
-            tf32_split(__fmul_rn(x[8 * as], f0), ah[h][1], al[h][1]);
-            tf32_split(__fmul_rn(x[4 * ak], f1), ah[h][2], al[h][2]);
-            tf32_split(__fmul_rn(x[8 * as + 4 * ak], f1), ah[h][3], al[h][3]);
+    for (int k = 0; k < STEPS; ++k) {
+        uint32_t ah[MT][4], al[MT][4], bh[PAIRS][4], bl[PAIRS][4];
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                tf32_split(y[8 * j * bj], bh[h][j][0], bl[h][j][0]);
-                tf32_split(y[8 * j * bj + 4 * bs], bh[h][j][1], bl[h][j][1]);
-            }
+        for (int m = 0; m < MT; ++m) {
+            if (AT) ldsm4_t(ah[m], a[m] + k * a_step), ldsm4_t(al[m], a[m] + k * a_step + a_low);
+            else ldsm4(ah[m], a[m] + k * a_step), ldsm4(al[m], a[m] + k * a_step + a_low);
         }
 #pragma unroll
-        for (int j = 0; j < NT; ++j) sum[j][0] = sum[j][1] = sum[j][2] = sum[j][3] = 0.0f;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-            for (int j = 0; j < NT; ++j) mma_tf32(sum[j], al[h], bh[h][j]);
-#pragma unroll
-            for (int j = 0; j < NT; ++j) mma_tf32(sum[j], ah[h], bl[h][j]);
+        for (int j = 0; j < PAIRS; ++j) {
+            const uint32_t at = b + k * b_step + j * b_pair;
+            if (2 * j + 1 == NT) ldsm2_t(bh[j], at), ldsm2_t(bl[j], at + b_low);
+            else if (BT) ldsm4_t(bh[j], at), ldsm4_t(bl[j], at + b_low);
+            else ldsm4(bh[j], at), ldsm4(bl[j], at + b_low);
         }
+        float sum[MT][NT][4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int j = 0; j < NT; ++j) mma_tf32(sum[j], ah[h], bh[h][j]);
+            for (int j = 0; j < NT; ++j) mma_f16_first(sum[m][j], al[m], bh[j >> 1][2 * (j & 1)], bh[j >> 1][2 * (j & 1) + 1]);
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) c[j][e] = __fadd_rn(c[j][e], sum[j][e]);
+            for (int j = 0; j < NT; ++j) mma_f16_16816(sum[m][j], ah[m][0], ah[m][1], ah[m][2], ah[m][3], bl[j >> 1][2 * (j & 1)], bl[j >> 1][2 * (j & 1) + 1]);
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) mma_f16_16816(sum[m][j], ah[m][0], ah[m][1], ah[m][2], ah[m][3], bh[j >> 1][2 * (j & 1)], bh[j >> 1][2 * (j & 1) + 1]);
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) c[m][j][e] = k == 0 ? sum[m][j][e] : __fadd_rn(c[m][j][e], sum[m][j][e]);
     }
 }
-template <int NT>
-__device__ __forceinline__ void gdc_product(float (&c)[NT][4], const float *a, int as, int ak, const float *b, int bs, int bj, int steps) {
-    gdc_product<NT>(c, a, as, ak, b, bs, bj, steps, [](int) { return 1.0f; });
-}
-__device__ __forceinline__ void cp_async4(void *dst, const void *src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory"); }
-// `rows` rows of COLS floats (row stride `from` in memory, `to` in shared memory) by the whole CTA, asynchronously; rows up to 64 are filled up with zeros.
-template <int COLS>
-__device__ __forceinline__ void gdc_load(float *dst, int to, const float *src, size_t from, int rows, bool vec, int cols = COLS) {
-    if (vec) {
-        for (int i = threadIdx.x; i < GDC_T * (COLS / 4); i += GDC_THREADS) {
-            const int r = i / (COLS / 4), c = 4 * (i % (COLS / 4));
-            if (c >= cols) continue;
-            if (r < rows) cp_async16(dst + r * to + c, src + r * from + c);
-            else *reinterpret_cast<float4 *>(dst + r * to + c) = make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-    } else {
-        for (int i = threadIdx.x; i < GDC_T * COLS; i += GDC_THREADS) {
-            const int r = i / COLS, c = i % COLS;
-            if (c >= cols) continue;
-            if (r < rows) cp_async4(dst + r * to + c, src + r * from + c);
-            else dst[r * to + c] = 0.0f;
-        }
-    }
-}
+// Lane's place in a matrix of rows of `stride` bytes: (rows, values) of A by rows; of B by rows (k) and of A by columns; of B by columns (n).
+__device__ __forceinline__ uint32_t gdc_at_rows(int lane, int stride) { return (lane & 15) * stride + (lane >> 4) * 16; }
+__device__ __forceinline__ uint32_t gdc_at_turned(int lane, int stride) { return ((lane & 7) + 8 * (lane >> 4)) * stride + ((lane >> 3) & 1) * 16; }
 
-// grid (chunks of all sequences and some that find none, key heads): K K^T and Q K^T once, then Tb and P for each value head of the key head.
-__global__ void __launch_bounds__(GDC_THREADS, 1) gdn_chunk_kernel(const __grid_constant__ GdnSeqs P, float *recs) {
-    extern __shared__ __align__(16) float gdc_smem[];
-    float *kt = gdc_smem, *qt = kt + GDC_T * GDC_KS, *kk = qt + GDC_T * GDC_KS, *qk = kk + GDC_T * GDC_TS, *at = qk + GDC_T * GDC_TS, *tt = at + GDC_T * GDC_TS;
-    double *gs = reinterpret_cast<double *>(tt + GDC_T * GDC_TS);
-    float *bs = reinterpret_cast<float *>(gs + GDC_T);
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int kh = blockIdx.y;
+// grid (chunks of all sequences and some that find none, key heads): planes of K and Q, a warp per row, lane = four values.
+__global__ void __launch_bounds__(GDC_THREADS) gdn_planes_kernel(const __grid_constant__ GdnSeqs P, uint8_t *kq_recs) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, kh = blockIdx.y;
     pdl_wait_prior_grid();
     pdl_launch_dependents();
     int seq, chunk;
@@ -217,137 +206,220 @@ __global__ void __launch_bounds__(GDC_THREADS, 1) gdn_chunk_kernel(const __grid_
     const SeqRange range = seq_range(P.start, seq, P.n_tok);
     const int n = min(GDC_T, range.n - chunk * GDC_T);
     const size_t tok = (size_t)range.begin + chunk * GDC_T;
-    const size_t stride = (size_t)P.n_k_heads * GDC_D;
+    uint8_t *rec = kq_recs + ((size_t)blockIdx.x * P.n_k_heads + kh) * GDC_KQ_REC;
     const bool vec = ((reinterpret_cast<uintptr_t>(P.k) | reinterpret_cast<uintptr_t>(P.q)) & 15u) == 0;
-    gdc_load<GDC_D>(kt, GDC_KS, P.k + (tok * P.n_k_heads + kh) * GDC_D, stride, n, vec);
-    gdc_load<GDC_D>(qt, GDC_KS, P.q + (tok * P.n_k_heads + kh) * GDC_D, stride, n, vec);
-    cp_async_commit();
-    cp_async_wait<0>();
-    __syncthreads();
-    {   // of rows 16 m .. the columns up to 16 m + 15; a sub-core's two warps take rows that add up to the same number of columns
-        const bool of_q = warp >= 4;
-        const int m = of_q ? 7 - warp : warp;
-        const float *a = (of_q ? qt : kt) + (16 * m + g) * GDC_KS + t;
-        float *dst = (of_q ? qk : kk) + (16 * m + g) * GDC_TS + 2 * t;
-        for (int j = 0; j <= m; ++j) {
-            float c[2][4] = {};
-            gdc_product<2>(c, a, GDC_KS, 1, kt + (16 * j + g) * GDC_KS + t, 1, GDC_KS, GDC_D / 8);
+    constexpr int ROWS = 2 * GDC_T / (GDC_THREADS / 32);
+    float4 x[ROWS];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                *reinterpret_cast<float2 *>(dst + 16 * j + 8 * h) = make_float2(c[h][0], c[h][1]);
-                *reinterpret_cast<float2 *>(dst + 16 * j + 8 * h + 8 * GDC_TS) = make_float2(c[h][2], c[h][3]);
-            }
-        }
+    for (int i = 0; i < ROWS; ++i) {
+        const int r = ROWS * warp + i, row = r & (GDC_T - 1);
+        const float *src = (r < GDC_T ? P.k : P.q) + ((tok + row) * P.n_k_heads + kh) * GDC_D + 4 * lane;
+        x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (row < n) x[i] = vec ? *reinterpret_cast<const float4 *>(src) : make_float4(src[0], src[1], src[2], src[3]);
     }
-    const int share = P.n_v_heads / P.n_k_heads;
-    for (int sub = 0; sub < share; ++sub) {
-        const int vh = kh * share + sub;
-        float *rec = recs + ((size_t)blockIdx.x * P.n_v_heads + vh) * GDC_REC;
-        bool odd = false;                       // something that sums may not hold: the chunk goes token by token
-        if (warp == 0) {
-            // a decay below e^-1000 is none; sums in 64 bits: of two that are far from zero the difference matters
-            double x[2];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int i = 2 * lane + h;
-                const float gi = i < n ? P.g[(tok + i) * P.n_v_heads + vh] : 0.0f, bi = i < n ? P.beta[(tok + i) * P.n_v_heads + vh] : 0.0f;
-                odd = odd || !(gi < 1e30f) || !(fabsf(bi) < 1e30f);
-                x[h] = (double)fmaxf(gi, -1000.0f);
-                bs[i] = bi;
-            }
-            x[1] += x[0];
-            double sum = x[1];
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const double y = __shfl_up_sync(0xffffffffu, sum, o);
-                if (lane >= o) sum += y;
-            }
-            const double before = sum - x[1], last = __shfl_sync(0xffffffffu, sum, 31);
-            gs[2 * lane] = before + x[0];
-            gs[2 * lane + 1] = sum;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const double gi = h ? sum : before + x[0];
-                rec[2 * GDC_T * GDC_T + 2 * lane + h] = expf((float)gi);
-                rec[2 * GDC_T * GDC_T + GDC_T + 2 * lane + h] = expf((float)(last - gi));
-            }
-        }
-        __syncthreads();
-        for (int e = tid; e < GDC_T * GDC_T; e += GDC_THREADS) {
-            const int i = e / GDC_T, j = e % GDC_T;
-            float a = 0.0f, p = 0.0f;
-            if (j <= i) {
-                const float decay = expf((float)(gs[i] - gs[j]));
-                p = i < n ? __fmul_rn(decay, qk[i * GDC_TS + j]) : 0.0f;
-                a = j < i ? __fmul_rn(__fmul_rn(bs[i], decay), kk[i * GDC_TS + j]) : 0.0f;
-                odd = odd || !(fabsf(p) < 1e30f) || !(fabsf(a) < 1e30f);
-            }
-            at[i * GDC_TS + j] = a;
-            rec[GDC_T * GDC_T + e] = p;
-        }
-        __syncthreads();
-        // inverses of the four 16 x 16 blocks on the diagonal: a half-warp each, lane = column, from the top row down
-        if (warp < 2) {
-            const int blk = 16 * (2 * warp + (lane >> 4)), c = lane & 15;
-            float x[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                float s = i == c ? 1.0f : 0.0f;
-#pragma unroll
-                for (int j = 0; j < i; ++j) s = __fmaf_rn(-at[(blk + i) * GDC_TS + blk + j], x[j], s);
-                x[i] = s;
-            }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) tt[(blk + i) * GDC_TS + blk + c] = x[i];
-        }
-        __syncthreads();
-        // below the diagonal, a row of blocks after the other: T_ij = -T_ii (sum of A_ik T_kj, j <= k < i).  A thread has four rows of one column.
-        for (int i = 1; i < 4; ++i) {
-            const int r0 = 16 * i + 4 * (tid & 3), col = tid >> 2;              // 64 columns, of which 16 i have work
-            float s[4] = {};
-            if (col < 16 * i) {
-                for (int k = col & ~15; k < 16 * i; ++k) {
-                    const float x = tt[k * GDC_TS + col];
-#pragma unroll
-                    for (int h = 0; h < 4; ++h) s[h] = __fmaf_rn(at[(r0 + h) * GDC_TS + k], x, s[h]);
-                }
-            }
-            __syncthreads();
-            if (col < 16 * i)
-#pragma unroll
-                for (int h = 0; h < 4; ++h) at[(r0 + h) * GDC_TS + col] = s[h];          // A's row of blocks has been read
-            __syncthreads();
-            if (col < 16 * i) {
-#pragma unroll
-                for (int h = 0; h < 4; ++h) s[h] = 0.0f;
-                for (int k = 0; k < 16; ++k) {
-                    const float x = at[(16 * i + k) * GDC_TS + col];
-#pragma unroll
-                    for (int h = 0; h < 4; ++h) s[h] = __fmaf_rn(tt[(r0 + h) * GDC_TS + 16 * i + k], x, s[h]);
-                }
-#pragma unroll
-                for (int h = 0; h < 4; ++h) tt[(r0 + h) * GDC_TS + col] = -s[h];
-            }
-            __syncthreads();
-        }
-        for (int e = tid; e < GDC_T * GDC_T; e += GDC_THREADS) {
-            const int i = e / GDC_T, j = e % GDC_T;
-            const float x = (j >> 4) <= (i >> 4) ? __fmul_rn(tt[i * GDC_TS + j], bs[j]) : 0.0f;
-            odd = odd || !(fabsf(x) < 1e30f);
-            rec[e] = x;
-        }
-        const int any = __syncthreads_or(odd ? 1 : 0);
-        if (tid == 0) rec[2 * GDC_T * GDC_T + 2 * GDC_T] = any ? 1.0f : 0.0f;
+    for (int i = 0; i < ROWS; ++i) {
+        const int r = ROWS * warp + i, row = r & (GDC_T - 1);
+        const uint32_t m = __reduce_max_sync(0xffffffffu, max(max(atc_abs_bits(x[i].x), atc_abs_bits(x[i].y)), max(atc_abs_bits(x[i].z), atc_abs_bits(x[i].w))));
+        const int s = atc_shift(m, 63);
+        const float f = atc_pow2(s);
+        uint2 hi, lo;
+        split_f16x2(__fmul_rn(x[i].x, f), __fmul_rn(x[i].y, f), hi.x, lo.x);
+        split_f16x2(__fmul_rn(x[i].z, f), __fmul_rn(x[i].w, f), hi.y, lo.y);
+        uint8_t *out = rec + (r < GDC_T ? 0 : 2 * GDC_KP) + row * GDC_KB + 8 * lane;
+        *reinterpret_cast<uint2 *>(out) = hi;
+        *reinterpret_cast<uint2 *>(out + GDC_KP) = lo;
+        if (lane == 0) reinterpret_cast<int *>(rec + 4 * GDC_KP)[r] = s;
     }
 }
 
-// grid (value heads x 3, sequences): columns 0 .. 47, 48 .. 87, 88 .. 127.  Warp w of eight: rows 16 (w % 4) .. of K S (w < 4) or Q S, and rows 16 w .. of the state, which
-// stay in registers; a copy of the state in shared memory is what the products read.
-__global__ void __launch_bounds__(GDC_THREADS, 1) gdn_scan_kernel(const __grid_constant__ GdnSeqs P, const float *recs) {
-    extern __shared__ __align__(16) float gdc_smem[];
-    float *kt0 = gdc_smem, *qt = kt0 + 2 * GDC_T * GDC_KS, *tb = qt + GDC_T * GDC_KS, *pt0 = tb + GDC_T * GDC_TS, *vt = pt0 + 2 * GDC_T * GDC_TS;           // K and P twice
-    float *st = vt + GDC_T * GDC_COLS, *rt = st + GDC_D * GDC_CS, *ut = rt + GDC_T * GDC_CS;
-    float *since0 = ut + GDC_T * GDC_CS, *flag = since0 + 4 * GDC_T;                   // e^G, behind it e^(G_63 - G), twice; [2]
+// grid (the same chunks, value heads): Tb and P.
+__global__ void __launch_bounds__(GDC_PREP_THREADS, 3) gdn_chunk_kernel(const __grid_constant__ GdnSeqs P, const uint8_t *kq_recs, uint8_t *tp_recs) {
+    extern __shared__ __align__(16) uint8_t gdc_smem[];
+    uint8_t *kp = gdc_smem, *qp = kp + 2 * GDC_KP;
+    float *at = reinterpret_cast<float *>(kp), *tt = at + GDC_T * GDC_TS, *pt = reinterpret_cast<float *>(qp);      // when the planes have been read
+    double *gs = reinterpret_cast<double *>(qp + 2 * GDC_KP);
+    float *bs = reinterpret_cast<float *>(gs + GDC_T);
+    int *shift = reinterpret_cast<int *>(bs + GDC_T);                        // [2][64] of K, of Q
+    uint64_t *full = reinterpret_cast<uint64_t *>(shift + 2 * GDC_T);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    constexpr int WARPS = GDC_PREP_THREADS / 32;
+    const int vh = blockIdx.y, share = P.n_v_heads / P.n_k_heads, kh = vh / share;
+    pdl_wait_prior_grid();
+    pdl_launch_dependents();
+    int seq, chunk;
+    if (!seq_of_item(P.start, P.n_seq, P.n_tok, (int)blockIdx.x, lane, [](int n) { return gdc_chunks(n); }, seq, chunk)) return;
+    const SeqRange range = seq_range(P.start, seq, P.n_tok);
+    const int n = min(GDC_T, range.n - chunk * GDC_T);
+    const size_t tok = (size_t)range.begin + chunk * GDC_T;
+    const uint8_t *kq = kq_recs + ((size_t)blockIdx.x * P.n_k_heads + kh) * GDC_KQ_REC;
+    uint8_t *rec = tp_recs + ((size_t)blockIdx.x * P.n_v_heads + vh) * GDC_TP_REC;
+    float *vec = reinterpret_cast<float *>(rec + GDC_TP_PLANES);
+    bool odd = false;                           // something that sums may not hold: the chunk goes token by token
+    if (tid == 0) {
+        const uint64_t pol = policy_evict_normal();
+        mbar_init(full, 1);
+        mbar_fence_init();
+        mbar_expect_tx(full, GDC_KQ_REC);
+        bulk_g2s(kp, kq, 4 * GDC_KP, full, pol);
+        bulk_g2s(shift, kq + 4 * GDC_KP, 2 * GDC_T * 4, full, pol);
+    }
+    if (warp == 0) {
+        // a decay below e^-1000 is none; sums in 64 bits: of two that are far from zero the difference matters
+        double x[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int i = 2 * lane + h;
+            const float gi = i < n ? P.g[(tok + i) * P.n_v_heads + vh] : 0.0f, bi = i < n ? P.beta[(tok + i) * P.n_v_heads + vh] : 0.0f;
+            odd = odd || !(gi < 1e30f) || !(fabsf(bi) < 1e30f);
+            x[h] = (double)fmaxf(gi, -1000.0f);
+            bs[i] = bi;
+        }
+        x[1] += x[0];
+        double sum = x[1];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const double y = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += y;
+        }
+        gs[2 * lane] = sum - x[1] + x[0];
+        gs[2 * lane + 1] = sum;
+    }
+    __syncthreads();
+    if (!__syncthreads_and(mbar_wait_hot(full, 0) ? 1 : 0)) return;          // (a wait ran out: the CTA leaves as a whole)
+    // ---- K K^T (two warps) and Q K^T, blocks of 16 x 16 on and below the diagonal: a warp has rows of blocks w and 3 - w, five blocks
+    float c[5][1][2][4];
+    const bool of_q = warp >= 2;
+    {
+        const uint32_t a0 = smem_u32(of_q ? qp : kp) + gdc_at_rows(lane, GDC_KB), b0 = smem_u32(kp) + gdc_at_turned(lane, GDC_KB);
+#pragma unroll
+        for (int i = 0; i < 5; ++i) {
+            const int top = warp & 1, m = i <= top ? top : 3 - top, j = i <= top ? i : i - top - 1;
+            const uint32_t a[1] = {a0 + 16 * m * GDC_KB};
+            gdc_product<1, 2, GDC_D / 16, false, false>(c[i], a, GDC_KP, 32, b0 + 16 * j * GDC_KB, GDC_KP, 32, 0);
+        }
+    }
+    __syncthreads();                            // the planes have been read: A, its inverse and P in fp32 take their place
+    if (tid < GDC_T) odd = odd || min(shift[tid], shift[GDC_T + tid]) <= 141 - (int)(ATC_HUGE >> 23);
+#pragma unroll
+    for (int i = 0; i < 5; ++i) {
+        const int top = warp & 1, m = i <= top ? top : 3 - top, jb = i <= top ? i : i - top - 1;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int row = 16 * m + g + 8 * ((e >> 1) & 1), col = 16 * jb + 8 * (e >> 2) + 2 * t + (e & 1);
+            float x = 0.0f;
+            if (col <= row && row < n) {
+                const float decay = expf((float)(gs[row] - gs[col])), f = atc_pow2(-shift[(of_q ? GDC_T : 0) + row]), f2 = atc_pow2(-shift[col]);
+                x = __fmul_rn(__fmul_rn(__fmul_rn(c[i][0][e >> 2][e & 3], f), f2), decay);
+                if (!of_q) x = col < row ? __fmul_rn(x, bs[row]) : 0.0f;
+                odd = odd || !(fabsf(x) < 1e30f);
+            }
+            (of_q ? pt : at)[row * GDC_TS + col] = x;
+        }
+    }
+    __syncthreads();
+    // ---- (1 + A)^-1: the four 16 x 16 blocks on the diagonal, a warp each, lane = column, from the top row down ...
+    if (lane < 16) {
+        const int blk = 16 * warp;
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            float s = i == lane ? 1.0f : 0.0f;
+#pragma unroll
+            for (int j = 0; j < i; ++j) s = __fmaf_rn(-at[(blk + i) * GDC_TS + blk + j], x[j], s);
+            x[i] = s;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) tt[(blk + i) * GDC_TS + blk + lane] = x[i];
+    }
+    __syncthreads();
+    // ... and below it, a row of blocks after the other: T_ij = -T_ii (sum of A_ik T_kj, j <= k < i).  A thread has eight rows of one column.
+    for (int i = 1; i < 4; ++i) {
+        const int r0 = 16 * i + 8 * (tid & 1), col = tid >> 1;          // 64 columns, of which 16 i have work
+        float s[8] = {};
+        if (col < 16 * i) {
+            for (int k = col & ~15; k < 16 * i; k += 4) {
+                const float x0 = tt[k * GDC_TS + col], x1 = tt[(k + 1) * GDC_TS + col], x2 = tt[(k + 2) * GDC_TS + col], x3 = tt[(k + 3) * GDC_TS + col];
+#pragma unroll
+                for (int h = 0; h < 8; ++h) {
+                    const float4 a = *reinterpret_cast<const float4 *>(at + (r0 + h) * GDC_TS + k);
+                    s[h] = __fmaf_rn(a.w, x3, __fmaf_rn(a.z, x2, __fmaf_rn(a.y, x1, __fmaf_rn(a.x, x0, s[h]))));
+                }
+            }
+        }
+        __syncthreads();
+        if (col < 16 * i)
+#pragma unroll
+            for (int h = 0; h < 8; ++h) at[(r0 + h) * GDC_TS + col] = s[h];          // A's row of blocks has been read
+        __syncthreads();
+        if (col < 16 * i) {
+#pragma unroll
+            for (int h = 0; h < 8; ++h) s[h] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 16; k += 4) {
+                const float *y = at + (16 * i + k) * GDC_TS + col;
+                const float x0 = y[0], x1 = y[GDC_TS], x2 = y[2 * GDC_TS], x3 = y[3 * GDC_TS];
+#pragma unroll
+                for (int h = 0; h < 8; ++h) {
+                    const float4 a = *reinterpret_cast<const float4 *>(tt + (r0 + h) * GDC_TS + 16 * i + k);
+                    s[h] = __fmaf_rn(a.w, x3, __fmaf_rn(a.z, x2, __fmaf_rn(a.y, x1, __fmaf_rn(a.x, x0, s[h]))));
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < 8; ++h) tt[(r0 + h) * GDC_TS + col] = -s[h];
+        }
+        __syncthreads();
+    }
+    // ---- planes of Tb and P: a warp per row, lane = two values
+#pragma unroll 4
+    for (int r = warp; r < 2 * GDC_T; r += WARPS) {
+        const int row = r & (GDC_T - 1), col = 2 * lane;
+        const bool there = (col >> 4) <= (row >> 4);
+        float2 x = make_float2(0.0f, 0.0f);
+        if (there) {
+            x = *reinterpret_cast<const float2 *>((r < GDC_T ? tt : pt) + row * GDC_TS + col);
+            if (r < GDC_T) x = make_float2(__fmul_rn(x.x, bs[col]), __fmul_rn(x.y, bs[col + 1]));
+        }
+        const uint32_t m = __reduce_max_sync(0xffffffffu, max(atc_abs_bits(x.x), atc_abs_bits(x.y)));
+        odd = odd || m >= ATC_HUGE;
+        const int s = atc_shift(m, 63);
+        const float f = atc_pow2(s);
+        uint32_t hi, lo;
+        split_f16x2(__fmul_rn(x.x, f), __fmul_rn(x.y, f), hi, lo);
+        uint8_t *out = rec + (r < GDC_T ? 0 : 2 * GDC_TP) + row * GDC_TB + 4 * lane;
+        *reinterpret_cast<uint32_t *>(out) = hi;
+        *reinterpret_cast<uint32_t *>(out + GDC_TP) = lo;
+        if (lane == 0) vec[3 * GDC_T + r] = atc_pow2(-s);
+    }
+    int least = 63;                             // K's smallest shift
+#pragma unroll
+    for (int h = 0; h < 2; ++h) least = min(least, shift[lane + 32 * h]);
+    least = __reduce_min_sync(0xffffffffu, least);
+    if (tid < GDC_T) {
+        const float eg = expf((float)gs[tid]);
+        vec[tid] = __fmul_rn(eg, atc_pow2(-shift[tid]));
+        vec[GDC_T + tid] = __fmul_rn(eg, atc_pow2(-shift[GDC_T + tid]));
+        const float left = __fmul_rn(expf((float)(gs[GDC_T - 1] - gs[tid])), atc_pow2(max(least - shift[tid], -126)));
+        vec[2 * GDC_T + tid] = left;
+        odd = odd || left >= 0x1p60f;
+    }
+    if (tid == 0) {
+        vec[5 * GDC_T] = expf((float)gs[GDC_T - 1]);
+        vec[5 * GDC_T + 1] = atc_pow2(-least);
+    }
+    const int any = __syncthreads_or(odd ? 1 : 0);
+    if (tid == 0) vec[5 * GDC_T + 2] = any ? 1.0f : 0.0f;
+}
+
+// grid (value heads x 3, sequences): columns 0 .. 47, 48 .. 87, 88 .. 127.  Warp w of eight: tokens 16 (w % 4) .. and half of the columns of all that has a row for each
+// token, and rows 16 w .. of the state, which stay in registers in fp32; its planes in shared memory are what the products read.
+__global__ void __launch_bounds__(GDC_THREADS, 1) gdn_scan_kernel(const __grid_constant__ GdnSeqs P, const uint8_t *kq_recs, const uint8_t *tp_recs) {
+    extern __shared__ __align__(16) uint8_t gdc_smem[];
+    uint8_t *kp0 = gdc_smem, *qp = kp0 + 4 * GDC_KP, *tp = qp + 2 * GDC_KP, *sp = tp + 4 * GDC_TP, *up = sp + 2 * GDC_SP;       // K twice; Tb, P; U, U times its factors
+    uint8_t *rp = qp;                                                   // V - e^G K S takes the place of Q when that has been read
+    float *vt = reinterpret_cast<float *>(up + 4 * GDC_UP), *vec = vt + GDC_T * GDC_COLS;
+    uint32_t *s_most = reinterpret_cast<uint32_t *>(vec + GDC_VEC), *r_most = s_most + 2 * 8, *u_most = r_most + 8;          // largest magnitudes of eight columns: S's of this chunk and of the next; U's, U's times its factors
+    uint64_t *kfull = reinterpret_cast<uint64_t *>(u_most + 2 * 8), *qvfull = kfull + 2, *tpfull = kfull + 3;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int vh = blockIdx.x / GDC_SLICES, slice = blockIdx.x % GDC_SLICES, s = blockIdx.y;
     const int c0 = slice == 0 ? 0 : 48 + 40 * (slice - 1), cols = slice == 0 ? 48 : 40;
@@ -366,158 +438,247 @@ __global__ void __launch_bounds__(GDC_THREADS, 1) gdn_scan_kernel(const __grid_c
     int first = 0;
     for (int i = lane; i < s; i += 32) first += gdc_chunks(max(0, seq_range(P.start, i, P.n_tok).n));
     first = __reduce_add_sync(0xffffffffu, first);
-    const float *rec0 = recs + ((size_t)first * P.n_v_heads + vh) * GDC_REC;
-    const size_t rec_stride = (size_t)P.n_v_heads * GDC_REC;
-    const bool vec = ((reinterpret_cast<uintptr_t>(P.k) | reinterpret_cast<uintptr_t>(P.q)) & 15u) == 0, vvec = (reinterpret_cast<uintptr_t>(P.v) & 15u) == 0;
-    const size_t kstride = (size_t)P.n_k_heads * GDC_D, vstride = (size_t)P.n_v_heads * GDC_D;
+    const uint8_t *kq = kq_recs + ((size_t)first * P.n_k_heads + kh) * GDC_KQ_REC, *rec = tp_recs + ((size_t)first * P.n_v_heads + vh) * GDC_TP_REC;
+    const size_t kq_stride = (size_t)P.n_k_heads * GDC_KQ_REC, rec_stride = (size_t)P.n_v_heads * GDC_TP_REC;
+    const size_t vstride = (size_t)P.n_v_heads * GDC_D;
+    const bool vvec = (reinterpret_cast<uintptr_t>(P.v) & 15u) == 0;
 
-    // what a chunk brings, in the order in which room for it becomes free
-    auto load_qv = [&](int c) {
-        const size_t tok = (size_t)range.begin + c * GDC_T;
+    // what a chunk brings, as room for it becomes free: bulk copies by one thread, V's rows by a warp
+    const uint64_t pol = policy_evict_normal();
+    auto load_k = [&](int c) {
+        mbar_expect_tx(kfull + (c & 1), 2 * GDC_KP);
+        bulk_g2s(kp0 + (c & 1) * 2 * GDC_KP, kq + c * kq_stride, 2 * GDC_KP, kfull + (c & 1), pol);
+    };
+    auto load_tp = [&](int c) {
+        mbar_expect_tx(tpfull, GDC_TP_REC);
+        bulk_g2s(tp, rec + c * rec_stride, GDC_TP_PLANES, tpfull, pol);
+        bulk_g2s(vec, rec + c * rec_stride + GDC_TP_PLANES, GDC_VEC * 4, tpfull, pol);
+    };
+    int v_row[3], v_col[3];                                     // a thread's three pieces of four values
+#pragma unroll
+    for (int e = 0; e < 3; ++e) v_row[e] = (tid + e * GDC_THREADS) / (GDC_COLS / 4), v_col[e] = 4 * ((tid + e * GDC_THREADS) % (GDC_COLS / 4));
+    auto load_qv = [&](int c) {                                 // the whole CTA (V by sixteen bytes each: 64 bulk copies of a row took a warp 3600 cycles)
+        const float *src = P.v + (((size_t)range.begin + c * GDC_T) * P.n_v_heads + vh) * GDC_D + c0;
         const int n = min(GDC_T, range.n - c * GDC_T);
-        gdc_load<GDC_D>(qt, GDC_KS, P.q + (tok * P.n_k_heads + kh) * GDC_D, kstride, n, vec);
-        gdc_load<GDC_COLS>(vt, GDC_COLS, P.v + (tok * P.n_v_heads + vh) * GDC_D + c0, vstride, n, vvec, cols);
+        if (tid == 0) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            mbar_expect_tx(qvfull, 2 * GDC_KP);
+            bulk_g2s(qp, kq + c * kq_stride + 2 * GDC_KP, 2 * GDC_KP, qvfull, pol);
+        }
+#pragma unroll
+        for (int e = 0; e < 3; ++e) {
+            float *dst = vt + v_row[e] * GDC_COLS + v_col[e];
+            const float *x = src + (size_t)v_row[e] * vstride + v_col[e];
+            if (v_row[e] >= n || v_col[e] >= cols) *reinterpret_cast<float4 *>(dst) = make_float4(0.f, 0.f, 0.f, 0.f);
+            else if (vvec) cp_async16(dst, x);
+            else *reinterpret_cast<float4 *>(dst) = make_float4(x[0], x[1], x[2], x[3]);
+        }
+        cp_async_commit();
     };
-    auto load_t = [&](int c) { gdc_load<GDC_T>(tb, GDC_TS, rec0 + c * rec_stride, GDC_T, GDC_T, true); };
-    auto load_kp = [&](int c) {
-        const size_t tok = (size_t)range.begin + c * GDC_T;
-        const int n = min(GDC_T, range.n - c * GDC_T), b = c & 1;
-        gdc_load<GDC_D>(kt0 + b * GDC_T * GDC_KS, GDC_KS, P.k + (tok * P.n_k_heads + kh) * GDC_D, kstride, n, vec);
-        const float *rec = rec0 + c * rec_stride + GDC_T * GDC_T;
-        gdc_load<GDC_T>(pt0 + b * GDC_T * GDC_TS, GDC_TS, rec, GDC_T, GDC_T, true);
-        if (tid < 2 * GDC_T / 4) cp_async16(since0 + 2 * GDC_T * b + 4 * tid, rec + GDC_T * GDC_T + 4 * tid);
-        if (tid == 2 * GDC_T / 4) cp_async4(flag + b, rec + GDC_T * GDC_T + 2 * GDC_T);
-    };
-    load_kp(0);
+    if (tid == 0) {
+        for (int b = 0; b < 4; ++b) mbar_init(kfull + b, 1);
+        mbar_fence_init();
+    }
+    if (tid < 5 * 8) s_most[tid] = 0u;
+    __syncthreads();
+    if (tid == 0) load_k(0);
     load_qv(0);
-    load_t(0);
-    cp_async_commit();
     float *Sg = P.state + ((size_t)slot * P.n_v_heads + vh) * GDC_D * GDC_D + c0;
     float S[GDC_NT][4];                                         // rows 16 warp + g, + 8; columns 8 nt + 2 t, + 1
 #pragma unroll
     for (int j = 0; j < GDC_NT; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) S[j][e] = 8 * j < cols ? Sg[(size_t)(16 * warp + g + 8 * (e >> 1)) * GDC_D + 8 * j + 2 * t + (e & 1)] : 0.0f;
-    auto store_s = [&] {
+    // the largest magnitude of each eight columns of a warp's 16 rows, into dst
+    auto tiles_most = [&](auto &x, uint32_t *dst) {
+        constexpr int N = sizeof(x) / sizeof(x[0]);
+        uint32_t mine = 0u;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const uint32_t m = __reduce_max_sync(0xffffffffu, max(max(atc_abs_bits(x[j][0]), atc_abs_bits(x[j][1])), max(atc_abs_bits(x[j][2]), atc_abs_bits(x[j][3]))));
+            if (lane == j) mine = m;
+        }
+        if (lane < N) atomicMax(dst + lane, mine);
+    };
+    // planes of two values of a row, times f
+    auto store_planes = [&](uint8_t *at, int low, float x, float y, float f) {
+        uint32_t hi, lo;
+        split_f16x2(__fmul_rn(x, f), __fmul_rn(y, f), hi, lo);
+        *reinterpret_cast<uint32_t *>(at) = hi;
+        *reinterpret_cast<uint32_t *>(at + low) = lo;
+    };
+    auto store_s = [&](const uint32_t *most) {
 #pragma unroll
         for (int j = 0; j < GDC_NT; ++j) {
-            *reinterpret_cast<float2 *>(st + (16 * warp + g) * GDC_CS + 8 * j + 2 * t) = make_float2(S[j][0], S[j][1]);
-            *reinterpret_cast<float2 *>(st + (16 * warp + g + 8) * GDC_CS + 8 * j + 2 * t) = make_float2(S[j][2], S[j][3]);
+            const float f = atc_pow2(atc_shift(most[j], 63));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) store_planes(sp + (16 * warp + g + 8 * h) * GDC_CB + 16 * j + 4 * t, GDC_SP, S[j][2 * h], S[j][2 * h + 1], f);
         }
     };
-    if (slice)                                                  // columns 40 .. 47 are nobody's: zeros
-        for (int i = tid; i < GDC_T * 8; i += GDC_THREADS) vt[(i / 8) * GDC_COLS + 40 + i % 8] = 0.0f;
-    store_s();
+    tiles_most(S, s_most);
+    __syncthreads();
+    store_s(s_most);
+    constexpr int NH = GDC_NT / 2;                              // column tiles of a warp that has tokens' rows, from j0 on
+    const int j0 = NH * (warp >> 2);
+    const uint32_t at_k = gdc_at_rows(lane, GDC_KB), at_t = gdc_at_rows(lane, GDC_TB), at_kt = gdc_at_turned(lane, GDC_KB);
+    const uint32_t b_s = smem_u32(sp) + gdc_at_rows(lane, GDC_CB), b_r = smem_u32(rp) + gdc_at_rows(lane, GDC_CB), b_u = smem_u32(up) + gdc_at_rows(lane, GDC_CB);
+    bool ok = true;
     for (int c = 0; c < nchunk; ++c) {
-        const int b = c & 1, n = min(GDC_T, range.n - c * GDC_T);
+        const int n = min(GDC_T, range.n - c * GDC_T);
         const size_t tok = (size_t)range.begin + c * GDC_T;
+        const uint32_t kb = smem_u32(kp0) + (c & 1) * 2 * GDC_KP;
+        uint32_t *most = s_most + (c & 1) * 8, *next = s_most + ((c & 1) ^ 1) * 8;
+        ok = mbar_wait_hot(kfull + (c & 1), (uint32_t)((c >> 1) & 1)) && ok;
+        ok = mbar_wait_hot(qvfull, (uint32_t)(c & 1)) && ok;
         cp_async_wait<0>();
-        __syncthreads();                                        // the chunk, and the state of the one before
-        if (c + 1 < nchunk) load_kp(c + 1);
-        const float *kt = kt0 + b * GDC_T * GDC_KS, *pt = pt0 + b * GDC_T * GDC_TS, *eg = since0 + 2 * GDC_T * b, *left = eg + GDC_T;
-        // ---- K S (then R = V - e^G K S) and Q S
-        float acc[GDC_NT][4];
+        if (!__syncthreads_and(ok ? 1 : 0)) return;             // the chunk's K, Q and V, and the planes of the state (a wait ran out: the CTA leaves as a whole)
+        if (tid == 0) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            load_tp(c);
+            if (c + 1 < nchunk) load_k(c + 1);
+        }
+        if (tid < 8) r_most[tid] = u_most[tid] = u_most[tid + 8] = next[tid] = 0u;
+        // ---- K S and Q S
+        float acc[2][NH][4];
+        {
+            const uint32_t a[2] = {kb + 16 * mt * GDC_KB + at_k, smem_u32(qp) + 16 * mt * GDC_KB + at_k};
+            gdc_product<2, NH, GDC_D / 16, false, true>(acc, a, GDC_KP, 32, b_s + 16 * j0, GDC_SP, 16 * GDC_CB, 32);
+        }
+        ok = mbar_wait_hot(tpfull, (uint32_t)(c & 1)) && ok;
+        if (!__syncthreads_and(ok ? 1 : 0)) return;             // Tb, P and the factors; the planes of Q have been read
+        bool odd = vec[5 * GDC_T + 2] != 0.0f;
 #pragma unroll
-        for (int j = 0; j < GDC_NT; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[j][e] = 0.0f;
-        gdc_product<GDC_NT>(acc, (warp < 4 ? kt : qt) + (16 * mt + g) * GDC_KS + t, GDC_KS, 1, st + t * GDC_CS + g, GDC_CS, 1, GDC_D / 8);
-        bool odd = flag[b] != 0.0f;
-#pragma unroll
-        for (int j = 0; j < GDC_NT; ++j)
+        for (int j = 0; j < NH; ++j) {
+            const float fs = atc_pow2(-atc_shift(most[j0 + j], 63));
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int i = 16 * mt + g + 8 * h, col = 8 * j + 2 * t;
-                float2 x = make_float2(__fmul_rn(acc[j][2 * h], eg[i]), __fmul_rn(acc[j][2 * h + 1], eg[i]));
-                if (warp < 4) {
-                    const float2 v = *reinterpret_cast<const float2 *>(vt + i * GDC_COLS + col);
-                    x = make_float2(__fsub_rn(v.x, x.x), __fsub_rn(v.y, x.y));
-                    *reinterpret_cast<float2 *>(rt + i * GDC_CS + col) = x;
+                const int i = 16 * mt + g + 8 * h;
+                const float fk = vec[i], fq = vec[GDC_T + i];
+                const float2 v = *reinterpret_cast<const float2 *>(vt + i * GDC_COLS + 8 * (j0 + j) + 2 * t);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float &x = acc[0][j][2 * h + e], &y = acc[1][j][2 * h + e];
+                    x = __fsub_rn(e ? v.y : v.x, __fmul_rn(__fmul_rn(x, fs), fk));          // V - e^G K S
+                    y = __fmul_rn(__fmul_rn(y, fs), fq);                                    // e^G Q S
+                    odd = odd || !(fabsf(x) < 0x1p60f) || !(fabsf(y) < 0x1p60f);
                 }
-                odd = odd || !(fabsf(x.x) < 1e30f) || !(fabsf(x.y) < 1e30f);
-                acc[j][2 * h] = x.x;
-                acc[j][2 * h + 1] = x.y;
             }
+        }
+        tiles_most(acc[0], r_most + j0);
         int slow = __syncthreads_or(odd ? 1 : 0);
-        // ---- U = Tb R, rows 16 mt .., half of the columns
+#pragma unroll
+        for (int j = 0; j < NH; ++j) {
+            const float f = atc_pow2(atc_shift(r_most[j0 + j], 63));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) store_planes(rp + (16 * mt + g + 8 * h) * GDC_CB + 16 * (j0 + j) + 4 * t, GDC_UP, acc[0][j][2 * h], acc[0][j][2 * h + 1], f);
+        }
+        __syncthreads();
+        // ---- U = Tb (V - e^G K S); x: the same times the factors of the state's update
         {
-            float u[GDC_NT / 2][4];
-#pragma unroll
-            for (int j = 0; j < GDC_NT / 2; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) u[j][e] = 0.0f;
-            const int h0 = (warp >> 2) * (GDC_COLS / 2);
-            gdc_product<GDC_NT / 2>(u, tb + (16 * mt + g) * GDC_TS + t, GDC_TS, 1, rt + t * GDC_CS + h0 + g, GDC_CS, 1, 2 * (mt + 1));
+            float u[1][NH][4], x[NH][4];
+            const uint32_t a[1] = {smem_u32(tp) + 16 * mt * GDC_TB + at_t};
+            gdc_product<1, NH, GDC_T / 16, false, true>(u, a, GDC_TP, 32, b_r + 16 * j0, GDC_UP, 16 * GDC_CB, 32);
             odd = false;
 #pragma unroll
-            for (int j = 0; j < GDC_NT / 2; ++j)
+            for (int j = 0; j < NH; ++j) {
+                const float fr = atc_pow2(-atc_shift(r_most[j0 + j], 63));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int i = 16 * mt + g + 8 * (e >> 1);
+                    u[0][j][e] = __fmul_rn(__fmul_rn(u[0][j][e], fr), vec[3 * GDC_T + i]);
+                    x[j][e] = __fmul_rn(u[0][j][e], vec[2 * GDC_T + i]);
+                    odd = odd || !(fabsf(u[0][j][e]) < 0x1p60f) || !(fabsf(x[j][e]) < 0x1p60f);
+                }
+            }
+            tiles_most(u[0], u_most + j0);
+            tiles_most(x, u_most + 8 + j0);
+            slow |= __syncthreads_or(odd ? 1 : 0);              // (V - e^G K S, in the place of Q, has been read)
+#pragma unroll
+            for (int j = 0; j < NH; ++j) {
+                const float fu = atc_pow2(atc_shift(u_most[j0 + j], 63)), fx = atc_pow2(atc_shift(u_most[8 + j0 + j], 63));
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    odd = odd || !(fabsf(u[j][2 * h]) < 1e30f) || !(fabsf(u[j][2 * h + 1]) < 1e30f);
-                    *reinterpret_cast<float2 *>(ut + (16 * mt + g + 8 * h) * GDC_CS + h0 + 8 * j + 2 * t) = make_float2(u[j][2 * h], u[j][2 * h + 1]);
+                    uint8_t *dst = up + (16 * mt + g + 8 * h) * GDC_CB + 16 * (j0 + j) + 4 * t;
+                    store_planes(dst, GDC_UP, u[0][j][2 * h], u[0][j][2 * h + 1], fu);
+                    store_planes(dst + 2 * GDC_UP, GDC_UP, x[j][2 * h], x[j][2 * h + 1], fx);
                 }
-        }
-        slow |= __syncthreads_or(odd ? 1 : 0);
-        if (!slow) {
-            if (c + 1 < nchunk) {                               // Q, V and Tb have been read
-                load_qv(c + 1);
-                load_t(c + 1);
             }
-            cp_async_commit();
+        }
+        __syncthreads();
+        if (!slow) {
+            if (c + 1 < nchunk) load_qv(c + 1);
             // ---- S = e^G_63 S + K^T (e^(G_63 - G) U)
-            const float decay = eg[GDC_T - 1];
+            {
+                float d[1][GDC_NT][4];
+                const uint32_t a[1] = {kb + 32 * warp + at_kt};
+                gdc_product<1, GDC_NT, GDC_T / 16, true, true>(d, a, GDC_KP, 16 * GDC_KB, b_u + 2 * GDC_UP, GDC_UP, 16 * GDC_CB, 32);
+                const float decay = vec[5 * GDC_T], kf = vec[5 * GDC_T + 1];
 #pragma unroll
-            for (int j = 0; j < GDC_NT; ++j)
+                for (int j = 0; j < GDC_NT; ++j) {
+                    const float f = __fmul_rn(kf, atc_pow2(-atc_shift(u_most[8 + j], 63)));
 #pragma unroll
-                for (int e = 0; e < 4; ++e) S[j][e] = __fmul_rn(S[j][e], decay);
-            gdc_product<GDC_NT>(S, kt + t * GDC_KS + 16 * warp + g, 1, GDC_KS, ut + t * GDC_CS + g, GDC_CS, 1, GDC_T / 8, [&](int k) { return left[k + t]; });
-            store_s();                                          // (K S and Q S were read in front of two barriers)
+                    for (int e = 0; e < 4; ++e) S[j][e] = __fmaf_rn(S[j][e], decay, __fmul_rn(d[0][j][e], f));
+                }
+            }
+            tiles_most(S, next);
             // ---- O = e^G Q S + P U
-            if (warp >= 4) {
-                gdc_product<GDC_NT>(acc, pt + (16 * mt + g) * GDC_TS + t, GDC_TS, 1, ut + t * GDC_CS + g, GDC_CS, 1, 2 * (mt + 1));
+            {
+                float o[1][NH][4];
+                const uint32_t a[1] = {smem_u32(tp) + 2 * GDC_TP + 16 * mt * GDC_TB + at_t};
+                gdc_product<1, NH, GDC_T / 16, false, true>(o, a, GDC_TP, 32, b_u + 16 * j0, GDC_UP, 16 * GDC_CB, 32);
 #pragma unroll
-                for (int j = 0; j < GDC_NT; ++j)
+                for (int j = 0; j < NH; ++j) {
+                    const float fu = atc_pow2(-atc_shift(u_most[j0 + j], 63));
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const int i = 16 * mt + g + 8 * h;
-                        if (i < n && 8 * j < cols) {
-                            float *o = P.out + ((tok + i) * P.n_v_heads + vh) * GDC_D + c0 + 8 * j + 2 * t;
-                            o[0] = acc[j][2 * h];
-                            o[1] = acc[j][2 * h + 1];
+                        const float f = vec[4 * GDC_T + i];
+                        if (i < n && 8 * (j0 + j) < cols) {
+                            float *dst = P.out + ((tok + i) * P.n_v_heads + vh) * GDC_D + c0 + 8 * (j0 + j) + 2 * t;
+                            dst[0] = __fmaf_rn(__fmul_rn(o[0][j][2 * h], f), fu, acc[1][j][2 * h]);
+                            dst[1] = __fmaf_rn(__fmul_rn(o[0][j][2 * h + 1], f), fu, acc[1][j][2 * h + 1]);
                         }
                     }
+                }
             }
         } else {
-            // ---- a value that sums may not hold: token by token, as the definition has it.  Thread = a column and every fifth row.
+            // ---- a value that sums may not hold: token by token, as the definition has it.  Thread = a column and every fifth row; the state in the place of its planes.
+            float *st = reinterpret_cast<float *>(sp), *x1 = reinterpret_cast<float *>(up), *x2 = x1 + 5 * GDC_COLS;
+#pragma unroll
+            for (int j = 0; j < GDC_NT; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) st[(16 * warp + g + 8 * (e >> 1)) * GDC_COLS + 8 * j + 2 * t + (e & 1)] = S[j][e];
+            __syncthreads();
             const int col = tid % GDC_COLS, part = tid / GDC_COLS;
             for (int i = 0; i < n; ++i) {
                 const float decay = expf(P.g[(tok + i) * P.n_v_heads + vh]), beta = P.beta[(tok + i) * P.n_v_heads + vh];
-                const float *k = kt + i * GDC_KS, *q = qt + i * GDC_KS;
-                float x = 0.0f;
-                if (part < 5)
+                const float *k = P.k + ((tok + i) * P.n_k_heads + kh) * GDC_D, *q = P.q + ((tok + i) * P.n_k_heads + kh) * GDC_D;
+                if (part < 5) {
+                    float x = 0.0f;
                     for (int r = part; r < GDC_D; r += 5) {
-                        const float y = __fmul_rn(st[r * GDC_CS + col], decay);
-                        st[r * GDC_CS + col] = y;
+                        const float y = __fmul_rn(st[r * GDC_COLS + col], decay);
+                        st[r * GDC_COLS + col] = y;
                         x = __fadd_rn(x, __fmul_rn(k[r], y));
                     }
-                if (part < 5) rt[part * GDC_CS + col] = x;
+                    x1[part * GDC_COLS + col] = x;
+                }
                 __syncthreads();
                 if (part < 5) {
-                    x = 0.0f;
-                    for (int p = 0; p < 5; ++p) x = __fadd_rn(x, rt[p * GDC_CS + col]);
+                    float x = 0.0f;
+                    for (int p = 0; p < 5; ++p) x = __fadd_rn(x, x1[p * GDC_COLS + col]);
                     const float d = __fsub_rn(vt[i * GDC_COLS + col], x);
                     x = 0.0f;
                     for (int r = part; r < GDC_D; r += 5) {
-                        const float y = __fadd_rn(st[r * GDC_CS + col], __fmul_rn(__fmul_rn(beta, k[r]), d));
-                        st[r * GDC_CS + col] = y;
+                        const float y = __fadd_rn(st[r * GDC_COLS + col], __fmul_rn(__fmul_rn(beta, k[r]), d));
+                        st[r * GDC_COLS + col] = y;
                         x = __fadd_rn(x, __fmul_rn(q[r], y));
                     }
-                    ut[part * GDC_CS + col] = x;
+                    x2[part * GDC_COLS + col] = x;
                 }
                 __syncthreads();
                 if (part == 0 && col < cols) {
-                    x = 0.0f;
-                    for (int p = 0; p < 5; ++p) x = __fadd_rn(x, ut[p * GDC_CS + col]);
+                    float x = 0.0f;
+                    for (int p = 0; p < 5; ++p) x = __fadd_rn(x, x2[p * GDC_COLS + col]);
                     P.out[((tok + i) * P.n_v_heads + vh) * GDC_D + c0 + col] = x;
                 }
             }
@@ -525,14 +686,12 @@ __global__ void __launch_bounds__(GDC_THREADS, 1) gdn_scan_kernel(const __grid_c
 #pragma unroll
             for (int j = 0; j < GDC_NT; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) S[j][e] = st[(16 * warp + g + 8 * (e >> 1)) * GDC_CS + 8 * j + 2 * t + (e & 1)];
-            __syncthreads();
-            if (c + 1 < nchunk) {
-                load_qv(c + 1);
-                load_t(c + 1);
-            }
-            cp_async_commit();
+                for (int e = 0; e < 4; ++e) S[j][e] = st[(16 * warp + g + 8 * (e >> 1)) * GDC_COLS + 8 * j + 2 * t + (e & 1)];
+            if (c + 1 < nchunk) load_qv(c + 1);
+            tiles_most(S, next);
         }
+        __syncthreads();                                        // the maxima; S's planes have long been read
+        store_s(next);
     }
 #pragma unroll
     for (int j = 0; j < GDC_NT; ++j)
