@@ -22,6 +22,7 @@
 #include "kv.cuh"
 #include "ops.cuh"
 #include "pages.cuh"
+#include "pages_tc.cuh"
 #include "probe.cuh"
 #include "ptq.cuh"
 #include "repack.cuh"
@@ -1915,23 +1916,42 @@ int check_pages(const bonsai_b200_pages *p, int layer, PageCache *C) {
     return 0;
 }
 
-// How pages_attn divides a call: 16 rowt rows a CTA, a span of pages a CTA, CTAs per kv head.
+// How pages_attn divides a call: 16 rowt rows a CTA, a span of pages a CTA, CTAs per kv head.  tc: sequences that may be on the tensor cores (0: none).
 struct PagesPlan {
-    int rowt, pages_per_split, splits;
-    int64_t tiles;
+    int rowt, pages_per_split, splits, max_pages;
+    int64_t tiles, tc;
+    int64_t part_bytes, image_bytes, redo_bytes;
+    int64_t bytes() const { return part_bytes + image_bytes + redo_bytes; }
 };
+constexpr int64_t PTC_IMAGE_LIMIT = int64_t(5) << 29;            // 2.5 GB: a full context of the 27B model
 PagesPlan plan_pages(int n_tok, int max_len, int n_seq, int n_head, int n_head_kv) {
-    PagesPlan p;
-    const int64_t rows = (int64_t)n_tok * (n_head / n_head_kv), each = (rows + n_seq - 1) / n_seq;
-    p.rowt = each <= 16 ? 1 : each <= 32 ? 2 : 4;
-    const int64_t high = 16 * p.rowt;
+    PagesPlan p = {};
+    const int64_t rows = (int64_t)n_tok * (n_head / n_head_kv), each = (rows + n_seq - 1) / n_seq, pages = std::max(1, (int)(((int64_t)max_len + PG_POS - 1) / PG_POS));
+    p.max_pages = (int)pages;
+    p.tc = std::min<int64_t>(n_seq, rows / PTC_ROWS);
+    if (rows < 2 * PTC_ROWS || p.tc * pages * n_head_kv > PTC_IMAGE_LIMIT / ATC_IMG_BYTES) p.tc = 0;
+    p.rowt = p.tc || each > 32 ? 4 : each > 16 ? 2 : 1;
+    const int64_t high = p.tc ? PTC_ROWS : 16 * p.rowt;
     p.tiles = (rows + (int64_t)std::min(n_seq, n_tok) * (high - 1)) / high;
-    // A span of pages for each of the CTAs that are resident at once.  Of several sequences the longest is known only: they are taken to hold 3 / 8 of that.
-    const int64_t items = std::max<int64_t>(1, (rows + high - 1) / high) * n_head_kv, pages = std::max(1, (int)(((int64_t)max_len + PG_POS - 1) / PG_POS));
-    const int64_t load = n_seq > 1 ? items * pages * 3 / 8 : items * pages;
-    const int64_t want = std::max<int64_t>(2, (load + 2 * SM_COUNT - 1) / (2 * SM_COUNT));
-    p.pages_per_split = (int)std::min(want, pages);
+    const int64_t items = std::max<int64_t>(1, (rows + high - 1) / high) * n_head_kv;
+    if (p.tc) {
+        // spans that fill the last round of CTAs, one per SM; a CTA's start and its share of the join are worth four pages
+        int64_t best = INT64_MAX;
+        for (int64_t s = 1; s <= std::min<int64_t>(pages, 16); ++s) {
+            const int64_t span = (pages + s - 1) / s, cost = ((items * s + SM_COUNT - 1) / SM_COUNT) * (span + 4);
+            if (cost < best) best = cost, p.pages_per_split = (int)span;
+        }
+    } else {
+        // A span of pages for each of the CTAs that are resident at once.  Of several sequences the longest is known only: they are taken to hold 3 / 8 of that.
+        const int64_t load = n_seq > 1 ? items * pages * 3 / 8 : items * pages;
+        const int64_t want = std::max<int64_t>(2, (load + 2 * SM_COUNT - 1) / (2 * SM_COUNT));
+        p.pages_per_split = (int)std::min(want, pages);
+    }
     p.splits = (int)((pages + p.pages_per_split - 1) / p.pages_per_split);
+    p.part_bytes = p.splits == 1 ? 0 : (int64_t)p.splits * n_tok * n_head * (KV_D + 2) * (int64_t)sizeof(float);
+    p.part_bytes = (p.part_bytes + 15) / 16 * 16;
+    p.image_bytes = p.tc * pages * n_head_kv * ATC_IMG_BYTES;
+    p.redo_bytes = p.tc ? (p.tiles * n_head_kv * p.splits * (int64_t)sizeof(int) + 15) / 16 * 16 : 0;
     return p;
 }
 inline bool pages_attn_sizes(int n_tok, int max_len, int n_seq, int n_head, int n_head_kv) {
@@ -1977,8 +1997,7 @@ int bonsai_b200_pages_append(const bonsai_b200_pages *pages, int layer, const fl
 
 int64_t bonsai_b200_pages_attn_workspace(int n_tok, int max_len, int n_seq, int n_head, int n_head_kv) {
     if (!pages_attn_sizes(n_tok, max_len, n_seq, n_head, n_head_kv)) return 0;
-    const PagesPlan plan = plan_pages(n_tok, max_len, n_seq, n_head, n_head_kv);
-    return plan.splits == 1 ? 0 : (int64_t)plan.splits * n_tok * n_head * (KV_D + 2) * (int64_t)sizeof(float);
+    return plan_pages(n_tok, max_len, n_seq, n_head, n_head_kv).bytes();
 }
 
 int bonsai_b200_pages_attn(const bonsai_b200_pages *pages, int layer, const float *q, float *out, int n_head, int max_len, void *workspace,
@@ -2000,19 +2019,35 @@ int bonsai_b200_pages_attn(const bonsai_b200_pages *pages, int layer, const floa
     P.pages_per_split = plan.pages_per_split;
     P.splits = plan.splits;
     P.scale = scale;
-    if (plan.splits > 1) {
-        const int64_t rows = (int64_t)plan.splits * C.n_tok * n_head;
-        if (!workspace || !aligned16(workspace) || workspace_bytes < rows * (KV_D + 2) * (int64_t)sizeof(float)) return 1;
-        P.part_acc = static_cast<float *>(workspace);
-        P.part_ml = reinterpret_cast<float2 *>(P.part_acc + rows * KV_D);
+    if (plan.bytes()) {
+        if (!workspace || !aligned16(workspace) || workspace_bytes < plan.bytes()) return 1;
+        uint8_t *w = static_cast<uint8_t *>(workspace);
+        P.images = w;
+        P.redo = reinterpret_cast<int *>(w + plan.image_bytes);
+        P.part_acc = reinterpret_cast<float *>(w + plan.image_bytes + plan.redo_bytes);
+        P.part_ml = reinterpret_cast<float2 *>(P.part_acc + (int64_t)plan.splits * C.n_tok * n_head * KV_D);
     }
-    static SmemOptIn opt[3];
-    auto run = [&](auto kernel, SmemOptIn &o) {
+    const cudaStream_t st = as_stream(stream);
+    static SmemOptIn opt[5];
+    auto run = [&](auto kernel, SmemOptIn &o, int64_t tiles, int threads, int smem) {
         const cudaError_t e = o.ensure(kernel);
         if (e != cudaSuccess) return e;
-        return launch(kernel, dim3((unsigned)plan.tiles, (unsigned)C.n_head_kv, (unsigned)plan.splits), dim3(PGA_THREADS), (size_t)pga_smem_bytes(plan.rowt), as_stream(stream), true, P);
+        return launch(kernel, dim3((unsigned)tiles, (unsigned)C.n_head_kv, (unsigned)plan.splits), dim3((unsigned)threads), (size_t)smem, st, true, P);
     };
-    cudaError_t e = plan.rowt == 1 ? run(pages_attn_kernel<1>, opt[0]) : plan.rowt == 2 ? run(pages_attn_kernel<2>, opt[1]) : run(pages_attn_kernel<4>, opt[2]);
+    const int smem = pga_smem_bytes(plan.rowt);
+    cudaError_t e;
+    if (plan.tc) {
+        if (2 * plan.tiles > INT32_MAX || plan.tc * plan.max_pages > INT32_MAX) return 1;
+        P.max_pages = plan.max_pages;
+        P.n_tc = (int)plan.tc;
+        e = launch(pages_planes_kernel, dim3((unsigned)(plan.tc * plan.max_pages), (unsigned)C.n_head_kv, 2), dim3(ATC_PREP_THREADS), 0, st, true, P);
+        if (e == cudaSuccess) e = run(pages_tc_kernel, opt[3], plan.tiles, ATC_THREADS, ATC_SMEM_BYTES);
+        if (e == cudaSuccess) e = run(pages_attn_kernel<4, true>, opt[4], 2 * plan.tiles, PGA_THREADS, smem);
+    } else {
+        e = plan.rowt == 1   ? run(pages_attn_kernel<1>, opt[0], plan.tiles, PGA_THREADS, smem)
+            : plan.rowt == 2 ? run(pages_attn_kernel<2>, opt[1], plan.tiles, PGA_THREADS, smem)
+                             : run(pages_attn_kernel<4>, opt[2], plan.tiles, PGA_THREADS, smem);
+    }
     if (e == cudaSuccess && plan.splits > 1) {
         const int roww = plan.splits >= 24 ? 8 : plan.splits >= 6 ? 2 : 1;
         const int64_t ctas = ((int64_t)C.n_tok * n_head * roww + PGJ_WARPS - 1) / PGJ_WARPS;

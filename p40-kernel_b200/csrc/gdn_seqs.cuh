@@ -39,31 +39,43 @@ __global__ void __launch_bounds__(GDN_WARPS * 32) gdn_seqs_step_kernel(const __g
     const int kh = vh / (P.n_v_heads / P.n_k_heads);
     pdl_wait_prior_grid();
     pdl_launch_dependents();
+    // the state and the first token are asked for beside each other, before the slot is known to be the sequence's own
+    const int mine = P.slot ? P.slot[s] : s;
     const SeqRange r = seq_range(P.start, s, P.n_tok);
     if (r.n <= 0 || r.n > most) {
         if (r.n < 0 && threadIdx.x == 0) bad_sequence();
         return;
     }
-    const int slot = gdn_slot_of(P, s);
-    if (slot < 0) {
-        if (threadIdx.x == 0) bad_sequence();
-        return;
-    }
-    float *Sg = P.state + ((size_t)slot * P.n_v_heads + vh) * P.K * P.V + j;
+    const bool there = mine >= 0 && mine < P.n_slots;
+    float *Sg = P.state + ((size_t)(there ? mine : 0) * P.n_v_heads + vh) * P.K * P.V + j;
     float col[GDN_RPW];
 #pragma unroll
     for (int i = 0; i < GDN_RPW; ++i) {
         const int row = warp + GDN_WARPS * i;
-        col[i] = row < P.K ? Sg[(size_t)row * P.V] : 0.0f;
+        col[i] = there && row < P.K ? Sg[(size_t)row * P.V] : 0.0f;
+    }
+    // a token's scalars and this thread's values of k or q (K <= 128: threads 0 .. 127 have k, the others q)
+    const int kq_at = threadIdx.x & (GDN_KMAX - 1);
+    const float *kq_src = threadIdx.x < GDN_KMAX ? P.k : P.q;
+    float b, vj, gt, kq;
+    auto fetch = [&](int t) {
+        const size_t tok = (size_t)(r.begin + t);
+        b = P.beta[tok * P.n_v_heads + vh];
+        vj = P.v[(tok * P.n_v_heads + vh) * P.V + j];
+        gt = P.g[tok * P.n_v_heads + vh];
+        kq = kq_at < P.K ? kq_src[(tok * P.n_k_heads + kh) * P.K + kq_at] : 0.0f;
+    };
+    fetch(0);
+    if (gdn_slot_of(P, s) < 0) {
+        if (threadIdx.x == 0) bad_sequence();
+        return;
     }
     for (int t = 0; t < r.n; ++t) {
         const int b2 = t & 1;
         const size_t tok = (size_t)(r.begin + t);
-        const float b = P.beta[tok * P.n_v_heads + vh], vj = P.v[(tok * P.n_v_heads + vh) * P.V + j], decay = expf(P.g[tok * P.n_v_heads + vh]);
-        for (int i = threadIdx.x; i < P.K; i += blockDim.x) {
-            ks[b2][i] = P.k[(tok * P.n_k_heads + kh) * P.K + i];
-            qs[b2][i] = P.q[(tok * P.n_k_heads + kh) * P.K + i];
-        }
+        const float beta = b, value = vj, decay = expf(gt);
+        (threadIdx.x < GDN_KMAX ? ks : qs)[b2][kq_at] = kq;
+        if (t + 1 < r.n) fetch(t + 1);                      // the next token's are on their way
         __syncthreads();
         float kv = 0.0f;
 #pragma unroll
@@ -79,13 +91,13 @@ __global__ void __launch_bounds__(GDN_WARPS * 32) gdn_seqs_step_kernel(const __g
         kv = 0.0f;
 #pragma unroll
         for (int w = 0; w < GDN_WARPS; ++w) kv = __fadd_rn(kv, part[0][w][lane]);
-        const float d = __fsub_rn(vj, kv);
+        const float d = __fsub_rn(value, kv);
         float o = 0.0f;
 #pragma unroll
         for (int i = 0; i < GDN_RPW; ++i) {
             const int row = warp + GDN_WARPS * i;
             if (row < P.K) {
-                col[i] = __fadd_rn(col[i], __fmul_rn(__fmul_rn(b, ks[b2][row]), d));
+                col[i] = __fadd_rn(col[i], __fmul_rn(__fmul_rn(beta, ks[b2][row]), d));
                 o = __fadd_rn(o, __fmul_rn(qs[b2][row], col[i]));
             }
         }

@@ -132,7 +132,16 @@ struct PageAttn {
     float2 *part_ml;            // [splits][token * n_head + head]: maximum, sum of weights
     int layer, n_head, group, pages_per_split, splits;
     float scale;
+    // the call's long sequences on the tensor cores (pages_tc.cuh): images [sequence][page][kv head], whether a CTA is to be done again [tile][kv head][split]
+    uint8_t *images;
+    int *redo;
+    int max_pages, n_tc;        // pages of a sequence that there are images for, 0: none; sequences
 };
+constexpr int PTC_ROWS = 128;
+// Whether a sequence is on the tensor cores.
+__device__ __forceinline__ bool pages_on_tc(const PageAttn &P, int n, int len) {
+    return n > 0 && (int64_t)n * P.group >= PTC_ROWS && len >= 0 && len <= (int64_t)P.max_pages * PG_POS && len <= (int64_t)P.C.table_stride * PG_POS;
+}
 
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
     float2 d;
@@ -167,8 +176,8 @@ __device__ __forceinline__ void pga_halves(uint32_t a, uint32_t b, uint32_t (&ou
     }
 }
 
-// grid (row tiles of all sequences and some that find none, kv heads, splits)
-template <int ROWT>
+// grid (row tiles of all sequences and some that find none, kv heads, splits).  BEHIND: behind pages_tc_kernel, two CTAs for each of its tiles: what it leaves.
+template <int ROWT, bool BEHIND = false>
 __global__ void __launch_bounds__(PGA_THREADS, 2) pages_attn_kernel(const __grid_constant__ PageAttn P) {
     constexpr int KEYW = PGA_WARPS / ROWT;              // warps that share the scores of 16 rows
     constexpr int KEYS = PG_POS / KEYW, NT = KEYS / 8, ROWS = 16 * ROWT;
@@ -198,8 +207,9 @@ __global__ void __launch_bounds__(PGA_THREADS, 2) pages_attn_kernel(const __grid
     pdl_wait_prior_grid();
     pdl_launch_dependents();
     // whose rows: the sequences' tiles one after the other, every warp for itself
+    constexpr int UNIT = BEHIND ? PTC_ROWS : ROWS;
     int seq, tile;
-    if (!seq_of_item(C.start, C.n_seq, C.n_tok, (int)blockIdx.x, lane, [&](int n) { return ((int64_t)n * P.group + ROWS - 1) / ROWS; }, seq, tile)) return;        // CTA-uniform
+    if (!seq_of_item(C.start, C.n_seq, C.n_tok, BEHIND ? (int)(blockIdx.x / 2) : (int)blockIdx.x, lane, [&](int n) { return ((int64_t)n * P.group + UNIT - 1) / UNIT; }, seq, tile)) return;        // CTA-uniform
     const SeqRange range = seq_range(C.start, seq, C.n_tok);
     const int page0 = split * P.pages_per_split;
     const int32_t *table = C.table + (size_t)seq * C.table_stride;
@@ -208,6 +218,12 @@ __global__ void __launch_bounds__(PGA_THREADS, 2) pages_attn_kernel(const __grid
     if (len < 0 || len > (int64_t)C.table_stride * PG_POS) {
         if (tid == 0) bad_sequence();
         return;
+    }
+    if (BEHIND) {
+        static_assert(!BEHIND || 2 * ROWS == PTC_ROWS, "");
+        if (pages_on_tc(P, range.n, len) && !P.redo[((size_t)(blockIdx.x / 2) * C.n_head_kv + kvh) * P.splits + split]) return;
+        tile = 2 * tile + (int)(blockIdx.x & 1);
+        if (tile * ROWS >= range.n * P.group) return;
     }
     const int n_rows = min(ROWS, range.n * P.group - tile * ROWS);                      // of this tile
     const int first_tok = tile * ROWS / P.group, last_tok = (tile * ROWS + n_rows - 1) / P.group;

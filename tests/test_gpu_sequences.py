@@ -297,7 +297,7 @@ def test_nothing_hidden_reaches_a_row(gpu):
     for new in (3, 150):
         c = Cache(gpu, [230], [new], seed=8)
         q = torch.randn(c.n_tok, 24, 256, generator=torch.Generator(device="cuda").manual_seed(8), device="cuda")
-        clean = run_attention(gpu, c, q)
+        clean, (want, size) = run_attention(gpu, c, q), attention(c, q)
         for what in (np.float16(np.inf), np.float16(np.nan)):
             pool = c.pool.copy()
             bad = np.frombuffer(what.tobytes(), np.uint8)
@@ -308,8 +308,12 @@ def test_nothing_hidden_reaches_a_row(gpu):
                 pool[c.table[0, p // 64], 0, :, :, p % 64, :, :2] = bad
             c.d_pool.copy_(torch.from_numpy(pool))
             out = run_attention(gpu, c, q)
-            assert torch.equal(out[:-1], clean[:-1])
-            assert bool((~out[-1, :12].isfinite()).all()) and torch.equal(out[-1, 12:], clean[-1, 12:])
+            if new == 3:
+                assert torch.equal(out[:-1], clean[:-1]) and torch.equal(out[-1, 12:], clean[-1, 12:])
+            # (of many tokens what the tensor cores' planes cannot hold goes to the other kernel, tile by tile: other bits, the same bound)
+            close(out[:-1], want[:-1], size[:-1], 4)
+            close(out[-1, 12:], want[-1, 12:], size[-1, 12:], 4)
+            assert bool((~out[-1, :12].isfinite()).all())
 
 
 def test_tokens_without_a_position_see_nothing(gpu):
