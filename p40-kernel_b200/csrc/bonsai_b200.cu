@@ -1916,40 +1916,41 @@ int check_pages(const bonsai_b200_pages *p, int layer, PageCache *C) {
     return 0;
 }
 
-// How pages_attn divides a call: 16 rowt rows a CTA, a span of pages a CTA, CTAs per kv head.  tc: sequences that may be on the tensor cores (0: none).
+// How pages_attn divides a call.  Sequences that may be on the tensor cores (tc of them at most, 0: none; pages_on_tc): tiles of 128 rows, a span of pages a CTA.  The others: rows
+// a tile; the spans are the device's to find, up to most_splits a tile.
 struct PagesPlan {
-    int rowt, pages_per_split, splits, max_pages;
+    int rowt, rows, most_splits, span, splits, max_pages;
     int64_t tiles, tc;
     int64_t part_bytes, image_bytes, redo_bytes;
     int64_t bytes() const { return part_bytes + image_bytes + redo_bytes; }
 };
 constexpr int64_t PTC_IMAGE_LIMIT = int64_t(5) << 29;            // 2.5 GB: a full context of the 27B model
+constexpr int PGA_SLOTS = 2 * SM_COUNT;
 PagesPlan plan_pages(int n_tok, int max_len, int n_seq, int n_head, int n_head_kv) {
     PagesPlan p = {};
-    const int64_t rows = (int64_t)n_tok * (n_head / n_head_kv), each = (rows + n_seq - 1) / n_seq, pages = std::max(1, (int)(((int64_t)max_len + PG_POS - 1) / PG_POS));
+    const int group = n_head / n_head_kv;
+    const int64_t rows = (int64_t)n_tok * group, each = (rows + n_seq - 1) / n_seq, pages = std::max(1, (int)(((int64_t)max_len + PG_POS - 1) / PG_POS));
     p.max_pages = (int)pages;
     p.tc = std::min<int64_t>(n_seq, rows / PTC_ROWS);
     if (rows < 2 * PTC_ROWS || p.tc * pages * n_head_kv > PTC_IMAGE_LIMIT / ATC_IMG_BYTES) p.tc = 0;
-    p.rowt = p.tc || each > 32 ? 4 : each > 16 ? 2 : 1;
-    const int64_t high = p.tc ? PTC_ROWS : 16 * p.rowt;
-    p.tiles = (rows + (int64_t)std::min(n_seq, n_tok) * (high - 1)) / high;
-    const int64_t items = std::max<int64_t>(1, (rows + high - 1) / high) * n_head_kv;
+    p.rowt = p.tc ? (group <= 8 ? 0 : 1) : each > 32 ? 4 : each > 16 ? 2 : each > 8 ? 1 : 0;
+    p.rows = p.rowt ? 16 * p.rowt : 8;
+    p.span = (int)pages;
     if (p.tc) {
         // spans that fill the last round of CTAs, one per SM; a CTA's start and its share of the join are worth four pages
+        p.tiles = (rows + (int64_t)std::min(n_seq, n_tok) * (PTC_ROWS - 1)) / PTC_ROWS;
+        const int64_t items = (rows + PTC_ROWS - 1) / PTC_ROWS * n_head_kv;
         int64_t best = INT64_MAX;
         for (int64_t s = 1; s <= std::min<int64_t>(pages, 16); ++s) {
             const int64_t span = (pages + s - 1) / s, cost = ((items * s + SM_COUNT - 1) / SM_COUNT) * (span + 4);
-            if (cost < best) best = cost, p.pages_per_split = (int)span;
+            if (cost < best) best = cost, p.span = (int)span;
         }
-    } else {
-        // A span of pages for each of the CTAs that are resident at once.  Of several sequences the longest is known only: they are taken to hold 3 / 8 of that.
-        const int64_t load = n_seq > 1 ? items * pages * 3 / 8 : items * pages;
-        const int64_t want = std::max<int64_t>(2, (load + 2 * SM_COUNT - 1) / (2 * SM_COUNT));
-        p.pages_per_split = (int)std::min(want, pages);
     }
-    p.splits = (int)((pages + p.pages_per_split - 1) / p.pages_per_split);
-    p.part_bytes = p.splits == 1 ? 0 : (int64_t)p.splits * n_tok * n_head * (KV_D + 2) * (int64_t)sizeof(float);
-    p.part_bytes = (p.part_bytes + 15) / 16 * 16;
+    p.splits = (int)((pages + p.span - 1) / p.span);
+    // beside prompts every split has room for all of their rows, so it is few
+    p.most_splits = (int)std::min<int64_t>((pages + 1) / 2, p.tc ? 8 : (PGA_SLOTS + n_head_kv - 1) / n_head_kv);
+    const int64_t splits = std::max(p.splits, p.most_splits), part = splits == 1 ? 0 : splits * n_tok * n_head * (KV_D + 2) * (int64_t)sizeof(float);
+    p.part_bytes = (part + 15) / 16 * 16;
     p.image_bytes = p.tc * pages * n_head_kv * ATC_IMG_BYTES;
     p.redo_bytes = p.tc ? (p.tiles * n_head_kv * p.splits * (int64_t)sizeof(int) + 15) / 16 * 16 : 0;
     return p;
@@ -2010,49 +2011,59 @@ int bonsai_b200_pages_attn(const bonsai_b200_pages *pages, int layer, const floa
     max_len = std::max(1, max_len);
     if (!q || !out || !aligned4(q) || !aligned4(out) || !pages_attn_sizes(C.n_tok, max_len, C.n_seq, n_head, C.n_head_kv)) return 1;
     const PagesPlan plan = plan_pages(C.n_tok, max_len, C.n_seq, n_head, C.n_head_kv);
-    if (plan.tiles > INT32_MAX || plan.splits > 65535) return 1;
+    if (2 * plan.tiles > INT32_MAX || plan.tc * plan.max_pages > INT32_MAX) return 1;
+    if (((int64_t)C.n_tok * (n_head / C.n_head_kv) / plan.rows + C.n_seq) * plan.most_splits * C.n_head_kv > INT32_MAX) return 1;
     P.q = q;
     P.out = out;
     P.layer = layer;
     P.n_head = n_head;
     P.group = n_head / C.n_head_kv;
-    P.pages_per_split = plan.pages_per_split;
+    P.span = plan.span;
     P.splits = plan.splits;
+    P.row_shift = 0;
+    while (1 << P.row_shift < plan.rows) ++P.row_shift;
+    P.most_splits = plan.most_splits;
     P.scale = scale;
     if (plan.bytes()) {
         if (!workspace || !aligned16(workspace) || workspace_bytes < plan.bytes()) return 1;
         uint8_t *w = static_cast<uint8_t *>(workspace);
         P.images = w;
         P.redo = reinterpret_cast<int *>(w + plan.image_bytes);
-        P.part_acc = reinterpret_cast<float *>(w + plan.image_bytes + plan.redo_bytes);
-        P.part_ml = reinterpret_cast<float2 *>(P.part_acc + (int64_t)plan.splits * C.n_tok * n_head * KV_D);
+        if (plan.part_bytes) {
+            P.part_acc = reinterpret_cast<float *>(w + plan.image_bytes + plan.redo_bytes);
+            P.part_ml = reinterpret_cast<float2 *>(P.part_acc + (int64_t)std::max(plan.splits, plan.most_splits) * C.n_tok * n_head * KV_D);
+        }
     }
     const cudaStream_t st = as_stream(stream);
-    static SmemOptIn opt[5];
-    auto run = [&](auto kernel, SmemOptIn &o, int64_t tiles, int threads, int smem) {
+    static SmemOptIn opt[6];
+    auto run = [&](auto kernel, SmemOptIn &o, dim3 grid, int threads, int smem) {
         const cudaError_t e = o.ensure(kernel);
-        if (e != cudaSuccess) return e;
-        return launch(kernel, dim3((unsigned)tiles, (unsigned)C.n_head_kv, (unsigned)plan.splits), dim3((unsigned)threads), (size_t)smem, st, true, P);
+        return e == cudaSuccess ? launch(kernel, grid, dim3((unsigned)threads), (size_t)smem, st, true, P) : e;
     };
-    const int smem = pga_smem_bytes(plan.rowt);
-    cudaError_t e;
+    cudaError_t e = cudaSuccess;
     if (plan.tc) {
-        if (2 * plan.tiles > INT32_MAX || plan.tc * plan.max_pages > INT32_MAX) return 1;
         P.max_pages = plan.max_pages;
         P.n_tc = (int)plan.tc;
-        e = launch(pages_planes_kernel, dim3((unsigned)(plan.tc * plan.max_pages), (unsigned)C.n_head_kv, 2), dim3(ATC_PREP_THREADS), 0, st, true, P);
-        if (e == cudaSuccess) e = run(pages_tc_kernel, opt[3], plan.tiles, ATC_THREADS, ATC_SMEM_BYTES);
-        if (e == cudaSuccess) e = run(pages_attn_kernel<4, true>, opt[4], 2 * plan.tiles, PGA_THREADS, smem);
-    } else {
-        e = plan.rowt == 1   ? run(pages_attn_kernel<1>, opt[0], plan.tiles, PGA_THREADS, smem)
-            : plan.rowt == 2 ? run(pages_attn_kernel<2>, opt[1], plan.tiles, PGA_THREADS, smem)
-                             : run(pages_attn_kernel<4>, opt[2], plan.tiles, PGA_THREADS, smem);
     }
-    if (e == cudaSuccess && plan.splits > 1) {
-        const int roww = plan.splits >= 24 ? 8 : plan.splits >= 6 ? 2 : 1;
+    {
+        const dim3 grid(PGA_SLOTS);
+        const int smem = pga_smem_bytes(plan.rowt), threads = 32 * pga_warps(plan.rowt);
+        e = plan.rowt == 0   ? run(pages_attn_kernel<0>, opt[0], grid, threads, smem)
+            : plan.rowt == 1 ? run(pages_attn_kernel<1>, opt[1], grid, threads, smem)
+            : plan.rowt == 2 ? run(pages_attn_kernel<2>, opt[2], grid, threads, smem)
+                             : run(pages_attn_kernel<4>, opt[3], grid, threads, smem);
+    }
+    if (plan.tc) {
+        const unsigned heads = (unsigned)C.n_head_kv, splits = (unsigned)plan.splits;
+        if (e == cudaSuccess) e = launch(pages_planes_kernel, dim3((unsigned)(plan.tc * plan.max_pages), heads, 2), dim3(ATC_PREP_THREADS), 0, st, true, P);
+        if (e == cudaSuccess) e = run(pages_tc_kernel, opt[4], dim3((unsigned)plan.tiles, heads, splits), ATC_THREADS, ATC_SMEM_BYTES);
+        if (e == cudaSuccess) e = run(pages_redo_kernel, opt[5], dim3(2 * (unsigned)plan.tiles, heads, splits), 32 * pga_warps(4), pga_smem_bytes(4));
+    }
+    if (e == cudaSuccess && P.part_acc) {
+        const int roww = plan.tc ? 1 : plan.most_splits >= 24 ? 8 : plan.most_splits >= 6 ? 2 : 1;
         const int64_t ctas = ((int64_t)C.n_tok * n_head * roww + PGJ_WARPS - 1) / PGJ_WARPS;
         if (ctas > INT32_MAX) return 1;
-        auto join = [&](auto kernel) { return launch(kernel, dim3((unsigned)ctas), dim3(32 * PGJ_WARPS), 0, as_stream(stream), true, P); };
+        auto join = [&](auto kernel) { return launch(kernel, dim3((unsigned)ctas), dim3(32 * PGJ_WARPS), 0, st, true, P, PGA_SLOTS); };
         e = roww == 8 ? join(pages_join_kernel<8>) : roww == 2 ? join(pages_join_kernel<2>) : join(pages_join_kernel<1>);
     }
     return (int)e;

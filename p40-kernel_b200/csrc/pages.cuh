@@ -107,21 +107,23 @@ __global__ void __launch_bounds__(PG_COPY_THREADS) pages_copy_kernel(const __gri
 //   score    scale * sum over the blocks of dq dk (q8 . k8)              int8 products on mma.sync (m16n8k32), int32 sums, scaled per block in fp32
 //   output   sum of p dv v8 / sum of p, p = e^(score - maximum)          p dv in two fp16 planes, v8 as fp16 (exact), fp32 sums
 //
-// Rows: a token's query heads that share a kv head are rows of one matrix: row r of a sequence is head r % group of new token r / group.  A CTA is four warps and
-// takes 16 ROWT rows of one kv head and one span of the sequence's pages, a page at a time:
+// Rows: a token's query heads that share a kv head are rows of one matrix: row r of a sequence is head r % group of new token r / group.  A CTA
+// takes 16 ROWT rows (ROWT = 0: 8) of one kv head and one span of the sequence's pages, a page at a time:
 //   scales   the page's fp16 scales as floats, the V ones of a block under a power of two of their own
-//   scores   a warp has 16 rows and all 64 positions (ROWT = 4), half of them (2) or a quarter (1); weights in fp32 to shared memory
-//   outputs  a warp has all rows and 64 dims (two blocks): V's bytes become fp16 once for all rows.  A page's sums are fresh ones, added to the fp32 output by rounded
-//            operations (the tensor core cuts the last bits of a sum off)
+//   scores   a warp has 16 rows and 8, 16 or all 64 positions (ROWT up to 1, 2, 4); weights in fp32 to shared memory
+//   outputs  a warp has all rows and 32 dims, a block (ROWT = 4: 64 dims); eight rows' high and low planes are the 16 rows of one product: V's bytes become fp16 once for all rows.  A page's sums are fresh ones, added to the fp32 output by
+//            rounded operations (the tensor core cuts the last bits of a sum off)
 // K and V rows come by one bulk copy each for a page; a page's room is given to the next but one when every warp has left it.
-constexpr int PGA_WARPS = 4, PGA_THREADS = 32 * PGA_WARPS, PGA_BUFS = 2;
+// Few rows have eight warps: what bounds them is a page's chain of latencies, which is half as long for a warp with one block of dims.
+constexpr int PGA_BUFS = 2;
+constexpr int pga_warps(int rowt) { return rowt == 4 ? 4 : 8; }       // (ROWT = 0: eight rows)
 constexpr int PGA_Q_STRIDE = 64 + 4;                            // words of a quantised row: 4 g + t are 32 different banks
 constexpr int PGA_W_STRIDE = PG_POS + 8;                        // weights of a row: pairs at 8 g + 2 t, of four rows, are 32 different banks
 constexpr int PGA_RING_BYTES = PGA_BUFS * 2 * PG_HEAD_BYTES;
 static_assert(64 * KV_D * 4 <= PGA_RING_BYTES, "the outputs reuse the ring");
 constexpr int pga_smem_bytes(int rowt) {
-    const int rows = 16 * rowt, keyw = PGA_WARPS / rowt;
-    return 128 + PGA_RING_BYTES + 3 * 8 * PG_POS * 4 + 16 * 4 + rows * (PGA_Q_STRIDE + 8 + PGA_W_STRIDE) * 4 + rows * (2 + 2 * keyw) * 4;
+    const int rows = rowt ? 16 * rowt : 8, keyw = pga_warps(rowt) / (rowt ? rowt : 1), q_rows = rowt ? rows : 16;
+    return 128 + PGA_RING_BYTES + 3 * 8 * PG_POS * 4 + 16 * 4 + q_rows * (PGA_Q_STRIDE + 8) * 4 + rows * PGA_W_STRIDE * 4 + rows * (2 + 2 * keyw) * 4;
 }
 
 struct PageAttn {
@@ -130,7 +132,9 @@ struct PageAttn {
     float *out;
     float *part_acc;            // [splits][token * n_head + head][256], with more than one split
     float2 *part_ml;            // [splits][token * n_head + head]: maximum, sum of weights
-    int layer, n_head, group, pages_per_split, splits;
+    int layer, n_head, group;
+    int span, splits;           // of the sequences on the tensor cores: pages of a CTA, CTAs of a tile
+    int row_shift, most_splits; // of the others: rows of a tile, as a power of two, CTAs of a tile at most
     float scale;
     // the call's long sequences on the tensor cores (pages_tc.cuh): images [sequence][page][kv head], whether a CTA is to be done again [tile][kv head][split]
     uint8_t *images;
@@ -140,7 +144,7 @@ struct PageAttn {
 constexpr int PTC_ROWS = 128;
 // Whether a sequence is on the tensor cores.
 __device__ __forceinline__ bool pages_on_tc(const PageAttn &P, int n, int len) {
-    return n > 0 && (int64_t)n * P.group >= PTC_ROWS && len >= 0 && len <= (int64_t)P.max_pages * PG_POS && len <= (int64_t)P.C.table_stride * PG_POS;
+    return P.max_pages > 0 && n > 0 && (int64_t)n * P.group >= PTC_ROWS && len >= 0 && len <= (int64_t)P.max_pages * PG_POS && len <= (int64_t)P.C.table_stride * PG_POS;
 }
 
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
@@ -176,12 +180,53 @@ __device__ __forceinline__ void pga_halves(uint32_t a, uint32_t b, uint32_t (&ou
     }
 }
 
-// grid (row tiles of all sequences and some that find none, kv heads, splits).  BEHIND: behind pages_tc_kernel, two CTAs for each of its tiles: what it leaves.
-template <int ROWT, bool BEHIND = false>
-__global__ void __launch_bounds__(PGA_THREADS, 2) pages_attn_kernel(const __grid_constant__ PageAttn P) {
-    constexpr int KEYW = PGA_WARPS / ROWT;              // warps that share the scores of 16 rows
-    constexpr int KEYS = PG_POS / KEYW, NT = KEYS / 8, ROWS = 16 * ROWT;
-    extern __shared__ __align__(128) uint8_t smem[];
+// ---- how the sequences with few rows are divided: by what they hold, which the device knows.  Every CTA finds the same.
+struct SeqWork { int tiles, pages; };       // no tiles: not one of them
+__device__ __forceinline__ SeqWork pages_work(const PageAttn &P, int s) {
+    if (s >= P.C.n_seq) return {0, 0};
+    const int n = seq_range(P.C.start, s, P.C.n_tok).n, len = P.C.len[s];
+    if (n <= 0 || pages_on_tc(P, n, len)) return {0, 0};
+    if (len < 0 || len > (int64_t)P.C.table_stride * PG_POS) return {1, 0};                 // one CTA says so
+    return {(n * P.group + (1 << P.row_shift) - 1) >> P.row_shift, (len + PG_POS - 1) / PG_POS};
+}
+__device__ __forceinline__ int pages_splits(const PageAttn &P, int pages, int span) { return max(1, min(P.most_splits, (pages + span - 1) / span)); }
+// Pages of a CTA such that one round of CTAs (two per SM) takes all of them.
+__device__ __noinline__ int pages_span(const PageAttn &P, int lane, int slots) {
+    int64_t total = 0;
+    for (int base = 0; base < P.C.n_seq; base += 32) {
+        const SeqWork w = pages_work(P, base + lane);
+        total += (int64_t)w.tiles * w.pages;
+    }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    int span = (int)max((int64_t)2, min((int64_t)(1 << 20), (total * P.C.n_head_kv + slots - 1) / slots));
+    if (P.C.n_seq > 128) return span;
+    for (int step = 0; step < 8; ++step) {              // (a sequence's last CTA has less: some more pages for each, until they fit)
+        int items = 0;
+        for (int base = 0; base < P.C.n_seq; base += 32) {
+            const SeqWork w = pages_work(P, base + lane);
+            items += w.tiles ? w.tiles * pages_splits(P, w.pages, span) : 0;
+        }
+        items = __reduce_add_sync(0xffffffffu, items);
+        if ((int64_t)items * P.C.n_head_kv <= slots) break;
+        span += max(1, span / 8);
+    }
+    return span;
+}
+
+// One item: rows `tile` of a sequence, one kv head, pages page0 .. page1 - 1 of those that the tile sees.
+template <int ROWT>
+struct PageItem {
+    int seq, tile, kvh, split, page0, page1;            // page1 < 0: to the last
+};
+
+template <int ROWT>
+__device__ __forceinline__ bool pages_attn_item(const PageAttn &P, const PageItem<ROWT> &I, uint8_t *smem, int &turn) {
+    constexpr int WARPS = pga_warps(ROWT), THREADS = 32 * WARPS, NB = 8 / WARPS;          // NB: blocks of dims of a warp
+    constexpr bool EIGHT = ROWT == 0;
+    constexpr int MT = EIGHT ? 1 : ROWT, HR = EIGHT ? 1 : 2;              // row tiles; rows of a thread in each
+    constexpr int KEYW = WARPS / MT;                    // warps that share the scores of a row tile
+    constexpr int KEYS = PG_POS / KEYW, NT = KEYS / 8, ROWS = EIGHT ? 8 : 16 * ROWT, QROWS = EIGHT ? 16 : ROWS;
     uint64_t *kfull = reinterpret_cast<uint64_t *>(smem), *vfull = kfull + PGA_BUFS;
     int *held = reinterpret_cast<int *>(vfull + PGA_BUFS);                       // [PGA_BUFS] positions of the page that there are
     int *wide0 = held + PGA_BUFS;                                                // [2][8] the block's scales of V are too far apart for one pair of planes
@@ -189,54 +234,37 @@ __global__ void __launch_bounds__(PGA_THREADS, 2) pages_attn_kernel(const __grid
     float *ks = reinterpret_cast<float *>(ring + PGA_RING_BYTES);                // [8 blocks][64 positions]
     float *vs0 = ks + 8 * PG_POS;                                                // the same of V times 2^(13 - e), e the exponent of the block's largest; pages alternate
     float *vfac0 = vs0 + 2 * 8 * PG_POS;                                         // [2][8] 2^(e - 13), negative: the block is to be looked at closely
-    uint32_t *q8 = reinterpret_cast<uint32_t *>(vfac0 + 16);                     // [ROWS][PGA_Q_STRIDE]
-    float *qd = reinterpret_cast<float *>(q8 + ROWS * PGA_Q_STRIDE);             // [ROWS][8] scales of the queries, times the softmax scale
-    float *wt = qd + ROWS * 8;                                                   // [ROWS][PGA_W_STRIDE] weights
+    uint32_t *q8 = reinterpret_cast<uint32_t *>(vfac0 + 16);                     // [QROWS][PGA_Q_STRIDE]
+    float *qd = reinterpret_cast<float *>(q8 + QROWS * PGA_Q_STRIDE);            // [QROWS][8] scales of the queries, times the softmax scale
+    float *wt = qd + QROWS * 8;                                                  // [ROWS][PGA_W_STRIDE] weights
     float *alphas = wt + ROWS * PGA_W_STRIDE, *sums = alphas + ROWS;             // [ROWS] each: e^(old maximum - new), sum of weights
     float *most = sums + ROWS, *part = most + KEYW * ROWS;                       // [KEYW][ROWS] each: a warp's maxima, its sums
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t = lane & 3;
     const int rt = warp / KEYW, kw = warp % KEYW;
-    const int kvh = blockIdx.y, split = blockIdx.z;
+    const int seq = I.seq, tile = I.tile, kvh = I.kvh, split = I.split;
     const PageCache &C = P.C;
-    if (tid == 0) {
-        for (int b = 0; b < PGA_BUFS; ++b) mbar_init(&kfull[b], 1), mbar_init(&vfull[b], 1);
-        mbar_fence_init();
-    }
-    pdl_wait_prior_grid();
-    pdl_launch_dependents();
-    // whose rows: the sequences' tiles one after the other, every warp for itself
-    constexpr int UNIT = BEHIND ? PTC_ROWS : ROWS;
-    int seq, tile;
-    if (!seq_of_item(C.start, C.n_seq, C.n_tok, BEHIND ? (int)(blockIdx.x / 2) : (int)blockIdx.x, lane, [&](int n) { return ((int64_t)n * P.group + UNIT - 1) / UNIT; }, seq, tile)) return;        // CTA-uniform
     const SeqRange range = seq_range(C.start, seq, C.n_tok);
-    const int page0 = split * P.pages_per_split;
     const int32_t *table = C.table + (size_t)seq * C.table_stride;
-    const int ahead[2] = {page0 < C.table_stride ? table[page0] : -1, page0 + 1 < C.table_stride ? table[page0 + 1] : -1};       // asked for beside the length
+    const int ahead[2] = {I.page0 < C.table_stride ? table[I.page0] : -1, I.page0 + 1 < C.table_stride ? table[I.page0 + 1] : -1};         // asked for beside the length
     const int len = C.len[seq];
     if (len < 0 || len > (int64_t)C.table_stride * PG_POS) {
         if (tid == 0) bad_sequence();
-        return;
-    }
-    if (BEHIND) {
-        static_assert(!BEHIND || 2 * ROWS == PTC_ROWS, "");
-        if (pages_on_tc(P, range.n, len) && !P.redo[((size_t)(blockIdx.x / 2) * C.n_head_kv + kvh) * P.splits + split]) return;
-        tile = 2 * tile + (int)(blockIdx.x & 1);
-        if (tile * ROWS >= range.n * P.group) return;
+        return true;
     }
     const int n_rows = min(ROWS, range.n * P.group - tile * ROWS);                      // of this tile
     const int first_tok = tile * ROWS / P.group, last_tok = (tile * ROWS + n_rows - 1) / P.group;
     const int before = len - range.n;                                                   // positions in front of the new tokens
-    // positions that any row of the tile sees, in pages; this split's
+    // positions that any row of the tile sees, in pages; this item's
     const int seen = min(len, before + last_tok + 1);
     const int pages = (max(seen, 0) + PG_POS - 1) / PG_POS;
-    const int page1 = split == P.splits - 1 ? pages : min(page0 + P.pages_per_split, pages);          // (the last takes what is left)
+    const int page0 = I.page0, page1 = I.page1 < 0 ? pages : min(I.page1, pages);
     const int ntiles = page1 - page0;
-    if (ntiles <= 0 && split > 0) return;               // (the first split writes the rows that see nothing)
+    if (ntiles <= 0 && split > 0) return true;          // (the first split writes the rows that see nothing)
 
     auto issue = [&](int i) {                           // one thread
-        const int b = i % PGA_BUFS, page = i < 2 ? ahead[i] : table[page0 + i];
+        const int b = (turn + i) % PGA_BUFS, page = i < 2 ? ahead[i] : table[page0 + i];
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         if (page < 0 || page >= C.n_pages) {
             bad_sequence();
@@ -255,18 +283,21 @@ __global__ void __launch_bounds__(PGA_THREADS, 2) pages_attn_kernel(const __grid
         mbar_expect_tx(&vfull[b], bytes);
         bulk_g2s(dst + PG_HEAD_BYTES, page_rows(C, page, P.layer, 1, kvh), bytes, &vfull[b], pol);
     };
-    __syncthreads();
-    if (tid == 0)
+    if (tid == THREADS - 32)
         for (int i = 0; i < min(ntiles, PGA_BUFS); ++i) issue(i);
     // the rows' queries, quantised as the cache rows are
     {
         const int blk = lane >> 2, sub = lane & 3;
         const bool vec = (reinterpret_cast<uintptr_t>(P.q) & 15u) == 0;
 #pragma unroll 4
-        for (int r = warp; r < ROWS; r += PGA_WARPS) {
+        for (int r = warp; r < QROWS; r += WARPS) {
             float x[8];
             const int row = tile * ROWS + r, tok = row / P.group, h = row - tok * P.group;
             const float *qr = P.q + ((size_t)(range.begin + tok) * P.n_head + kvh * P.group + h) * KV_D + blk * 32 + sub * 8;
+            if (EIGHT && r >= ROWS) {                   // the products' other eight rows are zeros
+                *reinterpret_cast<uint2 *>(q8 + r * PGA_Q_STRIDE + blk * 8 + 2 * sub) = make_uint2(0u, 0u);
+                continue;
+            }
             if (r >= n_rows) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) x[i] = 0.0f;
@@ -291,28 +322,30 @@ __global__ void __launch_bounds__(PGA_THREADS, 2) pages_attn_kernel(const __grid
             if (sub == 0) qd[r * 8 + blk] = __fmul_rn(f16_bits_to_f32(f32_to_f16_bits_ties_away(d)), P.scale);
         }
     }
-    float acc[ROWT][2][4][4];                           // row tile, the warp's block, byte of the slot; (row g | g + 8, slot 2 t | 2 t + 1)
+    float acc[MT][NB][4][2 * HR];                       // row tile, the warp's block, byte of the slot; (row g | g + 8, slot 2 t | 2 t + 1)
 #pragma unroll
-    for (int m = 0; m < ROWT; ++m)
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[m][b][j][i] = 0.0f;
-    float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.0f, 0.0f};            // rows 16 rt + g, + 8; l of this thread's columns
+                for (int i = 0; i < 2 * HR; ++i) acc[m][b][j][i] = 0.0f;
+    float m_run[HR], l_run[HR];                         // rows 16 rt + g, + 8; l of this thread's columns
     // the last position that they see
-    int limit[2];
+    int limit[HR];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < HR; ++i) {
         const int r = 16 * rt + g + 8 * i;
+        m_run[i] = -INFINITY;
+        l_run[i] = 0.0f;
         limit[i] = r < n_rows ? before + (tile * ROWS + r) / P.group : -1;
     }
     const int all_see = before + first_tok;             // every row of the tile sees the positions up to this one
     bool ok = true;
     for (int i = 0; i < ntiles; ++i) {
-        const int b = i % PGA_BUFS, p0 = (page0 + i) * PG_POS;
-        const uint32_t par = (uint32_t)((i / PGA_BUFS) & 1);
+        const int b = (turn + i) % PGA_BUFS, p0 = (page0 + i) * PG_POS;
+        const uint32_t par = (uint32_t)(((turn + i) / PGA_BUFS) & 1);
         const uint8_t *kt = ring + (size_t)b * 2 * PG_HEAD_BYTES, *vt = kt + PG_HEAD_BYTES;
         float *vs = vs0 + (i & 1) * 8 * PG_POS, *vfac = vfac0 + (i & 1) * 8;
         ok = mbar_wait_hot(&kfull[b], par) && ok;
@@ -320,7 +353,7 @@ __global__ void __launch_bounds__(PGA_THREADS, 2) pages_attn_kernel(const __grid
         const int n = held[b];
         // ---- scales; those behind the last position are zeros
 #pragma unroll
-        for (int blk = 2 * warp; blk < 2 * warp + 2; ++blk) {                    // a warp's two blocks, lane = position
+        for (int blk = NB * warp; blk < NB * warp + NB; ++blk) {                 // a warp's blocks, lane = position
             const int off = 34 * blk;
             float x[2];
             uint32_t top = 0, low = 0x7FFFu;
@@ -351,24 +384,24 @@ __global__ void __launch_bounds__(PGA_THREADS, 2) pages_attn_kernel(const __grid
             }
         }
         if (!__syncthreads_and(ok ? 1 : 0)) break;      // (a wait ran out: the CTA leaves as a whole)
-        if (tid == 0 && i > 0 && i - 1 + PGA_BUFS < ntiles) issue(i - 1 + PGA_BUFS);      // every warp is behind the page before
+        if (tid == THREADS - 32 && i > 0 && i - 1 + PGA_BUFS < ntiles) issue(i - 1 + PGA_BUFS);      // every warp is behind the page before
         // ---- scores: rows 16 rt .., positions KEYS kw ..
-        float s[NT][4];
+        float s[NT][2 * HR];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[nt][e] = 0.0f;
+            for (int e = 0; e < 2 * HR; ++e) s[nt][e] = 0.0f;
         {
             const uint32_t *qa = q8 + (16 * rt + g) * PGA_Q_STRIDE + t;
             const float *qs = qd + (16 * rt + g) * 8, *kd = ks + KEYS * kw + 2 * t;
             const uint32_t *kr = reinterpret_cast<const uint32_t *>(kt) + (size_t)(KEYS * kw + g) * (KV_ROW / 4);
             const float2 low = make_float2(-12582912.0f, -12582912.0f);
-#pragma unroll 1
+#pragma unroll(ROWT >= 2 ? 1 : 2)
             for (int pair = 0; pair < 4; ++pair, qa += 16, qs += 2, kd += 2 * PG_POS, kr += 17) {
 #pragma unroll
                 for (int odd = 0; odd < 2; ++odd) {
                     const uint32_t a0 = qa[8 * odd], a1 = qa[8 * odd + 8 * PGA_Q_STRIDE], a2 = qa[8 * odd + 4], a3 = qa[8 * odd + 4 + 8 * PGA_Q_STRIDE];
-                    const float dq0 = qs[odd], dq1 = qs[64 + odd];
+                    const float dq0 = qs[odd], dq1 = EIGHT ? 0.0f : qs[64 + odd];
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         const uint32_t *u = kr + nt * 8 * (KV_ROW / 4);
@@ -385,10 +418,13 @@ __global__ void __launch_bounds__(PGA_THREADS, 2) pages_attn_kernel(const __grid
                         pga_mma_s8(d, a0, a1, a2, a3, b0, b1);
                         const float2 dk = *reinterpret_cast<const float2 *>(kd + odd * PG_POS + 8 * nt);
                         const float2 x0 = mul2(add2(make_float2(__int_as_float(d[0]), __int_as_float(d[1])), low), dk);
-                        const float2 x1 = mul2(add2(make_float2(__int_as_float(d[2]), __int_as_float(d[3])), low), dk);
                         const float2 y0 = fma2(x0, make_float2(dq0, dq0), make_float2(s[nt][0], s[nt][1]));
-                        const float2 y1 = fma2(x1, make_float2(dq1, dq1), make_float2(s[nt][2], s[nt][3]));
-                        s[nt][0] = y0.x; s[nt][1] = y0.y; s[nt][2] = y1.x; s[nt][3] = y1.y;
+                        s[nt][0] = y0.x; s[nt][1] = y0.y;
+                        if (!EIGHT) {
+                            const float2 x1 = mul2(add2(make_float2(__int_as_float(d[2]), __int_as_float(d[3])), low), dk);
+                            const float2 y1 = fma2(x1, make_float2(dq1, dq1), make_float2(s[nt][2 * HR - 2], s[nt][2 * HR - 1]));
+                            s[nt][2 * HR - 2] = y1.x; s[nt][2 * HR - 1] = y1.y;
+                        }
                     }
                 }
             }
@@ -398,14 +434,14 @@ __global__ void __launch_bounds__(PGA_THREADS, 2) pages_attn_kernel(const __grid
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
+                for (int e = 0; e < 2 * HR; ++e) {
                     const int k = KEYS * kw + 8 * nt + 2 * t + (e & 1);
                     if (p0 + k > limit[e >> 1] || k >= n) s[nt][e] = -INFINITY;
                 }
         }
-        float mx[2];
+        float mx[HR];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < HR; ++h) {
             mx[h] = s[0][2 * h];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) mx[h] = fmaxf(mx[h], fmaxf(s[nt][2 * h], s[nt][2 * h + 1]));
@@ -413,15 +449,17 @@ __global__ void __launch_bounds__(PGA_THREADS, 2) pages_attn_kernel(const __grid
             mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
         }
         if (KEYW > 1) {
-            if (t == 0) most[kw * ROWS + 16 * rt + g] = mx[0], most[kw * ROWS + 16 * rt + g + 8] = mx[1];
+            if (t == 0)
+#pragma unroll
+                for (int h = 0; h < HR; ++h) most[kw * ROWS + 16 * rt + g + 8 * h] = mx[h];
             __syncthreads();
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < HR; ++h)
 #pragma unroll
                 for (int w = 0; w < KEYW; ++w) mx[h] = fmaxf(mx[h], most[w * ROWS + 16 * rt + g + 8 * h]);
         }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < HR; ++h) {
             const int r = 16 * rt + g + 8 * h;
             const float m_new = fmaxf(m_run[h], mx[h]), base = m_new == -INFINITY ? 0.0f : m_new;
             const float alpha = expf(__fsub_rn(m_run[h], base));
@@ -437,15 +475,16 @@ __global__ void __launch_bounds__(PGA_THREADS, 2) pages_attn_kernel(const __grid
             if (kw == 0 && t == 0) alphas[r] = alpha;
         }
         __syncthreads();
-        // ---- outputs: blocks 2 warp, 2 warp + 1
-        const uint32_t *vr0 = reinterpret_cast<const uint32_t *>(vt) + (size_t)(2 * t) * (KV_ROW / 4) + 17 * warp;
+        // ---- outputs: blocks NB warp ..
+        const uint32_t *vr0 = reinterpret_cast<const uint32_t *>(vt) + (size_t)(2 * t) * (KV_ROW / 4) + 17 * (NB * warp / 2);
 #pragma unroll
-        for (int bl = 0; bl < 2; ++bl) {
-            const float *dv0 = vs + (2 * warp + bl) * PG_POS + 2 * t;
-            const float fac = vfac[2 * warp + bl];
-            float o[ROWT][4][4];
+        for (int bl = 0; bl < NB; ++bl) {
+            const bool second = NB == 2 ? bl : (warp & 1);                       // of a pair of blocks
+            const float *dv0 = vs + (NB * warp + bl) * PG_POS + 2 * t;
+            const float fac = vfac[NB * warp + bl];
+            float o[MT][4][4];                          // EIGHT: rows g of the high plane, rows g of the low one
 #pragma unroll
-            for (int m = 0; m < ROWT; ++m)
+            for (int m = 0; m < MT; ++m)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -453,14 +492,14 @@ __global__ void __launch_bounds__(PGA_THREADS, 2) pages_attn_kernel(const __grid
             // CAREFUL: a position without weight adds nothing, whatever it holds; REST: what one pair of planes leaves, times 2^24
             auto pass = [&](auto carefulc, auto restc) {
                 constexpr bool CAREFUL = decltype(carefulc)::value, REST = decltype(restc)::value;
-#pragma unroll 1
+#pragma unroll(CAREFUL || ROWT == 4 ? 1 : 2)
                 for (int k = 0; k < PG_POS / 16; ++k) {
                     uint32_t w[4], b0[4], b1[4];
                     const uint32_t *u = vr0 + (size_t)(16 * k) * (KV_ROW / 4);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const uint32_t *x = u + ((e & 1) + 8 * (e >> 1)) * (KV_ROW / 4);
-                        if (bl) {
+                        if (second) {
                             w[e] = x[9 + g];
                         } else {
                             w[e] = x[g];
@@ -471,10 +510,10 @@ __global__ void __launch_bounds__(PGA_THREADS, 2) pages_attn_kernel(const __grid
                     pga_halves(w[2], w[3], b1);
                     const float2 dv[2] = {*reinterpret_cast<const float2 *>(dv0 + 16 * k), *reinterpret_cast<const float2 *>(dv0 + 16 * k + 8)};
 #pragma unroll
-                    for (int m = 0; m < ROWT; ++m) {
+                    for (int m = 0; m < MT; ++m) {
                         uint32_t ah[4], al[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {   // rows g, g + 8 of positions 2 t, then of 2 t + 8
+                        for (int e = 0; e < 4; e += EIGHT ? 2 : 1) {             // rows g, g + 8 of positions 2 t, then of 2 t + 8
                             const float2 p = *reinterpret_cast<const float2 *>(wt + (16 * m + g + 8 * (e & 1)) * PGA_W_STRIDE + 16 * k + 8 * (e >> 1) + 2 * t);
                             float2 x = mul2(p, dv[e >> 1]);
                             if (CAREFUL) {
@@ -484,20 +523,25 @@ __global__ void __launch_bounds__(PGA_THREADS, 2) pages_attn_kernel(const __grid
                             split_f16x2(x.x, x.y, ah[e], al[e]);
                             if (REST) split_rest_f16x2(x.x, x.y, ah[e], al[e]);
                         }
+                        if (EIGHT) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) mma_f16_16816(o[m][j], al[0], al[1], al[2], al[3], b0[j], b1[j]);
+                            for (int j = 0; j < 4; ++j) mma_f16_16816(o[m][j], ah[0], al[0], ah[2], al[2], b0[j], b1[j]);
+                        } else {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) mma_f16_16816(o[m][j], ah[0], ah[1], ah[2], ah[3], b0[j], b1[j]);
+                            for (int j = 0; j < 4; ++j) mma_f16_16816(o[m][j], al[0], al[1], al[2], al[3], b0[j], b1[j]);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) mma_f16_16816(o[m][j], ah[0], ah[1], ah[2], ah[3], b0[j], b1[j]);
+                        }
                     }
                 }
             };
             if (fac > 0.0f) {
                 pass(std::false_type{}, std::false_type{});
             } else {
-                if (wide0[(i & 1) * 8 + 2 * warp + bl]) {
+                if (wide0[(i & 1) * 8 + NB * warp + bl]) {
                     pass(std::true_type{}, std::true_type{});
 #pragma unroll
-                    for (int m = 0; m < ROWT; ++m)
+                    for (int m = 0; m < MT; ++m)
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -506,34 +550,42 @@ __global__ void __launch_bounds__(PGA_THREADS, 2) pages_attn_kernel(const __grid
                 pass(std::true_type{}, std::false_type{});
             }
 #pragma unroll
-            for (int m = 0; m < ROWT; ++m) {
-                const float al[2] = {alphas[16 * m + g], alphas[16 * m + g + 8]};
+            for (int m = 0; m < MT; ++m) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                for (int h = 0; h < HR; ++h) {
+                    const float al = alphas[16 * m + g + 8 * h];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[m][bl][j][e] = __fmaf_rn(o[m][j][e], fabsf(fac), __fmul_rn(acc[m][bl][j][e], al[e >> 1]));
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float x = EIGHT ? __fadd_rn(o[m][j][e], o[m][j][2 + e]) : o[m][j][2 * h + e];
+                            acc[m][bl][j][2 * h + e] = __fmaf_rn(x, fabsf(fac), __fmul_rn(acc[m][bl][j][2 * h + e], al));
+                        }
+                }
             }
         }
     }
     // ---- the sums leave by whole lines
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < HR; ++h) {
         float l = __fadd_rn(l_run[h], __shfl_xor_sync(0xffffffffu, l_run[h], 1));
         l = __fadd_rn(l, __shfl_xor_sync(0xffffffffu, l, 2));
         if (t == 0) part[kw * ROWS + 16 * rt + g + 8 * h] = l, most[kw * ROWS + 16 * rt + g + 8 * h] = m_run[h];
     }
-    if (!__syncthreads_and(ok ? 1 : 0)) return;         // (and every warp has left the last page)
+    turn += max(ntiles, 0);
+    if (!__syncthreads_and(ok ? 1 : 0)) return false;   // (and every warp has left the last page)
 #pragma unroll
-    for (int m = 0; m < ROWT; ++m)
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int bl = 0; bl < 2; ++bl)
+        for (int bl = 0; bl < NB; ++bl)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float *dst = reinterpret_cast<float *>(ring) + (size_t)(16 * m + g + 8 * h) * KV_D + 32 * (2 * warp + bl);
+            for (int h = 0; h < HR; ++h) {
+                const bool second = NB == 2 ? bl : (warp & 1);
+                float *dst = reinterpret_cast<float *>(ring) + (size_t)(16 * m + g + 8 * h) * KV_D + 32 * (NB * warp + bl);
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {           // slot 2 t + c of the block: four values from dim 4 slot (odd block) or 4 slot - 2 (even, round the end)
                     const int slot = 2 * t + c;
-                    float *d0 = dst + (bl ? 4 * slot : (slot ? 4 * slot - 2 : 0)), *d1 = dst + (bl ? 4 * slot + 2 : (slot ? 4 * slot : 30));
+                    float *d0 = dst + (second ? 4 * slot : (slot ? 4 * slot - 2 : 0)), *d1 = dst + (second ? 4 * slot + 2 : (slot ? 4 * slot : 30));
                     *reinterpret_cast<float2 *>(d0) = make_float2(acc[m][bl][0][2 * h + c], acc[m][bl][1][2 * h + c]);
                     *reinterpret_cast<float2 *>(d1) = make_float2(acc[m][bl][2][2 * h + c], acc[m][bl][3][2 * h + c]);
                 }
@@ -545,13 +597,13 @@ __global__ void __launch_bounds__(PGA_THREADS, 2) pages_attn_kernel(const __grid
         sums[tid] = l;
     }
     __syncthreads();
-    for (int i = tid; i < n_rows * (KV_D / 4); i += PGA_THREADS) {
+    for (int i = tid; i < n_rows * (KV_D / 4); i += THREADS) {
         const int r = i / (KV_D / 4), c = i % (KV_D / 4);
         float4 x = reinterpret_cast<const float4 *>(ring)[(size_t)r * (KV_D / 4) + c];
         const float l = sums[r];
         const int row = tile * ROWS + r, tok = row / P.group;
         const size_t at = (size_t)(range.begin + tok) * P.n_head + kvh * P.group + (row - tok * P.group);
-        if (P.splits == 1) {
+        if (P.part_acc == nullptr) {                    // nobody has more than one split
             const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);             // a row that sees nothing is zeros
             x = make_float4(__fmul_rn(x.x, inv), __fmul_rn(x.y, inv), __fmul_rn(x.z, inv), __fmul_rn(x.w, inv));
             float *o = P.out + at * KV_D + 4 * c;
@@ -566,12 +618,88 @@ __global__ void __launch_bounds__(PGA_THREADS, 2) pages_attn_kernel(const __grid
             if (c == 0) P.part_ml[at2] = make_float2(most[r], l);
         }
     }
+    return true;
+}
+
+// The sequences with few rows (pages_on_tc has the others).  grid: two CTAs per SM, which take items until there are none.
+template <int ROWT>
+__global__ void __launch_bounds__(32 * pga_warps(ROWT), 2) pages_attn_kernel(const __grid_constant__ PageAttn P) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    uint64_t *kfull = reinterpret_cast<uint64_t *>(smem), *vfull = kfull + PGA_BUFS;
+    const int lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int b = 0; b < PGA_BUFS; ++b) mbar_init(&kfull[b], 1), mbar_init(&vfull[b], 1);
+        mbar_fence_init();
+    }
+    pdl_wait_prior_grid();
+    pdl_launch_dependents();
+    const int span = pages_span(P, lane, gridDim.x);
+    const int heads = P.C.n_head_kv;
+    __syncthreads();
+    int turn = 0;
+    for (int item = blockIdx.x;; item += gridDim.x) {
+        // whose: the sequences' items one after the other, every warp for itself (the host has seen that they are countable)
+        int before = 0;
+        PageItem<ROWT> I = {-1, 0, 0, 0, 0, 0};
+        for (int base = 0; base < P.C.n_seq && I.seq < 0; base += 32) {
+            const SeqWork w = pages_work(P, base + lane);
+            const int splits = pages_splits(P, w.pages, span), own = w.tiles * splits * heads;
+            int sum = own;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += x;
+            }
+            const unsigned past = __ballot_sync(0xffffffffu, before + sum > item);
+            if (past) {
+                const int at = __ffs(past) - 1, rest = item - before - __shfl_sync(0xffffffffu, sum - own, at), n = __shfl_sync(0xffffffffu, splits, at);
+                const int pair = rest / heads;
+                I.seq = base + at;
+                I.kvh = rest - pair * heads;
+                I.tile = pair / n;
+                I.split = pair - I.tile * n;
+                I.page0 = I.split * span;
+                I.page1 = I.split == n - 1 ? -1 : I.page0 + span;
+            }
+            before += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        if (I.seq < 0) return;                          // CTA-uniform
+        if (!pages_attn_item<ROWT>(P, I, smem, turn)) return;        // (a wait ran out: the CTA leaves as a whole)
+        __syncthreads();
+    }
+}
+
+// Behind pages_tc_kernel, two CTAs for each of its tiles: what it could not hold.
+__global__ void __launch_bounds__(32 * pga_warps(4), 2) pages_redo_kernel(const __grid_constant__ PageAttn P) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    uint64_t *kfull = reinterpret_cast<uint64_t *>(smem), *vfull = kfull + PGA_BUFS;
+    const int lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int b = 0; b < PGA_BUFS; ++b) mbar_init(&kfull[b], 1), mbar_init(&vfull[b], 1);
+        mbar_fence_init();
+    }
+    pdl_wait_prior_grid();
+    pdl_launch_dependents();
+    PageItem<4> I;
+    if (!seq_of_item(P.C.start, P.C.n_seq, P.C.n_tok, (int)(blockIdx.x / 2), lane, [&](int n) { return ((int64_t)n * P.group + PTC_ROWS - 1) / PTC_ROWS; }, I.seq, I.tile)) return;
+    const int n = seq_range(P.C.start, I.seq, P.C.n_tok).n;
+    if (!pages_on_tc(P, n, P.C.len[I.seq])) return;
+    if (!P.redo[((size_t)(blockIdx.x / 2) * P.C.n_head_kv + blockIdx.y) * P.splits + blockIdx.z]) return;
+    I.tile = 2 * I.tile + (int)(blockIdx.x & 1);
+    if (I.tile * (PTC_ROWS / 2) >= n * P.group) return;
+    I.kvh = blockIdx.y;
+    I.split = blockIdx.z;
+    I.page0 = I.split * P.span;
+    I.page1 = I.split == P.splits - 1 ? -1 : I.page0 + P.span;
+    __syncthreads();
+    int turn = 0;
+    pages_attn_item<4>(P, I, smem, turn);
 }
 
 // The splits of a row added up: ROWW warps per row (token, head), four dims and four more a lane.  A row's splits are those that its own positions reach.
 constexpr int PGJ_WARPS = 8;
 template <int ROWW>
-__global__ void __launch_bounds__(32 * PGJ_WARPS) pages_join_kernel(const __grid_constant__ PageAttn P) {
+__global__ void __launch_bounds__(32 * PGJ_WARPS) pages_join_kernel(const __grid_constant__ PageAttn P, int slots) {
     __shared__ float4 sums[PGJ_WARPS][2][32];
     __shared__ float2 ml[PGJ_WARPS];
     const PageCache &C = P.C;
@@ -588,7 +716,10 @@ __global__ void __launch_bounds__(32 * PGJ_WARPS) pages_join_kernel(const __grid
             const int len = C.len[s];
             if (r.n > 0 && tok >= r.begin && len >= 0 && len <= (int64_t)C.table_stride * PG_POS) {
                 const int seen = len - r.n + (tok - r.begin) + 1;
-                n = max(1, min(P.splits, ((max(seen, 0) + PG_POS - 1) / PG_POS + P.pages_per_split - 1) / P.pages_per_split));
+                const int pages = (max(seen, 0) + PG_POS - 1) / PG_POS;
+                const bool tc = pages_on_tc(P, r.n, len);
+                const int span = tc ? P.span : pages_span(P, lane, slots);
+                n = max(1, min(tc ? P.splits : pages_splits(P, (len + PG_POS - 1) / PG_POS, span), (pages + span - 1) / span));
             }
         }
     }

@@ -11,8 +11,8 @@
 //   threads       outputs of page i - 1 added, weights of page i to tensor memory | scores of page i + 1 read, softmax
 // Tensor memory, all 512 columns: 256 output, 64 scores, 64 weights, 128 q low.  Shared memory: q high, k and v images of one page, 64 KB each.
 //
-// What one plane pair cannot hold beside the largest value (atc_too_wide, of the CTA's rows and pages) is left to pages_attn_kernel, which comes behind and does the CTAs that
-// said so, and the sequences with few new tokens.
+// What one plane pair cannot hold beside the largest value (atc_too_wide, of the CTA's rows and pages) is left to pages_redo_kernel, which comes behind and does the CTAs that said
+// so.  Sequences with few new tokens are pages_attn_kernel's.
 #pragma once
 
 #include "attn_tc.cuh"
@@ -156,12 +156,12 @@ __global__ void __launch_bounds__(ATC_THREADS, 1) pages_tc_kernel(const __grid_c
     if (!seq_of_item(C.start, C.n_seq, C.n_tok, (int)blockIdx.x, lane, [&](int n) { return ((int64_t)n * P.group + PTC_ROWS - 1) / PTC_ROWS; }, seq, tile)) return;      // CTA-uniform
     const SeqRange range = seq_range(C.start, seq, C.n_tok);
     const int len = C.len[seq];
-    if (!pages_on_tc(P, range.n, len)) return;                           // the kernel behind this one has it (and says what is wrong with it)
+    if (!pages_on_tc(P, range.n, len)) return;                           // pages_attn_kernel has it (and says what is wrong with it)
     const int n_rows = min(PTC_ROWS, range.n * P.group - tile * PTC_ROWS);
     const int first_tok = tile * PTC_ROWS / P.group, last_tok = (tile * PTC_ROWS + n_rows - 1) / P.group;
     const int before = len - range.n;
     const int seen_pos = min(len, before + last_tok + 1), pages = (max(seen_pos, 0) + PG_POS - 1) / PG_POS;
-    const int page0 = split * P.pages_per_split, page1 = split == P.splits - 1 ? pages : min(page0 + P.pages_per_split, pages);
+    const int page0 = split * P.span, page1 = split == P.splits - 1 ? pages : min(page0 + P.span, pages);
     const int ntiles = page1 - page0;
     if (ntiles <= 0 && split > 0) return;
     const int all_see = before + first_tok;
@@ -434,9 +434,9 @@ __global__ void __launch_bounds__(ATC_THREADS, 1) pages_tc_kernel(const __grid_c
     if (threadIdx.x == 0) P.redo[((size_t)blockIdx.x * C.n_head_kv + kvh) * P.splits + split] = redo && all_ok ? 1 : 0;
     if (redo || !all_ok) return;
     const float l = __fadd_rn(__fadd_rn(red[row], red[ATC_M + row]), __fadd_rn(red[2 * ATC_M + row], red[3 * ATC_M + row]));
-    const float inv = P.splits > 1 ? 1.0f : l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);           // a row that sees nothing is zeros
-    float *dst = P.splits > 1 ? P.part_acc + (size_t)split * C.n_tok * P.n_head * KV_D : P.out;
-    if (P.splits > 1 && cg == 0 && row < n_rows) P.part_ml[(size_t)split * C.n_tok * P.n_head + row_at(row) / KV_D] = make_float2(m_run, l);
+    const float inv = P.part_acc != nullptr ? 1.0f : l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);           // a row that sees nothing is zeros
+    float *dst = P.part_acc != nullptr ? P.part_acc + (size_t)split * C.n_tok * P.n_head * KV_D : P.out;
+    if (P.part_acc != nullptr && cg == 0 && row < n_rows) P.part_ml[(size_t)split * C.n_tok * P.n_head + row_at(row) / KV_D] = make_float2(m_run, l);
     if ((reinterpret_cast<uintptr_t>(dst) & 15u) == 0) {
 #pragma unroll
         for (int c = 0; c < 16; ++c)
