@@ -1979,11 +1979,13 @@ int bonsai_b200_qk_norm_rope(const float *q, const float *k, const float *q_weig
         if (one_head && !one_tok && ts < head_dim) return 1;
         vec = vec && aligned16(P.x[i]) && aligned16(P.w[i]) && aligned16(P.y[i]) && (one_tok || ts % 4 == 0) && (one_head || hs % 4 == 0);
     }
-    const int groups = (heads + QKN_MAX_WARPS - 1) / QKN_MAX_WARPS, warps = (heads + groups - 1) / groups;
-    if (groups > 65535) return 1;
-    auto run = [&](auto kernel) { return (int)launch(kernel, dim3((unsigned)n_tok, (unsigned)groups), dim3(32 * (unsigned)warps), 0, as_stream(stream), true, P); };
-    if (n_tok * groups <= SM_COUNT) return vec ? run(qk_norm_rope_kernel<true, true>) : run(qk_norm_rope_kernel<false, true>);
-    return vec ? run(qk_norm_rope_kernel<true, false>) : run(qk_norm_rope_kernel<false, false>);
+    auto run = [&](auto kernel, int per) {
+        const int groups = (heads + per * QKN_MAX_WARPS - 1) / (per * QKN_MAX_WARPS), warps = (heads + groups * per - 1) / (groups * per);
+        if (groups > 65535) return 1;
+        return (int)launch(kernel, dim3((unsigned)n_tok, (unsigned)groups), dim3(32 * (unsigned)warps), 0, as_stream(stream), true, P);
+    };
+    if (n_tok * ((heads + QKN_MAX_WARPS - 1) / QKN_MAX_WARPS) <= 2 * SM_COUNT) return vec ? run(qk_norm_rope_kernel<true, 1>, 1) : run(qk_norm_rope_kernel<false, 1>, 1);
+    return vec ? run(qk_norm_rope_kernel<true, 4>, 4) : run(qk_norm_rope_kernel<false, 4>, 4);
 }
 
 int bonsai_b200_pages_append(const bonsai_b200_pages *pages, int layer, const float *k, const float *v, bonsai_stream stream) {
@@ -2128,7 +2130,11 @@ int bonsai_b200_gdn_seqs(float *state, const float *q, const float *k, const flo
     if (chunks && (!workspace || !aligned16(workspace) || workspace_bytes < chunks * ((int64_t)n_k_heads * GDC_KQ_REC + (int64_t)n_v_heads * GDC_TP_REC))) return 1;
     const GdnSeqs P = {state, q, k, v, g, beta, out, start, slot, n_seq, n_slots, n_tok, n_k_heads, n_v_heads, K, V};
     const cudaStream_t st = as_stream(stream);
-    cudaError_t e = launch(gdn_seqs_step_kernel, dim3((unsigned)(n_v_heads * (V / 32)), (unsigned)n_seq), dim3(GDN_WARPS * 32), 0, st, true, P, chunks ? GDC_STEP_MOST : INT32_MAX);
+    // a CTA has 32 columns of a state, or 128 where there are enough of them for the SMs
+    const int most = chunks ? GDC_STEP_MOST : INT32_MAX;
+    cudaError_t e = V % 128 == 0 && aligned16(state) && aligned16(v) && aligned16(out) && (int64_t)n_v_heads * (V / 128) * n_seq >= SM_COUNT
+                        ? launch(gdn_seqs_step_kernel<4>, dim3((unsigned)(n_v_heads * (V / 128)), (unsigned)n_seq), dim3(GDN_WARPS * 32), 0, st, true, P, most)
+                        : launch(gdn_seqs_step_kernel<1>, dim3((unsigned)(n_v_heads * (V / 32)), (unsigned)n_seq), dim3(GDN_WARPS * 32), 0, st, true, P, most);
     if (!chunks || e != cudaSuccess) return (int)e;
     static SmemOptIn opt[2];
     uint8_t *kq = static_cast<uint8_t *>(workspace), *tp = kq + chunks * n_k_heads * GDC_KQ_REC;

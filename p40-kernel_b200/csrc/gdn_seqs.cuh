@@ -27,15 +27,35 @@ __device__ __forceinline__ int gdn_slot_of(const GdnSeqs &P, int s) {
 }
 
 // ---- token by token: the form for few tokens --------------------------------------------------------------------------------------------
-// As gdn_step_kernel: one CTA per (sequence, value head, 32 columns of the state), eight warps, lane = column, warp w holds rows w, w + 8, ... in
-// registers over all of the sequence's tokens: the state is read once and written once.  Sequences of more than `most` tokens are not its own.
+// As gdn_step_kernel: one CTA per (sequence, value head, 32 PER columns of the state), eight warps, lane = PER columns, warp w holds rows w, w + 8, ... in registers over all of
+// the sequence's tokens: the state is read once and written once.  Sequences of more than `most` tokens are not its own.
+template <int PER>
+struct GdnCols { float x[PER]; };
+template <int PER>
+__device__ __forceinline__ GdnCols<PER> gdn_load_cols(const float *p) {
+    GdnCols<PER> c;
+    if constexpr (PER == 4) {
+        const float4 v = *reinterpret_cast<const float4 *>(p);
+        c.x[0] = v.x; c.x[1] = v.y; c.x[2] = v.z; c.x[3] = v.w;
+    } else {
+        c.x[0] = p[0];
+    }
+    return c;
+}
+template <int PER>
+__device__ __forceinline__ void gdn_store_cols(float *p, const GdnCols<PER> &c) {
+    if constexpr (PER == 4) *reinterpret_cast<float4 *>(p) = make_float4(c.x[0], c.x[1], c.x[2], c.x[3]);
+    else p[0] = c.x[0];
+}
+template <int PER>
 __global__ void __launch_bounds__(GDN_WARPS * 32) gdn_seqs_step_kernel(const __grid_constant__ GdnSeqs P, int most) {
     __shared__ float ks[2][GDN_KMAX], qs[2][GDN_KMAX];
-    __shared__ float part[2][GDN_WARPS][32];
+    __shared__ __align__(16) float part[2][GDN_WARPS][32 * PER];
+    using Cols = GdnCols<PER>;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int tiles = P.V / 32, s = blockIdx.y;
+    const int tiles = P.V / (32 * PER), s = blockIdx.y;
     const int vh = blockIdx.x / tiles, vt = blockIdx.x - vh * tiles;
-    const int j = vt * 32 + lane;
+    const int j = (vt * 32 + lane) * PER;
     const int kh = vh / (P.n_v_heads / P.n_k_heads);
     pdl_wait_prior_grid();
     pdl_launch_dependents();
@@ -48,22 +68,37 @@ __global__ void __launch_bounds__(GDN_WARPS * 32) gdn_seqs_step_kernel(const __g
     }
     const bool there = mine >= 0 && mine < P.n_slots;
     float *Sg = P.state + ((size_t)(there ? mine : 0) * P.n_v_heads + vh) * P.K * P.V + j;
-    float col[GDN_RPW];
+    Cols col[GDN_RPW];
 #pragma unroll
     for (int i = 0; i < GDN_RPW; ++i) {
         const int row = warp + GDN_WARPS * i;
-        col[i] = there && row < P.K ? Sg[(size_t)row * P.V] : 0.0f;
+        if (there && row < P.K) col[i] = gdn_load_cols<PER>(Sg + (size_t)row * P.V);
+        else
+#pragma unroll
+            for (int c = 0; c < PER; ++c) col[i].x[c] = 0.0f;
     }
     // a token's scalars and this thread's values of k or q (K <= 128: threads 0 .. 127 have k, the others q)
     const int kq_at = threadIdx.x & (GDN_KMAX - 1);
     const float *kq_src = threadIdx.x < GDN_KMAX ? P.k : P.q;
-    float b, vj, gt, kq;
+    float b, gt, kq;
+    Cols vj;
     auto fetch = [&](int t) {
         const size_t tok = (size_t)(r.begin + t);
         b = P.beta[tok * P.n_v_heads + vh];
-        vj = P.v[(tok * P.n_v_heads + vh) * P.V + j];
+        vj = gdn_load_cols<PER>(P.v + (tok * P.n_v_heads + vh) * P.V + j);
         gt = P.g[tok * P.n_v_heads + vh];
         kq = kq_at < P.K ? kq_src[(tok * P.n_k_heads + kh) * P.K + kq_at] : 0.0f;
+    };
+    // (sums over the warps' rows, in ascending order of the warps)
+    auto joined = [&](const float (*p)[32 * PER]) {
+        Cols sum = gdn_load_cols<PER>(&p[0][lane * PER]);
+#pragma unroll
+        for (int w = 1; w < GDN_WARPS; ++w) {
+            const Cols x = gdn_load_cols<PER>(&p[w][lane * PER]);
+#pragma unroll
+            for (int c = 0; c < PER; ++c) sum.x[c] = __fadd_rn(sum.x[c], x.x[c]);
+        }
+        return sum;
     };
     fetch(0);
     if (gdn_slot_of(P, s) < 0) {
@@ -73,47 +108,52 @@ __global__ void __launch_bounds__(GDN_WARPS * 32) gdn_seqs_step_kernel(const __g
     for (int t = 0; t < r.n; ++t) {
         const int b2 = t & 1;
         const size_t tok = (size_t)(r.begin + t);
-        const float beta = b, value = vj, decay = expf(gt);
+        const float beta = b, decay = expf(gt);
+        const Cols value = vj;
         (threadIdx.x < GDN_KMAX ? ks : qs)[b2][kq_at] = kq;
         if (t + 1 < r.n) fetch(t + 1);                      // the next token's are on their way
         __syncthreads();
-        float kv = 0.0f;
+        Cols kv, o;
+#pragma unroll
+        for (int c = 0; c < PER; ++c) kv.x[c] = o.x[c] = 0.0f;
 #pragma unroll
         for (int i = 0; i < GDN_RPW; ++i) {
             const int row = warp + GDN_WARPS * i;
             if (row < P.K) {
-                col[i] = __fmul_rn(col[i], decay);
-                kv = __fadd_rn(kv, __fmul_rn(ks[b2][row], col[i]));
+                const float k = ks[b2][row];
+#pragma unroll
+                for (int c = 0; c < PER; ++c) {
+                    col[i].x[c] = __fmul_rn(col[i].x[c], decay);
+                    kv.x[c] = __fadd_rn(kv.x[c], __fmul_rn(k, col[i].x[c]));
+                }
             }
         }
-        part[0][warp][lane] = kv;
+        gdn_store_cols<PER>(&part[0][warp][lane * PER], kv);
         __syncthreads();
-        kv = 0.0f;
+        kv = joined(part[0]);
+        Cols d;
 #pragma unroll
-        for (int w = 0; w < GDN_WARPS; ++w) kv = __fadd_rn(kv, part[0][w][lane]);
-        const float d = __fsub_rn(value, kv);
-        float o = 0.0f;
+        for (int c = 0; c < PER; ++c) d.x[c] = __fsub_rn(value.x[c], kv.x[c]);
 #pragma unroll
         for (int i = 0; i < GDN_RPW; ++i) {
             const int row = warp + GDN_WARPS * i;
             if (row < P.K) {
-                col[i] = __fadd_rn(col[i], __fmul_rn(__fmul_rn(beta, ks[b2][row]), d));
-                o = __fadd_rn(o, __fmul_rn(qs[b2][row], col[i]));
+                const float k = __fmul_rn(beta, ks[b2][row]), q = qs[b2][row];
+#pragma unroll
+                for (int c = 0; c < PER; ++c) {
+                    col[i].x[c] = __fadd_rn(col[i].x[c], __fmul_rn(k, d.x[c]));
+                    o.x[c] = __fadd_rn(o.x[c], __fmul_rn(q, col[i].x[c]));
+                }
             }
         }
-        part[1][warp][lane] = o;
+        gdn_store_cols<PER>(&part[1][warp][lane * PER], o);
         __syncthreads();
-        if (warp == 0) {
-            o = 0.0f;
-#pragma unroll
-            for (int w = 0; w < GDN_WARPS; ++w) o = __fadd_rn(o, part[1][w][lane]);
-            P.out[(tok * P.n_v_heads + vh) * P.V + j] = o;
-        }
+        if (warp == 0) gdn_store_cols<PER>(P.out + (tok * P.n_v_heads + vh) * P.V + j, joined(part[1]));
     }
 #pragma unroll
     for (int i = 0; i < GDN_RPW; ++i) {
         const int row = warp + GDN_WARPS * i;
-        if (row < P.K) Sg[(size_t)row * P.V] = col[i];
+        if (row < P.K) gdn_store_cols<PER>(Sg + (size_t)row * P.V, col[i]);
     }
 }
 

@@ -33,62 +33,76 @@ __device__ __forceinline__ float2 rotation_of(int pos, double freq) {
     return make_float2(c, s);
 }
 
-// grid (tokens, groups of heads); a warp per head.  VEC: head_dim and the strides are multiples of 4, all pointers 16-byte aligned.
-template <bool VEC, bool EARLY>
+// grid (tokens, groups of heads); a warp has up to PER heads.  VEC: head_dim and the strides are multiples of 4, all pointers 16-byte aligned.
+// Bound by memory: 28 heads of 256 in and out are 57 KB a token.  PER = 4 asks for a token's heads at once and forms its angles once; of few tokens a warp has one head.  us, 24 + 4
+// heads, a head / four heads a warp: 2000 tokens 25.6 / see below.
+template <bool VEC, int PER>
 __global__ void __launch_bounds__(32 * QKN_MAX_WARPS) qk_norm_rope_kernel(const __grid_constant__ QkNormParams P) {
     __shared__ __align__(16) float rows[QKN_MAX_WARPS][QKN_MAX_DIM];
     __shared__ float2 turn[QKN_MAX_DIM / 2];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = (int)blockDim.x >> 5;
     const int64_t tok = blockIdx.x;
-    int head = (int)blockIdx.y * warps + warp;
-    const bool live = head < P.n_head[0] + P.n_head[1];
-    const int which = head >= P.n_head[0];
-    if (which) head -= P.n_head[0];
+    const int heads = P.n_head[0] + P.n_head[1], first = (int)blockIdx.y * warps * PER + warp;
     const int n = P.head_dim, half = P.n_rot >> 1;
     pdl_wait_prior_grid();
-    if (EARLY) pdl_launch_dependents();
-    float4 f[2], w[2];
-    if (live) {
-        const float *x = P.x[which] + tok * P.tok_stride[which] + head * P.head_stride[which];
+    if (PER == 1) pdl_launch_dependents();
+    float4 f[PER][2];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) f[j] = rms_load<VEC>(x, 128 * j + 4 * lane, n);
+    for (int r = 0; r < PER; ++r) {
+        int head = first + warps * r;
+        if (head < heads) {
+            const int which = head >= P.n_head[0];
+            if (which) head -= P.n_head[0];
+            const float *x = P.x[which] + tok * P.tok_stride[which] + head * P.head_stride[which];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) w[j] = rms_load<VEC>(P.w[which], 128 * j + 4 * lane, n);
+            for (int j = 0; j < 2; ++j) f[r][j] = rms_load<VEC>(x, 128 * j + 4 * lane, n);
+        }
     }
     for (int i = threadIdx.x; i < half; i += blockDim.x) turn[i] = rotation_of(P.pos[tok], P.freq[i]);
     __syncthreads();
-    if (!live) return;
-    const float sc = rms_scale(__fadd_rn(slice_sumsq(f[0]), n > 128 ? slice_sumsq(f[1]) : 0.0f), n, P.eps);
     float *row = rows[warp];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        f[j].x = __fmul_rn(__fmul_rn(f[j].x, sc), w[j].x);
-        f[j].y = __fmul_rn(__fmul_rn(f[j].y, sc), w[j].y);
-        f[j].z = __fmul_rn(__fmul_rn(f[j].z, sc), w[j].z);
-        f[j].w = __fmul_rn(__fmul_rn(f[j].w, sc), w[j].w);
-        reinterpret_cast<float4 *>(row)[32 * j + lane] = f[j];
-    }
-    __syncwarp();
-    float *y = P.y[which] + (tok * P.n_head[which] + head) * n;
-    auto turned = [&](int i, float own) {
-        if (i >= P.n_rot) return own;
-        const bool second = i >= half;
-        const float2 t = turn[second ? i - half : i];
-        const float other = row[second ? i - half : i + half];
-        return second ? __fmaf_rn(own, t.x, __fmul_rn(other, t.y)) : __fmaf_rn(own, t.x, -__fmul_rn(other, t.y));
-    };
+    for (int r = 0; r < PER; ++r) {
+        int head = first + warps * r;
+        if (head >= heads) break;
+        const int which = head >= P.n_head[0];
+        if (which) head -= P.n_head[0];
+        float4 w[2];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int i = 128 * j + 4 * lane;
-        if (i < n) {
-            const float4 o = make_float4(turned(i, f[j].x), turned(i + 1, f[j].y), turned(i + 2, f[j].z), turned(i + 3, f[j].w));
-            if (VEC) {
-                *reinterpret_cast<float4 *>(y + i) = o;
-            } else {
-                y[i] = o.x;
-                if (i + 1 < n) y[i + 1] = o.y;
-                if (i + 2 < n) y[i + 2] = o.z;
-                if (i + 3 < n) y[i + 3] = o.w;
+        for (int j = 0; j < 2; ++j) w[j] = rms_load<VEC>(P.w[which], 128 * j + 4 * lane, n);
+        const float sc = rms_scale(__fadd_rn(slice_sumsq(f[r][0]), n > 128 ? slice_sumsq(f[r][1]) : 0.0f), n, P.eps);
+        if (r) __syncwarp();                            // the row before has been read
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            f[r][j].x = __fmul_rn(__fmul_rn(f[r][j].x, sc), w[j].x);
+            f[r][j].y = __fmul_rn(__fmul_rn(f[r][j].y, sc), w[j].y);
+            f[r][j].z = __fmul_rn(__fmul_rn(f[r][j].z, sc), w[j].z);
+            f[r][j].w = __fmul_rn(__fmul_rn(f[r][j].w, sc), w[j].w);
+            if (128 * j < P.n_rot) reinterpret_cast<float4 *>(row)[32 * j + lane] = f[r][j];
+        }
+        __syncwarp();
+        float *y = P.y[which] + (tok * P.n_head[which] + head) * n;
+        auto turned = [&](int i, float own) {
+            if (i >= P.n_rot) return own;
+            const bool second = i >= half;
+            const float2 t = turn[second ? i - half : i];
+            const float other = row[second ? i - half : i + half];
+            return second ? __fmaf_rn(own, t.x, __fmul_rn(other, t.y)) : __fmaf_rn(own, t.x, -__fmul_rn(other, t.y));
+        };
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int i = 128 * j + 4 * lane;
+            if (i < n) {
+                float4 o = f[r][j];
+                if (i < P.n_rot) o = make_float4(turned(i, o.x), turned(i + 1, o.y), turned(i + 2, o.z), turned(i + 3, o.w));
+                if (VEC) {
+                    *reinterpret_cast<float4 *>(y + i) = o;
+                } else {
+                    y[i] = o.x;
+                    if (i + 1 < n) y[i + 1] = o.y;
+                    if (i + 2 < n) y[i + 2] = o.z;
+                    if (i + 3 < n) y[i + 3] = o.w;
+                }
             }
         }
     }
