@@ -2058,7 +2058,7 @@ int bonsai_b200_pages_attn(const bonsai_b200_pages *pages, int layer, const floa
     if (plan.tc) {
         const unsigned heads = (unsigned)C.n_head_kv, splits = (unsigned)plan.splits;
         if (e == cudaSuccess) e = launch(pages_planes_kernel, dim3((unsigned)(plan.tc * plan.max_pages), heads, 2), dim3(ATC_PREP_THREADS), 0, st, true, P);
-        if (e == cudaSuccess) e = run(pages_tc_kernel, opt[4], dim3((unsigned)plan.tiles, heads, splits), ATC_THREADS, ATC_SMEM_BYTES);
+        if (e == cudaSuccess) e = run(pages_tc_kernel, opt[4], dim3((unsigned)plan.tiles, heads, splits), PTC_THREADS, PTC_SMEM_BYTES);
         if (e == cudaSuccess) e = run(pages_redo_kernel, opt[5], dim3(2 * (unsigned)plan.tiles, heads, splits), 32 * pga_warps(4), pga_smem_bytes(4));
     }
     if (e == cudaSuccess && P.part_acc) {

@@ -728,15 +728,25 @@ __global__ void __launch_bounds__(32 * PGJ_WARPS) pages_join_kernel(const __grid
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-#pragma unroll 4
-    for (int i = mine; i < n; i += ROWW) {
-        const float2 x = P.part_ml[i * rows + row];
-        const float4 *src = reinterpret_cast<const float4 *>(P.part_acc) + (i * rows + row) * (KV_D / 4) + lane;
-        const float4 c = src[0], d = src[32];
-        const float w = x.x == m ? 1.0f : expf(__fsub_rn(x.x, m));
-        l = __fmaf_rn(x.y, w, l);
-        a = make_float4(__fmaf_rn(c.x, w, a.x), __fmaf_rn(c.y, w, a.y), __fmaf_rn(c.z, w, a.z), __fmaf_rn(c.w, w, a.w));
-        b = make_float4(__fmaf_rn(d.x, w, b.x), __fmaf_rn(d.y, w, b.y), __fmaf_rn(d.z, w, b.z), __fmaf_rn(d.w, w, b.w));
+    for (int i0 = mine; i0 < n; i0 += 4 * ROWW) {      // four splits' loads at once
+        float2 x[4];
+        float4 c[4], d[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int64_t at = (int64_t)min(i0 + e * ROWW, n - 1) * rows + row;
+            const float4 *src = reinterpret_cast<const float4 *>(P.part_acc) + at * (KV_D / 4) + lane;
+            x[e] = P.part_ml[at];
+            c[e] = src[0];
+            d[e] = src[32];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (i0 + e * ROWW >= n) break;
+            const float w = x[e].x == m ? 1.0f : expf(__fsub_rn(x[e].x, m));
+            l = __fmaf_rn(x[e].y, w, l);
+            a = make_float4(__fmaf_rn(c[e].x, w, a.x), __fmaf_rn(c[e].y, w, a.y), __fmaf_rn(c[e].z, w, a.z), __fmaf_rn(c[e].w, w, a.w));
+            b = make_float4(__fmaf_rn(d[e].x, w, b.x), __fmaf_rn(d[e].y, w, b.y), __fmaf_rn(d[e].z, w, b.z), __fmaf_rn(d[e].w, w, b.w));
+        }
     }
     if (ROWW > 1) {
         sums[warp][0][lane] = a;

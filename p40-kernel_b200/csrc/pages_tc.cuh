@@ -5,10 +5,11 @@
 //
 // pages_planes_kernel writes the pages of a call's long sequences once as tile images (attn_tc.cuh's, a page a tile).
 //
-// pages_tc_kernel: CTA = 128 rows (tokens times the heads that share a kv head) and one span of pages, 512 threads, each one row and a quarter of its columns.  The tensor core
-// has a page's scores and the outputs of the page before in flight while the threads form weights:
+// pages_tc_kernel: CTA = 128 rows (tokens times the heads that share a kv head) and one span of pages.  512 threads, each one row and a quarter of its columns, form weights and add
+// outputs; one warp more does the copies and issues the tensor core's instructions, which has a page's scores and the outputs of the page before in flight meanwhile:
 //   tensor core   q . k of page i + 1          | weights x v of page i
-//   threads       outputs of page i - 1 added, weights of page i to tensor memory | scores of page i + 1 read, softmax
+//   threads       weights of page i, outputs of page i - 1 added, weights to tensor memory | scores of page i + 1 read
+// (The issue is a warp's whole time: 2100 cycles for a page's scores, 1170 for its outputs.  By one of the sixteen warps a page took 8000 cycles.)
 // Tensor memory, all 512 columns: 256 output, 64 scores, 64 weights, 128 q low.  Shared memory: q high, k and v images of one page, 64 KB each.
 //
 // What one plane pair cannot hold beside the largest value (atc_too_wide, of the CTA's rows and pages) is left to pages_redo_kernel, which comes behind and does the CTAs that said
@@ -21,12 +22,16 @@
 namespace b200 {
 
 constexpr uint32_t PTC_COL_O = 0, PTC_COL_S = 256, PTC_COL_P = 320, PTC_COL_QL = 384;
+constexpr int PTC_THREADS = ATC_THREADS + 32;
+constexpr int PTC_SMEM_BYTES = 1024 + 3 * ATC_PLANES + (2 * ATC_KEYS + 2 * ATT_D + 2 * 4 * ATC_M) * 4 + 128;
+// Among the threads that have rows.
+__device__ __forceinline__ void ptc_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(ATC_THREADS) : "memory"); }
 static_assert(PG_POS == ATC_KEYS && KV_D == ATT_D && PTC_ROWS == ATC_M, "");
 
 // grid (sequences on the tensor cores x pages, kv heads, 2): z 0 = k (warp = eight positions, lane = eight dims), z 1 = v (thread = one dim, all 64 positions).
 __global__ void __launch_bounds__(ATC_PREP_THREADS) pages_planes_kernel(const __grid_constant__ PageAttn P) {
     __shared__ __align__(16) uint8_t rows[PG_HEAD_BYTES];
-    __shared__ uint32_t top[ATC_PREP_THREADS / 32][ATC_KEYS];
+    __shared__ uint32_t top[ATC_PREP_THREADS / 32];
     const PageCache &C = P.C;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, kvh = blockIdx.y;
     const int page_at = blockIdx.x % P.max_pages;
@@ -84,10 +89,10 @@ __global__ void __launch_bounds__(ATC_PREP_THREADS) pages_planes_kernel(const __
             *reinterpret_cast<uint4 *>(dst + ATC_KEYS * 128) = lo;
             if (lane == 0) reinterpret_cast<float *>(img + ATC_IMG_KF)[key] = atc_pow2(-s);
         }
-        if (lane == 0) top[warp][0] = seen;
+        if (lane == 0) top[warp] = seen;
         __syncthreads();
         if (warp == 0) {
-            const uint32_t m = __reduce_max_sync(0xffffffffu, top[lane & (ATC_PREP_THREADS / 32 - 1)][0]);
+            const uint32_t m = __reduce_max_sync(0xffffffffu, top[lane & (ATC_PREP_THREADS / 32 - 1)]);
             if (lane == 0) range[0] = m;
         }
     } else {
@@ -110,23 +115,21 @@ __global__ void __launch_bounds__(ATC_PREP_THREADS) pages_planes_kernel(const __
             *reinterpret_cast<uint4 *>(dst) = hi;
             *reinterpret_cast<uint4 *>(dst + 2 * ATC_CHUNK) = lo;
         }
-        // the positions' largest values: over the warp's 32 dims (lane e keeps positions e and e + 32), then over the warps
-        uint32_t own[2] = {0u, 0u};
-#pragma unroll
-        for (int e = 0; e < ATC_KEYS; ++e) {
-            const uint32_t m = __reduce_max_sync(0xffffffffu, atc_abs_bits(x[e]));
-            if (lane == (e & 31)) own[e >> 5] = m;
-        }
-        top[warp][lane] = own[0];
-        top[warp][lane + 32] = own[1];
+        // The positions' largest values, by their blocks' scales: 127 of a scale, which the quantiser's blocks reach (others reach less, and their rows stand for less than they say).
         const int tiny = __syncthreads_or(seen > 0u && seen < ATC_TINY ? 1 : 0);
         if (warp == 0) {
+            uint32_t most = 0u, least = ATC_NONE;
 #pragma unroll
-            for (int w = 0; w < ATC_PREP_THREADS / 32; ++w)
+            for (int h = 0; h < 2; ++h) {
+                uint32_t own = 0u;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) own[h] = max(own[h], top[w][lane + 32 * h]);
-            const uint32_t most = __reduce_max_sync(0xffffffffu, max(own[0], own[1]));
-            const uint32_t least = __reduce_min_sync(0xffffffffu, min(own[0] ? own[0] : ATC_NONE, own[1] ? own[1] : ATC_NONE));
+                for (int blk = 0; blk < KV_NBLK; ++blk) own = max(own, *reinterpret_cast<const uint16_t *>(rows + (lane + 32 * h) * KV_ROW + 34 * blk) & 0x7FFFu);
+                own = atc_abs_bits(__fmul_rn(f16_bits_to_f32(own), 127.0f));
+                most = max(most, own);
+                least = min(least, own ? own : ATC_NONE);
+            }
+            most = __reduce_max_sync(0xffffffffu, most);
+            least = __reduce_min_sync(0xffffffffu, least);
             if (lane == 0) {
                 range[1] = tiny ? ATC_NONE : most;
                 range[2] = least;
@@ -136,15 +139,17 @@ __global__ void __launch_bounds__(ATC_PREP_THREADS) pages_planes_kernel(const __
 }
 
 // grid (tiles of 128 rows of all sequences and some that find none, kv heads, splits)
-__global__ void __launch_bounds__(ATC_THREADS, 1) pages_tc_kernel(const __grid_constant__ PageAttn P) {
+__global__ void __launch_bounds__(PTC_THREADS, 1) pages_tc_kernel(const __grid_constant__ PageAttn P) {
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t *qhi = smem + ((1024u - (smem_u32(smem) & 1023u)) & 1023u);
     uint8_t *kpl = qhi + ATC_PLANES, *vpl = kpl + ATC_PLANES;
     float *kf = reinterpret_cast<float *>(vpl + ATC_PLANES);             // [2][64] 2^-s of the page's positions, pages alternate
     float *vf = kf + 2 * ATC_KEYS;                                       // [2][256] 2^-s of the dims (and the weights' 2^-14)
-    float *red = vf + 2 * ATT_D;                                         // [4][128] exchange between the four warps of a row
-    uint64_t *qk = reinterpret_cast<uint64_t *>(red + 4 * ATC_M), *pv = qk + 1, *kfull = qk + 2, *vfull = qk + 3;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(vfull + 1);
+    float *red0 = vf + 2 * ATT_D;                                        // [2][4][128] exchange between the four warps of a row, pages alternate
+    // pages alternate between two barriers of the copies: a phase ends when everybody has long waited for the one before
+    uint64_t *qk = reinterpret_cast<uint64_t *>(red0 + 2 * 4 * ATC_M), *pv = qk + 1, *scored = qk + 2, *weighed = qk + 3, *kfull = qk + 4, *vfull = qk + 6;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(vfull + 2);
+    volatile int *failed = reinterpret_cast<int *>(tmem_slot + 1);
 
     const PageCache &C = P.C;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -181,9 +186,11 @@ __global__ void __launch_bounds__(ATC_THREADS, 1) pages_tc_kernel(const __grid_c
     };
 
     if (threadIdx.x == 0) {
-        for (int b = 0; b < 4; ++b) mbar_init(qk + b, 1);
+        for (int b = 0; b < 8; ++b) mbar_init(qk + b, b == 2 || b == 3 ? ATC_WARPS : 1);
         mbar_fence_init();
+        *failed = 0;
     }
+    const bool driver = warp == ATC_WARPS;
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -193,25 +200,111 @@ __global__ void __launch_bounds__(ATC_THREADS, 1) pages_tc_kernel(const __grid_c
         const uint64_t pol = policy_evict_last_or_default();
         const uint8_t *src = img + (size_t)i * img_stride;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // the factors were read by ordinary loads
-        mbar_expect_tx(kfull, ATC_PLANES + ATC_KEYS * 4);
-        bulk_g2s(kf + (i & 1) * ATC_KEYS, src + ATC_IMG_KF, ATC_KEYS * 4, kfull, pol);
-        bulk_g2s(kpl, src, ATC_PLANES, kfull, pol);
+        mbar_expect_tx(kfull + (i & 1), ATC_PLANES + ATC_KEYS * 4);
+        bulk_g2s(kf + (i & 1) * ATC_KEYS, src + ATC_IMG_KF, ATC_KEYS * 4, kfull + (i & 1), pol);
+        bulk_g2s(kpl, src, ATC_PLANES, kfull + (i & 1), pol);
     };
     auto load_v = [&](int i) {
         const uint64_t pol = policy_evict_last_or_default();
         const uint8_t *src = img + (size_t)i * img_stride;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        mbar_expect_tx(vfull, ATC_PLANES + ATT_D * 4);
-        bulk_g2s(vf + (i & 1) * ATT_D, src + ATC_IMG_VF, ATT_D * 4, vfull, pol);
-        bulk_g2s(vpl, src + ATC_PLANES, ATC_PLANES, vfull, pol);
+        mbar_expect_tx(vfull + (i & 1), ATC_PLANES + ATT_D * 4);
+        bulk_g2s(vf + (i & 1) * ATT_D, src + ATC_IMG_VF, ATT_D * 4, vfull + (i & 1), pol);
+        bulk_g2s(vpl, src + ATC_PLANES, ATC_PLANES, vfull + (i & 1), pol);
     };
 
     // ---- q: row of the thread, 64 dims, quantised to Q8_0 (two blocks); high plane to shared memory, low plane to tensor memory.  Queries and outputs pass through shared
     // memory (the planes' of k and v, a warp's 32 rows of 64 values each, 16-byte pieces swizzled), where a row's values become a thread's.
     float4 *box = reinterpret_cast<float4 *>(kpl) + warp * 512;
     const int row0 = 32 * (warp & 3);
-    float qf;
-    uint32_t seen;                                                       // magnitude bits of the row's largest q
+    float qf = 0.0f;
+    uint32_t seen = 0;                                                   // magnitude bits of the row's largest q
+    __syncthreads();                                                     // the barriers, and where tensor memory is
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const uint32_t tlane = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+    // The tensor core's instructions, one elected lane of the driver's warp (the code stays warp-uniform).  Products with a low plane come first: the accumulator is small
+    // while they are added.
+    auto issue_qk = [&] {
+        tc_fence_after();
+        constexpr uint32_t LOW = (ATC_KEYS * 128) >> 4;
+        const uint32_t a0 = tc16_desc_lo(smem_u32(qhi)), b0 = tc16_desc_lo(smem_u32(kpl)), ql = tmem + PTC_COL_QL, d = tmem + PTC_COL_S;
+        auto at = [](int n) { return (uint32_t)((n >> 2) * (ATC_CHUNK >> 4) + 2 * (n & 3)); };
+        if (elect_one()) {
+            tc_mma_f16_ts<false>(d, ql, b0, atc_idesc(ATC_KEYS));
+#pragma unroll
+            for (int n = 1; n < 16; ++n) tc_mma_f16_ts<true>(d, ql + (uint32_t)(8 * n), b0 + at(n), atc_idesc(ATC_KEYS));
+#pragma unroll
+            for (int n = 0; n < 16; ++n) atc_mma_ss<atc_idesc(ATC_KEYS)>(d, a0 + at(n), b0 + LOW + at(n));
+#pragma unroll
+            for (int n = 0; n < 16; ++n) atc_mma_ss<atc_idesc(ATC_KEYS)>(d, a0 + at(n), b0 + at(n));
+            tc_commit(qk);
+        }
+        __syncwarp();
+    };
+    auto issue_pv = [&] {
+        tc_fence_after();
+        const uint32_t b0 = tc16_desc_lo(smem_u32(vpl)), ph = tmem + PTC_COL_P, pl = ph + 32u;
+        if (elect_one()) {
+#pragma unroll
+            for (int n = 0; n < 12; ++n) {
+                const uint32_t a = (n < 4 ? pl : ph) + (uint32_t)(8 * (n & 3));
+                const uint32_t b = b0 + (uint32_t)((n >= 4 && n < 8 ? (2 * ATC_CHUNK) >> 4 : 0) + 2 * (n & 3));
+                if (n == 0) tc_mma_f16_ts<false>(tmem + PTC_COL_O, a, b, atc_idesc(ATT_D));
+                else tc_mma_f16_ts<true>(tmem + PTC_COL_O, a, b, atc_idesc(ATT_D));
+            }
+            tc_commit(pv);
+        }
+        __syncwarp();
+    };
+    if (driver) {
+        __syncthreads();                                                 // q is in its places
+        bool ok = true;                                                  // after a wait that ran out nothing is waited for any more: the CTA comes to its end, and says so
+        if (ntiles > 0) {
+            if (lane == 0) {
+                load_k(0);
+                load_v(0);
+            }
+            __syncwarp();
+            ok = __all_sync(0xffffffffu, mbar_wait_try(kfull, 0));
+            issue_qk();
+        }
+        for (int i = 0; i < ntiles; ++i) {
+            const uint32_t par = (uint32_t)(i & 1);
+            const bool more = i + 1 < ntiles;
+            if (more) {
+                // what the page before leaves room for, as it does: scores read, then k of the next page; outputs done, then v of this one
+                bool k_done = false, v_done = i == 0;
+                for (uint32_t n = 0; ok && !(k_done && v_done); ++n) {           // (every lane's answer is the warp's)
+                    if (!k_done && __any_sync(0xffffffffu, mbar_test(scored, par))) {
+                        if (lane == 0) load_k(i + 1);
+                        k_done = true;
+                    }
+                    if (!v_done && __any_sync(0xffffffffu, mbar_test(pv, par ^ 1u))) {
+                        if (lane == 0) load_v(i);
+                        v_done = true;
+                    }
+                    __syncwarp();
+                    if (n > (1u << 22)) {
+                        atomicExch(&g_device_status, STATUS_MBARRIER_TIMEOUT);
+                        ok = false;
+                    }
+                }
+                ok = ok && __all_sync(0xffffffffu, mbar_wait_try(kfull + (par ^ 1u), (uint32_t)(((i + 1) >> 1) & 1)));
+                issue_qk();
+            } else if (i > 0) {
+                ok = ok && __all_sync(0xffffffffu, mbar_wait_try(pv, par ^ 1u));
+                if (lane == 0) load_v(i);
+                __syncwarp();
+            }
+            ok = ok && __all_sync(0xffffffffu, mbar_wait_try(weighed, par));
+            ok = ok && __all_sync(0xffffffffu, mbar_wait_try(vfull + par, (uint32_t)((i >> 1) & 1)));
+            issue_pv();
+        }
+        if (!ok) *failed = 1;
+        __syncthreads();
+        return;
+    }
     {
         float x[64];
         if ((reinterpret_cast<uintptr_t>(P.q) & 15u) == 0) {
@@ -246,11 +339,9 @@ __global__ void __launch_bounds__(ATC_THREADS, 1) pages_tc_kernel(const __grid_c
                 m = max(m, atc_abs_bits(x[32 * b + e]));
             }
         }
-        uint32_t *redu = reinterpret_cast<uint32_t *>(red);
+        uint32_t *redu = reinterpret_cast<uint32_t *>(red0);
         redu[cg * ATC_M + row] = m;
-        tc_fence_before();
-        __syncthreads();
-        tc_fence_after();
+        ptc_barrier();
 #pragma unroll
         for (int c = 0; c < 4; ++c) m = max(m, redu[c * ATC_M + row]);
         seen = m;
@@ -264,87 +355,40 @@ __global__ void __launch_bounds__(ATC_THREADS, 1) pages_tc_kernel(const __grid_c
             *reinterpret_cast<uint4 *>(qhi + cg * ATC_CHUNK + row * 128 + ((j ^ (row & 7)) * 16)) = hi;
             lo32[4 * j] = lo.x; lo32[4 * j + 1] = lo.y; lo32[4 * j + 2] = lo.z; lo32[4 * j + 3] = lo.w;
         }
-        tc_st32(*tmem_slot + ((uint32_t)(32 * (warp & 3)) << 16) + PTC_COL_QL + (uint32_t)(32 * cg), lo32);
+        tc_st32(tlane + PTC_COL_QL + (uint32_t)(32 * cg), lo32);
+        tc_st_wait();
     }
-    const uint32_t tmem = *tmem_slot;
-    const uint32_t tlane = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
-    // The tensor core's instructions, one elected lane of warp 0 (the code stays warp-uniform).  Products with a low plane come first: the accumulator is small
-    // while they are added.
-    auto issue_qk = [&] {
-        tc_fence_after();
-        constexpr uint32_t LOW = (ATC_KEYS * 128) >> 4;
-        const uint32_t a0 = tc16_desc_lo(smem_u32(qhi)), b0 = tc16_desc_lo(smem_u32(kpl)), ql = tmem + PTC_COL_QL, d = tmem + PTC_COL_S;
-        auto at = [](int n) { return (uint32_t)((n >> 2) * (ATC_CHUNK >> 4) + 2 * (n & 3)); };
-        if (elect_one()) {
-            tc_mma_f16_ts<false>(d, ql, b0, atc_idesc(ATC_KEYS));
-#pragma unroll
-            for (int n = 1; n < 16; ++n) tc_mma_f16_ts<true>(d, ql + (uint32_t)(8 * n), b0 + at(n), atc_idesc(ATC_KEYS));
-#pragma unroll
-            for (int n = 0; n < 16; ++n) atc_mma_ss<atc_idesc(ATC_KEYS)>(d, a0 + at(n), b0 + LOW + at(n));
-#pragma unroll
-            for (int n = 0; n < 16; ++n) atc_mma_ss<atc_idesc(ATC_KEYS)>(d, a0 + at(n), b0 + at(n));
-            tc_commit(qk);
-        }
-        __syncwarp();
-    };
-    auto issue_pv = [&] {
-        tc_fence_after();
-        const uint32_t b0 = tc16_desc_lo(smem_u32(vpl)), ph = tmem + PTC_COL_P, pl = ph + 32u;
-        if (elect_one()) {
-#pragma unroll
-            for (int n = 0; n < 12; ++n) {
-                const uint32_t a = (n < 4 ? pl : ph) + (uint32_t)(8 * (n & 3));
-                const uint32_t b = b0 + (uint32_t)((n >= 4 && n < 8 ? (2 * ATC_CHUNK) >> 4 : 0) + 2 * (n & 3));
-                if (n == 0) tc_mma_f16_ts<false>(tmem + PTC_COL_O, a, b, atc_idesc(ATT_D));
-                else tc_mma_f16_ts<true>(tmem + PTC_COL_O, a, b, atc_idesc(ATT_D));
-            }
-            tc_commit(pv);
-        }
-        __syncwarp();
-    };
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");        // q high: written here, read by the tensor core
-    tc_st_wait();
     tc_fence_before();
     __syncthreads();                                                    // (and the box has been read: k and v take its place)
     bool ok = true;
-    if (ntiles > 0) {
-        if (warp == 4 && lane == 0) {
-            load_k(0);
-            load_v(0);
-        }
-        if (warp == 0) {
-            ok = mbar_wait_try(kfull, 0);
-            issue_qk();
-        }
-    }
     float acc[64];                                                       // row, dims 64 cg ..
 #pragma unroll
     for (int e = 0; e < 64; ++e) acc[e] = 0.0f;
     float m_run = -INFINITY, l_run = 0.0f, alpha = 0.0f;                 // l_run: of the thread's 16 columns of every page
     auto add_page = [&](int par) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            int o[2][16];
-            tc_ld16(tlane + PTC_COL_O + (uint32_t)(64 * cg + 32 * h), o[0]);
-            tc_ld16(tlane + PTC_COL_O + (uint32_t)(64 * cg + 32 * h + 16), o[1]);
+        for (int h = 0; h < 8; ++h) {
+            int o[8];
+            tc_ld8(tlane + PTC_COL_O + (uint32_t)(64 * cg + 8 * h), o);
             tc_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-                const float4 f = *reinterpret_cast<const float4 *>(vf + par * ATT_D + 64 * cg + 32 * h + e);
-                float *a = acc + 32 * h + e;
-                const int *t = o[e >> 4] + (e & 15);
-                a[0] = __fmaf_rn(__int_as_float(t[0]), f.x, __fmul_rn(a[0], alpha));
-                a[1] = __fmaf_rn(__int_as_float(t[1]), f.y, __fmul_rn(a[1], alpha));
-                a[2] = __fmaf_rn(__int_as_float(t[2]), f.z, __fmul_rn(a[2], alpha));
-                a[3] = __fmaf_rn(__int_as_float(t[3]), f.w, __fmul_rn(a[3], alpha));
+            for (int e = 0; e < 8; e += 4) {
+                const float4 f = *reinterpret_cast<const float4 *>(vf + par * ATT_D + 64 * cg + 8 * h + e);
+                float *a = acc + 8 * h + e;
+                a[0] = __fmaf_rn(__int_as_float(o[e]), f.x, __fmul_rn(a[0], alpha));
+                a[1] = __fmaf_rn(__int_as_float(o[e + 1]), f.y, __fmul_rn(a[1], alpha));
+                a[2] = __fmaf_rn(__int_as_float(o[e + 2]), f.z, __fmul_rn(a[2], alpha));
+                a[3] = __fmaf_rn(__int_as_float(o[e + 3]), f.w, __fmul_rn(a[3], alpha));
             }
         }
     };
     for (int i = 0; i < ntiles; ++i) {
         const int p0 = (page0 + i) * PG_POS;
         const uint32_t par = (uint32_t)(i & 1);
+        float *red = red0 + par * 4 * ATC_M;
         float s[16], mx = -INFINITY;
-        ok = mbar_wait_both(kfull, par, qk, par) && ok;                  // (the first is long complete; it makes the copied factors visible)
+        ok = ok && mbar_wait_both(kfull + par, (uint32_t)((i >> 1) & 1), qk, par);       // (the first is long complete; it makes the copied factors visible)
         tc_fence_after();
         {
             int a[16];
@@ -353,6 +397,9 @@ __global__ void __launch_bounds__(ATC_THREADS, 1) pages_tc_kernel(const __grid_c
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[e] = __fmul_rn(__int_as_float(a[e]), __fmul_rn(qf, kf[par * ATC_KEYS + 16 * cg + e]));
         }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(scored);
         if (p0 + PG_POS - 1 > all_see) {                                 // some row does not see some position (one behind the last is behind every row's)
 #pragma unroll
             for (int e = 0; e < 16; ++e)
@@ -361,11 +408,7 @@ __global__ void __launch_bounds__(ATC_THREADS, 1) pages_tc_kernel(const __grid_c
 #pragma unroll
         for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[e]);
         red[cg * ATC_M + row] = mx;
-        tc_fence_before();
-        if (!__syncthreads_and(ok ? 1 : 0)) break;                       // every score has been read (a wait ran out: the CTA leaves as a whole)
-        tc_fence_after();
-        // (a barrier's next phase is begun only when the whole CTA has waited for this one)
-        if (warp == 4 && lane == 0 && i + 1 < ntiles) load_k(i + 1);
+        ptc_barrier();
         float m_new = m_run;
 #pragma unroll
         for (int c = 0; c < 4; ++c) m_new = fmaxf(m_new, red[c * ATC_M + row]);
@@ -382,33 +425,29 @@ __global__ void __launch_bounds__(ATC_THREADS, 1) pages_tc_kernel(const __grid_c
             }
             l_run = __fadd_rn(__fmul_rn(l_run, alpha_new), sum);
         }
-        if (i > 0) {                                                     // the outputs of the page before; its weights and values have been read
-            ok = mbar_wait_try(pv, par ^ 1u) && ok;
+        if (i > 0) {                                                     // the outputs of the page before; its weights have been read
+            ok = ok && mbar_wait_both(vfull + (par ^ 1u), (uint32_t)(((i - 1) >> 1) & 1), pv, par ^ 1u);
             tc_fence_after();
-            if (warp == 4 && lane == 0) load_v(i);
-            add_page((int)par ^ 1);
         }
-        alpha = alpha_new;
         tc_st8(tlane + PTC_COL_P + (uint32_t)(8 * cg), hi);
         tc_st8(tlane + PTC_COL_P + (uint32_t)(32 + 8 * cg), lo);
+        if (i > 0) add_page((int)par ^ 1);
+        alpha = alpha_new;
         tc_st_wait();
-        if (warp == 0 && i + 1 < ntiles) {
-            ok = mbar_wait_try(kfull, par ^ 1u) && ok;
-            issue_qk();
-        }
-        ok = mbar_wait_try(vfull, par) && ok;                            // in front of the CTA's barrier: load_v begins the next phase
         tc_fence_before();
-        __syncthreads();
-        if (warp == 0) issue_pv();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(weighed);
     }
     if (ntiles > 0) {
-        ok = mbar_wait_try(pv, (uint32_t)((ntiles - 1) & 1)) && ok;
+        ok = ok && mbar_wait_both(vfull + ((ntiles - 1) & 1), (uint32_t)(((ntiles - 1) >> 1) & 1), pv, (uint32_t)((ntiles - 1) & 1));
         tc_fence_after();
         add_page((ntiles - 1) & 1);
     }
-    __syncthreads();
-    red[cg * ATC_M + row] = l_run;
+    if (!ok) *failed = 1;
     tc_fence_before();
+    __syncthreads();
+    float *red = red0;
+    red[cg * ATC_M + row] = l_run;
     uint32_t k_most = 0, v_most = 0, v_least = ATC_NONE;
     for (int t = threadIdx.x; t < ntiles; t += ATC_THREADS) {
         const uint32_t *r = reinterpret_cast<const uint32_t *>(img + (size_t)t * img_stride + ATC_IMG_RANGE);
@@ -422,7 +461,8 @@ __global__ void __launch_bounds__(ATC_THREADS, 1) pages_tc_kernel(const __grid_c
     v_most = __reduce_max_sync(0xffffffffu, v_most);
     v_least = __reduce_min_sync(0xffffffffu, v_least);
     if (lane == 0) ranges[warp] = make_uint4(seen, k_most, v_most, v_least);
-    const int all_ok = __syncthreads_and(ok ? 1 : 0);
+    ptc_barrier();
+    const bool all_ok = *failed == 0;
     const uint4 r = ranges[lane & (ATC_WARPS - 1)];
     const uint32_t q_most = __reduce_max_sync(0xffffffffu, r.x);
     const bool redo = q_most >= ATC_HUGE || atc_too_wide(__float_as_uint(fabsf(__fmul_rn(__uint_as_float(q_most), P.scale))), __reduce_max_sync(0xffffffffu, r.y),
