@@ -6,10 +6,11 @@
 // pages_planes_kernel writes the pages of a call's long sequences once as tile images (attn_tc.cuh's, a page a tile).
 //
 // pages_tc_kernel: CTA = 128 rows (tokens times the heads that share a kv head) and one span of pages.  512 threads, each one row and a quarter of its columns, form weights and add
-// outputs; one warp more does the copies and issues the tensor core's instructions, which has a page's scores and the outputs of the page before in flight meanwhile:
+// outputs; of three warps more one issues the tensor core's instructions, which has a page's scores and the outputs of the page before in flight meanwhile, two copy k and v:
 //   tensor core   q . k of page i + 1          | weights x v of page i
 //   threads       weights of page i, outputs of page i - 1 added, weights to tensor memory | scores of page i + 1 read
-// (The issue is a warp's whole time: 2100 cycles for a page's scores, 1170 for its outputs.  By one of the sixteen warps a page took 8000 cycles.)
+// (The issue is a warp's whole time: 2100 cycles for a page's scores, 1100 for its outputs.  By one of the sixteen warps a page took 8000 cycles, with the copies from the issuing
+// warp 5850.)
 // Tensor memory, all 512 columns: 256 output, 64 scores, 64 weights, 128 q low.  Shared memory: q high, k and v images of one page, 64 KB each.
 //
 // What one plane pair cannot hold beside the largest value (atc_too_wide, of the CTA's rows and pages) is left to pages_redo_kernel, which comes behind and does the CTAs that said
@@ -22,7 +23,7 @@
 namespace b200 {
 
 constexpr uint32_t PTC_COL_O = 0, PTC_COL_S = 256, PTC_COL_P = 320, PTC_COL_QL = 384;
-constexpr int PTC_THREADS = ATC_THREADS + 32;
+constexpr int PTC_THREADS = ATC_THREADS + 96;
 constexpr int PTC_SMEM_BYTES = 1024 + 3 * ATC_PLANES + (2 * ATC_KEYS + 2 * ATT_D + 2 * 4 * ATC_M) * 4 + 128;
 // Among the threads that have rows.
 __device__ __forceinline__ void ptc_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(ATC_THREADS) : "memory"); }
@@ -190,7 +191,7 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) pages_tc_kernel(const __grid_c
         mbar_fence_init();
         *failed = 0;
     }
-    const bool driver = warp == ATC_WARPS;
+    const bool driver = warp >= ATC_WARPS;
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -260,46 +261,32 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) pages_tc_kernel(const __grid_c
     if (driver) {
         __syncthreads();                                                 // q is in its places
         bool ok = true;                                                  // after a wait that ran out nothing is waited for any more: the CTA comes to its end, and says so
-        if (ntiles > 0) {
-            if (lane == 0) {
-                load_k(0);
-                load_v(0);
-            }
-            __syncwarp();
-            ok = __all_sync(0xffffffffu, mbar_wait_try(kfull, 0));
-            issue_qk();
-        }
-        for (int i = 0; i < ntiles; ++i) {
-            const uint32_t par = (uint32_t)(i & 1);
-            const bool more = i + 1 < ntiles;
-            if (more) {
-                // what the page before leaves room for, as it does: scores read, then k of the next page; outputs done, then v of this one
-                bool k_done = false, v_done = i == 0;
-                for (uint32_t n = 0; ok && !(k_done && v_done); ++n) {           // (every lane's answer is the warp's)
-                    if (!k_done && __any_sync(0xffffffffu, mbar_test(scored, par))) {
-                        if (lane == 0) load_k(i + 1);
-                        k_done = true;
-                    }
-                    if (!v_done && __any_sync(0xffffffffu, mbar_test(pv, par ^ 1u))) {
-                        if (lane == 0) load_v(i);
-                        v_done = true;
-                    }
-                    __syncwarp();
-                    if (n > (1u << 22)) {
-                        atomicExch(&g_device_status, STATUS_MBARRIER_TIMEOUT);
-                        ok = false;
-                    }
+        auto wait = [&](uint64_t *bar, uint32_t parity) { ok = ok && __all_sync(0xffffffffu, mbar_wait_try(bar, parity)); };
+        if (warp == ATC_WARPS) {
+            for (int i = 0; i <= ntiles && ntiles > 0; ++i) {            // scores of page i, outputs of page i - 1
+                if (i < ntiles) {
+                    if (i > 0) wait(scored, (uint32_t)((i - 1) & 1));
+                    wait(kfull + (i & 1), (uint32_t)((i >> 1) & 1));
+                    issue_qk();
                 }
-                ok = ok && __all_sync(0xffffffffu, mbar_wait_try(kfull + (par ^ 1u), (uint32_t)(((i + 1) >> 1) & 1)));
-                issue_qk();
-            } else if (i > 0) {
-                ok = ok && __all_sync(0xffffffffu, mbar_wait_try(pv, par ^ 1u));
+                if (i > 0) {
+                    wait(weighed, (uint32_t)((i - 1) & 1));
+                    wait(vfull + ((i - 1) & 1), (uint32_t)(((i - 1) >> 1) & 1));
+                    issue_pv();
+                }
+            }
+        } else if (warp == ATC_WARPS + 1) {
+            for (int i = 0; i < ntiles; ++i) {                           // k when the scores of the page before have been read
+                if (i > 0) wait(scored, (uint32_t)((i - 1) & 1));
+                if (lane == 0) load_k(i);
+                __syncwarp();
+            }
+        } else {
+            for (int i = 0; i < ntiles; ++i) {                           // v when the outputs of the page before are there
+                if (i > 0) wait(pv, (uint32_t)((i - 1) & 1));
                 if (lane == 0) load_v(i);
                 __syncwarp();
             }
-            ok = ok && __all_sync(0xffffffffu, mbar_wait_try(weighed, par));
-            ok = ok && __all_sync(0xffffffffu, mbar_wait_try(vfull + par, (uint32_t)((i >> 1) & 1)));
-            issue_pv();
         }
         if (!ok) *failed = 1;
         __syncthreads();
