@@ -177,7 +177,7 @@ constexpr int GDC_COLS = 48, GDC_NT = GDC_COLS / 8, GDC_SLICES = 3;
 constexpr int GDC_KB = GDC_D * 2 + 16, GDC_TB = GDC_T * 2 + 16, GDC_CB = GDC_COLS * 2 + 16;
 constexpr int GDC_KP = GDC_T * GDC_KB, GDC_TP = GDC_T * GDC_TB, GDC_SP = GDC_D * GDC_CB, GDC_UP = GDC_T * GDC_CB;        // a plane of K or Q, Tb or P, S, U
 constexpr int GDC_TS = GDC_T + 4;                                     // floats: a row of A and of its inverse
-constexpr int GDC_STEP_MOST = 16;                                     // tokens of a sequence that go one by one
+constexpr int GDC_STEP_MOST = 24;                                     // tokens of a sequence that go one by one (us, one by one / in chunks: 16 19 / 28, 24 25 / 28, 48 45 / 28.6)
 // What the first two kernels leave, in bytes, planes with the row strides of shared memory so that one bulk copy fetches them: of a chunk and key head the planes of K and Q and
 // the exponents s of their rows' powers of two; of a chunk and value head the planes of Tb and P, then floats: per row e^G 2^-s of K, e^G 2^-s of Q, e^(G_63 - G) 2^(s_min - s) of K,
 // 2^-s of Tb, 2^-s of P; then e^G_63, 2^-s_min, whether the chunk is to go token by token.
@@ -197,11 +197,16 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
 __device__ __forceinline__ void ldsm2_t(uint32_t (&r)[4], uint32_t addr) {       // (into the first two)
     asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(addr) : "memory");
 }
-// The first product of a sum.
-__device__ __forceinline__ void mma_f16_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+// The products have no other effect than their sums, so that the compiler may put them where it likes.
+__device__ __forceinline__ void gdc_mma_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+__device__ __forceinline__ void gdc_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 // c[m] = A[m] B over 16 STEPS values, each A 16 rows, B 8 NT columns.  a[m], b: the lane's addresses of the high planes, the low ones a_low and b_low behind, a step a_step and
 // b_step behind the one before; of a pair of column tiles b_pair.  AT: A lies by columns; BT: B lies by rows.
@@ -227,15 +232,15 @@ __device__ __forceinline__ void gdc_product(float (&c)[MT][NT][4], const uint32_
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int j = 0; j < NT; ++j) mma_f16_first(sum[m][j], al[m], bh[j >> 1][2 * (j & 1)], bh[j >> 1][2 * (j & 1) + 1]);
+            for (int j = 0; j < NT; ++j) gdc_mma_first(sum[m][j], al[m], bh[j >> 1][2 * (j & 1)], bh[j >> 1][2 * (j & 1) + 1]);
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int j = 0; j < NT; ++j) mma_f16_16816(sum[m][j], ah[m][0], ah[m][1], ah[m][2], ah[m][3], bl[j >> 1][2 * (j & 1)], bl[j >> 1][2 * (j & 1) + 1]);
+            for (int j = 0; j < NT; ++j) gdc_mma(sum[m][j], ah[m], bl[j >> 1][2 * (j & 1)], bl[j >> 1][2 * (j & 1) + 1]);
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int j = 0; j < NT; ++j) mma_f16_16816(sum[m][j], ah[m][0], ah[m][1], ah[m][2], ah[m][3], bh[j >> 1][2 * (j & 1)], bh[j >> 1][2 * (j & 1) + 1]);
+            for (int j = 0; j < NT; ++j) gdc_mma(sum[m][j], ah[m], bh[j >> 1][2 * (j & 1)], bh[j >> 1][2 * (j & 1) + 1]);
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -356,16 +361,28 @@ __global__ void __launch_bounds__(GDC_PREP_THREADS, 3) gdn_chunk_kernel(const __
 #pragma unroll
     for (int i = 0; i < 5; ++i) {
         const int top = warp & 1, m = i <= top ? top : 3 - top, jb = i <= top ? i : i - top - 1;
+        double gr[2], gc[4];                    // of the lane's two rows and four columns: sums of g, factors
+        float fr[2], fc[4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int row = 16 * m + g + 8 * h;
+            gr[h] = gs[row];
+            fr[h] = atc_pow2(-shift[(of_q ? GDC_T : 0) + row]);
+            if (!of_q) fr[h] = __fmul_rn(fr[h], bs[row]);
+            if (row >= n) fr[h] = 0.0f;
+        }
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+            const int col = 16 * jb + 8 * (h >> 1) + 2 * t + (h & 1);
+            gc[h] = gs[col];
+            fc[h] = atc_pow2(-shift[col]);
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const int row = 16 * m + g + 8 * ((e >> 1) & 1), col = 16 * jb + 8 * (e >> 2) + 2 * t + (e & 1);
-            float x = 0.0f;
-            if (col <= row && row < n) {
-                const float decay = expf((float)(gs[row] - gs[col])), f = atc_pow2(-shift[(of_q ? GDC_T : 0) + row]), f2 = atc_pow2(-shift[col]);
-                x = __fmul_rn(__fmul_rn(__fmul_rn(c[i][0][e >> 2][e & 3], f), f2), decay);
-                if (!of_q) x = col < row ? __fmul_rn(x, bs[row]) : 0.0f;
-                odd = odd || !(fabsf(x) < 1e30f);
-            }
+            const int h = (e >> 1) & 1, v = 2 * (e >> 2) + (e & 1), row = 16 * m + g + 8 * h, col = 16 * jb + 8 * (e >> 2) + 2 * t + (e & 1);
+            float x = __fmul_rn(__fmul_rn(__fmul_rn(c[i][0][e >> 2][e & 3], fr[h]), fc[v]), expf((float)(gr[h] - gc[v])));
+            if (col > row || (!of_q && col == row)) x = 0.0f;
+            odd = odd || !(fabsf(x) < 1e30f);
             (of_q ? pt : at)[row * GDC_TS + col] = x;
         }
     }
@@ -378,7 +395,13 @@ __global__ void __launch_bounds__(GDC_PREP_THREADS, 3) gdn_chunk_kernel(const __
         for (int i = 0; i < 16; ++i) {
             float s = i == lane ? 1.0f : 0.0f;
 #pragma unroll
-            for (int j = 0; j < i; ++j) s = __fmaf_rn(-at[(blk + i) * GDC_TS + blk + j], x[j], s);
+            for (int j = 0; j < i; j += 4) {
+                const float4 a = *reinterpret_cast<const float4 *>(at + (blk + i) * GDC_TS + blk + j);
+                s = __fmaf_rn(-a.x, x[j], s);
+                if (j + 1 < i) s = __fmaf_rn(-a.y, x[j + 1], s);
+                if (j + 2 < i) s = __fmaf_rn(-a.z, x[j + 2], s);
+                if (j + 3 < i) s = __fmaf_rn(-a.w, x[j + 3], s);
+            }
             x[i] = s;
         }
 #pragma unroll
@@ -587,7 +610,10 @@ __global__ void __launch_bounds__(GDC_THREADS, 1) gdn_scan_kernel(const __grid_c
         if (tid == 0) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             load_tp(c);
-            if (c + 1 < nchunk) load_k(c + 1);
+        }
+        if (tid == 32 && c + 1 < nchunk) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            load_k(c + 1);
         }
         if (tid < 8) r_most[tid] = u_most[tid] = u_most[tid + 8] = next[tid] = 0u;
         // ---- K S and Q S
@@ -659,11 +685,13 @@ __global__ void __launch_bounds__(GDC_THREADS, 1) gdn_scan_kernel(const __grid_c
         __syncthreads();
         if (!slow) {
             if (c + 1 < nchunk) load_qv(c + 1);
-            // ---- S = e^G_63 S + K^T (e^(G_63 - G) U)
+            // ---- S = e^G_63 S + K^T (e^(G_63 - G) U), O = e^G Q S + P U
+            float o[1][NH][4];
             {
                 float d[1][GDC_NT][4];
-                const uint32_t a[1] = {kb + 32 * warp + at_kt};
+                const uint32_t a[1] = {kb + 32 * warp + at_kt}, ap[1] = {smem_u32(tp) + 2 * GDC_TP + 16 * mt * GDC_TB + at_t};
                 gdc_product<1, GDC_NT, GDC_T / 16, true, true>(d, a, GDC_KP, 16 * GDC_KB, b_u + 2 * GDC_UP, GDC_UP, 16 * GDC_CB, 32);
+                gdc_product<1, NH, GDC_T / 16, false, true>(o, ap, GDC_TP, 32, b_u + 16 * j0, GDC_UP, 16 * GDC_CB, 32);
                 const float decay = vec[5 * GDC_T], kf = vec[5 * GDC_T + 1];
 #pragma unroll
                 for (int j = 0; j < GDC_NT; ++j) {
@@ -673,11 +701,7 @@ __global__ void __launch_bounds__(GDC_THREADS, 1) gdn_scan_kernel(const __grid_c
                 }
             }
             tiles_most(S, next);
-            // ---- O = e^G Q S + P U
             {
-                float o[1][NH][4];
-                const uint32_t a[1] = {smem_u32(tp) + 2 * GDC_TP + 16 * mt * GDC_TB + at_t};
-                gdc_product<1, NH, GDC_T / 16, false, true>(o, a, GDC_TP, 32, b_u + 16 * j0, GDC_UP, 16 * GDC_CB, 32);
 #pragma unroll
                 for (int j = 0; j < NH; ++j) {
                     const float fu = atc_pow2(-atc_shift(u_most[j0 + j], 63));
