@@ -1919,7 +1919,7 @@ int check_pages(const bonsai_b200_pages *p, int layer, PageCache *C) {
 // How pages_attn divides a call.  Sequences that may be on the tensor cores (tc of them at most, 0: none; pages_on_tc): tiles of 128 rows, a span of pages a CTA.  The others: rows
 // a tile; the spans are the device's to find, up to most_splits a tile.
 struct PagesPlan {
-    int rowt, rows, most_splits, span, splits, max_pages;
+    int rowt, most_splits, span, splits, max_pages;
     int64_t tiles, tc;
     int64_t part_bytes, image_bytes, redo_bytes;
     int64_t bytes() const { return part_bytes + image_bytes + redo_bytes; }
@@ -1932,9 +1932,11 @@ PagesPlan plan_pages(int n_tok, int max_len, int n_seq, int n_head, int n_head_k
     const int64_t rows = (int64_t)n_tok * group, each = (rows + n_seq - 1) / n_seq, pages = std::max(1, (int)(((int64_t)max_len + PG_POS - 1) / PG_POS));
     p.max_pages = (int)pages;
     p.tc = std::min<int64_t>(n_seq, rows / PTC_ROWS);
-    if (rows < 2 * PTC_ROWS || p.tc * pages * n_head_kv > PTC_IMAGE_LIMIT / ATC_IMG_BYTES) p.tc = 0;
-    p.rowt = p.tc ? (group <= 8 ? 0 : 1) : each > 32 ? 4 : each > 16 ? 2 : each > 8 ? 1 : 0;
-    p.rows = p.rowt ? 16 * p.rowt : 8;
+    // Who has how many tokens only the device knows.  Many more tokens than sequences are taken to be prompts: a batch of few tokens each would pay for launches that find nothing, and its
+    // tiles be those of the tensor cores' neighbours (16 sequences of 3 tokens 131 us instead of 74).
+    const int64_t beyond = ((int64_t)n_tok - std::min(n_seq, n_tok)) * group;
+    if (rows < 2 * PTC_ROWS || beyond < 4 * PTC_ROWS || p.tc * pages * n_head_kv > PTC_IMAGE_LIMIT / ATC_IMG_BYTES) p.tc = 0;
+    p.rowt = each > 32 ? 4 : each > 16 ? 2 : each > 8 ? 1 : 0;             // (without the tensor cores; beside them eight rows and 64)
     p.span = (int)pages;
     if (p.tc) {
         // spans that fill the last round of CTAs, one per SM; a CTA's start and its share of the join are worth four pages
@@ -2014,7 +2016,7 @@ int bonsai_b200_pages_attn(const bonsai_b200_pages *pages, int layer, const floa
     if (!q || !out || !aligned4(q) || !aligned4(out) || !pages_attn_sizes(C.n_tok, max_len, C.n_seq, n_head, C.n_head_kv)) return 1;
     const PagesPlan plan = plan_pages(C.n_tok, max_len, C.n_seq, n_head, C.n_head_kv);
     if (2 * plan.tiles > INT32_MAX || plan.tc * plan.max_pages > INT32_MAX) return 1;
-    if (((int64_t)C.n_tok * (n_head / C.n_head_kv) / plan.rows + C.n_seq) * plan.most_splits * C.n_head_kv > INT32_MAX) return 1;
+    if (((int64_t)C.n_tok * (n_head / C.n_head_kv) / 8 + C.n_seq) * plan.most_splits * C.n_head_kv > INT32_MAX) return 1;
     P.q = q;
     P.out = out;
     P.layer = layer;
@@ -2022,8 +2024,10 @@ int bonsai_b200_pages_attn(const bonsai_b200_pages *pages, int layer, const floa
     P.group = n_head / C.n_head_kv;
     P.span = plan.span;
     P.splits = plan.splits;
-    P.row_shift = 0;
-    while (1 << P.row_shift < plan.rows) ++P.row_shift;
+    P.most_rows[0] = plan.tc ? 8 : INT32_MAX;
+    P.most_rows[1] = INT32_MAX;
+    P.row_shift[0] = plan.tc || plan.rowt == 0 ? 3 : plan.rowt == 1 ? 4 : plan.rowt == 2 ? 5 : 6;
+    P.row_shift[1] = 6;
     P.most_splits = plan.most_splits;
     P.scale = scale;
     if (plan.bytes()) {
@@ -2038,23 +2042,21 @@ int bonsai_b200_pages_attn(const bonsai_b200_pages *pages, int layer, const floa
     }
     const cudaStream_t st = as_stream(stream);
     static SmemOptIn opt[6];
-    auto run = [&](auto kernel, SmemOptIn &o, dim3 grid, int threads, int smem) {
+    auto run = [&](auto kernel, SmemOptIn &o, dim3 grid, int threads, int smem, auto... more) {
         const cudaError_t e = o.ensure(kernel);
-        return e == cudaSuccess ? launch(kernel, grid, dim3((unsigned)threads), (size_t)smem, st, true, P) : e;
+        return e == cudaSuccess ? launch(kernel, grid, dim3((unsigned)threads), (size_t)smem, st, true, P, more...) : e;
     };
-    cudaError_t e = cudaSuccess;
     if (plan.tc) {
         P.max_pages = plan.max_pages;
         P.n_tc = (int)plan.tc;
     }
-    {
-        const dim3 grid(PGA_SLOTS);
-        const int smem = pga_smem_bytes(plan.rowt), threads = 32 * pga_warps(plan.rowt);
-        e = plan.rowt == 0   ? run(pages_attn_kernel<0>, opt[0], grid, threads, smem)
-            : plan.rowt == 1 ? run(pages_attn_kernel<1>, opt[1], grid, threads, smem)
-            : plan.rowt == 2 ? run(pages_attn_kernel<2>, opt[2], grid, threads, smem)
-                             : run(pages_attn_kernel<4>, opt[3], grid, threads, smem);
-    }
+    auto few = [&](auto kernel, SmemOptIn &o, int rowt, int cls) { return run(kernel, o, dim3(PGA_SLOTS), 32 * pga_warps(rowt), pga_smem_bytes(rowt), cls); };
+    const int rowt = plan.tc ? 0 : plan.rowt;
+    cudaError_t e = rowt == 0   ? few(pages_attn_kernel<0>, opt[0], 0, 0)
+                    : rowt == 1 ? few(pages_attn_kernel<1>, opt[1], 1, 0)
+                    : rowt == 2 ? few(pages_attn_kernel<2>, opt[2], 2, 0)
+                                : few(pages_attn_kernel<4>, opt[3], 4, 0);
+    if (e == cudaSuccess && plan.tc) e = few(pages_attn_kernel<4>, opt[3], 4, 1);
     if (plan.tc) {
         const unsigned heads = (unsigned)C.n_head_kv, splits = (unsigned)plan.splits;
         if (e == cudaSuccess) e = launch(pages_planes_kernel, dim3((unsigned)(plan.tc * plan.max_pages), heads, 2), dim3(ATC_PREP_THREADS), 0, st, true, P);
@@ -2142,7 +2144,7 @@ int bonsai_b200_gdn_seqs(float *state, const float *q, const float *k, const flo
         e = launch(gdn_planes_kernel, dim3((unsigned)chunks, (unsigned)n_k_heads), dim3(GDC_THREADS), 0, st, true, P, kq);
     if (e == cudaSuccess) e = launch(gdn_chunk_kernel, dim3((unsigned)chunks, (unsigned)n_v_heads), dim3(GDC_PREP_THREADS), (size_t)gdc_prep_smem(), st, true, P, (const uint8_t *)kq, tp);
     if (e == cudaSuccess)
-        e = launch(gdn_scan_kernel, dim3((unsigned)(n_v_heads * GDC_SLICES), (unsigned)n_seq), dim3(GDC_THREADS), (size_t)gdc_scan_smem(), st, true, P, (const uint8_t *)kq, (const uint8_t *)tp);
+        e = launch(gdn_scan_kernel, dim3((unsigned)(n_v_heads * GDC_SLICES), (unsigned)n_seq), dim3(GDC_THREADS), (size_t)gdc_scan_smem(), st, true, P, (const uint8_t *)kq, (const uint8_t *)tp, (int)chunks);
     return (int)e;
 }
 

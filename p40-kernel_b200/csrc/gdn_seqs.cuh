@@ -488,7 +488,7 @@ __global__ void __launch_bounds__(GDC_PREP_THREADS, 3) gdn_chunk_kernel(const __
 
 // grid (value heads x 3, sequences): columns 0 .. 47, 48 .. 87, 88 .. 127.  Warp w of eight: tokens 16 (w % 4) .. and half of the columns of all that has a row for each
 // token, and rows 16 w .. of the state, which stay in registers in fp32; its planes in shared memory are what the products read.
-__global__ void __launch_bounds__(GDC_THREADS, 1) gdn_scan_kernel(const __grid_constant__ GdnSeqs P, const uint8_t *kq_recs, const uint8_t *tp_recs) {
+__global__ void __launch_bounds__(GDC_THREADS, 1) gdn_scan_kernel(const __grid_constant__ GdnSeqs P, const uint8_t *kq_recs, const uint8_t *tp_recs, int n_chunks) {
     extern __shared__ __align__(16) uint8_t gdc_smem[];
     uint8_t *kp0 = gdc_smem, *qp = kp0 + 4 * GDC_KP, *tp = qp + 2 * GDC_KP, *sp = tp + 4 * GDC_TP, *up = sp + 2 * GDC_SP;       // K twice; Tb, P; U, U times its factors
     uint8_t *rp = qp;                                                   // V - e^G K S takes the place of Q when that has been read
@@ -513,6 +513,10 @@ __global__ void __launch_bounds__(GDC_THREADS, 1) gdn_scan_kernel(const __grid_c
     int first = 0;
     for (int i = lane; i < s; i += 32) first += gdc_chunks(max(0, seq_range(P.start, i, P.n_tok).n));
     first = __reduce_add_sync(0xffffffffu, first);
+    if (first > n_chunks - nchunk) {                            // (rows that several sequences claim: there are not as many records)
+        if (tid == 0) bad_sequence();
+        return;
+    }
     const uint8_t *kq = kq_recs + ((size_t)first * P.n_k_heads + kh) * GDC_KQ_REC, *rec = tp_recs + ((size_t)first * P.n_v_heads + vh) * GDC_TP_REC;
     const size_t kq_stride = (size_t)P.n_k_heads * GDC_KQ_REC, rec_stride = (size_t)P.n_v_heads * GDC_TP_REC;
     const size_t vstride = (size_t)P.n_v_heads * GDC_D;

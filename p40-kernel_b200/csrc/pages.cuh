@@ -134,7 +134,8 @@ struct PageAttn {
     float2 *part_ml;            // [splits][token * n_head + head]: maximum, sum of weights
     int layer, n_head, group;
     int span, splits;           // of the sequences on the tensor cores: pages of a CTA, CTAs of a tile
-    int row_shift, most_splits; // of the others: rows of a tile, as a power of two, CTAs of a tile at most
+    // of the others, in one class or two by their rows, a launch each: rows of a sequence at most, rows of a tile (as a power of two); CTAs of a tile at most
+    int most_rows[2], row_shift[2], most_splits;
     float scale;
     // the call's long sequences on the tensor cores (pages_tc.cuh): images [sequence][page][kv head], whether a CTA is to be done again [tile][kv head][split]
     uint8_t *images;
@@ -182,19 +183,20 @@ __device__ __forceinline__ void pga_halves(uint32_t a, uint32_t b, uint32_t (&ou
 
 // ---- how the sequences with few rows are divided: by what they hold, which the device knows.  Every CTA finds the same.
 struct SeqWork { int tiles, pages; };       // no tiles: not one of them
-__device__ __forceinline__ SeqWork pages_work(const PageAttn &P, int s) {
+__device__ __forceinline__ int pages_class(const PageAttn &P, int n) { return (int64_t)n * P.group <= P.most_rows[0] ? 0 : 1; }
+__device__ __forceinline__ SeqWork pages_work(const PageAttn &P, int s, int cls) {
     if (s >= P.C.n_seq) return {0, 0};
     const int n = seq_range(P.C.start, s, P.C.n_tok).n, len = P.C.len[s];
-    if (n <= 0 || pages_on_tc(P, n, len)) return {0, 0};
+    if (n <= 0 || pages_on_tc(P, n, len) || pages_class(P, n) != cls) return {0, 0};
     if (len < 0 || len > (int64_t)P.C.table_stride * PG_POS) return {1, 0};                 // one CTA says so
-    return {(n * P.group + (1 << P.row_shift) - 1) >> P.row_shift, (len + PG_POS - 1) / PG_POS};
+    return {(n * P.group + (1 << P.row_shift[cls]) - 1) >> P.row_shift[cls], (len + PG_POS - 1) / PG_POS};
 }
 __device__ __forceinline__ int pages_splits(const PageAttn &P, int pages, int span) { return max(1, min(P.most_splits, (pages + span - 1) / span)); }
 // Pages of a CTA such that one round of CTAs (two per SM) takes all of them.
-__device__ __noinline__ int pages_span(const PageAttn &P, int lane, int slots) {
+__device__ __noinline__ int pages_span(const PageAttn &P, int cls, int lane, int slots) {
     int64_t total = 0;
     for (int base = 0; base < P.C.n_seq; base += 32) {
-        const SeqWork w = pages_work(P, base + lane);
+        const SeqWork w = pages_work(P, base + lane, cls);
         total += (int64_t)w.tiles * w.pages;
     }
 #pragma unroll
@@ -204,7 +206,7 @@ __device__ __noinline__ int pages_span(const PageAttn &P, int lane, int slots) {
     for (int step = 0; step < 8; ++step) {              // (a sequence's last CTA has less: some more pages for each, until they fit)
         int items = 0;
         for (int base = 0; base < P.C.n_seq; base += 32) {
-            const SeqWork w = pages_work(P, base + lane);
+            const SeqWork w = pages_work(P, base + lane, cls);
             items += w.tiles ? w.tiles * pages_splits(P, w.pages, span) : 0;
         }
         items = __reduce_add_sync(0xffffffffu, items);
@@ -623,7 +625,7 @@ __device__ __forceinline__ bool pages_attn_item(const PageAttn &P, const PageIte
 
 // The sequences with few rows (pages_on_tc has the others).  grid: two CTAs per SM, which take items until there are none.
 template <int ROWT>
-__global__ void __launch_bounds__(32 * pga_warps(ROWT), 2) pages_attn_kernel(const __grid_constant__ PageAttn P) {
+__global__ void __launch_bounds__(32 * pga_warps(ROWT), 2) pages_attn_kernel(const __grid_constant__ PageAttn P, int cls) {
     extern __shared__ __align__(128) uint8_t smem[];
     uint64_t *kfull = reinterpret_cast<uint64_t *>(smem), *vfull = kfull + PGA_BUFS;
     const int lane = threadIdx.x & 31;
@@ -633,7 +635,7 @@ __global__ void __launch_bounds__(32 * pga_warps(ROWT), 2) pages_attn_kernel(con
     }
     pdl_wait_prior_grid();
     pdl_launch_dependents();
-    const int span = pages_span(P, lane, gridDim.x);
+    const int span = pages_span(P, cls, lane, gridDim.x);
     const int heads = P.C.n_head_kv;
     __syncthreads();
     int turn = 0;
@@ -642,7 +644,7 @@ __global__ void __launch_bounds__(32 * pga_warps(ROWT), 2) pages_attn_kernel(con
         int before = 0;
         PageItem<ROWT> I = {-1, 0, 0, 0, 0, 0};
         for (int base = 0; base < P.C.n_seq && I.seq < 0; base += 32) {
-            const SeqWork w = pages_work(P, base + lane);
+            const SeqWork w = pages_work(P, base + lane, cls);
             const int splits = pages_splits(P, w.pages, span), own = w.tiles * splits * heads;
             int sum = own;
 #pragma unroll
@@ -718,7 +720,7 @@ __global__ void __launch_bounds__(32 * PGJ_WARPS) pages_join_kernel(const __grid
                 const int seen = len - r.n + (tok - r.begin) + 1;
                 const int pages = (max(seen, 0) + PG_POS - 1) / PG_POS;
                 const bool tc = pages_on_tc(P, r.n, len);
-                const int span = tc ? P.span : pages_span(P, lane, slots);
+                const int span = tc ? P.span : pages_span(P, pages_class(P, r.n), lane, slots);
                 n = max(1, min(tc ? P.splits : pages_splits(P, (len + PG_POS - 1) / PG_POS, span), (pages + span - 1) / span));
             }
         }
