@@ -291,37 +291,44 @@ __device__ __forceinline__ bool pages_attn_item(const PageAttn &P, const PageIte
     {
         const int blk = lane >> 2, sub = lane & 3;
         const bool vec = (reinterpret_cast<uintptr_t>(P.q) & 15u) == 0;
-#pragma unroll 4
-        for (int r = warp; r < QROWS; r += WARPS) {
-            float x[8];
-            const int row = tile * ROWS + r, tok = row / P.group, h = row - tok * P.group;
-            const float *qr = P.q + ((size_t)(range.begin + tok) * P.n_head + kvh * P.group + h) * KV_D + blk * 32 + sub * 8;
-            if (EIGHT && r >= ROWS) {                   // the products' other eight rows are zeros
-                *reinterpret_cast<uint2 *>(q8 + r * PGA_Q_STRIDE + blk * 8 + 2 * sub) = make_uint2(0u, 0u);
-                continue;
-            }
-            if (r >= n_rows) {
+        constexpr int BATCH = ROWS / WARPS < 4 ? ROWS / WARPS : 4;               // rows of a warp whose loads are on their way together
+        static_assert(ROWS % (WARPS * BATCH) == 0, "");
+        if (EIGHT)                                      // the products' other eight rows are zeros
+            for (int i = tid; i < 8 * PGA_Q_STRIDE; i += THREADS) q8[8 * PGA_Q_STRIDE + i] = 0u;
+#pragma unroll 1
+        for (int r0 = warp * BATCH; r0 < ROWS; r0 += WARPS * BATCH) {
+            float x[BATCH][8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = 0.0f;
-            } else if (vec) {
-                const float4 a = *reinterpret_cast<const float4 *>(qr), c = *reinterpret_cast<const float4 *>(qr + 4);
-                x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = c.x; x[5] = c.y; x[6] = c.z; x[7] = c.w;
-            } else {
+            for (int e = 0; e < BATCH; ++e) {
+                const int r = r0 + e, row = tile * ROWS + (r < n_rows ? r : 0), tok = row / P.group, h = row - tok * P.group;
+                const float *qr = P.q + ((size_t)(range.begin + tok) * P.n_head + kvh * P.group + h) * KV_D + blk * 32 + sub * 8;
+                if (vec) {
+                    const float4 a = *reinterpret_cast<const float4 *>(qr), c = *reinterpret_cast<const float4 *>(qr + 4);
+                    x[e][0] = a.x; x[e][1] = a.y; x[e][2] = a.z; x[e][3] = a.w; x[e][4] = c.x; x[e][5] = c.y; x[e][6] = c.z; x[e][7] = c.w;
+                } else {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = qr[i];
+                    for (int i = 0; i < 8; ++i) x[e][i] = qr[i];
+                }
             }
-            const float d = __fmul_rn(kv_amax_8(x), PG_SCALE), id = d > 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
-            uint32_t w[2];
-            kv_words_8(x, id, w);
-            // in the order in which the K rows are read: of an even block slot 0 = values 0, 1, 30, 31, slot i = values 4 i - 2 .. 4 i + 1
-            const uint32_t below = __shfl_up_sync(0xffffffffu, w[1], 1), last = __shfl_sync(0xffffffffu, w[1], lane | 3);
-            uint32_t s0 = w[0], s1 = w[1];
-            if (!(blk & 1)) {
-                s0 = sub ? __byte_perm(below, w[0], 0x5432) : __byte_perm(w[0], last, 0x7610);
-                s1 = __byte_perm(w[0], w[1], 0x5432);
+#pragma unroll
+            for (int e = 0; e < BATCH; ++e) {
+                const int r = r0 + e;
+                if (r >= n_rows)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[e][i] = 0.0f;
+                const float d = __fmul_rn(kv_amax_8(x[e]), PG_SCALE), id = d > 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
+                uint32_t w[2];
+                kv_words_8(x[e], id, w);
+                // in the order in which the K rows are read: of an even block slot 0 = values 0, 1, 30, 31, slot i = values 4 i - 2 .. 4 i + 1
+                const uint32_t below = __shfl_up_sync(0xffffffffu, w[1], 1), last = __shfl_sync(0xffffffffu, w[1], lane | 3);
+                uint32_t s0 = w[0], s1 = w[1];
+                if (!(blk & 1)) {
+                    s0 = sub ? __byte_perm(below, w[0], 0x5432) : __byte_perm(w[0], last, 0x7610);
+                    s1 = __byte_perm(w[0], w[1], 0x5432);
+                }
+                *reinterpret_cast<uint2 *>(q8 + r * PGA_Q_STRIDE + blk * 8 + 2 * sub) = make_uint2(s0, s1);
+                if (sub == 0) qd[r * 8 + blk] = __fmul_rn(f16_bits_to_f32(f32_to_f16_bits_ties_away(d)), P.scale);
             }
-            *reinterpret_cast<uint2 *>(q8 + r * PGA_Q_STRIDE + blk * 8 + 2 * sub) = make_uint2(s0, s1);
-            if (sub == 0) qd[r * 8 + blk] = __fmul_rn(f16_bits_to_f32(f32_to_f16_bits_ties_away(d)), P.scale);
         }
     }
     float acc[MT][NB][4][2 * HR];                       // row tile, the warp's block, byte of the slot; (row g | g + 8, slot 2 t | 2 t + 1)
