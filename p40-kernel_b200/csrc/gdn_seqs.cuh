@@ -1,4 +1,5 @@
-// gdn_seqs.cuh -- the gated delta rule over the tokens of several sequences.
+// gdn_seqs.cuh -- the gated delta rule over the tokens of several sequences: S <- e^g S, d = beta (v - k S), S <- S + k d, o = q S for each token in turn (gdn_step_kernel's step).
+// Sequences of up to GDC_STEP_MOST tokens go token by token, longer ones in chunks of 64 (K = V = 128; other shapes go token by token whatever their length).
 #pragma once
 
 #include "attn_tc.cuh"
@@ -29,6 +30,8 @@ __device__ __forceinline__ int gdn_slot_of(const GdnSeqs &P, int s) {
 // ---- token by token: the form for few tokens --------------------------------------------------------------------------------------------
 // As gdn_step_kernel: one CTA per (sequence, value head, 32 PER columns of the state), eight warps, lane = PER columns, warp w holds rows w, w + 8, ... in registers over all of
 // the sequence's tokens: the state is read once and written once.  Sequences of more than `most` tokens are not its own.
+// Bound by memory for many sequences (16 of one token: 101 MB in 23 us; of 32 columns a CTA 28.7, where a state's tile is 16 KB), for few tokens of one by latency: 7 us and about 0.8 a
+// token more.
 template <int PER>
 struct GdnCols { float x[PER]; };
 template <int PER>
@@ -290,7 +293,8 @@ __global__ void __launch_bounds__(GDC_THREADS) gdn_planes_kernel(const __grid_co
     }
 }
 
-// grid (the same chunks, value heads): Tb and P.
+// grid (the same chunks, value heads): Tb and P.  Bound by issue and latency with 12 warps per SM (what a CTA's planes leave room for): 75 us for 2048 tokens and 48 heads, 5000
+// instructions a warp: products 700, decays 1000, the inverse 2000, planes of the results 1400.
 __global__ void __launch_bounds__(GDC_PREP_THREADS, 3) gdn_chunk_kernel(const __grid_constant__ GdnSeqs P, const uint8_t *kq_recs, uint8_t *tp_recs) {
     extern __shared__ __align__(16) uint8_t gdc_smem[];
     uint8_t *kp = gdc_smem, *qp = kp + 2 * GDC_KP;
@@ -486,6 +490,10 @@ __global__ void __launch_bounds__(GDC_PREP_THREADS, 3) gdn_chunk_kernel(const __
     if (tid == 0) vec[5 * GDC_T + 2] = any ? 1.0f : 0.0f;
 }
 
+// A chunk is a chain: K S and Q S | V - e^G K S scaled | U | U scaled | K^T U and P U | S scaled, with a barrier between any two, on eight warps: 11 600 cycles, of which the tensor
+// core's products are 4500 (counted in a run of 32 chunks; K S and Q S 2300, U 1080, the last two 2200, the scalings and their maxima 2900, copies and waits 1900).  What was worth it:
+// products by fp16 planes instead of TF32 parts (389 -> 317 us of the scan over 2048 tokens), powers of two by eight columns instead of one and bulk copies (-> 249), tokens' rows and half of the
+// columns to a warp (-> 216).  Three slices of the columns put 144 CTAs on 148 SMs; two would leave a third of them idle, four make the fuller SMs do two.
 // grid (value heads x 3, sequences): columns 0 .. 47, 48 .. 87, 88 .. 127.  Warp w of eight: tokens 16 (w % 4) .. and half of the columns of all that has a row for each
 // token, and rows 16 w .. of the state, which stay in registers in fp32; its planes in shared memory are what the products read.
 __global__ void __launch_bounds__(GDC_THREADS, 1) gdn_scan_kernel(const __grid_constant__ GdnSeqs P, const uint8_t *kq_recs, const uint8_t *tp_recs, int n_chunks) {

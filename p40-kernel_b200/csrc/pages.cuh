@@ -84,7 +84,8 @@ __global__ void __launch_bounds__(32 * KV_APPEND_WARPS) pages_append_kernel(cons
 // ---- copies -----------------------------------------------------------------------------------------------------------------------------------
 constexpr int PG_COPY_PAIRS = 480, PG_COPY_THREADS = 256, PG_COPY_WORDS = 8;            // 16-byte words a thread holds
 struct PagePairs { int32_t src[PG_COPY_PAIRS], dst[PG_COPY_PAIRS]; };
-// No page is written twice or both read and written (the host has looked), so the order does not matter.
+// No page is written twice or both read and written (the host has looked), so the order does not matter.  Bound by memory: 300 pages of 2.2 MB, 1.34 GB read and written, 212 us
+// (6.3 TB/s); four pages 5.5 us, of which the launch is half.  The pairs are launch parameters: 480 are what fits beside the rest, more are more launches.
 __global__ void __launch_bounds__(PG_COPY_THREADS) pages_copy_kernel(const __grid_constant__ PagePairs L, uint8_t *pool, int64_t page_words, int64_t parts, int64_t items) {
     constexpr int PART = PG_COPY_THREADS * PG_COPY_WORDS;
     pdl_wait_prior_grid();
@@ -114,7 +115,11 @@ __global__ void __launch_bounds__(PG_COPY_THREADS) pages_copy_kernel(const __gri
 //   outputs  a warp has all rows and 32 dims, a block (ROWT = 4: 64 dims); eight rows' high and low planes are the 16 rows of one product: V's bytes become fp16 once for all rows.  A page's sums are fresh ones, added to the fp32 output by
 //            rounded operations (the tensor core cuts the last bits of a sum off)
 // K and V rows come by one bulk copy each for a page; a page's room is given to the next but one when every warp has left it.
-// Few rows have eight warps: what bounds them is a page's chain of latencies, which is half as long for a warp with one block of dims.
+// Few rows have eight warps: what bounds them is a page's chain of latencies (mma.sync sums, conversions, three barriers; issue slots half full with 16 warps per SM), which is
+// shorter for a warp with one block of dims.  us with append and join: 16 sequences of one token, 28 000 positions in all, 42; 5 tokens at 32700 58 (one page takes a
+// CTA 4 - 4.5 us, its start 5, its end 2.5).  Unrolling the loops over the blocks' pairs or over the steps of 16 positions further is no faster: the code no longer fits the
+// instruction cache beside itself (all unrolled: 512 tokens after 4000 700 us instead of 415).  Planes of dv v8 and of p instead of p dv and v8 (three products for two, a
+// third of the conversions): the same time to 1 % for 16 to 64 rows.
 constexpr int PGA_BUFS = 2;
 constexpr int pga_warps(int rowt) { return rowt == 4 ? 4 : 8; }       // (ROWT = 0: eight rows)
 constexpr int PGA_Q_STRIDE = 64 + 4;                            // words of a quantised row: 4 g + t are 32 different banks
