@@ -1952,7 +1952,7 @@ PagesPlan plan_pages(int n_tok, int max_len, int n_seq, int n_head, int n_head_k
     // beside prompts every split has room for all of their rows, so it is few
     p.most_splits = (int)std::min<int64_t>((pages + 1) / 2, p.tc ? 8 : (PGA_SLOTS + n_head_kv - 1) / n_head_kv);
     const int64_t splits = std::max(p.splits, p.most_splits), part = splits == 1 ? 0 : splits * n_tok * n_head * (KV_D + 2) * (int64_t)sizeof(float);
-    p.part_bytes = (part + 15) / 16 * 16;
+    p.part_bytes = part ? (part + 15) / 16 * 16 + 16 : 0;           // (and the spans that the device finds)
     p.image_bytes = p.tc * pages * n_head_kv * ATC_IMG_BYTES;
     p.redo_bytes = p.tc ? (p.tiles * n_head_kv * p.splits * (int64_t)sizeof(int) + 15) / 16 * 16 : 0;
     return p;
@@ -1969,7 +1969,7 @@ int bonsai_b200_qk_norm_rope(const float *q, const float *k, const float *q_weig
     const int heads = n_head + n_head_kv;
     if (n_tok <= 0 || heads == 0) return 0;
     if (n_tok > INT32_MAX || (n_rot && (!pos || !freq || !aligned4(pos) || !aligned8(freq)))) return 1;
-    QkNormParams P = {{q, k}, {q_weight, k_weight}, {q_out, k_out}, {q_tok_stride, k_tok_stride}, {q_head_stride, k_head_stride}, pos, freq, {n_head, n_head_kv}, head_dim, n_rot, eps};
+    QkNormParams P = {{q, k}, {q_weight, k_weight}, {q_out, k_out}, {q_tok_stride, k_tok_stride}, {q_head_stride, k_head_stride}, pos, freq, {n_head, n_head_kv}, head_dim, n_rot, 1.0f / (float)head_dim, eps};
     bool vec = head_dim % 4 == 0;
     for (int i = 0; i < 2; ++i) {
         if (!P.n_head[i]) continue;
@@ -2038,6 +2038,7 @@ int bonsai_b200_pages_attn(const bonsai_b200_pages *pages, int layer, const floa
         if (plan.part_bytes) {
             P.part_acc = reinterpret_cast<float *>(w + plan.image_bytes + plan.redo_bytes);
             P.part_ml = reinterpret_cast<float2 *>(P.part_acc + (int64_t)std::max(plan.splits, plan.most_splits) * C.n_tok * n_head * KV_D);
+            P.spans = reinterpret_cast<int *>(w + plan.bytes() - 16);
         }
     }
     const cudaStream_t st = as_stream(stream);
@@ -2067,7 +2068,7 @@ int bonsai_b200_pages_attn(const bonsai_b200_pages *pages, int layer, const floa
         const int roww = plan.tc ? 1 : plan.most_splits >= 24 ? 8 : plan.most_splits >= 6 ? 2 : 1;
         const int64_t ctas = ((int64_t)C.n_tok * n_head * roww + PGJ_WARPS - 1) / PGJ_WARPS;
         if (ctas > INT32_MAX) return 1;
-        auto join = [&](auto kernel) { return launch(kernel, dim3((unsigned)ctas), dim3(32 * PGJ_WARPS), 0, st, true, P, PGA_SLOTS); };
+        auto join = [&](auto kernel) { return launch(kernel, dim3((unsigned)ctas), dim3(32 * PGJ_WARPS), 0, st, true, P); };
         e = roww == 8 ? join(pages_join_kernel<8>) : roww == 2 ? join(pages_join_kernel<2>) : join(pages_join_kernel<1>);
     }
     return (int)e;

@@ -21,7 +21,7 @@ struct QkNormParams {
     const int32_t *pos;
     const double *freq;
     int n_head[2], head_dim, n_rot;
-    float eps;
+    float inv_dim, eps;                     // 1 / head_dim
 };
 
 // cos and sin of pos * freq.  Two parts of 2 pi (Cody and Waite's reduction): the rest is exact to 2^-50 for any int32 position and freq <= 1.
@@ -34,8 +34,8 @@ __device__ __forceinline__ float2 rotation_of(int pos, double freq) {
 }
 
 // grid (tokens, groups of heads); a warp has up to PER heads.  VEC: head_dim and the strides are multiples of 4, all pointers 16-byte aligned.
-// Bound by memory: 28 heads of 256 in and out are 57 KB a token, 2000 tokens 115 MB in 26 us (4.4 TB/s of inputs that lie apart).  PER = 4 forms a token's angles once for all
-// heads (a head a warp: the same 26 us, with four times the 64-bit operations); of few tokens a warp has one head, whose chain is shorter.
+// Bound by memory: 28 heads of 256 in and out are 57 KB a token, 2000 tokens 115 MB in 25 us (4.5 TB/s of inputs that lie apart).  PER = 4 forms a token's angles once for all
+// heads (a head a warp: the same time, with four times the 64-bit operations); of few tokens a warp has one head, whose chain is shorter.
 template <bool VEC, int PER>
 __global__ void __launch_bounds__(32 * QKN_MAX_WARPS) qk_norm_rope_kernel(const __grid_constant__ QkNormParams P) {
     __shared__ __align__(16) float rows[QKN_MAX_WARPS][QKN_MAX_DIM];
@@ -46,14 +46,16 @@ __global__ void __launch_bounds__(32 * QKN_MAX_WARPS) qk_norm_rope_kernel(const 
     const int n = P.head_dim, half = P.n_rot >> 1;
     pdl_wait_prior_grid();
     if (PER == 1) pdl_launch_dependents();
+    // (q's heads first, then k's)
+    const float *x0[2] = {P.x[0] + tok * P.tok_stride[0], P.x[1] + tok * P.tok_stride[1]};
+    float *y0[2] = {P.y[0] + tok * P.n_head[0] * n, P.y[1] + tok * P.n_head[1] * n};
     float4 f[PER][2];
 #pragma unroll
     for (int r = 0; r < PER; ++r) {
-        int head = first + warps * r;
+        const int head = first + warps * r;
         if (head < heads) {
-            const int which = head >= P.n_head[0];
-            if (which) head -= P.n_head[0];
-            const float *x = P.x[which] + tok * P.tok_stride[which] + head * P.head_stride[which];
+            const bool second = head >= P.n_head[0];
+            const float *x = second ? x0[1] + (head - P.n_head[0]) * P.head_stride[1] : x0[0] + head * P.head_stride[0];
 #pragma unroll
             for (int j = 0; j < 2; ++j) f[r][j] = rms_load<VEC>(x, 128 * j + 4 * lane, n);
         }
@@ -63,14 +65,16 @@ __global__ void __launch_bounds__(32 * QKN_MAX_WARPS) qk_norm_rope_kernel(const 
     float *row = rows[warp];
 #pragma unroll
     for (int r = 0; r < PER; ++r) {
-        int head = first + warps * r;
+        const int head = first + warps * r;
         if (head >= heads) break;
         const int which = head >= P.n_head[0];
-        if (which) head -= P.n_head[0];
         float4 w[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) w[j] = rms_load<VEC>(P.w[which], 128 * j + 4 * lane, n);
-        const float sc = rms_scale(__fadd_rn(slice_sumsq(f[r][0]), n > 128 ? slice_sumsq(f[r][1]) : 0.0f), n, P.eps);
+        float ss = __fadd_rn(lane_sumsq(f[r][0]), lane_sumsq(f[r][1]));          // (past the end there are zeros)
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) ss = __fadd_rn(ss, __shfl_xor_sync(0xffffffffu, ss, o));
+        const float sc = rsqrtf(__fmaf_rn(ss, P.inv_dim, P.eps));
         if (r) __syncwarp();                            // the row before has been read
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -81,7 +85,7 @@ __global__ void __launch_bounds__(32 * QKN_MAX_WARPS) qk_norm_rope_kernel(const 
             if (128 * j < P.n_rot) reinterpret_cast<float4 *>(row)[32 * j + lane] = f[r][j];
         }
         __syncwarp();
-        float *y = P.y[which] + (tok * P.n_head[which] + head) * n;
+        float *y = y0[which] + (which ? head - P.n_head[0] : head) * n;
         auto turned = [&](int i, float own) {
             if (i >= P.n_rot) return own;
             const bool second = i >= half;

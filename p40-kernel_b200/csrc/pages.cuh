@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(PG_COPY_THREADS) pages_copy_kernel(const __gri
 //            rounded operations (the tensor core cuts the last bits of a sum off)
 // K and V rows come by one bulk copy each for a page; a page's room is given to the next but one when every warp has left it.
 // Few rows have eight warps: what bounds them is a page's chain of latencies (mma.sync sums, conversions, three barriers; issue slots half full with 16 warps per SM), which is
-// shorter for a warp with one block of dims.  us with append and join: 16 sequences of one token, 28 000 positions in all, 42; 5 tokens at 32700 58 (one page takes a
+// shorter for a warp with one block of dims.  us with append and join: 16 sequences of one token, 28 000 positions in all, 39; 5 tokens at 32700 57 (one page takes a
 // CTA 4 - 4.5 us, its start 5, its end 2.5).  Unrolling the loops over the blocks' pairs or over the steps of 16 positions further is no faster: the code no longer fits the
 // instruction cache beside itself (all unrolled: 512 tokens after 4000 700 us instead of 415).  Planes of dv v8 and of p instead of p dv and v8 (three products for two, a
 // third of the conversions): the same time to 1 % for 16 to 64 rows.
@@ -137,6 +137,7 @@ struct PageAttn {
     float *out;
     float *part_acc;            // [splits][token * n_head + head][256], with more than one split
     float2 *part_ml;            // [splits][token * n_head + head]: maximum, sum of weights
+    int *spans;                 // [2] pages of a CTA, of each class below: what pages_attn_kernel found, for the join
     int layer, n_head, group;
     int span, splits;           // of the sequences on the tensor cores: pages of a CTA, CTAs of a tile
     // of the others, in one class or two by their rows, a launch each: rows of a sequence at most, rows of a tile (as a power of two); CTAs of a tile at most
@@ -648,6 +649,7 @@ __global__ void __launch_bounds__(32 * pga_warps(ROWT), 2) pages_attn_kernel(con
     pdl_wait_prior_grid();
     pdl_launch_dependents();
     const int span = pages_span(P, cls, lane, gridDim.x);
+    if (P.spans && blockIdx.x == 0 && threadIdx.x == 0) P.spans[cls] = span;
     const int heads = P.C.n_head_kv;
     __syncthreads();
     int turn = 0;
@@ -713,7 +715,7 @@ __global__ void __launch_bounds__(32 * pga_warps(4), 2) pages_redo_kernel(const 
 // The splits of a row added up: ROWW warps per row (token, head), four dims and four more a lane.  A row's splits are those that its own positions reach.
 constexpr int PGJ_WARPS = 8;
 template <int ROWW>
-__global__ void __launch_bounds__(32 * PGJ_WARPS) pages_join_kernel(const __grid_constant__ PageAttn P, int slots) {
+__global__ void __launch_bounds__(32 * PGJ_WARPS) pages_join_kernel(const __grid_constant__ PageAttn P) {
     __shared__ float4 sums[PGJ_WARPS][2][32];
     __shared__ float2 ml[PGJ_WARPS];
     const PageCache &C = P.C;
@@ -732,7 +734,7 @@ __global__ void __launch_bounds__(32 * PGJ_WARPS) pages_join_kernel(const __grid
                 const int seen = len - r.n + (tok - r.begin) + 1;
                 const int pages = (max(seen, 0) + PG_POS - 1) / PG_POS;
                 const bool tc = pages_on_tc(P, r.n, len);
-                const int span = tc ? P.span : pages_span(P, pages_class(P, r.n), lane, slots);
+                const int span = tc ? P.span : P.spans[pages_class(P, r.n)];
                 n = max(1, min(tc ? P.splits : pages_splits(P, (len + PG_POS - 1) / PG_POS, span), (pages + span - 1) / span));
             }
         }
