@@ -179,15 +179,17 @@ constexpr int GDC_COLS = 48, GDC_NT = GDC_COLS / 8, GDC_SLICES = 3;
 // row strides in bytes of planes in shared memory: 16-byte pieces of eight rows lie in different banks
 constexpr int GDC_KB = GDC_D * 2 + 16, GDC_TB = GDC_T * 2 + 16, GDC_CB = GDC_COLS * 2 + 16;
 constexpr int GDC_KP = GDC_T * GDC_KB, GDC_TP = GDC_T * GDC_TB, GDC_SP = GDC_D * GDC_CB, GDC_UP = GDC_T * GDC_CB;        // a plane of K or Q, Tb or P, S, U
+constexpr int GDC_VS = GDC_COLS + 8;                                  // floats: a row of V
 constexpr int GDC_TS = GDC_T + 4;                                     // floats: a row of A and of its inverse
 constexpr int GDC_STEP_MOST = 24;                                     // tokens of a sequence that go one by one (us, one by one / in chunks: 16 19 / 28, 24 25 / 28, 48 45 / 28.6)
 // What the first two kernels leave, in bytes, planes with the row strides of shared memory so that one bulk copy fetches them: of a chunk and key head the planes of K and Q and
 // the exponents s of their rows' powers of two; of a chunk and value head the planes of Tb and P, then floats: per row e^G 2^-s of K, e^G 2^-s of Q, e^(G_63 - G) 2^(s_min - s) of K,
 // 2^-s of Tb, 2^-s of P; then e^G_63, 2^-s_min, whether the chunk is to go token by token.
 constexpr int GDC_KQ_REC = 4 * GDC_KP + 2 * GDC_T * 4, GDC_TP_PLANES = 4 * GDC_TP, GDC_VEC = 5 * GDC_T + 4, GDC_TP_REC = GDC_TP_PLANES + GDC_VEC * 4;
-constexpr int gdc_prep_smem() { return 4 * GDC_KP + GDC_T * 8 + 3 * GDC_T * 4 + 32; }
-constexpr int gdc_scan_smem() { return 6 * GDC_KP + 4 * GDC_TP + GDC_T * GDC_COLS * 4 + 2 * GDC_SP + 4 * GDC_UP + GDC_VEC * 4 + 5 * 8 * 4 + 4 * 8; }
-static_assert(2 * GDC_UP <= 2 * GDC_KP && GDC_D * GDC_CB * 2 >= GDC_D * GDC_COLS * 4 && 2 * GDC_T * GDC_TS * 4 <= 2 * GDC_KP, "");
+constexpr int GDC_QB = 16 * GDC_KB;                                    // 16 rows of a plane of Q
+constexpr int gdc_prep_smem() { return 2 * GDC_KP + 4 * GDC_QB + GDC_T * 8 + 3 * GDC_T * 4 + 32; }
+constexpr int gdc_scan_smem() { return 6 * GDC_KP + 4 * GDC_TP + GDC_T * GDC_VS * 4 + 2 * GDC_SP + 6 * GDC_UP + GDC_VEC * 4 + 5 * 8 * 4 + 4 * 8; }
+static_assert(gdc_scan_smem() <= 227 * 1024 && 4 * gdc_prep_smem() <= 224 * 1024 && GDC_D * GDC_CB * 2 >= GDC_D * GDC_COLS * 4 && 2 * GDC_T * GDC_TS * 4 <= 2 * GDC_KP, "");
 
 __device__ __forceinline__ int gdc_chunks(int n) { return n > GDC_STEP_MOST ? (n + GDC_T - 1) / GDC_T : 0; }
 
@@ -214,10 +216,12 @@ __device__ __forceinline__ void gdc_mma(float (&c)[4], const uint32_t (&a)[4], u
 // c[m] = A[m] B over 16 STEPS values, each A 16 rows, B 8 NT columns.  a[m], b: the lane's addresses of the high planes, the low ones a_low and b_low behind, a step a_step and
 // b_step behind the one before; of a pair of column tiles b_pair.  AT: A lies by columns; BT: B lies by rows.
 template <int MT, int NT, int STEPS, bool AT, bool BT>
-__device__ __forceinline__ void gdc_product(float (&c)[MT][NT][4], const uint32_t (&a)[MT], uint32_t a_low, uint32_t a_step, uint32_t b, uint32_t b_low, uint32_t b_step, uint32_t b_pair) {
+__device__ __forceinline__ void gdc_product(float (&c)[MT][NT][4], const uint32_t (&a)[MT], uint32_t a_low, uint32_t a_step, uint32_t b, uint32_t b_low, uint32_t b_step, uint32_t b_pair,
+                                            int steps = STEPS) {
     constexpr int PAIRS = (NT + 1) / 2;
 #pragma unroll
     for (int k = 0; k < STEPS; ++k) {
+        if (k >= steps) break;
         uint32_t ah[MT][4], al[MT][4], bh[PAIRS][4], bl[PAIRS][4];
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
@@ -293,16 +297,16 @@ __global__ void __launch_bounds__(GDC_THREADS) gdn_planes_kernel(const __grid_co
     }
 }
 
-// grid (the same chunks, value heads): Tb and P.  Bound by issue and latency with 12 warps per SM (what a CTA's planes leave room for): 75 us for 2048 tokens and 48 heads, 5000
-// instructions a warp: products 700, decays 1000, the inverse 2000, planes of the results 1400.
-__global__ void __launch_bounds__(GDC_PREP_THREADS, 3) gdn_chunk_kernel(const __grid_constant__ GdnSeqs P, const uint8_t *kq_recs, uint8_t *tp_recs) {
+// grid (the same chunks, value heads): Tb and P.  Bound by issue and latency: 59 us for 2048 tokens and 48 heads, four CTAs per SM, whose rounds are three (with all of Q in
+// shared memory and P passing through it, three CTAs, four rounds, 75 us).  About 3900 instructions a warp, half of them the inverse.
+__global__ void __launch_bounds__(GDC_PREP_THREADS, 4) gdn_chunk_kernel(const __grid_constant__ GdnSeqs P, const uint8_t *kq_recs, uint8_t *tp_recs) {
     extern __shared__ __align__(16) uint8_t gdc_smem[];
-    uint8_t *kp = gdc_smem, *qp = kp + 2 * GDC_KP;
-    float *at = reinterpret_cast<float *>(kp), *tt = at + GDC_T * GDC_TS, *pt = reinterpret_cast<float *>(qp);      // when the planes have been read
-    double *gs = reinterpret_cast<double *>(qp + 2 * GDC_KP);
+    uint8_t *kp = gdc_smem, *qp = kp + 2 * GDC_KP;                           // Q: 16 rows of both planes of each of two warps
+    float *at = reinterpret_cast<float *>(kp), *tt = at + GDC_T * GDC_TS;    // when the planes of K have been read
+    double *gs = reinterpret_cast<double *>(qp + 4 * GDC_QB);
     float *bs = reinterpret_cast<float *>(gs + GDC_T);
     int *shift = reinterpret_cast<int *>(bs + GDC_T);                        // [2][64] of K, of Q
-    uint64_t *full = reinterpret_cast<uint64_t *>(shift + 2 * GDC_T);
+    uint64_t *full = reinterpret_cast<uint64_t *>(shift + 2 * GDC_T);       // K and its Q; the other 16 rows of Q of each of the two warps
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     constexpr int WARPS = GDC_PREP_THREADS / 32;
     const int vh = blockIdx.y, share = P.n_v_heads / P.n_k_heads, kh = vh / share;
@@ -317,13 +321,20 @@ __global__ void __launch_bounds__(GDC_PREP_THREADS, 3) gdn_chunk_kernel(const __
     uint8_t *rec = tp_recs + ((size_t)blockIdx.x * P.n_v_heads + vh) * GDC_TP_REC;
     float *vec = reinterpret_cast<float *>(rec + GDC_TP_PLANES);
     bool odd = false;                           // something that sums may not hold: the chunk goes token by token
+    const uint64_t pol = policy_evict_normal();
+    const bool of_q = warp >= 2;
+    const int top = warp & 1;
+    auto load_q = [&](int w, int m, uint64_t *bar) {
+        for (int p = 0; p < 2; ++p) bulk_g2s(qp + (2 * w + p) * GDC_QB, kq + (2 + p) * GDC_KP + m * GDC_QB, GDC_QB, bar, pol);
+    };
     if (tid == 0) {
-        const uint64_t pol = policy_evict_normal();
-        mbar_init(full, 1);
+        for (int b = 0; b < 3; ++b) mbar_init(full + b, 1);
         mbar_fence_init();
-        mbar_expect_tx(full, GDC_KQ_REC);
-        bulk_g2s(kp, kq, 4 * GDC_KP, full, pol);
+        mbar_expect_tx(full, 2 * GDC_KP + 2 * GDC_T * 4 + 4 * GDC_QB);
+        bulk_g2s(kp, kq, 2 * GDC_KP, full, pol);
         bulk_g2s(shift, kq + 4 * GDC_KP, 2 * GDC_T * 4, full, pol);
+        load_q(0, 0, full);
+        load_q(1, 1, full);
     }
     if (warp == 0) {
         // a decay below e^-1000 is none; sums in 64 bits: of two that are far from zero the difference matters
@@ -350,21 +361,30 @@ __global__ void __launch_bounds__(GDC_PREP_THREADS, 3) gdn_chunk_kernel(const __
     if (!__syncthreads_and(mbar_wait_hot(full, 0) ? 1 : 0)) return;          // (a wait ran out: the CTA leaves as a whole)
     // ---- K K^T (two warps) and Q K^T, blocks of 16 x 16 on and below the diagonal: a warp has rows of blocks w and 3 - w, five blocks
     float c[5][1][2][4];
-    const bool of_q = warp >= 2;
+    bool ok = true;
     {
-        const uint32_t a0 = smem_u32(of_q ? qp : kp) + gdc_at_rows(lane, GDC_KB), b0 = smem_u32(kp) + gdc_at_turned(lane, GDC_KB);
+        const uint32_t a_k = smem_u32(kp) + gdc_at_rows(lane, GDC_KB), a_q = smem_u32(qp) + 2 * top * GDC_QB + gdc_at_rows(lane, GDC_KB), b0 = smem_u32(kp) + gdc_at_turned(lane, GDC_KB);
 #pragma unroll
         for (int i = 0; i < 5; ++i) {
-            const int top = warp & 1, m = i <= top ? top : 3 - top, j = i <= top ? i : i - top - 1;
-            const uint32_t a[1] = {a0 + 16 * m * GDC_KB};
-            gdc_product<1, 2, GDC_D / 16, false, false>(c[i], a, GDC_KP, 32, b0 + 16 * j * GDC_KB, GDC_KP, 32, 0);
+            const int m = i <= top ? top : 3 - top, j = i <= top ? i : i - top - 1;
+            if (of_q && i == top + 1) {                                     // the rows of Q of the second row of blocks, in the place of the first's
+                __syncwarp();
+                if (lane == 0) {
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    mbar_expect_tx(full + 1 + top, 2 * GDC_QB);
+                    load_q(top, m, full + 1 + top);
+                }
+                ok = mbar_wait_hot(full + 1 + top, 0);
+            }
+            const uint32_t a[1] = {of_q ? a_q : a_k + 16 * m * GDC_KB};
+            gdc_product<1, 2, GDC_D / 16, false, false>(c[i], a, of_q ? GDC_QB : GDC_KP, 32, b0 + 16 * j * GDC_KB, GDC_KP, 32, 0);
         }
     }
-    __syncthreads();                            // the planes have been read: A, its inverse and P in fp32 take their place
+    if (!__syncthreads_and(ok ? 1 : 0)) return; // the planes have been read: A and its inverse in fp32 take the place of K's
     if (tid < GDC_T) odd = odd || min(shift[tid], shift[GDC_T + tid]) <= 141 - (int)(ATC_HUGE >> 23);
 #pragma unroll
     for (int i = 0; i < 5; ++i) {
-        const int top = warp & 1, m = i <= top ? top : 3 - top, jb = i <= top ? i : i - top - 1;
+        const int m = i <= top ? top : 3 - top, jb = i <= top ? i : i - top - 1;
         double gr[2], gc[4];                    // of the lane's two rows and four columns: sums of g, factors
         float fr[2], fc[4];
 #pragma unroll
@@ -387,7 +407,43 @@ __global__ void __launch_bounds__(GDC_PREP_THREADS, 3) gdn_chunk_kernel(const __
             float x = __fmul_rn(__fmul_rn(__fmul_rn(c[i][0][e >> 2][e & 3], fr[h]), fc[v]), expf((float)(gr[h] - gc[v])));
             if (col > row || (!of_q && col == row)) x = 0.0f;
             odd = odd || !(fabsf(x) < 1e30f);
-            (of_q ? pt : at)[row * GDC_TS + col] = x;
+            if (of_q) c[i][0][e >> 2][e & 3] = x;
+            else at[row * GDC_TS + col] = x;
+        }
+    }
+    if (of_q) {
+        // planes of P: a row lies in four lanes.  (Blocks above the diagonal are not read.)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int m = half ? 3 - top : top;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t most = 0u;
+#pragma unroll
+                for (int i = 0; i < 5; ++i)
+                    if ((i > top) == (half != 0))
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) most = max(most, atc_abs_bits(c[i][0][v >> 1][2 * h + (v & 1)]));
+                most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                odd = odd || most >= ATC_HUGE;
+                const int s = atc_shift(most, 63), row = 16 * m + g + 8 * h;
+                const float f = atc_pow2(s);
+                uint8_t *out = rec + 2 * GDC_TP + row * GDC_TB + 4 * t;
+#pragma unroll
+                for (int i = 0; i < 5; ++i)
+                    if ((i > top) == (half != 0)) {
+                        const int jb = i <= top ? i : i - top - 1;
+#pragma unroll
+                        for (int v = 0; v < 2; ++v) {
+                            uint32_t hi, lo;
+                            split_f16x2(__fmul_rn(c[i][0][v][2 * h], f), __fmul_rn(c[i][0][v][2 * h + 1], f), hi, lo);
+                            *reinterpret_cast<uint32_t *>(out + 32 * jb + 16 * v) = hi;
+                            *reinterpret_cast<uint32_t *>(out + 32 * jb + 16 * v + GDC_TP) = lo;
+                        }
+                    }
+                if (t == 0) vec[4 * GDC_T + row] = atc_pow2(-s);
+            }
         }
     }
     __syncthreads();
@@ -449,15 +505,14 @@ __global__ void __launch_bounds__(GDC_PREP_THREADS, 3) gdn_chunk_kernel(const __
         }
         __syncthreads();
     }
-    // ---- planes of Tb and P: a warp per row, lane = two values
+    // ---- planes of Tb: a warp per row, lane = two values
 #pragma unroll 4
-    for (int r = warp; r < 2 * GDC_T; r += WARPS) {
-        const int row = r & (GDC_T - 1), col = 2 * lane;
-        const bool there = (col >> 4) <= (row >> 4);
+    for (int row = warp; row < GDC_T; row += WARPS) {
+        const int col = 2 * lane;
         float2 x = make_float2(0.0f, 0.0f);
-        if (there) {
-            x = *reinterpret_cast<const float2 *>((r < GDC_T ? tt : pt) + row * GDC_TS + col);
-            if (r < GDC_T) x = make_float2(__fmul_rn(x.x, bs[col]), __fmul_rn(x.y, bs[col + 1]));
+        if ((col >> 4) <= (row >> 4)) {
+            x = *reinterpret_cast<const float2 *>(tt + row * GDC_TS + col);
+            x = make_float2(__fmul_rn(x.x, bs[col]), __fmul_rn(x.y, bs[col + 1]));
         }
         const uint32_t m = __reduce_max_sync(0xffffffffu, max(atc_abs_bits(x.x), atc_abs_bits(x.y)));
         odd = odd || m >= ATC_HUGE;
@@ -465,10 +520,10 @@ __global__ void __launch_bounds__(GDC_PREP_THREADS, 3) gdn_chunk_kernel(const __
         const float f = atc_pow2(s);
         uint32_t hi, lo;
         split_f16x2(__fmul_rn(x.x, f), __fmul_rn(x.y, f), hi, lo);
-        uint8_t *out = rec + (r < GDC_T ? 0 : 2 * GDC_TP) + row * GDC_TB + 4 * lane;
+        uint8_t *out = rec + row * GDC_TB + 4 * lane;
         *reinterpret_cast<uint32_t *>(out) = hi;
         *reinterpret_cast<uint32_t *>(out + GDC_TP) = lo;
-        if (lane == 0) vec[3 * GDC_T + r] = atc_pow2(-s);
+        if (lane == 0) vec[3 * GDC_T + row] = atc_pow2(-s);
     }
     int least = 63;                             // K's smallest shift
 #pragma unroll
@@ -490,23 +545,24 @@ __global__ void __launch_bounds__(GDC_PREP_THREADS, 3) gdn_chunk_kernel(const __
     if (tid == 0) vec[5 * GDC_T + 2] = any ? 1.0f : 0.0f;
 }
 
-// A chunk is a chain: K S and Q S | V - e^G K S scaled | U | U scaled | K^T U and P U | S scaled, with a barrier between any two, on eight warps: 11 600 cycles, of which the tensor
-// core's products are 4500 (counted in a run of 32 chunks; K S and Q S 2300, U 1080, the last two 2200, the scalings and their maxima 2900, copies and waits 1900).  What was worth it:
-// products by fp16 planes instead of TF32 parts (389 -> 317 us of the scan over 2048 tokens), powers of two by eight columns instead of one and bulk copies (-> 249), tokens' rows and half of the
-// columns to a warp (-> 216).  Three slices of the columns put 144 CTAs on 148 SMs; two would leave a third of them idle, four make the fuller SMs do two.
-// grid (value heads x 3, sequences): columns 0 .. 47, 48 .. 87, 88 .. 127.  Warp w of eight: tokens 16 (w % 4) .. and half of the columns of all that has a row for each
+// A chunk is a chain: K S | V - e^G K S scaled | U, and Q S beside it | U scaled | K^T U and P U | S scaled, with a barrier between any two, on eight warps: about 10 800 cycles, of which
+// the tensor core's products are 4200; shared memory's pipe is half busy.  What was worth it, in us of the scan over 2048 tokens: products by fp16 planes instead of TF32 parts
+// (389 -> 317), powers of two by eight columns instead of one and bulk copies (-> 249), tokens' rows and half of the columns to a warp (-> 216), no blocks above the
+// diagonals and rows of V in different banks (-> 209), Q S behind U (-> 204).  What was not: eight more warps for Q S, P U and V's copies beside the chain (they share its pipes: 216 -> 225), the
+// next chunk's Tb ahead of time, with a barrier less (204 -> 209).  Three slices of the columns put 144 CTAs on 148 SMs; two would leave a third of them idle, four make the
+// fuller SMs do two.
+// grid (value heads x 3, sequences): columns 0 .. 47, 48 .. 87, 88 .. 127.  Warp w of eight: 16 of the tokens and half of the columns of all that has a row for each
 // token, and rows 16 w .. of the state, which stay in registers in fp32; its planes in shared memory are what the products read.
 __global__ void __launch_bounds__(GDC_THREADS, 1) gdn_scan_kernel(const __grid_constant__ GdnSeqs P, const uint8_t *kq_recs, const uint8_t *tp_recs, int n_chunks) {
     extern __shared__ __align__(16) uint8_t gdc_smem[];
-    uint8_t *kp0 = gdc_smem, *qp = kp0 + 4 * GDC_KP, *tp = qp + 2 * GDC_KP, *sp = tp + 4 * GDC_TP, *up = sp + 2 * GDC_SP;       // K twice; Tb, P; U, U times its factors
-    uint8_t *rp = qp;                                                   // V - e^G K S takes the place of Q when that has been read
-    float *vt = reinterpret_cast<float *>(up + 4 * GDC_UP), *vec = vt + GDC_T * GDC_COLS;
+    uint8_t *kp0 = gdc_smem, *qp = kp0 + 4 * GDC_KP, *tp = qp + 2 * GDC_KP, *sp = tp + 4 * GDC_TP, *up = sp + 2 * GDC_SP, *rp = up + 4 * GDC_UP;       // K twice; Q; Tb, P; S; U, U times its factors; V - e^G K S
+    float *vt = reinterpret_cast<float *>(rp + 2 * GDC_UP), *vec = vt + GDC_T * GDC_VS;
     uint32_t *s_most = reinterpret_cast<uint32_t *>(vec + GDC_VEC), *r_most = s_most + 2 * 8, *u_most = r_most + 8;          // largest magnitudes of eight columns: S's of this chunk and of the next; U's, U's times its factors
     uint64_t *kfull = reinterpret_cast<uint64_t *>(u_most + 2 * 8), *qvfull = kfull + 2, *tpfull = kfull + 3;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int vh = blockIdx.x / GDC_SLICES, slice = blockIdx.x % GDC_SLICES, s = blockIdx.y;
     const int c0 = slice == 0 ? 0 : 48 + 40 * (slice - 1), cols = slice == 0 ? 48 : 40;
-    const int kh = vh / (P.n_v_heads / P.n_k_heads), mt = warp & 3;
+    const int kh = vh / (P.n_v_heads / P.n_k_heads), mt = warp < 4 ? warp : 7 - warp;           // (a scheduler's two warps: as many steps of Tb and P as any other's)
     pdl_wait_prior_grid();
     pdl_launch_dependents();
     const SeqRange range = seq_range(P.start, s, P.n_tok);
@@ -554,7 +610,7 @@ __global__ void __launch_bounds__(GDC_THREADS, 1) gdn_scan_kernel(const __grid_c
         }
 #pragma unroll
         for (int e = 0; e < 3; ++e) {
-            float *dst = vt + v_row[e] * GDC_COLS + v_col[e];
+            float *dst = vt + v_row[e] * GDC_VS + v_col[e];
             const float *x = src + (size_t)v_row[e] * vstride + v_col[e];
             if (v_row[e] >= n || v_col[e] >= cols) *reinterpret_cast<float4 *>(dst) = make_float4(0.f, 0.f, 0.f, 0.f);
             else if (vvec) cp_async16(dst, x);
@@ -628,14 +684,14 @@ __global__ void __launch_bounds__(GDC_THREADS, 1) gdn_scan_kernel(const __grid_c
             load_k(c + 1);
         }
         if (tid < 8) r_most[tid] = u_most[tid] = u_most[tid + 8] = next[tid] = 0u;
-        // ---- K S and Q S
-        float acc[2][NH][4];
+        // ---- V - e^G K S
+        float r[1][NH][4], y[1][NH][4];
         {
-            const uint32_t a[2] = {kb + 16 * mt * GDC_KB + at_k, smem_u32(qp) + 16 * mt * GDC_KB + at_k};
-            gdc_product<2, NH, GDC_D / 16, false, true>(acc, a, GDC_KP, 32, b_s + 16 * j0, GDC_SP, 16 * GDC_CB, 32);
+            const uint32_t a[1] = {kb + 16 * mt * GDC_KB + at_k};
+            gdc_product<1, NH, GDC_D / 16, false, true>(r, a, GDC_KP, 32, b_s + 16 * j0, GDC_SP, 16 * GDC_CB, 32);
         }
         ok = mbar_wait_hot(tpfull, (uint32_t)(c & 1)) && ok;
-        if (!__syncthreads_and(ok ? 1 : 0)) return;             // Tb, P and the factors; the planes of Q have been read
+        if (!__syncthreads_and(ok ? 1 : 0)) return;             // Tb, P and the factors
         bool odd = vec[5 * GDC_T + 2] != 0.0f;
 #pragma unroll
         for (int j = 0; j < NH; ++j) {
@@ -643,32 +699,43 @@ __global__ void __launch_bounds__(GDC_THREADS, 1) gdn_scan_kernel(const __grid_c
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int i = 16 * mt + g + 8 * h;
-                const float fk = vec[i], fq = vec[GDC_T + i];
-                const float2 v = *reinterpret_cast<const float2 *>(vt + i * GDC_COLS + 8 * (j0 + j) + 2 * t);
+                const float fk = vec[i];
+                const float2 v = *reinterpret_cast<const float2 *>(vt + i * GDC_VS + 8 * (j0 + j) + 2 * t);
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float &x = acc[0][j][2 * h + e], &y = acc[1][j][2 * h + e];
-                    x = __fsub_rn(e ? v.y : v.x, __fmul_rn(__fmul_rn(x, fs), fk));          // V - e^G K S
-                    y = __fmul_rn(__fmul_rn(y, fs), fq);                                    // e^G Q S
-                    odd = odd || !(fabsf(x) < 0x1p60f) || !(fabsf(y) < 0x1p60f);
+                    float &x = r[0][j][2 * h + e];
+                    x = __fsub_rn(e ? v.y : v.x, __fmul_rn(__fmul_rn(x, fs), fk));
+                    odd = odd || !(fabsf(x) < 0x1p60f);
                 }
             }
         }
-        tiles_most(acc[0], r_most + j0);
+        tiles_most(r[0], r_most + j0);
         int slow = __syncthreads_or(odd ? 1 : 0);
 #pragma unroll
         for (int j = 0; j < NH; ++j) {
             const float f = atc_pow2(atc_shift(r_most[j0 + j], 63));
 #pragma unroll
-            for (int h = 0; h < 2; ++h) store_planes(rp + (16 * mt + g + 8 * h) * GDC_CB + 16 * (j0 + j) + 4 * t, GDC_UP, acc[0][j][2 * h], acc[0][j][2 * h + 1], f);
+            for (int h = 0; h < 2; ++h) store_planes(rp + (16 * mt + g + 8 * h) * GDC_CB + 16 * (j0 + j) + 4 * t, GDC_UP, r[0][j][2 * h], r[0][j][2 * h + 1], f);
         }
         __syncthreads();
         // ---- U = Tb (V - e^G K S); x: the same times the factors of the state's update
         {
             float u[1][NH][4], x[NH][4];
             const uint32_t a[1] = {smem_u32(tp) + 16 * mt * GDC_TB + at_t};
-            gdc_product<1, NH, GDC_T / 16, false, true>(u, a, GDC_TP, 32, b_r + 16 * j0, GDC_UP, 16 * GDC_CB, 32);
+            gdc_product<1, NH, GDC_T / 16, false, true>(u, a, GDC_TP, 32, b_r + 16 * j0, GDC_UP, 16 * GDC_CB, 32, mt + 1);
             odd = false;
+            // e^G Q S here, between products that the whole chunk waits for: its instructions fill their latencies (2048 tokens: beside K S 277 us, here 272)
+            const uint32_t aq[1] = {smem_u32(qp) + 16 * mt * GDC_KB + at_k};
+            gdc_product<1, NH, GDC_D / 16, false, true>(y, aq, GDC_KP, 32, b_s + 16 * j0, GDC_SP, 16 * GDC_CB, 32);
+#pragma unroll
+            for (int j = 0; j < NH; ++j) {
+                const float fs = atc_pow2(-atc_shift(most[j0 + j], 63));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    y[0][j][e] = __fmul_rn(__fmul_rn(y[0][j][e], fs), vec[GDC_T + 16 * mt + g + 8 * (e >> 1)]);
+                    odd = odd || !(fabsf(y[0][j][e]) < 0x1p60f);
+                }
+            }
 #pragma unroll
             for (int j = 0; j < NH; ++j) {
                 const float fr = atc_pow2(-atc_shift(r_most[j0 + j], 63));
@@ -682,7 +749,7 @@ __global__ void __launch_bounds__(GDC_THREADS, 1) gdn_scan_kernel(const __grid_c
             }
             tiles_most(u[0], u_most + j0);
             tiles_most(x, u_most + 8 + j0);
-            slow |= __syncthreads_or(odd ? 1 : 0);              // (V - e^G K S, in the place of Q, has been read)
+            slow |= __syncthreads_or(odd ? 1 : 0);              // (Q and V - e^G K S have been read)
 #pragma unroll
             for (int j = 0; j < NH; ++j) {
                 const float fu = atc_pow2(atc_shift(u_most[j0 + j], 63)), fx = atc_pow2(atc_shift(u_most[8 + j0 + j], 63));
@@ -703,7 +770,7 @@ __global__ void __launch_bounds__(GDC_THREADS, 1) gdn_scan_kernel(const __grid_c
                 float d[1][GDC_NT][4];
                 const uint32_t a[1] = {kb + 32 * warp + at_kt}, ap[1] = {smem_u32(tp) + 2 * GDC_TP + 16 * mt * GDC_TB + at_t};
                 gdc_product<1, GDC_NT, GDC_T / 16, true, true>(d, a, GDC_KP, 16 * GDC_KB, b_u + 2 * GDC_UP, GDC_UP, 16 * GDC_CB, 32);
-                gdc_product<1, NH, GDC_T / 16, false, true>(o, ap, GDC_TP, 32, b_u + 16 * j0, GDC_UP, 16 * GDC_CB, 32);
+                gdc_product<1, NH, GDC_T / 16, false, true>(o, ap, GDC_TP, 32, b_u + 16 * j0, GDC_UP, 16 * GDC_CB, 32, mt + 1);
                 const float decay = vec[5 * GDC_T], kf = vec[5 * GDC_T + 1];
 #pragma unroll
                 for (int j = 0; j < GDC_NT; ++j) {
@@ -723,8 +790,8 @@ __global__ void __launch_bounds__(GDC_THREADS, 1) gdn_scan_kernel(const __grid_c
                         const float f = vec[4 * GDC_T + i];
                         if (i < n && 8 * (j0 + j) < cols) {
                             float *dst = P.out + ((tok + i) * P.n_v_heads + vh) * GDC_D + c0 + 8 * (j0 + j) + 2 * t;
-                            dst[0] = __fmaf_rn(__fmul_rn(o[0][j][2 * h], f), fu, acc[1][j][2 * h]);
-                            dst[1] = __fmaf_rn(__fmul_rn(o[0][j][2 * h + 1], f), fu, acc[1][j][2 * h + 1]);
+                            dst[0] = __fmaf_rn(__fmul_rn(o[0][j][2 * h], f), fu, y[0][j][2 * h]);
+                            dst[1] = __fmaf_rn(__fmul_rn(o[0][j][2 * h + 1], f), fu, y[0][j][2 * h + 1]);
                         }
                     }
                 }
@@ -754,7 +821,7 @@ __global__ void __launch_bounds__(GDC_THREADS, 1) gdn_scan_kernel(const __grid_c
                 if (part < 5) {
                     float x = 0.0f;
                     for (int p = 0; p < 5; ++p) x = __fadd_rn(x, x1[p * GDC_COLS + col]);
-                    const float d = __fsub_rn(vt[i * GDC_COLS + col], x);
+                    const float d = __fsub_rn(vt[i * GDC_VS + col], x);
                     x = 0.0f;
                     for (int r = part; r < GDC_D; r += 5) {
                         const float y = __fadd_rn(st[r * GDC_COLS + col], __fmul_rn(__fmul_rn(beta, k[r]), d));
