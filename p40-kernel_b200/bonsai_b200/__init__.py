@@ -422,13 +422,19 @@ class Pages:
                               table.shape[1], n_tok)
         self._p = C.addressof(self._s)
         self.page_bytes, self.n_pages, self.n_seq, self.n_tok = page, pool.numel() // page, n_seq, n_tok
+        self._here, self._device = torch.cuda.current_device, pool.device.index
+
+    def _struct(self):
+        if self._here() != self._device:
+            raise RuntimeError(f"the cache is on device {self._device}, the current device is {self._here()}")
+        return self._p
 
     def append(self, layer, k, v):
-        return _native().pages_append(self._p, layer, k, v)
+        return _native().pages_append(self._struct(), layer, k, v)
 
     def attn_workspace(self, max_len, n_head):
         return pages_attn_workspace(self.n_tok, max_len, self.n_seq, n_head, self._s.n_head_kv)
 
     def attn(self, layer, q, out, n_head, max_len, workspace, scale):
         """workspace: a tensor of attn_workspace(max_len, n_head) bytes, or None where that is 0."""
-        return _native().pages_attn(self._p, layer, q, out, n_head, max_len, workspace, 0 if workspace is None else workspace.nbytes, scale)
+        return _native().pages_attn(self._struct(), layer, q, out, n_head, max_len, workspace, 0 if workspace is None else workspace.nbytes, scale)

@@ -2016,7 +2016,9 @@ int bonsai_b200_pages_attn(const bonsai_b200_pages *pages, int layer, const floa
     if (!q || !out || !aligned4(q) || !aligned4(out) || !pages_attn_sizes(C.n_tok, max_len, C.n_seq, n_head, C.n_head_kv)) return 1;
     const PagesPlan plan = plan_pages(C.n_tok, max_len, C.n_seq, n_head, C.n_head_kv);
     if (2 * plan.tiles > INT32_MAX || plan.tc * plan.max_pages > INT32_MAX) return 1;
-    if (((int64_t)C.n_tok * (n_head / C.n_head_kv) / 8 + C.n_seq) * plan.most_splits * C.n_head_kv > INT32_MAX) return 1;
+    const int64_t most_items = ((int64_t)C.n_tok * (n_head / C.n_head_kv) / 8 + C.n_seq) * plan.most_splits * C.n_head_kv;
+    if (most_items > INT32_MAX) return 1;
+    P.most_items = (uint32_t)most_items;
     P.q = q;
     P.out = out;
     P.layer = layer;

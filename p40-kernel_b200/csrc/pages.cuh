@@ -40,6 +40,7 @@ __global__ void __launch_bounds__(32 * KV_APPEND_WARPS) pages_append_kernel(cons
     float kx[8], vx[8];
     pdl_wait_prior_grid();
     pdl_launch_dependents();
+    if (blockIdx.x == 0) report_ranges(C.start, C.n_seq, C.n_tok);
     const int s = seq_of_row(C.start, C.n_seq, tok, lane);
     if (VEC) {
         const float4 a = *reinterpret_cast<const float4 *>(kr), b = *reinterpret_cast<const float4 *>(kr + 4);
@@ -142,6 +143,7 @@ struct PageAttn {
     int span, splits;           // of the sequences on the tensor cores: pages of a CTA, CTAs of a tile
     // of the others, in one class or two by their rows, a launch each: rows of a sequence at most, rows of a tile (as a power of two); CTAs of a tile at most
     int most_rows[2], row_shift[2], most_splits;
+    uint32_t most_items;        // that a launch of theirs can have: more are rows that several sequences claim, and not served
     float scale;
     // the call's long sequences on the tensor cores (pages_tc.cuh): images [sequence][page][kv head], whether a CTA is to be done again [tile][kv head][split]
     uint8_t *images;
@@ -650,25 +652,27 @@ __global__ void __launch_bounds__(32 * pga_warps(ROWT), 2) pages_attn_kernel(con
     pdl_launch_dependents();
     const int span = pages_span(P, cls, lane, gridDim.x);
     if (P.spans && blockIdx.x == 0 && threadIdx.x == 0) P.spans[cls] = span;
+    if (cls == 0 && blockIdx.x == gridDim.x - 1) report_ranges(P.C.start, P.C.n_seq, P.C.n_tok);
     const int heads = P.C.n_head_kv;
     __syncthreads();
     int turn = 0;
-    for (int item = blockIdx.x;; item += gridDim.x) {
-        // whose: the sequences' items one after the other, every warp for itself (the host has seen that they are countable)
-        int before = 0;
+    for (uint32_t item = blockIdx.x; item < P.most_items; item += gridDim.x) {
+        // whose: the sequences' items one after the other, every warp for itself (a sequence has most_items at most, below 2^31; where several claim rows, sums stop there)
+        uint32_t before = 0;
         PageItem<ROWT> I = {-1, 0, 0, 0, 0, 0};
         for (int base = 0; base < P.C.n_seq && I.seq < 0; base += 32) {
             const SeqWork w = pages_work(P, base + lane, cls);
-            const int splits = pages_splits(P, w.pages, span), own = w.tiles * splits * heads;
-            int sum = own;
+            const int splits = pages_splits(P, w.pages, span);
+            uint32_t sum = (uint32_t)(w.tiles * splits * heads);
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const int x = __shfl_up_sync(0xffffffffu, sum, o);
-                if (lane >= o) sum += x;
+                const uint32_t x = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum = min(sum + x, (uint32_t)INT32_MAX);
             }
             const unsigned past = __ballot_sync(0xffffffffu, before + sum > item);
+            const uint32_t front = __shfl_up_sync(0xffffffffu, sum, 1);
             if (past) {
-                const int at = __ffs(past) - 1, rest = item - before - __shfl_sync(0xffffffffu, sum - own, at), n = __shfl_sync(0xffffffffu, splits, at);
+                const int at = __ffs(past) - 1, rest = (int)(item - before - __shfl_sync(0xffffffffu, lane ? front : 0u, at)), n = __shfl_sync(0xffffffffu, splits, at);
                 const int pair = rest / heads;
                 I.seq = base + at;
                 I.kvh = rest - pair * heads;

@@ -16,6 +16,12 @@ __device__ __forceinline__ SeqRange seq_range(const int32_t *start, int s, int n
     return {a, 0 <= a && a <= b && b <= n_tok ? b - a : -1};
 }
 
+// A CTA says so where a sequence's numbers are not rows of the call.
+__device__ __forceinline__ void report_ranges(const int32_t *start, int n_seq, int n_tok) {
+    for (int s = threadIdx.x; s < n_seq; s += blockDim.x)
+        if (seq_range(start, s, n_tok).n < 0) bad_sequence();
+}
+
 // The first sequence whose rows end behind row `tok`, found by a warp, 32 sequences a step.  n_seq: none, the row is nobody's.
 __device__ __forceinline__ int seq_of_row(const int32_t *start, int n_seq, int tok, int lane) {
     for (int base = 0; base < n_seq; base += 32) {

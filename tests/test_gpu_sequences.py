@@ -386,6 +386,50 @@ def test_numbers_that_do_not_fit_stop_their_sequence(gpu, new, max_len):
     start[2], start[3] = a - 1, 2 ** 31 - 1             # rows that run backwards, and past the call
     out = run_attention(gpu, c, q, max_len=max_len)
     assert torch.equal(out[:a], clean[:a]) and bool((out[a:] == 7).all())
+    assert gpu.device_status() == 3 and gpu.clear_status() == 0
+
+
+def test_rows_that_run_backwards_are_reported(gpu):
+    """Starts of which one sequence's run backwards, and no row is left to it: the status word says so, in every call."""
+    import torch
+    c = Cache(gpu, [300, 200, 150], [3, 3, 3], seed=15)
+    c.view._keep[3].copy_(ints([0, 5, 3, 9]))
+    q = torch.randn(c.n_tok, 24, 256, device="cuda")
+    k, v = torch.randn(c.n_tok, 4, 256, device="cuda"), torch.randn(c.n_tok, 4, 256, device="cuda")
+    assert gpu.clear_status() == 0 and c.view.append(0, k, v) == 0
+    assert gpu.device_status() == 3 and gpu.clear_status() == 0
+    run_attention(gpu, c, q)
+    assert gpu.device_status() == 3 and gpu.clear_status() == 0
+    args = delta_inputs(9, 2, 6, 128, 128, 3)
+    state, out = torch.zeros(3, 6, 128, 128, device="cuda"), torch.zeros(9, 6, 128, device="cuda")
+    assert gpu.gdn_seqs(state, *args, out, ints([0, 5, 3, 9]), None, None, 0, 3, 3, 9, 2, 6, 128, 128) == 0
+    assert gpu.device_status() == 3 and gpu.clear_status() == 0
+
+
+def test_rows_that_many_sequences_claim(gpu):
+    """64 sequences of which every other one claims all rows: no more work than the call's rows can be, and nothing outside the outputs is written."""
+    import torch
+    c = Cache(gpu, [70] * 64, [2] * 64, seed=16)
+    c.view._keep[3].copy_(ints([0, 128] * 32 + [0]))
+    q = torch.randn(c.n_tok, 24, 256, device="cuda")
+    before = c.d_pool.clone()
+    out = run_attention(gpu, c, q)
+    torch.cuda.synchronize()
+    assert torch.equal(before, c.d_pool) and bool(torch.isfinite(out).all())
+    assert gpu.device_status() == 3 and gpu.clear_status() == 0
+
+
+def test_cache_of_another_device(gpu, monkeypatch):
+    """The numbers of a cache are memory of its own device: a call on another one is refused."""
+    import torch
+    c = Cache(gpu, [70, 20], [2, 2], seed=17)
+    q = torch.randn(c.n_tok, 24, 256, device="cuda")
+    k = torch.randn(c.n_tok, 4, 256, device="cuda")
+    monkeypatch.setattr(c.view, "_device", c.view._device + 1)
+    with pytest.raises(RuntimeError, match="the cache is on device"):
+        c.view.append(0, k, k)
+    with pytest.raises(RuntimeError, match="the cache is on device"):
+        c.view.attn(0, q, torch.empty_like(q), 24, 70, None, 0.0625)
 
 
 def test_captured_attention_follows_the_numbers(gpu):
