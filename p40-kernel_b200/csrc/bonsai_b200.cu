@@ -1974,11 +1974,12 @@ int bonsai_b200_qk_norm_rope(const float *q, const float *k, const float *q_weig
     for (int i = 0; i < 2; ++i) {
         if (!P.n_head[i]) continue;
         if (!P.x[i] || !P.w[i] || !P.y[i] || !aligned4(P.x[i]) || !aligned4(P.w[i]) || !aligned4(P.y[i])) return 1;
-        // rows that overlap each other, or an output that is not the input row for row, would be read after they are written
+        // rows that overlap each other would be read after they are written.  They lie apart where one stride is a row and more, and the other passes over all that the first spans.
         const bool one_tok = n_tok == 1, one_head = P.n_head[i] == 1;
         const int64_t ts = P.tok_stride[i], hs = P.head_stride[i];
-        if ((!one_head && hs < head_dim) || (!one_tok && ts < 0) || (one_head ? false : (!one_tok && ts < (P.n_head[i] - 1) * hs + head_dim && hs < (n_tok - 1) * ts + head_dim))) return 1;
-        if (one_head && !one_tok && ts < head_dim) return 1;
+        const __int128 heads_span = (__int128)(P.n_head[i] - 1) * hs + head_dim, toks_span = (__int128)(n_tok - 1) * ts + head_dim;
+        if ((!one_head && hs < head_dim) || (!one_tok && ts < head_dim) || (!one_head && !one_tok && ts < heads_span && hs < toks_span)) return 1;
+        if ((one_head ? 0 : heads_span) + (one_tok ? 0 : toks_span) > INT64_MAX / 4) return 1;             // (floats that have no address)
         vec = vec && aligned16(P.x[i]) && aligned16(P.w[i]) && aligned16(P.y[i]) && (one_tok || ts % 4 == 0) && (one_head || hs % 4 == 0);
     }
     auto run = [&](auto kernel, int per) {

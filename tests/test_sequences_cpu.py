@@ -19,6 +19,21 @@ def test_head_norm_refusals():
     assert call(n_tok=0) == 0 and call(n_head=0, n_head_kv=0) == 0
 
 
+def test_head_norm_rows_that_overlap():
+    """Tokens that lie closer than a row, whichever of the strides is the larger one."""
+    import bonsai_b200
+    f = bonsai_b200.lib().bonsai_b200_qk_norm_rope
+
+    def call(n_tok, n_head, qt, qh, n_head_kv=0, kt=0, kh=0):
+        return f(ONE, ONE, ONE, ONE, ONE, ONE, ONE, ONE, n_tok, n_head, n_head_kv, 256, 64, qt, qh, kt, kh, 1e-6, None)
+    for qt, qh in ((0, 512), (100, 512), (255, 1024), (255, 1 << 40)):
+        assert call(2, 4, qt, qh) == 1, (qt, qh)
+        assert call(2, 0, 0, 0, 4, qt, qh) == 1, (qt, qh)
+    assert call(3, 4, 300, 512) == 1 and call(2, 4, 512, 300) == 1             # rows of one token in front of another's
+    assert call(1 << 20, 4, 1 << 61, 1 << 44) == 1                             # spans past 64 bits
+    assert call(2, 1, 255, 0) == 1
+
+
 def struct(**kw):
     import bonsai_b200
     have = dict(pool=ONE, table=ONE, len=ONE, start=ONE, n_pages=4, n_layers=2, n_head_kv=4, n_seq=2, table_stride=3, n_tok=5)
