@@ -1980,6 +1980,9 @@ int bonsai_b200_qk_norm_rope(const float *q, const float *k, const float *q_weig
         const __int128 heads_span = (__int128)(P.n_head[i] - 1) * hs + head_dim, toks_span = (__int128)(n_tok - 1) * ts + head_dim;
         if ((!one_head && hs < head_dim) || (!one_tok && ts < head_dim) || (!one_head && !one_tok && ts < heads_span && hs < toks_span)) return 1;
         if ((one_head ? 0 : heads_span) + (one_tok ? 0 : toks_span) > INT64_MAX / 4) return 1;             // (floats that have no address)
+        // an output in the place of its input is row for row the same memory, or rows are written before others read them; no output is the other input
+        const bool packed = (one_head || hs == head_dim) && (one_tok || ts == (int64_t)P.n_head[i] * head_dim);
+        if ((P.y[i] == P.x[i] && !packed) || (P.n_head[1 - i] && P.y[i] == P.x[1 - i])) return 1;
         vec = vec && aligned16(P.x[i]) && aligned16(P.w[i]) && aligned16(P.y[i]) && (one_tok || ts % 4 == 0) && (one_head || hs % 4 == 0);
     }
     auto run = [&](auto kernel, int per) {

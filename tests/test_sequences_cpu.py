@@ -34,6 +34,18 @@ def test_head_norm_rows_that_overlap():
     assert call(2, 1, 255, 0) == 1
 
 
+def test_head_norm_outputs_in_the_place_of_inputs():
+    """Only row for row: where the input is packed."""
+    import bonsai_b200
+    f = bonsai_b200.lib().bonsai_b200_qk_norm_rope
+
+    def call(q_out, k_out, n_tok=2, qt=1024, qh=256, n_head_kv=2, kt=512, kh=256):
+        return f(16, 32, ONE, ONE, ONE, ONE, q_out, k_out, n_tok, 4, n_head_kv, 256, 64, qt, qh, kt, kh, 1e-6, None)
+    assert call(16, 64, qt=2048, qh=512) == 1 and call(64, 32, kt=1024) == 1 and call(16, 64, n_tok=1, qh=512) == 1
+    assert call(16, 64, qt=256, qh=512) == 1            # heads first, then tokens
+    assert call(32, 64) == 1 and call(64, 16) == 1      # the other input
+
+
 def struct(**kw):
     import bonsai_b200
     have = dict(pool=ONE, table=ONE, len=ONE, start=ONE, n_pages=4, n_layers=2, n_head_kv=4, n_seq=2, table_stride=3, n_tok=5)
