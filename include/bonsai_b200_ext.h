@@ -161,7 +161,7 @@ int bonsai_b200_set_option(const char *key, int64_t value);
  * wait on the current device since the word was last cleared; 1 = a wait on a shared-memory barrier or
  * counter ran out; 2 = a wait for other CTAs or other ranks ran out (the launch still ends by itself and
  * the context stays usable; the outputs of that launch are incomplete); 3 = a call for several sequences met numbers on the device that do not
- * fit (it left what they concern alone).  Both calls synchronise the device
+ * fit (it left what they concern alone; it does not replace a 1 or 2 that is there).  Both calls synchronise the device
  * (cudaDeviceSynchronize), so neither may be made while a stream of the device is being captured.
  * Failures of the calls themselves come back as 1000 + the CUDA error code. */
 int bonsai_b200_device_status(void);

@@ -8,7 +8,8 @@ namespace b200 {
 
 enum : int { STATUS_BAD_SEQUENCE = 3 };
 
-__device__ __forceinline__ void bad_sequence() { atomicExch(&g_device_status, STATUS_BAD_SEQUENCE); }
+// (a wait that ran out is the graver report, and stays)
+__device__ __forceinline__ void bad_sequence() { atomicCAS(&g_device_status, 0, STATUS_BAD_SEQUENCE); }
 
 struct SeqRange { int begin, n; };      // n < 0: not rows of the call
 __device__ __forceinline__ SeqRange seq_range(const int32_t *start, int s, int n_tok) {
