@@ -266,7 +266,7 @@ int bonsai_b200_kv_splits(int n_pos, int resident8, int resident16, int64_t out[
  * says which rows are whose: sequence s has rows start[s] .. start[s + 1] - 1, none where the two are equal.  Rows from start[n_seq] on belong to nobody:
  * they are not read, and outputs leave theirs as they were.  What lies on the device (start, lengths, tables, slots) is read when the call runs, so a
  * captured call can be replayed with other numbers.  Numbers that do not fit (rows outside the call, a page that the pool does not have, a slot that
- * two sequences name) stop that sequence and no other: its outputs and states are incomplete or as they were, and the status word
+ * two sequences with new tokens name) stop that sequence and no other: its outputs and states are incomplete or as they were, and the status word
  * (bonsai_b200_device_status) becomes 3.  Workspaces belong to one call at a time: calls, and replays of graphs, that share one follow each other. */
 
 /* Norms of queries and keys for each head, with the position rotation in the same pass: row = x / sqrt(mean(x^2) + eps) * weight, then the pairs
@@ -307,7 +307,8 @@ int bonsai_b200_pages_copy(void *pool, int64_t page_bytes, int n_pages, const in
 
 /* The gated delta rule over the new tokens of several sequences: bonsai_p40_gdn_step for each token in turn (q, k [n_tok][n_k_heads][K], v, out
  * [n_tok][n_v_heads][V], g, beta [n_tok][n_v_heads]), the same shapes and within 1e-5 of the largest output.  state: n_slots states [n_v_heads][K][V],
- * updated in place; sequence s has state slot[s], or s where slot is NULL (then n_slots >= n_seq).  A sequence without new tokens keeps its state.
+ * updated in place; sequence s has state slot[s], or s where slot is NULL (then n_slots >= n_seq).  A sequence without new tokens keeps its state, and
+ * its slot is not looked at.
  * workspace: 16-byte aligned device memory of bonsai_b200_gdn_seqs_workspace(the same sizes) bytes (NULL where that is 0). */
 int64_t bonsai_b200_gdn_seqs_workspace(int n_tok, int n_seq, int n_k_heads, int n_v_heads, int K, int V);
 int bonsai_b200_gdn_seqs(float *state, const float *q, const float *k, const float *v, const float *g, const float *beta, float *out, const int32_t *start,

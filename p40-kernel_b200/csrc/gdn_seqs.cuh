@@ -18,12 +18,13 @@ struct GdnSeqs {
     int n_seq, n_slots, n_tok, n_k_heads, n_v_heads, K, V;
 };
 
-// Where sequence s keeps its state: its slot, or s itself.  -1 (every thread of the CTA): the slot is not one of the pool's, or another sequence names it too.
+// Where sequence s keeps its state: its slot, or s itself.  -1 (every thread of the CTA): the slot is not one of the pool's, or another sequence with new
+// tokens names it too (one without them does nothing with its state: a captured call's spare sequences may name any slot).
 __device__ __forceinline__ int gdn_slot_of(const GdnSeqs &P, int s) {
     const int mine = P.slot ? P.slot[s] : s;
     int bad = mine < 0 || mine >= P.n_slots;
     if (P.slot)
-        for (int i = threadIdx.x; i < P.n_seq; i += blockDim.x) bad |= i != s && P.slot[i] == mine;
+        for (int i = threadIdx.x; i < P.n_seq; i += blockDim.x) bad |= i != s && P.slot[i] == mine && seq_range(P.start, i, P.n_tok).n > 0;
     return __syncthreads_or(bad) ? -1 : mine;
 }
 
