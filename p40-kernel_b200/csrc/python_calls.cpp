@@ -22,8 +22,13 @@ namespace {
 // Kinds of argument beside plain numbers: device memory (a CUDA tensor or None), a handle (an integer or an object with
 // an integer `value`, as ctypes makes them), a truth value.
 struct Mem { void *p; };
-struct Dev { void *p; };                // device memory of the current device
-struct Strided { void *p; };            // ... whose strides are arguments of the call, so that it need not be contiguous
+// Device memory of the current device, of values of a type (Undefined: bytes, of whatever type the tensor is).
+template <at::ScalarType T> struct Dev { void *p; };
+template <at::ScalarType T> struct Strided { void *p; };        // ... whose strides are arguments of the call, so that it need not be contiguous
+using Floats = Dev<at::kFloat>;
+using Doubles = Dev<at::kDouble>;
+using Int32s = Dev<at::kInt>;
+using Bytes = Dev<at::ScalarType::Undefined>;
 struct Ints { const void *p; int64_t n; };      // host memory: an int32 tensor
 struct Handle { void *p; };
 struct Truth { int v; };
@@ -78,13 +83,19 @@ bool here(PyObject *o, const char *name) {
     if (at != now) PyErr_Format(PyExc_RuntimeError, "%s is on device %d, the current device is %d", name, at, now);
     return at == now;
 }
-bool get(PyObject *o, const char *name, Dev &out) {
+// A tensor's type is the one that the call reads it as.  (An object like a tensor says nothing of it.)
+bool of_type(PyObject *o, const char *name, at::ScalarType type) {
+    if (type == at::ScalarType::Undefined || !THPVariable_Check(o) || THPVariable_Unpack(o).scalar_type() == type) return true;
+    PyErr_Format(PyExc_RuntimeError, "%s must be a tensor of %s, not of %s", name, c10::toString(type), c10::toString(THPVariable_Unpack(o).scalar_type()));
+    return false;
+}
+template <at::ScalarType T> bool get(PyObject *o, const char *name, Dev<T> &out) {
     Mem m{};
-    if (!here(o, name) || !get(o, name, m)) return false;
+    if (!of_type(o, name, T) || !here(o, name) || !get(o, name, m)) return false;
     out.p = m.p;
     return true;
 }
-bool get(PyObject *o, const char *name, Strided &out) {
+template <at::ScalarType T> bool get(PyObject *o, const char *name, Strided<T> &out) {
     if (!THPVariable_Check(o)) {
         Mem m{};
         if (!get(o, name, m)) return false;
@@ -92,6 +103,7 @@ bool get(PyObject *o, const char *name, Strided &out) {
         return true;
     }
     const at::Tensor &t = THPVariable_Unpack(o);
+    if (!of_type(o, name, T)) return false;
     if (!t.is_cuda()) {
         PyErr_Format(PyExc_RuntimeError, "%s must be a CUDA tensor: this library has no CPU path", name);
         return false;
@@ -149,8 +161,8 @@ bool get(PyObject *o, const char *, float &out) {
 }
 
 void *raw(Mem m) { return m.p; }
-void *raw(Dev m) { return m.p; }
-void *raw(Strided m) { return m.p; }
+template <at::ScalarType T> void *raw(Dev<T> m) { return m.p; }
+template <at::ScalarType T> void *raw(Strided<T> m) { return m.p; }
 const void *raw(Ints m) { return m.p; }
 void *raw(Handle h) { return h.p; }
 int raw(Truth t) { return t.v; }
@@ -245,14 +257,14 @@ Call<Mem, Mem, Mem, int64_t, int64_t, Truth> quant_batch{"quant_batch", {"X", "s
 Call<Mem, Mem, Mem, Mem, Mem, int64_t, int64_t> linear{"linear", {"W", "x", "signs", "y", "xq_scratch", "n_out", "n_in"}};
 Call<Mem, Mem, Mem, Mem, int64_t, int64_t> linear_static{"linear_static", {"W", "x", "signs", "y", "n_out", "n_in"}};
 Call<Handle> chain_run{"chain_run", {"chain"}};
-Call<Strided, Strided, Dev, Dev, Dev, Dev, Dev, Dev, int64_t, int, int, int, int, int64_t, int64_t, int64_t, int64_t, float> qk_norm_rope{
+Call<Strided<at::kFloat>, Strided<at::kFloat>, Floats, Floats, Int32s, Doubles, Floats, Floats, int64_t, int, int, int, int, int64_t, int64_t, int64_t, int64_t, float> qk_norm_rope{
     "qk_norm_rope", {"q", "k", "q_weight", "k_weight", "pos", "freq", "q_out", "k_out", "n_tok", "n_head", "n_head_kv", "head_dim", "n_rot", "q_tok_stride",
                      "q_head_stride", "k_tok_stride", "k_head_stride", "eps"}};
-Call<Handle, int, Dev, Dev> pages_append{"pages_append", {"pages", "layer", "k", "v"}};
-Call<Handle, int, Dev, Dev, int, int, Dev, int64_t, float> pages_attn{
+Call<Handle, int, Floats, Floats> pages_append{"pages_append", {"pages", "layer", "k", "v"}};
+Call<Handle, int, Floats, Floats, int, int, Bytes, int64_t, float> pages_attn{
     "pages_attn", {"pages", "layer", "q", "out", "n_head", "max_len", "workspace", "workspace_bytes", "scale"}};
-Call<Dev, int64_t, int, Ints, Ints, int> pages_copy{"pages_copy", {"pool", "page_bytes", "n_pages", "src", "dst", "n"}};
-Call<Dev, Dev, Dev, Dev, Dev, Dev, Dev, Dev, Dev, Dev, int64_t, int, int, int, int, int, int, int> gdn_seqs{
+Call<Bytes, int64_t, int, Ints, Ints, int> pages_copy{"pages_copy", {"pool", "page_bytes", "n_pages", "src", "dst", "n"}};
+Call<Floats, Floats, Floats, Floats, Floats, Floats, Floats, Int32s, Int32s, Bytes, int64_t, int, int, int, int, int, int, int> gdn_seqs{
     "gdn_seqs", {"state", "q", "k", "v", "g", "beta", "out", "start", "slot", "workspace", "workspace_bytes", "n_seq", "n_slots", "n_tok", "n_k_heads",
                  "n_v_heads", "K", "V"}};
 // include/bonsai_kv.h
