@@ -30,6 +30,7 @@ FLAGS = [
 
 
 CALLS_SRC = os.path.join(CSRC, "python_calls.cpp")
+CALLS_HEADERS = sorted(glob.glob(os.path.join(HERE, "..", "include", "*.h")))
 CALLS = os.path.join(HERE, "bonsai_b200", "_calls" + sysconfig.get_config_var("EXT_SUFFIX"))
 CALLS_STAMP = os.path.join(HERE, "build", "calls.stamp")      # what the present _calls file was built for
 
@@ -65,7 +66,7 @@ def build_calls(force=False):
     except importlib.metadata.PackageNotFoundError:
         return None
     stamp = open(CALLS_STAMP).read() if os.path.exists(CALLS_STAMP) else ""
-    if not (force or stamp != made_for or stale(CALLS, [CALLS_SRC])):
+    if not (force or stamp != made_for or stale(CALLS, [CALLS_SRC, *CALLS_HEADERS])):
         return CALLS
     try:
         import torch

@@ -13,18 +13,23 @@
 
 #include <cstdint>
 #include <cstring>
+#include <initializer_list>
 #include <tuple>
 #include <type_traits>
 #include <utility>
 
+#include "../../include/bonsai_b200_ext.h"
+
 namespace {
+
+constexpr int64_t PAGE_ROW = 256;           // values of a paged cache's row
 
 // Kinds of argument beside plain numbers: device memory (a CUDA tensor or None), a handle (an integer or an object with
 // an integer `value`, as ctypes makes them), a truth value.
 struct Mem { void *p; };
-// Device memory of the current device, of values of a type (Undefined: bytes, of whatever type the tensor is).
-template <at::ScalarType T> struct Dev { void *p; };
-template <at::ScalarType T> struct Strided { void *p; };        // ... whose strides are arguments of the call, so that it need not be contiguous
+// Device memory of the current device, of values of a type (Undefined: bytes, of whatever type the tensor is), and how many there are (-1: None, or an object that does not say).
+template <at::ScalarType T> struct Dev { void *p; int64_t n; };
+template <at::ScalarType T> struct Strided { void *p; int64_t n; };     // ... whose strides are arguments of the call, so that it need not be contiguous
 using Floats = Dev<at::kFloat>;
 using Doubles = Dev<at::kDouble>;
 using Int32s = Dev<at::kInt>;
@@ -93,6 +98,7 @@ template <at::ScalarType T> bool get(PyObject *o, const char *name, Dev<T> &out)
     Mem m{};
     if (!of_type(o, name, T) || !here(o, name) || !get(o, name, m)) return false;
     out.p = m.p;
+    out.n = !THPVariable_Check(o) ? -1 : T == at::ScalarType::Undefined ? (int64_t)THPVariable_Unpack(o).nbytes() : THPVariable_Unpack(o).numel();
     return true;
 }
 template <at::ScalarType T> bool get(PyObject *o, const char *name, Strided<T> &out) {
@@ -100,6 +106,7 @@ template <at::ScalarType T> bool get(PyObject *o, const char *name, Strided<T> &
         Mem m{};
         if (!get(o, name, m)) return false;
         out.p = m.p;
+        out.n = -1;
         return true;
     }
     const at::Tensor &t = THPVariable_Unpack(o);
@@ -110,6 +117,7 @@ template <at::ScalarType T> bool get(PyObject *o, const char *name, Strided<T> &
     }
     if (!here(o, name)) return false;
     out.p = t.mutable_data_ptr();
+    out.n = (int64_t)(t.storage().nbytes() / t.element_size()) - t.storage_offset();       // to the end of its memory
     return true;
 }
 bool get(PyObject *o, const char *name, Ints &out) {
@@ -175,13 +183,25 @@ constexpr int MAX_ARGS = 20;
 template <typename T> bool long_enough(const T &, int64_t) { return true; }
 inline bool long_enough(const Ints &v, int64_t n) { return v.n >= n; }
 
-// One exported function: its address, filled in by bind(), and the names of its arguments.
+// Whether there are as many values as the sizes beside them say: the product of them.  Sizes that are no sizes are the library's to refuse.
+template <typename M> bool holds(const M &m, std::initializer_list<int64_t> sizes) {
+    unsigned __int128 all = 1;
+    for (int64_t x : sizes) {
+        if (x <= 0) return true;
+        all *= (unsigned __int128)x;
+        if (all > (unsigned __int128)INT64_MAX) all = (unsigned __int128)INT64_MAX + 1;         // (no tensor has them)
+    }
+    return m.n < 0 || all <= (unsigned __int128)m.n;
+}
+
+// One exported function: its address, filled in by bind(), the names of its arguments, and where the call has sizes what finds the tensor that is too small for them (its place, -1: none).
 template <typename... A>
 struct Call {
     using Fn = int (*)(Raw<A>..., void *);
     static constexpr int N = sizeof...(A);
     const char *name;
     const char *args[N];
+    int (*small)(const std::tuple<A...> &) = nullptr;
     Fn fn = nullptr;
 
     template <size_t... I>
@@ -193,6 +213,10 @@ struct Call {
                 PyErr_Format(PyExc_RuntimeError, "%s: a list is shorter than %s", name, args[N - 1]);
                 return nullptr;
             }
+        }
+        if (const int at = small ? small(a) : -1; at >= 0) {
+            PyErr_Format(PyExc_RuntimeError, "%s: %s is smaller than the sizes beside it say", name, args[at]);
+            return nullptr;
         }
         void *stream = c10::cuda::getCurrentCUDAStream().stream();
         int rc;
@@ -259,14 +283,62 @@ Call<Mem, Mem, Mem, Mem, int64_t, int64_t> linear_static{"linear_static", {"W", 
 Call<Handle> chain_run{"chain_run", {"chain"}};
 Call<Strided<at::kFloat>, Strided<at::kFloat>, Floats, Floats, Int32s, Doubles, Floats, Floats, int64_t, int, int, int, int, int64_t, int64_t, int64_t, int64_t, float> qk_norm_rope{
     "qk_norm_rope", {"q", "k", "q_weight", "k_weight", "pos", "freq", "q_out", "k_out", "n_tok", "n_head", "n_head_kv", "head_dim", "n_rot", "q_tok_stride",
-                     "q_head_stride", "k_tok_stride", "k_head_stride", "eps"}};
-Call<Handle, int, Floats, Floats> pages_append{"pages_append", {"pages", "layer", "k", "v"}};
+                     "q_head_stride", "k_tok_stride", "k_head_stride", "eps"},
+    [](const auto &a) {
+        const auto &[q, k, q_weight, k_weight, pos, freq, q_out, k_out, n_tok, n_head, n_head_kv, head_dim, n_rot, qt, qh, kt, kh, eps] = a;
+        // from the first row's begin to the last one's end; a stride of one row is not used
+        auto spans = [&](const auto &x, int64_t heads, int64_t tok_stride, int64_t head_stride) {
+            const __int128 last = (__int128)(n_tok - 1) * (n_tok > 1 ? tok_stride : 0) + (__int128)(heads - 1) * (heads > 1 ? head_stride : 0) + head_dim;
+            return n_tok <= 0 || heads <= 0 || head_dim <= 0 || x.n < 0 || last <= x.n;
+        };
+        if (n_tok <= 0 || (n_head <= 0 && n_head_kv <= 0)) return -1;
+        if (!spans(q, n_head, qt, qh)) return 0;
+        if (!spans(k, n_head_kv, kt, kh)) return 1;
+        if (n_head > 0 && !holds(q_weight, {head_dim})) return 2;
+        if (n_head_kv > 0 && !holds(k_weight, {head_dim})) return 3;
+        if (n_rot > 0 && !holds(pos, {n_tok})) return 4;
+        if (!holds(freq, {n_rot / 2})) return 5;
+        if (!holds(q_out, {n_tok, n_head, head_dim})) return 6;
+        return holds(k_out, {n_tok, n_head_kv, head_dim}) ? -1 : 7;
+    }};
+// (the struct's own memory is Pages.__init__'s to look at)
+Call<Handle, int, Floats, Floats> pages_append{"pages_append", {"pages", "layer", "k", "v"}, [](const auto &a) {
+        const auto &[pages, layer, k, v] = a;
+        const auto *p = static_cast<const bonsai_b200_pages *>(pages.p);
+        if (!p || p->n_seq <= 0) return -1;
+        if (!holds(k, {p->n_tok, p->n_head_kv, PAGE_ROW})) return 2;
+        return holds(v, {p->n_tok, p->n_head_kv, PAGE_ROW}) ? -1 : 3;
+    }};
 Call<Handle, int, Floats, Floats, int, int, Bytes, int64_t, float> pages_attn{
-    "pages_attn", {"pages", "layer", "q", "out", "n_head", "max_len", "workspace", "workspace_bytes", "scale"}};
-Call<Bytes, int64_t, int, Ints, Ints, int> pages_copy{"pages_copy", {"pool", "page_bytes", "n_pages", "src", "dst", "n"}};
+    "pages_attn", {"pages", "layer", "q", "out", "n_head", "max_len", "workspace", "workspace_bytes", "scale"},
+    [](const auto &a) {
+        const auto &[pages, layer, q, out, n_head, max_len, workspace, workspace_bytes, scale] = a;
+        const auto *p = static_cast<const bonsai_b200_pages *>(pages.p);
+        if (!p || p->n_seq <= 0) return -1;
+        if (!holds(q, {p->n_tok, n_head, PAGE_ROW})) return 2;
+        if (!holds(out, {p->n_tok, n_head, PAGE_ROW})) return 3;
+        return holds(workspace, {workspace_bytes}) ? -1 : 6;
+    }};
+Call<Bytes, int64_t, int, Ints, Ints, int> pages_copy{"pages_copy", {"pool", "page_bytes", "n_pages", "src", "dst", "n"}, [](const auto &a) {
+        return std::get<5>(a) <= 0 || holds(std::get<0>(a), {std::get<1>(a), std::get<2>(a)}) ? -1 : 0;
+    }};
 Call<Floats, Floats, Floats, Floats, Floats, Floats, Floats, Int32s, Int32s, Bytes, int64_t, int, int, int, int, int, int, int> gdn_seqs{
     "gdn_seqs", {"state", "q", "k", "v", "g", "beta", "out", "start", "slot", "workspace", "workspace_bytes", "n_seq", "n_slots", "n_tok", "n_k_heads",
-                 "n_v_heads", "K", "V"}};
+                 "n_v_heads", "K", "V"},
+    [](const auto &a) {
+        const auto &[state, q, k, v, g, beta, out, start, slot, workspace, workspace_bytes, n_seq, n_slots, n_tok, n_k_heads, n_v_heads, K, V] = a;
+        if (n_seq <= 0 || n_tok <= 0) return -1;
+        if (!holds(state, {n_slots, n_v_heads, K, V})) return 0;
+        if (!holds(q, {n_tok, n_k_heads, K})) return 1;
+        if (!holds(k, {n_tok, n_k_heads, K})) return 2;
+        if (!holds(v, {n_tok, n_v_heads, V})) return 3;
+        if (!holds(g, {n_tok, n_v_heads})) return 4;
+        if (!holds(beta, {n_tok, n_v_heads})) return 5;
+        if (!holds(out, {n_tok, n_v_heads, V})) return 6;
+        if (!holds(start, {(int64_t)n_seq + 1})) return 7;
+        if (!holds(slot, {n_seq})) return 8;
+        return holds(workspace, {workspace_bytes}) ? -1 : 9;
+    }};
 // include/bonsai_kv.h
 Call<Handle, int, int, Mem, Mem> kv_append{"kv_append", {"kv", "layer", "pos", "k", "v"}};
 Call<Handle, int, int, int, Mem, Mem> kv_append_batch{"kv_append_batch", {"kv", "layer", "pos0", "n_tok", "k", "v"}};
