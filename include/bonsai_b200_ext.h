@@ -296,8 +296,9 @@ int bonsai_b200_pages_append(const bonsai_b200_pages *pages, int layer, const fl
 /* Attention of the new tokens (q, out [n_tok][n_head][256]) of one layer over the cache, their own rows included: each as bonsai_kv_attn_decode computes it at
  * its position -- queries quantised to Q8_0 (as above), positions up to its own seen -- within 1e-5 of the largest output of a head.  A token without a position
  * (len[s] smaller than its new tokens) sees nothing: zeros.  max_len: no smaller than every len, for the division of the work; longer sequences are served
- * all the same, more slowly.  workspace: 16-byte aligned device memory of bonsai_b200_pages_attn_workspace(the same sizes) bytes (NULL where that is 0): parts of
- * rows, and beside prompts images of their pages, 133 KB a page and kv head, up to 2.5 GB (longer contexts do without). */
+ * all the same, more slowly.  workspace: 16-byte aligned device memory of bonsai_b200_pages_attn_workspace(the same sizes) bytes (NULL where that is 0): sums
+ * of rows whose pages several CTAs share (0.2 GB at most), and beside prompts images of pages: 133 KB a page and kv head, for max_len of each sequence that the call's tokens could make
+ * a prompt (128 rows, n_head / n_head_kv a token), 2.5 GB at most: a call that would need more has no images, and its prompts take about 1.7 times as long. */
 int64_t bonsai_b200_pages_attn_workspace(int n_tok, int max_len, int n_seq, int n_head, int n_head_kv);
 int bonsai_b200_pages_attn(const bonsai_b200_pages *pages, int layer, const float *q, float *out, int n_head, int max_len, void *workspace,
                            int64_t workspace_bytes, float scale, bonsai_stream stream);

@@ -1917,42 +1917,54 @@ int check_pages(const bonsai_b200_pages *p, int layer, PageCache *C) {
 }
 
 // How pages_attn divides a call.  Sequences that may be on the tensor cores (tc of them at most, 0: none; pages_on_tc): tiles of 128 rows, a span of pages a CTA.  The others: rows
-// a tile; the spans are the device's to find, up to most_splits a tile.
+// a tile, in one class or (beside the tensor cores) two; the spans are the device's to find, up to most_splits a tile.
 struct PagesPlan {
     int rowt, most_splits, span, splits, max_pages;
     int64_t tiles, tc;
-    int64_t part_bytes, image_bytes, redo_bytes;
-    int64_t bytes() const { return part_bytes + image_bytes + redo_bytes; }
+    int64_t items, parts[2];                            // of a class: CTAs' shares at most (pages_span), and of tiles that several share
+    int row_shift[2];
+    int64_t image_bytes, redo_bytes, tc_rows, part_rows[2];
+    int64_t bytes() const { return image_bytes + redo_bytes + rows_bytes(tc_rows) + rows_bytes(part_rows[0]) + rows_bytes(part_rows[1]) + (joined() ? 16 : 0); }
+    bool joined() const { return tc_rows || part_rows[0] || part_rows[1]; }
+    static int64_t rows_bytes(int64_t rows) { return rows * KV_D * (int64_t)sizeof(float) + (rows * (int64_t)sizeof(float2) + 15) / 16 * 16; }
 };
 constexpr int64_t PTC_IMAGE_LIMIT = int64_t(5) << 29;            // 2.5 GB: a full context of the 27B model
 constexpr int PGA_SLOTS = 2 * SM_COUNT;
 PagesPlan plan_pages(int n_tok, int max_len, int n_seq, int n_head, int n_head_kv) {
     PagesPlan p = {};
     const int group = n_head / n_head_kv;
-    const int64_t rows = (int64_t)n_tok * group, each = (rows + n_seq - 1) / n_seq, pages = std::max(1, (int)(((int64_t)max_len + PG_POS - 1) / PG_POS));
+    const int64_t rows = (int64_t)n_tok * group, each = (rows + n_seq - 1) / n_seq, pages = std::max(1, (int)(((int64_t)max_len + PG_POS - 1) / PG_POS)), seqs = std::min(n_seq, n_tok);
     p.max_pages = (int)pages;
     p.tc = std::min<int64_t>(n_seq, rows / PTC_ROWS);
     // Who has how many tokens only the device knows.  Many more tokens than sequences are taken to be prompts: a batch of few tokens each would pay for launches that find nothing, and its
     // tiles be those of the tensor cores' neighbours (16 sequences of 3 tokens 131 us instead of 74).
-    const int64_t beyond = ((int64_t)n_tok - std::min(n_seq, n_tok)) * group;
+    const int64_t beyond = ((int64_t)n_tok - seqs) * group;
     if (rows < 2 * PTC_ROWS || beyond < 4 * PTC_ROWS || p.tc * pages * n_head_kv > PTC_IMAGE_LIMIT / ATC_IMG_BYTES) p.tc = 0;
     p.rowt = each > 32 ? 4 : each > 16 ? 2 : each > 8 ? 1 : 0;             // (without the tensor cores; beside them eight rows and 64)
     p.span = (int)pages;
     if (p.tc) {
-        // spans that fill the last round of CTAs, one per SM; a CTA's start and its share of the join are worth four pages
-        p.tiles = (rows + (int64_t)std::min(n_seq, n_tok) * (PTC_ROWS - 1)) / PTC_ROWS;
-        const int64_t items = (rows + PTC_ROWS - 1) / PTC_ROWS * n_head_kv;
+        // spans that fill the last round of CTAs, one per SM; a CTA's start and its share of the join are worth four pages.  Eight rounds at most, since every CTA's sums take room: more than
+        // that are full enough with one CTA a tile.
+        p.tiles = (rows + seqs * (PTC_ROWS - 1)) / PTC_ROWS;
+        const int64_t items = (rows + PTC_ROWS - 1) / PTC_ROWS * n_head_kv, most = std::min<int64_t>({pages, 16, std::max<int64_t>(1, 8 * SM_COUNT / items)});
         int64_t best = INT64_MAX;
-        for (int64_t s = 1; s <= std::min<int64_t>(pages, 16); ++s) {
+        for (int64_t s = 1; s <= most; ++s) {
             const int64_t span = (pages + s - 1) / s, cost = ((items * s + SM_COUNT - 1) / SM_COUNT) * (span + 4);
             if (cost < best) best = cost, p.span = (int)span;
         }
     }
     p.splits = (int)((pages + p.span - 1) / p.span);
-    // beside prompts every split has room for all of their rows, so it is few
-    p.most_splits = (int)std::min<int64_t>((pages + 1) / 2, p.tc ? 8 : (PGA_SLOTS + n_head_kv - 1) / n_head_kv);
-    const int64_t splits = std::max(p.splits, p.most_splits), part = splits == 1 ? 0 : splits * n_tok * n_head * (KV_D + 2) * (int64_t)sizeof(float);
-    p.part_bytes = part ? (part + 15) / 16 * 16 + 16 : 0;           // (and the spans that the device finds)
+    p.most_splits = (int)std::min<int64_t>((pages + 1) / 2, (PGA_SLOTS + n_head_kv - 1) / n_head_kv);
+    p.row_shift[0] = p.tc || p.rowt == 0 ? 3 : p.rowt == 1 ? 4 : p.rowt == 2 ? 5 : 6;
+    p.row_shift[1] = 6;
+    p.items = n_head_kv * ((rows >> 3) + seqs);        // (tiles)
+    p.items = std::min(PGA_SLOTS + p.items, p.items * p.most_splits);
+    for (int c = 0; c < (p.tc ? 2 : 1) && p.most_splits > 1; ++c) {
+        const int64_t tiles = (rows >> p.row_shift[c]) + (c ? std::min(seqs, rows / 9) : seqs);
+        p.parts[c] = std::min<int64_t>(2 * PGA_SLOTS, tiles * p.most_splits * n_head_kv);
+        p.part_rows[c] = p.parts[c] << p.row_shift[c];
+    }
+    p.tc_rows = p.tc && p.splits > 1 ? (int64_t)p.splits * n_tok * n_head : 0;
     p.image_bytes = p.tc * pages * n_head_kv * ATC_IMG_BYTES;
     p.redo_bytes = p.tc ? (p.tiles * n_head_kv * p.splits * (int64_t)sizeof(int) + 15) / 16 * 16 : 0;
     return p;
@@ -2020,9 +2032,8 @@ int bonsai_b200_pages_attn(const bonsai_b200_pages *pages, int layer, const floa
     if (!q || !out || !aligned4(q) || !aligned4(out) || !pages_attn_sizes(C.n_tok, max_len, C.n_seq, n_head, C.n_head_kv)) return 1;
     const PagesPlan plan = plan_pages(C.n_tok, max_len, C.n_seq, n_head, C.n_head_kv);
     if (2 * plan.tiles > INT32_MAX || plan.tc * plan.max_pages > INT32_MAX) return 1;
-    const int64_t most_items = ((int64_t)C.n_tok * (n_head / C.n_head_kv) / 8 + C.n_seq) * plan.most_splits * C.n_head_kv;
-    if (most_items > INT32_MAX) return 1;
-    P.most_items = (uint32_t)most_items;
+    if (plan.items > INT32_MAX) return 1;
+    P.most_items = (uint32_t)plan.items;
     P.q = q;
     P.out = out;
     P.layer = layer;
@@ -2032,8 +2043,6 @@ int bonsai_b200_pages_attn(const bonsai_b200_pages *pages, int layer, const floa
     P.splits = plan.splits;
     P.most_rows[0] = plan.tc ? 8 : INT32_MAX;
     P.most_rows[1] = INT32_MAX;
-    P.row_shift[0] = plan.tc || plan.rowt == 0 ? 3 : plan.rowt == 1 ? 4 : plan.rowt == 2 ? 5 : 6;
-    P.row_shift[1] = 6;
     P.most_splits = plan.most_splits;
     P.scale = scale;
     if (plan.bytes()) {
@@ -2041,12 +2050,21 @@ int bonsai_b200_pages_attn(const bonsai_b200_pages *pages, int layer, const floa
         uint8_t *w = static_cast<uint8_t *>(workspace);
         P.images = w;
         P.redo = reinterpret_cast<int *>(w + plan.image_bytes);
-        if (plan.part_bytes) {
-            P.part_acc = reinterpret_cast<float *>(w + plan.image_bytes + plan.redo_bytes);
-            P.part_ml = reinterpret_cast<float2 *>(P.part_acc + (int64_t)std::max(plan.splits, plan.most_splits) * C.n_tok * n_head * KV_D);
-            P.spans = reinterpret_cast<int *>(w + plan.bytes() - 16);
+        w += plan.image_bytes + plan.redo_bytes;
+        auto take = [&](int64_t rows, float *&acc, float2 *&ml) {
+            if (!rows) return;
+            acc = reinterpret_cast<float *>(w);
+            ml = reinterpret_cast<float2 *>(acc + rows * KV_D);
+            w += PagesPlan::rows_bytes(rows);
+        };
+        take(plan.tc_rows, P.tc_acc, P.tc_ml);
+        for (int c = 0; c < 2; ++c) {
+            take(plan.part_rows[c], P.part_acc[c], P.part_ml[c]);
+            P.part_items[c] = (uint32_t)plan.parts[c];
         }
+        if (plan.joined()) P.spans = reinterpret_cast<int *>(w);
     }
+    for (int c = 0; c < 2; ++c) P.row_shift[c] = plan.row_shift[c];
     const cudaStream_t st = as_stream(stream);
     static SmemOptIn opt[6];
     auto run = [&](auto kernel, SmemOptIn &o, dim3 grid, int threads, int smem, auto... more) {
@@ -2070,7 +2088,7 @@ int bonsai_b200_pages_attn(const bonsai_b200_pages *pages, int layer, const floa
         if (e == cudaSuccess) e = run(pages_tc_kernel, opt[4], dim3((unsigned)plan.tiles, heads, splits), PTC_THREADS, PTC_SMEM_BYTES);
         if (e == cudaSuccess) e = run(pages_redo_kernel, opt[5], dim3(2 * (unsigned)plan.tiles, heads, splits), 32 * pga_warps(4), pga_smem_bytes(4));
     }
-    if (e == cudaSuccess && P.part_acc) {
+    if (e == cudaSuccess && plan.joined()) {
         const int roww = plan.tc ? 1 : plan.most_splits >= 24 ? 8 : plan.most_splits >= 6 ? 2 : 1;
         const int64_t ctas = ((int64_t)C.n_tok * n_head * roww + PGJ_WARPS - 1) / PGJ_WARPS;
         if (ctas > INT32_MAX) return 1;

@@ -125,6 +125,7 @@ constexpr int PGA_BUFS = 2;
 constexpr int pga_warps(int rowt) { return rowt == 4 ? 4 : 8; }       // (ROWT = 0: eight rows)
 constexpr int PGA_Q_STRIDE = 64 + 4;                            // words of a quantised row: 4 g + t are 32 different banks
 constexpr int PGA_W_STRIDE = PG_POS + 8;                        // weights of a row: pairs at 8 g + 2 t, of four rows, are 32 different banks
+constexpr int PGA_NUMBER_AT = 120;                               // (bytes: behind the barriers and flags)
 constexpr int PGA_RING_BYTES = PGA_BUFS * 2 * PG_HEAD_BYTES;
 static_assert(64 * KV_D * 4 <= PGA_RING_BYTES, "the outputs reuse the ring");
 constexpr int pga_smem_bytes(int rowt) {
@@ -136,14 +137,17 @@ struct PageAttn {
     PageCache C;
     const float *q;
     float *out;
-    float *part_acc;            // [splits][token * n_head + head][256], with more than one split
-    float2 *part_ml;            // [splits][token * n_head + head]: maximum, sum of weights
+    // Where a tile's pages are shared by several CTAs: a CTA's sums [256] of each row, and their maximum and sum of weights.  A tile of one CTA writes the outputs.
+    float *tc_acc;              // [splits][token * n_head + head], with more than one split: the sequences on the tensor cores
+    float2 *tc_ml;
+    float *part_acc[2];         // [part_items][rows of a tile], of each class below
+    float2 *part_ml[2];
     int *spans;                 // [2] pages of a CTA, of each class below: what pages_attn_kernel found, for the join
     int layer, n_head, group;
     int span, splits;           // of the sequences on the tensor cores: pages of a CTA, CTAs of a tile
     // of the others, in one class or two by their rows, a launch each: rows of a sequence at most, rows of a tile (as a power of two); CTAs of a tile at most
     int most_rows[2], row_shift[2], most_splits;
-    uint32_t most_items;        // that a launch of theirs can have: more are rows that several sequences claim, and not served
+    uint32_t most_items, part_items[2];         // that a launch of theirs can have, and how many of them share a tile: more are rows that several sequences claim, and not served
     float scale;
     // the call's long sequences on the tensor cores (pages_tc.cuh): images [sequence][page][kv head], whether a CTA is to be done again [tile][kv head][split]
     uint8_t *images;
@@ -200,7 +204,8 @@ __device__ __forceinline__ SeqWork pages_work(const PageAttn &P, int s, int cls)
     return {(n * P.group + (1 << P.row_shift[cls]) - 1) >> P.row_shift[cls], (len + PG_POS - 1) / PG_POS};
 }
 __device__ __forceinline__ int pages_splits(const PageAttn &P, int pages, int span) { return max(1, min(P.most_splits, (pages + span - 1) / span)); }
-// Pages of a CTA such that one round of CTAs (two per SM) takes all of them.
+// Pages of a CTA such that one round of CTAs (two per SM) takes all of them.  Where T tiles have N pages between them, span >= N heads / slots: their items are at most
+// slots + T heads, and those of tiles with several CTAs (more pages than a span, so fewer than twice as many CTAs as spans) at most 2 slots.
 __device__ __noinline__ int pages_span(const PageAttn &P, int cls, int lane, int slots) {
     int64_t total = 0;
     for (int base = 0; base < P.C.n_seq; base += 32) {
@@ -209,13 +214,13 @@ __device__ __noinline__ int pages_span(const PageAttn &P, int cls, int lane, int
     }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    int span = (int)max((int64_t)2, min((int64_t)(1 << 20), (total * P.C.n_head_kv + slots - 1) / slots));
+    int span = (int)max((int64_t)2, min((int64_t)(1 << 26), (total * P.C.n_head_kv + slots - 1) / slots));           // (no sequence has 2^26 pages)
     if (P.C.n_seq > 128) return span;
     for (int step = 0; step < 8; ++step) {              // (a sequence's last CTA has less: some more pages for each, until they fit)
         int items = 0;
         for (int base = 0; base < P.C.n_seq; base += 32) {
             const SeqWork w = pages_work(P, base + lane, cls);
-            items += w.tiles ? w.tiles * pages_splits(P, w.pages, span) : 0;
+            items += w.tiles ? min(w.tiles, 1 << 12) * pages_splits(P, w.pages, span) : 0;           // (2^12 tiles are more than there are slots)
         }
         items = __reduce_add_sync(0xffffffffu, items);
         if ((int64_t)items * P.C.n_head_kv <= slots) break;
@@ -223,15 +228,21 @@ __device__ __noinline__ int pages_span(const PageAttn &P, int cls, int lane, int
     }
     return span;
 }
+// Items of a sequence whose sums are left for the join: all of them or none.  (No more than one too many, so that sums over any sequences stay small.)
+__device__ __forceinline__ uint32_t pages_parts(const PageAttn &P, const SeqWork &w, int cls, int splits) {
+    const uint32_t most = P.part_items[cls] + 1u;       // (below 2^10, and splits times heads below 2^17: most_splits is the slots over the heads)
+    return splits > 1 ? min(min((uint32_t)w.tiles, most) * (uint32_t)(splits * P.C.n_head_kv), most) : 0u;
+}
 
 // One item: rows `tile` of a sequence, one kv head, pages page0 .. page1 - 1 of those that the tile sees.
 template <int ROWT>
 struct PageItem {
     int seq, tile, kvh, split, page0, page1;            // page1 < 0: to the last
+    bool whole;                                         // nobody else has the tile: the outputs are written
 };
 
-template <int ROWT>
-__device__ __forceinline__ bool pages_attn_item(const PageAttn &P, const PageItem<ROWT> &I, uint8_t *smem, int &turn) {
+template <int ROWT, bool TC = false>
+__device__ __forceinline__ bool pages_attn_item(const PageAttn &P, const PageItem<ROWT> &I, uint8_t *smem, int &turn, int cls = 0) {
     constexpr int WARPS = pga_warps(ROWT), THREADS = 32 * WARPS, NB = 8 / WARPS;          // NB: blocks of dims of a warp
     constexpr bool EIGHT = ROWT == 0;
     constexpr int MT = EIGHT ? 1 : ROWT, HR = EIGHT ? 1 : 2;              // row tiles; rows of a thread in each
@@ -240,6 +251,8 @@ __device__ __forceinline__ bool pages_attn_item(const PageAttn &P, const PageIte
     uint64_t *kfull = reinterpret_cast<uint64_t *>(smem), *vfull = kfull + PGA_BUFS;
     int *held = reinterpret_cast<int *>(vfull + PGA_BUFS);                       // [PGA_BUFS] positions of the page that there are
     int *wide0 = held + PGA_BUFS;                                                // [2][8] the block's scales of V are too far apart for one pair of planes
+    static_assert(2 * PGA_BUFS * 8 + PGA_BUFS * 4 + 16 * 4 <= PGA_NUMBER_AT, "");
+    const uint32_t *number = reinterpret_cast<const uint32_t *>(smem + PGA_NUMBER_AT);      // among the items that leave parts: written by a warp in front of the first barrier here
     uint8_t *ring = smem + 128;
     float *ks = reinterpret_cast<float *>(ring + PGA_RING_BYTES);                // [8 blocks][64 positions]
     float *vs0 = ks + 8 * PG_POS;                                                // the same of V times 2^(13 - e), e the exponent of the block's largest; pages alternate
@@ -614,13 +627,17 @@ __device__ __forceinline__ bool pages_attn_item(const PageAttn &P, const PageIte
         sums[tid] = l;
     }
     __syncthreads();
+    if (!TC && !I.whole && *number >= P.part_items[cls]) return true;              // (rows that several sequences claim)
+    float *const acc_at = TC ? P.tc_acc : P.part_acc[cls];
+    float2 *const ml_at = TC ? P.tc_ml : P.part_ml[cls];
+    const size_t part0 = I.whole ? 0 : TC ? (size_t)split * C.n_tok * P.n_head : (size_t)*number * ROWS;
     for (int i = tid; i < n_rows * (KV_D / 4); i += THREADS) {
         const int r = i / (KV_D / 4), c = i % (KV_D / 4);
         float4 x = reinterpret_cast<const float4 *>(ring)[(size_t)r * (KV_D / 4) + c];
         const float l = sums[r];
         const int row = tile * ROWS + r, tok = row / P.group;
         const size_t at = (size_t)(range.begin + tok) * P.n_head + kvh * P.group + (row - tok * P.group);
-        if (P.part_acc == nullptr) {                    // nobody has more than one split
+        if (I.whole) {
             const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);             // a row that sees nothing is zeros
             x = make_float4(__fmul_rn(x.x, inv), __fmul_rn(x.y, inv), __fmul_rn(x.z, inv), __fmul_rn(x.w, inv));
             float *o = P.out + at * KV_D + 4 * c;
@@ -630,9 +647,9 @@ __device__ __forceinline__ bool pages_attn_item(const PageAttn &P, const PageIte
                 o[0] = x.x; o[1] = x.y; o[2] = x.z; o[3] = x.w;
             }
         } else {
-            const size_t at2 = (size_t)split * C.n_tok * P.n_head + at;
-            reinterpret_cast<float4 *>(P.part_acc)[at2 * (KV_D / 4) + c] = x;
-            if (c == 0) P.part_ml[at2] = make_float2(most[r], l);
+            const size_t at2 = part0 + (TC ? at : (size_t)r);
+            reinterpret_cast<float4 *>(acc_at)[at2 * (KV_D / 4) + c] = x;
+            if (c == 0) ml_at[at2] = make_float2(most[r], l);
         }
     }
     return true;
@@ -658,8 +675,8 @@ __global__ void __launch_bounds__(32 * pga_warps(ROWT), 2) pages_attn_kernel(con
     int turn = 0;
     for (uint32_t item = blockIdx.x; item < P.most_items; item += gridDim.x) {
         // whose: the sequences' items one after the other, every warp for itself (a sequence has most_items at most, below 2^31; where several claim rows, sums stop there)
-        uint32_t before = 0;
-        PageItem<ROWT> I = {-1, 0, 0, 0, 0, 0};
+        uint32_t before = 0, parts = 0;
+        PageItem<ROWT> I = {-1, 0, 0, 0, 0, 0, true};
         for (int base = 0; base < P.C.n_seq && I.seq < 0; base += 32) {
             const SeqWork w = pages_work(P, base + lane, cls);
             const int splits = pages_splits(P, w.pages, span);
@@ -671,6 +688,10 @@ __global__ void __launch_bounds__(32 * pga_warps(ROWT), 2) pages_attn_kernel(con
             }
             const unsigned past = __ballot_sync(0xffffffffu, before + sum > item);
             const uint32_t front = __shfl_up_sync(0xffffffffu, sum, 1);
+            if (threadIdx.x < 32) {                     // (by a warp that does not issue copies: nobody needs it before the item's end)
+                const uint32_t own = lane < (past ? __ffs(past) - 1 : 32) ? pages_parts(P, w, cls, splits) : 0u;
+                parts = min(parts + __reduce_add_sync(0xffffffffu, own), 1u << 30);
+            }
             if (past) {
                 const int at = __ffs(past) - 1, rest = (int)(item - before - __shfl_sync(0xffffffffu, lane ? front : 0u, at)), n = __shfl_sync(0xffffffffu, splits, at);
                 const int pair = rest / heads;
@@ -680,11 +701,13 @@ __global__ void __launch_bounds__(32 * pga_warps(ROWT), 2) pages_attn_kernel(con
                 I.split = pair - I.tile * n;
                 I.page0 = I.split * span;
                 I.page1 = I.split == n - 1 ? -1 : I.page0 + span;
+                I.whole = n == 1;
+                if (threadIdx.x == 0) *reinterpret_cast<uint32_t *>(smem + PGA_NUMBER_AT) = parts + (uint32_t)rest;
             }
             before += __shfl_sync(0xffffffffu, sum, 31);
         }
         if (I.seq < 0) return;                          // CTA-uniform
-        if (!pages_attn_item<ROWT>(P, I, smem, turn)) return;        // (a wait ran out: the CTA leaves as a whole)
+        if (!pages_attn_item<ROWT>(P, I, smem, turn, cls)) return;        // (a wait ran out: the CTA leaves as a whole)
         __syncthreads();
     }
 }
@@ -711,9 +734,10 @@ __global__ void __launch_bounds__(32 * pga_warps(4), 2) pages_redo_kernel(const 
     I.split = blockIdx.z;
     I.page0 = I.split * P.span;
     I.page1 = I.split == P.splits - 1 ? -1 : I.page0 + P.span;
+    I.whole = P.tc_acc == nullptr;
     __syncthreads();
     int turn = 0;
-    pages_attn_item<4>(P, I, smem, turn);
+    pages_attn_item<4, true>(P, I, smem, turn);
 }
 
 // The splits of a row added up: ROWW warps per row (token, head), four dims and four more a lane.  A row's splits are those that its own positions reach.
@@ -727,7 +751,10 @@ __global__ void __launch_bounds__(32 * PGJ_WARPS) pages_join_kernel(const __grid
     const int64_t rows = (int64_t)C.n_tok * P.n_head, row = (int64_t)blockIdx.x * (PGJ_WARPS / ROWW) + warp / ROWW;
     pdl_wait_prior_grid();
     pdl_launch_dependents();
-    int n = 0;                                          // 0: not a row of a sequence that was served
+    int n = 0;                                          // 0: not a row of a sequence that was served, or its outputs are there
+    const float *acc = nullptr;                         // its first part; the others lie `step` rows behind each other
+    const float2 *pml = nullptr;
+    int64_t step = rows;
     if (row < rows) {
         const int tok = (int)(row / P.n_head);
         const int s = seq_of_row(C.start, C.n_seq, tok, lane);
@@ -737,14 +764,36 @@ __global__ void __launch_bounds__(32 * PGJ_WARPS) pages_join_kernel(const __grid
             if (r.n > 0 && tok >= r.begin && len >= 0 && len <= (int64_t)C.table_stride * PG_POS) {
                 const int seen = len - r.n + (tok - r.begin) + 1;
                 const int pages = (max(seen, 0) + PG_POS - 1) / PG_POS;
-                const bool tc = pages_on_tc(P, r.n, len);
-                const int span = tc ? P.span : P.spans[pages_class(P, r.n)];
-                n = max(1, min(tc ? P.splits : pages_splits(P, (len + PG_POS - 1) / PG_POS, span), (pages + span - 1) / span));
+                if (pages_on_tc(P, r.n, len)) {
+                    if (P.tc_acc) {
+                        n = max(1, min(P.splits, (pages + P.span - 1) / P.span));
+                        acc = P.tc_acc + row * KV_D;
+                        pml = P.tc_ml + row;
+                    }
+                } else {
+                    const int cls = pages_class(P, r.n), span = P.spans[cls];
+                    const int splits = pages_splits(P, (len + PG_POS - 1) / PG_POS, span);
+                    if (splits > 1) {
+                        uint32_t parts = 0;             // of the sequences in front
+                        for (int i = lane; i < s; i += 32) {
+                            const SeqWork x = pages_work(P, i, cls);
+                            parts = min(parts + pages_parts(P, x, cls, pages_splits(P, x.pages, span)), 1u << 20);
+                        }
+                        const int h = (int)(row - (int64_t)tok * P.n_head), kvh = h / P.group, at = (tok - r.begin) * P.group + (h - kvh * P.group), shift = P.row_shift[cls], tile = at >> shift;
+                        n = max(1, min(splits, (pages + span - 1) / span));
+                        const size_t first = (size_t)__reduce_add_sync(0xffffffffu, parts) + (size_t)tile * splits * C.n_head_kv + kvh;
+                        if (first + (size_t)(n - 1) * C.n_head_kv >= P.part_items[cls]) n = 0;
+                        const size_t from = (first << shift) + (at & ((1 << shift) - 1));
+                        step = (int64_t)C.n_head_kv << shift;
+                        acc = P.part_acc[cls] + from * KV_D;
+                        pml = P.part_ml[cls] + from;
+                    }
+                }
             }
         }
     }
     float m = -INFINITY, l = 0.0f;
-    for (int i = lane; i < n; i += 32) m = fmaxf(m, P.part_ml[i * rows + row].x);
+    for (int i = lane; i < n; i += 32) m = fmaxf(m, pml[i * step].x);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
@@ -753,9 +802,9 @@ __global__ void __launch_bounds__(32 * PGJ_WARPS) pages_join_kernel(const __grid
         float4 c[4], d[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int64_t at = (int64_t)min(i0 + e * ROWW, n - 1) * rows + row;
-            const float4 *src = reinterpret_cast<const float4 *>(P.part_acc) + at * (KV_D / 4) + lane;
-            x[e] = P.part_ml[at];
+            const int64_t at = (int64_t)min(i0 + e * ROWW, n - 1) * step;
+            const float4 *src = reinterpret_cast<const float4 *>(acc) + at * (KV_D / 4) + lane;
+            x[e] = pml[at];
             c[e] = src[0];
             d[e] = src[32];
         }

@@ -466,9 +466,9 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) pages_tc_kernel(const __grid_c
     if (threadIdx.x == 0) P.redo[((size_t)blockIdx.x * C.n_head_kv + kvh) * P.splits + split] = redo && all_ok ? 1 : 0;
     if (redo || !all_ok) return;
     const float l = __fadd_rn(__fadd_rn(red[row], red[ATC_M + row]), __fadd_rn(red[2 * ATC_M + row], red[3 * ATC_M + row]));
-    const float inv = P.part_acc != nullptr ? 1.0f : l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);           // a row that sees nothing is zeros
-    float *dst = P.part_acc != nullptr ? P.part_acc + (size_t)split * C.n_tok * P.n_head * KV_D : P.out;
-    if (P.part_acc != nullptr && cg == 0 && row < n_rows) P.part_ml[(size_t)split * C.n_tok * P.n_head + row_at(row) / KV_D] = make_float2(m_run, l);
+    const float inv = P.tc_acc != nullptr ? 1.0f : l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);             // a row that sees nothing is zeros
+    float *dst = P.tc_acc != nullptr ? P.tc_acc + (size_t)split * C.n_tok * P.n_head * KV_D : P.out;
+    if (P.tc_acc != nullptr && cg == 0 && row < n_rows) P.tc_ml[(size_t)split * C.n_tok * P.n_head + row_at(row) / KV_D] = make_float2(m_run, l);
     if ((reinterpret_cast<uintptr_t>(dst) & 15u) == 0) {
 #pragma unroll
         for (int c = 0; c < 16; ++c)

@@ -1,0 +1,85 @@
+"""How a call's attention is divided: long contexts beside prompts, many sequences, and workspaces that hold exactly what is asked for."""
+import math
+
+import numpy as np
+import pytest
+
+from test_gpu_sequences import Cache, attention, close, run_attention, status_is_clear  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def queries(c, n_head, seed=5):
+    import torch
+    return torch.randn(c.n_tok, n_head, 256, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda")
+
+
+def run_guarded(gpu, c, q, max_len):
+    """The call with a workspace of exactly the bytes asked for, 4 KB of marks on either side of it and of the outputs."""
+    import torch
+    size, n = c.view.attn_workspace(max_len, q.shape[1]), q.numel()
+    room = torch.full((size + 8192,), 0xA5, dtype=torch.uint8, device="cuda")
+    room[4096:4096 + size].view(torch.float32).fill_(math.nan)
+    outs = torch.full((n + 2048,), 7.0, device="cuda")
+    out = outs[1024:1024 + n].reshape(q.shape)
+    pool = c.d_pool.clone()
+    assert c.view.attn(0, q, out, q.shape[1], max_len, room[4096:4096 + size] if size else None, 0.0625) == 0
+    assert bool((room[:4096] == 0xA5).all()) and bool((room[4096 + size:] == 0xA5).all())
+    assert bool((outs[:1024] == 7).all()) and bool((outs[1024 + n:] == 7).all()) and torch.equal(pool, c.d_pool)
+    return out
+
+
+CASES = [  # lengths, new tokens, query heads, kv heads, max_len
+    ([20000, 300, 9000], [1, 200, 2], 24, 4, 20000),                           # two chats of long contexts beside a prompt: 8 rows a tile and 74 CTAs, 64 rows
+    ([13000, 700, 5000, 64, 8000], [5, 600, 1, 0, 21], 24, 4, 13000),          # the same with drafted tokens (64 rows a tile)
+    ([9000, 300], [2, 150], 8, 8, 9000), ([9000, 400], [3, 400], 5, 1, 9000),
+    ([9000], [1], 24, 4, 9000), ([9000], [9], 24, 4, 9000), ([9000, 30], [1, 1], 64, 64, 9000), ([5000] * 3, [7] * 3, 24, 4, 5000),
+    ([9000, 300], [2, 200], 24, 4, 300), ([9000, 9000], [2, 200], 24, 4, 129),         # longer than it was said to be
+    ([12000, 4000, 3000], [30, 25, 60], 24, 4, 1 << 22),                       # no room for images: everything on mma.sync
+    ([900, 200], [300, 200], 3, 1, 900)]
+
+
+@pytest.mark.parametrize("lens,new,n_head,n_head_kv,max_len", CASES)
+def test_long_contexts(gpu, lens, new, n_head, n_head_kv, max_len):
+    c = Cache(gpu, lens, new, n_head_kv=n_head_kv, behind=2, seed=sum(lens))
+    q = queries(c, n_head)
+    want, size = attention(c, q)
+    close(run_guarded(gpu, c, q, max_len), want, size, -(-max(lens) // 64))
+
+
+@pytest.mark.parametrize("n_seq,each,prompt", [(129, 1, 0), (300, 2, 0), (200, 1, 150), (140, 9, 0)])
+def test_many_sequences(gpu, n_seq, each, prompt):
+    """More sequences than spans are fitted to; a prompt among them; some pause."""
+    rng = np.random.default_rng(n_seq)
+    new = [0 if i % 7 == 3 else each for i in range(n_seq)]
+    lens = [int(n + rng.integers(0, 500)) for n in new]
+    lens[5] += 3000
+    if prompt:
+        new[n_seq // 2], lens[n_seq // 2] = prompt, prompt + 100
+    c = Cache(gpu, lens, new, n_head_kv=2, seed=n_seq)
+    q = queries(c, 8)
+    want, size = attention(c, q)
+    close(run_guarded(gpu, c, q, max(lens)), want, size, -(-max(lens) // 64))
+
+
+def test_long_context_of_few_tokens(gpu):
+    """Thousands of positions for 1 to 5 tokens, by every number of rows that a tile has."""
+    for new, n_head, n_head_kv in ((1, 24, 4), (2, 24, 4), (5, 24, 4), (4, 32, 1)):
+        c = Cache(gpu, [15000], [new], n_head_kv=n_head_kv, seed=new)
+        q = queries(c, n_head)
+        want, size = attention(c, q)
+        close(run_attention(gpu, c, q), want, size, 235)
+
+
+def test_a_sequence_does_not_change_with_its_neighbours_pages(gpu):
+    """A chat's outputs beside a prompt and alone: within the bound of both (the division differs, and with it the last bits)."""
+    c = Cache(gpu, [6000, 500], [1, 300], seed=21)
+    q = queries(c, 24)
+    want, size = attention(c, q)
+    out = run_guarded(gpu, c, q, 6000)
+    close(out, want, size, 94)
+    start = c.view._keep[3]
+    start[1:] = 1                                       # the prompt pauses: its rows are nobody's
+    alone = run_guarded(gpu, c, q, 6000)
+    close(alone[:1], want[:1], size[:1], 94)
+    assert bool((alone[1:] == 7).all())

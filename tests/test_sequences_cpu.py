@@ -90,6 +90,24 @@ def test_workspace_sizes():
         assert bb.gdn_seqs_workspace(*bad) == 0
 
 
+@pytest.mark.parametrize("n_head,n_head_kv", [(24, 4), (6, 6), (32, 1), (64, 64), (5, 1)])
+def test_workspaces_are_bounded(n_head, n_head_kv):
+    """Sums of CTAs that share a tile: at most twice as many tiles as CTAs run at once (2 per SM) of 8 and of 64 rows, and beside prompts 8 tiles of 128 rows per SM.  Images: 2.5 GB."""
+    import bonsai_b200 as bb
+    row = 4 * 256 + 8
+    few, tc = 2 * 2 * 148 * (8 + 64) * row, 8 * 148 * 128 * row
+    for n_tok in (1, 5, 33, 128, 512, 800, 2049, 5333, 16384, 100000):
+        for max_len in (1, 129, 2501, 20400, 40000, 262144, 1 << 30):
+            for n_seq in (1, 2, 16, 17, 1000, 100000):
+                size = bb.pages_attn_workspace(n_tok, max_len, n_seq, n_head, n_head_kv)
+                assert size <= few + tc + (5 << 29) + (1 << 24), (n_tok, max_len, n_seq, size)
+                if n_tok * (n_head // n_head_kv) < 256:         # no prompts
+                    assert size <= few + 64
+    # many tokens of sequences that may be long, for whose images there is no room
+    for n_tok, max_len, n_seq in ((2049, 262144, 2), (2015, 20400, 16), (8192, 40000, 16)):
+        assert bb.pages_attn_workspace(n_tok, max_len, n_seq, 24, 4) <= few + 64
+
+
 def test_copy_refusals():
     import bonsai_b200
     f = bonsai_b200.lib().bonsai_b200_pages_copy
