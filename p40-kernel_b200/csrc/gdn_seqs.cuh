@@ -172,6 +172,9 @@ __global__ void __launch_bounds__(GDN_WARPS * 32) gdn_seqs_step_kernel(const __g
 // Products are fp32 to about 2^-22: each operand is two fp16 planes, high and low, of its values times a power of two -- K, Q, Tb and P a row, S, V - e^G K S and U eight columns
 // -- of which a plane pair holds 2^-38 of the largest; three of the four products on mma.sync (m16n8k16), sums fp32.  (Two TF32 parts, which need no powers of
 // two, are four times the instructions for the same: the tensor core's 554 TFLOP/s of fp16 are 278 of TF32, and the parts were made anew by every warp.)
+// What eight columns of V - e^G K S hold less than 2^-20 of the largest (a token behind one that was 2^20 times as large and is forgotten, a column beside one that is: planes have
+// 18 bits left for it at most) would be lost to the state for good: such a chunk goes token by token, as one with values past 2^60 does.  It is looked for by pairs of neighbouring columns,
+// which of ordinary values are both that small once in 10^12.
 // The tensor core cuts the last bits of a sum off instead of rounding it, so a sum is of one step of 16 values, small products first, and rounded additions join the
 // steps.  (One sum over all steps, the state's own among them: error of 2048 tokens' outputs against 64 bits 1.6e-6, now 2.3e-7.)
 constexpr int GDC_T = 64, GDC_D = 128;
@@ -188,6 +191,7 @@ constexpr int GDC_STEP_MOST = 24;                                     // tokens 
 // 2^-s of Tb, 2^-s of P; then e^G_63, 2^-s_min, whether the chunk is to go token by token.
 constexpr int GDC_KQ_REC = 4 * GDC_KP + 2 * GDC_T * 4, GDC_TP_PLANES = 4 * GDC_TP, GDC_VEC = 5 * GDC_T + 4, GDC_TP_REC = GDC_TP_PLANES + GDC_VEC * 4;
 constexpr int GDC_QB = 16 * GDC_KB;                                    // 16 rows of a plane of Q
+constexpr uint32_t GDC_FAR = 20;                                       // (powers of two)
 constexpr int gdc_prep_smem() { return 2 * GDC_KP + 4 * GDC_QB + GDC_T * 8 + 3 * GDC_T * 4 + 32; }
 constexpr int gdc_scan_smem() { return 6 * GDC_KP + 4 * GDC_TP + GDC_T * GDC_VS * 4 + 2 * GDC_SP + 6 * GDC_UP + GDC_VEC * 4 + 5 * 8 * 4 + 4 * 8; }
 static_assert(gdc_scan_smem() <= 227 * 1024 && 4 * gdc_prep_smem() <= 224 * 1024 && GDC_D * GDC_CB * 2 >= GDC_D * GDC_COLS * 4 && 2 * GDC_T * GDC_TS * 4 <= 2 * GDC_KP, "");
@@ -712,9 +716,16 @@ __global__ void __launch_bounds__(GDC_THREADS, 1) gdn_scan_kernel(const __grid_c
         }
         tiles_most(r[0], r_most + j0);
         int slow = __syncthreads_or(odd ? 1 : 0);
+        bool far = false;                                       // values that the largest of their eight columns leaves fewer than 18 bits
 #pragma unroll
         for (int j = 0; j < NH; ++j) {
-            const float f = atc_pow2(atc_shift(r_most[j0 + j], 63));
+            const uint32_t largest = r_most[j0 + j];
+            const float f = atc_pow2(atc_shift(largest, 63));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t own = max(atc_abs_bits(r[0][j][2 * h]), atc_abs_bits(r[0][j][2 * h + 1]));
+                far = far || (own != 0u && own + (GDC_FAR << 23) < largest);
+            }
 #pragma unroll
             for (int h = 0; h < 2; ++h) store_planes(rp + (16 * mt + g + 8 * h) * GDC_CB + 16 * (j0 + j) + 4 * t, GDC_UP, r[0][j][2 * h], r[0][j][2 * h + 1], f);
         }
@@ -724,7 +735,7 @@ __global__ void __launch_bounds__(GDC_THREADS, 1) gdn_scan_kernel(const __grid_c
             float u[1][NH][4], x[NH][4];
             const uint32_t a[1] = {smem_u32(tp) + 16 * mt * GDC_TB + at_t};
             gdc_product<1, NH, GDC_T / 16, false, true>(u, a, GDC_TP, 32, b_r + 16 * j0, GDC_UP, 16 * GDC_CB, 32, mt + 1);
-            odd = false;
+            odd = far;
             // e^G Q S here, between products that the whole chunk waits for: its instructions fill their latencies (2048 tokens: beside K S 277 us, here 272)
             const uint32_t aq[1] = {smem_u32(qp) + 16 * mt * GDC_KB + at_k};
             gdc_product<1, NH, GDC_D / 16, false, true>(y, aq, GDC_KP, 32, b_s + 16 * j0, GDC_SP, 16 * GDC_CB, 32);
