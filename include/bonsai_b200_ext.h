@@ -282,8 +282,8 @@ int bonsai_b200_qk_norm_rope(const float *q, const float *k, const float *q_weig
 
 /* A K/V cache in pages.  The pool is the caller's memory (16-byte aligned), n_pages pages of
  *   [n_layers][K, V][n_head_kv][BONSAI_B200_PAGE_POSITIONS][256 / 32 blocks of 34 bytes]
- * with Q8_0 blocks as bonsai_kv_append lays them out.  A block's scale is its largest magnitude times 1 / 127, rounded once, in fp32 and then to fp16
- * (bonsai_kv_append divides: the scale's last bit differs in one block of 23, about one code in 10^7).  Sequence s has len[s] positions, the new tokens of the call (rows start[s] ..) being the last of them;
+ * with Q8_0 blocks as bonsai_kv_append lays them out.  A block's scale is its largest magnitude times 1 / 127, rounded once, in fp32 and then to fp16 (bonsai_kv_append divides: the
+ * stored scales are the same, a code whose quotient lies within 2^-16 of a half can be the neighbouring one, in one value of 10^7).  Sequence s has len[s] positions, the new tokens of the call (rows start[s] ..) being the last of them;
  * position p lies in page table[s * table_stride + p / 64], row p % 64.  Sequences may share pages that none of the call's rows goes to. */
 #define BONSAI_B200_PAGE_POSITIONS 64
 typedef struct bonsai_b200_pages {
@@ -294,7 +294,7 @@ typedef struct bonsai_b200_pages {
 /* Stores the rows k, v ([n_tok][n_head_kv][256]) of the new tokens of one layer. */
 int bonsai_b200_pages_append(const bonsai_b200_pages *pages, int layer, const float *k, const float *v, bonsai_stream stream);
 /* Attention of the new tokens (q, out [n_tok][n_head][256]) of one layer over the cache, their own rows included: each as bonsai_kv_attn_decode computes it at
- * its position -- queries quantised to Q8_0 (as above), positions up to its own seen -- within 1e-5 of the largest output of a head.  A token without a position
+ * its position on the same rows and codes -- queries quantised to Q8_0 (as above), positions up to its own seen -- within 1e-5 of the largest output of a head.  A token without a position
  * (len[s] smaller than its new tokens) sees nothing: zeros.  max_len: no smaller than every len, for the division of the work; longer sequences are served
  * all the same, more slowly.  workspace: 16-byte aligned device memory of bonsai_b200_pages_attn_workspace(the same sizes) bytes (NULL where that is 0): sums
  * of rows whose pages several CTAs share (0.2 GB at most), and beside prompts images of pages: 133 KB a page and kv head, for max_len of each sequence that the call's tokens could make

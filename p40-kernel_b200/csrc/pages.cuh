@@ -25,7 +25,8 @@ __device__ __forceinline__ uint8_t *page_rows(const PageCache &C, int page, int 
 
 // ---- append -----------------------------------------------------------------------------------------------------------------------------------
 // One warp per (token, kv head) row of K and of V, as kv_append_kernel.  A block's scale is its largest magnitude times 1 / 127, one rounded product where that kernel
-// divides: a scale's last bit differs in one block of 23, and with it about one code in 10^7.
+// divides: the fp32 scales differ in the last bit for one magnitude in 21, the fp16 ones that are stored for none (all 2^23 mantissas at every exponent looked at), and a code whose
+// quotient lies beside a half is the neighbouring one in one value of 10^7.
 constexpr float PG_SCALE = 1.0f / 127.0f;
 template <bool VEC>
 __global__ void __launch_bounds__(32 * KV_APPEND_WARPS) pages_append_kernel(const __grid_constant__ PageCache C, const float *ksrc, const float *vsrc, int layer) {

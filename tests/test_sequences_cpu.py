@@ -151,6 +151,21 @@ def test_python_refusals():
         bb.Pages(x.byte(), x.int().reshape(1, -1), x[:1].int(), x[:2].int(), 1, 1, 1)
 
 
+@pytest.mark.parametrize("exponent", [6, -8, -12, -20])
+def test_scales_by_product_and_by_quotient(exponent):
+    """Largest magnitude times 1 / 127 and over 127 are the same fp16 scale for every fp32 magnitude (normal ones and subnormal ones), though not the same fp32 scale."""
+    import numpy as np
+    x = (np.arange(1 << 23, dtype=np.uint32) | np.uint32(127 << 23)).view(np.float32) * np.float32(2.0 ** exponent)
+
+    def half(d):
+        d = d.astype(np.float64)
+        step = np.ldexp(1.0, np.maximum(np.frexp(d)[1] - 1, -14) - 10)
+        return np.floor(d / step + 0.5) * step
+    product, quotient = x * (np.float32(1) / np.float32(127)), x / np.float32(127)
+    assert 0.04 < (product != quotient).mean() < 0.05
+    assert np.array_equal(half(product), half(quotient))
+
+
 # ---- the book ------------------------------------------------------------------------------------------
 def check(book, n_pages):
     users = [0] * n_pages
