@@ -83,3 +83,32 @@ def test_attention(gpu, n, new):
     # each side is within 1e-5 of the largest output of the value (as its own tests have it)
     err = (out - want).abs().amax((1, 2)) / want.abs().amax((1, 2))
     assert err.max().item() <= 2e-5
+
+
+@pytest.mark.parametrize("new", [1, 3, 40, 130])
+def test_queries_that_are_no_numbers(gpu, new):
+    """An infinity or NaN in a query is its own row's: what bonsai_kv_attn_decode makes of it, and nothing of any other row's."""
+    import torch
+    n, layer = 400, 2
+    g = torch.Generator(device="cuda").manual_seed(new)
+    k, v = (whole_scales(torch.randn(n, HKV, D, generator=g, device="cuda")) for _ in range(2))
+    q = whole_scales(torch.randn(new, H, D, generator=g, device="cuda"))
+    q[new // 2, 3, 40], q[new // 2, 9, 0], q[new - 1, 23, 255] = float("inf"), float("nan"), float("-inf")
+    kv = gpu.KVCache(n)
+    assert kv.append_batch(layer, 0, n, k, v) == 0
+    c = Cache(gpu, [n], [n])
+    assert c.view.append(0, k, v) == 0
+    view = gpu.Pages(c.d_pool, ints(c.table), ints([n]), ints([0, new]), 1, HKV, new)
+    size = view.attn_workspace(n, H)
+    out, want = torch.empty_like(q), torch.empty_like(q)
+    assert view.attn(0, q, out, H, n, torch.empty(size, dtype=torch.uint8, device="cuda") if size else None, 0.0625) == 0
+    for t in range(new):
+        assert kv.attn_decode(layer, n - new + t, q[t], want[t]) == 0
+    torch.cuda.synchronize()
+    kv.close()
+    odd = [(new // 2, 3), (new - 1, 23)]
+    for t, h in odd:
+        assert bool((~out[t, h].isfinite()).all()) and bool((~want[t, h].isfinite()).all())
+        out[t, h] = want[t, h] = 0.0
+    assert bool(out.isfinite().all())
+    assert ((out - want).abs().amax((1, 2)) / want.abs().amax((1, 2))).max().item() <= 2e-5

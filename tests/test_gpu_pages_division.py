@@ -83,3 +83,33 @@ def test_a_sequence_does_not_change_with_its_neighbours_pages(gpu):
     alone = run_guarded(gpu, c, q, 6000)
     close(alone[:1], want[:1], size[:1], 94)
     assert bool((alone[1:] == 7).all())
+
+
+@pytest.mark.parametrize("lens,new,n_head,n_head_kv,scale", [([300], [2], 200, 1, 0.0625), ([300, 90], [5, 3], 200, 1, 0.0625), ([200], [40], 24, 4, -0.0625), ([200], [3], 24, 4, 0.0),
+                                                             ([300, 64], [150, 1], 24, 4, 0.0)])
+def test_wide_groups_and_other_scales(gpu, lens, new, n_head, n_head_kv, scale):
+    """More query heads to a kv head than a tile has rows; scores that are turned round, or all the same."""
+    import torch
+    c = Cache(gpu, lens, new, n_head_kv=n_head_kv, seed=n_head)
+    q = queries(c, n_head)
+    want, size = attention(c, q, scale=scale)
+    close(run_attention(gpu, c, q, scale=scale), want, size, -(-max(lens) // 64))
+
+
+def test_two_calls_at_once(gpu):
+    """Two caches on two streams, each with its own workspace, run over each other: the bits of each by itself."""
+    import torch
+    made = []
+    for i, (lens, new) in enumerate((([6000, 400], [1, 300]), ([3000, 2000, 900], [2, 2, 90]))):
+        c = Cache(gpu, lens, new, seed=30 + i)
+        q = queries(c, 24, 40 + i)
+        made.append((c, q, run_attention(gpu, c, q), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(5):
+        for i, (c, q, _, stream) in enumerate(made):
+            with torch.cuda.stream(stream):
+                outs[i].append(run_attention(gpu, c, q))
+    torch.cuda.synchronize()
+    for (_, _, want, _), got in zip(made, outs):
+        assert all(torch.equal(want, o) for o in got)
