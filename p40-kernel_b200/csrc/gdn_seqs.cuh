@@ -31,8 +31,8 @@ __device__ __forceinline__ int gdn_slot_of(const GdnSeqs &P, int s) {
 // ---- token by token: the form for few tokens --------------------------------------------------------------------------------------------
 // As gdn_step_kernel: one CTA per (sequence, value head, 32 PER columns of the state), eight warps, lane = PER columns, warp w holds rows w, w + 8, ... in registers over all of
 // the sequence's tokens: the state is read once and written once.  Sequences of more than `most` tokens are not its own.
-// Bound by memory for many sequences (16 of one token: 101 MB in 23 us; of 32 columns a CTA 28.7, where a state's tile is 16 KB), for few tokens of one by latency: 7 us and about 0.8 a
-// token more.
+// Bound by memory for many sequences (16 of one token: 101 MB in 23 us; of 32 columns a CTA 28.7, where a state's tile is 16 KB), for few tokens of one by latency: 4.3 us for
+// one token of 48 heads, about 1.0 for each one more (two sums over eight warps and three barriers).  gdn_step_kernel, which asks L2 for its state and inputs in front of the wait, takes 2.7.
 template <int PER>
 struct GdnCols { float x[PER]; };
 template <int PER>
@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(GDC_THREADS) gdn_planes_kernel(const __grid_co
     }
 }
 
-// grid (the same chunks, value heads): Tb and P.  Bound by issue and latency: 59 us for 2048 tokens and 48 heads, four CTAs per SM, whose rounds are three (with all of Q in
+// grid (the same chunks, value heads): Tb and P.  Bound by issue and latency: 59 us for 2048 tokens and 48 heads, four CTAs per SM (128 registers, 48 bytes spilled a thread), whose rounds are three (with all of Q in
 // shared memory and P passing through it, three CTAs, four rounds, 75 us).  About 3900 instructions a warp, half of them the inverse.
 __global__ void __launch_bounds__(GDC_PREP_THREADS, 4) gdn_chunk_kernel(const __grid_constant__ GdnSeqs P, const uint8_t *kq_recs, uint8_t *tp_recs) {
     extern __shared__ __align__(16) uint8_t gdc_smem[];
@@ -736,7 +736,7 @@ __global__ void __launch_bounds__(GDC_THREADS, 1) gdn_scan_kernel(const __grid_c
             const uint32_t a[1] = {smem_u32(tp) + 16 * mt * GDC_TB + at_t};
             gdc_product<1, NH, GDC_T / 16, false, true>(u, a, GDC_TP, 32, b_r + 16 * j0, GDC_UP, 16 * GDC_CB, 32, mt + 1);
             odd = far;
-            // e^G Q S here, between products that the whole chunk waits for: its instructions fill their latencies (2048 tokens: beside K S 277 us, here 272)
+            // e^G Q S here, between products that the whole chunk waits for: its instructions fill their latencies (2048 tokens: beside K S 277 us, here 272, each without the look for values far apart, 3 us)
             const uint32_t aq[1] = {smem_u32(qp) + 16 * mt * GDC_KB + at_k};
             gdc_product<1, NH, GDC_D / 16, false, true>(y, aq, GDC_KP, 32, b_s + 16 * j0, GDC_SP, 16 * GDC_CB, 32);
 #pragma unroll

@@ -9,6 +9,7 @@
 // outputs; of three warps more one issues the tensor core's instructions, which has a page's scores and the outputs of the page before in flight meanwhile, two copy k and v:
 //   tensor core   q . k of page i + 1          | weights x v of page i
 //   threads       weights of page i, outputs of page i - 1 added, weights to tensor memory | scores of page i + 1 read
+// (Its 19 warps leave a thread 96 registers, of which the 64 sums are most: 260 bytes of stores and 364 of loads spilled a thread.)
 // (The issue is a warp's whole time: 2100 cycles for a page's scores, 1100 for its outputs.  By one of the sixteen warps a page took 8000 cycles, with the copies from the issuing
 // warp 5850.)
 // Tensor memory, all 512 columns: 256 output, 64 scores, 64 weights, 128 q low.  Shared memory: q high, k and v images of one page, 64 KB each.
