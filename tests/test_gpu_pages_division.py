@@ -4,7 +4,7 @@ import math
 import numpy as np
 import pytest
 
-from test_gpu_sequences import Cache, attention, close, run_attention, status_is_clear  # noqa: F401
+from test_gpu_sequences import Cache, attn_bound, number, q8_0, run_attention, status_is_clear  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -12,6 +12,35 @@ pytestmark = pytest.mark.gpu
 def queries(c, n_head, seed=5):
     import torch
     return torch.randn(c.n_tok, n_head, 256, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda")
+
+
+def attention(c, q, layer=0, scale=0.0625):
+    """Each token over the positions up to its own in 64 bits, a kv head's rows at once; rows of nobody 7.  With it the size of an output's error, as test_gpu_sequences has it."""
+    import torch
+    n_head, group = q.shape[1], q.shape[1] // c.hkv
+    codes, d = q8_0(q.cpu().numpy())
+    qn = torch.from_numpy((codes.astype(np.float64) * d[..., None].astype(np.float64)).reshape(q.shape)).cuda()
+    out, size = torch.full(q.shape, 7.0, dtype=torch.float64, device="cuda"), torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+    for s, n in enumerate(c.new):
+        if n == 0:
+            continue
+        rows, length = slice(c.start[s], c.start[s] + n), c.lens[s]
+        seen = torch.arange(length, device="cuda")[None] <= torch.arange(length - n, length, device="cuda")[:, None]
+        held = c.pool[c.table[s, :-(-length // 64)], layer]
+        for j in range(c.hkv):
+            k, v = (torch.from_numpy(number(held[:, i, j].reshape(-1, 8, 34)[:length])).cuda() for i in range(2))
+            for h in range(j * group, (j + 1) * group):
+                x = (qn[rows, h] @ k.T * scale).masked_fill(~seen, -math.inf)
+                p = torch.softmax(x, -1)
+                out[rows, h] = p @ v
+                big = (qn[rows, h].abs() @ k.abs().T).masked_fill(~seen, 0.0).amax(-1, keepdim=True) * abs(scale)
+                size[rows, h] = (1 + big) * (p @ v.abs())
+    return out, size
+
+
+def close(got, want, size, n_pages):
+    over = (got.double() - want).abs() - attn_bound(size, n_pages)
+    assert not bool(over.isnan().any()) and over.max().item() <= 0, f"{((got.double() - want).abs() / attn_bound(size, n_pages).clamp(min=1e-300)).max().item():.2f} of the bound"
 
 
 def run_guarded(gpu, c, q, max_len):
@@ -33,7 +62,7 @@ CASES = [  # lengths, new tokens, query heads, kv heads, max_len
     ([20000, 300, 9000], [1, 200, 2], 24, 4, 20000),                           # two chats of long contexts beside a prompt: 8 rows a tile and 74 CTAs, 64 rows
     ([13000, 700, 5000, 64, 8000], [5, 600, 1, 0, 21], 24, 4, 13000),          # the same with drafted tokens (64 rows a tile)
     ([9000, 300], [2, 150], 8, 8, 9000), ([9000, 400], [3, 400], 5, 1, 9000),
-    ([9000], [1], 24, 4, 9000), ([9000], [9], 24, 4, 9000), ([9000, 30], [1, 1], 64, 64, 9000), ([5000] * 3, [7] * 3, 24, 4, 5000),
+    ([9000], [1], 24, 4, 9000), ([9000], [9], 24, 4, 9000), ([1500, 30], [1, 1], 64, 64, 1500), ([5000] * 3, [7] * 3, 24, 4, 5000),
     ([9000, 300], [2, 200], 24, 4, 300), ([9000, 9000], [2, 200], 24, 4, 129),         # longer than it was said to be
     ([12000, 4000, 3000], [30, 25, 60], 24, 4, 1 << 22),                       # no room for images: everything on mma.sync
     ([900, 200], [300, 200], 3, 1, 900)]
