@@ -289,7 +289,7 @@ int bonsai_b200_qk_norm_rope(const float *q, const float *k, const float *q_weig
 typedef struct bonsai_b200_pages {
     void *pool;
     const int32_t *table, *len, *start;       /* device memory: [n_seq][table_stride], [n_seq], [n_seq + 1] */
-    int32_t n_pages, n_layers, n_head_kv, n_seq, table_stride, n_tok;
+    int32_t n_pages, n_layers, n_head_kv, n_seq, table_stride, n_tok;         /* table_stride: 2^24 at most */
 } bonsai_b200_pages;
 /* Stores the rows k, v ([n_tok][n_head_kv][256]) of the new tokens of one layer. */
 int bonsai_b200_pages_append(const bonsai_b200_pages *pages, int layer, const float *k, const float *v, bonsai_stream stream);

@@ -1908,7 +1908,7 @@ inline bool aligned8(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 7
 
 // 0: a cache that calls may use; 1: not one; -1: one, but no new tokens.
 int check_pages(const bonsai_b200_pages *p, int layer, PageCache *C) {
-    if (!p || p->n_pages <= 0 || p->n_layers <= 0 || p->n_head_kv <= 0 || p->n_head_kv > 65535 || p->table_stride <= 0 || p->n_seq < 0 || p->n_tok < 0) return 1;
+    if (!p || p->n_pages <= 0 || p->n_layers <= 0 || p->n_head_kv <= 0 || p->n_head_kv > 65535 || p->table_stride <= 0 || p->table_stride > PG_MAX_PAGES || p->n_seq < 0 || p->n_tok < 0) return 1;
     if (layer < 0 || layer >= p->n_layers) return 1;
     if (p->n_seq == 0 || p->n_tok == 0) return -1;
     if (!p->pool || !p->table || !p->len || !p->start || !aligned16(p->pool) || !aligned4(p->table) || !aligned4(p->len) || !aligned4(p->start)) return 1;

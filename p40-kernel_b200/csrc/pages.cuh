@@ -12,6 +12,7 @@ namespace b200 {
 
 constexpr int PG_POS = 64, PG_HEAD_BYTES = PG_POS * KV_ROW;
 static_assert(PG_POS == KV_TILE, "");
+constexpr int PG_MAX_PAGES = 1 << 24;                            // of a sequence: its positions are counted in 32 bits
 
 struct PageCache {
     uint8_t *pool;

@@ -80,6 +80,18 @@ def test_cache_refusals():
     assert attn(max_len=30000) == 1 and attn(max_len=30000, ws=ONE, ws_bytes=need - 1) == 1 and attn(max_len=30000, ws=24, ws_bytes=need) == 1
 
 
+def test_tables_of_too_many_positions():
+    """Positions are counted in 32 bits: a table row has room for 2^30 of them at most."""
+    import bonsai_b200
+    L = bonsai_b200.lib()
+    for stride in ((1 << 24) + 1, 1 << 25, (1 << 31) - 1):
+        p = struct(table_stride=stride)
+        assert L.bonsai_b200_pages_append(C.byref(p), 0, ONE, ONE, None) == 1
+        assert L.bonsai_b200_pages_attn(C.byref(p), 0, ONE, ONE, 24, 1, None, 0, 0.0625, None) == 1
+    need = L.bonsai_b200_pages_attn_workspace(5, (1 << 31) - 1, 2, 24, 4)
+    assert 0 < need < 1 << 30
+
+
 def test_workspace_sizes():
     import bonsai_b200 as bb
     assert bb.pages_attn_workspace(1, 64, 1, 24, 4) == 0
