@@ -280,6 +280,26 @@ int bonsai_b200_qk_norm_rope(const float *q, const float *k, const float *q_weig
                              float *k_out, int64_t n_tok, int n_head, int n_head_kv, int head_dim, int n_rot, int64_t q_tok_stride, int64_t q_head_stride,
                              int64_t k_tok_stride, int64_t k_head_stride, float eps, bonsai_stream stream);
 
+/* Queries and keys turned by their positions, without norms: bonsai_b200_qk_norm_rope's arguments and refusals, with pairs of a head's halves (row[i], row[i + n_rot / 2]) or of
+ * neighbours (row[2 i], row[2 i + 1]), and an amplitude (a finite number) that the turned values are multiplied by.  Angles, sines and cosines are formed in 64 bits, times the amplitude rounded
+ * once; freq may be any finite numbers, pos negative (a turn back).  (For bonsai_b200_qk_norm_rope an amplitude is a factor of the first n_rot weights.) */
+#define BONSAI_B200_PAIRS_HALVES 0
+#define BONSAI_B200_PAIRS_NEXT 1
+int bonsai_b200_rope(const float *q, const float *k, const int32_t *pos, const double *freq, float *q_out, float *k_out, int64_t n_tok, int n_head, int n_head_kv, int head_dim, int n_rot,
+                     int pairs, float amplitude, int64_t q_tok_stride, int64_t q_head_stride, int64_t k_tok_stride, int64_t k_head_stride, bonsai_stream stream);
+/* Fills freq (n_rot / 2 numbers) and *amplitude, all HOST memory, for heads whose first n_rot values are turned: theta^(-2 i / n_rot), theta above 1.  Contexts that are `factor` (1 and more) times
+ * the trained ones:
+ *   LINEAR  frequencies divided by factor
+ *   BASE    theta times factor^(n_rot / (n_rot - 2)), n_rot at least 4: the slowest pair's frequency is divided by factor, the fastest one's stays
+ *   YARN    frequencies of pairs that turn 32 times and more in trained_positions stay, of those that turn less than once are divided by factor, between them in proportion to the
+ *           pair's number; amplitude 0.1 ln(factor) + 1
+ * PLAIN takes no notice of factor.  Returns 1 for other arguments. */
+#define BONSAI_B200_ROPE_PLAIN 0
+#define BONSAI_B200_ROPE_LINEAR 1
+#define BONSAI_B200_ROPE_BASE 2
+#define BONSAI_B200_ROPE_YARN 3
+int bonsai_b200_rope_freq(double *freq, float *amplitude, int n_rot, double theta, int scaling, double factor, int trained_positions);
+
 /* A K/V cache in pages.  The pool is the caller's memory (16-byte aligned), n_pages pages of
  *   [n_layers][K, V][n_head_kv][BONSAI_B200_PAGE_POSITIONS][256 / 32 blocks of 34 bytes]
  * with Q8_0 blocks as bonsai_kv_append lays them out.  A block's scale is its largest magnitude times 1 / 127, rounded once, in fp32 and then to fp16 (bonsai_kv_append divides: the
@@ -293,6 +313,20 @@ typedef struct bonsai_b200_pages {
 } bonsai_b200_pages;
 /* Stores the rows k, v ([n_tok][n_head_kv][256]) of the new tokens of one layer. */
 int bonsai_b200_pages_append(const bonsai_b200_pages *pages, int layer, const float *k, const float *v, bonsai_stream stream);
+/* The same from a layer's projections, in one pass: queries and keys normed for each head (x / sqrt(mean(x^2) + eps) * weight; a weight that is NULL: not normed) and turned (n_rot, pairs,
+ * amplitude as for bonsai_b200_rope, which it equals bit for bit; pos NULL: each row's position in its sequence), queries to q_out [n_tok][n_head][256], keys and values to their rows in the cache.
+ * Strides and places of q, k, v and q_out as bonsai_b200_qk_norm_rope has them (v like k); n_head may be 0.  Means and roots are formed in 64 bits and rounded once, everything else one
+ * rounded operation at a time.  Rows that no place fits (status word 3) have no output either. */
+int bonsai_b200_pages_write(const bonsai_b200_pages *pages, int layer, const float *q, const float *k, const float *v, const float *q_weight, const float *k_weight, const int32_t *pos,
+                            const double *freq, float *q_out, int n_head, int n_rot, int pairs, float amplitude, int64_t q_tok_stride, int64_t q_head_stride, int64_t k_tok_stride,
+                            int64_t k_head_stride, int64_t v_tok_stride, int64_t v_head_stride, float eps, bonsai_stream stream);
+/* Rows of one layer back as floats: row start[s] + i of k_out, v_out ([n_tok][n_head_kv][256], 16-byte aligned, of the type; one may be NULL) is position first[s] + i of sequence s, code times
+ * scale (exact in fp32, rounded once to fp16 or bf16).  first (n_seq numbers on the device) NULL: each sequence's last positions, as the other calls count them.  A position that the
+ * sequence does not have is left as it was (status word 3). */
+#define BONSAI_B200_ROWS_F32 0
+#define BONSAI_B200_ROWS_F16 1
+#define BONSAI_B200_ROWS_BF16 2
+int bonsai_b200_pages_read(const bonsai_b200_pages *pages, int layer, const int32_t *first, void *k_out, void *v_out, int type, bonsai_stream stream);
 /* Attention of the new tokens (q, out [n_tok][n_head][256]) of one layer over the cache, their own rows included: each as bonsai_kv_attn_decode computes it at
  * its position on the same rows and codes -- queries quantised to Q8_0 (as above), positions up to its own seen -- within 1e-5 of the largest output of a head.  A token without a position
  * (len[s] smaller than its new tokens) sees nothing: zeros.  max_len: no smaller than every len, for the division of the work; longer sequences are served
@@ -302,6 +336,16 @@ int bonsai_b200_pages_append(const bonsai_b200_pages *pages, int layer, const fl
 int64_t bonsai_b200_pages_attn_workspace(int n_tok, int max_len, int n_seq, int n_head, int n_head_kv);
 int bonsai_b200_pages_attn(const bonsai_b200_pages *pages, int layer, const float *q, float *out, int n_head, int max_len, void *workspace,
                            int64_t workspace_bytes, float scale, bonsai_stream stream);
+/* The same attention where groups of sequences begin with the same pages (a prompt that many answers continue, an instruction in front of many chats): what a group has in
+ * common is read and multiplied once for all of its tokens.  Group g are the sequences group[g] .. group[g + 1] - 1 (ascending numbers), and the first shared[g] pages of
+ * each, whole ones, are the same: only the table row of the first of them that has new tokens is read there.  New tokens lie behind them: len[s] less its new tokens is
+ * shared[g] * BONSAI_B200_PAGE_POSITIONS at least.  A sequence of no group, or of a group of one, shares nothing; n_groups (n_seq at most) may be 0.  group (n_groups + 1 numbers) and
+ * shared (n_groups) lie on the device like start.  A row of V with a scale that is no number or infinite makes the outputs of the tokens that see it NaN, and no others.
+ * Values of V that are smaller than 2^-22 of the largest of their block of 32 dims among 128 positions that follow each other count as multiples of 2^-40 of that.
+ * workspace: 16-byte aligned device memory of bonsai_b200_pages_attn_shared_workspace(the same sizes) bytes: 2 KB for each token and query head, and 7.3 MB. */
+int64_t bonsai_b200_pages_attn_shared_workspace(int n_tok, int n_seq, int n_groups, int n_head, int n_head_kv);
+int bonsai_b200_pages_attn_shared(const bonsai_b200_pages *pages, int layer, const int32_t *group, const int32_t *shared, int n_groups, const float *q, float *out, int n_head,
+                                  void *workspace, int64_t workspace_bytes, float scale, bonsai_stream stream);
 /* Copies pages of page_bytes (a multiple of 16) inside a pool: page src[i] to page dst[i], i < n.  src and dst are HOST memory, read before the call returns.  Returns 1,
  * and copies nothing, where a page is not one of the n_pages, is written twice or is both read and written. */
 int bonsai_b200_pages_copy(void *pool, int64_t page_bytes, int n_pages, const int32_t *src, const int32_t *dst, int n, bonsai_stream stream);

@@ -57,6 +57,12 @@ SIGNATURES = {
     "bonsai_b200_kv_arrays": (_INT, [_VP, _VP, _VP, _VP]),
     "bonsai_b200_kv_splits": (_INT, [_INT, _INT, _INT, _VP]),
     "bonsai_b200_qk_norm_rope": (_INT, [_VP] * 8 + [_I64] + [_INT] * 4 + [_I64] * 4 + [_F, _VP]),
+    "bonsai_b200_rope": (_INT, [_VP] * 6 + [_I64] + [_INT] * 5 + [_F] + [_I64] * 4 + [_VP]),
+    "bonsai_b200_rope_freq": (_INT, [_VP, _VP, _INT, C.c_double, _INT, C.c_double, _INT]),
+    "bonsai_b200_pages_write": (_INT, [_VP, _INT] + [_VP] * 8 + [_INT] * 3 + [_F] + [_I64] * 6 + [_F, _VP]),
+    "bonsai_b200_pages_read": (_INT, [_VP, _INT, _VP, _VP, _VP, _INT, _VP]),
+    "bonsai_b200_pages_attn_shared_workspace": (_I64, [_INT] * 5),
+    "bonsai_b200_pages_attn_shared": (_INT, [_VP, _INT, _VP, _VP, _INT, _VP, _VP, _INT, _VP, _I64, _F, _VP]),
     "bonsai_b200_pages_append": (_INT, [_VP, _INT, _VP, _VP, _VP]),
     "bonsai_b200_pages_attn_workspace": (_I64, [_INT] * 5),
     "bonsai_b200_pages_attn": (_INT, [_VP, _INT, _VP, _VP, _INT, _INT, _VP, _I64, _F, _VP]),
@@ -99,7 +105,7 @@ def lib():
 # and launched in about the time of the launch itself.  `_calls` name -> exported symbol.
 _NATIVE = {n: "bonsai_p40_" + n for n in ("gemv", "quant_activations", "gemm", "repack", "gemv_repack", "fwht", "rmsnorm", "gdn_step", "attn")}
 _NATIVE.update({n: "bonsai_b200_" + n for n in ("fwht_quant", "swiglu", "quant_batch", "linear", "linear_static", "chain_run", "qk_norm_rope", "pages_append", "pages_attn",
-                                               "pages_copy", "gdn_seqs")})
+                                               "pages_copy", "gdn_seqs", "rope", "pages_write", "pages_read", "pages_attn_shared")})
 _NATIVE.update({n: "bonsai_" + n for n in ("kv_append", "kv_append_batch", "kv_attn_decode")})
 _calls = None
 
@@ -262,6 +268,30 @@ def qk_norm_rope(q, k, q_weight, k_weight, pos, freq, q_out, k_out, n_tok, n_hea
     """q and k need not be contiguous: their strides are arguments, in floats."""
     return _native().qk_norm_rope(q, k, q_weight, k_weight, pos, freq, q_out, k_out, n_tok, n_head, n_head_kv, head_dim, n_rot, q_tok_stride, q_head_stride,
                                   k_tok_stride, k_head_stride, eps)
+
+
+PAIRS_HALVES, PAIRS_NEXT = 0, 1
+ROPE_SCALING = {"plain": 0, "linear": 1, "base": 2, "yarn": 3}
+
+
+def rope_freq(n_rot, theta, scaling="plain", factor=1.0, trained_positions=0):
+    """Radians per position of n_rot / 2 pairs (a float64 tensor in host memory) and the amplitude that goes with them."""
+    import torch
+    freq, amplitude = torch.empty(max(0, n_rot) // 2, dtype=torch.float64), C.c_float()
+    rc = lib().bonsai_b200_rope_freq(freq.data_ptr(), C.addressof(amplitude), n_rot, theta, ROPE_SCALING[scaling], factor, trained_positions)
+    if rc != 0:
+        raise RuntimeError(f"bonsai_b200_rope_freq returned {rc}")
+    return freq, amplitude.value
+
+
+def rope(q, k, pos, freq, q_out, k_out, n_tok, n_head, n_head_kv, head_dim, n_rot, pairs, amplitude, q_tok_stride, q_head_stride, k_tok_stride, k_head_stride):
+    """q and k need not be contiguous: their strides are arguments, in floats."""
+    return _native().rope(q, k, pos, freq, q_out, k_out, n_tok, n_head, n_head_kv, head_dim, n_rot, pairs, amplitude, q_tok_stride, q_head_stride, k_tok_stride,
+                          k_head_stride)
+
+
+def pages_attn_shared_workspace(n_tok, n_seq, n_groups, n_head, n_head_kv):
+    return lib().bonsai_b200_pages_attn_shared_workspace(n_tok, n_seq, n_groups, n_head, n_head_kv)
 
 
 def pages_attn_workspace(n_tok, max_len, n_seq, n_head, n_head_kv):
@@ -438,3 +468,31 @@ class Pages:
     def attn(self, layer, q, out, n_head, max_len, workspace, scale):
         """workspace: a tensor of attn_workspace(max_len, n_head) bytes, or None where that is 0."""
         return _native().pages_attn(self._struct(), layer, q, out, n_head, max_len, workspace, 0 if workspace is None else workspace.nbytes, scale)
+
+    def write(self, layer, q, k, v, q_weight, k_weight, pos, freq, q_out, n_head, n_rot, pairs, amplitude, q_tok_stride, q_head_stride, k_tok_stride, k_head_stride,
+              v_tok_stride, v_head_stride, eps):
+        """q, k and v need not be contiguous: their strides are arguments, in floats."""
+        return _native().pages_write(self._struct(), layer, q, k, v, q_weight, k_weight, pos, freq, q_out, n_head, n_rot, pairs, amplitude, q_tok_stride, q_head_stride,
+                                     k_tok_stride, k_head_stride, v_tok_stride, v_head_stride, eps)
+
+    def read(self, layer, first, k_out, v_out):
+        """k_out, v_out: float32, float16 or bfloat16 tensors [n_tok][n_head_kv][256] of one type, one of them may be None."""
+        import torch
+        types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+        outs = [t for t in (k_out, v_out) if t is not None]
+        if not outs or any(t.dtype not in types or t.dtype != outs[0].dtype for t in outs):
+            raise RuntimeError("k_out and v_out must be tensors of float32, float16 or bfloat16, both of one type")
+        for t in outs:
+            if t.device.type != "cuda" or t.device.index != self._device:
+                raise RuntimeError(f"k_out and v_out must be on device {self._device}")
+            if t.numel() < self.n_tok * self._s.n_head_kv * 256:
+                raise RuntimeError(f"k_out and v_out must have {self.n_tok} rows of {self._s.n_head_kv} heads")
+        return _native().pages_read(self._struct(), layer, first, k_out, v_out, types[outs[0].dtype])
+
+    def attn_shared_workspace(self, n_groups, n_head):
+        return pages_attn_shared_workspace(self.n_tok, self.n_seq, n_groups, n_head, self._s.n_head_kv)
+
+    def attn_shared(self, layer, group, shared, q, out, n_head, workspace, scale):
+        """group: int32 [groups + 1], shared: int32 [groups] (both may be None: no groups); workspace: a tensor of attn_shared_workspace(groups, n_head) bytes."""
+        n_groups = 0 if shared is None else shared.numel()
+        return _native().pages_attn_shared(self._struct(), layer, group, shared, n_groups, q, out, n_head, workspace, 0 if workspace is None else workspace.nbytes, scale)

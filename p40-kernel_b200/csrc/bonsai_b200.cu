@@ -22,15 +22,19 @@
 #include "kv.cuh"
 #include "ops.cuh"
 #include "pages.cuh"
+#include "pages_rows.cuh"
+#include "pages_shared.cuh"
 #include "pages_tc.cuh"
 #include "probe.cuh"
 #include "ptq.cuh"
 #include "repack.cuh"
+#include "rotary.cuh"
 #include "scratch.cuh"
 #include "synth.cuh"
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstring>
 #include <iterator>
 #include <mutex>
@@ -2095,6 +2099,189 @@ int bonsai_b200_pages_attn(const bonsai_b200_pages *pages, int layer, const floa
         auto join = [&](auto kernel) { return launch(kernel, dim3((unsigned)ctas), dim3(32 * PGJ_WARPS), 0, st, true, P); };
         e = roww == 8 ? join(pages_join_kernel<8>) : roww == 2 ? join(pages_join_kernel<2>) : join(pages_join_kernel<1>);
     }
+    return (int)e;
+}
+
+namespace {
+// Strides of rows that may not overlap: one is a row and more, and the other passes over all that the first spans (a stride of one row is not looked at).  And no address past 2^61 floats.
+bool rows_lie_apart(int64_t n_tok, int n_head, int dim, int64_t ts, int64_t hs) {
+    const bool one_tok = n_tok == 1, one_head = n_head == 1;
+    const __int128 heads_span = (__int128)(n_head - 1) * hs + dim, toks_span = (__int128)(n_tok - 1) * ts + dim;
+    if ((!one_head && hs < dim) || (!one_tok && ts < dim) || (!one_head && !one_tok && ts < heads_span && hs < toks_span)) return false;
+    return (one_head ? 0 : heads_span) + (one_tok ? 0 : toks_span) <= INT64_MAX / 4;
+}
+bool strides_by(int64_t n_tok, int n_head, int64_t ts, int64_t hs, int by) { return (n_tok == 1 || ts % by == 0) && (n_head == 1 || hs % by == 0); }
+bool rotation_args(const void *freq, int dim, int n_rot, int pairs, float amplitude) {
+    return n_rot >= 0 && n_rot <= dim && n_rot % 2 == 0 && (pairs == PAIRS_HALVES || pairs == PAIRS_NEXT) && std::isfinite(amplitude) && (n_rot == 0 || (freq && aligned8(freq)));
+}
+}  // namespace
+
+int bonsai_b200_rope_freq(double *freq, float *amplitude, int n_rot, double theta, int scaling, double factor, int trained_positions) {
+    if (!freq || !amplitude || n_rot <= 0 || n_rot % 2 != 0 || !(theta > 1.0) || !std::isfinite(theta) || !(factor >= 1.0) || !std::isfinite(factor)) return 1;
+    if (scaling != BONSAI_B200_ROPE_PLAIN && scaling != BONSAI_B200_ROPE_LINEAR && scaling != BONSAI_B200_ROPE_BASE && scaling != BONSAI_B200_ROPE_YARN) return 1;
+    if ((scaling == BONSAI_B200_ROPE_YARN && trained_positions <= 0) || (scaling == BONSAI_B200_ROPE_BASE && n_rot < 4)) return 1;
+    const int pairs = n_rot / 2;
+    const double pi2 = 6.283185307179586476925286766559;
+    double low = 0.0, high = 0.0;
+    if (scaling == BONSAI_B200_ROPE_BASE) theta *= std::pow(factor, (double)n_rot / (n_rot - 2));
+    if (scaling == BONSAI_B200_ROPE_YARN) {             // the pairs that turn 32 times and once in the positions that were trained
+        auto at = [&](double turns) { return n_rot * std::log(trained_positions / (turns * pi2)) / (2.0 * std::log(theta)); };
+        low = std::max(0.0, std::floor(at(32.0)));
+        high = std::min(n_rot - 1.0, std::ceil(at(1.0)));
+    }
+    for (int i = 0; i < pairs; ++i) {
+        double f = std::pow(theta, -(double)i / pairs);
+        if (scaling == BONSAI_B200_ROPE_LINEAR) f /= factor;
+        if (scaling == BONSAI_B200_ROPE_YARN && factor > 1.0) {
+            const double slowed = std::min(1.0, std::max(0.0, (i - low) / std::max(high - low, 0.001)));
+            f = f * (1.0 - slowed) + f / factor * slowed;
+        }
+        freq[i] = f;
+    }
+    *amplitude = scaling == BONSAI_B200_ROPE_YARN ? (float)(0.1 * std::log(factor) + 1.0) : 1.0f;
+    return 0;
+}
+
+int bonsai_b200_rope(const float *q, const float *k, const int32_t *pos, const double *freq, float *q_out, float *k_out, int64_t n_tok, int n_head, int n_head_kv, int head_dim, int n_rot,
+                     int pairs, float amplitude, int64_t q_tok_stride, int64_t q_head_stride, int64_t k_tok_stride, int64_t k_head_stride, bonsai_stream stream) {
+    if (head_dim <= 0 || head_dim > ROPE_MAX_DIM || n_head < 0 || n_head_kv < 0 || n_head > (1 << 18) || n_head_kv > (1 << 18) || !rotation_args(freq, head_dim, n_rot, pairs, amplitude)) return 1;
+    const int heads = n_head + n_head_kv;
+    if (n_tok <= 0 || heads == 0) return 0;
+    if (n_tok > INT32_MAX || (n_rot && (!pos || !aligned4(pos)))) return 1;
+    const RopeParams P = {{q, k}, {q_out, k_out}, {q_tok_stride, k_tok_stride}, {q_head_stride, k_head_stride}, pos, freq, {n_head, n_head_kv}, head_dim, n_rot, pairs, amplitude};
+    bool vec = head_dim % 8 == 0 && n_rot % 8 == 0;
+    for (int i = 0; i < 2; ++i) {
+        if (!P.n_head[i]) continue;
+        const int64_t ts = P.tok_stride[i], hs = P.head_stride[i];
+        if (!P.x[i] || !P.y[i] || !aligned4(P.x[i]) || !aligned4(P.y[i]) || !rows_lie_apart(n_tok, P.n_head[i], head_dim, ts, hs)) return 1;
+        // an output in the place of its input is row for row the same memory; no output is the other input
+        const bool packed = (P.n_head[i] == 1 || hs == head_dim) && (n_tok == 1 || ts == (int64_t)P.n_head[i] * head_dim);
+        if ((P.y[i] == P.x[i] && !packed) || (P.n_head[1 - i] && P.y[i] == P.x[1 - i])) return 1;
+        vec = vec && aligned16(P.x[i]) && aligned16(P.y[i]) && strides_by(n_tok, P.n_head[i], ts, hs, 4);
+    }
+    const int64_t each = vec ? n_rot / 8 + (head_dim - n_rot) / 4 : n_rot / 2 + head_dim - n_rot, items = heads * each;
+    // a token's items by CTAs: as many as threads hold (vec), fewer of few tokens
+    const int64_t most = ROPE_THREADS * (vec ? (n_tok <= 2 * SM_COUNT ? 1 : ROPE_MAX_ITEMS) : 4), parts = (items + most - 1) / most;
+    if (parts > 65535 || items > INT32_MAX) return 1;
+    const int per = (int)((items + parts - 1) / parts);
+    const dim3 grid((unsigned)n_tok, (unsigned)parts);
+    return (int)(vec ? launch(rope_kernel<true>, grid, dim3(ROPE_THREADS), 0, as_stream(stream), true, P, (int)items, per)
+                     : launch(rope_kernel<false>, grid, dim3(ROPE_THREADS), 0, as_stream(stream), true, P, (int)items, per));
+}
+
+int bonsai_b200_pages_write(const bonsai_b200_pages *pages, int layer, const float *q, const float *k, const float *v, const float *q_weight, const float *k_weight, const int32_t *pos,
+                            const double *freq, float *q_out, int n_head, int n_rot, int pairs, float amplitude, int64_t q_tok_stride, int64_t q_head_stride, int64_t k_tok_stride,
+                            int64_t k_head_stride, int64_t v_tok_stride, int64_t v_head_stride, float eps, bonsai_stream stream) {
+    PageWrite P = {};
+    if (n_head < 0 || n_head > (1 << 18) || !rotation_args(freq, KV_D, n_rot, pairs, amplitude)) return 1;
+    const int rc = check_pages(pages, layer, &P.C);
+    if (rc) return rc < 0 ? 0 : rc;
+    const int heads[3] = {n_head, P.C.n_head_kv, P.C.n_head_kv};
+    const float *x[3] = {q, k, v};
+    const int64_t ts[3] = {q_tok_stride, k_tok_stride, v_tok_stride}, hs[3] = {q_head_stride, k_head_stride, v_head_stride};
+    bool vec = true;
+    for (int i = 0; i < 3; ++i) {
+        if (!heads[i]) continue;
+        if (!x[i] || !aligned4(x[i]) || !rows_lie_apart(P.C.n_tok, heads[i], KV_D, ts[i], hs[i])) return 1;
+        vec = vec && aligned16(x[i]) && strides_by(P.C.n_tok, heads[i], ts[i], hs[i], 4);
+        P.x[i] = x[i];
+        P.tok_stride[i] = ts[i];
+        P.head_stride[i] = hs[i];
+    }
+    if (n_head) {
+        const bool packed = (n_head == 1 || hs[0] == KV_D) && (P.C.n_tok == 1 || ts[0] == (int64_t)n_head * KV_D);
+        if (!q_out || !aligned4(q_out) || (q_out == q && !packed) || q_out == k || q_out == v) return 1;
+        vec = vec && aligned16(q_out);
+    }
+    if ((q_weight && !aligned4(q_weight)) || (k_weight && !aligned4(k_weight)) || (pos && !aligned4(pos))) return 1;
+    P.w[0] = q_weight;
+    P.w[1] = k_weight;
+    P.q_out = q_out;
+    P.pos = pos;
+    P.freq = freq;
+    P.n_head = n_head;
+    P.n_rot = n_rot;
+    P.pairs = pairs;
+    P.layer = layer;
+    P.amplitude = amplitude;
+    P.eps = eps;
+    const int64_t rows = (int64_t)n_head + 2 * (int64_t)P.C.n_head_kv;
+    auto run = [&](auto kernel, int per) {
+        const int64_t groups = (rows + per * PGW_WARPS - 1) / (per * PGW_WARPS);
+        if (groups > 65535) return 1;
+        return (int)launch(kernel, dim3((unsigned)P.C.n_tok, (unsigned)groups), dim3(32 * PGW_WARPS), 0, as_stream(stream), true, P);
+    };
+    if (P.C.n_tok * ((rows + PGW_WARPS - 1) / PGW_WARPS) <= 2 * SM_COUNT) return vec ? run(pages_write_kernel<true, 1>, 1) : run(pages_write_kernel<false, 1>, 1);
+    return vec ? run(pages_write_kernel<true, 4>, 4) : run(pages_write_kernel<false, 4>, 4);
+}
+
+int bonsai_b200_pages_read(const bonsai_b200_pages *pages, int layer, const int32_t *first, void *k_out, void *v_out, int type, bonsai_stream stream) {
+    PageRead P = {};
+    if (type != BONSAI_B200_ROWS_F32 && type != BONSAI_B200_ROWS_F16 && type != BONSAI_B200_ROWS_BF16) return 1;
+    const int rc = check_pages(pages, layer, &P.C);
+    if (rc) return rc < 0 ? 0 : rc;
+    if ((!k_out && !v_out) || k_out == v_out || (k_out && !aligned16(k_out)) || (v_out && !aligned16(v_out)) || (first && !aligned4(first))) return 1;
+    P.first = first;
+    P.out[0] = k_out;
+    P.out[1] = v_out;
+    P.layer = layer;
+    const unsigned ctas = (unsigned)(((int64_t)P.C.n_tok + PGR_WARPS - 1) / PGR_WARPS);
+    auto run = [&](auto kernel) { return (int)launch(kernel, dim3(ctas), dim3(32 * PGR_WARPS), 0, as_stream(stream), true, P); };
+    return type == BONSAI_B200_ROWS_F32 ? run(pages_read_kernel<ROWS_F32>) : type == BONSAI_B200_ROWS_F16 ? run(pages_read_kernel<ROWS_F16>) : run(pages_read_kernel<ROWS_BF16>);
+}
+
+namespace {
+// Parts of pages_attn_shared: rows of the groups and of the sequences (each call row once in either), and one tile for each CTA.
+inline int64_t shared_rows(int n_tok, int n_head) { return 2 * (int64_t)n_tok * n_head; }
+inline int64_t shared_part_bytes(int n_tok, int n_head) {
+    const int64_t rows = shared_rows(n_tok, n_head) + (int64_t)SM_COUNT * PSH_ROWS;
+    return rows * KV_D * (int64_t)sizeof(float) + (rows * (int64_t)sizeof(float2) + 15) / 16 * 16;
+}
+inline bool shared_sizes(int n_tok, int n_seq, int n_groups, int n_head, int n_head_kv) {
+    return n_groups >= 0 && n_groups <= n_seq && (int64_t)n_groups + n_seq <= INT32_MAX - PSH_THREADS && pages_attn_sizes(n_tok, 1, n_seq, n_head, n_head_kv);
+}
+}  // namespace
+
+int64_t bonsai_b200_pages_attn_shared_workspace(int n_tok, int n_seq, int n_groups, int n_head, int n_head_kv) {
+    if (!shared_sizes(n_tok, n_seq, n_groups, n_head, n_head_kv)) return 0;
+    return shared_part_bytes(n_tok, n_head) + (1 + (int64_t)n_groups + n_seq) * (int64_t)sizeof(PshPlan);
+}
+
+int bonsai_b200_pages_attn_shared(const bonsai_b200_pages *pages, int layer, const int32_t *group, const int32_t *shared, int n_groups, const float *q, float *out, int n_head,
+                                  void *workspace, int64_t workspace_bytes, float scale, bonsai_stream stream) {
+    PageShared P = {};
+    if (n_head <= 0 || n_groups < 0) return 1;
+    const int rc = check_pages(pages, layer, &P.C);
+    if (rc) return rc < 0 ? 0 : rc;
+    const PageCache &C = P.C;
+    if (!q || !out || !aligned4(q) || !aligned4(out) || !shared_sizes(C.n_tok, C.n_seq, n_groups, n_head, C.n_head_kv)) return 1;
+    if (n_groups && (!group || !shared || !aligned4(group) || !aligned4(shared))) return 1;
+    if (!workspace || !aligned16(workspace) || workspace_bytes < bonsai_b200_pages_attn_shared_workspace(C.n_tok, C.n_seq, n_groups, n_head, C.n_head_kv)) return 1;
+    const int64_t join_ctas = ((int64_t)C.n_tok * n_head + PSJ_WARPS - 1) / PSJ_WARPS;
+    if (join_ctas > INT32_MAX) return 1;
+    P.q = q;
+    P.out = out;
+    P.layer = layer;
+    P.n_head = n_head;
+    P.group = n_head / C.n_head_kv;
+    P.n_groups = n_groups;
+    P.group_first = group;
+    P.group_pages = shared;
+    P.scale = scale;
+    P.part_rows = shared_rows(C.n_tok, n_head);
+    P.part = static_cast<float *>(workspace);
+    P.part_ml = reinterpret_cast<float2 *>(P.part + (P.part_rows + (int64_t)SM_COUNT * PSH_ROWS) * KV_D);
+    P.plan = reinterpret_cast<PshPlan *>(static_cast<uint8_t *>(workspace) + shared_part_bytes(C.n_tok, n_head));
+    static SmemOptIn opt;
+    cudaError_t e = opt.ensure(pages_shared_kernel);
+    // what the warps' shares of the registers add up to is what the launch has to bring: one that asked for more would wait for them for good
+    static const int regs = [] {
+        cudaFuncAttributes a = {};
+        return cudaFuncGetAttributes(&a, pages_shared_kernel) == cudaSuccess ? a.numRegs : 0;
+    }();
+    if (e == cudaSuccess && regs * PSH_THREADS < PSH_REGS) e = cudaErrorLaunchOutOfResources;
+    if (e == cudaSuccess) e = launch(pages_shared_kernel, dim3(SM_COUNT), dim3(PSH_THREADS), (size_t)PSH_SMEM_BYTES, as_stream(stream), true, P);
+    if (e == cudaSuccess) e = launch(pages_shared_join_kernel, dim3((unsigned)join_ctas), dim3(32 * PSJ_WARPS), 0, as_stream(stream), true, P);
     return (int)e;
 }
 

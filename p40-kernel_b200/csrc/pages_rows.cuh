@@ -1,0 +1,226 @@
+// pages_rows.cuh -- rows of a paged Q8_0 cache written straight from a layer's projections, and read back as floats.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "pages.cuh"
+#include "rotary.cuh"
+
+namespace b200 {
+
+// ---- write: norms of queries and keys, their rotation, keys and values quantised into the cache ---------------------------------------------------
+//   q, k: x / sqrt(mean x^2 + eps) * w (where there are weights), turned as in rotary.cuh; k and v to Q8_0 as pages_append_kernel stores them
+// The mean and its root are formed in 64 bits and rounded once, each product and sum of the rest is one rounded operation: the codes do not depend on the order
+// of a sum.
+struct PageWrite {
+    PageCache C;
+    const float *x[3], *w[2];               // q, k, v; weights of the norms, or NULL
+    float *q_out;
+    int64_t tok_stride[3], head_stride[3];
+    const int32_t *pos;                     // or NULL: where the row lies in its sequence
+    const double *freq;
+    int n_head, n_rot, pairs, layer;
+    float amplitude, eps;
+};
+constexpr int PGW_WARPS = 8;
+
+// grid (tokens, groups of rows); a warp has up to PER rows (query heads, then k and v heads), eight values a lane.  VEC: strides are multiples of 4, pointers 16-byte aligned.
+template <bool VEC, int PER>
+__global__ void __launch_bounds__(32 * PGW_WARPS) pages_write_kernel(const __grid_constant__ PageWrite P) {
+    __shared__ __align__(16) float rows[PGW_WARPS][KV_D];
+    __shared__ float2 turn[KV_D / 2];
+    const PageCache &C = P.C;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tok = blockIdx.x;
+    const int all = P.n_head + 2 * C.n_head_kv, first = (int)blockIdx.y * PGW_WARPS * PER + warp, half = P.n_rot >> 1;
+    pdl_wait_prior_grid();
+    if (PER == 1) pdl_launch_dependents();
+    auto which = [&](int r, int &h) {       // 0 q, 1 k, 2 v
+        const int kind = r < P.n_head ? 0 : r < P.n_head + C.n_head_kv ? 1 : 2;
+        h = kind == 0 ? r : r - P.n_head - (kind - 1) * C.n_head_kv;
+        return kind;
+    };
+    float x[PER][8];
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+        const int r = first + PGW_WARPS * e;
+        if (r >= all) break;
+        int h;
+        const int kind = which(r, h);
+        const float *src = P.x[kind] + (int64_t)tok * P.tok_stride[kind] + h * P.head_stride[kind] + 8 * lane;
+        if (VEC) {
+            const float4 a = *reinterpret_cast<const float4 *>(src), b = *reinterpret_cast<const float4 *>(src + 4);
+            x[e][0] = a.x; x[e][1] = a.y; x[e][2] = a.z; x[e][3] = a.w; x[e][4] = b.x; x[e][5] = b.y; x[e][6] = b.z; x[e][7] = b.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[e][i] = src[i];
+        }
+    }
+    if (blockIdx.x == 0 && blockIdx.y == 0) report_ranges(C.start, C.n_seq, C.n_tok);
+    const int s = seq_of_row(C.start, C.n_seq, tok, lane);
+    if (s >= C.n_seq) return;               // rows behind the last sequence (the CTA's warps agree)
+    const SeqRange range = seq_range(C.start, s, C.n_tok);
+    const int64_t at = (int64_t)C.len[s] - range.n + (tok - range.begin);
+    int page = -1;
+    if (range.n > 0 && tok >= range.begin && at >= 0 && at / PG_POS < C.table_stride) page = C.table[(size_t)s * C.table_stride + at / PG_POS];
+    if (page < 0 || page >= C.n_pages) {
+        if (threadIdx.x == 0 && blockIdx.y == 0) bad_sequence();
+        return;
+    }
+    if (half) {
+        const int pos = P.pos ? P.pos[tok] : (int)at;
+        for (int i = threadIdx.x; i < half; i += 32 * PGW_WARPS) turn[i] = turn_of(pos, P.freq[i], (double)P.amplitude);
+    }
+    __syncthreads();
+    float *row = rows[warp];
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+        const int r = first + PGW_WARPS * e;
+        if (r >= all) break;
+        int h;
+        const int kind = which(r, h);
+        if (kind < 2) {
+            if (P.w[kind]) {
+                double ss = 0.0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) ss = __fma_rn((double)x[e][i], (double)x[e][i], ss);
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) ss = __dadd_rn(ss, __shfl_xor_sync(0xffffffffu, ss, o));
+                const float sc = __double2float_rn(__ddiv_rn(1.0, __dsqrt_rn(__dadd_rn(__dmul_rn(ss, 1.0 / KV_D), (double)P.eps))));
+                const float *w = P.w[kind] + 8 * lane;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[e][i] = __fmul_rn(__fmul_rn(x[e][i], sc), w[i]);
+            }
+            if (half && P.pairs == PAIRS_NEXT) {
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    const int a = 8 * lane + i;
+                    if (a >= P.n_rot) break;
+                    const float2 p = turned_pair(x[e][i], x[e][i + 1], turn[a >> 1]);
+                    x[e][i] = p.x;
+                    x[e][i + 1] = p.y;
+                }
+            } else if (half) {
+                __syncwarp();               // the row before has been read
+                if (8 * lane < P.n_rot) {
+                    *reinterpret_cast<float4 *>(row + 8 * lane) = make_float4(x[e][0], x[e][1], x[e][2], x[e][3]);
+                    *reinterpret_cast<float4 *>(row + 8 * lane + 4) = make_float4(x[e][4], x[e][5], x[e][6], x[e][7]);
+                }
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int a = 8 * lane + i;
+                    if (a < half) x[e][i] = turned_pair(x[e][i], row[a + half], turn[a]).x;
+                    else if (a < P.n_rot) x[e][i] = turned_pair(row[a - half], x[e][i], turn[a - half]).y;
+                }
+            }
+        }
+        if (kind == 0) {
+            float *dst = P.q_out + ((int64_t)tok * P.n_head + h) * KV_D + 8 * lane;
+            if (VEC) {
+                *reinterpret_cast<float4 *>(dst) = make_float4(x[e][0], x[e][1], x[e][2], x[e][3]);
+                *reinterpret_cast<float4 *>(dst + 4) = make_float4(x[e][4], x[e][5], x[e][6], x[e][7]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) dst[i] = x[e][i];
+            }
+        } else {
+            const int blk = lane >> 2, sub = lane & 3;
+            const float d = __fmul_rn(kv_amax_8(x[e]), PG_SCALE), id = d > 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
+            uint32_t w[2];
+            kv_words_8(x[e], id, w);
+            __syncwarp();
+            uint8_t *bytes = reinterpret_cast<uint8_t *>(row);              // put together by halfwords, stored by 16-byte words
+            unsigned short *p = reinterpret_cast<unsigned short *>(bytes + 34 * blk);
+            if (sub == 0) p[0] = (unsigned short)f32_to_f16_bits_ties_away(d);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                p[1 + 4 * sub + 2 * j] = (unsigned short)(w[j] & 0xFFFFu);
+                p[2 + 4 * sub + 2 * j] = (unsigned short)(w[j] >> 16);
+            }
+            __syncwarp();
+            uint4 *dst = reinterpret_cast<uint4 *>(page_rows(C, page, P.layer, kind - 1, h) + (size_t)(at % PG_POS) * KV_ROW);
+            if (lane < KV_ROW / 16) dst[lane] = reinterpret_cast<const uint4 *>(bytes)[lane];
+        }
+    }
+}
+
+// ---- read: rows of a layer as floats ---------------------------------------------------------------------------------------------------------------
+//   row start[s] + i of the outputs is position first[s] + i of sequence s: code times scale, one product, exact in fp32 and rounded once to fewer bits
+enum : int { ROWS_F32 = 0, ROWS_F16 = 1, ROWS_BF16 = 2 };
+struct PageRead {
+    PageCache C;
+    const int32_t *first;                   // or NULL: each sequence's last positions
+    void *out[2];                           // K, V; one may be NULL
+    int layer;
+};
+constexpr int PGR_WARPS = 4, PGR_BATCH = 4;
+
+// A warp per token, its rows (K and V of every kv head) PGR_BATCH at a time; a lane has eight values.
+template <int TYPE>
+__global__ void __launch_bounds__(32 * PGR_WARPS) pages_read_kernel(const __grid_constant__ PageRead P) {
+    const PageCache &C = P.C;
+    const int lane = threadIdx.x & 31, tok = (int)blockIdx.x * PGR_WARPS + (threadIdx.x >> 5), heads = C.n_head_kv;
+    pdl_wait_prior_grid();
+    pdl_launch_dependents();
+    if (blockIdx.x == 0) report_ranges(C.start, C.n_seq, C.n_tok);
+    if (tok >= C.n_tok) return;
+    const int s = seq_of_row(C.start, C.n_seq, tok, lane);
+    if (s >= C.n_seq) return;               // nobody's
+    const SeqRange range = seq_range(C.start, s, C.n_tok);
+    const int len = C.len[s];
+    const int64_t at = (P.first ? (int64_t)P.first[s] : (int64_t)len - range.n) + (tok - range.begin);
+    int page = -1;
+    if (range.n > 0 && tok >= range.begin && at >= 0 && at < len && at / PG_POS < C.table_stride) page = C.table[(size_t)s * C.table_stride + at / PG_POS];
+    if (page < 0 || page >= C.n_pages) {
+        if (lane == 0) bad_sequence();
+        return;
+    }
+    const int blk = lane >> 2, sub = lane & 3, code0 = 34 * blk + 2 + 8 * sub;
+    const bool both = P.out[0] && P.out[1];
+    const int n = both ? 2 * heads : heads;
+    for (int r0 = 0; r0 < n; r0 += PGR_BATCH) {
+        uint32_t w[PGR_BATCH][3], d[PGR_BATCH];
+#pragma unroll
+        for (int e = 0; e < PGR_BATCH; ++e) {
+            const int r = min(r0 + e, n - 1), kv = both ? r / heads : P.out[0] ? 0 : 1, h = both ? r - kv * heads : r;
+            const uint8_t *row = page_rows(C, page, P.layer, kv, h) + (size_t)(at % PG_POS) * KV_ROW;
+            const uint32_t *src = reinterpret_cast<const uint32_t *>(row + (code0 & ~3));
+            d[e] = *reinterpret_cast<const uint16_t *>(row + 34 * blk);
+            w[e][0] = src[0];
+            w[e][1] = src[1];
+            w[e][2] = code0 & 2 ? src[2] : 0u;
+        }
+#pragma unroll
+        for (int e = 0; e < PGR_BATCH; ++e) {
+            const int r = r0 + e;
+            if (r >= n) break;
+            const int kv = both ? r / heads : P.out[0] ? 0 : 1, h = both ? r - kv * heads : r;
+            const uint32_t a = code0 & 2 ? __byte_perm(w[e][0], w[e][1], 0x5432) : w[e][0], b = code0 & 2 ? __byte_perm(w[e][1], w[e][2], 0x5432) : w[e][1];
+            const float sc = f16_bits_to_f32(d[e]);
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = __fmul_rn((float)(int8_t)((i < 4 ? a : b) >> (8 * (i & 3)) & 0xFFu), sc);
+            const size_t to = ((size_t)tok * heads + h) * KV_D + 8 * lane;
+            if (TYPE == ROWS_F32) {
+                float4 *dst = reinterpret_cast<float4 *>(static_cast<float *>(P.out[kv]) + to);
+                dst[0] = make_float4(x[0], x[1], x[2], x[3]);
+                dst[1] = make_float4(x[4], x[5], x[6], x[7]);
+            } else {
+                uint32_t y[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (TYPE == ROWS_F16) {
+                        const __half2 v = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+                        y[i] = *reinterpret_cast<const uint32_t *>(&v);
+                    } else {
+                        const __nv_bfloat162 v = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+                        y[i] = *reinterpret_cast<const uint32_t *>(&v);
+                    }
+                }
+                *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(P.out[kv]) + to) = make_uint4(y[0], y[1], y[2], y[3]);
+            }
+        }
+    }
+}
+
+}  // namespace b200

@@ -177,7 +177,7 @@ int raw(Truth t) { return t.v; }
 template <typename T> T raw(T v) { return v; }
 template <typename T> using Raw = decltype(raw(std::declval<T>()));
 
-constexpr int MAX_ARGS = 20;
+constexpr int MAX_ARGS = 24;
 
 // Host lists are as long as the call's last argument says.
 template <typename T> bool long_enough(const T &, int64_t) { return true; }
@@ -319,6 +319,58 @@ Call<Handle, int, Floats, Floats, int, int, Bytes, int64_t, float> pages_attn{
         if (!holds(out, {p->n_tok, n_head, PAGE_ROW})) return 3;
         return holds(workspace, {workspace_bytes}) ? -1 : 6;
     }};
+// From the first row's begin to the last one's end; a stride of one row is not used.
+template <typename M> bool spans(const M &x, int64_t n_tok, int64_t heads, int64_t dim, int64_t tok_stride, int64_t head_stride) {
+    const __int128 last = (__int128)(n_tok - 1) * (n_tok > 1 ? tok_stride : 0) + (__int128)(heads - 1) * (heads > 1 ? head_stride : 0) + dim;
+    return n_tok <= 0 || heads <= 0 || dim <= 0 || x.n < 0 || last <= x.n;
+}
+Call<Strided<at::kFloat>, Strided<at::kFloat>, Int32s, Doubles, Floats, Floats, int64_t, int, int, int, int, int, float, int64_t, int64_t, int64_t, int64_t> rope{
+    "rope", {"q", "k", "pos", "freq", "q_out", "k_out", "n_tok", "n_head", "n_head_kv", "head_dim", "n_rot", "pairs", "amplitude", "q_tok_stride", "q_head_stride", "k_tok_stride",
+             "k_head_stride"},
+    [](const auto &a) {
+        const auto &[q, k, pos, freq, q_out, k_out, n_tok, n_head, n_head_kv, head_dim, n_rot, pairs, amplitude, qt, qh, kt, kh] = a;
+        if (n_tok <= 0 || (n_head <= 0 && n_head_kv <= 0)) return -1;
+        if (!spans(q, n_tok, n_head, head_dim, qt, qh)) return 0;
+        if (!spans(k, n_tok, n_head_kv, head_dim, kt, kh)) return 1;
+        if (n_rot > 0 && !holds(pos, {n_tok})) return 2;
+        if (!holds(freq, {n_rot / 2})) return 3;
+        if (!holds(q_out, {n_tok, n_head, head_dim})) return 4;
+        return holds(k_out, {n_tok, n_head_kv, head_dim}) ? -1 : 5;
+    }};
+Call<Handle, int, Strided<at::kFloat>, Strided<at::kFloat>, Strided<at::kFloat>, Floats, Floats, Int32s, Doubles, Floats, int, int, int, float, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t,
+     float>
+    pages_write{"pages_write", {"pages", "layer", "q", "k", "v", "q_weight", "k_weight", "pos", "freq", "q_out", "n_head", "n_rot", "pairs", "amplitude", "q_tok_stride", "q_head_stride",
+                                "k_tok_stride", "k_head_stride", "v_tok_stride", "v_head_stride", "eps"},
+                [](const auto &a) {
+                    const auto &[pages, layer, q, k, v, q_weight, k_weight, pos, freq, q_out, n_head, n_rot, pairs, amplitude, qt, qh, kt, kh, vt, vh, eps] = a;
+                    const auto *p = static_cast<const bonsai_b200_pages *>(pages.p);
+                    if (!p || p->n_seq <= 0 || p->n_tok <= 0) return -1;
+                    if (!spans(q, p->n_tok, n_head, PAGE_ROW, qt, qh)) return 2;
+                    if (!spans(k, p->n_tok, p->n_head_kv, PAGE_ROW, kt, kh)) return 3;
+                    if (!spans(v, p->n_tok, p->n_head_kv, PAGE_ROW, vt, vh)) return 4;
+                    if (q_weight.p && n_head > 0 && !holds(q_weight, {PAGE_ROW})) return 5;
+                    if (k_weight.p && !holds(k_weight, {PAGE_ROW})) return 6;
+                    if (pos.p && n_rot > 0 && !holds(pos, {p->n_tok})) return 7;
+                    if (!holds(freq, {n_rot / 2})) return 8;
+                    return holds(q_out, {p->n_tok, n_head, PAGE_ROW}) ? -1 : 9;
+                }};
+Call<Handle, int, Int32s, Mem, Mem, int> pages_read{"pages_read", {"pages", "layer", "first", "k_out", "v_out", "type"}, [](const auto &a) {
+        const auto &[pages, layer, first, k_out, v_out, type] = a;
+        const auto *p = static_cast<const bonsai_b200_pages *>(pages.p);
+        return !p || p->n_seq <= 0 || p->n_tok <= 0 || !first.p || holds(first, {p->n_seq}) ? -1 : 2;       // (the outputs are Pages.read's to look at)
+    }};
+Call<Handle, int, Int32s, Int32s, int, Floats, Floats, int, Bytes, int64_t, float> pages_attn_shared{
+    "pages_attn_shared", {"pages", "layer", "group", "shared", "n_groups", "q", "out", "n_head", "workspace", "workspace_bytes", "scale"},
+    [](const auto &a) {
+        const auto &[pages, layer, group, shared, n_groups, q, out, n_head, workspace, workspace_bytes, scale] = a;
+        const auto *p = static_cast<const bonsai_b200_pages *>(pages.p);
+        if (!p || p->n_seq <= 0) return -1;
+        if (n_groups > 0 && !holds(group, {(int64_t)n_groups + 1})) return 2;
+        if (!holds(shared, {n_groups})) return 3;
+        if (!holds(q, {p->n_tok, n_head, PAGE_ROW})) return 5;
+        if (!holds(out, {p->n_tok, n_head, PAGE_ROW})) return 6;
+        return holds(workspace, {workspace_bytes}) ? -1 : 8;
+    }};
 Call<Bytes, int64_t, int, Ints, Ints, int> pages_copy{"pages_copy", {"pool", "page_bytes", "n_pages", "src", "dst", "n"}, [](const auto &a) {
         return std::get<5>(a) <= 0 || holds(std::get<0>(a), {std::get<1>(a), std::get<2>(a)}) ? -1 : 0;
     }};
@@ -347,7 +399,8 @@ Call<Handle, int, int, Mem, Mem> kv_attn_decode{"kv_attn_decode", {"kv", "layer"
 #define EACH_CALL(X)                                                                                                  \
     X(gemv) X(quant_activations) X(gemm) X(repack) X(gemv_repack) X(fwht) X(rmsnorm) X(gdn_step) X(attn)                \
     X(fwht_quant) X(swiglu) X(quant_batch) X(linear) X(linear_static) X(chain_run) X(kv_append) X(kv_append_batch)      \
-    X(kv_attn_decode) X(qk_norm_rope) X(pages_append) X(pages_attn) X(pages_copy) X(gdn_seqs)
+    X(kv_attn_decode) X(qk_norm_rope) X(pages_append) X(pages_attn) X(pages_copy) X(gdn_seqs) X(rope) X(pages_write)      \
+    X(pages_read) X(pages_attn_shared)
 
 #define WRAPPER(f)                                                                                                    \
     PyObject *py_##f(PyObject *, PyObject *const *v, Py_ssize_t n, PyObject *kw) { return f.call(v, n, kw); }
