@@ -61,7 +61,7 @@ SIGNATURES = {
     "bonsai_b200_rope_freq": (_INT, [_VP, _VP, _INT, C.c_double, _INT, C.c_double, _INT]),
     "bonsai_b200_pages_write": (_INT, [_VP, _INT] + [_VP] * 8 + [_INT] * 3 + [_F] + [_I64] * 6 + [_F, _VP]),
     "bonsai_b200_pages_read": (_INT, [_VP, _INT, _VP, _VP, _VP, _INT, _VP]),
-    "bonsai_b200_pages_attn_shared_workspace": (_I64, [_INT] * 5),
+    "bonsai_b200_pages_attn_shared_workspace": (_I64, [_VP, _INT, _INT]),
     "bonsai_b200_pages_attn_shared": (_INT, [_VP, _INT, _VP, _VP, _INT, _VP, _VP, _INT, _VP, _I64, _F, _VP]),
     "bonsai_b200_pages_append": (_INT, [_VP, _INT, _VP, _VP, _VP]),
     "bonsai_b200_pages_attn_workspace": (_I64, [_INT] * 5),
@@ -290,10 +290,6 @@ def rope(q, k, pos, freq, q_out, k_out, n_tok, n_head, n_head_kv, head_dim, n_ro
                           k_head_stride)
 
 
-def pages_attn_shared_workspace(n_tok, n_seq, n_groups, n_head, n_head_kv):
-    return lib().bonsai_b200_pages_attn_shared_workspace(n_tok, n_seq, n_groups, n_head, n_head_kv)
-
-
 def pages_attn_workspace(n_tok, max_len, n_seq, n_head, n_head_kv):
     return lib().bonsai_b200_pages_attn_workspace(n_tok, max_len, n_seq, n_head, n_head_kv)
 
@@ -490,7 +486,7 @@ class Pages:
         return _native().pages_read(self._struct(), layer, first, k_out, v_out, types[outs[0].dtype])
 
     def attn_shared_workspace(self, n_groups, n_head):
-        return pages_attn_shared_workspace(self.n_tok, self.n_seq, n_groups, n_head, self._s.n_head_kv)
+        return lib().bonsai_b200_pages_attn_shared_workspace(self._p, n_groups, n_head)
 
     def attn_shared(self, layer, group, shared, q, out, n_head, workspace, scale):
         """group: int32 [groups + 1], shared: int32 [groups] (both may be None: no groups); workspace: a tensor of attn_shared_workspace(groups, n_head) bytes."""

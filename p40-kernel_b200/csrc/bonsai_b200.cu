@@ -24,6 +24,7 @@
 #include "pages.cuh"
 #include "pages_rows.cuh"
 #include "pages_shared.cuh"
+#include "pages_shared_tc.cuh"
 #include "pages_tc.cuh"
 #include "probe.cuh"
 #include "ptq.cuh"
@@ -2231,20 +2232,34 @@ int bonsai_b200_pages_read(const bonsai_b200_pages *pages, int layer, const int3
 }
 
 namespace {
-// Parts of pages_attn_shared: rows of the groups and of the sequences (each call row once in either), and one tile for each CTA.
-inline int64_t shared_rows(int n_tok, int n_head) { return 2 * (int64_t)n_tok * n_head; }
-inline int64_t shared_part_bytes(int n_tok, int n_head) {
-    const int64_t rows = shared_rows(n_tok, n_head) + (int64_t)SM_COUNT * PSH_ROWS;
-    return rows * KV_D * (int64_t)sizeof(float) + (rows * (int64_t)sizeof(float2) + 15) / 16 * 16;
+static_assert(SM_COUNT <= PSH_CTAS, "");
+// The workspace of pages_attn_shared: parts of rows of the groups and of the sequences (each call row once in either) and a tile for each CTA, on either line; images of the pages of entities
+// of many rows; the plan.
+struct SharedPlan {
+    int64_t part_rows, all_rows, images;
+    int64_t part_bytes() const { return all_rows * KV_D * (int64_t)sizeof(float) + (all_rows * (int64_t)sizeof(float2) + 15) / 16 * 16; }
+    int64_t image_bytes(int n_head_kv) const { return images * n_head_kv * ATC_IMG_BYTES; }
+};
+SharedPlan plan_shared(int n_tok, int n_head, int n_head_kv, int n_pages, int table_stride) {
+    SharedPlan p = {};
+    const int64_t rows = (int64_t)n_tok * (n_head / n_head_kv), many = 2 * rows / (PST_MIN_ROWS + 1);        // entities that can have so many rows
+    p.part_rows = 2 * (int64_t)n_tok * n_head;
+    p.images = rows > PST_MIN_ROWS ? std::min<int64_t>({n_pages, many * table_stride, PTC_IMAGE_LIMIT / ATC_IMG_BYTES / n_head_kv}) : 0;
+    p.all_rows = p.part_rows + (int64_t)SM_COUNT * (PSH_ROWS + (p.images ? PST_ROWS : 0));
+    return p;
 }
-inline bool shared_sizes(int n_tok, int n_seq, int n_groups, int n_head, int n_head_kv) {
-    return n_groups >= 0 && n_groups <= n_seq && (int64_t)n_groups + n_seq <= INT32_MAX - PSH_THREADS && pages_attn_sizes(n_tok, 1, n_seq, n_head, n_head_kv);
+bool shared_sizes(const bonsai_b200_pages *p, int n_groups, int n_head) {
+    return n_groups >= 0 && n_groups <= p->n_seq && (int64_t)n_groups + p->n_seq <= INT32_MAX - PSP_THREADS && n_head > 0 && pages_attn_sizes(p->n_tok, 1, p->n_seq, n_head, p->n_head_kv);
+}
+int64_t shared_bytes(const bonsai_b200_pages *p, int n_groups, int n_head) {
+    const SharedPlan s = plan_shared(p->n_tok, n_head, p->n_head_kv, p->n_pages, p->table_stride);
+    return s.image_bytes(p->n_head_kv) + s.part_bytes() + psh_plan_bytes((int64_t)n_groups + p->n_seq);
 }
 }  // namespace
 
-int64_t bonsai_b200_pages_attn_shared_workspace(int n_tok, int n_seq, int n_groups, int n_head, int n_head_kv) {
-    if (!shared_sizes(n_tok, n_seq, n_groups, n_head, n_head_kv)) return 0;
-    return shared_part_bytes(n_tok, n_head) + (1 + (int64_t)n_groups + n_seq) * (int64_t)sizeof(PshPlan);
+int64_t bonsai_b200_pages_attn_shared_workspace(const bonsai_b200_pages *pages, int n_groups, int n_head) {
+    if (!pages || pages->n_pages <= 0 || pages->table_stride <= 0 || pages->n_head_kv > 65535 || !shared_sizes(pages, n_groups, n_head)) return 0;
+    return shared_bytes(pages, n_groups, n_head);
 }
 
 int bonsai_b200_pages_attn_shared(const bonsai_b200_pages *pages, int layer, const int32_t *group, const int32_t *shared, int n_groups, const float *q, float *out, int n_head,
@@ -2254,11 +2269,18 @@ int bonsai_b200_pages_attn_shared(const bonsai_b200_pages *pages, int layer, con
     const int rc = check_pages(pages, layer, &P.C);
     if (rc) return rc < 0 ? 0 : rc;
     const PageCache &C = P.C;
-    if (!q || !out || !aligned4(q) || !aligned4(out) || !shared_sizes(C.n_tok, C.n_seq, n_groups, n_head, C.n_head_kv)) return 1;
+    if (!q || !out || !aligned4(q) || !aligned4(out) || !shared_sizes(pages, n_groups, n_head)) return 1;
     if (n_groups && (!group || !shared || !aligned4(group) || !aligned4(shared))) return 1;
-    if (!workspace || !aligned16(workspace) || workspace_bytes < bonsai_b200_pages_attn_shared_workspace(C.n_tok, C.n_seq, n_groups, n_head, C.n_head_kv)) return 1;
+    if (!workspace || !aligned16(workspace) || workspace_bytes < shared_bytes(pages, n_groups, n_head)) return 1;
     const int64_t join_ctas = ((int64_t)C.n_tok * n_head + PSJ_WARPS - 1) / PSJ_WARPS;
     if (join_ctas > INT32_MAX) return 1;
+    const SharedPlan plan = plan_shared(C.n_tok, n_head, C.n_head_kv, C.n_pages, C.table_stride);
+    uint8_t *w = static_cast<uint8_t *>(workspace);
+    P.images = w;
+    w += plan.image_bytes(C.n_head_kv);
+    P.part = reinterpret_cast<float *>(w);
+    P.part_ml = reinterpret_cast<float2 *>(P.part + plan.all_rows * KV_D);
+    P.plan = reinterpret_cast<PshPlan *>(w + plan.part_bytes());
     P.q = q;
     P.out = out;
     P.layer = layer;
@@ -2268,20 +2290,25 @@ int bonsai_b200_pages_attn_shared(const bonsai_b200_pages *pages, int layer, con
     P.group_first = group;
     P.group_pages = shared;
     P.scale = scale;
-    P.part_rows = shared_rows(C.n_tok, n_head);
-    P.part = static_cast<float *>(workspace);
-    P.part_ml = reinterpret_cast<float2 *>(P.part + (P.part_rows + (int64_t)SM_COUNT * PSH_ROWS) * KV_D);
-    P.plan = reinterpret_cast<PshPlan *>(static_cast<uint8_t *>(workspace) + shared_part_bytes(C.n_tok, n_head));
-    static SmemOptIn opt;
-    cudaError_t e = opt.ensure(pages_shared_kernel);
+    P.part_rows = plan.part_rows;
+    P.image_room = (int)plan.images;
+    P.ctas = SM_COUNT;
+    static SmemOptIn opt[2];
     // what the warps' shares of the registers add up to is what the launch has to bring: one that asked for more would wait for them for good
     static const int regs = [] {
         cudaFuncAttributes a = {};
         return cudaFuncGetAttributes(&a, pages_shared_kernel) == cudaSuccess ? a.numRegs : 0;
     }();
-    if (e == cudaSuccess && regs * PSH_THREADS < PSH_REGS) e = cudaErrorLaunchOutOfResources;
-    if (e == cudaSuccess) e = launch(pages_shared_kernel, dim3(SM_COUNT), dim3(PSH_THREADS), (size_t)PSH_SMEM_BYTES, as_stream(stream), true, P);
-    if (e == cudaSuccess) e = launch(pages_shared_join_kernel, dim3((unsigned)join_ctas), dim3(32 * PSJ_WARPS), 0, as_stream(stream), true, P);
+    const cudaStream_t st = as_stream(stream);
+    cudaError_t e = regs * PSH_THREADS < PSH_REGS ? cudaErrorLaunchOutOfResources : opt[0].ensure(pages_shared_kernel);
+    if (e == cudaSuccess && P.image_room) e = opt[1].ensure(pages_shared_tc_kernel);
+    if (e == cudaSuccess) e = launch(pages_shared_plan_kernel, dim3(1), dim3(PSP_THREADS), 0, st, true, P);
+    if (P.image_room) {
+        if (e == cudaSuccess) e = launch(pages_shared_planes_kernel, dim3(4 * SM_COUNT, 1, 2), dim3(ATC_PREP_THREADS), 0, st, true, P);
+        if (e == cudaSuccess) e = launch(pages_shared_tc_kernel, dim3(SM_COUNT), dim3(PST_THREADS), (size_t)PST_SMEM_BYTES, st, true, P);
+    }
+    if (e == cudaSuccess) e = launch(pages_shared_kernel, dim3(SM_COUNT), dim3(PSH_THREADS), (size_t)PSH_SMEM_BYTES, st, true, P);
+    if (e == cudaSuccess) e = launch(pages_shared_join_kernel, dim3((unsigned)join_ctas), dim3(32 * PSJ_WARPS), 0, st, true, P);
     return (int)e;
 }
 

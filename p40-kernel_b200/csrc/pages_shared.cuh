@@ -9,11 +9,11 @@
 //
 // A fragment on the tensor cores (tcgen05.mma.kind::f16), positions as the rows of both products:
 //   S^T [128 positions x rows] = K Q^T        K as A from tensor memory, Q as B from shared memory, both as two fp16 planes
-//   O^T [256 dims x rows]     = V^T P         V as A and the weights P as B from shared memory, two planes each
+//   O^T [256 dims x rows]     = V^T P         V as A from tensor memory, the weights P as B from shared memory, two planes each
 // three of the four products of planes.  A product's time goes with its rows in steps of 16, so a tile of one token's six heads costs a third of a full one.
 //
-// Warps: 0 - 7 weights and outputs (a thread has a position of S^T, or two dims of O^T, and half of the columns), 8 - 11 K (a position a thread), 12 - 15 V (a
-// position and two of eight blocks a thread), 16 says what the fragments are, 17 copies pages, 18 issues the products.
+// Warps: 0 - 7 weights and outputs (a thread has a position of S^T, or two dims of O^T, and half of the columns), 8 - 15 V (a dim a thread), 16 - 19 K (a position a
+// thread), 20 says what the fragments are and copies pages of V, 21 copies those of K, 22 and 23 issue the products of scores and of outputs.
 #pragma once
 
 #include "attn_tc.cuh"
@@ -21,57 +21,84 @@
 
 namespace b200 {
 
-constexpr int PSH_ROWS = 48, PSH_STEP = 2 * PG_POS, PSH_STAGE = 32, PSH_STAGES = 2, PSH_VSLOTS = 3, PSH_DESCS = 4;
+constexpr int PSH_ROWS = 48, PSH_STEP = 2 * PG_POS, PSH_STAGE = 32, PSH_CHUNK = 64, PSH_DESCS = 4;
+constexpr int PSH_KSLOTS = 4, PSH_VSLOTS = 3;                    // pages of K and of V in shared memory
+constexpr int PSH_KRING = 2, PSH_VRING = 2;      // in tensor memory: 64 dims of a step's K, 32 positions of V
 constexpr int PSH_START = 1;                                     // what a fragment's begin is worth, in steps
-constexpr int PSH_THREADS = 640, PSH_SUM_WARPS = 8, PSH_K_WARP = 8, PSH_V_WARP = 12, PSH_PLAN_WARP = 16, PSH_LOAD_WARP = 17, PSH_MMA_WARP = 18;
-// registers a thread: 2 x 136 + 2 x 80 + 48 = 5 x 96, what the launch has
-constexpr int PSH_REGS_SUM = 136, PSH_REGS_PLANES = 80, PSH_REGS_REST = 48;
-constexpr int PSH_REGS = 32 * (PSH_SUM_WARPS * PSH_REGS_SUM + 8 * PSH_REGS_PLANES + 4 * PSH_REGS_REST);
+constexpr int PSH_THREADS = 768, PSH_SUM_WARPS = 8, PSH_V_WARP = 8, PSH_K_WARP = 16, PSH_PLAN_WARP = 20, PSH_LOAD_WARP = 21, PSH_SCORE_WARP = 22, PSH_OUT_WARP = 23;
+// registers a thread: 2 x 136 + 2 x 48 + 64 + 48 = 6 x 80, what the launch has
+constexpr int PSH_REGS_SUM = 136, PSH_REGS_V = 48, PSH_REGS_K = 64, PSH_REGS_REST = 48;
+constexpr int PSH_REGS = 32 * (8 * PSH_REGS_SUM + 8 * PSH_REGS_V + 4 * PSH_REGS_K + 4 * PSH_REGS_REST);
 constexpr int PSH_Q_CHUNK = PSH_ROWS * 128, PSH_Q_PLANE = 4 * PSH_Q_CHUNK;              // 64 dims of the rows; a plane of them
-constexpr int PSH_V_PLANE = PSH_STAGE * KV_D * 2, PSH_V_STAGE = 2 * PSH_V_PLANE;
-constexpr int PSH_P_GROUP = PSH_ROWS / 8 * 128, PSH_P_PLANE = PSH_STEP / 8 * PSH_P_GROUP;       // 8 positions of the rows
-constexpr int PSH_AT_V = 2 * PSH_Q_PLANE, PSH_AT_P = PSH_AT_V + PSH_STAGES * PSH_V_STAGE, PSH_AT_RAWK = PSH_AT_P + 2 * PSH_P_PLANE,
-              PSH_AT_RAWV = PSH_AT_RAWK + 2 * PG_HEAD_BYTES, PSH_AT_SMALL = PSH_AT_RAWV + PSH_VSLOTS * PG_HEAD_BYTES;
-constexpr uint32_t PSH_COL_K = 0, PSH_COL_S = 256, PSH_COL_O = 320, PSH_O_BUF = 2 * PSH_ROWS;   // tensor memory: K planes, scores, two buffers of outputs
-static_assert(PSH_COL_S + PSH_ROWS <= PSH_COL_O && PSH_COL_O + 2 * PSH_O_BUF <= 512, "");
+constexpr int PSH_P_GROUP = PSH_ROWS / 8 * 128, PSH_P_PLANE = PSH_STEP / 8 * PSH_P_GROUP, PSH_P_BUF = 2 * PSH_P_PLANE;       // 8 positions of the rows
+constexpr int PSH_AT_P = 2 * PSH_Q_PLANE, PSH_AT_RAWK = PSH_AT_P + 2 * PSH_P_BUF, PSH_AT_RAWV = PSH_AT_RAWK + PSH_KSLOTS * PG_HEAD_BYTES,
+              PSH_AT_D = PSH_AT_RAWV + PSH_VSLOTS * PG_HEAD_BYTES, PSH_AT_SMALL = PSH_AT_D + KV_NBLK * PSH_STEP * 2;
+// tensor memory, all 512 columns: K (64 dims: high, low), V (two halves of the dims x high, low), scores, two buffers of outputs
+constexpr uint32_t PSH_COL_K = 0, PSH_COL_V = PSH_KRING * 64, PSH_COL_S = PSH_COL_V + PSH_VRING * 64, PSH_COL_O = PSH_COL_S + PSH_ROWS, PSH_O_BUF = 2 * PSH_ROWS;
+static_assert(PSH_COL_O + 2 * PSH_O_BUF <= 512 && (PSH_VRING & (PSH_VRING - 1)) == 0, "");
+static_assert(PSH_ROWS * KV_D * 4 <= 2 * PSH_P_BUF, "a fragment's queries come by the weights' place");
 
 struct PshFragment {
     int begin, row0, n_rows;            // first token of the entity; of its rows the tile's first, and how many
     int kvh, pos0, steps, end;          // first position; steps (negative: no more fragments); positions that any row sees end here
     int before;                         // the last position that row r sees is before + r / group; INT32_MAX: all up to end
-    int group, seq;                     // whose table: of a group's sequences the first that has it (seq < 0), or the sequence's
+    int seq;                            // whose table
     long long part;                     // the first row's place among the parts
 };
-struct PshSmall {
-    float kf[2][PSH_STEP];              // 2^-s of the step's K rows; steps alternate
-    float vf[4][KV_NBLK];               // 2^-s of the step's V blocks; of four steps: V is at most three ahead of who adds the outputs
-    uint32_t v_bad[4][4][4];            // positions whose V is no number, by warp
+struct alignas(16) PshSmall {
+    int8_t ks[4][PSH_STEP];             // powers of two of the steps' K rows
+    // 2^-s of the step's V blocks, whether scales are no numbers, and at which positions.  Of eight steps: V is at most two stages ahead of the products, and who adds the outputs
+    // a step behind
+    float vf[8][KV_NBLK];
+    uint8_t v_odd[8][KV_NBLK];
+    uint32_t v_bad[8][4][KV_NBLK];
     float qf[PSH_ROWS];                 // 2^-s of the query rows times scale and log2 e
     int limit[PSH_ROWS];                // the last position that a row sees
-    float ref[PSH_ROWS], change[PSH_ROWS], red[4][PSH_ROWS];
+    float less[PSH_ROWS], change[PSH_ROWS], red[4][PSH_ROWS];        // less: a row's reference, negative
+    uint8_t none[PSH_ROWS];             // a row has seen a V that is no number
     PshFragment desc[PSH_DESCS];
-    uint64_t dfull[PSH_DESCS], dempty[PSH_DESCS], rkfull[2], rkempty[2], rvfull[PSH_VSLOTS], rvempty[PSH_VSLOTS], vready[PSH_STAGES], vempty[PSH_STAGES];
-    uint64_t qready, kready, qkdone, sempty, pready, pvdone, done;
-    int held_k[2], held_v[PSH_VSLOTS];  // rows of a page that there are
+    uint64_t dfull[PSH_DESCS], dempty[PSH_DESCS], rkfull[PSH_KSLOTS], rkempty[PSH_KSLOTS], rvfull[PSH_VSLOTS], rvempty[PSH_VSLOTS], kready[PSH_KRING], kempty[PSH_KRING],
+        vready[PSH_VRING], vempty[PSH_VRING];
+    uint64_t qready, qkdone, sempty, pready[2], pvdone[2], oempty[2], done[2];
+    int held_k[PSH_KSLOTS], held_v[PSH_VSLOTS];          // rows of a page that there are
     uint32_t tmem;
     int failed;
-    // the division
-    long long warp_sum[2][PSH_THREADS / 32], found[2], total;
-    int found_at;
 };
 constexpr int PSH_SMEM_BYTES = 1024 + PSH_AT_SMALL + (int)sizeof(PshSmall);
 static_assert(PSH_SMEM_BYTES <= 227 * 1024, "");
 
-struct PshPlan { long long unit, row; };                         // of an entity: units and rows of parts in front
+// Entities of many rows are pages_shared_tc_kernel's (pages_shared_tc.cuh): tiles of 128 rows, steps of a page, a line of their own.
+constexpr int PST_ROWS = 128, PST_MIN_ROWS = 96, PST_START = 2;
+constexpr float PSH_LIFT = 1.0f + 6 * 0x1p-23f;
+
+// What there is to do, found by pages_shared_plan_kernel: a group over its shared pages, or a sequence over its own positions.
+struct alignas(16) PshEntity {
+    int begin, tokens;                  // rows of tokens
+    int page0, end;                     // first page, end of its positions
+    int before;                         // the last position that token i sees is before + i; INT32_MAX: all up to end
+    int steps;                          // (pages, of an entity of many rows) 0: nothing; -1: numbers that do not fit
+    int seq, group;                     // whose table; the group that a sequence shares page0 pages with
+    int image;                          // of an entity of many rows: its first page's image; others -1
+    long long unit, row;                // units and rows of parts in front, on its line (unit negative: not served)
+};
+constexpr int PSH_CTAS = 160;                                    // most CTAs of a launch
+struct PshPlan {
+    long long total, per;               // units; of a CTA
+    long long tc_total, tc_per, tc_row; // the same of the other line, and where its parts begin
+    int images, first[PSH_CTAS], tc_first[PSH_CTAS];             // images; the entity that a CTA's units begin in
+    PshEntity entity[1];                // groups, then sequences
+};
+constexpr int64_t psh_plan_bytes(int64_t entities) { return (int64_t)sizeof(PshPlan) + entities * (int64_t)sizeof(PshEntity); }
 struct PageShared {
     PageCache C;
     const float *q;
     float *out, *part;                  // [part_rows][256]
     float2 *part_ml;                    // maximum (as a power of two's exponent) and sum of a part's rows
-    PshPlan *plan;                      // [1 + entities]; the first says how many units a CTA has
+    PshPlan *plan;
+    uint8_t *images;                    // [image_room][kv head]
     const int32_t *group_first, *group_pages;
     long long part_rows;                // of entities; CTAs' own come beside them
-    int n_groups, layer, n_head, group;
+    int n_groups, layer, n_head, group, ctas, image_room;
     float scale;
 };
 
@@ -98,54 +125,44 @@ __device__ __forceinline__ int psh_group_of(const PageShared &P, int s) {
     }
     return lo < P.n_groups && P.group_first[lo] <= s ? lo : P.n_groups;
 }
-struct PshWork {
-    int begin, tokens, page0, end, before, steps;                // steps 0: nothing; -1: numbers that do not fit
-};
-__device__ __forceinline__ PshWork psh_sequence(const PageShared &P, int s) {
+__device__ __forceinline__ int psh_steps(int positions) { return (positions + PSH_STEP - 1) / PSH_STEP; }
+__device__ __forceinline__ PshEntity psh_entity(const PageShared &P, int e) {
     const PageCache &C = P.C;
+    PshEntity E = {0, 0, 0, 0, INT32_MAX, 0, -1, 0, -1, 0, 0};
+    if (e < P.n_groups) {
+        const PshGroup G = psh_group(P, e);
+        E.begin = G.begin;
+        E.tokens = G.end - G.begin;
+        E.end = max(G.pages, 0) * PG_POS;
+        if (E.tokens > 0) E.steps = psh_steps(E.end);
+        return E;
+    }
+    const int s = e - P.n_groups, len = C.len[s];
     const SeqRange r = seq_range(C.start, s, C.n_tok);
-    PshWork W = {r.begin, r.n, 0, 0, 0, 0};
-    if (r.n <= 0) {
-        if (r.n < 0) W.steps = -1;
-        return W;
-    }
-    const int len = C.len[s], g = psh_group_of(P, s);
-    if (len < 0 || len > (int64_t)C.table_stride * PG_POS) {
-        W.steps = -1;
-        return W;
-    }
-    if (g < P.n_groups) {
-        const PshGroup G = psh_group(P, g);
+    E.begin = r.begin;
+    E.tokens = max(r.n, 0);
+    E.seq = s;
+    E.group = psh_group_of(P, s);
+    if (r.n < 0) E.steps = -1;
+    if (r.n <= 0) return E;
+    bool fits = len >= 0 && len <= (int64_t)C.table_stride * PG_POS;
+    if (E.group < P.n_groups) {
+        const PshGroup G = psh_group(P, E.group);
+        E.page0 = max(G.pages, 0);
         // (its new tokens lie behind what it shares)
-        if (G.pages < 0 || (G.pages > 0 && (r.begin < G.begin || r.begin + r.n > G.end || (int64_t)len - r.n < (int64_t)G.pages * PG_POS))) {
-            W.steps = -1;
-            return W;
-        }
-        W.page0 = G.pages;
+        fits = fits && G.pages >= 0 && (G.pages == 0 || (r.begin >= G.begin && r.begin + r.n <= G.end && (int64_t)len - r.n >= (int64_t)G.pages * PG_POS));
     }
-    W.end = len;
-    W.before = len - r.n;
-    W.steps = (len - W.page0 * PG_POS + PSH_STEP - 1) / PSH_STEP;
-    return W;
+    E.end = len;
+    E.before = len - r.n;
+    E.steps = fits ? psh_steps(len - E.page0 * PG_POS) : -1;
+    return E;
 }
-__device__ __forceinline__ PshWork psh_work(const PageShared &P, int e) {
-    if (e >= P.n_groups) return psh_sequence(P, e - P.n_groups);
-    const PshGroup G = psh_group(P, e);
-    PshWork W = {G.begin, G.end - G.begin, 0, max(G.pages, 0) * PG_POS, INT32_MAX, 0};
-    if (W.tokens > 0) W.steps = (W.end + PSH_STEP - 1) / PSH_STEP;
-    return W;
+// Where what a tile sees ends: with its last row.
+__device__ __forceinline__ int psh_tile_end(int group, const PshEntity &E, int row0, int rows) {
+    if (E.before == INT32_MAX) return E.end;
+    const int last = min(row0 + rows, E.tokens * group) - 1;
+    return max(E.page0 * PG_POS, min(E.end, E.before + last / group + 1));
 }
-__device__ __forceinline__ long long psh_rows(const PageShared &P, const PshWork &W) { return W.steps > 0 ? (long long)W.tokens * P.n_head : 0; }
-__device__ __forceinline__ long long psh_units(const PageShared &P, const PshWork &W) {
-    return W.steps > 0 ? ((long long)W.tokens * P.group + PSH_ROWS - 1) / PSH_ROWS * P.C.n_head_kv * (W.steps + PSH_START) : 0;
-}
-// Steps of a tile: those that its last row sees.
-__device__ __forceinline__ int psh_tile_end(const PageShared &P, const PshWork &W, long long row0) {
-    if (W.before == INT32_MAX) return W.end;
-    const long long last = min(row0 + PSH_ROWS, (long long)W.tokens * P.group) - 1;
-    return max(W.page0 * PG_POS, min(W.end, W.before + (int)(last / P.group) + 1));
-}
-__device__ __forceinline__ int psh_tile_steps(const PshWork &W, int end) { return (end - W.page0 * PG_POS + PSH_STEP - 1) / PSH_STEP; }
 
 __device__ __forceinline__ long long psh_scan(long long x, int lane) {
 #pragma unroll
@@ -156,81 +173,92 @@ __device__ __forceinline__ long long psh_scan(long long x, int lane) {
     return x;
 }
 
-// Units of a CTA, and where this one's begin: entity small.found_at, which has found[0] units and found[1] rows in front.  By the whole CTA; the last one leaves the
-// plan for the join, and says what does not fit.
-__device__ __forceinline__ long long psh_divide(const PageShared &P, PshSmall &S) {
+// One CTA.  The work of every entity, and what lies in front of it.  (Each CTA of the attention finding that by itself took it 9 us, most of them instructions that are not in the cache
+// yet; here they are few, and the attention's CTAs start meanwhile.)
+constexpr int PSP_THREADS = 512;
+__global__ void __launch_bounds__(PSP_THREADS) pages_shared_plan_kernel(const __grid_constant__ PageShared P) {
+    __shared__ long long sums[PSP_THREADS / 32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, entities = P.n_groups + P.C.n_seq;
-    const bool writer = blockIdx.x == gridDim.x - 1;
-    long long unit0 = 0, row0 = 0, per = 0;
-    long long units = 0, rows = 0, unit_end = 0, row_end = 0;
-    for (int pass = 0; pass < 2; ++pass) {               // how many; whose the CTA's first is
-        unit0 = row0 = 0;
-        for (int base = 0; base < entities; base += PSH_THREADS) {
-            const int e = base + tid;
-            if (pass == 0 || entities > PSH_THREADS) {
-                PshWork W = {0, 0, 0, 0, 0, 0};
-                if (e < entities) W = psh_work(P, e);
-                if (pass == 0 && writer && W.steps < 0) bad_sequence();
-                units = psh_units(P, W);
-                rows = psh_rows(P, W);
-                row_end = psh_scan(rows, lane);
-                if (lane == 31) S.warp_sum[1][warp] = row_end;
-                __syncthreads();
-                for (int w = 0; w < warp; ++w) row_end += S.warp_sum[1][w];
-                row_end += row0;
-                if (row_end > P.part_rows) {             // rows that several sequences claim
-                    if (pass == 0 && writer && rows) bad_sequence();
-                    units = 0;
-                }
-                unit_end = psh_scan(units, lane);
-                if (lane == 31) S.warp_sum[0][warp] = unit_end;
-                __syncthreads();
-                long long all = 0, all_rows = 0;
-                for (int w = 0; w < PSH_THREADS / 32; ++w) {
-                    if (w == warp) unit_end += all;
-                    all += S.warp_sum[0][w];
-                    all_rows += S.warp_sum[1][w];
-                }
-                unit_end += unit0;
-                unit0 += all;
-                row0 += all_rows;
-                __syncthreads();
-            }
-            if (pass == 1) {
-                const long long first = per * blockIdx.x;
-                if (units && unit_end - units <= first && first < unit_end) {
-                    S.found_at = e;
-                    S.found[0] = unit_end - units;
-                    S.found[1] = row_end - rows;
-                }
-                if (writer && e < entities) P.plan[1 + e] = {units ? unit_end - units : -1, row_end - rows};
-            }
-        }
-        if (pass == 0) per = (unit0 + gridDim.x - 1) / gridDim.x;
-        if (pass == 0 && tid == 0) {
-            S.total = unit0;
-            S.found_at = entities;
-            if (writer) P.plan[0] = {per, unit0};
+    PshPlan &plan = *P.plan;
+    pdl_wait_prior_grid();
+    pdl_launch_dependents();
+    // what lies in front of a thread's x, and of the next 512 threads' (front)
+    auto in_front = [&](long long x, long long &front) {
+        long long y = psh_scan(x, lane);
+        if (lane == 31) sums[warp] = y;
+        __syncthreads();
+        long long all = 0;
+        for (int w = 0; w < PSP_THREADS / 32; ++w) {
+            if (w == warp) y += all;
+            all += sums[w];
         }
         __syncthreads();
+        y += front - x;
+        front += all;
+        return y;
+    };
+    auto tiles = [&](const PshEntity &E) { return (long long)((E.tokens * P.group + (E.image < 0 ? PSH_ROWS : PST_ROWS) - 1) / (E.image < 0 ? PSH_ROWS : PST_ROWS)) * P.C.n_head_kv; };
+    auto units = [&](const PshEntity &E) { return tiles(E) * (E.steps + (E.image < 0 ? PSH_START : PST_START)); };        // (rows of a call are below 2^30)
+    long long rows0 = 0, images0 = 0, unit0 = 0, row0 = 0, tc_unit0 = 0, tc_row0 = 0;
+#pragma unroll 1
+    for (int base = 0; base < entities; base += PSP_THREADS) {
+        const int e = base + tid;
+        PshEntity E = {0, 0, 0, 0, 0, 0, -1, 0, -1, 0, 0};
+        if (e < entities) E = psh_entity(P, e);
+        if (E.steps < 0) bad_sequence();
+        long long rows = E.steps > 0 ? (long long)E.tokens * P.n_head : 0;
+        if (in_front(rows, rows0) + rows > P.part_rows && rows) {        // rows that several sequences claim
+            bad_sequence();
+            rows = 0;
+        }
+        const int pages = (E.end + PG_POS - 1) / PG_POS - E.page0;
+        const long long images = rows && P.image_room && E.tokens * P.group > PST_MIN_ROWS ? pages : 0, image = in_front(images, images0);
+        const bool many = images && image + images <= P.image_room;
+        if (many) E.image = (int)image, E.steps = pages;
+        const long long own = rows ? units(E) : 0;
+        const long long a = in_front(many ? 0 : own, unit0), b = in_front(many ? own : 0, tc_unit0), c = in_front(many ? 0 : rows, row0), d = in_front(many ? rows : 0, tc_row0);
+        E.unit = !rows ? -1 : many ? b : a;
+        E.row = many ? d : c;
+        if (e < entities) plan.entity[e] = E;
     }
-    return per;
+    const long long per = (unit0 + P.ctas - 1) / P.ctas, tc_per = (tc_unit0 + P.ctas - 1) / P.ctas;
+    if (tid < PSH_CTAS) plan.first[tid] = plan.tc_first[tid] = entities;
+    if (tid == 0) {
+        plan.total = unit0;
+        plan.per = per;
+        plan.tc_total = tc_unit0;
+        plan.tc_per = tc_per;
+        plan.tc_row = row0 + (long long)P.ctas * PSH_ROWS;
+        plan.images = (int)min(images0, (long long)P.image_room);
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int e = tid; e < entities; e += PSP_THREADS) {          // (its own entities)
+        PshEntity &E = plan.entity[e];
+        if (E.unit < 0) continue;
+        const long long end = E.unit + units(E), own = E.image < 0 ? per : tc_per;
+        int *const first = E.image < 0 ? plan.first : plan.tc_first;
+        for (long long c = (E.unit + own - 1) / own; c * own < end; ++c) first[c] = e;
+        // the table of a group: of its first sequence that has the pages in common
+        if (e < P.n_groups)
+            for (int s = P.group_first[e]; s < P.group_first[e + 1] && E.seq < 0; ++s)
+                if (plan.entity[P.n_groups + s].steps > 0) E.seq = s;
+    }
 }
 
 // ---- small pieces -------------------------------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ void psh_mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, bool add) {
-    // A: V planes, dims by 64 side by side (128-byte swizzle, 8 positions a kilobyte); B: weights, 8 rows x 8 positions a piece of 128 bytes
-    constexpr uint32_t A_HI = (uint32_t)(1024 >> 4) | (1u << 14) | (2u << 29), B_HI = (uint32_t)(128 >> 4) | (1u << 14);
+// A from tensor memory, B the weights: 8 rows x 8 positions a piece of 128 bytes, rows side by side.
+template <bool ADD>
+__device__ __forceinline__ void psh_mma_weights(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc) {
     asm volatile(
         "{\n\t"
         ".reg .pred p;\n\t"
-        ".reg .b64 da, db;\n\t"
-        "mov.b64 da, {%1, %4};\n\t"
-        "mov.b64 db, {%2, %5};\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t"
+        ".reg .b64 db;\n\t"
+        "mov.b64 db, {%2, %4};\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t"
         "}\n"
-        ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(A_HI), "r"(B_HI), "r"(add ? 1u : 0u)
+        ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "r"((uint32_t)(128 >> 4) | (1u << 14)), "n"(ADD ? 1 : 0)
         : "memory");
 }
 __device__ __forceinline__ float psh_exp2(float x) {
@@ -238,27 +266,38 @@ __device__ __forceinline__ float psh_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));        // 2^-22 of the value
     return y;
 }
-// Among the four warps of a half of the columns.
-__device__ __forceinline__ void psh_half_barrier(int half) { asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory"); }
-__device__ __forceinline__ bool psh_half_any(int half, bool x) {
+// Eight of a warp's columns (all lanes the same), at this place in the code: a thread has no registers to have them early.
+template <typename T>
+__device__ __forceinline__ void psh_lds8(const T *p, T (&x)[8]) {
+    uint32_t (&y)[8] = reinterpret_cast<uint32_t (&)[8]>(x);
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(y[0]), "=r"(y[1]), "=r"(y[2]), "=r"(y[3]) : "r"(smem_u32(p)) : "memory");
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(y[4]), "=r"(y[5]), "=r"(y[6]), "=r"(y[7]) : "r"(smem_u32(p) + 16u) : "memory");
+}
+// Barriers of some warps: 1 and 2 of the four of a half of the columns, 3 of both halves.
+template <int THREADS>
+__device__ __forceinline__ void psh_barrier(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(THREADS) : "memory"); }
+template <int THREADS>
+__device__ __forceinline__ bool psh_any(int id, bool x) {
     uint32_t y;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(y) : "r"(x ? 1u : 0u), "r"(1 + half) : "memory");
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(y) : "r"(x ? 1u : 0u), "r"(id), "n"(THREADS) : "memory");
     return y != 0;
 }
 // A pair of codes (bytes 0 and 1, or 2 and 3, of w) as fp16, exactly: 1024 + (byte ^ 128) - 1152; w comes with its bytes' signs turned.
-__device__ __forceinline__ __half2 psh_pair(uint32_t w, bool upper) {
-    const uint32_t x = __byte_perm(w, 0x64646464u, upper ? 0x4342 : 0x4140);
-    return __hsub2_rn(*reinterpret_cast<const __half2 *>(&x), __half2half2(__ushort_as_half((unsigned short)0x6480)));
+__device__ __forceinline__ uint32_t psh_pair(uint32_t w, bool upper) {
+    uint32_t y;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(__byte_perm(w, 0x64646464u, upper ? 0x4342 : 0x4140)), "r"(0x64806480u));
+    return y;
 }
 // Codes times a scale of two fp16 planes: the rounded product and, exactly, what it leaves.
-__device__ __forceinline__ void psh_planes(__half2 codes, __half2 d, uint32_t &hi, uint32_t &lo) {
-    const __half2 h = __hmul2_rn(codes, d), l = __hfma2(codes, d, __hneg2(h));
-    hi = *reinterpret_cast<const uint32_t *>(&h);
-    lo = *reinterpret_cast<const uint32_t *>(&l);
+__device__ __forceinline__ void psh_planes(uint32_t codes, uint32_t d, uint32_t &hi, uint32_t &lo) {
+    asm("{\n\t.reg .b32 n;\n\tmul.rn.f16x2 %0, %2, %3;\n\tneg.f16x2 n, %0;\n\tfma.rn.f16x2 %1, %2, %3, n;\n\t}" : "=&r"(hi), "=r"(lo) : "r"(codes), "r"(d));
 }
 // s with 2^7 <= d 2^s < 2^8 for the largest scale d of those under one power of two (magnitude bits of an fp16; no number, zero: 0)
 __device__ __forceinline__ int psh_shift(uint32_t mag) { return mag == 0 || mag >= 0x7C00u ? 0 : 134 - (int)(__float_as_uint(f16_bits_to_f32(mag)) >> 23); }
-__device__ __forceinline__ __half2 psh_scale(uint32_t d16, float up) { return __half2half2(__float2half_rn(__fmul_rn(f16_bits_to_f32(d16), up))); }
+__device__ __forceinline__ uint32_t psh_scale(uint32_t d16, float up) {
+    const uint32_t d = __half_as_ushort(__float2half_rn(__fmul_rn(f16_bits_to_f32(d16), up)));
+    return d | (d << 16);
+}
 __device__ __forceinline__ int psh_key(float x) {                // ordered as the floats are
     const int b = __float_as_int(x);
     return b ^ ((b >> 31) & 0x7FFFFFFF);
@@ -277,14 +316,34 @@ __device__ __forceinline__ PshStep psh_step(const PshFragment &F, int i) {
 }
 
 // ---- the warps ----------------------------------------------------------------------------------------------------------------------------------
-// A wait that runs out: nothing is waited for any more, the CTA comes to its end and leaves its parts unfinished.
+// A wait that runs out (a second at most): nothing is waited for any more, the CTA comes to its end and leaves its parts unfinished.  (One loop for a wait: what bounds this
+// kernel next to the tensor core is instructions that are not in the cache.)
+__device__ __forceinline__ bool psh_wait(uint64_t *bar, uint32_t parity) {
+    uint32_t left;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "mov.u32 %0, 0x40000;\n\t"
+        "PSH_LOOP:\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "@p bra PSH_DONE;\n\t"
+        "sub.u32 %0, %0, 1;\n\t"
+        "setp.ne.u32 p, %0, 0;\n\t"
+        "@p bra PSH_LOOP;\n\t"
+        "PSH_DONE:\n\t"
+        "}"
+        : "=&r"(left)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return left != 0;
+}
 struct PshWait {
     PshSmall &S;
     bool ok = true;
     __device__ __forceinline__ PshWait(PshSmall &s) : S(s) {}
     __device__ __forceinline__ void operator()(uint64_t *bar, uint32_t parity) {
         if (!ok) return;
-        ok = __all_sync(0xffffffffu, mbar_wait_try(bar, parity));
+        ok = __all_sync(0xffffffffu, psh_wait(bar, parity));
         if (!ok) *(volatile int *)&S.failed = 1;
     }
 };
@@ -303,371 +362,440 @@ struct PshReader {
     }
 };
 
-__device__ __forceinline__ void psh_plan_warp(const PageShared &P, PshSmall &S, long long per) {
-    const int lane = threadIdx.x & 31, entities = P.n_groups + P.C.n_seq, heads = P.C.n_head_kv;
-    PshWait wait(S);
-    long long at = per * blockIdx.x;
-    const long long last = min(at + per, S.total);
+// Pages to shared memory, KV 0: K, 1: V.
+template <int KV>
+struct PshLoader {
+    static constexpr int SLOTS = KV ? PSH_VSLOTS : PSH_KSLOTS;
+    const PageShared &P;
+    PshSmall &S;
+    PshWait &wait;
+    uint8_t *raw;
     int n = 0;
+    __device__ __forceinline__ PshLoader(const PageShared &p, PshSmall &s, PshWait &w, uint8_t *smem) : P(p), S(s), wait(w), raw(smem + (KV ? PSH_AT_RAWV : PSH_AT_RAWK)) {}
+    __device__ __forceinline__ void load(const PshFragment &F) {
+        const PageCache &C = P.C;
+        uint64_t *const fulls = KV ? S.rvfull : S.rkfull, *const empties = KV ? S.rvempty : S.rkempty;
+        int *const helds = KV ? S.held_v : S.held_k;
+        const int lane = threadIdx.x & 31;
+        const int32_t *table = C.table + (size_t)max(F.seq, 0) * C.table_stride + F.pos0 / PG_POS;
+        const int pages = (min(F.end, F.pos0 + F.steps * PSH_STEP) - F.pos0 + PG_POS - 1) / PG_POS;
+        int own = -1;                                    // 32 pages, a lane each
+#pragma unroll 1
+        for (int p = 0; p < pages && wait.ok; ++p, ++n) {
+            if ((p & 31) == 0) own = F.seq >= 0 && p + lane < pages ? table[p + lane] : -1;
+            const int page = __shfl_sync(0xffffffffu, own, p & 31), rows = min(PG_POS, F.end - F.pos0 - p * PG_POS), j = n % SLOTS;
+            const bool there = page >= 0 && page < C.n_pages;
+            if (!there && lane == 0) bad_sequence();
+            if (n >= SLOTS) wait(&empties[j], (uint32_t)((n / SLOTS - 1) & 1));
+            if (lane == 0) {                             // (a wait that ran out: nothing is copied, but those who wait for it are let go)
+                helds[j] = there && wait.ok ? rows : 0;
+                if (there && wait.ok) {
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    mbar_expect_tx(&fulls[j], (uint32_t)rows * KV_ROW);
+                    bulk_g2s(raw + j * PG_HEAD_BYTES, page_rows(C, page, P.layer, KV, F.kvh), (uint32_t)rows * KV_ROW, &fulls[j], policy_evict_normal());
+                } else {
+                    mbar_arrive(&fulls[j]);
+                }
+            }
+            __syncwarp();
+        }
+    }
+    __device__ __forceinline__ void end() {              // no copy outlives the CTA
+        uint64_t *const fulls = KV ? S.rvfull : S.rkfull;
+        for (int k = max(0, n - SLOTS); k < n; ++k) psh_wait(&fulls[k % SLOTS], (uint32_t)((k / SLOTS) & 1));
+    }
+};
+__device__ __forceinline__ void psh_load_k_warp(const PageShared &P, PshSmall &S, uint8_t *smem) {
+    PshWait wait(S);
+    PshReader frags{S, wait};
+    PshLoader<0> loader(P, S, wait, smem);
+    PshFragment F;
+    while (frags.next(F)) loader.load(F);
+    loader.end();
+}
+// Says what the CTA's fragments are, and copies their pages of V.
+__device__ __forceinline__ void psh_plan_warp(const PageShared &P, PshSmall &S, uint8_t *smem) {
+    const int lane = threadIdx.x & 31, entities = P.n_groups + P.C.n_seq, heads = P.C.n_head_kv;
+    const PshPlan &plan = *P.plan;
+    PshWait wait(S);
+    PshLoader<1> loader(P, S, wait, smem);
+    const long long per = plan.per, last = min(per * (blockIdx.x + 1), plan.total);
+    long long at = per * blockIdx.x;
+    int said = 0;
     auto say = [&](const PshFragment &F) {
-        if (n >= PSH_DESCS) wait(&S.dempty[n % PSH_DESCS], (uint32_t)((n / PSH_DESCS - 1) & 1));
+        if (said >= PSH_DESCS) wait(&S.dempty[said % PSH_DESCS], (uint32_t)((said / PSH_DESCS - 1) & 1));
         if (lane == 0) {
-            S.desc[n % PSH_DESCS] = F;
-            mbar_arrive(&S.dfull[n % PSH_DESCS]);
+            S.desc[said % PSH_DESCS] = F;
+            mbar_arrive(&S.dfull[said % PSH_DESCS]);
         }
         __syncwarp();
-        ++n;
+        ++said;
+        if (F.steps > 0) loader.load(F);
     };
-    long long unit0 = S.found[0], row0 = S.found[1];
-    for (int base = S.found_at; base < entities && at < last && wait.ok; base += 32) {
-        PshWork W = {0, 0, 0, 0, 0, 0};
-        if (base + lane < entities) W = psh_work(P, base + lane);
-        const long long rows = psh_rows(P, W), row_end = row0 + psh_scan(rows, lane);
-        const long long units = row_end > P.part_rows ? 0 : psh_units(P, W), unit_end = unit0 + psh_scan(units, lane);
-        for (int l = 0; l < 32 && at < last && wait.ok; ++l) {
-            const long long e_end = __shfl_sync(0xffffffffu, unit_end, l), e_units = __shfl_sync(0xffffffffu, units, l);
-            if (e_units == 0 || e_end <= at) continue;
-            PshWork X;
-            X.begin = __shfl_sync(0xffffffffu, W.begin, l);
-            X.tokens = __shfl_sync(0xffffffffu, W.tokens, l);
-            X.page0 = __shfl_sync(0xffffffffu, W.page0, l);
-            X.end = __shfl_sync(0xffffffffu, W.end, l);
-            X.before = __shfl_sync(0xffffffffu, W.before, l);
-            X.steps = __shfl_sync(0xffffffffu, W.steps, l);
-            const long long e_row = __shfl_sync(0xffffffffu, row_end - rows, l);
-            const int e = base + l, size = X.steps + PSH_START;
-            const long long unit = e_end - e_units;
-            while (at < e_end && at < last && wait.ok) {
-                const long long pair = (at - unit) / size, tile = pair / heads, begin = unit + pair * size;      // the tile and kv head that the next unit lies in
-                PshFragment F;
-                F.kvh = (int)(pair - tile * heads);
-                F.begin = X.begin;
-                F.row0 = (int)(tile * PSH_ROWS);
-                F.n_rows = (int)min((long long)PSH_ROWS, (long long)X.tokens * P.group - F.row0);
-                F.end = psh_tile_end(P, X, F.row0);
-                F.before = X.before;
-                F.group = e < P.n_groups ? e : -1;
-                F.seq = e < P.n_groups ? -1 : e - P.n_groups;
-                F.part = e_row + tile * PSH_ROWS * heads + (long long)F.kvh * F.n_rows + (long long)blockIdx.x * PSH_ROWS;
-                const long long stop = min(last, begin + size);
-                const int s0 = (int)max(0ll, at - begin - PSH_START), s1 = (int)min(stop - begin - PSH_START, (long long)psh_tile_steps(X, F.end));
-                F.pos0 = X.page0 * PG_POS + s0 * PSH_STEP;
-                F.steps = s1 - s0;
-                if (F.steps > 0) say(F);
-                at = stop;
-            }
-        }
-        unit0 = __shfl_sync(0xffffffffu, unit_end, 31);
-        row0 = __shfl_sync(0xffffffffu, row_end, 31);
-    }
     PshFragment F = {};
     F.steps = -1;
-    say(F);
-}
-
-__device__ __forceinline__ void psh_load_warp(const PageShared &P, PshSmall &S, uint8_t *smem) {
-    const PageCache &C = P.C;
-    const int lane = threadIdx.x & 31;
-    PshWait wait(S);
-    PshReader frags{S, wait};
-    PshFragment F;
-    int nk[2] = {0, 0}, nv = 0;
-    while (frags.next(F)) {
-        int seq = F.seq;
-        if (seq < 0) {                                   // the first sequence of the group that has the pages in common: one with new tokens behind them
-            const int first = P.group_first[F.group], last = P.group_first[F.group + 1];
-            for (int base = first; base < last && seq < 0; base += 32) {
-                bool has = false;
-                if (base + lane < last) {
-                    const PshWork W = psh_sequence(P, base + lane);
-                    has = W.steps > 0;
-                }
-                const unsigned found = __ballot_sync(0xffffffffu, has);
-                if (found) seq = base + __ffs(found) - 1;
-            }
-        }
-        const int32_t *table = C.table + (size_t)max(seq, 0) * C.table_stride;
-        const int page0 = F.pos0 / PG_POS, pages = (F.end - F.pos0 + PG_POS - 1) / PG_POS;
-        const uint64_t pol = policy_evict_normal();
-        for (int i = 0; i < F.steps && wait.ok; ++i) {
-            const PshStep T = psh_step(F, i);
-            int own = -1;
-            if (lane < T.pages && seq >= 0 && 2 * i + lane < pages) own = table[page0 + 2 * i + lane];
-            for (int j = 0; j < T.pages; ++j) {
-                int page = __shfl_sync(0xffffffffu, own, j);
-                const bool there = page >= 0 && page < C.n_pages;
-                if (!there && lane == 0) bad_sequence();
-                const int n = min(PG_POS, T.valid - j * PG_POS);
-                const uint32_t bytes = (uint32_t)n * KV_ROW;
-                auto copy = [&](int kv, uint8_t *dst, uint64_t *full, int *held) {
-                    if (lane) return;
-                    *held = there ? n : 0;
-                    if (there) {
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                        mbar_expect_tx(full, bytes);
-                        bulk_g2s(dst, page_rows(C, page, P.layer, kv, F.kvh), bytes, full, pol);
-                    } else {
-                        mbar_arrive(full);
-                    }
-                };
-                if (nk[j] > 0) wait(&S.rkempty[j], (uint32_t)((nk[j] - 1) & 1));
-                if (!wait.ok) break;
-                copy(0, smem + PSH_AT_RAWK + j * PG_HEAD_BYTES, &S.rkfull[j], &S.held_k[j]);
-                ++nk[j];
-                __syncwarp();
-            }
-            for (int j = 0; j < T.pages && wait.ok; ++j) {
-                int page = __shfl_sync(0xffffffffu, own, j);
-                const bool there = page >= 0 && page < C.n_pages;
-                const int n = min(PG_POS, T.valid - j * PG_POS), slot = nv % PSH_VSLOTS;
-                const uint32_t bytes = (uint32_t)n * KV_ROW;
-                if (nv >= PSH_VSLOTS) wait(&S.rvempty[slot], (uint32_t)((nv / PSH_VSLOTS - 1) & 1));
-                if (!wait.ok) break;
-                if (lane == 0) {
-                    S.held_v[slot] = there ? n : 0;
-                    if (there) {
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                        mbar_expect_tx(&S.rvfull[slot], bytes);
-                        bulk_g2s(smem + PSH_AT_RAWV + slot * PG_HEAD_BYTES, page_rows(C, page, P.layer, 1, F.kvh), bytes, &S.rvfull[slot], pol);
-                    } else {
-                        mbar_arrive(&S.rvfull[slot]);
-                    }
-                }
-                ++nv;
-                __syncwarp();
-            }
+#pragma unroll 1
+    for (int e = plan.first[blockIdx.x]; e < entities && at < last && wait.ok; ++e) {
+        const PshEntity E = plan.entity[e];
+        if (E.unit < 0 || E.image >= 0) continue;
+        const int size = E.steps + PSH_START, rows = E.tokens * P.group, pairs = (rows + PSH_ROWS - 1) / PSH_ROWS * heads;
+        // the tile and kv head that the next unit lies in
+        int pair = (int)((at - E.unit) / size);
+#pragma unroll 1
+        for (long long begin = E.unit + (long long)pair * size; pair < pairs && begin < last && wait.ok; ++pair, begin += size) {
+            const int tile = pair / heads;
+            F.kvh = pair - tile * heads;
+            F.begin = E.begin;
+            F.row0 = tile * PSH_ROWS;
+            F.n_rows = min(PSH_ROWS, rows - F.row0);
+            F.end = psh_tile_end(P.group, E, F.row0, PSH_ROWS);
+            F.before = E.before;
+            F.seq = E.seq;
+            F.part = E.row + (long long)F.row0 * heads + F.kvh * F.n_rows + (long long)blockIdx.x * PSH_ROWS;
+            const int s0 = (int)max(0ll, at - begin - PSH_START), s1 = min((int)min(last - begin, (long long)size) - PSH_START, psh_steps(F.end - E.page0 * PG_POS));
+            F.pos0 = E.page0 * PG_POS + s0 * PSH_STEP;
+            F.steps = s1 - s0;
+            if (F.steps > 0) say(F);
+            at = begin + size;
         }
     }
-    // no copy outlives the CTA
-    for (int j = 0; j < 2; ++j)
-        if (nk[j]) mbar_wait_try(&S.rkfull[j], (uint32_t)((nk[j] - 1) & 1));
-    for (int k = max(0, nv - PSH_VSLOTS); k < nv; ++k) mbar_wait_try(&S.rvfull[k % PSH_VSLOTS], (uint32_t)((k / PSH_VSLOTS) & 1));
+    F.steps = -1;
+    say(F);
+    loader.end();
 }
 
-// K rows to planes in tensor memory: a position a thread.
+// 64 dims of a row (words w: a scale's halfword, 32 codes, again) to planes.
+template <int FIRST>
+__device__ __forceinline__ void psh_k_chunk(const uint32_t *w, uint32_t none, float up, uint32_t to) {
+    constexpr int half0 = FIRST ? 34 : 0;                // of w's halfwords the chunk's first
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+        const int s = half0 + 17 * b;
+        const uint32_t d = psh_scale((s & 1 ? w[s >> 1] >> 16 : w[s >> 1] & 0xFFFFu) & none, up);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            uint32_t hi[8], lo[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int half = s + 1 + 8 * k + e;
+                psh_planes(psh_pair(w[half >> 1] ^ 0x80808080u, half & 1), d, hi[e], lo[e]);
+            }
+            tc_st8(to + (uint32_t)(16 * b + 8 * k), hi);
+            tc_st8(to + (uint32_t)(32 + 16 * b + 8 * k), lo);
+        }
+    }
+}
+// K rows to planes in tensor memory: a position a thread, 64 dims at a time.
 __device__ __forceinline__ void psh_k_warps(const PageShared &P, PshSmall &S, uint8_t *smem, uint32_t tmem) {
-    const int lane = threadIdx.x & 31, quarter = (threadIdx.x >> 5) & 3, pos = 32 * quarter + lane, slot = quarter >> 1;
-    const uint32_t to = tmem + PSH_COL_K + ((uint32_t)(32 * quarter) << 16);
-    const uint8_t *row = smem + PSH_AT_RAWK + slot * PG_HEAD_BYTES + (pos & (PG_POS - 1)) * KV_ROW;
+    const int lane = threadIdx.x & 31, quarter = (threadIdx.x >> 5) & 3, pos = 32 * quarter + lane;
+    const uint32_t lanes = tmem + PSH_COL_K + ((uint32_t)(32 * quarter) << 16);
     PshWait wait(S);
     PshReader frags{S, wait};
     PshFragment F;
-    int it = 0, n = 0;                                   // steps; pages of the slot
+    int it = 0, n = 0, chunk = 0, slot = 0;              // steps, pages; 64 dims: how many, and where in tensor memory
     while (frags.next(F)) {
+#pragma unroll 1
         for (int i = 0; i < F.steps && wait.ok; ++i, ++it) {
             const PshStep T = psh_step(F, i);
-            const bool mine = T.pages > slot;
-            if (it > 0) wait(&S.qkdone, (uint32_t)((it - 1) & 1));                // the planes have been read
-            tc_fence_after();
+            const bool mine = T.pages > quarter >> 1;
+            const int page = (n + (quarter >> 1)) % PSH_KSLOTS;
+            const uint8_t *row = smem + PSH_AT_RAWK + page * PG_HEAD_BYTES + (pos & (PG_POS - 1)) * KV_ROW;
+            uint32_t w[18], none = 0u;
+            float up = 1.0f;
             if (mine) {
-                wait(&S.rkfull[slot], (uint32_t)(n & 1));
-                ++n;
-                const bool there = (pos & (PG_POS - 1)) < S.held_k[slot];
+                wait(&S.rkfull[page], (uint32_t)(((n + (quarter >> 1)) / PSH_KSLOTS) & 1));
+                none = (pos & (PG_POS - 1)) < S.held_k[page] ? 0xFFFFFFFFu : 0u;
                 uint32_t top = 0;
 #pragma unroll
                 for (int b = 0; b < KV_NBLK; ++b) top = max(top, (uint32_t)*reinterpret_cast<const uint16_t *>(row + 34 * b) & 0x7FFFu);
-                const int s = there ? psh_shift(top) : 0;
-                const float up = atc_pow2(s);
-                S.kf[it & 1][pos] = atc_pow2(-s);
+                const int s = psh_shift(top & none);
+                up = atc_pow2(s);
+                S.ks[it & 3][pos] = (int8_t)s;
+            }
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c, ++chunk) {
+                if (mine) {                              // (words of an odd chunk begin in the middle of eight bytes: one that is there already, and eight pairs)
+                    const uint8_t *src = row + 136 * (c >> 1);
+                    if (c & 1) {
+                        w[0] = w[17];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {            // blocks 4 h ..: bytes 0 .. 143, 128 .. 271
-                    uint32_t w[36];
-#pragma unroll
-                    for (int j = 0; j < 9; ++j) {
-                        const uint4 x = *reinterpret_cast<const uint4 *>(row + 128 * h + 16 * j);
-                        w[4 * j] = x.x; w[4 * j + 1] = x.y; w[4 * j + 2] = x.z; w[4 * j + 3] = x.w;
-                    }
-#pragma unroll
-                    for (int b = 0; b < 4; ++b) {
-                        const int byte = 34 * (4 * h + b) - 128 * h, at = byte >> 2;              // of the block, in w
-                        const bool odd = byte & 2;
-                        const uint32_t d16 = odd ? w[at] >> 16 : w[at] & 0xFFFFu;
-                        const __half2 d = psh_scale(there ? d16 : 0u, up);
-                        uint32_t hi[16], lo[16];
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) {   // halfword 1 + e of the block
-                            const int half = (byte >> 1) + 1 + e;
-                            psh_planes(psh_pair(w[half >> 1] ^ 0x80808080u, half & 1), d, hi[e], lo[e]);
+                        for (int j = 0; j < 8; ++j) {
+                            const uint2 x = *reinterpret_cast<const uint2 *>(src + 72 + 8 * j);
+                            w[1 + 2 * j] = x.x;
+                            w[2 + 2 * j] = x.y;
                         }
-                        tc_st16(to + (uint32_t)(16 * (4 * h + b)), hi);
-                        tc_st16(to + (uint32_t)(128 + 16 * (4 * h + b)), lo);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 9; ++j) {
+                            const uint2 x = *reinterpret_cast<const uint2 *>(src + 8 * j);
+                            w[2 * j] = x.x;
+                            w[2 * j + 1] = x.y;
+                        }
                     }
                 }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&S.rkempty[slot]);
-                tc_st_wait();
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&S.kready);
-        }
-    }
-}
-
-// V rows to planes in shared memory, 32 positions a stage: a warp has two of the eight blocks, under one power of two each for a step.
-template <int W>
-__device__ __forceinline__ void psh_v_rows(const uint8_t *row, const float (&up)[2], bool there, uint8_t *dst, uint32_t lane) {
-    uint32_t w[20];
-#pragma unroll
-    for (int j = 0; j < 5; ++j) {
-        const uint4 x = *reinterpret_cast<const uint4 *>(row + 64 * W + 16 * j);
-        w[4 * j] = x.x; w[4 * j + 1] = x.y; w[4 * j + 2] = x.z; w[4 * j + 3] = x.w;
-    }
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-        const int byte = 4 * W + 34 * b;
-        const uint32_t d16 = b ? w[byte >> 2] >> 16 : w[byte >> 2] & 0xFFFFu;
-        const bool number = (d16 & 0x7FFFu) < 0x7C00u;
-        const __half2 d = psh_scale(there && number ? d16 : 0u, up[b]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int half = (byte >> 1) + 1 + 4 * j + e;
-                psh_planes(psh_pair(w[half >> 1] ^ 0x80808080u, half & 1), d, hi[e], lo[e]);
-            }
-            uint8_t *to = dst + (((uint32_t)(4 * b + j) ^ (lane & 7u)) << 4);
-            *reinterpret_cast<uint4 *>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            *reinterpret_cast<uint4 *>(to + PSH_V_PLANE) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        }
-    }
-}
-__device__ __forceinline__ void psh_v_warps(const PageShared &P, PshSmall &S, uint8_t *smem) {
-    const uint32_t lane = threadIdx.x & 31, quarter = (threadIdx.x >> 5) & 3;
-    PshWait wait(S);
-    PshReader frags{S, wait};
-    PshFragment F;
-    int it = 0, nv = 0, stage = 0;
-    while (frags.next(F)) {
-        for (int i = 0; i < F.steps && wait.ok; ++i, ++it) {
-            const PshStep T = psh_step(F, i);
-            const uint8_t *page[2] = {nullptr, nullptr};
-            int held[2] = {0, 0};
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                if (j >= T.pages) break;
-                const int slot = (nv + j) % PSH_VSLOTS;
-                wait(&S.rvfull[slot], (uint32_t)(((nv + j) / PSH_VSLOTS) & 1));
-                page[j] = smem + PSH_AT_RAWV + slot * PG_HEAD_BYTES;
-                held[j] = S.held_v[slot];
-            }
-            uint32_t top[2] = {0, 0};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {                // a lane's position of each stage
-                const int at = 32 * (j & 1) + (int)lane;
-                bool bad = false;
-                if (j < T.stages && at < held[j >> 1]) {
-#pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        const uint32_t mag = *reinterpret_cast<const uint16_t *>(page[j >> 1] + at * KV_ROW + 34 * (2 * quarter + b)) & 0x7FFFu;
-                        if (mag < 0x7C00u) top[b] = max(top[b], mag);
-                        else bad = true;
-                    }
+                if (chunk >= PSH_KRING) wait(&S.kempty[slot], (uint32_t)((chunk / PSH_KRING - 1) & 1));
+                tc_fence_after();
+                if (mine) {
+                    psh_k_chunk<0>(w, none, up, lanes + (uint32_t)(64 * slot));
+                    tc_st_wait();
                 }
-                const uint32_t mask = __ballot_sync(0xffffffffu, bad);
-                if (lane == 0) S.v_bad[it & 3][quarter][j] = mask;
-            }
-            float up[2];
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const int s = psh_shift(__reduce_max_sync(0xffffffffu, top[b]));
-                up[b] = atc_pow2(s);
-                if (lane == 0) S.vf[it & 3][2 * quarter + b] = atc_pow2(-s);
-            }
-            for (int j = 0; j < T.stages && wait.ok; ++j, ++stage) {
-                if (stage >= PSH_STAGES) wait(&S.vempty[stage % PSH_STAGES], (uint32_t)((stage / PSH_STAGES - 1) & 1));
-                const int at = 32 * (j & 1) + (int)lane;
-                const uint8_t *row = (j >> 1 ? page[1] : page[0]) + at * KV_ROW;
-                const bool there = at < (j >> 1 ? held[1] : held[0]);
-                uint8_t *dst = smem + PSH_AT_V + (stage % PSH_STAGES) * PSH_V_STAGE + quarter * (PSH_STAGE * 128) + lane * 128;
-                if (quarter == 0) psh_v_rows<0>(row, up, there, dst, lane);
-                else if (quarter == 1) psh_v_rows<1>(row, up, there, dst, lane);
-                else if (quarter == 2) psh_v_rows<2>(row, up, there, dst, lane);
-                else psh_v_rows<3>(row, up, there, dst, lane);
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                tc_fence_before();
                 __syncwarp();
                 if (lane == 0) {
-                    mbar_arrive(&S.vready[stage % PSH_STAGES]);
-                    if ((j & 1) || j == T.stages - 1) mbar_arrive(&S.rvempty[(nv + (j >> 1)) % PSH_VSLOTS]);
+                    mbar_arrive(&S.kready[slot]);
+                    if (mine && c == 3) mbar_arrive(&S.rkempty[page]);
                 }
+                slot = slot == PSH_KRING - 1 ? 0 : slot + 1;
             }
-            nv += T.pages;
+            n += T.pages;
         }
     }
 }
 
-__device__ __forceinline__ void psh_mma_warp(const PageShared &P, PshSmall &S, uint8_t *smem, uint32_t tmem) {
-    constexpr uint32_t MAJOR_MN = (1u << 15) | (1u << 16);
+// V to planes in tensor memory, 32 positions at a time: a dim a thread, a block of 32 dims a warp, so that a position has one scale.
+__device__ __forceinline__ void psh_v_warps(const PageShared &P, PshSmall &S, uint8_t *smem, uint32_t tmem) {
+    const int lane = threadIdx.x & 31, block = (threadIdx.x >> 5) - PSH_V_WARP;
+    const uint32_t lanes = tmem + PSH_COL_V + (uint32_t)(32 * (block >> 2)) + ((uint32_t)(32 * (block & 3)) << 16);
+    // the dim's byte in a row: which word, which of its bytes (of two rows' words)
+    const int byte = 34 * block + 2 + lane;
+    const uint32_t pick2 = (uint32_t)(byte & 3) | ((uint32_t)(byte & 3) + 4u) << 8;        // byte 0 and byte 2 of the result
     PshWait wait(S);
     PshReader frags{S, wait};
     PshFragment F;
-    int it = 0, stage = 0, frag = 0;
-    const uint32_t q0 = tc16_desc_lo(smem_u32(smem));
-    const uint32_t v0 = ((smem_u32(smem + PSH_AT_V) >> 4) & 0x3FFFu) | ((uint32_t)(PSH_STAGE * 128 >> 4) << 16);
-    const uint32_t p0 = ((smem_u32(smem + PSH_AT_P) >> 4) & 0x3FFFu) | ((uint32_t)(PSH_P_GROUP >> 4) << 16);
+    uint16_t *const scales = reinterpret_cast<uint16_t *>(smem + PSH_AT_D) + block * PSH_STEP;
+    int it = 0, nv = 0, stage = 0;
     while (frags.next(F)) {
-        const int n = (F.n_rows + 15) / 16 * 16;
-        const uint32_t idesc = atc_idesc(n);
-        for (int i = 0; i <= F.steps && wait.ok; ++i) {
-            if (i < F.steps) {                           // scores of step i
-                if (i == 0) wait(&S.qready, (uint32_t)(frag & 1));
-                wait(&S.kready, (uint32_t)(it & 1));
-                if (it > 0) wait(&S.sempty, (uint32_t)((it - 1) & 1));
-                tc_fence_after();
-                if (elect_one()) {
-                    const uint32_t k = tmem + PSH_COL_K, d = tmem + PSH_COL_S;
-                    auto at = [](int c) { return (uint32_t)((c >> 2) * (PSH_Q_CHUNK >> 4) + 2 * (c & 3)); };
-                    tc_mma_f16_ts<false>(d, k + 128u, q0, idesc);
+#pragma unroll 1
+        for (int i = 0; i < F.steps && wait.ok; ++i, ++it) {
+            const PshStep T = psh_step(F, i);
+            // the block's scales of the step, under one power of two; a lane has a position of each stage
+            const int slot0 = nv % PSH_VSLOTS, slot1 = slot0 == PSH_VSLOTS - 1 ? 0 : slot0 + 1;
+            wait(&S.rvfull[slot0], (uint32_t)((nv / PSH_VSLOTS) & 1));
+            if (T.pages > 1) wait(&S.rvfull[slot1], (uint32_t)(((nv + 1) / PSH_VSLOTS) & 1));
+            {
+                const int held0 = S.held_v[slot0], held1 = T.pages > 1 ? S.held_v[slot1] : 0;
+                const uint8_t *own = smem + PSH_AT_RAWV + lane * KV_ROW + 34 * block;
+                uint32_t d[4], top = 0;
 #pragma unroll
-                    for (int c = 1; c < 16; ++c) tc_mma_f16_ts<true>(d, k + 128u + (uint32_t)(8 * c), q0 + at(c), idesc);
-#pragma unroll
-                    for (int c = 0; c < 16; ++c) tc_mma_f16_ts<true>(d, k + (uint32_t)(8 * c), q0 + (uint32_t)(PSH_Q_PLANE >> 4) + at(c), idesc);
-#pragma unroll
-                    for (int c = 0; c < 16; ++c) tc_mma_f16_ts<true>(d, k + (uint32_t)(8 * c), q0 + at(c), idesc);
-                    tc_commit(&S.qkdone);
+                for (int j = 0; j < 4; ++j) {
+                    d[j] = *reinterpret_cast<const uint16_t *>(own + (j >> 1 ? slot1 : slot0) * PG_HEAD_BYTES + 32 * (j & 1) * KV_ROW);
+                    if (32 * (j & 1) + lane >= (j >> 1 ? held1 : held0)) d[j] = 0;
+                    top = max(top, d[j] & 0x7FFFu);
                 }
+                const bool odd = __any_sync(0xffffffffu, top >= 0x7C00u);
+                if (odd) {                               // scales that are no numbers
+                    top = 0;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const bool bad = (d[j] & 0x7FFFu) >= 0x7C00u;
+                        const uint32_t mask = __ballot_sync(0xffffffffu, bad);
+                        if (lane == 0) S.v_bad[it & 7][j][block] = mask;
+                        if (bad) d[j] = 0;
+                        top = max(top, d[j] & 0x7FFFu);
+                    }
+                }
+                const int s = psh_shift(__reduce_max_sync(0xffffffffu, top));
+                if (lane == 0) {
+                    S.vf[it & 7][block] = atc_pow2(-s);
+                    S.v_odd[it & 7][block] = odd;
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) scales[32 * j + lane] = (uint16_t)psh_scale(d[j], atc_pow2(s));
                 __syncwarp();
             }
-            if (i > 0) {                                 // outputs of step i - 1, whose number is pv
-                const int pv = it - 1;
-                const PshStep T = psh_step(F, i - 1);
-                wait(&S.pready, (uint32_t)(pv & 1));
-                for (int j = 0; j < T.stages; ++j, ++stage) {
-                    wait(&S.vready[stage % PSH_STAGES], (uint32_t)((stage / PSH_STAGES) & 1));
-                    tc_fence_after();
-                    if (elect_one()) {
-                        const uint32_t va = v0 + (uint32_t)((stage % PSH_STAGES) * (PSH_V_STAGE >> 4)), pb = p0 + (uint32_t)(j * (PSH_STAGE / 8) * (PSH_P_GROUP >> 4));
+            const uint8_t *src = smem + PSH_AT_RAWV + slot0 * PG_HEAD_BYTES + (byte & ~3);
+            const uint4 *ds = reinterpret_cast<const uint4 *>(scales);
+#pragma unroll 1
+            for (int j = 0; j < T.stages && wait.ok; ++j, ++stage) {
+                const int at = stage & (PSH_VRING - 1);
+                const uint32_t to = lanes + (uint32_t)(64 * at);
+                if (j == 2) src += (slot1 - slot0) * PG_HEAD_BYTES - 64 * KV_ROW;
+                if (stage >= PSH_VRING) wait(&S.vempty[at], (uint32_t)((stage / PSH_VRING - 1) & 1));
+                tc_fence_after();
 #pragma unroll
-                        for (int m = 0; m < 2; ++m) {
-                            const uint32_t d = tmem + PSH_COL_O + (uint32_t)((pv & 1) * PSH_O_BUF + m * PSH_ROWS);
-                            const uint32_t a = va + (uint32_t)(m * (2 * PSH_STAGE * 128 >> 4));
+                for (int k = 0; k < 2; ++k) {            // 16 positions
+                    uint32_t hi[8], lo[8];
 #pragma unroll
-                            for (int pr = 0; pr < 3; ++pr)               // low V, low weights, both high
+                    for (int h = 0; h < 2; ++h) {
+                        const uint4 d4 = ds[2 * k + h];
+                        const uint32_t d[4] = {d4.x, d4.y, d4.z, d4.w};
 #pragma unroll
-                                for (int c = 0; c < 2; ++c)
-                                    psh_mma_ss(d, a + (uint32_t)((pr == 0 ? PSH_V_PLANE : 0) >> 4) + (uint32_t)(c * (2048 >> 4)),
-                                               pb + (uint32_t)((pr == 1 ? PSH_P_PLANE : 0) >> 4) + (uint32_t)(2 * c * (PSH_P_GROUP >> 4)), idesc | MAJOR_MN, j + pr + c > 0);
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t *x = reinterpret_cast<const uint32_t *>(src + (16 * k + 8 * h + 2 * e) * KV_ROW);
+                            const uint32_t both = __byte_perm(x[0], x[KV_ROW / 4], pick2);
+                            uint32_t c;
+                            asm("lop3.b32 %0, %1, 0x00FF00FF, 0x64806480, 0x6A;" : "=r"(c) : "r"(both));           // (both & mask) ^ 1024 + 128
+                            asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(c) : "r"(0x64806480u));
+                            psh_planes(c, d[e], hi[4 * h + e], lo[4 * h + e]);
                         }
-                        tc_commit(&S.vempty[stage % PSH_STAGES]);
-                        if (j == T.stages - 1) tc_commit(&S.pvdone);
                     }
-                    __syncwarp();
+                    tc_st8(to + (uint32_t)(8 * k), hi);
+                    tc_st8(to + (uint32_t)(16 + 8 * k), lo);
                 }
+                tc_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&S.vready[at]);
+                    if ((j & 1) || j == T.stages - 1) mbar_arrive(&S.rvempty[j >> 1 ? slot1 : slot0]);
+                }
+                src += 32 * KV_ROW;
+                ds += 4;
             }
-            if (i < F.steps) ++it;
+            nv += T.pages;
+            __syncwarp();                                // (the scales have been read)
+        }
+    }
+}
+
+__device__ __forceinline__ void psh_score_warp(const PageShared &P, PshSmall &S, uint8_t *smem, uint32_t tmem) {
+    PshWait wait(S);
+    PshReader frags{S, wait};
+    PshFragment F;
+    int it = 0, frag = 0, chunk = 0, slot = 0;
+    const uint32_t q0 = tc16_desc_lo(smem_u32(smem));
+    while (frags.next(F)) {
+        const uint32_t idesc = atc_idesc((F.n_rows + 15) / 16 * 16);
+        wait(&S.qready, (uint32_t)(frag & 1));
+#pragma unroll 1
+        for (int i = 0; i < F.steps && wait.ok; ++i, ++it) {
+            if (it > 0) wait(&S.sempty, (uint32_t)((it - 1) & 1));
+            const uint32_t d = tmem + PSH_COL_S;
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c, ++chunk) {       // 64 dims: low K, low queries, both high
+                wait(&S.kready[slot], (uint32_t)((chunk / PSH_KRING) & 1));
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint32_t a = tmem + PSH_COL_K + (uint32_t)(64 * slot), b = q0 + (uint32_t)(c * (PSH_Q_CHUNK >> 4));
+                    if (c == 0) tc_mma_f16_ts<false>(d, a + 32u, b, idesc);
+                    else tc_mma_f16_ts<true>(d, a + 32u, b, idesc);
+#pragma unroll
+                    for (int k = 1; k < 4; ++k) tc_mma_f16_ts<true>(d, a + 32u + (uint32_t)(8 * k), b + (uint32_t)(2 * k), idesc);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) tc_mma_f16_ts<true>(d, a + (uint32_t)(8 * k), b + (uint32_t)(PSH_Q_PLANE >> 4) + (uint32_t)(2 * k), idesc);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) tc_mma_f16_ts<true>(d, a + (uint32_t)(8 * k), b + (uint32_t)(2 * k), idesc);
+                    tc_commit(&S.kempty[slot]);
+                    if (c == 3) tc_commit(&S.qkdone);
+                }
+                __syncwarp();
+                slot = slot == PSH_KRING - 1 ? 0 : slot + 1;
+            }
         }
         ++frag;
     }
-    if (elect_one()) tc_commit(&S.done);                 // everything that was issued
+    if (elect_one()) tc_commit(&S.done[0]);              // everything that was issued
     __syncwarp();
-    mbar_wait_try(&S.done, 0);
+    psh_wait(&S.done[0], 0);
+}
+__device__ __forceinline__ void psh_out_warp(const PageShared &P, PshSmall &S, uint8_t *smem, uint32_t tmem) {
+    PshWait wait(S);
+    PshReader frags{S, wait};
+    PshFragment F;
+    int it = 0, stage = 0;
+    const uint32_t p0 = ((smem_u32(smem + PSH_AT_P) >> 4) & 0x3FFFu) | ((uint32_t)(PSH_P_GROUP >> 4) << 16);
+    while (frags.next(F)) {
+        const uint32_t idesc = atc_idesc((F.n_rows + 15) / 16 * 16) | (1u << 16);        // (weights: rows side by side)
+#pragma unroll 1
+        for (int i = 0; i < F.steps && wait.ok; ++i, ++it) {
+            const PshStep T = psh_step(F, i);
+            wait(&S.pready[it & 1], (uint32_t)((it >> 1) & 1));
+            if (it > 1) wait(&S.oempty[it & 1], (uint32_t)(((it - 2) >> 1) & 1));
+#pragma unroll 1
+            for (int j = 0; j < T.stages; ++j, ++stage) {
+                wait(&S.vready[stage % PSH_VRING], (uint32_t)((stage / PSH_VRING) & 1));
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint32_t v = tmem + PSH_COL_V + (uint32_t)(64 * (stage % PSH_VRING)), o = tmem + PSH_COL_O + (uint32_t)((it & 1) * PSH_O_BUF);
+                    const uint32_t b = p0 + (uint32_t)((it & 1) * (PSH_P_BUF >> 4) + j * (PSH_STAGE / 8) * (PSH_P_GROUP >> 4));
+                    constexpr uint32_t LOW = PSH_P_PLANE >> 4, K16 = 2 * PSH_P_GROUP >> 4;
+#pragma unroll
+                    for (int m = 0; m < 2; ++m) {        // low V, low weights, both high
+                        const uint32_t a = v + (uint32_t)(32 * m), d = o + (uint32_t)(m * PSH_ROWS);
+                        if (j == 0) psh_mma_weights<false>(d, a + 16u, b, idesc);
+                        else psh_mma_weights<true>(d, a + 16u, b, idesc);
+                        psh_mma_weights<true>(d, a + 24u, b + K16, idesc);
+                        psh_mma_weights<true>(d, a, b + LOW, idesc);
+                        psh_mma_weights<true>(d, a + 8u, b + LOW + K16, idesc);
+                        psh_mma_weights<true>(d, a, b, idesc);
+                        psh_mma_weights<true>(d, a + 8u, b + K16, idesc);
+                    }
+                    tc_commit(&S.vempty[stage % PSH_VRING]);
+                    if (j == T.stages - 1) tc_commit(&S.pvdone[it & 1]);
+                }
+                __syncwarp();
+            }
+        }
+    }
+    if (elect_one()) tc_commit(&S.done[1]);              // everything that was issued
+    __syncwarp();
+    psh_wait(&S.done[1], 0);
 }
 
+// A fragment's queries, quantised as the cache rows are, to planes: a row a warp.  They come by the place of the weights, which nobody reads now.
+__device__ __forceinline__ void psh_queries(const PageShared &P, PshSmall &S, uint8_t *smem, const PshFragment &F, int n) {
+    constexpr float LOG2E = 1.44269504088896340736f;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint8_t *box = smem + PSH_AT_P + 32 * lane;
+#pragma unroll 1
+    for (int r = warp; r < F.n_rows; r += PSH_SUM_WARPS) {
+        const int row = F.row0 + r, tok = row / P.group;
+        const float *src = P.q + ((size_t)(F.begin + tok) * P.n_head + F.kvh * P.group + (row - tok * P.group)) * KV_D + 8 * lane;
+        const uint32_t dst = smem_u32(box + r * (KV_D * 4));
+        if ((reinterpret_cast<uintptr_t>(P.q) & 15u) == 0) {
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + 16u), "l"(src + 4) : "memory");
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + 4u * e), "l"(src + e) : "memory");
+        }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");     // (a lane reads what it has copied itself)
+#pragma unroll 1
+    for (int r = warp; r < n; r += PSH_SUM_WARPS) {
+        float x[8];
+        const float4 a = *reinterpret_cast<const float4 *>(box + r * (KV_D * 4)), b = *reinterpret_cast<const float4 *>(box + r * (KV_D * 4) + 16);
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+        const float d = __fmul_rn(kv_amax_8(x), PG_SCALE), id = d > 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
+        const uint32_t d16 = r < F.n_rows ? f32_to_f16_bits_ties_away(d) : 0u;           // (rows behind the last: zeros)
+        const int s = psh_shift(__reduce_max_sync(0xffffffffu, d16));
+        const uint32_t sc = psh_scale(d16, atc_pow2(s));
+        uint32_t w[2], hi[4], lo[4];
+        kv_words_8(x, id, w);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) psh_planes(psh_pair(w[j >> 1] ^ 0x80808080u, j & 1), sc, hi[j], lo[j]);
+        uint8_t *dst = smem + (lane >> 3) * PSH_Q_CHUNK + r * 128 + (((lane & 7) ^ (r & 7)) << 4);
+        *reinterpret_cast<uint4 *>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4 *>(dst + PSH_Q_PLANE) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        if (lane == 0) {
+            S.qf[r] = __fmul_rn(__fmul_rn(__fmul_rn(P.scale, LOG2E), PSH_LIFT), atc_pow2(-s));
+            S.limit[r] = F.before == INT32_MAX ? F.end - 1 : F.before + (F.row0 + min(r, F.n_rows - 1)) / P.group;
+            S.less[r] = 1e30f;
+            S.none[r] = 0;
+        }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    psh_barrier<256>(3);                                 // every row's numbers
+    if (lane == 0) mbar_arrive(&S.qready);
+}
+
+// Sums over a warp of eight values: of value 4 b4 + 2 b3 + b2 at lanes with these bits.
+__device__ __forceinline__ float psh_sum8(const float2 (&v)[4], int lane) {
+    float x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float a = k & 1 ? v[k >> 1].y : v[k >> 1].x, b = k & 1 ? v[2 + (k >> 1)].y : v[2 + (k >> 1)].x;
+        x[k] = __fadd_rn(lane & 16 ? b : a, __shfl_xor_sync(0xffffffffu, lane & 16 ? a : b, 16));
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) x[k] = __fadd_rn(lane & 8 ? x[k + 2] : x[k], __shfl_xor_sync(0xffffffffu, lane & 8 ? x[k] : x[k + 2], 8));
+    x[0] = __fadd_rn(lane & 4 ? x[1] : x[0], __shfl_xor_sync(0xffffffffu, lane & 4 ? x[0] : x[1], 4));
+    x[0] = __fadd_rn(x[0], __shfl_xor_sync(0xffffffffu, x[0], 2));
+    return __fadd_rn(x[0], __shfl_xor_sync(0xffffffffu, x[0], 1));
+}
 __device__ __forceinline__ void psh_sum_warps(const PageShared &P, PshSmall &S, uint8_t *smem, uint32_t tmem) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quarter = warp & 3, half = warp >> 2, pos = 32 * quarter + lane;
     const uint32_t tlane = tmem + ((uint32_t)(32 * quarter) << 16);
-    constexpr float LOG2E = 1.44269504088896340736f;
     constexpr float BASE = 7.0f, MOST = 15.0f;           // a weight is 2^7 at its row's reference and 2^15 at most
     PshWait wait(S);
     PshReader frags{S, wait};
@@ -675,221 +803,192 @@ __device__ __forceinline__ void psh_sum_warps(const PageShared &P, PshSmall &S, 
     int it = 0;
     while (true) {
         // (the eight warps go on, and leave, together: they meet at barriers)
-        const bool more = frags.next(F);
-        uint32_t all;
-        asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, 3, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(all) : "r"(more ? 1u : 0u) : "memory");
-        if (!all) break;
-        // ---- queries, quantised as the cache rows are, to planes
+        if (psh_any<256>(3, !frags.next(F))) break;
         const int n = (F.n_rows + 15) / 16 * 16;
-        {
-            const bool vec = (reinterpret_cast<uintptr_t>(P.q) & 15u) == 0;
-            float x[PSH_ROWS / PSH_SUM_WARPS][8];
-#pragma unroll
-            for (int e = 0; e < PSH_ROWS / PSH_SUM_WARPS; ++e) {
-                const int r = warp + PSH_SUM_WARPS * e;
-                if (r >= n) break;
-                const int row = F.row0 + min(r, F.n_rows - 1), tok = row / P.group;
-                const float *src = P.q + ((size_t)(F.begin + tok) * P.n_head + F.kvh * P.group + (row - tok * P.group)) * KV_D + 8 * lane;
-                if (vec) {
-                    const float4 a = *reinterpret_cast<const float4 *>(src), b = *reinterpret_cast<const float4 *>(src + 4);
-                    x[e][0] = a.x; x[e][1] = a.y; x[e][2] = a.z; x[e][3] = a.w; x[e][4] = b.x; x[e][5] = b.y; x[e][6] = b.z; x[e][7] = b.w;
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) x[e][j] = src[j];
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < PSH_ROWS / PSH_SUM_WARPS; ++e) {
-                const int r = warp + PSH_SUM_WARPS * e;
-                if (r >= n) break;
-                const float d = __fmul_rn(kv_amax_8(x[e]), PG_SCALE), id = d > 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
-                const uint32_t d16 = r < F.n_rows ? f32_to_f16_bits_ties_away(d) : 0u;
-                const int s = psh_shift(__reduce_max_sync(0xffffffffu, d16));
-                const __half2 sc = psh_scale(d16, atc_pow2(s));
-                uint32_t hi[4], lo[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int a = max(-127, min(127, round_ties_away(__fmul_rn(x[e][2 * j], id)))), b = max(-127, min(127, round_ties_away(__fmul_rn(x[e][2 * j + 1], id))));
-                    psh_planes(__halves2half2(__int2half_rn(a), __int2half_rn(b)), sc, hi[j], lo[j]);
-                }
-                uint8_t *dst = smem + (lane >> 3) * PSH_Q_CHUNK + r * 128 + (((lane & 7) ^ (r & 7)) << 4);
-                *reinterpret_cast<uint4 *>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                *reinterpret_cast<uint4 *>(dst + PSH_Q_PLANE) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                if (lane == 0) {
-                    S.qf[r] = __fmul_rn(__fmul_rn(P.scale, LOG2E), atc_pow2(-s));
-                    S.limit[r] = r >= F.n_rows ? -1 : F.before == INT32_MAX ? F.end - 1 : F.before + (F.row0 + r) / P.group;
-                    S.ref[r] = -1e30f;
-                }
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            asm volatile("bar.sync 3, 256;" ::: "memory");               // every row's numbers
-            if (lane == 0) mbar_arrive(&S.qready);
-        }
+        psh_queries(P, S, smem, F, n);
         const int all_see = F.before == INT32_MAX ? F.end - 1 : F.before + F.row0 / P.group;
         const int groups = (n - 8 * half + 15) / 16;     // of eight columns: 16 c + 8 half ..
-        float acc[2][3][8], l[3][8];
+        float2 acc[2][3][4], l[3][4];
 #pragma unroll
         for (int c = 0; c < 3; ++c)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) acc[0][c][e] = acc[1][c][e] = l[c][e] = 0.0f;
-        bool changed = false;
-        const int first = it;
-        auto drain = [&](int i) {                        // outputs of step i
-            const uint32_t from = tlane + PSH_COL_O + (uint32_t)((i & 1) * PSH_O_BUF + 8 * half);
+            for (int e = 0; e < 4; ++e) acc[0][c][e] = acc[1][c][e] = l[c][e] = make_float2(0.0f, 0.0f);
+        bool dead = false;
+#pragma unroll 1
+        for (int i = 0; i <= F.steps; ++i, ++it) {
+            const int p0 = F.pos0 + i * PSH_STEP;
+            bool changed = false;
+            if (i < F.steps) {
+                const bool hidden = p0 + PSH_STEP - 1 > all_see;         // some row does not see some position
+                wait(&S.qkdone, (uint32_t)(it & 1));
+                tc_fence_after();
+                const float kf = atc_pow2(-(int)S.ks[it & 3][pos]);
+                float s[3][8];                           // scores in powers of two, less the rows' references
+#pragma unroll 1
+                for (int turn = 0; turn < 2; ++turn) {
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                const float f = S.vf[i & 3][4 * m + quarter];
-#pragma unroll
-                for (int c = 0; c < 3; ++c) {
-                    if (c >= groups) break;
-                    int o[8];
-                    tc_ld8(from + (uint32_t)(m * PSH_ROWS + 16 * c), o);
+                    for (int c = 0; c < 3; ++c)
+                        if (c < groups) tc_ld8(tlane + PSH_COL_S + (uint32_t)(16 * c + 8 * half), reinterpret_cast<int (&)[8]>(s[c]));
                     tc_ld_wait();
+                    float most = wait.ok ? -INFINITY : INFINITY;
+#pragma unroll
+                    for (int c = 0; c < 3; ++c)
+                        if (c < groups) {
+                            float f[8], r[8];
+                            psh_lds8(S.qf + 16 * c + 8 * half, f);
+                            psh_lds8(S.less + 16 * c + 8 * half, r);
+#pragma unroll
+                            for (int e = 0; e < 8; e += 2) {
+                                const float2 y = fma2(mul2(make_float2(s[c][e], s[c][e + 1]), make_float2(kf, kf)), make_float2(f[e], f[e + 1]), make_float2(r[e], r[e + 1]));
+                                s[c][e] = y.x;
+                                s[c][e + 1] = y.y;
+                            }
+                            if (hidden) {
+                                int limit[8];
+                                psh_lds8(S.limit + 16 * c + 8 * half, limit);
+#pragma unroll
+                                for (int e = 0; e < 8; ++e)
+                                    if (p0 + pos > limit[e]) s[c][e] = -INFINITY;
+                            }
+#pragma unroll
+                            for (int e = 0; e < 8; e += 2) most = fmaxf(most, fmaxf(s[c][e], s[c][e + 1]));
+                        }
+                    if (turn || !psh_any<128>(1 + half, most > MOST)) break;
+                    // a row's first step, then where its scores grow by much: the references move
+                    dead = psh_any<128>(1 + half, !wait.ok);
+                    if (dead) break;
+#pragma unroll 1
+                    for (int c = 0; c < groups; ++c) {
+                        int x[8];
+                        tc_ld8(tlane + PSH_COL_S + (uint32_t)(16 * c + 8 * half), x);
+                        tc_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const int col = 16 * c + 8 * half + e;
+                            float y = __fmul_rn(__fmul_rn(__int_as_float(x[e]), kf), S.qf[col]);
+                            if (p0 + pos > S.limit[col]) y = -INFINITY;
+                            const float m = psh_from_key(__reduce_max_sync(0xffffffffu, psh_key(y)));
+                            if (lane == 0) S.red[quarter][col] = m;
+                        }
+                    }
+                    psh_barrier<128>(1 + half);
+                    if (quarter == 0 && lane < 8 * groups) {
+                        const int col = 16 * (lane >> 3) + 8 * half + (lane & 7);
+                        const float was = -S.less[col];
+                        float m = S.red[0][col];
+#pragma unroll
+                        for (int w = 1; w < 4; ++w) m = S.red[w][col] > m || S.red[w][col] != S.red[w][col] ? S.red[w][col] : m;
+                        m = __fsub_rn(m, BASE);
+                        const float now = m > was || m != m ? m : was;
+                        S.less[col] = -now;
+                        S.change[col] = psh_exp2(__fsub_rn(was, now));
+                    }
+                    psh_barrier<128>(1 + half);
+                    changed = i > 0;
+#pragma unroll
+                    for (int c = 0; c < 3; ++c)
+                        if (c < groups) {
+                            float f[8];
+                            psh_lds8(S.change + 16 * c + 8 * half, f);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const float2 g = make_float2(f[2 * e], f[2 * e + 1]);
+                                l[c][e] = mul2(l[c][e], g);
+                                acc[0][c][e] = mul2(acc[0][c][e], g);
+                                acc[1][c][e] = mul2(acc[1][c][e], g);
+                            }
+                        }
+                }
+                if (dead) break;
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&S.sempty);
+                uint8_t *dst = smem + PSH_AT_P + (it & 1) * PSH_P_BUF + (pos >> 3) * PSH_P_GROUP + half * 128 + (pos & 7) * 16;
+#pragma unroll
+                for (int c = 0; c < 3; ++c)
+                    if (c < groups) {
+                        uint32_t hi[4], lo[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float2 a = make_float2(psh_exp2(s[c][2 * e]), psh_exp2(s[c][2 * e + 1]));
+                            l[c][e] = add2(l[c][e], a);
+                            const __half2 h = __floats2half2_rn(a.x, a.y);
+                            const float2 rest = fma2(__half22float2(h), make_float2(-1.0f, -1.0f), a);       // exact
+                            const __half2 r = __floats2half2_rn(rest.x, rest.y);
+                            hi[e] = *reinterpret_cast<const uint32_t *>(&h);
+                            lo[e] = *reinterpret_cast<const uint32_t *>(&r);
+                        }
+                        *reinterpret_cast<uint4 *>(dst + 256 * c) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        *reinterpret_cast<uint4 *>(dst + 256 * c + PSH_P_PLANE) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&S.pready[it & 1]);
+            }
+            if (i == 0) continue;
+            // ---- outputs of the step before
+            const int o = it - 1;
+            wait(&S.pvdone[o & 1], (uint32_t)((o >> 1) & 1));
+            tc_fence_after();
+            const uint32_t from = tlane + PSH_COL_O + (uint32_t)((o & 1) * PSH_O_BUF + 8 * half);
+            const float *vf = S.vf[o & 7] + quarter;
+            const float f0 = *(volatile const float *)vf, f1 = *(volatile const float *)(vf + 4);
+#pragma unroll
+            for (int c = 0; c < 3; ++c) {
+                if (c >= groups) break;
+                int x[2][8];
+                tc_ld8(from + (uint32_t)(16 * c), x[0]);
+                tc_ld8(from + (uint32_t)(PSH_ROWS + 16 * c), x[1]);
+                tc_ld_wait();
+                if (changed) {
+                    float g[8];
+                    psh_lds8(S.change + 16 * c + 8 * half, g);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        const float g = changed ? __fmul_rn(f, S.change[16 * c + 8 * half + e]) : f;
-                        acc[m][c][e] = __fmaf_rn(__int_as_float(o[e]), g, acc[m][c][e]);
+                        x[0][e] = __float_as_int(__fmul_rn(__int_as_float(x[0][e]), g[e]));
+                        x[1][e] = __float_as_int(__fmul_rn(__int_as_float(x[1][e]), g[e]));
                     }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    acc[0][c][e] = fma2(make_float2(__int_as_float(x[0][2 * e]), __int_as_float(x[0][2 * e + 1])), make_float2(f0, f0), acc[0][c][e]);
+                    acc[1][c][e] = fma2(make_float2(__int_as_float(x[1][2 * e]), __int_as_float(x[1][2 * e + 1])), make_float2(f1, f1), acc[1][c][e]);
                 }
             }
             tc_fence_before();
-        };
-        // rows that see a position whose V is no number are no numbers
-        auto poison = [&](int i, int p0) {
-            const uint32_t (*bad)[4] = S.v_bad[i & 3];
-            if ((bad[0][quarter] | bad[1][quarter] | bad[2][quarter] | bad[3][quarter]) >> lane & 1u)
-#pragma unroll
-                for (int c = 0; c < 3; ++c)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (c < groups && p0 + pos <= S.limit[16 * c + 8 * half + e]) l[c][e] = __int_as_float(0x7FC00000);
-        };
-        for (int i = 0; i < F.steps; ++i, ++it) {
-            const int p0 = F.pos0 + i * PSH_STEP;
-            wait(&S.qkdone, (uint32_t)(it & 1));
-            tc_fence_after();
-            float s[3][8];
-            {
-                int x[3][8];
-#pragma unroll
-                for (int c = 0; c < 3; ++c)
-                    if (c < groups) tc_ld8(tlane + PSH_COL_S + (uint32_t)(16 * c + 8 * half), x[c]);
-                tc_ld_wait();
-                const float kf = S.kf[it & 1][pos];
-#pragma unroll
-                for (int c = 0; c < 3; ++c)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) s[c][e] = c < groups ? __fmul_rn(__int_as_float(x[c][e]), __fmul_rn(kf, S.qf[16 * c + 8 * half + e])) : 0.0f;
-            }
-            tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&S.sempty);
-            if (p0 + PSH_STEP - 1 > all_see) {           // some row does not see some position
-#pragma unroll
-                for (int c = 0; c < 3; ++c)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (c < groups && p0 + pos > S.limit[16 * c + 8 * half + e]) s[c][e] = -INFINITY;
+            if (lane == 0) mbar_arrive(&S.oempty[o & 1]);
+            // rows that see a position whose V is no number are no numbers
+            if (*reinterpret_cast<const volatile unsigned long long *>(S.v_odd[o & 7])) {
+                bool bad = false;
+#pragma unroll 1
+                for (int b = 0; b < KV_NBLK; ++b) bad = bad || (S.v_odd[o & 7][b] && (S.v_bad[o & 7][quarter][b] >> lane & 1u));
+#pragma unroll 1
+                for (int r = 0; bad && r < F.n_rows; ++r)
+                    if (p0 - PSH_STEP + pos <= S.limit[r]) S.none[r] = 1;
             }
-            bool above = !wait.ok;
-#pragma unroll
-            for (int c = 0; c < 3; ++c)
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (c < groups) above = above || s[c][e] > __fadd_rn(S.ref[16 * c + 8 * half + e], MOST);
-            if (psh_half_any(half, above)) {             // (a row's first step, then where its scores grow by much: the references move)
-                if (psh_half_any(half, !wait.ok)) break;
-#pragma unroll
-                for (int c = 0; c < 3; ++c)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (c < groups) {
-                            const float m = psh_from_key(__reduce_max_sync(0xffffffffu, psh_key(s[c][e])));
-                            if (lane == 0) S.red[quarter][16 * c + 8 * half + e] = m;
-                        }
-                psh_half_barrier(half);
-                if (quarter == 0 && lane < 8 * groups) {
-                    const int col = 16 * (lane >> 3) + 8 * half + (lane & 7);
-                    const float was = S.ref[col];
-                    float m = S.red[0][col];
-#pragma unroll
-                    for (int w = 1; w < 4; ++w) m = S.red[w][col] > m || S.red[w][col] != S.red[w][col] ? S.red[w][col] : m;
-                    m = __fsub_rn(m, BASE);
-                    const float now = m > was || m != m ? m : was;
-                    S.ref[col] = now;
-                    S.change[col] = psh_exp2(__fsub_rn(was, now));
-                }
-                psh_half_barrier(half);
-                changed = it > first;
-#pragma unroll
-                for (int c = 0; c < 3; ++c)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (c < groups) {
-                            const float f = S.change[16 * c + 8 * half + e];
-                            l[c][e] = __fmul_rn(l[c][e], f);
-                            acc[0][c][e] = __fmul_rn(acc[0][c][e], f);
-                            acc[1][c][e] = __fmul_rn(acc[1][c][e], f);
-                        }
-            }
-            uint32_t hi[3][4], lo[3][4];
-#pragma unroll
-            for (int c = 0; c < 3; ++c)
-#pragma unroll
-                for (int e = 0; e < 8; e += 2)
-                    if (c < groups) {
-                        const float a = psh_exp2(__fsub_rn(s[c][e], S.ref[16 * c + 8 * half + e])), b = psh_exp2(__fsub_rn(s[c][e + 1], S.ref[16 * c + 8 * half + e + 1]));
-                        l[c][e] = __fadd_rn(l[c][e], a);
-                        l[c][e + 1] = __fadd_rn(l[c][e + 1], b);
-                        split_f16x2(a, b, hi[c][e >> 1], lo[c][e >> 1]);
-                    }
-            if (it > first) {
-                wait(&S.pvdone, (uint32_t)((it - 1) & 1));               // the weights before have been read
-                tc_fence_after();
-            }
-            uint8_t *dst = smem + PSH_AT_P + (pos >> 3) * PSH_P_GROUP + half * 128 + (pos & 7) * 16;
-#pragma unroll
-            for (int c = 0; c < 3; ++c)
-                if (c < groups) {
-                    *reinterpret_cast<uint4 *>(dst + 256 * c) = make_uint4(hi[c][0], hi[c][1], hi[c][2], hi[c][3]);
-                    *reinterpret_cast<uint4 *>(dst + 256 * c + PSH_P_PLANE) = make_uint4(lo[c][0], lo[c][1], lo[c][2], lo[c][3]);
-                }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&S.pready);
-            if (it > first) {
-                drain(it - 1);
-                poison(it - 1, p0 - PSH_STEP);
-            }
-            changed = false;
         }
-        wait(&S.pvdone, (uint32_t)((it - 1) & 1));
-        tc_fence_after();
-        drain(it - 1);
-        poison(it - 1, F.pos0 + (F.steps - 1) * PSH_STEP);
+        --it;                                            // (the last turn had outputs only)
         // ---- the fragment's sums
         const bool good = *(volatile int *)&S.failed == 0;
+        float *dst = P.part + (F.part + 8 * half) * KV_D + pos;
 #pragma unroll
         for (int c = 0; c < 3; ++c)
+            if (c < groups) {
+                const float x = psh_sum8(l[c], lane);
+                if ((lane & 3) == 0) S.red[quarter][16 * c + 8 * half + (lane >> 2 & 1) + (lane >> 2 & 2) + (lane >> 2 & 4)] = x;
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (c < groups) {
-                    float x = l[c][e];
-#pragma unroll
-                    for (int o = 1; o < 32; o <<= 1) x = __fadd_rn(x, __shfl_xor_sync(0xffffffffu, x, o));
-                    const int col = 16 * c + 8 * half + e;
-                    if (lane == 0) S.red[quarter][col] = x;
-                    if (col < F.n_rows && good) {
-                        float *dst = P.part + (F.part + col) * KV_D + pos;
-                        dst[0] = acc[0][c][e];
-                        dst[128] = acc[1][c][e];
+                for (int e = 0; e < 8; ++e)
+                    if (16 * c + 8 * half + e < F.n_rows && good) {
+                        dst[(16 * c + e) * KV_D] = e & 1 ? acc[0][c][e >> 1].y : acc[0][c][e >> 1].x;
+                        dst[(16 * c + e) * KV_D + 128] = e & 1 ? acc[1][c][e >> 1].y : acc[1][c][e >> 1].x;
                     }
-                }
-        psh_half_barrier(half);
+            }
+        psh_barrier<256>(3);                             // (rows that have seen no number are said by both halves)
         if (quarter == 0 && lane < 8 * groups) {
             const int col = 16 * (lane >> 3) + 8 * half + (lane & 7);
             if (col < F.n_rows && good)
-                P.part_ml[F.part + col] = make_float2(S.ref[col], __fadd_rn(__fadd_rn(S.red[0][col], S.red[1][col]), __fadd_rn(S.red[2][col], S.red[3][col])));
+                P.part_ml[F.part + col] = make_float2(-S.less[col], S.none[col] ? __int_as_float(0x7FC00000) : __fadd_rn(__fadd_rn(S.red[0][col], S.red[1][col]), __fadd_rn(S.red[2][col], S.red[3][col])));
         }
     }
 }
@@ -900,47 +999,48 @@ __global__ void __launch_bounds__(PSH_THREADS, 1) pages_shared_kernel(const __gr
     PshSmall &S = *reinterpret_cast<PshSmall *>(smem + PSH_AT_SMALL);
     const int warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < PSH_DESCS; ++i) mbar_init(&S.dfull[i], 1), mbar_init(&S.dempty[i], PSH_SUM_WARPS + 10);
-        for (int i = 0; i < 2; ++i) mbar_init(&S.rkfull[i], 1), mbar_init(&S.rkempty[i], 2);
-        for (int i = 0; i < PSH_VSLOTS; ++i) mbar_init(&S.rvfull[i], 1), mbar_init(&S.rvempty[i], 4);
-        for (int i = 0; i < PSH_STAGES; ++i) mbar_init(&S.vready[i], 4), mbar_init(&S.vempty[i], 1);
+        for (int i = 0; i < PSH_DESCS; ++i) mbar_init(&S.dfull[i], 1), mbar_init(&S.dempty[i], PSH_THREADS / 32 - 1);
+        for (int i = 0; i < PSH_KSLOTS; ++i) mbar_init(&S.rkfull[i], 1), mbar_init(&S.rkempty[i], 2);
+        for (int i = 0; i < PSH_VSLOTS; ++i) mbar_init(&S.rvfull[i], 1), mbar_init(&S.rvempty[i], 8);
+        for (int i = 0; i < PSH_KRING; ++i) mbar_init(&S.kready[i], 4), mbar_init(&S.kempty[i], 1);
+        for (int i = 0; i < PSH_VRING; ++i) mbar_init(&S.vready[i], 8), mbar_init(&S.vempty[i], 1);
+        for (int i = 0; i < 2; ++i) mbar_init(&S.pready[i], PSH_SUM_WARPS), mbar_init(&S.pvdone[i], 1), mbar_init(&S.oempty[i], PSH_SUM_WARPS);
         mbar_init(&S.qready, PSH_SUM_WARPS);
-        mbar_init(&S.kready, 4);
         mbar_init(&S.qkdone, 1);
         mbar_init(&S.sempty, PSH_SUM_WARPS);
-        mbar_init(&S.pready, PSH_SUM_WARPS);
-        mbar_init(&S.pvdone, 1);
-        mbar_init(&S.done, 1);
+        mbar_init(&S.done[0], 1);
+        mbar_init(&S.done[1], 1);
         mbar_fence_init();
         S.failed = 0;
     }
-    pdl_wait_prior_grid();
+    pdl_wait_prior_grid();                               // (the plan)
     pdl_launch_dependents();
-    if (warp == PSH_MMA_WARP) {
+    if (warp == PSH_OUT_WARP) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&S.tmem)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    const long long per = psh_divide(P, S);              // (and its barriers: the ones above are there)
+    __syncthreads();
     tc_fence_after();
     const uint32_t tmem = S.tmem;
     if (warp < PSH_SUM_WARPS) {
         psh_set_registers<PSH_REGS_SUM>(true);
         psh_sum_warps(P, S, smem, tmem);
-    } else if (warp < PSH_V_WARP) {
-        psh_set_registers<PSH_REGS_PLANES>(false);
-        psh_k_warps(P, S, smem, tmem);
+    } else if (warp < PSH_K_WARP) {
+        psh_set_registers<PSH_REGS_V>(false);
+        psh_v_warps(P, S, smem, tmem);
     } else if (warp < PSH_PLAN_WARP) {
-        psh_set_registers<PSH_REGS_PLANES>(false);
-        psh_v_warps(P, S, smem);
+        psh_set_registers<PSH_REGS_K>(false);
+        psh_k_warps(P, S, smem, tmem);
     } else {
         psh_set_registers<PSH_REGS_REST>(false);
-        if (warp == PSH_PLAN_WARP) psh_plan_warp(P, S, per);
-        else if (warp == PSH_LOAD_WARP) psh_load_warp(P, S, smem);
-        else if (warp == PSH_MMA_WARP) psh_mma_warp(P, S, smem, tmem);
+        if (warp == PSH_PLAN_WARP) psh_plan_warp(P, S, smem);
+        else if (warp == PSH_LOAD_WARP) psh_load_k_warp(P, S, smem);
+        else if (warp == PSH_SCORE_WARP) psh_score_warp(P, S, smem, tmem);
+        else psh_out_warp(P, S, smem, tmem);
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == PSH_MMA_WARP) {
+    if (warp == PSH_OUT_WARP) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     }
@@ -958,35 +1058,31 @@ __global__ void __launch_bounds__(32 * PSJ_WARPS) pages_shared_join_kernel(const
     const int tok = (int)(row / P.n_head), h = (int)(row - (int64_t)tok * P.n_head), kvh = h / P.group;
     const int s = seq_of_row(C.start, C.n_seq, tok, lane);
     if (s >= C.n_seq) return;                            // nobody's
-    const PshWork own = psh_sequence(P, s);
+    const PshPlan &plan = *P.plan;
+    const PshEntity own = plan.entity[P.n_groups + s];
     if (own.steps < 0 || tok < own.begin || tok >= own.begin + own.tokens) return;
-    const long long per = P.plan[0].unit;
     const float *acc[2] = {nullptr, nullptr};
     const float2 *ml[2] = {nullptr, nullptr};
-    int n[2] = {0, 0};
+    int n[2] = {0, 0}, gap[2] = {0, 0};                  // a row's parts, and how far apart they are
     bool served = true;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {                        // its own positions; what it shares
-        PshWork W = own;
-        int e = P.n_groups + s;
-        if (i == 1) {
-            if (own.page0 == 0) break;
-            e = psh_group_of(P, s);
-            W = psh_work(P, e);
-        }
-        if (W.steps <= 0) continue;
-        const PshPlan plan = P.plan[1 + e];
-        if (plan.unit < 0) {
+        if (i == 1 && own.page0 == 0) break;
+        const PshEntity E = i ? plan.entity[own.group] : own;
+        if (E.steps <= 0) continue;
+        if (E.unit < 0) {
             served = false;
             break;
         }
-        const long long at = (long long)(tok - W.begin) * P.group + (h - kvh * P.group), tile = at / PSH_ROWS;
-        const long long begin = plan.unit + (tile * heads + kvh) * (W.steps + PSH_START) + PSH_START;
-        const int steps = psh_tile_steps(W, psh_tile_end(P, W, tile * PSH_ROWS));
+        const bool many = E.image >= 0;
+        const int size = many ? PST_ROWS : PSH_ROWS, start = many ? PST_START : PSH_START;
+        const int at = (tok - E.begin) * P.group + (h - kvh * P.group), tile = at / size, row0 = tile * size, end = psh_tile_end(P.group, E, row0, size);
+        const int steps = many ? (end + PG_POS - 1) / PG_POS - E.page0 : psh_steps(end - E.page0 * PG_POS);
         if (steps <= 0) continue;
+        const long long per = many ? plan.tc_per : plan.per, begin = E.unit + (long long)(tile * heads + kvh) * (E.steps + start) + start;
         const long long c0 = begin / per, c1 = (begin + steps - 1) / per;
-        const long long tile_rows = min((long long)PSH_ROWS, (long long)W.tokens * P.group - tile * PSH_ROWS);
-        const long long first = plan.row + tile * PSH_ROWS * heads + kvh * tile_rows + c0 * PSH_ROWS + (at - tile * PSH_ROWS);
+        const long long first = (many ? plan.tc_row : 0) + E.row + (long long)row0 * heads + kvh * min(size, E.tokens * P.group - row0) + c0 * size + (at - row0);
+        gap[i] = size;
         n[i] = (int)(c1 - c0 + 1);
         acc[i] = P.part + first * KV_D;
         ml[i] = P.part_ml + first;
@@ -994,7 +1090,7 @@ __global__ void __launch_bounds__(32 * PSJ_WARPS) pages_shared_join_kernel(const
     if (!served) return;
     const int all = n[0] + n[1];
     float m = -INFINITY, l = 0.0f;
-    for (int i = lane; i < all; i += 32) m = fmaxf(m, i < n[0] ? ml[0][(size_t)i * PSH_ROWS].x : ml[1][(size_t)(i - n[0]) * PSH_ROWS].x);
+    for (int i = lane; i < all; i += 32) m = fmaxf(m, i < n[0] ? ml[0][(size_t)i * gap[0]].x : ml[1][(size_t)(i - n[0]) * gap[1]].x);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
@@ -1004,8 +1100,9 @@ __global__ void __launch_bounds__(32 * PSJ_WARPS) pages_shared_join_kernel(const
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int i = min(i0 + e, all - 1);
-            const float2 *pml = i < n[0] ? ml[0] + (size_t)i * PSH_ROWS : ml[1] + (size_t)(i - n[0]) * PSH_ROWS;
-            const float4 *src = reinterpret_cast<const float4 *>(i < n[0] ? acc[0] + (size_t)i * PSH_ROWS * KV_D : acc[1] + (size_t)(i - n[0]) * PSH_ROWS * KV_D) + lane;
+            const size_t step = i < n[0] ? (size_t)i * gap[0] : (size_t)(i - n[0]) * gap[1];
+            const float2 *pml = (i < n[0] ? ml[0] : ml[1]) + step;
+            const float4 *src = reinterpret_cast<const float4 *>((i < n[0] ? acc[0] : acc[1]) + step * KV_D) + lane;
             x[e] = *pml;
             c[e] = src[0];
             d[e] = src[32];

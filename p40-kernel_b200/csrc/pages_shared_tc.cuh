@@ -1,0 +1,441 @@
+// pages_shared_tc.cuh -- pages_shared.cuh's attention for entities of many rows (a long prompt's questions, hundreds of answers): 128 rows a tile, rows as the rows of both products.
+//
+// pages_shared_kernel turns the cache's codes into planes for 48 rows at a time; with that many rows the planes are worth writing down.  pages_shared_planes_kernel writes each page of
+// these entities once, as a tile image (attn_tc.cuh's: planes split, swizzled, v transposed), and pages_shared_tc_kernel multiplies as pages_tc_kernel does: 512 threads, each a row and a
+// quarter of its columns, form weights and add outputs; a warp issues the products, of which the next page's scores and this page's outputs are in flight together; two warps copy
+// images.  Tensor memory: 256 outputs, 64 scores, 64 weights, 128 q low; shared memory: q high, k and v of one page.
+#pragma once
+
+#include "pages_shared.cuh"
+
+namespace b200 {
+
+constexpr uint32_t PST_COL_O = 0, PST_COL_S = 256, PST_COL_P = 320, PST_COL_QL = 384;
+constexpr int PST_THREADS = ATC_THREADS + 96;
+constexpr int PST_SMEM_BYTES = 1024 + 3 * ATC_PLANES + (2 * ATC_KEYS + 2 * ATT_D + 2 * 4 * ATC_M) * 4 + 160;
+constexpr int PST_IMG_BAD = ATC_IMG_RANGE + 16;                  // 8 bytes of an image: positions whose v is no number
+static_assert(PST_IMG_BAD + 8 <= ATC_IMG_BYTES && PST_ROWS == ATC_M && PG_POS == ATC_KEYS && KV_D == ATT_D, "");
+__device__ __forceinline__ void pst_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(ATC_THREADS) : "memory"); }        // among the threads that have rows
+
+// Images of the pages of the entities of many rows: image E.image + i is page page0 + i, [kv head] beside each other.  z 0 = k (warp = eight positions, lane = eight dims), z 1 = v
+// (thread = one dim, all 64 positions).
+__global__ void __launch_bounds__(ATC_PREP_THREADS) pages_shared_planes_kernel(const __grid_constant__ PageShared P) {
+    __shared__ __align__(16) uint8_t rows[PG_HEAD_BYTES];
+    __shared__ uint32_t odd[2];
+    const PageCache &C = P.C;
+    const PshPlan &plan = *P.plan;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, entities = P.n_groups + C.n_seq;
+    pdl_wait_prior_grid();
+    pdl_launch_dependents();
+    const int images = plan.images;
+    int e = 0;
+#pragma unroll 1
+    for (int item = blockIdx.x; item < images * C.n_head_kv; item += gridDim.x) {
+        const int image = item / C.n_head_kv, kvh = item - image * C.n_head_kv;
+        // whose: the last entity whose images begin at or in front of it
+        for (int at = -1; at < 0; e += 32) {
+            const bool mine = e + lane < entities && plan.entity[e + lane].image >= 0 && plan.entity[e + lane].image <= image &&
+                              image < plan.entity[e + lane].image + (plan.entity[e + lane].end + PG_POS - 1) / PG_POS - plan.entity[e + lane].page0;
+            const unsigned found = __ballot_sync(0xffffffffu, mine);
+            if (found || e >= entities) {
+                at = found ? e + __ffs(found) - 1 : entities;
+                e = min(at, entities) - 32;              // (the loop adds them again)
+            }
+        }
+        if (e >= entities) return;
+        const PshEntity E = plan.entity[e];
+        const int page_at = E.page0 + image - E.image, n = min(PG_POS, E.end - page_at * PG_POS);
+        const int page = E.seq >= 0 ? C.table[(size_t)E.seq * C.table_stride + page_at] : -1;
+        const bool there = page >= 0 && page < C.n_pages;
+        if (!there && threadIdx.x == 0) bad_sequence();
+        {
+            const uint4 *src = reinterpret_cast<const uint4 *>(page_rows(C, there ? page : 0, P.layer, blockIdx.z, kvh));
+            const int words = there ? n * (KV_ROW / 16) : 0;
+            for (int i = threadIdx.x; i < PG_HEAD_BYTES / 16; i += ATC_PREP_THREADS) reinterpret_cast<uint4 *>(rows)[i] = i < words ? src[i] : make_uint4(0u, 0u, 0u, 0u);
+        }
+        if (threadIdx.x < 2) odd[threadIdx.x] = 0;
+        __syncthreads();
+        uint8_t *img = P.images + (size_t)item * ATC_IMG_BYTES;
+        if (blockIdx.z == 0) {
+            constexpr int ROWS = ATC_KEYS / (ATC_PREP_THREADS / 32);
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                const int key = ROWS * warp + r;
+                const uint16_t *b = reinterpret_cast<const uint16_t *>(rows + key * KV_ROW + 34 * (lane >> 2));
+                const float d = f16_bits_to_f32(b[0]);
+                float x[8];
+                uint32_t m = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t w = b[1 + 4 * (lane & 3) + i];
+                    x[2 * i] = __fmul_rn((float)(int8_t)(w & 0xFFu), d);
+                    x[2 * i + 1] = __fmul_rn((float)(int8_t)(w >> 8), d);
+                    m = max(m, max(atc_abs_bits(x[2 * i]), atc_abs_bits(x[2 * i + 1])));
+                }
+                const int s = atc_shift(min(__reduce_max_sync(0xffffffffu, m), 0x7F7FFFFFu), 63);
+                uint4 hi, lo;
+                atc_split8(x, atc_pow2(s), hi, lo);
+                uint8_t *dst = img + (lane >> 3) * ATC_CHUNK + key * 128 + (((lane & 7) ^ (key & 7)) * 16);
+                *reinterpret_cast<uint4 *>(dst) = hi;
+                *reinterpret_cast<uint4 *>(dst + ATC_KEYS * 128) = lo;
+                if (lane == 0) reinterpret_cast<float *>(img + ATC_IMG_KF)[key] = atc_pow2(-s);
+            }
+        } else {
+            const int d = threadIdx.x;
+            float x[ATC_KEYS];
+            const uint8_t *b = rows + 34 * (d >> 5);
+            uint32_t seen = 0;
+#pragma unroll
+            for (int i = 0; i < ATC_KEYS; ++i) {
+                float sc = f16_bits_to_f32(*reinterpret_cast<const uint16_t *>(b + i * KV_ROW));
+                if (!isfinite(sc)) {                     // (its rows are told apart by who has weights for them)
+                    sc = 0.0f;
+                    if ((d & 31) == 0) atomicOr(&odd[i >> 5], 1u << (i & 31));
+                }
+                x[i] = __fmul_rn((float)(int8_t)b[i * KV_ROW + 2 + (d & 31)], sc);
+                seen = max(seen, atc_abs_bits(x[i]));
+            }
+            const int s = atc_shift(seen, 112);
+            reinterpret_cast<float *>(img + ATC_IMG_VF)[d] = atc_pow2(-s - 14);          // (and the weights' 2^-14)
+#pragma unroll
+            for (int g = 0; g < ATC_KEYS / 8; ++g) {
+                uint4 hi, lo;
+                atc_split8(x + 8 * g, atc_pow2(s), hi, lo);
+                uint8_t *dst = img + ATC_PLANES + d * 128 + ((g ^ (d & 7)) * 16);
+                *reinterpret_cast<uint4 *>(dst) = hi;
+                *reinterpret_cast<uint4 *>(dst + 2 * ATC_CHUNK) = lo;
+            }
+            __syncthreads();
+            if (d < 2) reinterpret_cast<uint32_t *>(img + PST_IMG_BAD)[d] = odd[d];
+        }
+        __syncthreads();                                 // the next item's rows take the place of these
+    }
+}
+
+__global__ void __launch_bounds__(PST_THREADS, 1) pages_shared_tc_kernel(const __grid_constant__ PageShared P) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    uint8_t *qhi = smem + ((1024u - (smem_u32(smem) & 1023u)) & 1023u);
+    uint8_t *kpl = qhi + ATC_PLANES, *vpl = kpl + ATC_PLANES;
+    float *kf = reinterpret_cast<float *>(vpl + ATC_PLANES);             // [2][64] 2^-s of the page's positions, pages alternate
+    float *vf = kf + 2 * ATC_KEYS;                                       // [2][256] 2^-s of the dims (and the weights' 2^-14)
+    float *red0 = vf + 2 * ATT_D;                                        // [2][4][128] exchange between the four warps of a row, pages alternate
+    uint64_t *qk = reinterpret_cast<uint64_t *>(red0 + 2 * 4 * ATC_M), *pv = qk + 1, *scored = qk + 2, *weighed = qk + 3, *kfull = qk + 4, *vfull = qk + 6;
+    unsigned long long *bad = reinterpret_cast<unsigned long long *>(vfull + 2);         // [2] positions of the page whose v is no number
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bad + 2);
+    volatile int *failed = reinterpret_cast<int *>(tmem_slot + 1);
+
+    const PageCache &C = P.C;
+    const PshPlan &plan = *P.plan;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, heads = C.n_head_kv, entities = P.n_groups + C.n_seq;
+    const int cg = warp >> 2, row = 32 * (warp & 3) + lane;              // a thread's row, and its quarter of the row's columns
+    const bool driver = warp >= ATC_WARPS;
+    if (threadIdx.x == 0) {
+        for (int b = 0; b < 8; ++b) mbar_init(qk + b, b == 2 || b == 3 ? ATC_WARPS : 1);
+        mbar_fence_init();
+        *failed = 0;
+    }
+    pdl_wait_prior_grid();                                               // the plan and the images
+    pdl_launch_dependents();
+    const long long per = plan.tc_per, last = min(per * (blockIdx.x + 1), plan.tc_total);
+    long long at = per * blockIdx.x;
+    if (at >= last) return;                                              // CTA-uniform
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    __syncthreads();                                                     // the barriers, and where tensor memory is
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const uint32_t tlane = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+    const size_t img_stride = (size_t)heads * ATC_IMG_BYTES;
+    int it0 = 0;                                                         // pages of the fragments before
+    bool ok = true;
+    auto issue_qk = [&] {
+        tc_fence_after();
+        constexpr uint32_t LOW = (ATC_KEYS * 128) >> 4;
+        const uint32_t a0 = tc16_desc_lo(smem_u32(qhi)), b0 = tc16_desc_lo(smem_u32(kpl)), ql = tmem + PST_COL_QL, d = tmem + PST_COL_S;
+        auto off = [](int n) { return (uint32_t)((n >> 2) * (ATC_CHUNK >> 4) + 2 * (n & 3)); };
+        if (elect_one()) {                                               // products with a low plane first: the accumulator is small while they are added
+            tc_mma_f16_ts<false>(d, ql, b0, atc_idesc(ATC_KEYS));
+#pragma unroll
+            for (int n = 1; n < 16; ++n) tc_mma_f16_ts<true>(d, ql + (uint32_t)(8 * n), b0 + off(n), atc_idesc(ATC_KEYS));
+#pragma unroll
+            for (int n = 0; n < 16; ++n) atc_mma_ss<atc_idesc(ATC_KEYS)>(d, a0 + off(n), b0 + LOW + off(n));
+#pragma unroll
+            for (int n = 0; n < 16; ++n) atc_mma_ss<atc_idesc(ATC_KEYS)>(d, a0 + off(n), b0 + off(n));
+            tc_commit(qk);
+        }
+        __syncwarp();
+    };
+    auto issue_pv = [&] {
+        tc_fence_after();
+        const uint32_t b0 = tc16_desc_lo(smem_u32(vpl)), ph = tmem + PST_COL_P, pl = ph + 32u;
+        if (elect_one()) {
+#pragma unroll
+            for (int n = 0; n < 12; ++n) {
+                const uint32_t a = (n < 4 ? pl : ph) + (uint32_t)(8 * (n & 3));
+                const uint32_t b = b0 + (uint32_t)((n >= 4 && n < 8 ? (2 * ATC_CHUNK) >> 4 : 0) + 2 * (n & 3));
+                if (n == 0) tc_mma_f16_ts<false>(tmem + PST_COL_O, a, b, atc_idesc(ATT_D));
+                else tc_mma_f16_ts<true>(tmem + PST_COL_O, a, b, atc_idesc(ATT_D));
+            }
+            tc_commit(pv);
+        }
+        __syncwarp();
+    };
+#pragma unroll 1
+    for (int e = plan.tc_first[blockIdx.x]; e < entities && at < last && ok; ++e) {
+        const PshEntity E = plan.entity[e];
+        if (E.unit < 0 || E.image < 0) continue;
+        const int size = E.steps + PST_START, all_rows = E.tokens * P.group, pairs = (all_rows + PST_ROWS - 1) / PST_ROWS * heads;
+        int pair = (int)((at - E.unit) / size);
+#pragma unroll 1
+        for (long long begin = E.unit + (long long)pair * size; pair < pairs && begin < last && ok; ++pair, begin += size) {
+            const int tile = pair / heads, kvh = pair - tile * heads, row0 = tile * PST_ROWS, n_rows = min(PST_ROWS, all_rows - row0);
+            const int end = psh_tile_end(P.group, E, row0, PST_ROWS);
+            const int page0 = (int)max(0ll, at - begin - PST_START);
+            const int ntiles = min((int)min(last - begin, (long long)size) - PST_START, (end + PG_POS - 1) / PG_POS - E.page0) - page0;
+            at = begin + size;
+            if (ntiles <= 0) continue;
+            const bool whole = E.before == INT32_MAX;
+            const int all_see = whole ? end - 1 : E.before + row0 / P.group;
+            const int limit = whole ? end - 1 : row < n_rows ? E.before + (row0 + row) / P.group : -1;       // the last position that the thread's row sees
+            const uint8_t *img = P.images + ((size_t)(E.image + page0) * heads + kvh) * ATC_IMG_BYTES;
+            const size_t part = (size_t)(plan.tc_row + E.row + (long long)row0 * heads + (long long)kvh * n_rows + (long long)blockIdx.x * PST_ROWS);
+            auto row_at = [&](int r) {                                   // where a row of the tile lies in q
+                const int x = row0 + r, tok = x / P.group;
+                return ((size_t)(E.begin + tok) * P.n_head + kvh * P.group + (x - tok * P.group)) * KV_D;
+            };
+            if (driver) {
+                __syncthreads();                                         // q is in its places
+                auto wait = [&](uint64_t *bar, uint32_t parity) { ok = ok && __all_sync(0xffffffffu, psh_wait(bar, parity)); };
+                if (warp == ATC_WARPS) {
+#pragma unroll 1
+                    for (int i = 0; i <= ntiles; ++i) {                  // scores of page i, outputs of page i - 1
+                        const int it = it0 + i;
+                        if (i < ntiles) {
+                            if (it > 0) wait(scored, (uint32_t)((it - 1) & 1));
+                            wait(kfull + (it & 1), (uint32_t)((it >> 1) & 1));
+                            issue_qk();
+                        }
+                        if (i > 0) {
+                            wait(weighed, (uint32_t)((it - 1) & 1));
+                            wait(vfull + ((it - 1) & 1), (uint32_t)(((it - 1) >> 1) & 1));
+                            issue_pv();
+                        }
+                    }
+                } else {
+                    const bool v = warp == ATC_WARPS + 2;
+#pragma unroll 1
+                    for (int i = 0; i < ntiles; ++i) {                   // k when the scores of the page before have been read, v when its outputs are there
+                        const int it = it0 + i;
+                        if (it > 0) wait(v ? pv : scored, (uint32_t)((it - 1) & 1));
+                        if (lane == 0) {
+                            const uint64_t pol = policy_evict_last_or_default();
+                            const uint8_t *src = img + (size_t)i * img_stride;
+                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");         // the factors were read by ordinary loads
+                            if (v) {
+                                bad[it & 1] = *reinterpret_cast<const unsigned long long *>(src + PST_IMG_BAD);
+                                mbar_expect_tx(vfull + (it & 1), ATC_PLANES + ATT_D * 4);
+                                bulk_g2s(vf + (it & 1) * ATT_D, src + ATC_IMG_VF, ATT_D * 4, vfull + (it & 1), pol);
+                                bulk_g2s(vpl, src + ATC_PLANES, ATC_PLANES, vfull + (it & 1), pol);
+                            } else {
+                                mbar_expect_tx(kfull + (it & 1), ATC_PLANES + ATC_KEYS * 4);
+                                bulk_g2s(kf + (it & 1) * ATC_KEYS, src + ATC_IMG_KF, ATC_KEYS * 4, kfull + (it & 1), pol);
+                                bulk_g2s(kpl, src, ATC_PLANES, kfull + (it & 1), pol);
+                            }
+                        }
+                        __syncwarp();
+                    }
+                }
+                if (!ok) *failed = 1;
+                __syncthreads();
+                ok = *failed == 0;
+                __syncthreads();
+                it0 += ntiles;
+                continue;
+            }
+            // ---- q: row of the thread, 64 dims, quantised to Q8_0 (two blocks); high plane to shared memory, low plane to tensor memory, through shared memory (the planes' of k and
+            // v, a warp's 32 rows of 64 values each, 16-byte pieces swizzled)
+            float4 *box = reinterpret_cast<float4 *>(kpl) + warp * 512;
+            const int box0 = 32 * (warp & 3);
+            float qf = 0.0f;
+            {
+                float x[64];
+                if ((reinterpret_cast<uintptr_t>(P.q) & 15u) == 0) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int r = 2 * i + (lane >> 4), c = lane & 15;
+                        if (box0 + r < n_rows) cp_async16(box + r * 16 + (c ^ (r & 15)), P.q + row_at(box0 + r) + 64 * cg + 4 * c);
+                    }
+                    cp_async_commit();
+                    cp_async_wait<0>();
+                    __syncwarp();
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) {
+                        const float4 a = row < n_rows ? box[lane * 16 + (c ^ (lane & 15))] : make_float4(0.f, 0.f, 0.f, 0.f);
+                        x[4 * c] = a.x; x[4 * c + 1] = a.y; x[4 * c + 2] = a.z; x[4 * c + 3] = a.w;
+                    }
+                } else {
+                    const float *src = P.q + (row < n_rows ? row_at(row) : 0) + 64 * cg;
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) x[i] = row < n_rows ? src[i] : 0.0f;
+                }
+                uint32_t m = 0;
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    float amax = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) amax = fmaxf(amax, fabsf(x[32 * b + i]));
+                    const float d = __fmul_rn(amax, PG_SCALE), id = d > 0.0f ? __fdiv_rn(1.0f, d) : 0.0f, d16 = f16_bits_to_f32(f32_to_f16_bits_ties_away(d));
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        x[32 * b + i] = __fmul_rn((float)max(-127, min(127, round_ties_away(__fmul_rn(x[32 * b + i], id)))), d16);
+                        m = max(m, atc_abs_bits(x[32 * b + i]));
+                    }
+                }
+                uint32_t *redu = reinterpret_cast<uint32_t *>(red0);
+                redu[cg * ATC_M + row] = m;
+                pst_barrier();
+#pragma unroll
+                for (int c = 0; c < 4; ++c) m = max(m, redu[c * ATC_M + row]);
+                const int s = atc_shift(min(m, 0x7F7FFFFFu), 63);
+                qf = __fmul_rn(atc_pow2(-s), P.scale);
+                uint32_t lo32[32];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    uint4 hi, lo;
+                    atc_split8(x + 8 * j, atc_pow2(s), hi, lo);
+                    *reinterpret_cast<uint4 *>(qhi + cg * ATC_CHUNK + row * 128 + ((j ^ (row & 7)) * 16)) = hi;
+                    lo32[4 * j] = lo.x; lo32[4 * j + 1] = lo.y; lo32[4 * j + 2] = lo.z; lo32[4 * j + 3] = lo.w;
+                }
+                tc_st32(tlane + PST_COL_QL + (uint32_t)(32 * cg), lo32);
+                tc_st_wait();
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");        // q high: written here, read by the tensor core
+            tc_fence_before();
+            __syncthreads();                                            // (and the box has been read: k and v take its place)
+            float acc[64];                                              // row, dims 64 cg ..
+#pragma unroll
+            for (int i = 0; i < 64; ++i) acc[i] = 0.0f;
+            float m_run = -INFINITY, l_run = 0.0f, alpha = 0.0f;        // l_run: of the thread's 16 columns of every page
+            auto add_page = [&](int par) {
+#pragma unroll
+                for (int h = 0; h < 8; ++h) {
+                    int o[8];
+                    tc_ld8(tlane + PST_COL_O + (uint32_t)(64 * cg + 8 * h), o);
+                    tc_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 8; i += 4) {
+                        const float4 f = *reinterpret_cast<const float4 *>(vf + par * ATT_D + 64 * cg + 8 * h + i);
+                        float *a = acc + 8 * h + i;
+                        a[0] = __fmaf_rn(__int_as_float(o[i]), f.x, __fmul_rn(a[0], alpha));
+                        a[1] = __fmaf_rn(__int_as_float(o[i + 1]), f.y, __fmul_rn(a[1], alpha));
+                        a[2] = __fmaf_rn(__int_as_float(o[i + 2]), f.z, __fmul_rn(a[2], alpha));
+                        a[3] = __fmaf_rn(__int_as_float(o[i + 3]), f.w, __fmul_rn(a[3], alpha));
+                    }
+                }
+            };
+            // rows that see a position whose v is no number are no numbers
+            auto poison = [&](int par, int p0) {
+                const unsigned long long who = bad[par];
+                if (who && (limit - p0 >= 63 ? true : limit >= p0 && (who & ((2ull << (limit - p0)) - 1)))) l_run = __int_as_float(0x7FC00000);
+            };
+#pragma unroll 1
+            for (int i = 0; i <= ntiles; ++i) {
+                const int it = it0 + i, p0 = (E.page0 + page0 + i) * PG_POS;
+                const uint32_t par = (uint32_t)(it & 1);
+                uint32_t hi[8], lo[8];
+                float alpha_new = 0.0f;
+                if (i < ntiles) {
+                    float *red = red0 + par * 4 * ATC_M;
+                    float s[16], mx = -INFINITY;
+                    ok = ok && mbar_wait_both(kfull + par, (uint32_t)((it >> 1) & 1), qk, par);       // (the first is long complete; it makes the copied factors visible)
+                    tc_fence_after();
+                    {
+                        int a[16];
+                        tc_ld16(tlane + PST_COL_S + (uint32_t)(16 * cg), a);
+                        tc_ld_wait();
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) s[j] = __fmul_rn(__int_as_float(a[j]), __fmul_rn(qf, kf[par * ATC_KEYS + 16 * cg + j]));
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(scored);
+                    if (p0 + PG_POS - 1 > all_see) {                    // some row does not see some position (one behind the last is behind every row's)
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            if (p0 + 16 * cg + j > limit) s[j] = -INFINITY;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[j]);
+                    red[cg * ATC_M + row] = mx;
+                    pst_barrier();
+                    float m_new = m_run;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) m_new = fmaxf(m_new, red[c * ATC_M + row]);
+                    const float base = m_new == -INFINITY ? 0.0f : m_new;
+                    alpha_new = expf(__fsub_rn(m_run, base));
+                    m_run = m_new;
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 16; j += 2) {
+                        const float x = expf(__fsub_rn(s[j], base)), y = expf(__fsub_rn(s[j + 1], base));
+                        sum = __fadd_rn(sum, __fadd_rn(x, y));
+                        split_f16x2(__fmul_rn(x, 16384.0f), __fmul_rn(y, 16384.0f), hi[j >> 1], lo[j >> 1]);
+                    }
+                    l_run = __fadd_rn(__fmul_rn(l_run, alpha_new), sum);
+                }
+                if (i > 0) {                                            // the outputs of the page before; its weights have been read
+                    const uint32_t was = par ^ 1u;
+                    ok = ok && mbar_wait_both(vfull + was, (uint32_t)(((it - 1) >> 1) & 1), pv, was);
+                    tc_fence_after();
+                }
+                if (i < ntiles) {
+                    tc_st8(tlane + PST_COL_P + (uint32_t)(8 * cg), hi);
+                    tc_st8(tlane + PST_COL_P + (uint32_t)(32 + 8 * cg), lo);
+                }
+                if (i > 0) {
+                    add_page((int)par ^ 1);
+                    poison((int)par ^ 1, p0 - PG_POS);
+                }
+                alpha = alpha_new;
+                tc_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0 && i < ntiles) mbar_arrive(weighed);
+            }
+            it0 += ntiles;
+            if (!ok) *failed = 1;
+            tc_fence_before();
+            __syncthreads();
+            ok = *failed == 0;
+            float *red = red0;
+            red[cg * ATC_M + row] = l_run;
+            pst_barrier();
+            if (ok) {
+                if (cg == 0 && row < n_rows) {
+                    const float l = __fadd_rn(__fadd_rn(red[row], red[ATC_M + row]), __fadd_rn(red[2 * ATC_M + row], red[3 * ATC_M + row]));
+                    P.part_ml[part + row] = make_float2(__fmul_rn(m_run, 1.44269504088896340736f), l);
+                }
+                float *dst = P.part + part * KV_D;
+#pragma unroll
+                for (int c = 0; c < 16; ++c) box[lane * 16 + (c ^ (lane & 15))] = make_float4(acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]);
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int x = 2 * i + (lane >> 4), c = lane & 15;
+                    if (box0 + x < n_rows) *reinterpret_cast<float4 *>(dst + (size_t)(box0 + x) * KV_D + 64 * cg + 4 * c) = box[x * 16 + (c ^ (x & 15))];
+                }
+            }
+            __syncthreads();
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+}  // namespace b200
