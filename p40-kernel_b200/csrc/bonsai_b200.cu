@@ -2207,13 +2207,14 @@ int bonsai_b200_pages_write(const bonsai_b200_pages *pages, int layer, const flo
     P.amplitude = amplitude;
     P.eps = eps;
     const int64_t rows = (int64_t)n_head + 2 * (int64_t)P.C.n_head_kv;
-    auto run = [&](auto kernel, int per) {
-        const int64_t groups = (rows + per * PGW_WARPS - 1) / (per * PGW_WARPS);
+    // few tokens: a warp has one row; many: a CTA four tokens, up to 64 rows of each
+    auto run = [&](auto kernel, int tok, int each) {
+        const int64_t groups = (rows + each - 1) / each;
         if (groups > 65535) return 1;
-        return (int)launch(kernel, dim3((unsigned)P.C.n_tok, (unsigned)groups), dim3(32 * PGW_WARPS), 0, as_stream(stream), true, P);
+        return (int)launch(kernel, dim3((unsigned)((P.C.n_tok + tok - 1) / tok), (unsigned)groups), dim3(32 * PGW_WARPS), 0, as_stream(stream), true, P, each);
     };
-    if (P.C.n_tok * ((rows + PGW_WARPS - 1) / PGW_WARPS) <= 2 * SM_COUNT) return vec ? run(pages_write_kernel<true, 1>, 1) : run(pages_write_kernel<false, 1>, 1);
-    return vec ? run(pages_write_kernel<true, 4>, 4) : run(pages_write_kernel<false, 4>, 4);
+    if (P.C.n_tok * ((rows + PGW_WARPS - 1) / PGW_WARPS) <= 4 * SM_COUNT) return vec ? run(pages_write_kernel<true, 1>, 1, PGW_WARPS) : run(pages_write_kernel<false, 1>, 1, PGW_WARPS);
+    return vec ? run(pages_write_kernel<true, 4>, 4, 64) : run(pages_write_kernel<false, 4>, 4, 64);
 }
 
 int bonsai_b200_pages_read(const bonsai_b200_pages *pages, int layer, const int32_t *first, void *k_out, void *v_out, int type, bonsai_stream stream) {
@@ -2272,7 +2273,9 @@ int bonsai_b200_pages_attn_shared(const bonsai_b200_pages *pages, int layer, con
     if (!q || !out || !aligned4(q) || !aligned4(out) || !shared_sizes(pages, n_groups, n_head)) return 1;
     if (n_groups && (!group || !shared || !aligned4(group) || !aligned4(shared))) return 1;
     if (!workspace || !aligned16(workspace) || workspace_bytes < shared_bytes(pages, n_groups, n_head)) return 1;
-    const int64_t join_ctas = ((int64_t)C.n_tok * n_head + PSJ_WARPS - 1) / PSJ_WARPS;
+    const int64_t out_rows = (int64_t)C.n_tok * n_head;
+    const int roww = out_rows <= 4 * SM_COUNT ? 8 : out_rows <= 32 * SM_COUNT ? 2 : 1;         // few rows have the more parts each, and leave warps free
+    const int64_t join_ctas = (out_rows * roww + PSJ_WARPS - 1) / PSJ_WARPS;
     if (join_ctas > INT32_MAX) return 1;
     const SharedPlan plan = plan_shared(C.n_tok, n_head, C.n_head_kv, C.n_pages, C.table_stride);
     uint8_t *w = static_cast<uint8_t *>(workspace);
@@ -2295,12 +2298,13 @@ int bonsai_b200_pages_attn_shared(const bonsai_b200_pages *pages, int layer, con
     P.ctas = SM_COUNT;
     static SmemOptIn opt[2];
     // what the warps' shares of the registers add up to is what the launch has to bring: one that asked for more would wait for them for good
-    static const int regs = [] {
-        cudaFuncAttributes a = {};
-        return cudaFuncGetAttributes(&a, pages_shared_kernel) == cudaSuccess ? a.numRegs : 0;
+    static const bool regs = [] {
+        cudaFuncAttributes a = {}, b = {};
+        return cudaFuncGetAttributes(&a, pages_shared_kernel) == cudaSuccess && a.numRegs * PSH_THREADS >= PSH_REGS && cudaFuncGetAttributes(&b, pages_shared_tc_kernel) == cudaSuccess &&
+               b.numRegs * PST_THREADS >= PST_REGS;
     }();
     const cudaStream_t st = as_stream(stream);
-    cudaError_t e = regs * PSH_THREADS < PSH_REGS ? cudaErrorLaunchOutOfResources : opt[0].ensure(pages_shared_kernel);
+    cudaError_t e = !regs ? cudaErrorLaunchOutOfResources : opt[0].ensure(pages_shared_kernel);
     if (e == cudaSuccess && P.image_room) e = opt[1].ensure(pages_shared_tc_kernel);
     if (e == cudaSuccess) e = launch(pages_shared_plan_kernel, dim3(1), dim3(PSP_THREADS), 0, st, true, P);
     if (P.image_room) {
@@ -2308,7 +2312,8 @@ int bonsai_b200_pages_attn_shared(const bonsai_b200_pages *pages, int layer, con
         if (e == cudaSuccess) e = launch(pages_shared_tc_kernel, dim3(SM_COUNT), dim3(PST_THREADS), (size_t)PST_SMEM_BYTES, st, true, P);
     }
     if (e == cudaSuccess) e = launch(pages_shared_kernel, dim3(SM_COUNT), dim3(PSH_THREADS), (size_t)PSH_SMEM_BYTES, st, true, P);
-    if (e == cudaSuccess) e = launch(pages_shared_join_kernel, dim3((unsigned)join_ctas), dim3(32 * PSJ_WARPS), 0, st, true, P);
+    auto join = [&](auto kernel) { return launch(kernel, dim3((unsigned)join_ctas), dim3(32 * PSJ_WARPS), 0, st, true, P); };
+    if (e == cudaSuccess) e = roww == 8 ? join(pages_shared_join_kernel<8>) : roww == 2 ? join(pages_shared_join_kernel<2>) : join(pages_shared_join_kernel<1>);
     return (int)e;
 }
 

@@ -24,123 +24,145 @@ struct PageWrite {
 };
 constexpr int PGW_WARPS = 8;
 
-// grid (tokens, groups of rows); a warp has up to PER rows (query heads, then k and v heads), eight values a lane.  VEC: strides are multiples of 4, pointers 16-byte aligned.
-template <bool VEC, int PER>
-__global__ void __launch_bounds__(32 * PGW_WARPS) pages_write_kernel(const __grid_constant__ PageWrite P) {
+// A row of a warp, eight values a lane: normed (w not NULL), turned, and stored.
+__device__ __forceinline__ void page_row_norm(float (&x)[8], const float *w, float eps, int lane) {
+    double ss[4];                           // (four sums and their sum: sums in 64 bits are no more alike for being one chain)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ss[i] = __fma_rn((double)x[i + 4], (double)x[i + 4], __dmul_rn((double)x[i], (double)x[i]));
+    double all = __dadd_rn(__dadd_rn(ss[0], ss[1]), __dadd_rn(ss[2], ss[3]));
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) all = __dadd_rn(all, __shfl_xor_sync(0xffffffffu, all, o));
+    const float sc = __double2float_rn(__ddiv_rn(1.0, __dsqrt_rn(__dadd_rn(__dmul_rn(all, 1.0 / KV_D), (double)eps))));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(__fmul_rn(x[i], sc), w[8 * lane + i]);
+}
+__device__ __forceinline__ void page_row_turn(float (&x)[8], const float2 *turn, float *row, int n_rot, int pairs, int lane) {
+    if (pairs == PAIRS_NEXT) {
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            const int a = 8 * lane + i;
+            if (a >= n_rot) break;
+            const float2 p = turned_pair(x[i], x[i + 1], turn[a >> 1]);
+            x[i] = p.x;
+            x[i + 1] = p.y;
+        }
+        return;
+    }
+    const int half = n_rot >> 1;
+    __syncwarp();                           // the row before has been read
+    if (8 * lane < n_rot) {
+        *reinterpret_cast<float4 *>(row + 8 * lane) = make_float4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<float4 *>(row + 8 * lane + 4) = make_float4(x[4], x[5], x[6], x[7]);
+    }
+    __syncwarp();
+    if (8 * lane >= n_rot) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int a = 8 * lane + i;
+        if (a < half) x[i] = turned_pair(x[i], row[a + half], turn[a]).x;
+        else if (a < n_rot) x[i] = turned_pair(row[a - half], x[i], turn[a - half]).y;
+    }
+}
+__device__ __forceinline__ void page_row_store(const float (&x)[8], uint8_t *dst, float *row, int lane) {
+    const int blk = lane >> 2, sub = lane & 3;
+    const float d = __fmul_rn(kv_amax_8(x), PG_SCALE), id = d > 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
+    uint32_t w[2];
+    kv_words_8(x, id, w);
+    __syncwarp();
+    uint8_t *bytes = reinterpret_cast<uint8_t *>(row);                      // put together by halfwords, stored by 16-byte words
+    unsigned short *p = reinterpret_cast<unsigned short *>(bytes + 34 * blk);
+    if (sub == 0) p[0] = (unsigned short)f32_to_f16_bits_ties_away(d);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        p[1 + 4 * sub + 2 * j] = (unsigned short)(w[j] & 0xFFFFu);
+        p[2 + 4 * sub + 2 * j] = (unsigned short)(w[j] >> 16);
+    }
+    __syncwarp();
+    if (lane < KV_ROW / 16) reinterpret_cast<uint4 *>(dst)[lane] = reinterpret_cast<const uint4 *>(bytes)[lane];
+}
+
+// grid (tokens / TOK, groups of rows).  A CTA finds where its tokens go and forms their angles, then a warp has a row at a time (query heads, then k and v heads of a token; two, so that
+// the next one's values are on their way), eight values a lane.  VEC: strides are multiples of 4, pointers 16-byte aligned.
+template <bool VEC, int TOK>
+__global__ void __launch_bounds__(32 * PGW_WARPS) pages_write_kernel(const __grid_constant__ PageWrite P, int rows_each) {
     __shared__ __align__(16) float rows[PGW_WARPS][KV_D];
-    __shared__ float2 turn[KV_D / 2];
+    __shared__ float2 turn[TOK][KV_D / 2];
+    __shared__ int64_t place[TOK];          // page * 64 + row, -1: nowhere
     const PageCache &C = P.C;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tok = blockIdx.x;
-    const int all = P.n_head + 2 * C.n_head_kv, first = (int)blockIdx.y * PGW_WARPS * PER + warp, half = P.n_rot >> 1;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tok0 = (int)blockIdx.x * TOK, toks = min(TOK, C.n_tok - tok0);
+    const int all = P.n_head + 2 * C.n_head_kv, first = (int)blockIdx.y * rows_each, each = min(rows_each, all - first), half = P.n_rot >> 1;
     pdl_wait_prior_grid();
-    if (PER == 1) pdl_launch_dependents();
+    if (TOK == 1) pdl_launch_dependents();
     auto which = [&](int r, int &h) {       // 0 q, 1 k, 2 v
         const int kind = r < P.n_head ? 0 : r < P.n_head + C.n_head_kv ? 1 : 2;
         h = kind == 0 ? r : r - P.n_head - (kind - 1) * C.n_head_kv;
         return kind;
     };
-    float x[PER][8];
-#pragma unroll
-    for (int e = 0; e < PER; ++e) {
-        const int r = first + PGW_WARPS * e;
-        if (r >= all) break;
+    auto load = [&](int item, float (&x)[8]) {
+        const int t = item / each;
         int h;
-        const int kind = which(r, h);
-        const float *src = P.x[kind] + (int64_t)tok * P.tok_stride[kind] + h * P.head_stride[kind] + 8 * lane;
+        const int kind = which(first + item - t * each, h);
+        const float *src = P.x[kind] + (int64_t)(tok0 + t) * P.tok_stride[kind] + h * P.head_stride[kind] + 8 * lane;
         if (VEC) {
             const float4 a = *reinterpret_cast<const float4 *>(src), b = *reinterpret_cast<const float4 *>(src + 4);
-            x[e][0] = a.x; x[e][1] = a.y; x[e][2] = a.z; x[e][3] = a.w; x[e][4] = b.x; x[e][5] = b.y; x[e][6] = b.z; x[e][7] = b.w;
+            x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[e][i] = src[i];
+            for (int i = 0; i < 8; ++i) x[i] = src[i];
         }
-    }
+    };
+    const int items = toks * each;
+    float x[2][8];
+    if (warp < items) load(warp, x[0]);
+    if (warp + PGW_WARPS < items) load(warp + PGW_WARPS, x[1]);
     if (blockIdx.x == 0 && blockIdx.y == 0) report_ranges(C.start, C.n_seq, C.n_tok);
-    const int s = seq_of_row(C.start, C.n_seq, tok, lane);
-    if (s >= C.n_seq) return;               // rows behind the last sequence (the CTA's warps agree)
-    const SeqRange range = seq_range(C.start, s, C.n_tok);
-    const int64_t at = (int64_t)C.len[s] - range.n + (tok - range.begin);
-    int page = -1;
-    if (range.n > 0 && tok >= range.begin && at >= 0 && at / PG_POS < C.table_stride) page = C.table[(size_t)s * C.table_stride + at / PG_POS];
-    if (page < 0 || page >= C.n_pages) {
-        if (threadIdx.x == 0 && blockIdx.y == 0) bad_sequence();
-        return;
-    }
-    if (half) {
-        const int pos = P.pos ? P.pos[tok] : (int)at;
-        for (int i = threadIdx.x; i < half; i += 32 * PGW_WARPS) turn[i] = turn_of(pos, P.freq[i], (double)P.amplitude);
+    for (int t = warp; t < toks; t += PGW_WARPS) {
+        const int tok = tok0 + t, s = seq_of_row(C.start, C.n_seq, tok, lane);
+        int64_t to = -1;
+        int pos = 0;
+        if (s < C.n_seq) {                  // (rows behind the last sequence are nobody's)
+            const SeqRange range = seq_range(C.start, s, C.n_tok);
+            const int64_t at = (int64_t)C.len[s] - range.n + (tok - range.begin);
+            int page = -1;
+            if (range.n > 0 && tok >= range.begin && at >= 0 && at / PG_POS < C.table_stride) page = C.table[(size_t)s * C.table_stride + at / PG_POS];
+            if (page >= 0 && page < C.n_pages) to = (int64_t)page * PG_POS + at % PG_POS;
+            else if (lane == 0 && blockIdx.y == 0) bad_sequence();
+            pos = P.pos && half ? P.pos[tok] : (int)at;
+        }
+        if (lane == 0) place[t] = to;
+        for (int i = lane; i < half; i += 32) turn[t][i] = turn_of(pos, P.freq[i], (double)P.amplitude);
     }
     __syncthreads();
     float *row = rows[warp];
-#pragma unroll
-    for (int e = 0; e < PER; ++e) {
-        const int r = first + PGW_WARPS * e;
-        if (r >= all) break;
+    auto finish = [&](int item, float (&v)[8]) {
+        const int t = item / each;
         int h;
-        const int kind = which(r, h);
+        const int kind = which(first + item - t * each, h);
+        const int64_t to = place[t];
+        if (to < 0) return;
         if (kind < 2) {
-            if (P.w[kind]) {
-                double ss = 0.0;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) ss = __fma_rn((double)x[e][i], (double)x[e][i], ss);
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) ss = __dadd_rn(ss, __shfl_xor_sync(0xffffffffu, ss, o));
-                const float sc = __double2float_rn(__ddiv_rn(1.0, __dsqrt_rn(__dadd_rn(__dmul_rn(ss, 1.0 / KV_D), (double)P.eps))));
-                const float *w = P.w[kind] + 8 * lane;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[e][i] = __fmul_rn(__fmul_rn(x[e][i], sc), w[i]);
-            }
-            if (half && P.pairs == PAIRS_NEXT) {
-#pragma unroll
-                for (int i = 0; i < 8; i += 2) {
-                    const int a = 8 * lane + i;
-                    if (a >= P.n_rot) break;
-                    const float2 p = turned_pair(x[e][i], x[e][i + 1], turn[a >> 1]);
-                    x[e][i] = p.x;
-                    x[e][i + 1] = p.y;
-                }
-            } else if (half) {
-                __syncwarp();               // the row before has been read
-                if (8 * lane < P.n_rot) {
-                    *reinterpret_cast<float4 *>(row + 8 * lane) = make_float4(x[e][0], x[e][1], x[e][2], x[e][3]);
-                    *reinterpret_cast<float4 *>(row + 8 * lane + 4) = make_float4(x[e][4], x[e][5], x[e][6], x[e][7]);
-                }
-                __syncwarp();
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int a = 8 * lane + i;
-                    if (a < half) x[e][i] = turned_pair(x[e][i], row[a + half], turn[a]).x;
-                    else if (a < P.n_rot) x[e][i] = turned_pair(row[a - half], x[e][i], turn[a - half]).y;
-                }
-            }
+            if (P.w[kind]) page_row_norm(v, P.w[kind], P.eps, lane);
+            if (half) page_row_turn(v, turn[t], row, P.n_rot, P.pairs, lane);
         }
         if (kind == 0) {
-            float *dst = P.q_out + ((int64_t)tok * P.n_head + h) * KV_D + 8 * lane;
+            float *dst = P.q_out + ((int64_t)(tok0 + t) * P.n_head + h) * KV_D + 8 * lane;
             if (VEC) {
-                *reinterpret_cast<float4 *>(dst) = make_float4(x[e][0], x[e][1], x[e][2], x[e][3]);
-                *reinterpret_cast<float4 *>(dst + 4) = make_float4(x[e][4], x[e][5], x[e][6], x[e][7]);
+                *reinterpret_cast<float4 *>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+                *reinterpret_cast<float4 *>(dst + 4) = make_float4(v[4], v[5], v[6], v[7]);
             } else {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) dst[i] = x[e][i];
+                for (int i = 0; i < 8; ++i) dst[i] = v[i];
             }
         } else {
-            const int blk = lane >> 2, sub = lane & 3;
-            const float d = __fmul_rn(kv_amax_8(x[e]), PG_SCALE), id = d > 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
-            uint32_t w[2];
-            kv_words_8(x[e], id, w);
-            __syncwarp();
-            uint8_t *bytes = reinterpret_cast<uint8_t *>(row);              // put together by halfwords, stored by 16-byte words
-            unsigned short *p = reinterpret_cast<unsigned short *>(bytes + 34 * blk);
-            if (sub == 0) p[0] = (unsigned short)f32_to_f16_bits_ties_away(d);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                p[1 + 4 * sub + 2 * j] = (unsigned short)(w[j] & 0xFFFFu);
-                p[2 + 4 * sub + 2 * j] = (unsigned short)(w[j] >> 16);
-            }
-            __syncwarp();
-            uint4 *dst = reinterpret_cast<uint4 *>(page_rows(C, page, P.layer, kind - 1, h) + (size_t)(at % PG_POS) * KV_ROW);
-            if (lane < KV_ROW / 16) dst[lane] = reinterpret_cast<const uint4 *>(bytes)[lane];
+            page_row_store(v, page_rows(C, (int)(to / PG_POS), P.layer, kind - 1, h) + (size_t)(to % PG_POS) * KV_ROW, row, lane);
         }
+    };
+#pragma unroll 1
+    for (int item = warp; item < items; item += 2 * PGW_WARPS) {
+        finish(item, x[0]);
+        if (item + 2 * PGW_WARPS < items) load(item + 2 * PGW_WARPS, x[0]);
+        if (item + PGW_WARPS < items) finish(item + PGW_WARPS, x[1]);
+        if (item + 3 * PGW_WARPS < items) load(item + 3 * PGW_WARPS, x[1]);
     }
 }
 

@@ -24,7 +24,7 @@ namespace b200 {
 constexpr int PSH_ROWS = 48, PSH_STEP = 2 * PG_POS, PSH_STAGE = 32, PSH_CHUNK = 64, PSH_DESCS = 4;
 constexpr int PSH_KSLOTS = 4, PSH_VSLOTS = 3;                    // pages of K and of V in shared memory
 constexpr int PSH_KRING = 2, PSH_VRING = 2;      // in tensor memory: 64 dims of a step's K, 32 positions of V
-constexpr int PSH_START = 1;                                     // what a fragment's begin is worth, in steps
+constexpr int PSH_START = 2;                                     // what a fragment's begin is worth, in steps
 constexpr int PSH_THREADS = 768, PSH_SUM_WARPS = 8, PSH_V_WARP = 8, PSH_K_WARP = 16, PSH_PLAN_WARP = 20, PSH_LOAD_WARP = 21, PSH_SCORE_WARP = 22, PSH_OUT_WARP = 23;
 // registers a thread: 2 x 136 + 2 x 48 + 64 + 48 = 6 x 80, what the launch has
 constexpr int PSH_REGS_SUM = 136, PSH_REGS_V = 48, PSH_REGS_K = 64, PSH_REGS_REST = 48;
@@ -68,7 +68,7 @@ constexpr int PSH_SMEM_BYTES = 1024 + PSH_AT_SMALL + (int)sizeof(PshSmall);
 static_assert(PSH_SMEM_BYTES <= 227 * 1024, "");
 
 // Entities of many rows are pages_shared_tc_kernel's (pages_shared_tc.cuh): tiles of 128 rows, steps of a page, a line of their own.
-constexpr int PST_ROWS = 128, PST_MIN_ROWS = 96, PST_START = 2;
+constexpr int PST_ROWS = 128, PST_MIN_ROWS = 192, PST_MIN_PAGES = 16, PST_START = 4;
 constexpr float PSH_LIFT = 1.0f + 6 * 0x1p-23f;
 
 // What there is to do, found by pages_shared_plan_kernel: a group over its shared pages, or a sequence over its own positions.
@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(PSP_THREADS) pages_shared_plan_kernel(const __
             rows = 0;
         }
         const int pages = (E.end + PG_POS - 1) / PG_POS - E.page0;
-        const long long images = rows && P.image_room && E.tokens * P.group > PST_MIN_ROWS ? pages : 0, image = in_front(images, images0);
+        const long long images = rows && P.image_room && E.tokens * P.group > PST_MIN_ROWS && pages >= PST_MIN_PAGES ? pages : 0, image = in_front(images, images0);
         const bool many = images && image + images <= P.image_room;
         if (many) E.image = (int)image, E.steps = pages;
         const long long own = rows ? units(E) : 0;
@@ -298,11 +298,6 @@ __device__ __forceinline__ uint32_t psh_scale(uint32_t d16, float up) {
     const uint32_t d = __half_as_ushort(__float2half_rn(__fmul_rn(f16_bits_to_f32(d16), up)));
     return d | (d << 16);
 }
-__device__ __forceinline__ int psh_key(float x) {                // ordered as the floats are
-    const int b = __float_as_int(x);
-    return b ^ ((b >> 31) & 0x7FFFFFFF);
-}
-__device__ __forceinline__ float psh_from_key(int k) { return __int_as_float(k ^ ((k >> 31) & 0x7FFFFFFF)); }
 template <int N>
 __device__ __forceinline__ void psh_set_registers(bool more) {
     if (more) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -335,6 +330,7 @@ __device__ __forceinline__ bool psh_wait(uint64_t *bar, uint32_t parity) {
         : "=&r"(left)
         : "r"(smem_u32(bar)), "r"(parity)
         : "memory");
+    if (left == 0) atomicExch(&g_device_status, STATUS_MBARRIER_TIMEOUT);
     return left != 0;
 }
 struct PshWait {
@@ -779,20 +775,22 @@ __device__ __forceinline__ void psh_queries(const PageShared &P, PshSmall &S, ui
     if (lane == 0) mbar_arrive(&S.qready);
 }
 
-// Sums over a warp of eight values: of value 4 b4 + 2 b3 + b2 at lanes with these bits.
-__device__ __forceinline__ float psh_sum8(const float2 (&v)[4], int lane) {
+// Eight values reduced over a warp: value psh_of_lane(lane) at each lane.
+template <typename F>
+__device__ __forceinline__ float psh_over8(const float2 (&v)[4], int lane, F op) {
     float x[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         const float a = k & 1 ? v[k >> 1].y : v[k >> 1].x, b = k & 1 ? v[2 + (k >> 1)].y : v[2 + (k >> 1)].x;
-        x[k] = __fadd_rn(lane & 16 ? b : a, __shfl_xor_sync(0xffffffffu, lane & 16 ? a : b, 16));
+        x[k] = op(lane & 16 ? b : a, __shfl_xor_sync(0xffffffffu, lane & 16 ? a : b, 16));
     }
 #pragma unroll
-    for (int k = 0; k < 2; ++k) x[k] = __fadd_rn(lane & 8 ? x[k + 2] : x[k], __shfl_xor_sync(0xffffffffu, lane & 8 ? x[k] : x[k + 2], 8));
-    x[0] = __fadd_rn(lane & 4 ? x[1] : x[0], __shfl_xor_sync(0xffffffffu, lane & 4 ? x[0] : x[1], 4));
-    x[0] = __fadd_rn(x[0], __shfl_xor_sync(0xffffffffu, x[0], 2));
-    return __fadd_rn(x[0], __shfl_xor_sync(0xffffffffu, x[0], 1));
+    for (int k = 0; k < 2; ++k) x[k] = op(lane & 8 ? x[k + 2] : x[k], __shfl_xor_sync(0xffffffffu, lane & 8 ? x[k] : x[k + 2], 8));
+    x[0] = op(lane & 4 ? x[1] : x[0], __shfl_xor_sync(0xffffffffu, lane & 4 ? x[0] : x[1], 4));
+    x[0] = op(x[0], __shfl_xor_sync(0xffffffffu, x[0], 2));
+    return op(x[0], __shfl_xor_sync(0xffffffffu, x[0], 1));
 }
+__device__ __forceinline__ int psh_of_lane(int lane) { return (lane >> 2) & 7; }
 __device__ __forceinline__ void psh_sum_warps(const PageShared &P, PshSmall &S, uint8_t *smem, uint32_t tmem) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quarter = warp & 3, half = warp >> 2, pos = 32 * quarter + lane;
     const uint32_t tlane = tmem + ((uint32_t)(32 * quarter) << 16);
@@ -859,17 +857,20 @@ __device__ __forceinline__ void psh_sum_warps(const PageShared &P, PshSmall &S, 
                     if (dead) break;
 #pragma unroll 1
                     for (int c = 0; c < groups; ++c) {
-                        int x[8];
-                        tc_ld8(tlane + PSH_COL_S + (uint32_t)(16 * c + 8 * half), x);
+                        const int col = 16 * c + 8 * half;
+                        float x[8], f[8];
+                        int limit[8];
+                        tc_ld8(tlane + PSH_COL_S + (uint32_t)col, reinterpret_cast<int (&)[8]>(x));
+                        psh_lds8(S.qf + col, f);
+                        psh_lds8(S.limit + col, limit);
                         tc_ld_wait();
+                        float2 y[4];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const int col = 16 * c + 8 * half + e;
-                            float y = __fmul_rn(__fmul_rn(__int_as_float(x[e]), kf), S.qf[col]);
-                            if (p0 + pos > S.limit[col]) y = -INFINITY;
-                            const float m = psh_from_key(__reduce_max_sync(0xffffffffu, psh_key(y)));
-                            if (lane == 0) S.red[quarter][col] = m;
-                        }
+                        for (int e = 0; e < 4; ++e)
+                            y[e] = make_float2(p0 + pos > limit[2 * e] ? -INFINITY : __fmul_rn(__fmul_rn(x[2 * e], kf), f[2 * e]),
+                                               p0 + pos > limit[2 * e + 1] ? -INFINITY : __fmul_rn(__fmul_rn(x[2 * e + 1], kf), f[2 * e + 1]));
+                        const float m = psh_over8(y, lane, [](float a, float b) { return fmaxf(a, b); });
+                        if ((lane & 3) == 0) S.red[quarter][col + psh_of_lane(lane)] = m;
                     }
                     psh_barrier<128>(1 + half);
                     if (quarter == 0 && lane < 8 * groups) {
@@ -975,8 +976,8 @@ __device__ __forceinline__ void psh_sum_warps(const PageShared &P, PshSmall &S, 
 #pragma unroll
         for (int c = 0; c < 3; ++c)
             if (c < groups) {
-                const float x = psh_sum8(l[c], lane);
-                if ((lane & 3) == 0) S.red[quarter][16 * c + 8 * half + (lane >> 2 & 1) + (lane >> 2 & 2) + (lane >> 2 & 4)] = x;
+                const float x = psh_over8(l[c], lane, [](float a, float b) { return __fadd_rn(a, b); });
+                if ((lane & 3) == 0) S.red[quarter][16 * c + 8 * half + psh_of_lane(lane)] = x;
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
                     if (16 * c + 8 * half + e < F.n_rows && good) {
@@ -1046,76 +1047,92 @@ __global__ void __launch_bounds__(PSH_THREADS, 1) pages_shared_kernel(const __gr
     }
 }
 
-// A row's parts added up: a warp per row (token, head), eight dims a lane.
+// A row's parts added up: ROWW warps per row (token, head), four dims and four more a lane.
 constexpr int PSJ_WARPS = 8;
+template <int ROWW>
 __global__ void __launch_bounds__(32 * PSJ_WARPS) pages_shared_join_kernel(const __grid_constant__ PageShared P) {
+    __shared__ float4 sums[PSJ_WARPS][2][32];
+    __shared__ float lsum[PSJ_WARPS];
     const PageCache &C = P.C;
-    const int lane = threadIdx.x & 31, heads = C.n_head_kv;
-    const int64_t row = (int64_t)blockIdx.x * PSJ_WARPS + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, mine = warp % ROWW, heads = C.n_head_kv;
+    const int64_t row = (int64_t)blockIdx.x * (PSJ_WARPS / ROWW) + warp / ROWW;
     pdl_wait_prior_grid();
     pdl_launch_dependents();
-    if (row >= (int64_t)C.n_tok * P.n_head) return;
-    const int tok = (int)(row / P.n_head), h = (int)(row - (int64_t)tok * P.n_head), kvh = h / P.group;
-    const int s = seq_of_row(C.start, C.n_seq, tok, lane);
-    if (s >= C.n_seq) return;                            // nobody's
-    const PshPlan &plan = *P.plan;
-    const PshEntity own = plan.entity[P.n_groups + s];
-    if (own.steps < 0 || tok < own.begin || tok >= own.begin + own.tokens) return;
     const float *acc[2] = {nullptr, nullptr};
     const float2 *ml[2] = {nullptr, nullptr};
     int n[2] = {0, 0}, gap[2] = {0, 0};                  // a row's parts, and how far apart they are
-    bool served = true;
+    bool served = false;
+    const int tok = (int)(row / P.n_head), h = (int)(row - (int64_t)tok * P.n_head), kvh = h / P.group;
+    const int s = row < (int64_t)C.n_tok * P.n_head ? seq_of_row(C.start, C.n_seq, tok, lane) : C.n_seq;
+    if (s < C.n_seq) {                                   // (a row behind the last sequence is nobody's)
+        const PshPlan &plan = *P.plan;
+        const PshEntity own = plan.entity[P.n_groups + s];
+        served = own.steps >= 0 && tok >= own.begin && tok < own.begin + own.tokens;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {                        // its own positions; what it shares
-        if (i == 1 && own.page0 == 0) break;
-        const PshEntity E = i ? plan.entity[own.group] : own;
-        if (E.steps <= 0) continue;
-        if (E.unit < 0) {
-            served = false;
-            break;
+        for (int i = 0; i < 2; ++i) {                    // its own positions; what it shares
+            if (!served || (i == 1 && own.page0 == 0)) break;
+            const PshEntity E = i ? plan.entity[own.group] : own;
+            if (E.steps <= 0) continue;
+            if (E.unit < 0) {
+                served = false;
+                break;
+            }
+            const bool many = E.image >= 0;
+            const int size = many ? PST_ROWS : PSH_ROWS, start = many ? PST_START : PSH_START;
+            const int at = (tok - E.begin) * P.group + (h - kvh * P.group), tile = at / size, row0 = tile * size, end = psh_tile_end(P.group, E, row0, size);
+            const int steps = many ? (end + PG_POS - 1) / PG_POS - E.page0 : psh_steps(end - E.page0 * PG_POS);
+            if (steps <= 0) continue;
+            const long long per = many ? plan.tc_per : plan.per, begin = E.unit + (long long)(tile * heads + kvh) * (E.steps + start) + start;
+            const long long c0 = begin / per, c1 = (begin + steps - 1) / per;
+            const long long first = (many ? plan.tc_row : 0) + E.row + (long long)row0 * heads + kvh * min(size, E.tokens * P.group - row0) + c0 * size + (at - row0);
+            n[i] = (int)(c1 - c0 + 1);
+            gap[i] = size;
+            acc[i] = P.part + first * KV_D;
+            ml[i] = P.part_ml + first;
         }
-        const bool many = E.image >= 0;
-        const int size = many ? PST_ROWS : PSH_ROWS, start = many ? PST_START : PSH_START;
-        const int at = (tok - E.begin) * P.group + (h - kvh * P.group), tile = at / size, row0 = tile * size, end = psh_tile_end(P.group, E, row0, size);
-        const int steps = many ? (end + PG_POS - 1) / PG_POS - E.page0 : psh_steps(end - E.page0 * PG_POS);
-        if (steps <= 0) continue;
-        const long long per = many ? plan.tc_per : plan.per, begin = E.unit + (long long)(tile * heads + kvh) * (E.steps + start) + start;
-        const long long c0 = begin / per, c1 = (begin + steps - 1) / per;
-        const long long first = (many ? plan.tc_row : 0) + E.row + (long long)row0 * heads + kvh * min(size, E.tokens * P.group - row0) + c0 * size + (at - row0);
-        gap[i] = size;
-        n[i] = (int)(c1 - c0 + 1);
-        acc[i] = P.part + first * KV_D;
-        ml[i] = P.part_ml + first;
     }
-    if (!served) return;
-    const int all = n[0] + n[1];
+    const int all = served ? n[0] + n[1] : 0;
     float m = -INFINITY, l = 0.0f;
     for (int i = lane; i < all; i += 32) m = fmaxf(m, i < n[0] ? ml[0][(size_t)i * gap[0]].x : ml[1][(size_t)(i - n[0]) * gap[1]].x);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-    for (int i0 = 0; i0 < all; i0 += 4) {                // four parts' loads at once
+    for (int i0 = mine; i0 < all; i0 += 4 * ROWW) {      // four parts' loads at once
         float2 x[4];
         float4 c[4], d[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int i = min(i0 + e, all - 1);
+            const int i = min(i0 + e * ROWW, all - 1);
             const size_t step = i < n[0] ? (size_t)i * gap[0] : (size_t)(i - n[0]) * gap[1];
-            const float2 *pml = (i < n[0] ? ml[0] : ml[1]) + step;
             const float4 *src = reinterpret_cast<const float4 *>((i < n[0] ? acc[0] : acc[1]) + step * KV_D) + lane;
-            x[e] = *pml;
+            x[e] = (i < n[0] ? ml[0] : ml[1])[step];
             c[e] = src[0];
             d[e] = src[32];
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            if (i0 + e >= all) break;
+            if (i0 + e * ROWW >= all) break;
             const float w = x[e].x == m ? 1.0f : psh_exp2(__fsub_rn(x[e].x, m));
             l = __fmaf_rn(x[e].y, w, l);
             a = make_float4(__fmaf_rn(c[e].x, w, a.x), __fmaf_rn(c[e].y, w, a.y), __fmaf_rn(c[e].z, w, a.z), __fmaf_rn(c[e].w, w, a.w));
             b = make_float4(__fmaf_rn(d[e].x, w, b.x), __fmaf_rn(d[e].y, w, b.y), __fmaf_rn(d[e].z, w, b.z), __fmaf_rn(d[e].w, w, b.w));
         }
     }
+    if (ROWW > 1) {
+        sums[warp][0][lane] = a;
+        sums[warp][1][lane] = b;
+        if (lane == 0) lsum[warp] = l;
+        __syncthreads();
+        if (mine) return;
+#pragma unroll
+        for (int w = 1; w < ROWW; ++w) {
+            const float4 c = sums[warp + w][0][lane], d = sums[warp + w][1][lane];
+            l = __fadd_rn(l, lsum[warp + w]);
+            a = make_float4(__fadd_rn(a.x, c.x), __fadd_rn(a.y, c.y), __fadd_rn(a.z, c.z), __fadd_rn(a.w, c.w));
+            b = make_float4(__fadd_rn(b.x, d.x), __fadd_rn(b.y, d.y), __fadd_rn(b.z, d.z), __fadd_rn(b.w, d.w));
+        }
+    }
+    if (!served) return;
     const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);     // a row that sees nothing is zeros
     float *o = P.out + row * KV_D + 4 * lane;
     const float x[8] = {__fmul_rn(a.x, inv), __fmul_rn(a.y, inv), __fmul_rn(a.z, inv), __fmul_rn(a.w, inv),

@@ -11,8 +11,18 @@
 namespace b200 {
 
 constexpr uint32_t PST_COL_O = 0, PST_COL_S = 256, PST_COL_P = 320, PST_COL_QL = 384;
-constexpr int PST_THREADS = ATC_THREADS + 96;
-constexpr int PST_SMEM_BYTES = 1024 + 3 * ATC_PLANES + (2 * ATC_KEYS + 2 * ATT_D + 2 * 4 * ATC_M) * 4 + 160;
+// a fragment: pages of one tile and kv head
+struct PstFragment {
+    long long part;                     // the first row's place among the parts
+    const uint8_t *img;                 // its first page's image
+    int begin, row0, n_rows, kvh;       // first token of the entity; of its rows the tile's first, and how many
+    int ntiles, pos0;                   // pages (0: no more fragments), first position
+    int before, end, all_see;           // row r sees up to before + r / group (INT32_MAX: end - 1); every row sees up to all_see
+};
+constexpr int PST_THREADS = ATC_THREADS + 128, PST_SCORE_WARP = ATC_WARPS, PST_V_WARP = ATC_WARPS + 2, PST_OUT_WARP = ATC_WARPS + 3;      // (and k's pages)
+constexpr int PST_REGS_ROWS = 104, PST_REGS_REST = 64;           // 4 x 104 + 64 = 5 x 96, what the launch has
+constexpr int PST_REGS = 32 * (ATC_WARPS * PST_REGS_ROWS + 4 * PST_REGS_REST);
+constexpr int PST_SMEM_BYTES = 1024 + 3 * ATC_PLANES + (2 * ATC_KEYS + 2 * ATT_D + 2 * 4 * ATC_M) * 4 + 208 + 2 * (int)sizeof(PstFragment);
 constexpr int PST_IMG_BAD = ATC_IMG_RANGE + 16;                  // 8 bytes of an image: positions whose v is no number
 static_assert(PST_IMG_BAD + 8 <= ATC_IMG_BYTES && PST_ROWS == ATC_M && PG_POS == ATC_KEYS && KV_D == ATT_D, "");
 __device__ __forceinline__ void pst_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(ATC_THREADS) : "memory"); }        // among the threads that have rows
@@ -112,148 +122,195 @@ __global__ void __launch_bounds__(ATC_PREP_THREADS) pages_shared_planes_kernel(c
     }
 }
 
-__global__ void __launch_bounds__(PST_THREADS, 1) pages_shared_tc_kernel(const __grid_constant__ PageShared P) {
-    extern __shared__ __align__(128) uint8_t smem[];
-    uint8_t *qhi = smem + ((1024u - (smem_u32(smem) & 1023u)) & 1023u);
-    uint8_t *kpl = qhi + ATC_PLANES, *vpl = kpl + ATC_PLANES;
-    float *kf = reinterpret_cast<float *>(vpl + ATC_PLANES);             // [2][64] 2^-s of the page's positions, pages alternate
-    float *vf = kf + 2 * ATC_KEYS;                                       // [2][256] 2^-s of the dims (and the weights' 2^-14)
-    float *red0 = vf + 2 * ATT_D;                                        // [2][4][128] exchange between the four warps of a row, pages alternate
-    uint64_t *qk = reinterpret_cast<uint64_t *>(red0 + 2 * 4 * ATC_M), *pv = qk + 1, *scored = qk + 2, *weighed = qk + 3, *kfull = qk + 4, *vfull = qk + 6;
-    unsigned long long *bad = reinterpret_cast<unsigned long long *>(vfull + 2);         // [2] positions of the page whose v is no number
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bad + 2);
-    volatile int *failed = reinterpret_cast<int *>(tmem_slot + 1);
-
-    const PageCache &C = P.C;
+// The warps without rows: one issues the products of scores, one says what the fragments are and issues those of outputs, two copy images.
+__device__ __forceinline__ void pst_drivers(const PageShared &P, PstFragment *desc, uint8_t *qhi, uint8_t *kpl, uint8_t *vpl, float *kf, float *vf, uint64_t *qk, unsigned long long *bad,
+                                            volatile int *failed, uint32_t tmem) {
+    uint64_t *pv = qk + 1, *scored = qk + 2, *weighed = qk + 3, *vfull = qk + 4, *kfull = qk + 6, *kfree = qk + 10, *ffull = qk + 14, *vfree = qk + 16, *gfull = qk + 18;
     const PshPlan &plan = *P.plan;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, heads = C.n_head_kv, entities = P.n_groups + C.n_seq;
-    const int cg = warp >> 2, row = 32 * (warp & 3) + lane;              // a thread's row, and its quarter of the row's columns
-    const bool driver = warp >= ATC_WARPS;
-    if (threadIdx.x == 0) {
-        for (int b = 0; b < 8; ++b) mbar_init(qk + b, b == 2 || b == 3 ? ATC_WARPS : 1);
-        mbar_fence_init();
-        *failed = 0;
-    }
-    pdl_wait_prior_grid();                                               // the plan and the images
-    pdl_launch_dependents();
-    const long long per = plan.tc_per, last = min(per * (blockIdx.x + 1), plan.tc_total);
-    long long at = per * blockIdx.x;
-    if (at >= last) return;                                              // CTA-uniform
-    if (warp == 0) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    __syncthreads();                                                     // the barriers, and where tensor memory is
-    tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
-    const uint32_t tlane = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, heads = P.C.n_head_kv, entities = P.n_groups + P.C.n_seq;
     const size_t img_stride = (size_t)heads * ATC_IMG_BYTES;
-    int it0 = 0;                                                         // pages of the fragments before
     bool ok = true;
-    auto issue_qk = [&] {
-        tc_fence_after();
+    auto wait = [&](uint64_t *bar, uint32_t parity) { ok = ok && __all_sync(0xffffffffu, psh_wait(bar, parity)); };
+    // 64 dims of k, 128 of v give their place to the next page's when they are done.  (Waits between the products cost 250 cycles each, and nothing is multiplied meanwhile.)
+    auto issue_qk = [&](int it) {
         constexpr uint32_t LOW = (ATC_KEYS * 128) >> 4;
-        const uint32_t a0 = tc16_desc_lo(smem_u32(qhi)), b0 = tc16_desc_lo(smem_u32(kpl)), ql = tmem + PST_COL_QL, d = tmem + PST_COL_S;
-        auto off = [](int n) { return (uint32_t)((n >> 2) * (ATC_CHUNK >> 4) + 2 * (n & 3)); };
-        if (elect_one()) {                                               // products with a low plane first: the accumulator is small while they are added
-            tc_mma_f16_ts<false>(d, ql, b0, atc_idesc(ATC_KEYS));
+        const uint32_t a0 = tc16_desc_lo(smem_u32(qhi)), b0 = tc16_desc_lo(smem_u32(kpl)), d = tmem + PST_COL_S;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) wait(kfull + c, (uint32_t)(it & 1));
+        tc_fence_after();
+        if (elect_one()) {
 #pragma unroll
-            for (int n = 1; n < 16; ++n) tc_mma_f16_ts<true>(d, ql + (uint32_t)(8 * n), b0 + off(n), atc_idesc(ATC_KEYS));
+            for (int c = 0; c < 4; ++c) {                // products with a low plane first
+                const uint32_t a = a0 + (uint32_t)(c * (ATC_CHUNK >> 4)), b = b0 + (uint32_t)(c * (ATC_CHUNK >> 4)), ql = tmem + PST_COL_QL + (uint32_t)(32 * c);
+                if (c == 0) tc_mma_f16_ts<false>(d, ql, b, atc_idesc(ATC_KEYS));
+                else tc_mma_f16_ts<true>(d, ql, b, atc_idesc(ATC_KEYS));
 #pragma unroll
-            for (int n = 0; n < 16; ++n) atc_mma_ss<atc_idesc(ATC_KEYS)>(d, a0 + off(n), b0 + LOW + off(n));
+                for (int n = 1; n < 4; ++n) tc_mma_f16_ts<true>(d, ql + (uint32_t)(8 * n), b + (uint32_t)(2 * n), atc_idesc(ATC_KEYS));
 #pragma unroll
-            for (int n = 0; n < 16; ++n) atc_mma_ss<atc_idesc(ATC_KEYS)>(d, a0 + off(n), b0 + off(n));
+                for (int n = 0; n < 4; ++n) atc_mma_ss<atc_idesc(ATC_KEYS)>(d, a + (uint32_t)(2 * n), b + LOW + (uint32_t)(2 * n));
+#pragma unroll
+                for (int n = 0; n < 4; ++n) atc_mma_ss<atc_idesc(ATC_KEYS)>(d, a + (uint32_t)(2 * n), b + (uint32_t)(2 * n));
+                tc_commit(kfree + c);
+            }
             tc_commit(qk);
         }
         __syncwarp();
     };
-    auto issue_pv = [&] {
-        tc_fence_after();
+    auto issue_pv = [&](int it) {
         const uint32_t b0 = tc16_desc_lo(smem_u32(vpl)), ph = tmem + PST_COL_P, pl = ph + 32u;
+        wait(vfull, (uint32_t)(it & 1));
+        wait(vfull + 1, (uint32_t)(it & 1));
+        tc_fence_after();
         if (elect_one()) {
 #pragma unroll
-            for (int n = 0; n < 12; ++n) {
-                const uint32_t a = (n < 4 ? pl : ph) + (uint32_t)(8 * (n & 3));
-                const uint32_t b = b0 + (uint32_t)((n >= 4 && n < 8 ? (2 * ATC_CHUNK) >> 4 : 0) + 2 * (n & 3));
-                if (n == 0) tc_mma_f16_ts<false>(tmem + PST_COL_O, a, b, atc_idesc(ATT_D));
-                else tc_mma_f16_ts<true>(tmem + PST_COL_O, a, b, atc_idesc(ATT_D));
+            for (int c = 0; c < 2; ++c) {
+                const uint32_t d = tmem + PST_COL_O + (uint32_t)(128 * c), b1 = b0 + (uint32_t)(c * (ATC_CHUNK >> 4));
+#pragma unroll
+                for (int n = 0; n < 12; ++n) {
+                    const uint32_t a = (n < 4 ? pl : ph) + (uint32_t)(8 * (n & 3));
+                    const uint32_t b = b1 + (uint32_t)((n >= 4 && n < 8 ? (2 * ATC_CHUNK) >> 4 : 0) + 2 * (n & 3));
+                    if (n == 0) tc_mma_f16_ts<false>(d, a, b, atc_idesc(ATT_D / 2));
+                    else tc_mma_f16_ts<true>(d, a, b, atc_idesc(ATT_D / 2));
+                }
+                tc_commit(vfree + c);
             }
             tc_commit(pv);
         }
         __syncwarp();
     };
-#pragma unroll 1
-    for (int e = plan.tc_first[blockIdx.x]; e < entities && at < last && ok; ++e) {
-        const PshEntity E = plan.entity[e];
-        if (E.unit < 0 || E.image < 0) continue;
-        const int size = E.steps + PST_START, all_rows = E.tokens * P.group, pairs = (all_rows + PST_ROWS - 1) / PST_ROWS * heads;
-        int pair = (int)((at - E.unit) / size);
-#pragma unroll 1
-        for (long long begin = E.unit + (long long)pair * size; pair < pairs && begin < last && ok; ++pair, begin += size) {
-            const int tile = pair / heads, kvh = pair - tile * heads, row0 = tile * PST_ROWS, n_rows = min(PST_ROWS, all_rows - row0);
-            const int end = psh_tile_end(P.group, E, row0, PST_ROWS);
-            const int page0 = (int)max(0ll, at - begin - PST_START);
-            const int ntiles = min((int)min(last - begin, (long long)size) - PST_START, (end + PG_POS - 1) / PG_POS - E.page0) - page0;
+    // the next fragment of the CTA's line
+    const long long per = plan.tc_per, last = min(per * (blockIdx.x + 1), plan.tc_total);
+    long long at = per * blockIdx.x;
+    int e = plan.tc_first[blockIdx.x];
+    auto next = [&](PstFragment &F) {
+        F.ntiles = 0;
+        while (at < last && e < entities) {
+            const PshEntity E = plan.entity[e];
+            const int size = E.steps + PST_START, rows = E.tokens * P.group;
+            const long long tiles = (rows + PST_ROWS - 1) / PST_ROWS, pair = E.unit < 0 || E.image < 0 ? tiles * heads : (at - E.unit) / size;
+            if (pair >= tiles * heads) {
+                ++e;
+                continue;
+            }
+            const long long begin = E.unit + pair * size;
+            const int tile = (int)(pair / heads), page0 = (int)max(0ll, at - begin - PST_START);
+            F.kvh = (int)(pair - (long long)tile * heads);
+            F.row0 = tile * PST_ROWS;
+            F.n_rows = min(PST_ROWS, rows - F.row0);
+            F.end = psh_tile_end(P.group, E, F.row0, PST_ROWS);
+            F.ntiles = max(0, min((int)min(last - begin, (long long)size) - PST_START, (F.end + PG_POS - 1) / PG_POS - E.page0) - page0);
+            F.begin = E.begin;
+            F.before = E.before;
+            F.pos0 = (E.page0 + page0) * PG_POS;
+            F.all_see = E.before == INT32_MAX ? F.end - 1 : E.before + F.row0 / P.group;
+            F.img = P.images + ((size_t)(E.image + page0) * heads + F.kvh) * ATC_IMG_BYTES;
+            F.part = plan.tc_row + E.row + (long long)F.row0 * heads + (long long)F.kvh * F.n_rows + (long long)blockIdx.x * PST_ROWS;
             at = begin + size;
-            if (ntiles <= 0) continue;
-            const bool whole = E.before == INT32_MAX;
-            const int all_see = whole ? end - 1 : E.before + row0 / P.group;
-            const int limit = whole ? end - 1 : row < n_rows ? E.before + (row0 + row) / P.group : -1;       // the last position that the thread's row sees
-            const uint8_t *img = P.images + ((size_t)(E.image + page0) * heads + kvh) * ATC_IMG_BYTES;
-            const size_t part = (size_t)(plan.tc_row + E.row + (long long)row0 * heads + (long long)kvh * n_rows + (long long)blockIdx.x * PST_ROWS);
-            auto row_at = [&](int r) {                                   // where a row of the tile lies in q
-                const int x = row0 + r, tok = x / P.group;
-                return ((size_t)(E.begin + tok) * P.n_head + kvh * P.group + (x - tok * P.group)) * KV_D;
-            };
-            if (driver) {
-                __syncthreads();                                         // q is in its places
-                auto wait = [&](uint64_t *bar, uint32_t parity) { ok = ok && __all_sync(0xffffffffu, psh_wait(bar, parity)); };
-                if (warp == ATC_WARPS) {
+            if (F.ntiles > 0) return;
+        }
+    };
+    if (warp == PST_OUT_WARP) {
+        PstFragment F;
+        int it = 0;
+        next(F);
+        if (lane == 0) desc[0] = F;
+        for (int f = 0;; ++f) {
+            __syncthreads();
+            const int ntiles = F.ntiles;
+            if (ntiles == 0 || *failed) return;
+            next(F);                                     // (its place is the last one's, which everybody has left)
+            if (lane == 0) desc[(f + 1) & 1] = F;
+            __syncthreads();
 #pragma unroll 1
-                    for (int i = 0; i <= ntiles; ++i) {                  // scores of page i, outputs of page i - 1
-                        const int it = it0 + i;
-                        if (i < ntiles) {
-                            if (it > 0) wait(scored, (uint32_t)((it - 1) & 1));
-                            wait(kfull + (it & 1), (uint32_t)((it >> 1) & 1));
-                            issue_qk();
-                        }
-                        if (i > 0) {
-                            wait(weighed, (uint32_t)((it - 1) & 1));
-                            wait(vfull + ((it - 1) & 1), (uint32_t)(((it - 1) >> 1) & 1));
-                            issue_pv();
-                        }
-                    }
-                } else {
-                    const bool v = warp == ATC_WARPS + 2;
+            for (int i = 0; i < ntiles; ++i, ++it) {     // outputs
+                wait(weighed, (uint32_t)(it & 1));
+                issue_pv(it);
+            }
+            if (!ok) *failed = 1;
+            __syncthreads();
+            __syncthreads();
+        }
+    }
+    int it0 = 0;                                         // pages of the fragments before
+    for (int f = 0;; ++f) {
+        __syncthreads();
+        const int ntiles = desc[f & 1].ntiles;
+        const uint8_t *img = desc[f & 1].img;
+        if (ntiles == 0 || *failed) return;
+        __syncthreads();
+        if (warp == PST_SCORE_WARP) {
 #pragma unroll 1
-                    for (int i = 0; i < ntiles; ++i) {                   // k when the scores of the page before have been read, v when its outputs are there
-                        const int it = it0 + i;
-                        if (it > 0) wait(v ? pv : scored, (uint32_t)((it - 1) & 1));
+            for (int i = 0; i < ntiles; ++i) {           // scores
+                const int it = it0 + i;
+                if (it > 0) wait(scored, (uint32_t)((it - 1) & 1));
+                issue_qk(it);
+            }
+        } else {
+            const uint64_t pol = policy_evict_last_or_default();
+#pragma unroll 1
+            for (int i = 0; i < ntiles; ++i, img += img_stride) {
+                const int it = it0 + i;
+                if (warp == PST_V_WARP) {
+#pragma unroll 1
+                    for (int c = 0; c < 2; ++c) {
+                        if (it > 0) wait(vfree + c, (uint32_t)((it - 1) & 1));
                         if (lane == 0) {
-                            const uint64_t pol = policy_evict_last_or_default();
-                            const uint8_t *src = img + (size_t)i * img_stride;
                             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");         // the factors were read by ordinary loads
-                            if (v) {
-                                bad[it & 1] = *reinterpret_cast<const unsigned long long *>(src + PST_IMG_BAD);
-                                mbar_expect_tx(vfull + (it & 1), ATC_PLANES + ATT_D * 4);
-                                bulk_g2s(vf + (it & 1) * ATT_D, src + ATC_IMG_VF, ATT_D * 4, vfull + (it & 1), pol);
-                                bulk_g2s(vpl, src + ATC_PLANES, ATC_PLANES, vfull + (it & 1), pol);
-                            } else {
-                                mbar_expect_tx(kfull + (it & 1), ATC_PLANES + ATC_KEYS * 4);
-                                bulk_g2s(kf + (it & 1) * ATC_KEYS, src + ATC_IMG_KF, ATC_KEYS * 4, kfull + (it & 1), pol);
-                                bulk_g2s(kpl, src, ATC_PLANES, kfull + (it & 1), pol);
+                            if (c == 0) {                // (their place is the page's before the last: its outputs were added in front of the weights that page `it - 1` waited for)
+                                bad[it & 1] = *reinterpret_cast<const unsigned long long *>(img + PST_IMG_BAD);
+                                mbar_expect_tx(gfull + (it & 1), ATT_D * 4);
+                                bulk_g2s(vf + (it & 1) * ATT_D, img + ATC_IMG_VF, ATT_D * 4, gfull + (it & 1), pol);
                             }
+                            mbar_expect_tx(vfull + c, 2 * ATC_CHUNK);
+                            bulk_g2s(vpl + c * ATC_CHUNK, img + ATC_PLANES + c * ATC_CHUNK, ATC_CHUNK, vfull + c, pol);
+                            bulk_g2s(vpl + (2 + c) * ATC_CHUNK, img + ATC_PLANES + (2 + c) * ATC_CHUNK, ATC_CHUNK, vfull + c, pol);
                         }
                         __syncwarp();
                     }
+                    continue;
                 }
-                if (!ok) *failed = 1;
-                __syncthreads();
-                ok = *failed == 0;
-                __syncthreads();
-                it0 += ntiles;
-                continue;
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    if (it > 0) wait(kfree + c, (uint32_t)((it - 1) & 1));
+                    if (lane == 0) {
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        if (c == 0) {
+                            mbar_expect_tx(ffull + (it & 1), ATC_KEYS * 4);
+                            bulk_g2s(kf + (it & 1) * ATC_KEYS, img + ATC_IMG_KF, ATC_KEYS * 4, ffull + (it & 1), pol);
+                        }
+                        mbar_expect_tx(kfull + c, ATC_CHUNK);
+                        bulk_g2s(kpl + c * ATC_CHUNK, img + c * ATC_CHUNK, ATC_CHUNK, kfull + c, pol);
+                    }
+                    __syncwarp();
+                }
             }
+        }
+        it0 += ntiles;
+        if (!ok) *failed = 1;
+        __syncthreads();
+        __syncthreads();
+    }
+}
+// The warps with rows.
+__device__ __forceinline__ void pst_rows(const PageShared &P, const PstFragment *desc, uint8_t *qhi, uint8_t *kpl, float *kf, float *vf, float *red0, uint64_t *qk, unsigned long long *bad,
+                                         volatile int *failed, uint32_t tmem) {
+    uint64_t *pv = qk + 1, *scored = qk + 2, *weighed = qk + 3, *ffull = qk + 14, *gfull = qk + 18;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cg = warp >> 2, row = 32 * (warp & 3) + lane;         // a thread's row, and its quarter of the row's columns
+    const uint32_t tlane = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+    int it0 = 0;                                         // pages of the fragments before
+    bool ok = true;
+#pragma unroll 1
+    for (int f = 0;; ++f) {
+            __syncthreads();
+            const PstFragment &F = desc[f & 1];
+            const int ntiles = F.ntiles, n_rows = F.n_rows;
+            if (ntiles == 0 || *failed) return;
+            // the last position that the thread's row sees
+            const int limit = F.before == INT32_MAX ? F.end - 1 : row < n_rows ? F.before + (F.row0 + row) / P.group : -1, all_see = F.all_see, pos0 = F.pos0;
+            auto row_at = [&](int r) {                   // where a row of the tile lies in q
+                const int x = F.row0 + r, tok = x / P.group;
+                return ((size_t)(F.begin + tok) * P.n_head + F.kvh * P.group + (x - tok * P.group)) * KV_D;
+            };
             // ---- q: row of the thread, 64 dims, quantised to Q8_0 (two blocks); high plane to shared memory, low plane to tensor memory, through shared memory (the planes' of k and
             // v, a warp's 32 rows of 64 values each, 16-byte pieces swizzled)
             float4 *box = reinterpret_cast<float4 *>(kpl) + warp * 512;
@@ -299,7 +356,7 @@ __global__ void __launch_bounds__(PST_THREADS, 1) pages_shared_tc_kernel(const _
 #pragma unroll
                 for (int c = 0; c < 4; ++c) m = max(m, redu[c * ATC_M + row]);
                 const int s = atc_shift(min(m, 0x7F7FFFFFu), 63);
-                qf = __fmul_rn(atc_pow2(-s), P.scale);
+                qf = __fmul_rn(atc_pow2(-s), __fmul_rn(__fmul_rn(P.scale, 1.44269504088896340736f), PSH_LIFT));        // scores as powers of two
                 uint32_t lo32[32];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
@@ -314,11 +371,14 @@ __global__ void __launch_bounds__(PST_THREADS, 1) pages_shared_tc_kernel(const _
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");        // q high: written here, read by the tensor core
             tc_fence_before();
             __syncthreads();                                            // (and the box has been read: k and v take its place)
-            float acc[64];                                              // row, dims 64 cg ..
+            float2 acc[32];                                             // row, dims 64 cg ..
 #pragma unroll
-            for (int i = 0; i < 64; ++i) acc[i] = 0.0f;
-            float m_run = -INFINITY, l_run = 0.0f, alpha = 0.0f;        // l_run: of the thread's 16 columns of every page
+            for (int i = 0; i < 32; ++i) acc[i] = make_float2(0.0f, 0.0f);
+            float m_run = -INFINITY, l_run = 0.0f, alpha = 1.0f;        // l_run: of the thread's 16 columns of every page
             auto add_page = [&](int par) {
+                if (__any_sync(0xffffffffu, alpha != 1.0f))
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) acc[i] = mul2(acc[i], make_float2(alpha, alpha));
 #pragma unroll
                 for (int h = 0; h < 8; ++h) {
                     int o[8];
@@ -327,11 +387,9 @@ __global__ void __launch_bounds__(PST_THREADS, 1) pages_shared_tc_kernel(const _
 #pragma unroll
                     for (int i = 0; i < 8; i += 4) {
                         const float4 f = *reinterpret_cast<const float4 *>(vf + par * ATT_D + 64 * cg + 8 * h + i);
-                        float *a = acc + 8 * h + i;
-                        a[0] = __fmaf_rn(__int_as_float(o[i]), f.x, __fmul_rn(a[0], alpha));
-                        a[1] = __fmaf_rn(__int_as_float(o[i + 1]), f.y, __fmul_rn(a[1], alpha));
-                        a[2] = __fmaf_rn(__int_as_float(o[i + 2]), f.z, __fmul_rn(a[2], alpha));
-                        a[3] = __fmaf_rn(__int_as_float(o[i + 3]), f.w, __fmul_rn(a[3], alpha));
+                        float2 *a = acc + 4 * h + (i >> 1);
+                        a[0] = fma2(make_float2(__int_as_float(o[i]), __int_as_float(o[i + 1])), make_float2(f.x, f.y), a[0]);
+                        a[1] = fma2(make_float2(__int_as_float(o[i + 2]), __int_as_float(o[i + 3])), make_float2(f.z, f.w), a[1]);
                     }
                 }
             };
@@ -342,21 +400,23 @@ __global__ void __launch_bounds__(PST_THREADS, 1) pages_shared_tc_kernel(const _
             };
 #pragma unroll 1
             for (int i = 0; i <= ntiles; ++i) {
-                const int it = it0 + i, p0 = (E.page0 + page0 + i) * PG_POS;
+                const int it = it0 + i, p0 = pos0 + i * PG_POS;
                 const uint32_t par = (uint32_t)(it & 1);
                 uint32_t hi[8], lo[8];
-                float alpha_new = 0.0f;
+                float alpha_new = 1.0f;
                 if (i < ntiles) {
                     float *red = red0 + par * 4 * ATC_M;
                     float s[16], mx = -INFINITY;
-                    ok = ok && mbar_wait_both(kfull + par, (uint32_t)((it >> 1) & 1), qk, par);       // (the first is long complete; it makes the copied factors visible)
+                    ok = ok && psh_wait(ffull + par, (uint32_t)((it >> 1) & 1)) && psh_wait(qk, par);        // (the first is long complete; it makes the copied factors visible)
                     tc_fence_after();
-                    {
-                        int a[16];
-                        tc_ld16(tlane + PST_COL_S + (uint32_t)(16 * cg), a);
-                        tc_ld_wait();
+                    tc_ld16(tlane + PST_COL_S + (uint32_t)(16 * cg), reinterpret_cast<int (&)[16]>(s));
+                    tc_ld_wait();
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) s[j] = __fmul_rn(__int_as_float(a[j]), __fmul_rn(qf, kf[par * ATC_KEYS + 16 * cg + j]));
+                    for (int j = 0; j < 16; j += 4) {
+                        const float4 f = *reinterpret_cast<const float4 *>(kf + par * ATC_KEYS + 16 * cg + j);
+                        const float2 a = mul2(make_float2(s[j], s[j + 1]), mul2(make_float2(qf, qf), make_float2(f.x, f.y)));
+                        const float2 b = mul2(make_float2(s[j + 2], s[j + 3]), mul2(make_float2(qf, qf), make_float2(f.z, f.w)));
+                        s[j] = a.x; s[j + 1] = a.y; s[j + 2] = b.x; s[j + 3] = b.y;
                     }
                     tc_fence_before();
                     __syncwarp();
@@ -367,27 +427,32 @@ __global__ void __launch_bounds__(PST_THREADS, 1) pages_shared_tc_kernel(const _
                             if (p0 + 16 * cg + j > limit) s[j] = -INFINITY;
                     }
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[j]);
+                    for (int j = 0; j < 16; j += 2) mx = fmaxf(mx, fmaxf(s[j], s[j + 1]));
                     red[cg * ATC_M + row] = mx;
                     pst_barrier();
                     float m_new = m_run;
 #pragma unroll
                     for (int c = 0; c < 4; ++c) m_new = fmaxf(m_new, red[c * ATC_M + row]);
                     const float base = m_new == -INFINITY ? 0.0f : m_new;
-                    alpha_new = expf(__fsub_rn(m_run, base));
+                    alpha_new = m_new == m_run ? 1.0f : psh_exp2(__fsub_rn(m_run, base));
                     m_run = m_new;
-                    float sum = 0.0f;
+                    const float less = __fsub_rn(14.0f, base);          // (weights come as 2^14 of themselves)
+                    float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
                     for (int j = 0; j < 16; j += 2) {
-                        const float x = expf(__fsub_rn(s[j], base)), y = expf(__fsub_rn(s[j + 1], base));
-                        sum = __fadd_rn(sum, __fadd_rn(x, y));
-                        split_f16x2(__fmul_rn(x, 16384.0f), __fmul_rn(y, 16384.0f), hi[j >> 1], lo[j >> 1]);
+                        const float2 t = add2(make_float2(s[j], s[j + 1]), make_float2(less, less)), w = make_float2(psh_exp2(t.x), psh_exp2(t.y));
+                        sum = add2(sum, w);
+                        const __half2 h = __floats2half2_rn(w.x, w.y);
+                        const float2 rest = fma2(__half22float2(h), make_float2(-1.0f, -1.0f), w);       // exact
+                        const __half2 r = __floats2half2_rn(rest.x, rest.y);
+                        hi[j >> 1] = *reinterpret_cast<const uint32_t *>(&h);
+                        lo[j >> 1] = *reinterpret_cast<const uint32_t *>(&r);
                     }
-                    l_run = __fadd_rn(__fmul_rn(l_run, alpha_new), sum);
+                    l_run = __fmaf_rn(l_run, alpha_new, __fadd_rn(sum.x, sum.y));
                 }
                 if (i > 0) {                                            // the outputs of the page before; its weights have been read
                     const uint32_t was = par ^ 1u;
-                    ok = ok && mbar_wait_both(vfull + was, (uint32_t)(((it - 1) >> 1) & 1), pv, was);
+                    ok = ok && psh_wait(pv, was) && psh_wait(gfull + was, (uint32_t)(((it - 1) >> 1) & 1));
                     tc_fence_after();
                 }
                 if (i < ntiles) {
@@ -412,14 +477,15 @@ __global__ void __launch_bounds__(PST_THREADS, 1) pages_shared_tc_kernel(const _
             float *red = red0;
             red[cg * ATC_M + row] = l_run;
             pst_barrier();
+            const size_t part = (size_t)F.part;
             if (ok) {
                 if (cg == 0 && row < n_rows) {
                     const float l = __fadd_rn(__fadd_rn(red[row], red[ATC_M + row]), __fadd_rn(red[2 * ATC_M + row], red[3 * ATC_M + row]));
-                    P.part_ml[part + row] = make_float2(__fmul_rn(m_run, 1.44269504088896340736f), l);
+                    P.part_ml[part + row] = make_float2(m_run, __fmul_rn(l, 0x1p-14f));
                 }
                 float *dst = P.part + part * KV_D;
 #pragma unroll
-                for (int c = 0; c < 16; ++c) box[lane * 16 + (c ^ (lane & 15))] = make_float4(acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]);
+                for (int c = 0; c < 16; ++c) box[lane * 16 + (c ^ (lane & 15))] = make_float4(acc[2 * c].x, acc[2 * c].y, acc[2 * c + 1].x, acc[2 * c + 1].y);
                 __syncwarp();
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
@@ -428,7 +494,45 @@ __global__ void __launch_bounds__(PST_THREADS, 1) pages_shared_tc_kernel(const _
                 }
             }
             __syncthreads();
-        }
+    }
+}
+
+__global__ void __launch_bounds__(PST_THREADS, 1) pages_shared_tc_kernel(const __grid_constant__ PageShared P) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    uint8_t *qhi = smem + ((1024u - (smem_u32(smem) & 1023u)) & 1023u);
+    uint8_t *kpl = qhi + ATC_PLANES, *vpl = kpl + ATC_PLANES;
+    float *kf = reinterpret_cast<float *>(vpl + ATC_PLANES);             // [2][64] 2^-s of the page's positions, pages alternate
+    float *vf = kf + 2 * ATC_KEYS;                                       // [2][256] 2^-s of the dims (and the weights' 2^-14)
+    float *red0 = vf + 2 * ATT_D;                                        // [2][4][128] exchange between the four warps of a row, pages alternate
+    uint64_t *qk = reinterpret_cast<uint64_t *>(red0 + 2 * 4 * ATC_M);               // scores there, outputs there, scores read, weights there; k and v, by 64 and 128 dims, there and free; factors
+    unsigned long long *bad = reinterpret_cast<unsigned long long *>(qk + 20);         // [2] positions of the page whose v is no number
+    PstFragment *desc = reinterpret_cast<PstFragment *>(bad + 2);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(desc + 2);
+    volatile int *failed = reinterpret_cast<int *>(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5;
+    if (threadIdx.x == 0) {
+        for (int b = 0; b < 20; ++b) mbar_init(qk + b, b == 2 || b == 3 ? ATC_WARPS : 1);
+        mbar_fence_init();
+        *failed = 0;
+    }
+    pdl_wait_prior_grid();                                               // the plan and the images
+    pdl_launch_dependents();
+    if (P.plan->tc_per * blockIdx.x >= P.plan->tc_total) return;         // CTA-uniform
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    __syncthreads();                                                     // the barriers, and where tensor memory is
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    // Every warp is at four barriers of the CTA for a fragment: (1) it is known, (2) q is in its places, (3) its pages are done, (4) its sums are out.
+    if (warp >= ATC_WARPS) {
+        psh_set_registers<PST_REGS_REST>(false);
+        pst_drivers(P, desc, qhi, kpl, vpl, kf, vf, qk, bad, failed, tmem);
+    } else {
+        psh_set_registers<PST_REGS_ROWS>(true);
+        pst_rows(P, desc, qhi, kpl, kf, vf, red0, qk, bad, failed, tmem);
     }
     tc_fence_before();
     __syncthreads();
