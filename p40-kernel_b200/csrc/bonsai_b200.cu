@@ -2195,6 +2195,7 @@ int bonsai_b200_pages_write(const bonsai_b200_pages *pages, int layer, const flo
         vec = vec && aligned16(q_out);
     }
     if ((q_weight && !aligned4(q_weight)) || (k_weight && !aligned4(k_weight)) || (pos && !aligned4(pos))) return 1;
+    vec = vec && (!q_weight || aligned16(q_weight)) && (!k_weight || aligned16(k_weight));
     P.w[0] = q_weight;
     P.w[1] = k_weight;
     P.q_out = q_out;
@@ -2214,7 +2215,7 @@ int bonsai_b200_pages_write(const bonsai_b200_pages *pages, int layer, const flo
         return (int)launch(kernel, dim3((unsigned)((P.C.n_tok + tok - 1) / tok), (unsigned)groups), dim3(32 * PGW_WARPS), 0, as_stream(stream), true, P, each);
     };
     if (P.C.n_tok * ((rows + PGW_WARPS - 1) / PGW_WARPS) <= 4 * SM_COUNT) return vec ? run(pages_write_kernel<true, 1>, 1, PGW_WARPS) : run(pages_write_kernel<false, 1>, 1, PGW_WARPS);
-    return vec ? run(pages_write_kernel<true, 4>, 4, 64) : run(pages_write_kernel<false, 4>, 4, 64);
+    return vec ? run(pages_write_kernel<true, 2>, 2, 64) : run(pages_write_kernel<false, 2>, 2, 64);
 }
 
 int bonsai_b200_pages_read(const bonsai_b200_pages *pages, int layer, const int32_t *first, void *k_out, void *v_out, int type, bonsai_stream stream) {

@@ -24,8 +24,35 @@ struct PageWrite {
 };
 constexpr int PGW_WARPS = 8;
 
-// A row of a warp, eight values a lane: normed (w not NULL), turned, and stored.
+// A row of a warp, eight values a lane: loaded, normed, turned, and stored.
+template <bool VEC>
+__device__ __forceinline__ void page_row_load(const float *src, float (&x)[8]) {
+    if (VEC) {
+        const float4 a = *reinterpret_cast<const float4 *>(src), b = *reinterpret_cast<const float4 *>(src + 4);
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = src[i];
+    }
+}
+// Where value a of a row, or angle a of pairs of halves, lies in shared memory: the first four of each eight, then the other four, so that lanes which read eight
+// each read 16 bytes side by side.  (In their own order, one value a load, the banks of the 8 x 3 loads took 60 % of the kernel's time.)
+template <int N>
+__device__ __forceinline__ int page_row_at(int a) {
+    return (a >> 2 & 1) * (N / 2) + (a >> 3) * 4 + (a & 3);
+}
+template <int N>
+__device__ __forceinline__ void page_row_lds(const float *at, int a, float (&x)[8]) {
+    const float4 u = *reinterpret_cast<const float4 *>(at + (a >> 3) * 4), v = *reinterpret_cast<const float4 *>(at + N / 2 + (a >> 3) * 4);
+    x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w; x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
+}
+struct PageTurn {
+    float c[KV_D / 2], s[KV_D / 2];
+};
+template <bool VEC>
 __device__ __forceinline__ void page_row_norm(float (&x)[8], const float *w, float eps, int lane) {
+    float wx[8];
+    page_row_load<VEC>(w + 8 * lane, wx);
     double ss[4];                           // (four sums and their sum: sums in 64 bits are no more alike for being one chain)
 #pragma unroll
     for (int i = 0; i < 4; ++i) ss[i] = __fma_rn((double)x[i + 4], (double)x[i + 4], __dmul_rn((double)x[i], (double)x[i]));
@@ -34,33 +61,45 @@ __device__ __forceinline__ void page_row_norm(float (&x)[8], const float *w, flo
     for (int o = 1; o < 32; o <<= 1) all = __dadd_rn(all, __shfl_xor_sync(0xffffffffu, all, o));
     const float sc = __double2float_rn(__ddiv_rn(1.0, __dsqrt_rn(__dadd_rn(__dmul_rn(all, 1.0 / KV_D), (double)eps))));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(__fmul_rn(x[i], sc), w[8 * lane + i]);
+    for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(__fmul_rn(x[i], sc), wx[i]);
 }
-__device__ __forceinline__ void page_row_turn(float (&x)[8], const float2 *turn, float *row, int n_rot, int pairs, int lane) {
+__device__ __forceinline__ void page_row_turn(float (&x)[8], const PageTurn &turn, float *row, int n_rot, int pairs, int lane) {
     if (pairs == PAIRS_NEXT) {
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
             const int a = 8 * lane + i;
             if (a >= n_rot) break;
-            const float2 p = turned_pair(x[i], x[i + 1], turn[a >> 1]);
+            const float2 p = turned_pair(x[i], x[i + 1], make_float2(turn.c[a >> 1], turn.s[a >> 1]));
             x[i] = p.x;
             x[i + 1] = p.y;
         }
         return;
     }
-    const int half = n_rot >> 1;
+    const int half = n_rot >> 1, a0 = 8 * lane;
     __syncwarp();                           // the row before has been read
-    if (8 * lane < n_rot) {
-        *reinterpret_cast<float4 *>(row + 8 * lane) = make_float4(x[0], x[1], x[2], x[3]);
-        *reinterpret_cast<float4 *>(row + 8 * lane + 4) = make_float4(x[4], x[5], x[6], x[7]);
+    if (a0 < n_rot) {
+        *reinterpret_cast<float4 *>(row + 4 * lane) = make_float4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<float4 *>(row + KV_D / 2 + 4 * lane) = make_float4(x[4], x[5], x[6], x[7]);
     }
     __syncwarp();
-    if (8 * lane >= n_rot) return;
+    if (a0 >= n_rot) return;
+    if (half % 8 == 0) {                    // a lane's eight are of one half, their partners one lane's
+        const bool high = a0 >= half;
+        float y[8], c[8], s[8];
+        page_row_lds<KV_D>(row, high ? a0 - half : a0 + half, y);
+        page_row_lds<KV_D / 2>(turn.c, high ? a0 - half : a0, c);
+        page_row_lds<KV_D / 2>(turn.s, high ? a0 - half : a0, s);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = high ? turned_pair(y[i], x[i], make_float2(c[i], s[i])).y : turned_pair(x[i], y[i], make_float2(c[i], s[i])).x;
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const int a = 8 * lane + i;
-        if (a < half) x[i] = turned_pair(x[i], row[a + half], turn[a]).x;
-        else if (a < n_rot) x[i] = turned_pair(row[a - half], x[i], turn[a - half]).y;
+        const int a = a0 + i, j = page_row_at<KV_D / 2>(a < half ? a : a - half);
+        if (a >= n_rot) break;
+        const float u = row[page_row_at<KV_D>(a < half ? a : a - half)], v = row[page_row_at<KV_D>(a < half ? a + half : a)];
+        const float2 p = turned_pair(u, v, make_float2(turn.c[j], turn.s[j]));
+        x[i] = a < half ? p.x : p.y;
     }
 }
 __device__ __forceinline__ void page_row_store(const float (&x)[8], uint8_t *dst, float *row, int lane) {
@@ -82,11 +121,11 @@ __device__ __forceinline__ void page_row_store(const float (&x)[8], uint8_t *dst
 }
 
 // grid (tokens / TOK, groups of rows).  A CTA finds where its tokens go and forms their angles, then a warp has a row at a time (query heads, then k and v heads of a token; two, so that
-// the next one's values are on their way), eight values a lane.  VEC: strides are multiples of 4, pointers 16-byte aligned.
+// the next one's values are on their way), eight values a lane.  VEC: strides are multiples of 4, pointers (weights' too) 16-byte aligned.
 template <bool VEC, int TOK>
 __global__ void __launch_bounds__(32 * PGW_WARPS) pages_write_kernel(const __grid_constant__ PageWrite P, int rows_each) {
     __shared__ __align__(16) float rows[PGW_WARPS][KV_D];
-    __shared__ float2 turn[TOK][KV_D / 2];
+    __shared__ __align__(16) PageTurn turn[TOK];
     __shared__ int64_t place[TOK];          // page * 64 + row, -1: nowhere
     const PageCache &C = P.C;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tok0 = (int)blockIdx.x * TOK, toks = min(TOK, C.n_tok - tok0);
@@ -102,14 +141,7 @@ __global__ void __launch_bounds__(32 * PGW_WARPS) pages_write_kernel(const __gri
         const int t = item / each;
         int h;
         const int kind = which(first + item - t * each, h);
-        const float *src = P.x[kind] + (int64_t)(tok0 + t) * P.tok_stride[kind] + h * P.head_stride[kind] + 8 * lane;
-        if (VEC) {
-            const float4 a = *reinterpret_cast<const float4 *>(src), b = *reinterpret_cast<const float4 *>(src + 4);
-            x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = src[i];
-        }
+        page_row_load<VEC>(P.x[kind] + (int64_t)(tok0 + t) * P.tok_stride[kind] + h * P.head_stride[kind] + 8 * lane, x);
     };
     const int items = toks * each;
     float x[2][8];
@@ -130,7 +162,12 @@ __global__ void __launch_bounds__(32 * PGW_WARPS) pages_write_kernel(const __gri
             pos = P.pos && half ? P.pos[tok] : (int)at;
         }
         if (lane == 0) place[t] = to;
-        for (int i = lane; i < half; i += 32) turn[t][i] = turn_of(pos, P.freq[i], (double)P.amplitude);
+        for (int i = lane; i < half; i += 32) {
+            const float2 angle = turn_of(pos, P.freq[i], (double)P.amplitude);
+            const int at = P.pairs == PAIRS_NEXT ? i : page_row_at<KV_D / 2>(i);
+            turn[t].c[at] = angle.x;
+            turn[t].s[at] = angle.y;
+        }
     }
     __syncthreads();
     float *row = rows[warp];
@@ -141,7 +178,7 @@ __global__ void __launch_bounds__(32 * PGW_WARPS) pages_write_kernel(const __gri
         const int64_t to = place[t];
         if (to < 0) return;
         if (kind < 2) {
-            if (P.w[kind]) page_row_norm(v, P.w[kind], P.eps, lane);
+            if (P.w[kind]) page_row_norm<VEC>(v, P.w[kind], P.eps, lane);
             if (half) page_row_turn(v, turn[t], row, P.n_rot, P.pairs, lane);
         }
         if (kind == 0) {
