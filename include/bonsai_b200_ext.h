@@ -341,9 +341,10 @@ int bonsai_b200_pages_attn(const bonsai_b200_pages *pages, int layer, const floa
  * each, whole ones, are the same: only the table row of the first of them that has new tokens is read there.  New tokens lie behind them: len[s] less its new tokens is
  * shared[g] * BONSAI_B200_PAGE_POSITIONS at least.  A sequence of no group, or of a group of one, shares nothing; n_groups (n_seq at most) may be 0.  group (n_groups + 1 numbers) and
  * shared (n_groups) lie on the device like start.  A row of V with a scale that is no number or infinite makes the outputs of the tokens that see it NaN, and no others.
- * Values of V that are smaller than 2^-22 of the largest of their block of 32 dims among 128 positions that follow each other count as multiples of 2^-40 of that.
+ * Scales below 2^-21 of the largest of their row of K, or of their block of 32 dims of V among 128 positions that follow each other, count as multiples of 2^-32 of that.
  * workspace: 16-byte aligned device memory of bonsai_b200_pages_attn_shared_workspace(the same cache and sizes; it reads the struct's numbers, not its memory) bytes: 2 KB for each token and
- * query head, 7.3 MB, and in calls of more than 96 rows (n_head / n_head_kv a token) 20 MB and 133 KB a kv head for each page that may be one of entities with as many, 2.5 GB at most. */
+ * query head, 7.3 MB, and in calls of more than 640 rows (n_head / n_head_kv a token) 20 MB and 133 KB a kv head for
+ * each page that as many rows may have in common, 2.5 GB at most. */
 int64_t bonsai_b200_pages_attn_shared_workspace(const bonsai_b200_pages *pages, int n_groups, int n_head);
 int bonsai_b200_pages_attn_shared(const bonsai_b200_pages *pages, int layer, const int32_t *group, const int32_t *shared, int n_groups, const float *q, float *out, int n_head,
                                   void *workspace, int64_t workspace_bytes, float scale, bonsai_stream stream);

@@ -14,6 +14,10 @@
 //
 // Warps: 0 - 7 weights and outputs (a thread has a position of S^T, or two dims of O^T, and half of the columns), 8 - 15 V (a dim a thread), 16 - 19 K (a position a
 // thread), 20 says what the fragments are and copies pages of V, 21 copies those of K, 22 and 23 issue the products of scores and of outputs.
+//
+// What bounds it: turning codes into planes.  A step's 128 positions of K and V are 65536 values, four instructions a pair of them (byte permute, subtraction, product, remainder) and
+// their way to tensor memory: about 7400 cycles a step, where the products of 48 rows take 3900 and the step's bytes 3000.  48 rows a tile: K and V planes, scores and two buffers of outputs then fill
+// tensor memory.  Positions as rows keep the matrix instructions' 128 rows full whatever the number of tokens (tokens as rows: 6 of 128 used by one token).
 #pragma once
 
 #include "attn_tc.cuh"
@@ -23,8 +27,8 @@ namespace b200 {
 
 constexpr int PSH_ROWS = 48, PSH_STEP = 2 * PG_POS, PSH_STAGE = 32, PSH_CHUNK = 64, PSH_DESCS = 4;
 constexpr int PSH_KSLOTS = 4, PSH_VSLOTS = 3;                    // pages of K and of V in shared memory
-constexpr int PSH_KRING = 2, PSH_VRING = 2;      // in tensor memory: 64 dims of a step's K, 32 positions of V
-constexpr int PSH_START = 2;                                     // what a fragment's begin is worth, in steps
+constexpr int PSH_KRING = 2, PSH_VRING = 2;                      // in tensor memory: 64 dims of a step's K, 32 positions of V
+constexpr int PSH_START = 2;                                     // what a fragment's begin is worth, in steps (1 and 4: 146 us where 2 has 142)
 constexpr int PSH_THREADS = 768, PSH_SUM_WARPS = 8, PSH_V_WARP = 8, PSH_K_WARP = 16, PSH_PLAN_WARP = 20, PSH_LOAD_WARP = 21, PSH_SCORE_WARP = 22, PSH_OUT_WARP = 23;
 // registers a thread: 2 x 136 + 2 x 48 + 64 + 48 = 6 x 80, what the launch has
 constexpr int PSH_REGS_SUM = 136, PSH_REGS_V = 48, PSH_REGS_K = 64, PSH_REGS_REST = 48;
@@ -67,8 +71,13 @@ struct alignas(16) PshSmall {
 constexpr int PSH_SMEM_BYTES = 1024 + PSH_AT_SMALL + (int)sizeof(PshSmall);
 static_assert(PSH_SMEM_BYTES <= 227 * 1024, "");
 
-// Entities of many rows are pages_shared_tc_kernel's (pages_shared_tc.cuh): tiles of 128 rows, steps of a page, a line of their own.
-constexpr int PST_ROWS = 128, PST_MIN_ROWS = 192, PST_MIN_PAGES = 16, PST_START = 4;
+// Entities of many rows are pages_shared_tc_kernel's (pages_shared_tc.cuh): tiles of 128 rows, steps of a page, a line of their own.  Measured, whole calls in us, as 48 rows a tile
+// against as images (4 kv heads, one token of 6 heads each): 384 rows over 64 and 256 pages 93 / 102 and 179 / 201; 642 rows over 16, 32, 64 and 256 pages 87 / 92, 101 / 102,
+// 132 / 123 and 269 / 276; 900 rows over 16, 64 and 256 pages 112 / 115, 167 / 152 and 359 / 338; 1200 rows over 500 pages 760 / 656.
+constexpr int PST_ROWS = 128, PST_MIN_ROWS = 640, PST_MIN_PAGES = 32;
+constexpr int PST_START = 8;                                     // what a fragment's begin is worth, in pages (2: 378 us where 8 has 364 and 20 has 379)
+// The tensor core drops what a sum has behind its 24 bits: sums come out low by about 2^-24 for each of the twelve or so that a score is made of.  Scores are lifted by the mean of that
+// (root mean square of the outputs' error 3.4e-6 without, 1.3e-6 with it).
 constexpr float PSH_LIFT = 1.0f + 6 * 0x1p-23f;
 
 // What there is to do, found by pages_shared_plan_kernel: a group over its shared pages, or a sequence over its own positions.
@@ -461,12 +470,10 @@ __device__ __forceinline__ void psh_plan_warp(const PageShared &P, PshSmall &S, 
 }
 
 // 64 dims of a row (words w: a scale's halfword, 32 codes, again) to planes.
-template <int FIRST>
 __device__ __forceinline__ void psh_k_chunk(const uint32_t *w, uint32_t none, float up, uint32_t to) {
-    constexpr int half0 = FIRST ? 34 : 0;                // of w's halfwords the chunk's first
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-        const int s = half0 + 17 * b;
+        const int s = 17 * b;                            // the block's first halfword
         const uint32_t d = psh_scale((s & 1 ? w[s >> 1] >> 16 : w[s >> 1] & 0xFFFFu) & none, up);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
@@ -532,7 +539,7 @@ __device__ __forceinline__ void psh_k_warps(const PageShared &P, PshSmall &S, ui
                 if (chunk >= PSH_KRING) wait(&S.kempty[slot], (uint32_t)((chunk / PSH_KRING - 1) & 1));
                 tc_fence_after();
                 if (mine) {
-                    psh_k_chunk<0>(w, none, up, lanes + (uint32_t)(64 * slot));
+                    psh_k_chunk(w, none, up, lanes + (uint32_t)(64 * slot));
                     tc_st_wait();
                 }
                 tc_fence_before();

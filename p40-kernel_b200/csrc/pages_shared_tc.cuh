@@ -1,9 +1,14 @@
 // pages_shared_tc.cuh -- pages_shared.cuh's attention for entities of many rows (a long prompt's questions, hundreds of answers): 128 rows a tile, rows as the rows of both products.
 //
 // pages_shared_kernel turns the cache's codes into planes for 48 rows at a time; with that many rows the planes are worth writing down.  pages_shared_planes_kernel writes each page of
-// these entities once, as a tile image (attn_tc.cuh's: planes split, swizzled, v transposed), and pages_shared_tc_kernel multiplies as pages_tc_kernel does: 512 threads, each a row and a
-// quarter of its columns, form weights and add outputs; a warp issues the products, of which the next page's scores and this page's outputs are in flight together; two warps copy
-// images.  Tensor memory: 256 outputs, 64 scores, 64 weights, 128 q low; shared memory: q high, k and v of one page.
+// these entities once, as a tile image (attn_tc.cuh's: planes split, swizzled, v transposed), and pages_shared_tc_kernel multiplies: 512 threads, each a row and a quarter of its columns,
+// form weights and add outputs; a warp issues the products of scores, one those of outputs, so that the next page's scores and this page's outputs are in flight together; two warps copy
+// images, 64 dims of k and 128 of v at a time, each part as soon as its products are done.  Tensor memory: 256 outputs, 64 scores, 64 weights, 128 q low; shared memory: q high, k and v
+// of one page.
+//
+// What bounds it: a chain.  A page takes about 4450 cycles, of which the products of its outputs 1700 (three of four products of planes, 128 x 256 x 64), and adding them and writing the
+// next weights 1430: there is one buffer of outputs, since tensor memory has no room for two.  With k, v and both products' waits in one warp it was 6700.  Writing the images takes a
+// fifth of a call (62 us for 1000 of them, 131 MB), mostly conversions; beyond 126 MB they also come back from memory.
 #pragma once
 
 #include "pages_shared.cuh"
