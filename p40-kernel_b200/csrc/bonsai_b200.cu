@@ -2134,7 +2134,7 @@ int bonsai_b200_rope_freq(double *freq, float *amplitude, int n_rot, double thet
         double f = std::pow(theta, -(double)i / pairs);
         if (scaling == BONSAI_B200_ROPE_LINEAR) f /= factor;
         if (scaling == BONSAI_B200_ROPE_YARN && factor > 1.0) {
-            const double slowed = std::min(1.0, std::max(0.0, (i - low) / std::max(high - low, 0.001)));
+            const double slowed = i >= high ? 1.0 : i <= low ? 0.0 : (i - low) / (high - low);
             f = f * (1.0 - slowed) + f / factor * slowed;
         }
         freq[i] = f;
