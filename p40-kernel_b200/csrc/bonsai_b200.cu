@@ -2309,7 +2309,7 @@ int bonsai_b200_pages_attn_shared(const bonsai_b200_pages *pages, int layer, con
     if (e == cudaSuccess && P.image_room) e = opt[1].ensure(pages_shared_tc_kernel);
     if (e == cudaSuccess) e = launch(pages_shared_plan_kernel, dim3(1), dim3(PSP_THREADS), 0, st, true, P);
     if (P.image_room) {
-        if (e == cudaSuccess) e = launch(pages_shared_planes_kernel, dim3(4 * SM_COUNT, 1, 2), dim3(ATC_PREP_THREADS), 0, st, true, P);
+        if (e == cudaSuccess) e = launch(pages_shared_planes_kernel, dim3(3 * SM_COUNT, 1, 2), dim3(ATC_PREP_THREADS), 0, st, true, P);
         if (e == cudaSuccess) e = launch(pages_shared_tc_kernel, dim3(SM_COUNT), dim3(PST_THREADS), (size_t)PST_SMEM_BYTES, st, true, P);
     }
     if (e == cudaSuccess) e = launch(pages_shared_kernel, dim3(SM_COUNT), dim3(PSH_THREADS), (size_t)PSH_SMEM_BYTES, st, true, P);

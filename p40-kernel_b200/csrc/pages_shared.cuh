@@ -297,6 +297,13 @@ __device__ __forceinline__ uint32_t psh_pair(uint32_t w, bool upper) {
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(__byte_perm(w, 0x64646464u, upper ? 0x4342 : 0x4140)), "r"(0x64806480u));
     return y;
 }
+// The same of one byte of each of two words: pick says which byte of x comes first, and which of y third.
+__device__ __forceinline__ uint32_t psh_codes(uint32_t x, uint32_t y, uint32_t pick) {
+    uint32_t c;
+    asm("lop3.b32 %0, %1, 0x00FF00FF, 0x64806480, 0x6A;" : "=r"(c) : "r"(__byte_perm(x, y, pick)));                   // (both & mask) ^ 1024 + 128
+    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(c) : "r"(0x64806480u));
+    return c;
+}
 // Codes times a scale of two fp16 planes: the rounded product and, exactly, what it leaves.
 __device__ __forceinline__ void psh_planes(uint32_t codes, uint32_t d, uint32_t &hi, uint32_t &lo) {
     asm("{\n\t.reg .b32 n;\n\tmul.rn.f16x2 %0, %2, %3;\n\tneg.f16x2 n, %0;\n\tfma.rn.f16x2 %1, %2, %3, n;\n\t}" : "=&r"(hi), "=r"(lo) : "r"(codes), "r"(d));
@@ -625,11 +632,7 @@ __device__ __forceinline__ void psh_v_warps(const PageShared &P, PshSmall &S, ui
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const uint32_t *x = reinterpret_cast<const uint32_t *>(src + (16 * k + 8 * h + 2 * e) * KV_ROW);
-                            const uint32_t both = __byte_perm(x[0], x[KV_ROW / 4], pick2);
-                            uint32_t c;
-                            asm("lop3.b32 %0, %1, 0x00FF00FF, 0x64806480, 0x6A;" : "=r"(c) : "r"(both));           // (both & mask) ^ 1024 + 128
-                            asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(c) : "r"(0x64806480u));
-                            psh_planes(c, d[e], hi[4 * h + e], lo[4 * h + e]);
+                            psh_planes(psh_codes(x[0], x[KV_ROW / 4], pick2), d[e], hi[4 * h + e], lo[4 * h + e]);
                         }
                     }
                     tc_st8(to + (uint32_t)(8 * k), hi);

@@ -8,7 +8,7 @@
 //
 // What bounds it: a chain.  A page takes about 4450 cycles, of which the products of its outputs 1700 (three of four products of planes, 128 x 256 x 64), and adding them and writing the
 // next weights 1430: there is one buffer of outputs, since tensor memory has no room for two.  With k, v and both products' waits in one warp it was 6700.  Writing the images takes a
-// fifth of a call (62 us for 1000 of them, 131 MB), mostly conversions; beyond 126 MB they also come back from memory.
+// seventh of a call (50 us for 1000 of them, 131 MB; with conversions by fp32 62); beyond 126 MB they also come back from memory.
 #pragma once
 
 #include "pages_shared.cuh"
@@ -33,10 +33,11 @@ static_assert(PST_IMG_BAD + 8 <= ATC_IMG_BYTES && PST_ROWS == ATC_M && PG_POS ==
 __device__ __forceinline__ void pst_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(ATC_THREADS) : "memory"); }        // among the threads that have rows
 
 // Images of the pages of the entities of many rows: image E.image + i is page page0 + i, [kv head] beside each other.  z 0 = k (warp = eight positions, lane = eight dims), z 1 = v
-// (thread = one dim, all 64 positions).
+// (thread = one dim, all 64 positions).  Six CTAs of 40 registers fit an SM, and a launch has as many.
 __global__ void __launch_bounds__(ATC_PREP_THREADS) pages_shared_planes_kernel(const __grid_constant__ PageShared P) {
     __shared__ __align__(16) uint8_t rows[PG_HEAD_BYTES];
-    __shared__ uint32_t odd[2];
+    __shared__ uint32_t odd[2][KV_NBLK];
+    __shared__ __align__(16) uint16_t scales[KV_NBLK][ATC_KEYS];
     const PageCache &C = P.C;
     const PshPlan &plan = *P.plan;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, entities = P.n_groups + C.n_seq;
@@ -68,60 +69,64 @@ __global__ void __launch_bounds__(ATC_PREP_THREADS) pages_shared_planes_kernel(c
             const int words = there ? n * (KV_ROW / 16) : 0;
             for (int i = threadIdx.x; i < PG_HEAD_BYTES / 16; i += ATC_PREP_THREADS) reinterpret_cast<uint4 *>(rows)[i] = i < words ? src[i] : make_uint4(0u, 0u, 0u, 0u);
         }
-        if (threadIdx.x < 2) odd[threadIdx.x] = 0;
         __syncthreads();
         uint8_t *img = P.images + (size_t)item * ATC_IMG_BYTES;
-        if (blockIdx.z == 0) {
+        uint32_t hi[4], lo[4];
+        if (blockIdx.z == 0) {                           // a row's scales under one power of two, as pages_shared_kernel has them
             constexpr int ROWS = ATC_KEYS / (ATC_PREP_THREADS / 32);
-#pragma unroll
+#pragma unroll 2
             for (int r = 0; r < ROWS; ++r) {
                 const int key = ROWS * warp + r;
                 const uint16_t *b = reinterpret_cast<const uint16_t *>(rows + key * KV_ROW + 34 * (lane >> 2));
-                const float d = f16_bits_to_f32(b[0]);
-                float x[8];
-                uint32_t m = 0;
+                const int s = psh_shift(__reduce_max_sync(0xffffffffu, (uint32_t)b[0] & 0x7FFFu));
+                const uint32_t d = psh_scale(b[0], atc_pow2(s));
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t w = b[1 + 4 * (lane & 3) + i];
-                    x[2 * i] = __fmul_rn((float)(int8_t)(w & 0xFFu), d);
-                    x[2 * i + 1] = __fmul_rn((float)(int8_t)(w >> 8), d);
-                    m = max(m, max(atc_abs_bits(x[2 * i]), atc_abs_bits(x[2 * i + 1])));
-                }
-                const int s = atc_shift(min(__reduce_max_sync(0xffffffffu, m), 0x7F7FFFFFu), 63);
-                uint4 hi, lo;
-                atc_split8(x, atc_pow2(s), hi, lo);
+                for (int i = 0; i < 4; ++i) psh_planes(psh_pair((uint32_t)b[1 + 4 * (lane & 3) + i] ^ 0x8080u, false), d, hi[i], lo[i]);
                 uint8_t *dst = img + (lane >> 3) * ATC_CHUNK + key * 128 + (((lane & 7) ^ (key & 7)) * 16);
-                *reinterpret_cast<uint4 *>(dst) = hi;
-                *reinterpret_cast<uint4 *>(dst + ATC_KEYS * 128) = lo;
+                *reinterpret_cast<uint4 *>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                *reinterpret_cast<uint4 *>(dst + ATC_KEYS * 128) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 if (lane == 0) reinterpret_cast<float *>(img + ATC_IMG_KF)[key] = atc_pow2(-s);
             }
-        } else {
-            const int d = threadIdx.x;
-            float x[ATC_KEYS];
-            const uint8_t *b = rows + 34 * (d >> 5);
-            uint32_t seen = 0;
+        } else {                                         // a warp has a block of 32 dims: its scales under one power of two, those that are no numbers zero
+            const int dim = threadIdx.x;
+            uint32_t d[2], m = 0;
 #pragma unroll
-            for (int i = 0; i < ATC_KEYS; ++i) {
-                float sc = f16_bits_to_f32(*reinterpret_cast<const uint16_t *>(b + i * KV_ROW));
-                if (!isfinite(sc)) {                     // (its rows are told apart by who has weights for them)
-                    sc = 0.0f;
-                    if ((d & 31) == 0) atomicOr(&odd[i >> 5], 1u << (i & 31));
-                }
-                x[i] = __fmul_rn((float)(int8_t)b[i * KV_ROW + 2 + (d & 31)], sc);
-                seen = max(seen, atc_abs_bits(x[i]));
+            for (int j = 0; j < 2; ++j) {
+                d[j] = *reinterpret_cast<const uint16_t *>(rows + (32 * j + lane) * KV_ROW + 34 * warp);
+                const bool bad = (d[j] & 0x7FFFu) >= 0x7C00u;
+                const uint32_t mask = __ballot_sync(0xffffffffu, bad);       // (its rows are told apart by who has weights for them)
+                if (lane == 0) odd[j][warp] = mask;
+                if (bad) d[j] = 0;
+                m = max(m, d[j] & 0x7FFFu);
             }
-            const int s = atc_shift(seen, 112);
-            reinterpret_cast<float *>(img + ATC_IMG_VF)[d] = atc_pow2(-s - 14);          // (and the weights' 2^-14)
+            const int s = psh_shift(__reduce_max_sync(0xffffffffu, m));
 #pragma unroll
+            for (int j = 0; j < 2; ++j) scales[warp][32 * j + lane] = (uint16_t)psh_scale(d[j], atc_pow2(s));
+            __syncwarp();
+            reinterpret_cast<float *>(img + ATC_IMG_VF)[dim] = atc_pow2(-s - 14);        // (and the weights' 2^-14)
+            const int byte = 34 * warp + 2 + lane;
+            const uint32_t pick = (uint32_t)(byte & 3) | ((uint32_t)(byte & 3) + 4u) << 8;
+            const uint32_t *src = reinterpret_cast<const uint32_t *>(rows + (byte & ~3));
+#pragma unroll 2
             for (int g = 0; g < ATC_KEYS / 8; ++g) {
-                uint4 hi, lo;
-                atc_split8(x + 8 * g, atc_pow2(s), hi, lo);
-                uint8_t *dst = img + ATC_PLANES + d * 128 + ((g ^ (d & 7)) * 16);
-                *reinterpret_cast<uint4 *>(dst) = hi;
-                *reinterpret_cast<uint4 *>(dst + 2 * ATC_CHUNK) = lo;
+                const uint4 d4 = *reinterpret_cast<const uint4 *>(&scales[warp][8 * g]);
+                const uint32_t dd[4] = {d4.x, d4.y, d4.z, d4.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t *x = src + (8 * g + 2 * e) * (KV_ROW / 4);
+                    psh_planes(psh_codes(x[0], x[KV_ROW / 4], pick), dd[e], hi[e], lo[e]);
+                }
+                uint8_t *dst = img + ATC_PLANES + dim * 128 + ((g ^ (dim & 7)) * 16);
+                *reinterpret_cast<uint4 *>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                *reinterpret_cast<uint4 *>(dst + 2 * ATC_CHUNK) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
             }
             __syncthreads();
-            if (d < 2) reinterpret_cast<uint32_t *>(img + PST_IMG_BAD)[d] = odd[d];
+            if (dim < 2) {
+                uint32_t all = 0;
+#pragma unroll
+                for (int b = 0; b < KV_NBLK; ++b) all |= odd[dim][b];
+                reinterpret_cast<uint32_t *>(img + PST_IMG_BAD)[dim] = all;
+            }
         }
         __syncthreads();                                 // the next item's rows take the place of these
     }
