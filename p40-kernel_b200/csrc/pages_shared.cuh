@@ -15,9 +15,11 @@
 // Warps: 0 - 7 weights and outputs (a thread has a position of S^T, or two dims of O^T, and half of the columns), 8 - 15 V (a dim a thread), 16 - 19 K (a position a
 // thread), 20 says what the fragments are and copies pages of V, 21 copies those of K, 22 and 23 issue the products of scores and of outputs.
 //
-// What bounds it: turning codes into planes.  A step's 128 positions of K and V are 65536 values, four instructions a pair of them (byte permute, subtraction, product, remainder) and
-// their way to tensor memory: about 7400 cycles a step, where the products of 48 rows take 3900 and the step's bytes 3000.  48 rows a tile: K and V planes, scores and two buffers of outputs then fill
-// tensor memory.  Positions as rows keep the matrix instructions' 128 rows full whatever the number of tokens (tokens as rows: 6 of 128 used by one token).
+// What bounds it: chains of latencies, that of K's planes first.  A step takes about 8000 cycles.  K's four warps take as long: 1100 for its page and scales, and for each 64 dims 450 to load codes,
+// 350 to see that their place is free, 850 for 32 pairs (byte permute, subtraction, product, remainder) and their way to tensor memory.  V's eight take 6500, the products of 48 rows 3900,
+// the step's bytes 3000.  (4 x 5 tokens over 32000 positions: 122 us; planes of zeros for K, V and both 108, 112 and 99.  Eight warps for K, 48 registers each: 136.)  48 rows a tile: planes,
+// scores and two buffers of outputs then fill tensor memory.  Positions as rows keep the matrix instructions' 128 rows full whatever the number of tokens (tokens as rows: 6 of 128
+// used by one token).
 #pragma once
 
 #include "attn_tc.cuh"
