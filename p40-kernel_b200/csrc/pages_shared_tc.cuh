@@ -140,7 +140,7 @@ __device__ __forceinline__ void pst_drivers(const PageShared &P, PstFragment *de
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, heads = P.C.n_head_kv, entities = P.n_groups + P.C.n_seq;
     const size_t img_stride = (size_t)heads * ATC_IMG_BYTES;
     bool ok = true;
-    auto wait = [&](uint64_t *bar, uint32_t parity) { ok = ok && __all_sync(0xffffffffu, psh_wait(bar, parity)); };
+    auto wait = [&](uint64_t *bar, uint32_t parity) { ok = ok && __all_sync(0xffffffffu, psh_wait<true>(bar, parity)); };
     // 64 dims of k, 128 of v give their place to the next page's when they are done.  (Waits between the products cost 250 cycles each, and nothing is multiplied meanwhile.)
     auto issue_qk = [&](int it) {
         constexpr uint32_t LOW = (ATC_KEYS * 128) >> 4;
@@ -417,7 +417,7 @@ __device__ __forceinline__ void pst_rows(const PageShared &P, const PstFragment 
                 if (i < ntiles) {
                     float *red = red0 + par * 4 * ATC_M;
                     float s[16], mx = -INFINITY;
-                    ok = ok && psh_wait(ffull + par, (uint32_t)((it >> 1) & 1)) && psh_wait(qk, par);        // (the first is long complete; it makes the copied factors visible)
+                    ok = ok && psh_wait<true>(ffull + par, (uint32_t)((it >> 1) & 1)) && psh_wait<true>(qk, par);        // (the first is long complete; it makes the copied factors visible)
                     tc_fence_after();
                     tc_ld16(tlane + PST_COL_S + (uint32_t)(16 * cg), reinterpret_cast<int (&)[16]>(s));
                     tc_ld_wait();
@@ -462,7 +462,7 @@ __device__ __forceinline__ void pst_rows(const PageShared &P, const PstFragment 
                 }
                 if (i > 0) {                                            // the outputs of the page before; its weights have been read
                     const uint32_t was = par ^ 1u;
-                    ok = ok && psh_wait(pv, was) && psh_wait(gfull + was, (uint32_t)(((it - 1) >> 1) & 1));
+                    ok = ok && psh_wait<true>(pv, was) && psh_wait<true>(gfull + was, (uint32_t)(((it - 1) >> 1) & 1));
                     tc_fence_after();
                 }
                 if (i < ntiles) {

@@ -8,7 +8,7 @@ import subprocess
 import pytest
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-MOST = {"pages_shared_kernel": 96, "pages_shared_tc_kernel": 180}       # bytes of stores a thread; none of the others spills
+MOST = {"pages_shared_kernel": 96, "pages_shared_tc_kernel": 184}       # bytes of stores a thread; none of the others spills
 USED = {"pages_shared_kernel": 80, "pages_shared_tc_kernel": 96}        # what their warps' shares add up to
 FORMS = """#include "rotary.cuh"
 #include "pages_rows.cuh"
