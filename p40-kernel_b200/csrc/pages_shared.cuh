@@ -331,7 +331,7 @@ __device__ __forceinline__ PshStep psh_step(const PshFragment &F, int i) {
 // ---- the warps ----------------------------------------------------------------------------------------------------------------------------------
 // A wait that runs out (a second at most): nothing is waited for any more, the CTA comes to its end and leaves its parts unfinished.  (One loop for a wait: what bounds this
 // kernel next to the tensor core is instructions that are not in the cache.)
-// TEST: a look without a wait in front of it.  12 questions of 15 to 150 tokens, pages_shared_tc_kernel's, whose waits are mostly over: 344 us with it, 360 without; 20 tokens of this kernel's: 125 and 122.
+// TEST: a look without a wait in front of it.  pages_shared_tc_kernel, whose waits are mostly over, takes 266 us of a call with it and 273 without; 20 tokens of this kernel's 125 and 122.
 template <bool TEST = false>
 __device__ __forceinline__ bool psh_wait(uint64_t *bar, uint32_t parity) {
     if (TEST) {
