@@ -2161,8 +2161,9 @@ int bonsai_b200_rope(const float *q, const float *k, const int32_t *pos, const d
         vec = vec && aligned16(P.x[i]) && aligned16(P.y[i]) && strides_by(n_tok, P.n_head[i], ts, hs, 4);
     }
     const int64_t each = vec ? n_rot / 8 + (head_dim - n_rot) / 4 : n_rot / 2 + head_dim - n_rot, items = heads * each;
-    // a token's items by CTAs: as many as threads hold (vec), fewer of few tokens
-    const int64_t most = ROPE_THREADS * (vec ? (n_tok <= 2 * SM_COUNT ? 1 : ROPE_MAX_ITEMS) : 4), parts = (items + most - 1) / most;
+    // a token's items by CTAs: as many as threads hold (vec), one of few tokens.  (28 heads of 256, us by one / by as many: 1 token 2.0 / 2.8, 16 2.0 / 2.7, 64 3.2 / 2.9, 148 4.9 / 3.3, 1000 27 / 16.5.)
+    const int64_t least = (items + ROPE_THREADS - 1) / ROPE_THREADS;
+    const int64_t most = ROPE_THREADS * (vec ? (n_tok * least <= 2 * SM_COUNT ? 1 : ROPE_MAX_ITEMS) : 4), parts = (items + most - 1) / most;
     if (parts > 65535 || items > INT32_MAX) return 1;
     const int per = (int)((items + parts - 1) / parts);
     const dim3 grid((unsigned)n_tok, (unsigned)parts);
@@ -2208,13 +2209,14 @@ int bonsai_b200_pages_write(const bonsai_b200_pages *pages, int layer, const flo
     P.amplitude = amplitude;
     P.eps = eps;
     const int64_t rows = (int64_t)n_head + 2 * (int64_t)P.C.n_head_kv;
-    // few tokens: a warp has one row; many: a CTA four tokens, up to 64 rows of each
+    // few rows: a warp has one; many: a CTA has up to 64 of two tokens, whose angles it forms once.  (32 rows a token, us, few / many: 1 token 3.5 / 6.7, 64 4.1 / 10.9, 300 9.2 / 12.5, 600 16.8 / 17.2,
+    // 1000 24.2 / 20.7, 3000 62.7 / 49.4.)
     auto run = [&](auto kernel, int tok, int each) {
         const int64_t groups = (rows + each - 1) / each;
         if (groups > 65535) return 1;
         return (int)launch(kernel, dim3((unsigned)((P.C.n_tok + tok - 1) / tok), (unsigned)groups), dim3(32 * PGW_WARPS), 0, as_stream(stream), true, P, each);
     };
-    if (P.C.n_tok * ((rows + PGW_WARPS - 1) / PGW_WARPS) <= 4 * SM_COUNT) return vec ? run(pages_write_kernel<true, 1>, 1, PGW_WARPS) : run(pages_write_kernel<false, 1>, 1, PGW_WARPS);
+    if (P.C.n_tok * ((rows + PGW_WARPS - 1) / PGW_WARPS) <= 16 * SM_COUNT) return vec ? run(pages_write_kernel<true, 1>, 1, PGW_WARPS) : run(pages_write_kernel<false, 1>, 1, PGW_WARPS);
     return vec ? run(pages_write_kernel<true, 2>, 2, 64) : run(pages_write_kernel<false, 2>, 2, 64);
 }
 
@@ -2275,7 +2277,8 @@ int bonsai_b200_pages_attn_shared(const bonsai_b200_pages *pages, int layer, con
     if (n_groups && (!group || !shared || !aligned4(group) || !aligned4(shared))) return 1;
     if (!workspace || !aligned16(workspace) || workspace_bytes < shared_bytes(pages, n_groups, n_head)) return 1;
     const int64_t out_rows = (int64_t)C.n_tok * n_head;
-    const int roww = out_rows <= 4 * SM_COUNT ? 8 : out_rows <= 32 * SM_COUNT ? 2 : 1;         // few rows have the more parts each, and leave warps free
+    const int roww = out_rows <= 4 * SM_COUNT ? 8 : out_rows <= 32 * SM_COUNT ? 2 : 1;
+    // (few rows have the more parts each, and leave warps free: whole calls by 8 / 2 / 1 warps a row, 384 rows 57 / 59 / 63 us, 1536 146 / 142 / 146, 4800 409 / 388 / 386, 16 900 447 / 382 / 370)
     const int64_t join_ctas = (out_rows * roww + PSJ_WARPS - 1) / PSJ_WARPS;
     if (join_ctas > INT32_MAX) return 1;
     const SharedPlan plan = plan_shared(C.n_tok, n_head, C.n_head_kv, C.n_pages, C.table_stride);

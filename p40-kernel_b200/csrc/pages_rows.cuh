@@ -36,7 +36,7 @@ __device__ __forceinline__ void page_row_load(const float *src, float (&x)[8]) {
     }
 }
 // Where value a of a row, or angle a of pairs of halves, lies in shared memory: the first four of each eight, then the other four, so that lanes which read eight
-// each read 16 bytes side by side.  (In their own order, one value a load, the banks of the 8 x 3 loads took 60 % of the kernel's time.)
+// each read 16 bytes side by side.  (In their own order, one value a load, the banks of the 8 x 3 loads took a third of the kernel's time: 2000 tokens 52.9 us, now 33.7.)
 template <int N>
 __device__ __forceinline__ int page_row_at(int a) {
     return (a >> 2 & 1) * (N / 2) + (a >> 3) * 4 + (a & 3);
@@ -120,7 +120,8 @@ __device__ __forceinline__ void page_row_store(const float (&x)[8], uint8_t *dst
     if (lane < KV_ROW / 16) reinterpret_cast<uint4 *>(dst)[lane] = reinterpret_cast<const uint4 *>(bytes)[lane];
 }
 
-// grid (tokens / TOK, groups of rows).  A CTA finds where its tokens go and forms their angles, then a warp has a row at a time (query heads, then k and v heads of a token; two, so that
+// grid (tokens / TOK, groups of rows).  What bounds it: a token's place and angles, a chain of three loads and sines in 64 bits, then issue slots (half of them)
+// and memory (0.54 of its rate).  A CTA finds where its tokens go and forms their angles, then a warp has a row at a time (query heads, then k and v heads of a token; two, so that
 // the next one's values are on their way), eight values a lane.  VEC: strides are multiples of 4, pointers (weights' too) 16-byte aligned.
 template <bool VEC, int TOK>
 __global__ void __launch_bounds__(32 * PGW_WARPS) pages_write_kernel(const __grid_constant__ PageWrite P, int rows_each) {
@@ -204,6 +205,7 @@ __global__ void __launch_bounds__(32 * PGW_WARPS) pages_write_kernel(const __gri
 }
 
 // ---- read: rows of a layer as floats ---------------------------------------------------------------------------------------------------------------
+// What bounds it: memory (35 003 rows of 4 heads to bf16 in 46 us, 0.72 of the copy rate).
 //   row start[s] + i of the outputs is position first[s] + i of sequence s: code times scale, one product, exact in fp32 and rounded once to fewer bits
 enum : int { ROWS_F32 = 0, ROWS_F16 = 1, ROWS_BF16 = 2 };
 struct PageRead {

@@ -107,7 +107,7 @@ def plain_rows(x, w, pos, freq, n_rot, pairs, amplitude, eps):
 
 ROWS = [  # lengths, new tokens, query heads, kv heads, rows of nobody
     ([1], [1], 24, 4, 0), ([65], [2], 3, 1, 3), ([200, 3, 64, 0, 129], [70, 3, 1, 0, 0], 24, 4, 2), ([40] * 30, [1] * 30, 8, 2, 0), ([700], [500], 24, 4, 1), ([130], [128], 0, 3, 0),
-    ([90], [90], 70, 2, 0), ([1, 64, 65], [1, 1, 1], 5, 5, 0)]
+    ([90], [90], 70, 2, 0), ([1300], [1201], 14, 1, 1), ([1, 64, 65], [1, 1, 1], 5, 5, 0)]
 
 
 @pytest.mark.parametrize("lens,new,n_head,n_head_kv,behind", ROWS)
