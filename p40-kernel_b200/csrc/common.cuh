@@ -274,6 +274,8 @@ __device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
+// Of n uses of m barriers in turn: how many were barrier c's.  (The last one's parity is one less than that, & 1.)
+__device__ __forceinline__ int in_turn(int n, int m, int c) { return (n + m - 1 - c) / m; }
 // 1-D bulk copy global -> shared of `bytes` (multiple of 16, both addresses 16-byte aligned),
 // completion counted on `bar`.
 __device__ __forceinline__ void bulk_g2s(void *dst, const void *src, uint32_t bytes, uint64_t *bar, uint64_t policy) {

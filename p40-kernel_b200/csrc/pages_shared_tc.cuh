@@ -27,7 +27,8 @@ struct PstFragment {
 constexpr int PST_THREADS = ATC_THREADS + 128, PST_SCORE_WARP = ATC_WARPS, PST_V_WARP = ATC_WARPS + 2, PST_OUT_WARP = ATC_WARPS + 3;      // (and k's pages)
 constexpr int PST_REGS_ROWS = 104, PST_REGS_REST = 64;           // 4 x 104 + 64 = 5 x 96, what the launch has
 constexpr int PST_REGS = 32 * (ATC_WARPS * PST_REGS_ROWS + 4 * PST_REGS_REST);
-constexpr int PST_SMEM_BYTES = 1024 + 3 * ATC_PLANES + (2 * ATC_KEYS + 2 * ATT_D + 2 * 4 * ATC_M) * 4 + 208 + 2 * (int)sizeof(PstFragment);
+constexpr int PST_BARS = 22;
+constexpr int PST_SMEM_BYTES = 1024 + 3 * ATC_PLANES + (2 * ATC_KEYS + 2 * ATT_D + 2 * 4 * ATC_M) * 4 + 8 * PST_BARS + 16 + 2 * (int)sizeof(PstFragment) + 8;
 constexpr int PST_IMG_BAD = ATC_IMG_RANGE + 16;                  // 8 bytes of an image: positions whose v is no number
 static_assert(PST_IMG_BAD + 8 <= ATC_IMG_BYTES && PST_ROWS == ATC_M && PG_POS == ATC_KEYS && KV_D == ATT_D, "");
 __device__ __forceinline__ void pst_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(ATC_THREADS) : "memory"); }        // among the threads that have rows
@@ -135,18 +136,35 @@ __global__ void __launch_bounds__(ATC_PREP_THREADS) pages_shared_planes_kernel(c
 // The warps without rows: one issues the products of scores, one says what the fragments are and issues those of outputs, two copy images.
 __device__ __forceinline__ void pst_drivers(const PageShared &P, PstFragment *desc, uint8_t *qhi, uint8_t *kpl, uint8_t *vpl, float *kf, float *vf, uint64_t *qk, unsigned long long *bad,
                                             volatile int *failed, uint32_t tmem) {
-    uint64_t *pv = qk + 1, *scored = qk + 2, *weighed = qk + 3, *vfull = qk + 4, *kfull = qk + 6, *kfree = qk + 10, *ffull = qk + 14, *vfree = qk + 16, *gfull = qk + 18;
+    uint64_t *pv = qk + 1, *scored = qk + 2, *weighed = qk + 3, *vfull = qk + 4, *kfull = qk + 6, *kfree = qk + 10, *ffull = qk + 14, *vfree = qk + 16, *gfull = qk + 18, *done = qk + 20;
     const PshPlan &plan = *P.plan;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, heads = P.C.n_head_kv, entities = P.n_groups + P.C.n_seq;
     const size_t img_stride = (size_t)heads * ATC_IMG_BYTES;
+    // After a wait that ran out a warp waits for nothing more, copies nothing and issues nothing.  What it has begun ends before the CTA does: tensor memory is given back then, and shared
+    // memory becomes another CTA's.
     bool ok = true;
     auto wait = [&](uint64_t *bar, uint32_t parity) { ok = ok && __all_sync(0xffffffffu, psh_wait<true>(bar, parity)); };
+    auto copies_end = [&](int begun, uint64_t *full, int parts, uint64_t *factors) {
+#pragma unroll 1
+        for (int c = 0; c < parts; ++c)
+            if (begun > c) psh_wait<true>(full + c, (uint32_t)((in_turn(begun, parts, c) - 1) & 1));
+        const int pages = in_turn(begun, parts, 0);
+#pragma unroll 1
+        for (int c = 0; c < 2; ++c)
+            if (pages > c) psh_wait<true>(factors + c, (uint32_t)((in_turn(pages, 2, c) - 1) & 1));
+    };
+    auto products_end = [&](uint64_t *bar) {
+        if (elect_one()) tc_commit(bar);
+        __syncwarp();
+        psh_wait<true>(bar, 0);
+    };
     // 64 dims of k, 128 of v give their place to the next page's when they are done.  (Waits between the products cost 250 cycles each, and nothing is multiplied meanwhile.)
     auto issue_qk = [&](int it) {
         constexpr uint32_t LOW = (ATC_KEYS * 128) >> 4;
         const uint32_t a0 = tc16_desc_lo(smem_u32(qhi)), b0 = tc16_desc_lo(smem_u32(kpl)), d = tmem + PST_COL_S;
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) wait(kfull + c, (uint32_t)(it & 1));
+        if (!ok) return;
         tc_fence_after();
         if (elect_one()) {
 #pragma unroll
@@ -170,6 +188,7 @@ __device__ __forceinline__ void pst_drivers(const PageShared &P, PstFragment *de
         const uint32_t b0 = tc16_desc_lo(smem_u32(vpl)), ph = tmem + PST_COL_P, pl = ph + 32u;
         wait(vfull, (uint32_t)(it & 1));
         wait(vfull + 1, (uint32_t)(it & 1));
+        if (!ok) return;
         tc_fence_after();
         if (elect_one()) {
 #pragma unroll
@@ -227,12 +246,12 @@ __device__ __forceinline__ void pst_drivers(const PageShared &P, PstFragment *de
         for (int f = 0;; ++f) {
             __syncthreads();
             const int ntiles = F.ntiles;
-            if (ntiles == 0 || *failed) return;
+            if (ntiles == 0 || *failed) break;
             next(F);                                     // (its place is the last one's, which everybody has left)
             if (lane == 0) desc[(f + 1) & 1] = F;
             __syncthreads();
 #pragma unroll 1
-            for (int i = 0; i < ntiles; ++i, ++it) {     // outputs
+            for (int i = 0; i < ntiles && ok; ++i, ++it) {         // outputs
                 wait(weighed, (uint32_t)(it & 1));
                 issue_pv(it);
             }
@@ -240,65 +259,81 @@ __device__ __forceinline__ void pst_drivers(const PageShared &P, PstFragment *de
             __syncthreads();
             __syncthreads();
         }
+        products_end(done);
+        return;
     }
-    int it0 = 0;                                         // pages of the fragments before
-    for (int f = 0;; ++f) {
-        __syncthreads();
-        const int ntiles = desc[f & 1].ntiles;
-        const uint8_t *img = desc[f & 1].img;
-        if (ntiles == 0 || *failed) return;
-        __syncthreads();
-        if (warp == PST_SCORE_WARP) {
+    // the fragments one after the other: a warp's part of n pages, their images from img on
+    auto fragments = [&](auto part) {
+        for (int f = 0;; ++f) {
+            __syncthreads();
+            const int ntiles = desc[f & 1].ntiles;
+            const uint8_t *img = desc[f & 1].img;
+            if (ntiles == 0 || *failed) break;
+            __syncthreads();
+            part(ntiles, img);
+            if (!ok) *failed = 1;
+            __syncthreads();
+            __syncthreads();
+        }
+    };
+    if (warp == PST_SCORE_WARP) {
+        int it = 0;
+        fragments([&](int n, const uint8_t *) {
 #pragma unroll 1
-            for (int i = 0; i < ntiles; ++i) {           // scores
-                const int it = it0 + i;
+            for (int i = 0; i < n && ok; ++i, ++it) {    // scores
                 if (it > 0) wait(scored, (uint32_t)((it - 1) & 1));
                 issue_qk(it);
             }
-        } else {
-            const uint64_t pol = policy_evict_last_or_default();
+        });
+        products_end(done + 1);
+    } else if (warp == PST_V_WARP) {
+        const uint64_t pol = policy_evict_last_or_default();
+        int begun = 0;                                   // parts of pages
+        fragments([&](int n, const uint8_t *img) {
 #pragma unroll 1
-            for (int i = 0; i < ntiles; ++i, img += img_stride) {
-                const int it = it0 + i;
-                if (warp == PST_V_WARP) {
-#pragma unroll 1
-                    for (int c = 0; c < 2; ++c) {
-                        if (it > 0) wait(vfree + c, (uint32_t)((it - 1) & 1));
-                        if (lane == 0) {
-                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");         // the factors were read by ordinary loads
-                            if (c == 0) {                // (their place is the page's before the last: its outputs were added in front of the weights that page `it - 1` waited for)
-                                bad[it & 1] = *reinterpret_cast<const unsigned long long *>(img + PST_IMG_BAD);
-                                mbar_expect_tx(gfull + (it & 1), ATT_D * 4);
-                                bulk_g2s(vf + (it & 1) * ATT_D, img + ATC_IMG_VF, ATT_D * 4, gfull + (it & 1), pol);
-                            }
-                            mbar_expect_tx(vfull + c, 2 * ATC_CHUNK);
-                            bulk_g2s(vpl + c * ATC_CHUNK, img + ATC_PLANES + c * ATC_CHUNK, ATC_CHUNK, vfull + c, pol);
-                            bulk_g2s(vpl + (2 + c) * ATC_CHUNK, img + ATC_PLANES + (2 + c) * ATC_CHUNK, ATC_CHUNK, vfull + c, pol);
-                        }
-                        __syncwarp();
+            for (int i = 0; i < 2 * n; ++i, ++begun) {
+                const int it = begun >> 1, c = begun & 1;
+                if (it > 0) wait(vfree + c, (uint32_t)((it - 1) & 1));
+                if (!ok) break;
+                if (lane == 0) {
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");         // the factors were read by ordinary loads
+                    if (c == 0) {                        // (their place is the page's before the last: its outputs were added in front of the weights that page `it - 1` waited for)
+                        bad[it & 1] = *reinterpret_cast<const unsigned long long *>(img + PST_IMG_BAD);
+                        mbar_expect_tx(gfull + (it & 1), ATT_D * 4);
+                        bulk_g2s(vf + (it & 1) * ATT_D, img + ATC_IMG_VF, ATT_D * 4, gfull + (it & 1), pol);
                     }
-                    continue;
+                    mbar_expect_tx(vfull + c, 2 * ATC_CHUNK);
+                    bulk_g2s(vpl + c * ATC_CHUNK, img + ATC_PLANES + c * ATC_CHUNK, ATC_CHUNK, vfull + c, pol);
+                    bulk_g2s(vpl + (2 + c) * ATC_CHUNK, img + ATC_PLANES + (2 + c) * ATC_CHUNK, ATC_CHUNK, vfull + c, pol);
                 }
-#pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
-                    if (it > 0) wait(kfree + c, (uint32_t)((it - 1) & 1));
-                    if (lane == 0) {
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                        if (c == 0) {
-                            mbar_expect_tx(ffull + (it & 1), ATC_KEYS * 4);
-                            bulk_g2s(kf + (it & 1) * ATC_KEYS, img + ATC_IMG_KF, ATC_KEYS * 4, ffull + (it & 1), pol);
-                        }
-                        mbar_expect_tx(kfull + c, ATC_CHUNK);
-                        bulk_g2s(kpl + c * ATC_CHUNK, img + c * ATC_CHUNK, ATC_CHUNK, kfull + c, pol);
-                    }
-                    __syncwarp();
-                }
+                __syncwarp();
+                if (c == 1) img += img_stride;
             }
-        }
-        it0 += ntiles;
-        if (!ok) *failed = 1;
-        __syncthreads();
-        __syncthreads();
+        });
+        copies_end(begun, vfull, 2, gfull);
+    } else {
+        const uint64_t pol = policy_evict_last_or_default();
+        int begun = 0;
+        fragments([&](int n, const uint8_t *img) {
+#pragma unroll 1
+            for (int i = 0; i < 4 * n; ++i, ++begun) {
+                const int it = begun >> 2, c = begun & 3;
+                if (it > 0) wait(kfree + c, (uint32_t)((it - 1) & 1));
+                if (!ok) break;
+                if (lane == 0) {
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    if (c == 0) {
+                        mbar_expect_tx(ffull + (it & 1), ATC_KEYS * 4);
+                        bulk_g2s(kf + (it & 1) * ATC_KEYS, img + ATC_IMG_KF, ATC_KEYS * 4, ffull + (it & 1), pol);
+                    }
+                    mbar_expect_tx(kfull + c, ATC_CHUNK);
+                    bulk_g2s(kpl + c * ATC_CHUNK, img + c * ATC_CHUNK, ATC_CHUNK, kfull + c, pol);
+                }
+                __syncwarp();
+                if (c == 3) img += img_stride;
+            }
+        });
+        copies_end(begun, kfull, 4, ffull);
     }
 }
 // The warps with rows.
@@ -514,15 +549,15 @@ __global__ void __launch_bounds__(PST_THREADS, 1) pages_shared_tc_kernel(const _
     float *kf = reinterpret_cast<float *>(vpl + ATC_PLANES);             // [2][64] 2^-s of the page's positions, pages alternate
     float *vf = kf + 2 * ATC_KEYS;                                       // [2][256] 2^-s of the dims (and the weights' 2^-14)
     float *red0 = vf + 2 * ATT_D;                                        // [2][4][128] exchange between the four warps of a row, pages alternate
-    uint64_t *qk = reinterpret_cast<uint64_t *>(red0 + 2 * 4 * ATC_M);               // scores there, outputs there, scores read, weights there; k and v, by 64 and 128 dims, there and free; factors
-    unsigned long long *bad = reinterpret_cast<unsigned long long *>(qk + 20);         // [2] positions of the page whose v is no number
+    uint64_t *qk = reinterpret_cast<uint64_t *>(red0 + 2 * 4 * ATC_M);               // scores there, outputs there, scores read, weights there; k and v, by 64 and 128 dims, there and free; factors; all products done
+    unsigned long long *bad = reinterpret_cast<unsigned long long *>(qk + PST_BARS);        // [2] positions of the page whose v is no number
     PstFragment *desc = reinterpret_cast<PstFragment *>(bad + 2);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(desc + 2);
     volatile int *failed = reinterpret_cast<int *>(tmem_slot + 1);
 
     const int warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) {
-        for (int b = 0; b < 20; ++b) mbar_init(qk + b, b == 2 || b == 3 ? ATC_WARPS : 1);
+        for (int b = 0; b < PST_BARS; ++b) mbar_init(qk + b, b == 2 || b == 3 ? ATC_WARPS : 1);
         mbar_fence_init();
         *failed = 0;
     }
