@@ -30,7 +30,7 @@ namespace b200 {
 
 constexpr uint32_t PTC_COL_O = 0, PTC_COL_S = 256, PTC_COL_P = 320, PTC_COL_QL = 384;
 constexpr int PTC_THREADS = ATC_THREADS + 96;
-constexpr int PTC_SMEM_BYTES = 1024 + 3 * ATC_PLANES + (2 * ATC_KEYS + 2 * ATT_D + 2 * 4 * ATC_M) * 4 + 128;
+constexpr int PTC_SMEM_BYTES = 1024 + 3 * ATC_PLANES + (2 * ATC_KEYS + 2 * ATT_D + 2 * 4 * ATC_M) * 4 + 192;
 // Among the threads that have rows.
 __device__ __forceinline__ void ptc_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(ATC_THREADS) : "memory"); }
 static_assert(PG_POS == ATC_KEYS && KV_D == ATT_D && PTC_ROWS == ATC_M, "");
@@ -154,9 +154,10 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) pages_tc_kernel(const __grid_c
     float *vf = kf + 2 * ATC_KEYS;                                       // [2][256] 2^-s of the dims (and the weights' 2^-14)
     float *red0 = vf + 2 * ATT_D;                                        // [2][4][128] exchange between the four warps of a row, pages alternate
     // pages alternate between two barriers of the copies: a phase ends when everybody has long waited for the one before
-    uint64_t *qk = reinterpret_cast<uint64_t *>(red0 + 2 * 4 * ATC_M), *pv = qk + 1, *scored = qk + 2, *weighed = qk + 3, *kfull = qk + 4, *vfull = qk + 6;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(vfull + 2);
+    uint64_t *qk = reinterpret_cast<uint64_t *>(red0 + 2 * 4 * ATC_M), *pv = qk + 1, *scored = qk + 2, *weighed = qk + 3, *kfull = qk + 4, *vfull = qk + 6, *done = qk + 8;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(done + 1);
     volatile int *failed = reinterpret_cast<int *>(tmem_slot + 1);
+    uint32_t *seen = tmem_slot + 2;                                      // [16] magnitude bits of a warp's rows' largest q
 
     const PageCache &C = P.C;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -193,7 +194,7 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) pages_tc_kernel(const __grid_c
     };
 
     if (threadIdx.x == 0) {
-        for (int b = 0; b < 8; ++b) mbar_init(qk + b, b == 2 || b == 3 ? ATC_WARPS : 1);
+        for (int b = 0; b < 9; ++b) mbar_init(qk + b, b == 2 || b == 3 ? ATC_WARPS : 1);
         mbar_fence_init();
         *failed = 0;
     }
@@ -225,7 +226,6 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) pages_tc_kernel(const __grid_c
     float4 *box = reinterpret_cast<float4 *>(kpl) + warp * 512;
     const int row0 = 32 * (warp & 3);
     float qf = 0.0f;
-    uint32_t seen = 0;                                                   // magnitude bits of the row's largest q
     __syncthreads();                                                     // the barriers, and where tensor memory is
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
@@ -266,33 +266,43 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) pages_tc_kernel(const __grid_c
     };
     if (driver) {
         __syncthreads();                                                 // q is in its places
-        bool ok = true;                                                  // after a wait that ran out nothing is waited for any more: the CTA comes to its end, and says so
+        // After a wait that ran out a warp waits for nothing more, copies nothing and issues nothing: the CTA comes to its end, and says so.  What was begun ends first: tensor
+        // memory is given back then, and shared memory becomes another CTA's.
+        bool ok = true;
         auto wait = [&](uint64_t *bar, uint32_t parity) { ok = ok && __all_sync(0xffffffffu, mbar_wait_try(bar, parity)); };
+        int i = 0;
         if (warp == ATC_WARPS) {
-            for (int i = 0; i <= ntiles && ntiles > 0; ++i) {            // scores of page i, outputs of page i - 1
+            for (; i <= ntiles && ntiles > 0; ++i) {                     // scores of page i, outputs of page i - 1
                 if (i < ntiles) {
                     if (i > 0) wait(scored, (uint32_t)((i - 1) & 1));
                     wait(kfull + (i & 1), (uint32_t)((i >> 1) & 1));
+                    if (!ok) break;
                     issue_qk();
                 }
                 if (i > 0) {
                     wait(weighed, (uint32_t)((i - 1) & 1));
                     wait(vfull + ((i - 1) & 1), (uint32_t)(((i - 1) >> 1) & 1));
+                    if (!ok) break;
                     issue_pv();
                 }
             }
-        } else if (warp == ATC_WARPS + 1) {
-            for (int i = 0; i < ntiles; ++i) {                           // k when the scores of the page before have been read
-                if (i > 0) wait(scored, (uint32_t)((i - 1) & 1));
-                if (lane == 0) load_k(i);
-                __syncwarp();
-            }
+            if (elect_one()) tc_commit(done);
+            __syncwarp();
+            mbar_wait_try(done, 0);
         } else {
-            for (int i = 0; i < ntiles; ++i) {                           // v when the outputs of the page before are there
-                if (i > 0) wait(pv, (uint32_t)((i - 1) & 1));
-                if (lane == 0) load_v(i);
+            uint64_t *const full = warp == ATC_WARPS + 1 ? kfull : vfull;
+            for (; i < ntiles; ++i) {                                    // k when the scores of the page before have been read, v when the outputs of the page before are there
+                if (i > 0) wait(warp == ATC_WARPS + 1 ? scored : pv, (uint32_t)((i - 1) & 1));
+                if (!ok) break;
+                if (lane == 0) {
+                    if (warp == ATC_WARPS + 1) load_k(i);
+                    else load_v(i);
+                }
                 __syncwarp();
             }
+            // the last copy of each of the two barriers
+            if (i > 0) mbar_wait_try(full + ((i - 1) & 1), (uint32_t)(((i - 1) >> 1) & 1));
+            if (i > 1) mbar_wait_try(full + (i & 1), (uint32_t)(((i - 2) >> 1) & 1));
         }
         if (!ok) *failed = 1;
         __syncthreads();
@@ -337,7 +347,10 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) pages_tc_kernel(const __grid_c
         ptc_barrier();
 #pragma unroll
         for (int c = 0; c < 4; ++c) m = max(m, redu[c * ATC_M + row]);
-        seen = m;
+        {
+            const uint32_t most = __reduce_max_sync(0xffffffffu, m);
+            if (lane == 0) seen[warp] = most;
+        }
         const int s = atc_shift(m, 63);
         qf = __fmul_rn(atc_pow2(-s), P.scale);
         uint32_t lo32[32];
@@ -449,11 +462,10 @@ __global__ void __launch_bounds__(PTC_THREADS, 1) pages_tc_kernel(const __grid_c
         v_least = min(v_least, r[2]);
     }
     uint4 *ranges = reinterpret_cast<uint4 *>(kf);                       // a warp each; every page's factors have been read
-    seen = __reduce_max_sync(0xffffffffu, seen);
     k_most = __reduce_max_sync(0xffffffffu, k_most);
     v_most = __reduce_max_sync(0xffffffffu, v_most);
     v_least = __reduce_min_sync(0xffffffffu, v_least);
-    if (lane == 0) ranges[warp] = make_uint4(seen, k_most, v_most, v_least);
+    if (lane == 0) ranges[warp] = make_uint4(seen[warp], k_most, v_most, v_least);
     ptc_barrier();
     const bool all_ok = *failed == 0;
     const uint4 r = ranges[lane & (ATC_WARPS - 1)];

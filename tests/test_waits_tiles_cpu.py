@@ -54,3 +54,17 @@ def test_shared_pages():
     used = [b for first, n in at for b in range(first, first + size.get(n, 1))]
     bars = int(re.search(r"PST_BARS = (\d+)", open(os.path.join(CSRC, "pages_shared_tc.cuh")).read())[1])
     assert sorted([0, *used]) == list(range(bars))
+
+
+def test_pages_of_one_sequence():
+    text = body("pages_tc_kernel")
+    driver = text[text.index("if (driver) {"):]
+    driver = driver[:driver.index("return;\n    }\n    {")]
+    assert looked_at(driver, r"\b(?:load_[kv]|issue_(?:qk|pv))\(") == 4
+    assert re.search(r"tc_commit\(done\);\s*__syncwarp\(\);\s*mbar_wait_try\(done, 0\);", driver)
+    # the last copy of each barrier, by its parity: copy i is use i >> 1 of barrier i & 1
+    ends = re.findall(r"if \(i > (\d)\) mbar_wait_try\(full \+ (\(.*?\)), \(uint32_t\)\((.*?)\)\);", driver)
+    for i in range(12):
+        last = {j & 1: (j >> 1) & 1 for j in range(i)}
+        assert {eval(bar, {"i": i}): eval(parity, {"i": i}) for least, bar, parity in ends if i > int(least)} == last
+    assert "*done = qk + 8;" in text and "b < 9" in text and "done + 1" in text
