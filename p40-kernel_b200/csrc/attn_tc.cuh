@@ -231,8 +231,8 @@ __global__ void __launch_bounds__(ATC_THREADS, 1) attn_tc_kernel(const float *q,
     float *kf = reinterpret_cast<float *>(vpl + ATC_PLANES);             // [2][64] 2^-s of the tile's keys, tiles alternate
     float *vf = kf + 2 * ATC_KEYS;                                       // [2][256] 2^-s of the dims (and the weights' 2^-14)
     float *red = vf + 2 * ATT_D;                                         // [4][128] exchange between the four warps of a row
-    uint64_t *qk = reinterpret_cast<uint64_t *>(red + 4 * ATC_M), *pv = qk + 1, *kfull = qk + 2, *vfull = qk + 3;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(vfull + 1);
+    uint64_t *qk = reinterpret_cast<uint64_t *>(red + 4 * ATC_M), *pv = qk + 1, *kfull = qk + 2, *vfull = qk + 3, *done = qk + 4;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(done + 1);
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int cg = warp >> 2, row = 32 * (warp & 3) + lane;              // a thread's row, and its quarter of the row's columns
@@ -246,6 +246,7 @@ __global__ void __launch_bounds__(ATC_THREADS, 1) attn_tc_kernel(const float *q,
     if (threadIdx.x == 0) {
         mbar_init(qk, 2);                                                // an arrival of each issuing warp
         for (int b = 1; b < 4; ++b) mbar_init(qk + b, 1);
+        mbar_init(done, 2);
         mbar_fence_init();
     }
     if (warp == 0) {
@@ -344,28 +345,30 @@ __global__ void __launch_bounds__(ATC_THREADS, 1) attn_tc_kernel(const float *q,
 #pragma unroll
         for (int n = N0; n < N0 + STEPS; ++n) atc_mma_ss<atc_idesc(ATC_KEYS)>(d, a0 + at(n), b0 + at(n));
     };
+    // After a wait that ran out a thread copies and issues nothing more, and the CTA leaves as a whole when what was begun has ended.
+    bool ok = true;
     // Two warps issue the scores' products, half of the sums each: from one warp 16 dims take 39 (q low) or 55 cycles, and its chain of waits and
     // issues is not overlapped.  (One warp, a barrier for each half of the dims, waits polled back to back: 2048 tokens 287 us, 600 tokens 60.6;
     // with two 279 and 58.9, when queries and outputs still went by a row per thread.)
     auto issue_qk_a = [&] {                                              // dims 0 .. 63, two sums, into the score columns
         tc_fence_after();
         if (warp == 0) {
-            if (elect_one()) sum_of(tmem + ATC_COL_S, std::integral_constant<int, 0>{}, std::integral_constant<int, 2>{});
+            if (elect_one() && ok) sum_of(tmem + ATC_COL_S, std::integral_constant<int, 0>{}, std::integral_constant<int, 2>{});
         } else {
-            if (elect_one()) sum_of(tmem + ATC_COL_S + ATC_KEYS, std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{});
+            if (elect_one() && ok) sum_of(tmem + ATC_COL_S + ATC_KEYS, std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{});
         }
         __syncwarp();
     };
     auto issue_qk_b = [&] {                                              // dims 64 .. 255, four sums, into the output columns; the commit covers the others too
         tc_fence_after();
         if (warp == 0) {
-            if (elect_one()) {
+            if (elect_one() && ok) {
                 sum_of(tmem + ATC_COL_O, std::integral_constant<int, 4>{}, std::integral_constant<int, 3>{});
                 sum_of(tmem + ATC_COL_O + ATC_KEYS, std::integral_constant<int, 7>{}, std::integral_constant<int, 3>{});
                 tc_commit(qk);
             }
         } else {
-            if (elect_one()) {
+            if (elect_one() && ok) {
                 sum_of(tmem + ATC_COL_O + 2 * ATC_KEYS, std::integral_constant<int, 10>{}, std::integral_constant<int, 3>{});
                 sum_of(tmem + ATC_COL_O + 3 * ATC_KEYS, std::integral_constant<int, 13>{}, std::integral_constant<int, 3>{});
                 tc_commit(qk);
@@ -376,7 +379,7 @@ __global__ void __launch_bounds__(ATC_THREADS, 1) attn_tc_kernel(const float *q,
     auto issue_pv = [&] {
         tc_fence_after();
         const uint32_t b0 = tc16_desc_lo(smem_u32(vpl)), ph = tmem + ATC_COL_S, pl = ph + 32u;
-        if (elect_one()) {
+        if (elect_one() && ok) {
 #pragma unroll
             for (int n = 0; n < 12; ++n) {
                 const uint32_t a = (n < 4 ? pl : ph) + (uint32_t)(8 * (n & 3));
@@ -398,7 +401,6 @@ __global__ void __launch_bounds__(ATC_THREADS, 1) attn_tc_kernel(const float *q,
     tc_st_wait();
     tc_fence_before();
     __syncthreads();
-    bool ok = true;
     if (warp < 2) {
         ok = mbar_wait_try(kfull, 0);
         issue_qk_a();
@@ -461,7 +463,7 @@ __global__ void __launch_bounds__(ATC_THREADS, 1) attn_tc_kernel(const float *q,
         }
         red[cg * ATC_M + row] = mx;
         tc_fence_before();
-        if (!__syncthreads_and(ok ? 1 : 0)) break;                       // (a wait ran out: the CTA leaves as a whole)
+        if (!__syncthreads_and(ok ? 1 : 0)) break;                       // (a wait ran out)
         tc_fence_after();                                                // every score has been read: the weights take their place
         // (a barrier's next phase is begun only when the whole CTA has waited for this one: a thread that came later than a
         // phase's successor would wait for a parity that has passed)
@@ -492,7 +494,7 @@ __global__ void __launch_bounds__(ATC_THREADS, 1) attn_tc_kernel(const float *q,
         ok = mbar_wait_try(pv, par) && ok;
         tc_fence_after();
         if (i + 1 < ntiles) {
-            if (warp == 4 && lane == 0) load_v(i + 1);
+            if (warp == 4 && lane == 0 && ok) load_v(i + 1);
             if (warp < 2) {
                 ok = mbar_wait_try(kfull, par ^ 1u) && ok;
                 issue_qk_a();
@@ -505,7 +507,20 @@ __global__ void __launch_bounds__(ATC_THREADS, 1) attn_tc_kernel(const float *q,
             if (warp < 2) issue_qk_b();
         }
     }
-    __syncthreads();
+    if (!__syncthreads_and(ok ? 1 : 0)) {
+        if (warp < 2) {
+            if (elect_one()) tc_commit(done);
+            __syncwarp();
+            mbar_wait_try(done, 0);
+        }
+        if ((warp == 4 || warp == 5) && lane == 0) {
+            // whichever phase is the last one begun (a barrier without a copy in flight lets one of the waits run out; counting the copies cost 1 % of a call)
+            uint64_t *const full = warp == 4 ? kfull : vfull;
+            mbar_wait_try(full, 0);
+            mbar_wait_try(full, 1);
+        }
+        __syncthreads();
+    }
     red[cg * ATC_M + row] = l_run;
     tc_fence_before();
     uint32_t k_most = 0, v_most = 0, v_least = ATC_NONE;

@@ -68,3 +68,17 @@ def test_pages_of_one_sequence():
         last = {j & 1: (j >> 1) & 1 for j in range(i)}
         assert {eval(bar, {"i": i}): eval(parity, {"i": i}) for least, bar, parity in ends if i > int(least)} == last
     assert "*done = qk + 8;" in text and "b < 9" in text and "done + 1" in text
+
+
+def test_a_prompt_by_itself():
+    text = body("attn_tc_kernel")
+    loop = text[text.index("for (int i = 0; i < ntiles; ++i)"):]
+    end = loop.index("if (!__syncthreads_and(ok ? 1 : 0)) {")
+    # products and copies: by a thread none of whose waits has run out, or behind a barrier that says so of all
+    assert re.search(r"[^\n]*load_v\(i \+ 1\)", loop[:end])[0].count("&& ok)") == 1
+    assert text.count("if (elect_one() && ok)") == 5 and text.count("elect_one()") == 6
+    assert loop.index("if (!__syncthreads_and(ok ? 1 : 0)) break;") < loop.index("load_k(i + 1)")
+    way_out = loop[end:loop.index("red[cg * ATC_M + row] = l_run;")]
+    assert re.search(r"tc_commit\(done\);\s*__syncwarp\(\);\s*mbar_wait_try\(done, 0\);", way_out) and way_out.rstrip().endswith("__syncthreads();\n    }")
+    assert "mbar_init(done, 2);" in text
+    assert re.findall(r"mbar_wait_try\(full, (\d)\)", way_out) == ["0", "1"] and "warp == 4 ? kfull : vfull" in way_out
