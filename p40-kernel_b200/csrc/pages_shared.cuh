@@ -408,9 +408,10 @@ struct PshLoader {
             const bool there = page >= 0 && page < C.n_pages;
             if (!there && lane == 0) bad_sequence();
             if (n >= SLOTS) wait(&empties[j], (uint32_t)((n / SLOTS - 1) & 1));
-            if (lane == 0) {                             // (a wait that ran out: nothing is copied, but those who wait for it are let go)
-                helds[j] = there && wait.ok ? rows : 0;
-                if (there && wait.ok) {
+            if (!wait.ok) break;                         // (the slot's last copy may be in flight: nothing is counted on its barrier then)
+            if (lane == 0) {
+                helds[j] = there ? rows : 0;
+                if (there) {
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     mbar_expect_tx(&fulls[j], (uint32_t)rows * KV_ROW);
                     bulk_g2s(raw + j * PG_HEAD_BYTES, page_rows(C, page, P.layer, KV, F.kvh), (uint32_t)rows * KV_ROW, &fulls[j], policy_evict_normal());
@@ -445,6 +446,7 @@ __device__ __forceinline__ void psh_plan_warp(const PageShared &P, PshSmall &S, 
     int said = 0;
     auto say = [&](const PshFragment &F) {
         if (said >= PSH_DESCS) wait(&S.dempty[said % PSH_DESCS], (uint32_t)((said / PSH_DESCS - 1) & 1));
+        if (!wait.ok) return;                            // (somebody may be reading what lies there; who waits for the next one gives up as well)
         if (lane == 0) {
             S.desc[said % PSH_DESCS] = F;
             mbar_arrive(&S.dfull[said % PSH_DESCS]);

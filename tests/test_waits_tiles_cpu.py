@@ -82,3 +82,16 @@ def test_a_prompt_by_itself():
     assert re.search(r"tc_commit\(done\);\s*__syncwarp\(\);\s*mbar_wait_try\(done, 0\);", way_out) and way_out.rstrip().endswith("__syncthreads();\n    }")
     assert "mbar_init(done, 2);" in text
     assert re.findall(r"mbar_wait_try\(full, (\d)\)", way_out) == ["0", "1"] and "warp == 4 ? kfull : vfull" in way_out
+
+
+def test_pages_in_slots():
+    """A barrier that counts a copy is arrived at once a phase, and what a fragment is said to be is not written over while it may be read: neither behind a wait that ran out."""
+    source = open(os.path.join(CSRC, "pages_shared.cuh")).read()
+    load = source[source.index("__device__ __forceinline__ void load(const PshFragment &F)"):]
+    load = load[:load.index("void end()")]
+    wait = load.index("wait(&empties[j]")
+    look = load.index("if (!wait.ok) break;", wait)
+    assert all(look < load.index(x) for x in ("mbar_expect_tx(&fulls[j]", "mbar_arrive(&fulls[j])", "bulk_g2s(")) and "++p, ++n)" in load[:wait]
+    say = body("psh_plan_warp")
+    say = say[say.index("auto say = "):]
+    assert say.index("wait(&S.dempty") < say.index("if (!wait.ok) return;") < say.index("S.desc[said % PSH_DESCS] = F;")
