@@ -273,7 +273,7 @@ int bonsai_b200_kv_splits(int n_pos, int resident8, int resident16, int64_t out[
  * (row[i], row[i + n_rot / 2]), i < n_rot / 2, turned by the angle pos[token] * freq[i]; values from n_rot on are not turned.  q holds n_tok x n_head
  * rows of head_dim floats (1 .. 256; n_rot even, at most head_dim) at token * q_tok_stride + head * q_head_stride floats, k likewise n_head_kv: a
  * projection that also gives something else per head needs no copy.  Rows may not overlap.  q_out, k_out are packed [n_tok][heads][head_dim]; they
- * may be q and k where those are packed too, and may not overlap the inputs in any other way.  Weights have head_dim floats; pos is int32, freq
+ * may be q and k where those are packed too, and may not overlap the inputs in any other way, nor each other.  Weights have head_dim floats; pos is int32, freq
  * double (radians per position, n_rot / 2 of them, up to 1): the angle is formed in 64 bits, however far the position.  n_head or n_head_kv may be 0.  Returns 1 for
  * sizes and strides that are not those, 0 without a launch if n_tok <= 0. */
 int bonsai_b200_qk_norm_rope(const float *q, const float *k, const float *q_weight, const float *k_weight, const int32_t *pos, const double *freq, float *q_out,

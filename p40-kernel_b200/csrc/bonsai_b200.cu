@@ -1986,6 +1986,7 @@ int bonsai_b200_qk_norm_rope(const float *q, const float *k, const float *q_weig
     const int heads = n_head + n_head_kv;
     if (n_tok <= 0 || heads == 0) return 0;
     if (n_tok > INT32_MAX || (n_rot && (!pos || !freq || !aligned4(pos) || !aligned8(freq)))) return 1;
+    if (n_head && n_head_kv && q_out == k_out) return 1;
     QkNormParams P = {{q, k}, {q_weight, k_weight}, {q_out, k_out}, {q_tok_stride, k_tok_stride}, {q_head_stride, k_head_stride}, pos, freq, {n_head, n_head_kv}, head_dim, n_rot, 1.0f / (float)head_dim, eps};
     bool vec = head_dim % 4 == 0;
     for (int i = 0; i < 2; ++i) {
@@ -2149,6 +2150,7 @@ int bonsai_b200_rope(const float *q, const float *k, const int32_t *pos, const d
     const int heads = n_head + n_head_kv;
     if (n_tok <= 0 || heads == 0) return 0;
     if (n_tok > INT32_MAX || (n_rot && (!pos || !aligned4(pos)))) return 1;
+    if (n_head && n_head_kv && q_out == k_out) return 1;
     const RopeParams P = {{q, k}, {q_out, k_out}, {q_tok_stride, k_tok_stride}, {q_head_stride, k_head_stride}, pos, freq, {n_head, n_head_kv}, head_dim, n_rot, pairs, amplitude};
     bool vec = head_dim % 8 == 0 && n_rot % 8 == 0;
     for (int i = 0; i < 2; ++i) {
