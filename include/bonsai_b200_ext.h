@@ -346,7 +346,8 @@ int bonsai_b200_pages_attn(const bonsai_b200_pages *pages, int layer, const floa
  * Scales below 2^-21 of the largest of their row of K, or of their block of 32 dims of V among 128 positions that follow each other, count as multiples of 2^-32 of that.
  * workspace: 16-byte aligned device memory of bonsai_b200_pages_attn_shared_workspace(the same cache and sizes; it reads the struct's numbers, not its memory) bytes: 2 KB for each token and
  * query head, 7.3 MB, and in calls of more than 640 rows (n_head / n_head_kv a token) 20 MB and 133 KB a kv head for
- * each page that as many rows may have in common, 2.5 GB at most. */
+ * each page that as many rows may have in common, 2.5 GB at most.  (Such calls need that room whether their numbers turn out to use it or not.  Pages of which there are more than room is left
+ * for are served without, as those of fewer rows are; the others of the call are not held up by them.) */
 int64_t bonsai_b200_pages_attn_shared_workspace(const bonsai_b200_pages *pages, int n_groups, int n_head);
 int bonsai_b200_pages_attn_shared(const bonsai_b200_pages *pages, int layer, const int32_t *group, const int32_t *shared, int n_groups, const float *q, float *out, int n_head,
                                   void *workspace, int64_t workspace_bytes, float scale, bonsai_stream stream);

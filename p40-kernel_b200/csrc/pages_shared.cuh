@@ -189,6 +189,7 @@ __device__ __forceinline__ long long psh_scan(long long x, int lane) {
 constexpr int PSP_THREADS = 512;
 __global__ void __launch_bounds__(PSP_THREADS) pages_shared_plan_kernel(const __grid_constant__ PageShared P) {
     __shared__ long long sums[PSP_THREADS / 32];
+    __shared__ int place[PSP_THREADS], taken;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, entities = P.n_groups + P.C.n_seq;
     PshPlan &plan = *P.plan;
     pdl_wait_prior_grid();
@@ -223,8 +224,27 @@ __global__ void __launch_bounds__(PSP_THREADS) pages_shared_plan_kernel(const __
             rows = 0;
         }
         const int pages = (E.end + PG_POS - 1) / PG_POS - E.page0;
-        const long long images = rows && P.image_room && E.tokens * P.group > PST_MIN_ROWS && pages >= PST_MIN_PAGES ? pages : 0, image = in_front(images, images0);
-        const bool many = images && image + images <= P.image_room;
+        const int images = rows && E.tokens * P.group > PST_MIN_ROWS && pages >= PST_MIN_PAGES && pages <= P.image_room ? pages : 0;
+        const long long before = images0;
+        long long image = in_front(images, images0);
+        if (images0 > P.image_room) {        // there is no room for all of them: each in its turn that finds some (the same for all threads)
+            place[tid] = images;
+            __syncthreads();
+            if (tid == 0) {
+                int at = (int)before;
+                for (int i = 0; i < PSP_THREADS; ++i) {
+                    const int n = place[i];
+                    if (n == 0) continue;
+                    place[i] = n <= P.image_room - at ? at : -1;
+                    at += place[i] < 0 ? 0 : n;
+                }
+                taken = at;
+            }
+            __syncthreads();
+            image = place[tid];
+            images0 = taken;
+        }
+        const bool many = images && image >= 0;
         if (many) E.image = (int)image, E.steps = pages;
         const long long own = rows ? units(E) : 0;
         const long long a = in_front(many ? 0 : own, unit0), b = in_front(many ? own : 0, tc_unit0), c = in_front(many ? 0 : rows, row0), d = in_front(many ? rows : 0, tc_row0);
@@ -240,7 +260,7 @@ __global__ void __launch_bounds__(PSP_THREADS) pages_shared_plan_kernel(const __
         plan.tc_total = tc_unit0;
         plan.tc_per = tc_per;
         plan.tc_row = row0 + (long long)P.ctas * PSH_ROWS;
-        plan.images = (int)min(images0, (long long)P.image_room);
+        plan.images = (int)images0;
     }
     __syncthreads();
 #pragma unroll 1
