@@ -2300,7 +2300,7 @@ int bonsai_b200_pages_attn_shared(const bonsai_b200_pages *pages, int layer, con
     P.group_pages = shared;
     P.scale = scale;
     P.part_rows = plan.part_rows;
-    P.image_room = (int)plan.images;
+    P.image_room = pst_rows_many((int64_t)C.n_tok * P.group, C.n_head_kv) ? (int)plan.images : 0;       // (two launches that would find nothing)
     P.ctas = SM_COUNT;
     static SmemOptIn opt[2];
     // what the warps' shares of the registers add up to is what the launch has to bring: one that asked for more would wait for them for good

@@ -73,10 +73,21 @@ struct alignas(16) PshSmall {
 constexpr int PSH_SMEM_BYTES = 1024 + PSH_AT_SMALL + (int)sizeof(PshSmall);
 static_assert(PSH_SMEM_BYTES <= 227 * 1024, "");
 
-// Entities of many rows are pages_shared_tc_kernel's (pages_shared_tc.cuh): tiles of 128 rows, steps of a page, a line of their own.  Measured, whole calls in us, as 48 rows a tile
-// against as images (4 kv heads, one token of 6 heads each): 384 rows over 64 and 256 pages 93 / 102 and 179 / 201; 642 rows over 16, 32, 64 and 256 pages 87 / 92, 101 / 102,
-// 132 / 123 and 269 / 276; 900 rows over 16, 64 and 256 pages 112 / 115, 167 / 152 and 359 / 338; 1200 rows over 500 pages 760 / 656.
-constexpr int PST_ROWS = 128, PST_MIN_ROWS = 640, PST_MIN_PAGES = 32;
+// Entities of many rows are pages_shared_tc_kernel's (pages_shared_tc.cuh): tiles of 128 rows, steps of a page, a line of their own.  Two launches more cost 10 to 20 us, and what images save
+// goes with the rows and pages of all kv heads.  Measured, whole calls in us, as 48 rows a tile against as images (one new token a sequence behind a common prefix):
+//   4 kv heads of 6   642 rows over 16, 32, 64, 256 pages 80 / 81, 92 / 91, 119 / 110, 261 / 255; 384 rows 60 / 70, 69 / 76, 83 / 90, 166 / 183; 1200 rows 124 / 115, 146 / 126, 191 / 156, 444 / 347
+//   8 of 4            644 rows over 32, 64, 256 pages 186 / 157, 237 / 205, 521 / 516; 384 rows 125 / 123, 157 / 159, 320 / 337        8 of 8    648 rows 138 / 129, 189 / 177, 472 / 487
+//   3 of 4            700 rows over 32, 64, 128 pages 94 / 93, 113 / 108, 154 / 144
+//   2 of 8            704 rows over 32, 128, 256 pages 61 / 74, 98 / 104, 147 / 152; 1040 rows over 32, 64, 128, 256 pages 74 / 78, 94 / 91, 130 / 119, 207 / 177; 1504 rows over 32, 64 95 / 94, 124 / 108
+//   1 of 8            1800 rows over 32, 64, 128, 256 pages 71 / 77, 86 / 86, 117 / 104, 181 / 142; 3000 rows 96 / 95, 128 / 109, 177 / 139, 286 / 190
+//   1 of 6            642 rows over 64, 256 pages 55 / 68, 92 / 96; 900 rows 63 / 77, 109 / 114; 1200 rows 71 / 81, 137 / 122; 2400 rows 113 / 101, 243 / 169
+//   1 of 24           two sequences: 2064 rows over 32, 64 pages 60 / 73, 76 / 84; 3000 rows 69 / 80, 101 / 94
+// With three kv heads and more the first two numbers decide.
+constexpr int PST_ROWS = 128, PST_MIN_ROWS = 640, PST_MIN_PAGES = 32, PST_ALL_ROWS = 1024, PST_ALL_WORK = 95000;
+__host__ __device__ __forceinline__ bool pst_rows_many(int64_t rows, int n_head_kv) { return rows > PST_MIN_ROWS && rows * n_head_kv > PST_ALL_ROWS; }
+__device__ __forceinline__ bool pst_many(int64_t rows, int pages, int n_head_kv) {
+    return pst_rows_many(rows, n_head_kv) && pages >= PST_MIN_PAGES && (float)rows * (float)n_head_kv * ((float)pages * (float)n_head_kv) >= (float)PST_ALL_WORK;
+}
 constexpr int PST_START = 8;                                     // what a fragment's begin is worth, in pages (2: 378 us where 8 has 364 and 20 has 379)
 // The tensor core drops what a sum has behind its 24 bits: sums come out low by about 2^-24 for each of the twelve or so that a score is made of.  Scores are lifted by the mean of that
 // (root mean square of the outputs' error 3.4e-6 without, 1.3e-6 with it).
@@ -224,7 +235,7 @@ __global__ void __launch_bounds__(PSP_THREADS) pages_shared_plan_kernel(const __
             rows = 0;
         }
         const int pages = (E.end + PG_POS - 1) / PG_POS - E.page0;
-        const int images = rows && E.tokens * P.group > PST_MIN_ROWS && pages >= PST_MIN_PAGES && pages <= P.image_room ? pages : 0;
+        const int images = rows && pst_many((int64_t)E.tokens * P.group, pages, P.C.n_head_kv) && pages <= P.image_room ? pages : 0;
         const long long before = images0;
         long long image = in_front(images, images0);
         if (images0 > P.image_room) {        // there is no room for all of them: each in its turn that finds some (the same for all threads)

@@ -9,14 +9,14 @@ from test_gpu_sequences import Cache, ints, starts, status_is_clear  # noqa: F40
 from test_sequences_cpu import struct
 
 pytestmark = pytest.mark.gpu
-GROUP = 24                      # query heads of a kv head
+GROUP = 8                       # query heads of a kv head
 NEW = -(-MANY // GROUP)         # tokens that make a sequence one of many rows
 
 
-def room_for(gpu, n_pages, n_tok, stride, heads_kv):
+def room_for(gpu, n_pages, n_tok, stride, heads_kv, group=GROUP):
     """Bytes of the workspace, and of one page's image."""
     size = lambda n: gpu.lib().bonsai_b200_pages_attn_shared_workspace(  # noqa: E731
-        C.byref(struct(n_pages=n, n_layers=1, n_head_kv=heads_kv, n_seq=1, table_stride=stride, n_tok=n_tok)), 0, GROUP * heads_kv)
+        C.byref(struct(n_pages=n, n_layers=1, n_head_kv=heads_kv, n_seq=1, table_stride=stride, n_tok=n_tok)), 0, group * heads_kv)
     return size(n_pages) - size(n_pages - 1)
 
 
@@ -41,7 +41,7 @@ def cache_of(gpu, n_pages, pages, new, heads_kv, seed=0):
     (90, [40, 40], [NEW, NEW - 1], [40, 0]), (40, [39, 40, 41], [1, NEW, NEW], [0, 40, 0]),
     # the ones that find none in front of many others: more entities than are looked at at once
     (70, [71, LONG] + [1] * 520 + [71, LONG, LONG], [NEW, NEW] + [1] * 520 + [NEW, NEW, NEW], [0, LONG] + [0] * 521 + [LONG, 0])])
-@pytest.mark.parametrize("heads_kv", [1, 2])
+@pytest.mark.parametrize("heads_kv", [4, 5])
 def test_images_for_those_that_fit(gpu, n_pages, pages, new, images, heads_kv):
     import torch
     c = cache_of(gpu, n_pages, pages, new, heads_kv, seed=n_pages)
@@ -63,10 +63,10 @@ def test_images_for_those_that_fit(gpu, n_pages, pages, new, images, heads_kv):
 def test_a_captured_call_with_other_lengths(gpu):
     """The same graph, whose sequences fit or do not by their lengths when it is replayed."""
     import torch
-    c = cache_of(gpu, 64, [64, LONG, 40], [NEW] * 3, 1, seed=9)
-    q = queries(c, GROUP)
-    ws, out = torch.empty(c.view.attn_shared_workspace(0, GROUP), dtype=torch.uint8, device="cuda"), torch.empty_like(q)
-    step = lambda: c.view.attn_shared(0, None, None, q, out, GROUP, ws, 0.0625)  # noqa: E731
+    c = cache_of(gpu, 64, [64, LONG, 40], [NEW] * 3, 4, seed=9)
+    q = queries(c, 4 * GROUP)
+    ws, out = torch.empty(c.view.attn_shared_workspace(0, 4 * GROUP), dtype=torch.uint8, device="cuda"), torch.empty_like(q)
+    step = lambda: c.view.attn_shared(0, None, None, q, out, 4 * GROUP, ws, 0.0625)  # noqa: E731
     st, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
     with torch.cuda.stream(st):
         assert step() == 0
@@ -76,7 +76,7 @@ def test_a_captured_call_with_other_lengths(gpu):
     rng = np.random.default_rng(1)
     c.table[:] = rng.integers(0, 64, c.table.shape)
     c.view._keep[1].copy_(ints(c.table))
-    for lens in ([64 * 64, 64 * LONG, 64 * 40], [64 * 40, 64 * LONG, 64 * 33], [100, 64 * 64, 64 * LONG], [64 * LONG, 64 * LONG - 3, 50]):
+    for lens in ([64 * 64, 64 * LONG, 64 * 40], [64 * 40, 64 * LONG, 64 * 33], [100, 64 * 64, 64 * LONG], [64 * LONG, 64 * LONG - 3, 90]):
         c.lens = lens
         c.view._keep[2].copy_(ints(lens))
         got = []
