@@ -341,8 +341,13 @@ int bonsai_b200_pages_attn(const bonsai_b200_pages *pages, int layer, const floa
  * each, whole ones, are the same: only the table row of the first of them that has new tokens is read there.  New tokens lie behind them: len[s] less its new tokens is
  * shared[g] * BONSAI_B200_PAGE_POSITIONS at least.  A sequence of no group, or of a group of one, shares nothing; n_groups (n_seq at most) may be 0.  group (n_groups + 1 numbers) and
  * shared (n_groups) lie on the device like start.  A row of V with a scale that is no number or infinite makes the outputs of the tokens that see it NaN, and no others.
- * Scores are sums that the tensor core cuts off behind 24 bits, so outputs are within 1e-5 of the largest output of a head while the magnitudes of a score's products (scale included) add up to
- * 40 or so, and off in proportion beyond (2e-5 at 80, where bonsai_b200_pages_attn is off by 5e-6).  Weights come in two parts of 11 bits, and as multiples of 2^-32 of a row's largest.
+ * Less exact than bonsai_b200_pages_attn, for every sequence of the call, those of no group too: scores are sums that the tensor core cuts off behind 24 bits.  Outputs are within 1e-5 of the largest
+ * output of a head while the magnitudes of a score's products (scale included) add up to 40 or so, and off in proportion beyond (2e-5 at 80).  On the same inputs errors are 3 to 5 times the other
+ * attention's where sequences have few new tokens (1 to 2e-6 by root mean square), alike for prompts, and where sums are 70 to 90 the worst rows 4 to 32 times (16 in the median).  Weights come
+ * in two parts of 11 bits, and as multiples of 2^-32 of a row's largest.
+ * Which of the two: this one is faster from about 30 000 positions saved (a group's sequences less one, times what they share) with up to 16 sequences of one new token, 60 000 with 64, 100 000 with
+ * 200 (4 sequences behind 32 768 positions 59 us, the other 100; 16 behind 8192 51 and 108; 200 behind 4096 163 and 587).  Below that its launches that plan and join cost more than they save
+ * (2 behind 256 24 us, the other 14; 64 behind 256 50 and 30), and one sequence's token was slower at every length (32 768 positions 53 and 37).
  * Scales below 2^-21 of the largest of their row of K, or of their block of 32 dims of V among 128 positions that follow each other, count as multiples of 2^-32 of that.
  * workspace: 16-byte aligned device memory of bonsai_b200_pages_attn_shared_workspace(the same cache and sizes; it reads the struct's numbers, not its memory) bytes: 2 KB for each token and
  * query head, 7.3 MB, and in calls of more than 640 rows (n_head / n_head_kv a token) 20 MB and 133 KB a kv head for

@@ -2163,7 +2163,7 @@ int bonsai_b200_rope(const float *q, const float *k, const int32_t *pos, const d
         vec = vec && aligned16(P.x[i]) && aligned16(P.y[i]) && strides_by(n_tok, P.n_head[i], ts, hs, 4);
     }
     const int64_t each = vec ? n_rot / 8 + (head_dim - n_rot) / 4 : n_rot / 2 + head_dim - n_rot, items = heads * each;
-    // a token's items by CTAs: as many as threads hold (vec), one of few tokens.  (28 heads of 256, us by one / by as many: 1 token 2.0 / 2.8, 16 2.0 / 2.7, 64 3.2 / 2.9, 148 4.9 / 3.3, 1000 27 / 16.5.)
+    // a token's items by CTAs: as many as threads hold (vec), one of few tokens.  (28 heads of 256, us by one / by as many, replayed over four states that lie partly in L2: 1 token 2.0 / 2.8, 16 2.0 / 2.7, 64 3.2 / 2.9, 148 4.9 / 3.3, 1000 27 / 16.5.)
     const int64_t least = (items + ROPE_THREADS - 1) / ROPE_THREADS;
     const int64_t most = ROPE_THREADS * (vec ? (n_tok * least <= 2 * SM_COUNT ? 1 : ROPE_MAX_ITEMS) : 4), parts = (items + most - 1) / most;
     if (parts > 65535 || items > INT32_MAX) return 1;
@@ -2211,7 +2211,8 @@ int bonsai_b200_pages_write(const bonsai_b200_pages *pages, int layer, const flo
     P.amplitude = amplitude;
     P.eps = eps;
     const int64_t rows = (int64_t)n_head + 2 * (int64_t)P.C.n_head_kv;
-    // few rows: a warp has one; many: a CTA has up to 64 of two tokens, whose angles it forms once.  (32 rows a token, us, few / many: 1 token 3.5 / 6.7, 64 4.1 / 10.9, 300 9.2 / 12.5, 600 16.8 / 17.2,
+    // few rows: a warp has one; many: a CTA has up to 64 of two tokens, whose angles it forms once.  (32 rows a token, us, few / many, replayed over four states that lie partly in L2 (from memory
+    // one token takes 9.6): 1 token 3.5 / 6.7, 64 4.1 / 10.9, 300 9.2 / 12.5, 600 16.8 / 17.2,
     // 1000 24.2 / 20.7, 3000 62.7 / 49.4.)
     auto run = [&](auto kernel, int tok, int each) {
         const int64_t groups = (rows + each - 1) / each;

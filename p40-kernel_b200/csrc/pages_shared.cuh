@@ -17,7 +17,8 @@
 //
 // What bounds it: chains of latencies, that of K's planes first.  A step takes about 8000 cycles.  K's four warps take as long: 1100 for its page and scales, and for each 64 dims 450 to load codes,
 // 350 to see that their place is free, 850 for 32 pairs (byte permute, subtraction, product, remainder) and their way to tensor memory.  V's eight take 6500, the products of 48 rows 3900,
-// the step's bytes 3000.  (4 x 5 tokens over 32000 positions: 122 us; planes of zeros for K, V and both 108, 112 and 99.  Eight warps for K, 48 registers each: 136.)  48 rows a tile: planes,
+// the step's bytes 3000.  (4 x 5 tokens over 32000 positions: 114 us.  Tried when it was 122: planes of zeros for K, V and both 108, 112 and 99; eight warps for K, 48 registers each, 136.  The
+// warps' code in 80 registers spills 84 bytes of stores a thread.)  48 rows a tile: planes,
 // scores and two buffers of outputs then fill tensor memory.  Positions as rows keep the matrix instructions' 128 rows full whatever the number of tokens (tokens as rows: 6 of 128
 // used by one token).
 #pragma once
@@ -30,7 +31,7 @@ namespace b200 {
 constexpr int PSH_ROWS = 48, PSH_STEP = 2 * PG_POS, PSH_STAGE = 32, PSH_CHUNK = 64, PSH_DESCS = 4;
 constexpr int PSH_KSLOTS = 4, PSH_VSLOTS = 3;                    // pages of K and of V in shared memory
 constexpr int PSH_KRING = 2, PSH_VRING = 2;                      // in tensor memory: 64 dims of a step's K, 32 positions of V
-constexpr int PSH_START = 2;                                     // what a fragment's begin is worth, in steps (1 and 4: 146 us where 2 has 142)
+constexpr int PSH_START = 2;                                     // what a fragment's begin is worth, in steps (1, 2 and 4, us: 4 x 5 tokens 125, 114 and 117, ragged batch 138, 129 and 133, 64 chats 105, 108 and 114)
 constexpr int PSH_THREADS = 768, PSH_SUM_WARPS = 8, PSH_V_WARP = 8, PSH_K_WARP = 16, PSH_PLAN_WARP = 20, PSH_LOAD_WARP = 21, PSH_SCORE_WARP = 22, PSH_OUT_WARP = 23;
 // registers a thread: 2 x 136 + 2 x 48 + 64 + 48 = 6 x 80, what the launch has
 constexpr int PSH_REGS_SUM = 136, PSH_REGS_V = 48, PSH_REGS_K = 64, PSH_REGS_REST = 48;
@@ -88,9 +89,11 @@ __host__ __device__ __forceinline__ bool pst_rows_many(int64_t rows, int n_head_
 __device__ __forceinline__ bool pst_many(int64_t rows, int pages, int n_head_kv) {
     return pst_rows_many(rows, n_head_kv) && pages >= PST_MIN_PAGES && (float)rows * (float)n_head_kv * ((float)pages * (float)n_head_kv) >= (float)PST_ALL_WORK;
 }
-constexpr int PST_START = 8;                                     // what a fragment's begin is worth, in pages (2: 378 us where 8 has 364 and 20 has 379)
+constexpr int PST_START = 8;                                     // what a fragment's begin is worth, in pages (2, 8 and 20, us: 200 answers 383, 371 and 381, 12 questions 370, 372 and 370)
 // The tensor core drops what a sum has behind its 24 bits: sums come out low by about 2^-24 for each of the twelve or so that a score is made of.  Scores are lifted by the mean of that
-// (root mean square of the outputs' error 3.4e-6 without, 1.3e-6 with it).
+// (root mean square of the outputs' error 3.4e-6 without, 1.3e-6 with it).  A score of few large products is cut less and lifted all the same.  What that can do is bounded: scores times
+// 1 + L move an output by L times the covariance of scores and values under the weights, which is at most the largest |v| times sqrt(ln(n)^2 / 4 + 1) of n positions, the largest standard
+// deviation that scores have under their own weights: 3.0e-6 of it at 4000 positions, 3.8e-6 at 32 000.
 constexpr float PSH_LIFT = 1.0f + 6 * 0x1p-23f;
 
 // What there is to do, found by pages_shared_plan_kernel: a group over its shared pages, or a sequence over its own positions.
@@ -360,9 +363,10 @@ __device__ __forceinline__ PshStep psh_step(const PshFragment &F, int i) {
 }
 
 // ---- the warps ----------------------------------------------------------------------------------------------------------------------------------
-// A wait that runs out (a second at most): nothing is waited for any more, the CTA comes to its end and leaves its parts unfinished.  (One loop for a wait: what bounds this
-// kernel next to the tensor core is instructions that are not in the cache.)
-// TEST: a look without a wait in front of it.  pages_shared_tc_kernel, whose waits are mostly over, takes 266 us of a call with it and 273 without; 20 tokens of this kernel's 125 and 122.
+// A wait that runs out (2^18 looks, each of which the unit holds for as long as it sees fit; not a time that is known): nothing is waited for any more, the CTA comes to its end and leaves its
+// parts unfinished.  One that waits for it runs out behind it.  (One loop for a wait: what bounds this kernel next to the tensor core is instructions that are not in the cache.)
+// TEST: a look without a wait in front of it.  pages_shared_tc_kernel, whose waits are mostly over: 200 answers 371 us with it and 377 without.  In this kernel 4 x 5 tokens would take 113 of
+// 114 us, but the code then spills more than its 84 bytes a thread.
 template <bool TEST = false>
 __device__ __forceinline__ bool psh_wait(uint64_t *bar, uint32_t parity) {
     if (TEST) {

@@ -8,7 +8,8 @@
 //
 // What bounds it: a chain.  A page takes about 4450 cycles, of which the products of its outputs 1700 (three of four products of planes, 128 x 256 x 64), and adding them and writing the
 // next weights 1430: there is one buffer of outputs, since tensor memory has no room for two.  With k, v and both products' waits in one warp it was 6700.  Writing the images takes a
-// seventh of a call (50 us for 1000 of them, 131 MB; with conversions by fp32 62); beyond 126 MB they also come back from memory.
+// seventh of a call (53 us for 1000 of them, 131 MB; with conversions by fp32 it took 12 more); beyond 126 MB they also come back from memory.  Its warps' code in 96 registers spills 112 bytes of
+// stores a thread.
 #pragma once
 
 #include "pages_shared.cuh"

@@ -9,12 +9,12 @@
 // outputs; of three warps more one issues the tensor core's instructions, which has a page's scores and the outputs of the page before in flight meanwhile, two copy k and v:
 //   tensor core   q . k of page i + 1          | weights x v of page i
 //   threads       weights of page i, outputs of page i - 1 added, weights to tensor memory | scores of page i + 1 read
-// (Its 19 warps leave a thread 96 registers, of which the 64 sums are most: 260 bytes of stores and 364 of loads spilled a thread.)
+// (Its 19 warps leave a thread 96 registers, of which the 64 sums are most: 200 bytes of stores and 252 of loads spilled a thread.)
 // (The issue is a warp's whole time: 2100 cycles for a page's scores, 1100 for its outputs.  By one of the sixteen warps a page took 8000 cycles, with the copies from the issuing
 // warp 5850.)
 // Tensor memory, all 512 columns: 256 output, 64 scores, 64 weights, 128 q low.  Shared memory: q high, k and v images of one page, 64 KB each.
 //
-// us with append, planes and join, 24 heads over 4: 512 tokens after 4000 240 (on mma.sync 415), with 48 pages in two rounds of CTAs at about 2.3 each, 20 of a CTA's start and
+// us with append, planes and join, 24 heads over 4: 512 tokens after 4000 232 (on mma.sync 415), with 48 pages in two rounds of CTAs at about 2.2 each, 20 of a CTA's start and
 // end and 25 of the launches around it.  A page's time is the copy of k behind the scores, the scores' products (N = 64: 44 cycles each, 33 were the rows in tensor memory) and the
 // softmax's first part, one after the other; the rest runs beside them.  Scores are one sum over 256 dims, small products first: relative error of the outputs 6e-7 there (fp32
 // torch 1.3e-6), 4.3e-7 for fresh prompts; six sums as in attn_tc.cuh leave no columns for two pages in flight.

@@ -35,9 +35,11 @@ struct RopeParams {
     float amplitude;
 };
 
-// What bounds it: memory (2999 tokens of 40 heads of 128 in 26.6 us, 0.70 of the copy rate); the angles, in 64 bits, are formed once a CTA while its values are on their way.
+// What bounds it: memory (2999 tokens of 40 heads of 128, all turned, in 26.6 us, 0.70 of the copy rate; a plain copy of as many bytes, timed alike, 26.1); the angles, in 64 bits, are formed
+// once a CTA while its values are on their way.  Of 28 heads of 256 with 64 turned a token is two CTAs of 784 items for 256 threads, a fourth round for sixteen of them: 3000 tokens 40.9 us,
+// the copy 32.7 (1000 tokens 15.9 and 15.7).
 // grid (tokens, parts of a token's items).  An item is what one thread turns: eight values (four pairs of halves, or two times two of neighbours) or four that are
-// not turned.  VEC: head_dim, n_rot and the strides are multiples of 8 (n_rot / 2 of 4), pointers 16-byte aligned; otherwise an item is a pair or a value.
+// not turned.  VEC: head_dim and n_rot are multiples of 8, strides of 4, pointers 16-byte aligned; otherwise an item is a pair or a value.
 template <bool VEC>
 __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const __grid_constant__ RopeParams P, int items, int per) {
     __shared__ float2 turn[ROPE_MAX_DIM / 2];
